@@ -24,6 +24,8 @@ from .gemm import (DEFAULT_GEMM_TILE, DEFAULT_GROUPED_GEMM_TILE, GemmTile, Nvfp4
                    rows_quantize)
 from .fp8 import (Fp8Gemm, Fp8GroupedGemmView, Fp8Matrix, Fp8Scaling, HostFp8Matrix, fp8_gemm, fp8_gemm_view,
                   fp8_grouped_gemm_q, fp8_grouped_gemm_view, quantize_fp8)
+from .speculative import (TREE_MAX_NODES, Kv8Cache, kv8_append, kv8_keep, kv8_read, tree_attention,
+                          tree_attention_workspace_bytes, tree_verify)
 from .checkpoint import (Checkpoint, CheckpointError, Fp8Config, HostBf16Weight, ModelOptConfig, Quantization,
                          SafetensorsFile, WeightFormat, check_companions, load_experts, load_weight, stack_weights,
                          verify_formats)

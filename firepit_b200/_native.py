@@ -193,6 +193,14 @@ SIGNATURES: dict[str, tuple] = {
     "fpb_moe_decode_route": (i32, [vp, sz, C.c_longlong, sz, sz, sz, sz, vp, vp, vp, vp, sz, vp, vp]),
     "fpb_nvfp4_moe_gemv": (i32, [vp, sz, vp, vp, i32, vp, i32, sz, i32, vp, i32, vp]),
     "fpb_moe_decode_combine_add_norm": (i32, [vp, vp, vp, sz, sz, vp, vp, sz, sz, C.c_float, vp, vp, i32, vp]),
+    "fpb_kv8_append": (i32, [vp, sz, sz, vp, sz, vp, sz, i32, vp, vp, vp, vp, sz, sz, sz, sz, sz, sz, C.c_float,
+                             C.c_float, sz, vp, i32, vp, vp, vp, vp, vp]),
+    "fpb_kv8_read": (i32, [vp, vp, vp, vp, sz, sz, sz, sz, vp, sz, sz, vp, vp, i32, vp]),
+    "fpb_kv8_keep": (i32, [vp, vp, vp, vp, sz, sz, sz, sz, vp, vp, sz, vp]),
+    "fpb_tree_attn_workspace_bytes": (sz, [sz, sz, sz, sz, sz, sz]),
+    "fpb_tree_attn": (i32, [vp, i32, sz, sz, vp, vp, vp, vp, vp, vp, vp, sz, sz, sz, sz, sz, sz, sz, sz, C.c_float, vp,
+                            sz, vp, vp]),
+    "fpb_tree_verify": (i32, [vp, i32, sz, vp, sz, vp, vp, vp, vp, sz, sz, sz, sz, C.c_float, vp, vp, vp, vp]),
     "fpb_comm_available": (i32, []),
     "fpb_comm_version": (i32, [C.POINTER(i32)]),
     "fpb_comm_unique_id": (i32, [vp]),

@@ -737,6 +737,90 @@ int fpb_moe_decode_combine_add_norm(const float *routed, const int32_t *map, con
                                     size_t hidden, float eps, float *out, void *normed, int normed_dtype,
                                     void *stream);
 
+/* ---- speculative decoding over an 8-bit key/value cache -----------------------
+ * No reference counterpart (its cache is f32 and its decode takes one token a
+ * step, attention.rs:6-30, generation.rs:34-42).  A step drafts a tree of
+ * tokens, runs them through the model together and keeps the path that the
+ * target accepts.
+ *
+ * Cache: k_codes, v_codes [batch, max_seq, kv_heads, head_dim] e4m3 and k_exp,
+ * v_exp [batch, max_seq, kv_heads], one exponent byte a head vector: value =
+ * code * 2^(byte - 127); head_dim a multiple of 16 up to 256, codes 16-byte
+ * aligned.  The exponent is the smallest e with max |x| <= 448 * 2^e within
+ * [-100, 120] (-8 for zeros); codes round to nearest even; an infinity is
+ * held as +-448 * 2^120 and a NaN stays one.
+ *
+ * Tree: parents [batch, nodes] int32, nodes <= 64: -1 for node 0 (the token
+ * after the cache's first `position` rows), an earlier node for the others;
+ * -2 for a node that is not there (then neither are its descendants; at node 0:
+ * no tree in this session).  parents NULL: a chain of any length (a prompt, or
+ * a chain of drafts).  Node i lies in cache row position + i; it sees rows
+ * [0, position), its ancestors and itself, and is rotated by position +
+ * depth(i).  Rows of q_out and attention outputs of nodes that are not there
+ * are zeros, and nothing is written for them.  Device errors (fpb_device_error):
+ * 502 a row outside [0, max_seq) (the node counts as not there), 504 a parent
+ * that is not an earlier node (likewise) or a path that does not ascend, 505 a
+ * token outside the vocabulary (refused). */
+/* q [batch * nodes rows of q_pitch, heads of q_head_pitch] (null with q_heads 0:
+ * keys and values only), k, v [rows of k_pitch / v_pitch, kv_heads * head_dim],
+ * f32 or bf16: RMSNorm of each head of q and k (gammas [head_dim] f32, 16-byte
+ * aligned; null: no norm), rotation of the first rotary_dim dims (halves as
+ * pairs, angle position * theta^(-2 i / rotary_dim), theta >= 1), k and v
+ * quantised into the cache, q to q_out [batch * nodes, q_heads, head_dim] (f32
+ * or bf16).  One launch. */
+int fpb_kv8_append(const void *q, size_t q_pitch, size_t q_head_pitch, const void *k, size_t k_pitch, const void *v,
+                   size_t v_pitch, int dtype, const float *q_gamma, const float *k_gamma, const int32_t *positions,
+                   const int32_t *parents, size_t batch, size_t nodes, size_t q_heads, size_t kv_heads,
+                   size_t head_dim, size_t rotary_dim, float theta, float eps, size_t max_seq, void *q_out,
+                   int q_out_dtype, uint8_t *k_codes, uint8_t *v_codes, uint8_t *k_exp, uint8_t *v_exp, void *stream);
+/* The values of rows [begin, begin + count) (begins non-null: [batch] device
+ * int32, one first row a session) to k_out, v_out [batch, count, kv_heads,
+ * head_dim] f32 or bf16 (exact in both).  A session whose range leaves the
+ * cache gets zeros and device error 502. */
+int fpb_kv8_read(const uint8_t *k_codes, const uint8_t *v_codes, const uint8_t *k_exp, const uint8_t *v_exp,
+                 size_t batch, size_t max_seq, size_t kv_heads, size_t head_dim, const int32_t *begins, size_t begin,
+                 size_t count, void *k_out, void *v_out, int out_dtype, void *stream);
+/* Moves an accepted path's rows together: row position + d becomes row
+ * position + path[d] (path [batch, nodes] ascending, -1 after its end, as
+ * fpb_tree_verify writes it). */
+int fpb_kv8_keep(uint8_t *k_codes, uint8_t *v_codes, uint8_t *k_exp, uint8_t *v_exp, size_t batch, size_t max_seq,
+                 size_t kv_heads, size_t head_dim, const int32_t *positions, const int32_t *path, size_t nodes,
+                 void *stream);
+/* Attention of the nodes over the cache (their own rows already appended):
+ * q [batch * nodes rows of q_pitch, q_heads of q_head_pitch] f32 or bf16, query
+ * head h reads kv head h / (q_heads / kv_heads); out [batch * nodes, q_heads *
+ * head_dim] bf16 = softmax(scale q . k) v, times sigmoid(gate) where gate
+ * [batch * nodes rows of gate_pitch, heads of gate_head_pitch] f32 is given.
+ * Rows of the cache that a node does not see never reach its output, whatever
+ * they hold. */
+size_t fpb_tree_attn_workspace_bytes(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, size_t head_dim,
+                                     size_t max_seq);
+int fpb_tree_attn(const void *q, int q_dtype, size_t q_pitch, size_t q_head_pitch, const uint8_t *k_codes,
+                  const uint8_t *v_codes, const uint8_t *k_exp, const uint8_t *v_exp, const int32_t *positions,
+                  const int32_t *parents, const float *gate, size_t gate_pitch, size_t gate_head_pitch, size_t batch,
+                  size_t nodes, size_t q_heads, size_t kv_heads, size_t head_dim, size_t max_seq, float scale,
+                  void *workspace, size_t workspace_bytes, void *out_bf16, void *stream);
+/* The walk from node 0 over logits [batch * nodes rows of logits_pitch, vocab]
+ * (f32 or bf16; non-finite ones count as -inf) and the drafted tokens [batch,
+ * nodes].  At a node, r = softmax(logits / temperature); its children are tried
+ * in order: child c with token x is taken when accept[c] * q(x) < r(x), q row
+ * `node` of draft [batch * nodes rows of draft_pitch, vocab] (the probabilities
+ * that the children were drawn from), or 1 where draft is null (certain
+ * drafts); a refused child leaves max(r - q, 0), or r without x, normalised
+ * (where nothing is left over, r stays).  At the last node next = argmax r /
+ * noise (noise [batch rows of noise_pitch, vocab] exponential variates > 0, lowest
+ * index among equals).  accept [batch, nodes] uniform in [0, 1).  temperature
+ * 0: a child is taken when it is the largest finite logit's index (lowest
+ * among equals), which is also `next`; accept, noise and draft are not read.
+ * Writes path [batch, nodes] (the accepted nodes, 0 first, then -1), count
+ * [batch] (their number) and next [batch] (the token after them); a session
+ * with no tree: count 0, next -1.  nodes <= 64, vocab <= 442368
+ * (FPB_ERR_UNSUPPORTED above).  One launch; rows off the path are not read. */
+int fpb_tree_verify(const void *logits, int logits_dtype, size_t logits_pitch, const float *draft, size_t draft_pitch,
+                    const int32_t *tokens, const int32_t *parents, const float *accept, const float *noise,
+                    size_t noise_pitch, size_t batch, size_t nodes, size_t vocab, float temperature, int32_t *path,
+                    int32_t *count, int32_t *next, void *stream);
+
 /* ---- collectives (NCCL) ------------------------------------------------------
  * The reference runs on one GPU and has no collectives.  These are the
  * exchange steps of the multi-GPU paths: the all-gather of each rank's output
