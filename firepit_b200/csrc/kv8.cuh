@@ -24,6 +24,13 @@ __device__ __forceinline__ float kv8_factor(uint32_t byte) {
   return __uint_as_float(byte ? byte << 23 : 0x00400000u);
 }
 
+// A value vector's exponent as the attention uses it: within the cache's
+// range whatever a row that nobody wrote may hold, so that it and its inverse
+// stay finite.
+__device__ __forceinline__ float kv8_value_exponent(uint32_t byte) {
+  return (float)min(kKv8MaxExp, max(kKv8MinExp, (int)byte - 127));
+}
+
 // The exponent for a head vector whose largest magnitude is amax: 448 = 1.75
 // * 2^8, so with amax = m * 2^x, m in [1, 2), it is x - 8, or x - 7 past 1.75.
 // Zero vectors take a middling exponent (the attention weighs each row by it).

@@ -5,6 +5,8 @@
 //   out = sum_t softmax(s)_t v_t, times sigmoid(gate) where a gate is given.
 #include <algorithm>
 #include <cmath>
+#include <mutex>
+#include <vector>
 
 #include "kv8.cuh"
 
@@ -17,77 +19,538 @@ struct TreeArgs {
   const uint8_t *k_codes, *v_codes, *k_exp, *v_exp;
   const int32_t *positions, *parents;
   long long q_pitch, q_head, gate_pitch, gate_head;  // elements
-  int nodes, q_heads, kv_heads, head_dim, max_seq, q_bf16;
-  float scale;
+  int nodes, q_heads, kv_heads, group, head_dim, max_seq, q_bf16, splits;
+  float scale_log2;  // scale * log2(e): scores and maxima are held in powers of two
   __nv_bfloat16 *out;
+  float *part;     // [session, kv head, row tile][split][row][head_dim] numerators
+  float2 *part_ml; // [session, kv head, row tile][split][row] maximum, sum
   int *error;
 };
 
-// One warp per (session, node, query head): eight columns a lane, the running
-// maximum and sum of the softmax over the rows one by one.
-__global__ void __launch_bounds__(256) tree_attn_kernel(const __grid_constant__ TreeArgs a) {
-  pdl_enter();
-  const int lane = threadIdx.x & 31, D = a.head_dim, c0 = lane * 8;
-  const int h = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (h >= a.q_heads) return;
-  const int b = blockIdx.y / a.nodes, n = blockIdx.y % a.nodes;
-  const int kvh = h / (a.q_heads / a.kv_heads);
-  const int32_t *par = a.parents ? a.parents + (size_t)b * a.nodes : nullptr;
-  const int pos = a.positions[b];
-  bool bad = false;
-  int depth = tree_depth(par, n, &bad);
-  if (depth >= 0 && (pos < 0 || pos >= a.max_seq - n)) {
-    depth = -1;
+// What a row (node n's query head) sees: rows before `pos`, then the tree
+// rows of `bits` (a tree), or the first `upto` of them (a chain); upto < 0:
+// the node is not there.
+struct Sight {
+  int upto;
+  uint64_t bits;
+  __device__ __forceinline__ bool sees(int t, int pos, bool tree) const {
+    const int j = t - pos;
+    if (j < 0) return true;
+    return tree ? j < kTreeMaxNodes && (bits >> j & 1) : j < upto;
+  }
+};
+
+__device__ __forceinline__ Sight sight_of(const TreeArgs &a, int b, int n, int pos) {
+  Sight s{-1, 0};
+  if (n >= a.nodes) return s;
+  if (pos < 0 || pos >= a.max_seq - n) {
     if (a.error) atomicCAS(a.error, 0, kErrPosition);
+    return s;
   }
-  if (bad && a.error) atomicCAS(a.error, 0, kErrParent);
-  float q[8], acc[8];
-  const size_t row = (size_t)b * a.nodes + n;
+  if (!a.parents) {
+    s.upto = n + 1;
+    return s;
+  }
+  const int32_t *par = a.parents + (size_t)b * a.nodes;
+  bool bad = false;
+  if (tree_depth(par, n, &bad) >= 0) {
+    s.upto = n + 1;
+    for (int j = n; j > 0; j = par[j]) s.bits |= 1ull << j;
+    s.bits |= 1;
+  } else if (bad && a.error) {
+    atomicCAS(a.error, 0, kErrParent);
+  }
+  return s;
+}
+
+// Rows of the cache that this session's nodes can see (0: none).
+__device__ __forceinline__ int seen_rows(const TreeArgs &a, int pos, int last_node) {
+  if (pos < 0 || pos >= a.max_seq) return 0;
+  return min(pos + last_node + 1, a.max_seq);
+}
+
+__device__ __forceinline__ float load_q(const TreeArgs &a, size_t at) {
+  return a.q_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(a.q)[at])
+                  : static_cast<const float *>(a.q)[at];
+}
+
+// Power of two that takes a query row into f16: its largest magnitude to
+// [2^8, 2^9), so that f16's 11 bits hold down to 2^-22 of it (f16 products
+// round at 2^-11; the scores' f32 sums and the factor are exact in it).
+__device__ __forceinline__ int q_exponent(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  if (u < 0x00800000u || u >= 0x7f800000u) return 0;  // zero, subnormal, infinite
+  return max(-118, (int)(u >> 23) - 127 - 8);
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Weights are held as 2^(y - m + kHead), y the score (in powers of two) plus
+// the value vector's own exponent: f16 then holds a weight down to 2^-32 of
+// the row's largest, and the exponent costs no multiplication.  The maximum
+// may lag by kLag before the sums are rescaled (weights up to 2^(kHead + kLag)).
+constexpr float kHead = 7.0f, kLag = 8.0f;
+
+// ---- few rows: tokens streamed through registers ---------------------------------------------
+// Block (split, session * kv head * row tile): NR rows (8 or 16) of one kv
+// head, four warps that take steps of 16 tokens in turn, all on their own:
+// codes go from memory to registers to the tensor cores with no shared memory
+// between.
+//  S = Q K^T   m16n8k16, the rows as M (NR = 8 leaves half of it zero).  The
+//              order of the summed dimension is free as long as both sides
+//              agree, so a lane's 16-byte piece of a key (16 dimensions) is
+//              its operand of four instructions as it lies.
+//  O^T = V^T P^T  the dimensions as M, the rows as N: P^T's operand is S's
+//              result as it lies.  V's needs pairs of tokens in a word: byte
+//              permutes of two tokens' pieces before the conversion.
+// Each e4m3 is converted to f16 (exact); the key's factor goes to the score,
+// the value's to the weight's exponent.
+constexpr int kRowsThreads = 128, kRowsWarps = 4;
+
+template <int DP, int NR>
+struct RowsShape {
+  static constexpr bool kQShared = NR * DP > 16 * 128;  // 64 registers of queries are too many beside 128 of sums
+  static constexpr int kQPitch = DP + 8;                // f16 elements: 16-byte reads of eight rows on distinct banks
+  static constexpr size_t smem = (size_t)kRowsWarps * NR * (DP + 2) * 4;
+};
+
+template <int DP, int NR>
+__global__ void __launch_bounds__(kRowsThreads, 2) tree_attn_rows_kernel(const __grid_constant__ TreeArgs a) {
+  pdl_enter();
+  using Sh = RowsShape<DP, NR>;
+  constexpr int kPieces = DP / 64, kVPieces = DP >= 128 ? DP / 128 : 1, kVBytes = DP >= 128 ? 16 : 8;
+  constexpr int kMT = DP / 16, kNT = NR / 8;
+  extern __shared__ __align__(16) float sm[];  // queries (f16) first, then the warps' results
+  __shared__ float m_s[kRowsWarps][NR], l_s[kRowsWarps][NR];
+  __shared__ float fac_s[NR];
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, c = lane & 3;
+  const int rows = a.nodes * a.group, tiles = (rows + NR - 1) / NR;
+  const int item = blockIdx.y, tile = item % tiles, bk = item / tiles;
+  const int b = bk / a.kv_heads, kvh = bk % a.kv_heads, D = a.head_dim;
+  const int pos = a.positions[b];
+  const bool tree = a.parents != nullptr;
+  const int last = min(a.nodes - 1, (tile * NR + NR - 1) / a.group);
+  const int total = seen_rows(a, pos, last);
+  // this split's tokens, in whole steps
+  const int steps = (total + 15) / 16, per = (steps + a.splits - 1) / a.splits;
+  const int s0 = blockIdx.x * per, s1 = min(steps, s0 + per);
+
+  // queries: a warp takes rows w, w + 4, ...; eight columns a lane
+  __half *qs = reinterpret_cast<__half *>(sm);
+  for (int r = w; r < NR; r += kRowsWarps) {
+    const int row = tile * NR + r, n = row / a.group, h = kvh * a.group + row % a.group;
+    float x[8];
+    float amax = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const size_t at = row * a.q_pitch + (size_t)h * a.q_head + c0 + i;
-    q[i] = c0 >= D ? 0.0f
-           : a.q_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(a.q)[at])
-                      : static_cast<const float *>(a.q)[at];
-    acc[i] = 0.0f;
-  }
-  float m = -INFINITY, l = 0.0f;
-  auto visit = [&](int t) {
-    const size_t vec = ((size_t)b * a.max_seq + t) * a.kv_heads + kvh;
-    uint2 kw = make_uint2(0, 0), vw = make_uint2(0, 0);
-    if (c0 < D) {
-      kw = *reinterpret_cast<const uint2 *>(a.k_codes + vec * D + c0);
-      vw = *reinterpret_cast<const uint2 *>(a.v_codes + vec * D + c0);
+    for (int i = 0; i < 8; ++i) {
+      const int col = lane * 8 + i;
+      x[i] = row < rows && col < D
+                 ? load_q(a, ((size_t)b * a.nodes + n) * a.q_pitch + (size_t)h * a.q_head + col) : 0.0f;
+      amax = fmaxf(amax, fabsf(x[i]));
     }
-    const uint64_t k8 = (uint64_t)kw.y << 32 | kw.x, v8 = (uint64_t)vw.y << 32 | vw.x;
-    float s = 0.0f;
+    amax = warp_max(amax);
+    const int e = q_exponent(amax);
+    const float f = pow2i(-e);
+    if (lane * 8 < DP) {
+      uint4 o;
+      o.x = pack_f16x2(x[0] * f, x[1] * f);
+      o.y = pack_f16x2(x[2] * f, x[3] * f);
+      o.z = pack_f16x2(x[4] * f, x[5] * f);
+      o.w = pack_f16x2(x[6] * f, x[7] * f);
+      *reinterpret_cast<uint4 *>(qs + r * Sh::kQPitch + lane * 8) = o;
+    }
+    if (lane == 0) fac_s[r] = pow2i(e) * a.scale_log2;
+  }
+  __syncthreads();
+  // the lane's rows of S: g and, with 16 rows, g + 8
+  Sight sight[kNT];
+  float fac[kNT];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s = fmaf(q[i], e4m3_to_f32((uint8_t)(k8 >> (8 * i))), s);
+  for (int i = 0; i < kNT; ++i) {
+    const int row = tile * NR + g + 8 * i;
+    sight[i] = sight_of(a, b, row < rows ? row / a.group : a.nodes, pos);
+    fac[i] = fac_s[g + 8 * i];
+  }
+  // Q operands of piece p: row's dimensions 64 p + 16 c + [0, 16)
+  uint32_t qr[Sh::kQShared ? 1 : kPieces * kNT * 8];
+  if constexpr (!Sh::kQShared) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    s *= kv8_factor(a.k_exp[vec]) * a.scale;
-    const float mn = fmaxf(m, s), old = m == -INFINITY ? 0.0f : expf(m - mn), p = expf(s - mn);
-    const float f = p * kv8_factor(a.v_exp[vec]);
+    for (int p = 0; p < kPieces; ++p)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = fmaf(f, e4m3_to_f32((uint8_t)(v8 >> (8 * i))), acc[i] * old);
-    l = l * old + p;
-    m = mn;
+      for (int i = 0; i < kNT; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint4 v = *reinterpret_cast<const uint4 *>(qs + (g + 8 * i) * Sh::kQPitch + 64 * p + 16 * c + 8 * j);
+          uint32_t *o = qr + (p * kNT + i) * 8 + 4 * j;
+          o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
+        }
+  }
+
+  const size_t pitch = (size_t)a.kv_heads * D;
+  const uint8_t *kc = a.k_codes + ((size_t)b * a.max_seq * a.kv_heads + kvh) * D;
+  const uint8_t *vc = a.v_codes + ((size_t)b * a.max_seq * a.kv_heads + kvh) * D;
+  const uint8_t *ex = (lane < 16 ? a.k_exp : a.v_exp) + (size_t)b * a.max_seq * a.kv_heads + kvh;
+  uint4 kr[2][kPieces];
+  uint32_t vr[4][kVPieces][kVBytes / 4];
+  uint32_t xr = 0;
+  auto load_k = [&](int step) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int t = step * 16 + 8 * u + g;
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) {
+        const int d = 64 * p + 16 * c;
+        kr[u][p] = t < total && d < D ? __ldg(reinterpret_cast<const uint4 *>(kc + (size_t)t * pitch + d))
+                                      : make_uint4(0, 0, 0, 0);
+      }
+    }
+    const int t = step * 16 + (lane & 15);
+    xr = t < total ? ex[(size_t)t * a.kv_heads] : 127;
   };
-  if (depth >= 0) {
-    for (int t = 0; t < pos; ++t) visit(t);
-    if (par)
-      for (int j = n; j >= 0; j = par[j]) visit(pos + j);
-    else
-      for (int j = 0; j <= n; ++j) visit(pos + j);
-  }
-  if (c0 >= D) return;
+  auto load_v = [&](int step) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float o = depth >= 0 ? acc[i] / l : 0.0f;
-    if (a.gate && depth >= 0)
-      o /= 1.0f + expf(-a.gate[row * a.gate_pitch + (size_t)h * a.gate_head + c0 + i]);
-    a.out[(row * a.q_heads + h) * D + c0 + i] = __float2bfloat16_rn(o);
+    for (int i = 0; i < 4; ++i) {
+      const int t = step * 16 + 2 * c + (i & 1) + 8 * (i >> 1);
+#pragma unroll
+      for (int p = 0; p < kVPieces; ++p) {
+        const int d = 128 * p + kVBytes * g;
+        if constexpr (kVBytes == 16) {
+          const uint4 v = t < total && d < D ? __ldg(reinterpret_cast<const uint4 *>(vc + (size_t)t * pitch + d))
+                                             : make_uint4(0, 0, 0, 0);
+          vr[i][p][0] = v.x; vr[i][p][1] = v.y; vr[i][p][2] = v.z; vr[i][p][3] = v.w;
+        } else {
+          const uint2 v = t < total && d < D ? __ldg(reinterpret_cast<const uint2 *>(vc + (size_t)t * pitch + d))
+                                             : make_uint2(0, 0);
+          vr[i][p][0] = v.x; vr[i][p][1] = v.y;
+        }
+      }
+    }
+  };
+
+  float acc[kMT][kNT][4];
+#pragma unroll
+  for (int i = 0; i < kMT; ++i)
+#pragma unroll
+    for (int j = 0; j < kNT; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[i][j][k] = 0.0f;
+  float m[kNT], l[kNT];
+#pragma unroll
+  for (int i = 0; i < kNT; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.0f;
   }
+  int step = s0 + w;
+  if (step < s1) {
+    load_k(step);
+    load_v(step);
+  }
+  for (; step < s1; step += kRowsWarps) {
+    // scores of 16 tokens: s[u] tokens 8 u + 2 c, 2 c + 1 of row g (and g + 8)
+    float s[2][4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[u][k] = 0.0f;
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      uint32_t q0[8], q1[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q1[j] = 0;
+      if constexpr (Sh::kQShared) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint4 v = *reinterpret_cast<const uint4 *>(qs + g * Sh::kQPitch + 64 * p + 16 * c + 8 * j);
+          q0[4 * j] = v.x; q0[4 * j + 1] = v.y; q0[4 * j + 2] = v.z; q0[4 * j + 3] = v.w;
+          if constexpr (NR == 16) {
+            const uint4 y = *reinterpret_cast<const uint4 *>(qs + (g + 8) * Sh::kQPitch + 64 * p + 16 * c + 8 * j);
+            q1[4 * j] = y.x; q1[4 * j + 1] = y.y; q1[4 * j + 2] = y.z; q1[4 * j + 3] = y.w;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          q0[j] = qr[p * kNT * 8 + j];
+          if constexpr (NR == 16) q1[j] = qr[(p * kNT + 1) * 8 + j];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t kw[4] = {kr[u][p].x, kr[u][p].y, kr[u][p].z, kr[u][p].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          mma_f16(s[u], q0[2 * j], q1[2 * j], q0[2 * j + 1], q1[2 * j + 1], e4m3x2_to_f16x2((uint16_t)kw[j]),
+                  e4m3x2_to_f16x2((uint16_t)(kw[j] >> 16)));
+      }
+    }
+    const uint32_t xb = xr;
+    const int t0 = step * 16;
+    const bool open = t0 + 16 > pos;  // warp-uniform: the tree's rows, or the end
+    if (step + kRowsWarps < s1) load_k(step + kRowsWarps);
+    uint32_t nan[4] = {0, 0, 0, 0};
+    if (open) {  // a value vector that some row does not see must not reach it through 0 * NaN
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int p = 0; p < kVPieces; ++p)
+#pragma unroll
+          for (int j = 0; j < kVBytes / 4; ++j) {
+            const uint32_t bad = __vcmpeq4(vr[i][p][j] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            vr[i][p][j] &= ~bad;
+            nan[i] |= bad;
+          }
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) nan[i] |= __shfl_xor_sync(0xffffffffu, nan[i], o);
+      }
+    }
+    // y = score + the value's exponent, and the rows' maxima
+    float y[kNT][4], ve[4], mx[kNT];
+#pragma unroll
+    for (int i = 0; i < kNT; ++i) mx[i] = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int u = k >> 1, e = k & 1, tl = 8 * u + 2 * c + e, t = t0 + tl;
+      const float kf = kv8_factor(__shfl_sync(0xffffffffu, xb, tl));
+      ve[k] = kv8_value_exponent(__shfl_sync(0xffffffffu, xb, 16 + tl));
+#pragma unroll
+      for (int i = 0; i < kNT; ++i) {
+        float v = fmaf(s[u][2 * i + e], kf * fac[i], ve[k]);
+        if (open) {
+          if (nan[k]) v = __int_as_float(0x7fc00000);
+          if (t >= total || !sight[i].sees(t, pos, tree)) v = -INFINITY;
+        }
+        y[i][k] = v;
+        mx[i] = fmaxf(mx[i], v);
+      }
+    }
+    bool grow = false;
+#pragma unroll
+    for (int i = 0; i < kNT; ++i) {
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+      grow |= mx[i] > m[i] + kLag || (m[i] == -INFINITY && mx[i] > m[i]);
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+      float old[kNT];
+#pragma unroll
+      for (int i = 0; i < kNT; ++i) {
+        const float mn = fmaxf(m[i], mx[i]);
+        old[i] = m[i] == -INFINITY ? 0.0f : exp2_approx(m[i] - mn);
+        l[i] *= old[i];
+        m[i] = mn;
+      }
+#pragma unroll
+      for (int j = 0; j < kNT; ++j)  // the sums hold rows 2 c, 2 c + 1 (+ 8 j): their factors are lanes 8 c and 8 c + 4's
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float f = __shfl_sync(0xffffffffu, old[j], 8 * c + 4 * e);
+#pragma unroll
+          for (int i = 0; i < kMT; ++i) {
+            acc[i][j][e] *= f;
+            acc[i][j][2 + e] *= f;
+          }
+        }
+    }
+    uint32_t pb[kNT][2];
+#pragma unroll
+    for (int i = 0; i < kNT; ++i) {
+      const float base = m[i] == -INFINITY ? 0.0f : kHead - m[i];
+      float p[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        p[k] = exp2_approx(y[i][k] + base);
+        l[i] = fmaf(p[k], pow2i(-(int)ve[k]), l[i]);
+      }
+      pb[i][0] = pack_f16x2(p[0], p[1]);
+      pb[i][1] = pack_f16x2(p[2], p[3]);
+    }
+#pragma unroll
+    for (int p = 0; p < kVPieces; ++p)
+#pragma unroll
+      for (int j = 0; j < kVBytes / 4; ++j) {
+        const uint32_t x0 = __byte_perm(vr[0][p][j], vr[1][p][j], 0x5140);
+        const uint32_t x1 = __byte_perm(vr[0][p][j], vr[1][p][j], 0x7362);
+        const uint32_t z0 = __byte_perm(vr[2][p][j], vr[3][p][j], 0x5140);
+        const uint32_t z1 = __byte_perm(vr[2][p][j], vr[3][p][j], 0x7362);
+        const int mt = (p * kVBytes / 4 + j) * 2;
+#pragma unroll
+        for (int i = 0; i < kNT; ++i) {
+          mma_f16(acc[mt][i], e4m3x2_to_f16x2((uint16_t)x0), e4m3x2_to_f16x2((uint16_t)(x0 >> 16)),
+                  e4m3x2_to_f16x2((uint16_t)z0), e4m3x2_to_f16x2((uint16_t)(z0 >> 16)), pb[i][0], pb[i][1]);
+          mma_f16(acc[mt + 1][i], e4m3x2_to_f16x2((uint16_t)x1), e4m3x2_to_f16x2((uint16_t)(x1 >> 16)),
+                  e4m3x2_to_f16x2((uint16_t)z1), e4m3x2_to_f16x2((uint16_t)(z1 >> 16)), pb[i][0], pb[i][1]);
+        }
+      }
+    if (step + kRowsWarps < s1) load_v(step + kRowsWarps);
+  }
+
+  // the warps' results meet: maxima, then sums over one maximum in warp order
+#pragma unroll
+  for (int i = 0; i < kNT; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    if (c == 0) {
+      m_s[w][g + 8 * i] = m[i];
+      l_s[w][g + 8 * i] = l[i];
+    }
+  }
+  __syncthreads();  // also: every warp is done with the queries that `sm` held
+  float *mine = sm + (size_t)w * NR * (DP + 2);
+#pragma unroll
+  for (int p = 0; p < kVPieces; ++p)
+#pragma unroll
+    for (int j = 0; j < kVBytes / 4; ++j)
+#pragma unroll
+      for (int i = 0; i < kNT; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int mt = (p * kVBytes / 4 + j) * 2, d = 128 * p + kVBytes * g + 4 * j;
+          float *o = mine + (size_t)(8 * i + 2 * c + e) * (DP + 2) + d;
+          *reinterpret_cast<float2 *>(o) = make_float2(acc[mt][i][e], acc[mt][i][2 + e]);
+          *reinterpret_cast<float2 *>(o + 2) = make_float2(acc[mt + 1][i][e], acc[mt + 1][i][2 + e]);
+        }
+  __syncthreads();
+  for (int r = w; r < NR; r += kRowsWarps) {
+    const int row = tile * NR + r;
+    if (row >= rows) break;
+    float mt = -INFINITY, f[kRowsWarps], lt = 0.0f;
+#pragma unroll
+    for (int x = 0; x < kRowsWarps; ++x) mt = fmaxf(mt, m_s[x][r]);
+#pragma unroll
+    for (int x = 0; x < kRowsWarps; ++x) {
+      f[x] = m_s[x][r] == -INFINITY ? 0.0f : exp2_approx(m_s[x][r] - mt);
+      lt += l_s[x][r] * f[x];
+    }
+    const int n = row / a.group, h = kvh * a.group + row % a.group;
+    const bool there = sight_of(a, b, n, pos).upto >= 0;
+    for (int d = lane * 2; d < D; d += 64) {
+      float2 o = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int x = 0; x < kRowsWarps; ++x) {
+        const float2 v = *reinterpret_cast<const float2 *>(sm + ((size_t)x * NR + r) * (DP + 2) + d);
+        o.x = fmaf(v.x, f[x], o.x);
+        o.y = fmaf(v.y, f[x], o.y);
+      }
+      if (a.splits > 1) {
+        *reinterpret_cast<float2 *>(a.part + (((size_t)item * a.splits + blockIdx.x) * NR + r) * D + d) = o;
+      } else {
+        const size_t node = (size_t)b * a.nodes + n;
+        const float inv = there ? 1.0f / lt : 0.0f;
+        o.x = there ? o.x * inv : 0.0f;
+        o.y = there ? o.y * inv : 0.0f;
+        if (a.gate && there) {
+          const float *gt = a.gate + node * a.gate_pitch + (size_t)h * a.gate_head + d;
+          o.x /= 1.0f + expf(-gt[0]);
+          o.y /= 1.0f + expf(-gt[1]);
+        }
+        *reinterpret_cast<uint32_t *>(a.out + (node * a.q_heads + h) * D + d) = pack_bf16x2(o.x, o.y);
+      }
+    }
+    if (a.splits > 1 && lane == 0)
+      a.part_ml[((size_t)item * a.splits + blockIdx.x) * NR + r] = make_float2(mt, lt);
+  }
+}
+
+// The splits of a row meet: one warp a (session, node, query head), the
+// splits in order.
+__global__ void __launch_bounds__(256) tree_attn_merge_kernel(const __grid_constant__ TreeArgs a, int NR, int count) {
+  pdl_enter();
+  const int lane = threadIdx.x & 31, i = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (i >= count) return;
+  const int h = i % a.q_heads, node = i / a.q_heads, b = node / a.nodes, n = node % a.nodes, D = a.head_dim;
+  const int kvh = h / a.group, row = n * a.group + h % a.group;
+  const int tiles = (a.nodes * a.group + NR - 1) / NR;
+  const size_t item = ((size_t)b * a.kv_heads + kvh) * tiles + row / NR;
+  const int r = row % NR, pos = a.positions[b];
+  const bool there = sight_of(a, b, n, pos).upto >= 0;
+  const float2 *ml = a.part_ml + item * a.splits * NR + r;
+  float m = -INFINITY, l = 0.0f;
+  for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, ml[(size_t)s * NR].x);
+  m = warp_max(m);
+  float acc[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
+  const int d = lane * 8;
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 v = ml[(size_t)s * NR];
+    const float f = v.x == -INFINITY ? 0.0f : exp2_approx(v.x - m);
+    l = fmaf(v.y, f, l);
+    if (d < D && f != 0.0f) {
+      const float4 *p = reinterpret_cast<const float4 *>(a.part + ((item * a.splits + s) * NR + r) * D + d);
+      const float4 x = p[0], z = p[1];
+      acc[0] = fmaf(x.x, f, acc[0]); acc[1] = fmaf(x.y, f, acc[1]);
+      acc[2] = fmaf(x.z, f, acc[2]); acc[3] = fmaf(x.w, f, acc[3]);
+      acc[4] = fmaf(z.x, f, acc[4]); acc[5] = fmaf(z.y, f, acc[5]);
+      acc[6] = fmaf(z.z, f, acc[6]); acc[7] = fmaf(z.w, f, acc[7]);
+    }
+  }
+  if (d >= D) return;
+  const float inv = 1.0f / l;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    acc[k] = there ? acc[k] * inv : 0.0f;
+    if (there && a.gate)
+      acc[k] /= 1.0f + expf(-a.gate[(size_t)node * a.gate_pitch + (size_t)h * a.gate_head + d + k]);
+  }
+  *reinterpret_cast<uint4 *>(a.out + ((size_t)node * a.q_heads + h) * D + d) =
+      make_uint4(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]), pack_bf16x2(acc[4], acc[5]),
+                 pack_bf16x2(acc[6], acc[7]));
+}
+
+// How a call is cut: rows a tile, tiles, splits of the tokens.
+struct Plan {
+  int rows_tile, splits;
+  size_t items;
+};
+
+Plan plan_for(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, size_t max_seq) {
+  Plan p;
+  const size_t rows = nodes * (q_heads / kv_heads);
+  p.rows_tile = rows <= 8 ? 8 : 16;
+  p.items = batch * kv_heads * ((rows + p.rows_tile - 1) / p.rows_tile);
+  // two blocks an SM; at least 64 tokens a split (a step for each warp)
+  const size_t want = ((size_t)sm_count() * 2 + p.items - 1) / p.items;
+  p.splits = (int)std::max<size_t>(1, std::min(want, (max_seq + 63) / 64));
+  return p;
+}
+
+template <int DP, int NR>
+int run_rows(const TreeArgs &a, const Plan &p, cudaStream_t s) {
+  constexpr size_t smem = std::max(RowsShape<DP, NR>::smem, (size_t)NR * RowsShape<DP, NR>::kQPitch * 2);
+  if (smem > 40 * 1024) {
+    static std::mutex mu;
+    static std::vector<int> done;
+    int dev = 0;
+    FPB_CUDA_TRY(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lock(mu);
+    if (std::find(done.begin(), done.end(), dev) == done.end()) {
+      FPB_CUDA_TRY(cudaFuncSetAttribute(tree_attn_rows_kernel<DP, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)smem));
+      done.push_back(dev);
+    }
+  }
+  cudaError_t e = launch_pdl(tree_attn_rows_kernel<DP, NR>, dim3((unsigned)p.splits, (unsigned)p.items), kRowsThreads,
+                             smem, s, a);
+  if (e != cudaSuccess) return cuda_fail(e, "tree_attn_rows_kernel");
+  FPB_LAUNCH_CHECK("tree_attn_rows_kernel");
+  return FPB_OK;
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -99,8 +562,9 @@ using namespace fpb;
 
 extern "C" size_t fpb_tree_attn_workspace_bytes(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads,
                                                 size_t head_dim, size_t max_seq) {
-  (void)batch, (void)nodes, (void)q_heads, (void)kv_heads, (void)head_dim, (void)max_seq;
-  return 16;
+  if (batch == 0 || nodes == 0 || kv_heads == 0 || q_heads == 0 || q_heads % kv_heads) return 16;
+  const Plan p = plan_for(batch, nodes, q_heads, kv_heads, max_seq);
+  return p.splits == 1 ? 16 : p.items * p.splits * p.rows_tile * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int fpb_tree_attn(const void *q, int q_dtype, size_t q_pitch, size_t q_head_pitch, const uint8_t *k_codes,
@@ -126,6 +590,9 @@ extern "C" int fpb_tree_attn(const void *q, int q_dtype, size_t q_pitch, size_t 
   const size_t need = fpb_tree_attn_workspace_bytes(batch, nodes, q_heads, kv_heads, head_dim, max_seq);
   if (workspace_bytes < need)
     return fail(FPB_ERR_WORKSPACE, "fpb_tree_attn: workspace %zu < %zu bytes", workspace_bytes, need);
+  const Plan p = plan_for(batch, nodes, q_heads, kv_heads, max_seq);
+  if (p.items > 65535)
+    return fail(FPB_ERR_SHAPE, "fpb_tree_attn: %zu tiles of rows in one call (at most 65535)", p.items);
   TreeArgs a{};
   a.q = q;
   a.gate = gate;
@@ -142,15 +609,26 @@ extern "C" int fpb_tree_attn(const void *q, int q_dtype, size_t q_pitch, size_t 
   a.nodes = (int)nodes;
   a.q_heads = (int)q_heads;
   a.kv_heads = (int)kv_heads;
+  a.group = (int)(q_heads / kv_heads);
   a.head_dim = (int)head_dim;
   a.max_seq = (int)max_seq;
   a.q_bf16 = q_dtype == FPB_BF16;
-  a.scale = scale;
+  a.splits = p.splits;
+  a.scale_log2 = scale * 1.4426950408889634f;
   a.out = static_cast<__nv_bfloat16 *>(out_bf16);
+  a.part = static_cast<float *>(workspace);
+  a.part_ml = reinterpret_cast<float2 *>(a.part + p.items * p.splits * p.rows_tile * head_dim);
   a.error = device_error_ptr();
-  cudaError_t e = launch_pdl(tree_attn_kernel, dim3((unsigned)((q_heads + 7) / 8), (unsigned)(batch * nodes)), 256, 0,
-                             as_stream(stream), a);
-  if (e != cudaSuccess) return cuda_fail(e, "tree_attn_kernel");
-  FPB_LAUNCH_CHECK("tree_attn_kernel");
+  cudaStream_t s = as_stream(stream);
+  const bool few = p.rows_tile == 8;
+  const int st = head_dim <= 64    ? (few ? run_rows<64, 8>(a, p, s) : run_rows<64, 16>(a, p, s))
+                 : head_dim <= 128 ? (few ? run_rows<128, 8>(a, p, s) : run_rows<128, 16>(a, p, s))
+                                   : (few ? run_rows<256, 8>(a, p, s) : run_rows<256, 16>(a, p, s));
+  if (st || p.splits == 1) return st;
+  const int count = (int)(batch * nodes * q_heads);
+  cudaError_t e = launch_pdl(tree_attn_merge_kernel, dim3((unsigned)((count + 7) / 8)), 256, 0, s, a, p.rows_tile,
+                             count);
+  if (e != cudaSuccess) return cuda_fail(e, "tree_attn_merge_kernel");
+  FPB_LAUNCH_CHECK("tree_attn_merge_kernel");
   return FPB_OK;
 }

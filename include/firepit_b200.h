@@ -747,7 +747,7 @@ int fpb_moe_decode_combine_add_norm(const float *routed, const int32_t *map, con
  * v_exp [batch, max_seq, kv_heads], one exponent byte a head vector: value =
  * code * 2^(byte - 127); head_dim a multiple of 16 up to 256, codes 16-byte
  * aligned.  The exponent is the smallest e with max |x| <= 448 * 2^e within
- * [-100, 120] (-8 for zeros); codes round to nearest even; an infinity is
+ * [-100, 120], bytes 27 to 247 (-8 for zeros); codes round to nearest even; an infinity is
  * held as +-448 * 2^120 and a NaN stays one.
  *
  * Tree: parents [batch, nodes] int32, nodes <= 64: -1 for node 0 (the token
