@@ -9,9 +9,12 @@
 #include <vector>
 
 #include "kv8.cuh"
+#include "sm100.cuh"
 
 namespace fpb {
 namespace {
+
+using namespace sm100;
 
 struct TreeArgs {
   const void *q;
@@ -19,7 +22,7 @@ struct TreeArgs {
   const uint8_t *k_codes, *v_codes, *k_exp, *v_exp;
   const int32_t *positions, *parents;
   long long q_pitch, q_head, gate_pitch, gate_head;  // elements
-  int nodes, q_heads, kv_heads, group, head_dim, max_seq, q_bf16, splits;
+  int batch, nodes, q_heads, kv_heads, group, head_dim, max_seq, q_bf16, q_vec, splits;
   float scale_log2;  // scale * log2(e): scores and maxima are held in powers of two
   __nv_bfloat16 *out;
   float *part;     // [session, kv head, row tile][split][row][head_dim] numerators
@@ -514,21 +517,737 @@ __global__ void __launch_bounds__(256) tree_attn_merge_kernel(const __grid_const
                  pack_bf16x2(acc[6], acc[7]));
 }
 
-// How a call is cut: rows a tile, tiles, splits of the tokens.
+// ---- many rows: tiles on tcgen05 ----------------------------------------------------------------
+// Block: a share of the call's (session, kv head, 128-row tile, token tile)
+// units, in that order, so that sessions of any lengths load the SMs evenly;
+// a (row tile)'s token tiles that fall to several blocks meet in the merge.
+//   warps 0-3   softmax: thread r owns row r (TMEM lane r)
+//   warp 4      issues the MMAs
+//   warps 5-12  read codes and convert them to f16 tiles in shared memory
+// S = Q K^T and O += P V with Q and P as the A operand in TMEM, so shared
+// memory carries only what K and V need: 64 KB written and 64 KB read a tile
+// of 16384 elements each, against 1024 cycles of MMA.  A tile is 64 tokens at
+// head_dim 256, else 128: TMEM then holds O [DP], two S [BT] (P overwrites
+// its S) and Q [DP / 2 columns].
+//   K tile: tokens as rows of 128-byte swizzled lines, 64 dimensions a chunk
+//           (K-major).  Its codes take their exponent relative to the tile's
+//           largest on the way (exact until 2^-24 of it), which leaves one
+//           factor a tile for the scores.  Not so in a tile that some row does
+//           not see whole: what lies in rows that it does not see, which may
+//           be anything, would set that factor; the scores there take each
+//           token's own.
+//   V tile: the same bytes read as the transposed operand (N-major), its
+//           exponents in the weights (see kHead).
+constexpr int kTileWarps = 13, kTileThreads = kTileWarps * 32, kConvThreads = 256, kTileRows = 128;
+constexpr int kErrTileWait = 503;
+
+template <int DP>
+struct TileShape {
+  static constexpr int BT = DP == 256 ? 64 : 128, ST = 3, META = 8;
+  static constexpr uint32_t kBytes = BT * DP * 2;
+  static constexpr uint32_t kTmemO = 0, kTmemS = DP, kTmemQ = DP + 2 * BT;
+  static constexpr int kPieces = BT * DP / 16 / kConvThreads;  // 16-byte pieces of codes a thread and tile
+  static constexpr size_t smem = 1024 + 2 * ST * (size_t)kBytes + META * BT * 12;
+};
+
+// Token tiles of session b (0: none of its nodes is there).
+__device__ __forceinline__ int session_tiles(const TreeArgs &a, int b, int BT) {
+  if (a.parents && a.parents[(size_t)b * a.nodes] != -1) return 0;
+  return (seen_rows(a, a.positions[b], a.nodes - 1) + BT - 1) / BT;
+}
+
+// Units before session b (b = batch: all), warp-collective.
+__device__ __forceinline__ long long units_before(const TreeArgs &a, int b, int BT, int items) {
+  long long n = 0;
+  const int lane = threadIdx.x & 31;
+  for (int i = lane; i < b; i += 32) n += session_tiles(a, i, BT);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  return n * items;
+}
+
+struct Segment {
+  int b, kvh, rt, j0, j1, pos, total;
+  bool whole;
+};
+
+// A block's units, one segment (token tiles [j0, j1) of one row tile) at a time.
+struct Walk {
+  int b, tiles, row_tiles;
+  long long rem, left;
+  __device__ __forceinline__ bool next(const TreeArgs &a, int BT, Segment &s) {
+    if (left <= 0) return false;
+    const int items = a.kv_heads * row_tiles;
+    while (rem >= (long long)items * tiles) {
+      rem -= (long long)items * tiles;
+      tiles = session_tiles(a, ++b, BT);
+    }
+    const int item = (int)(rem / tiles);
+    s.j0 = (int)(rem % tiles);
+    const int n = (int)min(left, (long long)(tiles - s.j0));
+    s.whole = n == tiles;
+    left -= n;
+    rem += n;
+    s.b = b;
+    s.kvh = item / row_tiles;
+    s.rt = item % row_tiles;
+    s.pos = a.positions[b];
+    // a chain's row tile ends at its last node's own row
+    s.total = seen_rows(a, s.pos, min(a.nodes - 1, (s.rt * kTileRows + kTileRows - 1) / a.group));
+    s.j1 = min(s.j0 + n, (s.total + BT - 1) / BT);
+    return true;
+  }
+};
+
+__device__ __forceinline__ void give_up(int *error, volatile int *abort) {
+  *abort = 1;
+  if (error) atomicCAS(error, 0, kErrTileWait);
+}
+
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// One row of S [BT] from TMEM: y = s * f + the value's exponent; returns the
+// largest y.  WEIGH: also the weights 2^(y + base) as f16 pairs in p and their
+// sum without the exponents in l.  OPEN: a tile that not every row sees whole.
+template <int BT, bool OPEN, bool WEIGH>
+__device__ __forceinline__ float softmax_pass(uint32_t s_tmem, const float4 *meta, const float *kf, float f, float base,
+                                              const Sight &sight, int t0, int pos, int total, bool tree,
+                                              uint32_t (&p)[BT / 2], uint64_t &l) {
+  const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
+  float mx = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < BT / 32; ++c) {
+    uint32_t r[32];
+    tmem_ld32(s_tmem + c * 32, r);
+    tmem_ld_wait(r);
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      const float4 mt = meta[(c * 32 + e) / 2];  // exponents, then their inverse powers
+      float s0 = __uint_as_float(r[e]), s1 = __uint_as_float(r[e + 1]);
+      if (OPEN) {
+        s0 *= kf[c * 32 + e];
+        s1 *= kf[c * 32 + e + 1];
+      }
+      uint64_t y = fma2(pack2(s0, s1), f2, pack2(mt.x, mt.y));
+      float y0, y1;
+      unpack2(y, y0, y1);
+      if (OPEN) {
+        const int t = t0 + c * 32 + e;
+        if (t >= total || !sight.sees(t, pos, tree)) y0 = -INFINITY;
+        if (t + 1 >= total || !sight.sees(t + 1, pos, tree)) y1 = -INFINITY;
+        y = pack2(y0, y1);
+      }
+      mx = fmaxf(mx, fmaxf(y0, y1));
+      if (WEIGH) {
+        float p0, p1;
+        unpack2(add2(y, b2), p0, p1);
+        p0 = exp2_approx(p0);
+        p1 = exp2_approx(p1);
+        l = fma2(pack2(p0, p1), pack2(mt.z, mt.w), l);
+        p[(c * 32 + e) / 2] = pack_f16x2(p0, p1);
+      }
+    }
+  }
+  return mx;
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kTileThreads, 1) tree_attn_tile_kernel(const __grid_constant__ TreeArgs a) {
+  pdl_enter();
+  using Sh = TileShape<DP>;
+  constexpr int BT = Sh::BT, ST = Sh::ST, META = Sh::META;
+  extern __shared__ uint8_t raw_sm[];
+  __shared__ uint64_t kfull[ST], kempty[ST], vfull[ST], vempty[ST], sfull[2], pready[2], metafull[META], qready, drain;
+  __shared__ int kref_s[META];
+  __shared__ uint32_t tmem_s;
+  __shared__ int abort_word, never_s, b_s, tiles_s;
+  __shared__ long long rem_s, left_s;
+  volatile int *abort_s = &abort_word;
+  uint8_t *sK = reinterpret_cast<uint8_t *>(((uintptr_t)raw_sm + 1023) & ~(uintptr_t)1023);
+  uint8_t *sV = sK + ST * Sh::kBytes;
+  float4 *meta_s = reinterpret_cast<float4 *>(sV + ST * Sh::kBytes);  // [META][BT / 2]
+  float *kf_s = reinterpret_cast<float *>(meta_s + META * (BT / 2));   // [META][BT], open tiles only
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rows = a.nodes * a.group, row_tiles = (rows + kTileRows - 1) / kTileRows, D = a.head_dim;
+  const bool tree = a.parents != nullptr;
+  if (warp == 0) {  // this block's share of the units
+    const int items = a.kv_heads * row_tiles;
+    const long long units = units_before(a, a.batch, BT, items);
+    const long long blocks = min((long long)gridDim.x, units);
+    long long u0 = 0, u1 = 0;
+    if (blockIdx.x < blocks) {
+      u0 = units * blockIdx.x / blocks;
+      u1 = units * (blockIdx.x + 1) / blocks;
+    }
+    int b = 0;  // the session that holds unit u0
+    long long before = 0;
+    if (u1 > u0)
+      for (int i0 = 0; i0 < a.batch; i0 += 32) {
+        const int n = i0 + lane < a.batch ? session_tiles(a, i0 + lane, BT) : 0;
+        long long sum = (long long)n * items;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long v = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += v;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, before + sum > u0);
+        if (past) {
+          const int k = __ffs(past) - 1;
+          b = i0 + k;
+          before += __shfl_sync(0xffffffffu, sum - (long long)n * items, k);
+          break;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+      }
+    if (lane == 0) {
+      b_s = b;
+      tiles_s = u1 > u0 ? session_tiles(a, b, BT) : 1;
+      rem_s = u0 - before;
+      left_s = u1 - u0;
+    }
+  }
+  if (warp == 4) {
+    if (lane == 0) {
+      for (int i = 0; i < ST; ++i) {
+        mbar_init(&kfull[i], kConvThreads / 32);
+        mbar_init(&vfull[i], kConvThreads / 32);
+        mbar_init(&kempty[i], 1);
+        mbar_init(&vempty[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sfull[i], 1);
+        mbar_init(&pready[i], 4);
+      }
+      for (int i = 0; i < META; ++i) mbar_init(&metafull[i], 1);
+      mbar_init(&qready, 4);
+      mbar_init(&drain, 1);
+      abort_word = never_s = 0;
+      fence_barrier_init();
+    }
+    __syncwarp();
+    tmem_alloc(&tmem_s, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_s;
+  Walk walk{b_s, tiles_s, row_tiles, rem_s, left_s};
+  Segment sg;
+
+  if (warp < 4) {
+    // ---- softmax ----
+    const uint32_t my = tmem + ((uint32_t)(warp * 32) << 16);
+    uint32_t g = 0;  // tiles so far
+    bool ok = true;
+    for (int seg = 0; ok && walk.next(a, BT, sg); ++seg) {
+      const int row = sg.rt * kTileRows + tid, n = row / a.group, h = sg.kvh * a.group + row % a.group;
+      const bool in = row < rows;
+      const Sight sight = sight_of(a, sg.b, in ? n : a.nodes, sg.pos);
+      const size_t node = (size_t)sg.b * a.nodes + n;
+      float m = -INFINITY, fac;
+      uint64_t l2 = 0;
+      {  // the row's query, scaled into f16, to TMEM
+        const size_t at = node * a.q_pitch + (size_t)h * a.q_head;
+        auto piece = [&](int d, float(&x)[8]) {
+          if (!in || d >= D) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+          } else if (!a.q_vec) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = load_q(a, at + d + i);
+          } else if (a.q_bf16) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) + at + d);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              x[2 * i] = __uint_as_float(w[i] << 16);
+              x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+          } else {
+            const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at + d);
+            const float4 u = p[0], v = p[1];
+            x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+            x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+          }
+        };
+        float amax = 0.0f;
+        for (int d = 0; d < D; d += 8) {
+          float x[8];
+          piece(d, x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
+        }
+        const int e = q_exponent(amax);
+        const float inv = pow2i(-e);
+        fac = pow2i(e) * a.scale_log2;
+        for (int d = 0; d < D; d += 64) {
+          uint32_t w[32];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float x[8];
+            piece(d + 8 * j, x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[4 * j + i] = pack_f16x2(x[2 * i] * inv, x[2 * i + 1] * inv);
+          }
+          tmem_st32(my + Sh::kTmemQ + d / 2, w);
+        }
+        tmem_st_wait();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&qready);
+      for (int j = sg.j0; j < sg.j1; ++j, ++g) {
+        const int t0 = j * BT;
+        const bool open = t0 + BT > sg.pos;
+        ok = mbar_wait(&sfull[g & 1], (g >> 1) & 1, abort_s) && mbar_wait(&metafull[g % META], (g / META) & 1, abort_s);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {
+          give_up(a.error, abort_s);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t s_tmem = my + Sh::kTmemS + (g & 1) * BT;
+        const float4 *meta = meta_s + (size_t)(g % META) * (BT / 2);
+        const float *kf = kf_s + (size_t)(g % META) * BT;
+        const float f = fac * pow2i(kref_s[g % META]);
+        uint32_t p[BT / 2];
+        const uint64_t l_old = l2;
+        bool grow = true;
+        float mx;
+        if (j > sg.j0) {  // with the maximum so far; again where it has grown too much
+          const float base = m == -INFINITY ? 0.0f : kHead - m;
+          mx = open ? softmax_pass<BT, true, true>(s_tmem, meta, kf, f, base, sight, t0, sg.pos, sg.total, tree, p, l2)
+                    : softmax_pass<BT, false, true>(s_tmem, meta, kf, f, base, sight, t0, sg.pos, sg.total, tree, p, l2);
+          grow = mx > m + kLag || (m == -INFINITY && mx > m);
+          grow = __any_sync(0xffffffffu, grow);
+        } else {
+          mx = open ? softmax_pass<BT, true, false>(s_tmem, meta, kf, f, 0.0f, sight, t0, sg.pos, sg.total, tree, p, l2)
+                    : softmax_pass<BT, false, false>(s_tmem, meta, kf, f, 0.0f, sight, t0, sg.pos, sg.total, tree, p, l2);
+        }
+        if (grow) {
+          const float mn = fmaxf(m, mx);
+          const float old = m == -INFINITY ? 0.0f : exp2_approx(m - mn);
+          m = mn;
+          l2 = fma2(l_old, pack2(old, old), 0);
+          if (j > sg.j0) {  // O of the tiles before takes the new maximum, once they are in it
+            const uint32_t q = g - 1;
+            ok = __all_sync(0xffffffffu, mbar_wait(&vempty[q % ST], (q / ST) & 1, abort_s));
+            if (!ok) {
+              give_up(a.error, abort_s);
+              break;
+            }
+            tc_fence_after();
+            for (int d = 0; d < D; d += 32) {
+              uint32_t r[32];
+              tmem_ld32(my + Sh::kTmemO + d, r);
+              tmem_ld_wait(r);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * old);
+              tmem_st32(my + Sh::kTmemO + d, r);
+            }
+          }
+          const float base = m == -INFINITY ? 0.0f : kHead - m;
+          if (open)
+            softmax_pass<BT, true, true>(s_tmem, meta, kf, f, base, sight, t0, sg.pos, sg.total, tree, p, l2);
+          else
+            softmax_pass<BT, false, true>(s_tmem, meta, kf, f, base, sight, t0, sg.pos, sg.total, tree, p, l2);
+        }
+#pragma unroll
+        for (int i = 0; i < BT / 64; ++i) tmem_st32(s_tmem + 32 * i, p + 32 * i);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pready[g & 1]);
+      }
+      if (!ok) break;
+      float l0, l1;
+      unpack2(l2, l0, l1);
+      const float l = l0 + l1;
+      if (sg.j1 > sg.j0) {
+        const uint32_t q = g - 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&vempty[q % ST], (q / ST) & 1, abort_s));
+        if (!ok) {
+          give_up(a.error, abort_s);
+          break;
+        }
+        tc_fence_after();
+      }
+      const size_t slot = ((size_t)blockIdx.x * 2 + (seg ? 1 : 0)) * kTileRows + tid;
+      if (!sg.whole) a.part_ml[slot] = make_float2(sg.j1 > sg.j0 ? m : -INFINITY, l);
+      const bool there = sight.upto >= 0;
+      const float inv = there ? 1.0f / l : 0.0f;
+      for (int d = 0; d < D && sg.j1 > sg.j0; d += 32) {
+        uint32_t r[32];
+        tmem_ld32(my + Sh::kTmemO + d, r);
+        tmem_ld_wait(r);
+        if (!sg.whole) {
+          float4 *o = reinterpret_cast<float4 *>(a.part + slot * D + d);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (d + 4 * i < D)
+              o[i] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]),
+                                 __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
+        } else if (in) {
+          float x[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = there ? __uint_as_float(r[i]) * inv : 0.0f;
+          if (a.gate && there) {
+            const float *gt = a.gate + node * a.gate_pitch + (size_t)h * a.gate_head + d;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (d + i < D) x[i] /= 1.0f + expf(-gt[i]);
+          }
+          uint4 *o = reinterpret_cast<uint4 *>(a.out + (node * a.q_heads + h) * D + d);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (d + 8 * i < D)
+              o[i] = make_uint4(pack_bf16x2(x[8 * i], x[8 * i + 1]), pack_bf16x2(x[8 * i + 2], x[8 * i + 3]),
+                                pack_bf16x2(x[8 * i + 4], x[8 * i + 5]), pack_bf16x2(x[8 * i + 6], x[8 * i + 7]));
+        }
+      }
+      tc_fence_before();  // O is read: the next segment's products may overwrite it
+    }
+  } else if (warp == 4) {
+    // ---- MMA issue ----
+    if (lane == 0) {
+      const uint32_t idesc_s = idesc_f16(128, BT, false), idesc_o = idesc_f16(128, D, true);
+      uint32_t g = 0;
+      bool ok = true;
+      auto scores = [&](uint32_t i) {
+        const int st = i % ST;
+        ok = ok && mbar_wait(&kfull[st], (i / ST) & 1, abort_s);
+        // S of tile i lies where P of tile i - 2 was: its product is done
+        if (ok && i >= 2) ok = mbar_wait(&vempty[(i - 2) % ST], ((i - 2) / ST) & 1, abort_s);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t base = smem_u32(sK + st * Sh::kBytes);
+        for (int k = 0; k < D / 16; ++k)
+          mma_f16_ts(tmem + Sh::kTmemS + (i & 1) * BT, tmem + Sh::kTmemQ + 8 * k,
+                     smem_desc(base + (k >> 2) * (BT * 128) + (k & 3) * 32, 16, 1024, 2), idesc_s, k > 0);
+        tc_commit(&kempty[st]);
+        tc_commit(&sfull[i & 1]);
+      };
+      for (int seg = 0; ok && walk.next(a, BT, sg); ++seg) {
+        ok = mbar_wait(&qready, seg & 1, abort_s);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t g0 = g, g1 = g + max(0, sg.j1 - sg.j0);
+        if (g1 > g0) scores(g0);
+        for (; ok && g < g1; ++g) {
+          if (g + 1 < g1) scores(g + 1);
+          const int st = g % ST;
+          ok = ok && mbar_wait(&pready[g & 1], (g >> 1) & 1, abort_s) && mbar_wait(&vfull[st], (g / ST) & 1, abort_s);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t base = smem_u32(sV + st * Sh::kBytes);
+          for (int k = 0; k < BT / 16; ++k)
+            mma_f16_ts(tmem + Sh::kTmemO, tmem + Sh::kTmemS + (g & 1) * BT + 8 * k,
+                       smem_desc(base + k * 2048, BT * 128, 1024, 2), idesc_o, g > g0 || k > 0);
+          tc_commit(&vempty[st]);
+        }
+      }
+      if (!ok) {  // what was issued ends before its TMEM is given back
+        give_up(a.error, abort_s);
+        tc_commit(&drain);
+        mbar_wait(&drain, 0, &never_s);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- codes to f16 tiles ----
+    const int ct = tid - 5 * 32, cw = ct >> 5;
+    constexpr int P = Sh::kPieces, X = BT / 32;
+    const int per = D / 16;  // pieces a token
+    int tok[P];
+    uint32_t src[P], dst[P];
+    bool flip = false;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int idx = i * kConvThreads + ct;
+      tok[i] = idx / per;
+      const int ch = idx % per;
+      src[i] = (uint32_t)ch * 16;
+      // the lanes of odd chunks write their second half first, so that eight
+      // lanes' 16-byte stores fall on all banks
+      const int first = (ch >> 2) & 1;
+      flip = first;
+      dst[i] = (uint32_t)((ch >> 2) * (BT * 128) + tok[i] * 128 + (((2 * (ch & 3) + first) ^ (tok[i] & 7)) * 16));
+      if (tok[i] >= BT) tok[i] = 1 << 30;
+      if (flip) src[i] |= 1u << 31;
+    }
+    Walk ahead = walk;
+    Segment na;
+    int jn = 0;
+    bool more = ahead.next(a, BT, na);
+    while (more && na.j1 <= na.j0) more = ahead.next(a, BT, na);
+    jn = more ? na.j0 : 0;
+    uint4 kb[P], vb[P];
+    uint32_t xk[P], xa[X], xv[X];
+    auto load_k = [&]() {
+      const size_t row = (size_t)na.b * a.max_seq + jn * BT;
+      const uint8_t *e = a.k_exp + row * a.kv_heads + na.kvh;
+      const uint8_t *c = a.k_codes + (row * a.kv_heads + na.kvh) * D;
+      const int live = na.total - jn * BT;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const bool in = tok[i] < live && tok[i] < BT;
+        kb[i] = in ? __ldg(reinterpret_cast<const uint4 *>(c + (size_t)tok[i] * a.kv_heads * D + (src[i] & 0x7fffffffu)))
+                   : make_uint4(0, 0, 0, 0);
+        xk[i] = in ? e[(size_t)tok[i] * a.kv_heads] : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < X; ++i) {
+        const int t = lane + 32 * i;
+        xa[i] = t < live ? e[(size_t)t * a.kv_heads] : 0;
+      }
+      if (cw == 0) {
+        const uint8_t *ev = a.v_exp + row * a.kv_heads + na.kvh;
+#pragma unroll
+        for (int i = 0; i < X; ++i) {
+          const int t = lane + 32 * i;
+          xv[i] = t < live ? ev[(size_t)t * a.kv_heads] : 127;
+        }
+      }
+    };
+    auto load_v = [&]() {
+      const size_t row = (size_t)na.b * a.max_seq + jn * BT;
+      const uint8_t *c = a.v_codes + (row * a.kv_heads + na.kvh) * D;
+      const int live = na.total - jn * BT;
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        vb[i] = tok[i] < live && tok[i] < BT
+                    ? __ldg(reinterpret_cast<const uint4 *>(c + (size_t)tok[i] * a.kv_heads * D + (src[i] & 0x7fffffffu)))
+                    : make_uint4(0, 0, 0, 0);
+    };
+    auto store = [&](uint8_t *stage, int i, uint4 v, __half2 f, bool scaled) {
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      uint32_t o[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        o[k] = e4m3x2_to_f16x2((uint16_t)(w[k >> 1] >> (16 * (k & 1))));
+        if (scaled) {
+          const __half2 x = __hmul2(*reinterpret_cast<__half2 *>(&o[k]), f);
+          o[k] = *reinterpret_cast<const uint32_t *>(&x);
+        }
+      }
+      const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+      const bool fl = src[i] >> 31;
+      *reinterpret_cast<uint4 *>(stage + dst[i]) = fl ? hi : lo;
+      *reinterpret_cast<uint4 *>(stage + (dst[i] ^ 16)) = fl ? lo : hi;
+    };
+    if (more) {
+      load_k();
+      load_v();
+    }
+    // After a wait that ran out this role goes on to its end without waiting
+    // (the results are void): its warps meet at a barrier in open tiles.
+    bool ok = true;
+    for (uint32_t g = 0; more; ++g) {
+      const int st = g % ST;
+      const bool open = (jn + 1) * BT > na.pos;
+      // what the softmax needs of this tile's tokens
+      int ref = 0;
+#pragma unroll
+      for (int i = 0; i < X; ++i) ref = max(ref, (int)xa[i]);
+      ref = open ? 0 : min(kKv8MaxExp, max(kKv8MinExp, (int)__reduce_max_sync(0xffffffffu, (unsigned)ref) - 127));
+      float *mt = reinterpret_cast<float *>(meta_s + (size_t)(g % META) * (BT / 2));
+      if (g >= ST && ok) ok = mbar_wait(&kempty[st], ((g / ST) - 1) & 1, abort_s);
+      ok = __all_sync(0xffffffffu, ok);
+      if (cw == 0) {
+#pragma unroll
+        for (int i = 0; i < X; ++i) {
+          const int t = lane + 32 * i;
+          const float ve = kv8_value_exponent(xv[i]);
+          mt[(t >> 1) * 4 + (t & 1)] = ve;
+          mt[(t >> 1) * 4 + 2 + (t & 1)] = pow2i(-(int)ve);
+          if (open) kf_s[(g % META) * BT + t] = kv8_factor(xa[i]);
+        }
+        if (lane == 0) kref_s[g % META] = ref;
+      }
+      if (open) {  // values that are not a number: zero in the product, and the token's score NaN for those who see it
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          uint32_t w[4] = {vb[i].x, vb[i].y, vb[i].z, vb[i].w}, any = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t bad = __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            w[k] &= ~bad;
+            any |= bad;
+          }
+          vb[i] = make_uint4(w[0], w[1], w[2], w[3]);
+          if (any && tok[i] < BT) mt[(tok[i] >> 1) * 4 + (tok[i] & 1)] = __int_as_float(0x7fc00000);
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+      __syncwarp();
+      if (cw == 0 && lane == 0) mbar_arrive(&metafull[g % META]);
+      uint8_t *stage = sK + st * Sh::kBytes;
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        if (tok[i] < BT)
+          store(stage, i, kb[i], __float2half2_rn(pow2i(open ? 0 : max(-30, min(0, (int)xk[i] - 127 - ref)))), true);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&kfull[st]);
+      // the next tile's keys are on their way while this one's values are stored
+      const bool last = jn + 1 >= na.j1;
+      if (last) {
+        more = ahead.next(a, BT, na);
+        while (more && na.j1 <= na.j0) more = ahead.next(a, BT, na);
+        jn = more ? na.j0 : 0;
+      } else {
+        ++jn;
+      }
+      if (more) load_k();
+      if (g >= ST && ok) ok = mbar_wait(&vempty[st], ((g / ST) - 1) & 1, abort_s);
+      ok = __all_sync(0xffffffffu, ok);
+      stage = sV + st * Sh::kBytes;
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        if (tok[i] < BT) store(stage, i, vb[i], __half2(), false);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&vfull[st]);
+      if (more) load_v();
+    }
+    if (!ok) give_up(a.error, abort_s);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// The blocks that share a row's tokens meet, in order: one warp a (session,
+// node, query head).  Rows of one block are written already; rows of nodes
+// that are not there become zeros.
+__global__ void __launch_bounds__(256) tree_attn_tile_merge_kernel(const __grid_constant__ TreeArgs a, int BT,
+                                                                   int grid, int count) {
+  pdl_enter();
+  const int lane = threadIdx.x & 31, i = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (i >= count) return;
+  const int h = i % a.q_heads, node = i / a.q_heads, b = node / a.nodes, n = node % a.nodes, D = a.head_dim;
+  const int kvh = h / a.group, row = n * a.group + h % a.group;
+  const int row_tiles = (a.nodes * a.group + kTileRows - 1) / kTileRows, items = a.kv_heads * row_tiles;
+  const int d = lane * 8;
+  uint4 *out = reinterpret_cast<uint4 *>(a.out + ((size_t)node * a.q_heads + h) * D + d);
+  const int tiles = session_tiles(a, b, BT);
+  if (tiles == 0 || sight_of(a, b, n, a.positions[b]).upto < 0) {
+    if (d < D) *out = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const long long before = units_before(a, b, BT, items), units = units_before(a, a.batch, BT, items);
+  const long long blocks = min((long long)grid, units);
+  const long long ua = before + (long long)(kvh * row_tiles + row / kTileRows) * tiles, ub = ua + tiles;
+  const int c0 = (int)(((ua + 1) * blocks - 1) / units), c1 = (int)((ub * blocks - 1) / units);
+  if (c0 == c1) return;
+  // the block that the row tile begins in holds it as its last segment, unless it begins there
+  const int first = units * c0 / blocks < ua ? 1 : 0;
+  auto slot = [&](int c) { return ((size_t)c * 2 + (c == c0 ? first : 0)) * kTileRows + row % kTileRows; };
+  float m = -INFINITY, l = 0.0f;
+  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, a.part_ml[slot(c)].x);
+  m = warp_max(m);
+  float acc[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c) {
+    const size_t s = slot(c);
+    const float2 v = a.part_ml[s];
+    if (v.x == -INFINITY) continue;
+    const float f = exp2_approx(v.x - m);
+    l = fmaf(v.y, f, l);
+    if (d < D) {
+      const float4 *p = reinterpret_cast<const float4 *>(a.part + s * D + d);
+      const float4 x = p[0], z = p[1];
+      acc[0] = fmaf(x.x, f, acc[0]); acc[1] = fmaf(x.y, f, acc[1]);
+      acc[2] = fmaf(x.z, f, acc[2]); acc[3] = fmaf(x.w, f, acc[3]);
+      acc[4] = fmaf(z.x, f, acc[4]); acc[5] = fmaf(z.y, f, acc[5]);
+      acc[6] = fmaf(z.z, f, acc[6]); acc[7] = fmaf(z.w, f, acc[7]);
+    }
+  }
+  if (d >= D) return;
+  const float inv = 1.0f / l;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    acc[k] *= inv;
+    if (a.gate) acc[k] /= 1.0f + expf(-a.gate[(size_t)node * a.gate_pitch + (size_t)h * a.gate_head + d + k]);
+  }
+  *out = make_uint4(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]), pack_bf16x2(acc[4], acc[5]),
+                    pack_bf16x2(acc[6], acc[7]));
+}
+
+// How a call is cut.  tiles: the tcgen05 kernel, `blocks` of them; else rows a
+// tile, tiles and splits of the tokens.
 struct Plan {
-  int rows_tile, splits;
+  bool tiles;
+  int rows_tile, splits, blocks, BT;
   size_t items;
 };
 
-Plan plan_for(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, size_t max_seq) {
-  Plan p;
+Plan plan_for(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, size_t head_dim, size_t max_seq) {
+  Plan p{};
   const size_t rows = nodes * (q_heads / kv_heads);
+  if (rows > 16) {
+    p.tiles = true;
+    p.BT = head_dim > 128 ? 64 : 128;
+    p.items = batch * kv_heads * ((rows + kTileRows - 1) / kTileRows);
+    const size_t most = p.items * ((max_seq + p.BT - 1) / p.BT);
+    p.blocks = (int)std::min<size_t>(sm_count(), most);
+    return p;
+  }
   p.rows_tile = rows <= 8 ? 8 : 16;
   p.items = batch * kv_heads * ((rows + p.rows_tile - 1) / p.rows_tile);
   // two blocks an SM; at least 64 tokens a split (a step for each warp)
   const size_t want = ((size_t)sm_count() * 2 + p.items - 1) / p.items;
   p.splits = (int)std::max<size_t>(1, std::min(want, (max_seq + 63) / 64));
   return p;
+}
+
+template <int DP>
+int run_tiles(const TreeArgs &a, const Plan &p, cudaStream_t s) {
+  constexpr size_t smem = TileShape<DP>::smem;
+  {
+    static std::mutex mu;
+    static std::vector<int> done;
+    int dev = 0;
+    FPB_CUDA_TRY(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lock(mu);
+    if (std::find(done.begin(), done.end(), dev) == done.end()) {
+      FPB_CUDA_TRY(cudaFuncSetAttribute(tree_attn_tile_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)smem));
+      done.push_back(dev);
+    }
+  }
+  cudaError_t e = launch_pdl(tree_attn_tile_kernel<DP>, dim3((unsigned)p.blocks), kTileThreads, smem, s, a);
+  if (e != cudaSuccess) return cuda_fail(e, "tree_attn_tile_kernel");
+  FPB_LAUNCH_CHECK("tree_attn_tile_kernel");
+  const int count = a.batch * a.nodes * a.q_heads;
+  e = launch_pdl(tree_attn_tile_merge_kernel, dim3((unsigned)((count + 7) / 8)), 256, 0, s, a, p.BT, p.blocks, count);
+  if (e != cudaSuccess) return cuda_fail(e, "tree_attn_tile_merge_kernel");
+  FPB_LAUNCH_CHECK("tree_attn_tile_merge_kernel");
+  return FPB_OK;
 }
 
 template <int DP, int NR>
@@ -563,7 +1282,8 @@ using namespace fpb;
 extern "C" size_t fpb_tree_attn_workspace_bytes(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads,
                                                 size_t head_dim, size_t max_seq) {
   if (batch == 0 || nodes == 0 || kv_heads == 0 || q_heads == 0 || q_heads % kv_heads) return 16;
-  const Plan p = plan_for(batch, nodes, q_heads, kv_heads, max_seq);
+  const Plan p = plan_for(batch, nodes, q_heads, kv_heads, head_dim, max_seq);
+  if (p.tiles) return (size_t)p.blocks * 2 * kTileRows * (head_dim + 2) * sizeof(float);
   return p.splits == 1 ? 16 : p.items * p.splits * p.rows_tile * (head_dim + 2) * sizeof(float);
 }
 
@@ -590,8 +1310,8 @@ extern "C" int fpb_tree_attn(const void *q, int q_dtype, size_t q_pitch, size_t 
   const size_t need = fpb_tree_attn_workspace_bytes(batch, nodes, q_heads, kv_heads, head_dim, max_seq);
   if (workspace_bytes < need)
     return fail(FPB_ERR_WORKSPACE, "fpb_tree_attn: workspace %zu < %zu bytes", workspace_bytes, need);
-  const Plan p = plan_for(batch, nodes, q_heads, kv_heads, max_seq);
-  if (p.items > 65535)
+  const Plan p = plan_for(batch, nodes, q_heads, kv_heads, head_dim, max_seq);
+  if (p.items > 65535 || batch * nodes * q_heads > 0x7fffffff)
     return fail(FPB_ERR_SHAPE, "fpb_tree_attn: %zu tiles of rows in one call (at most 65535)", p.items);
   TreeArgs a{};
   a.q = q;
@@ -606,6 +1326,7 @@ extern "C" int fpb_tree_attn(const void *q, int q_dtype, size_t q_pitch, size_t 
   a.q_head = (long long)q_head_pitch;
   a.gate_pitch = (long long)gate_pitch;
   a.gate_head = (long long)gate_head_pitch;
+  a.batch = (int)batch;
   a.nodes = (int)nodes;
   a.q_heads = (int)q_heads;
   a.kv_heads = (int)kv_heads;
@@ -613,13 +1334,17 @@ extern "C" int fpb_tree_attn(const void *q, int q_dtype, size_t q_pitch, size_t 
   a.head_dim = (int)head_dim;
   a.max_seq = (int)max_seq;
   a.q_bf16 = q_dtype == FPB_BF16;
+  a.q_vec = aligned16(q) && (q_pitch | q_head_pitch) * (q_dtype == FPB_F32 ? 4 : 2) % 16 == 0;
   a.splits = p.splits;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.out = static_cast<__nv_bfloat16 *>(out_bf16);
   a.part = static_cast<float *>(workspace);
-  a.part_ml = reinterpret_cast<float2 *>(a.part + p.items * p.splits * p.rows_tile * head_dim);
+  a.part_ml = reinterpret_cast<float2 *>(
+      a.part + (p.tiles ? (size_t)p.blocks * 2 * kTileRows : p.items * p.splits * p.rows_tile) * head_dim);
   a.error = device_error_ptr();
   cudaStream_t s = as_stream(stream);
+  if (p.tiles)
+    return head_dim <= 64 ? run_tiles<64>(a, p, s) : head_dim <= 128 ? run_tiles<128>(a, p, s) : run_tiles<256>(a, p, s);
   const bool few = p.rows_tile == 8;
   const int st = head_dim <= 64    ? (few ? run_rows<64, 8>(a, p, s) : run_rows<64, 16>(a, p, s))
                  : head_dim <= 128 ? (few ? run_rows<128, 8>(a, p, s) : run_rows<128, 16>(a, p, s))

@@ -758,6 +758,7 @@ int fpb_moe_decode_combine_add_norm(const float *routed, const int32_t *map, con
  * [0, position), its ancestors and itself, and is rotated by position +
  * depth(i).  Rows of q_out and attention outputs of nodes that are not there
  * are zeros, and nothing is written for them.  Device errors (fpb_device_error):
+ * 503 a wait inside a kernel ran out (the results are not to be used),
  * 502 a row outside [0, max_seq) (the node counts as not there), 504 a parent
  * that is not an earlier node (likewise) or a path that does not ascend, 505 a
  * token outside the vocabulary (refused). */
