@@ -36,6 +36,17 @@ struct TreeArgs {
 struct Sight {
   int upto;
   uint64_t bits;
+  // Which of the 64 rows from t0 on it sees.
+  __device__ __forceinline__ uint64_t seen64(int t0, int pos, bool tree) const {
+    const int k = pos - t0;  // rows of the context among them
+    if (!tree) {
+      const int c = k + max(upto, 0);
+      return c >= 64 ? ~0ull : c <= 0 ? 0ull : (1ull << c) - 1;
+    }
+    if (k >= 64) return ~0ull;
+    if (k > 0) return ((1ull << k) - 1) | bits << k;
+    return k > -64 ? bits >> -k : 0ull;
+  }
   __device__ __forceinline__ bool sees(int t, int pos, bool tree) const {
     const int j = t - pos;
     if (j < 0) return true;
@@ -43,25 +54,43 @@ struct Sight {
   }
 };
 
+// The tree is walked through the warp's registers: all 32 lanes call this, each
+// with its own node (n >= nodes: none).
 __device__ __forceinline__ Sight sight_of(const TreeArgs &a, int b, int n, int pos) {
   Sight s{-1, 0};
-  if (n >= a.nodes) return s;
-  if (pos < 0 || pos >= a.max_seq - n) {
-    if (a.error) atomicCAS(a.error, 0, kErrPosition);
-    return s;
-  }
+  const bool in = n < a.nodes;
+  const bool inside = pos >= 0 && pos < a.max_seq - n;
+  if (in && !inside && a.error) atomicCAS(a.error, 0, kErrPosition);
   if (!a.parents) {
-    s.upto = n + 1;
+    if (in && inside) s.upto = n + 1;
     return s;
   }
   const int32_t *par = a.parents + (size_t)b * a.nodes;
-  bool bad = false;
-  if (tree_depth(par, n, &bad) >= 0) {
+  const int lane = threadIdx.x & 31;
+  const int p0 = lane < a.nodes ? par[lane] : -2, p1 = lane + 32 < a.nodes ? par[lane + 32] : -2;
+  const int root = __shfl_sync(0xffffffffu, p0, 0);  // (by every lane, outside the conditions)
+  bool there = in && inside && root == -1;
+  bool going = there && n > 0;
+  int j = in ? n : 0;
+  while (__any_sync(0xffffffffu, going)) {
+    const int lo = __shfl_sync(0xffffffffu, p0, j & 31), hi = __shfl_sync(0xffffffffu, p1, j & 31);
+    const int p = j < 32 ? lo : hi;
+    if (going) {
+      if (p < 0 || p >= j) {
+        if (p >= j && a.error) atomicCAS(a.error, 0, kErrParent);
+        there = going = false;
+      } else {
+        s.bits |= 1ull << j;
+        j = p;
+        going = j > 0;
+      }
+    }
+  }
+  if (there) {
     s.upto = n + 1;
-    for (int j = n; j > 0; j = par[j]) s.bits |= 1ull << j;
     s.bits |= 1;
-  } else if (bad && a.error) {
-    atomicCAS(a.error, 0, kErrParent);
+  } else {
+    s.bits = 0;
   }
   return s;
 }
@@ -109,7 +138,7 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
 // the value vector's own exponent: f16 then holds a weight down to 2^-32 of
 // the row's largest, and the exponent costs no multiplication.  The maximum
 // may lag by kLag before the sums are rescaled (weights up to 2^(kHead + kLag)).
-constexpr float kHead = 7.0f, kLag = 8.0f;
+constexpr float kHead = 7.0f, kLag = 8.0f, kMost = 32768.0f, kLowest = -1e30f;
 
 // ---- few rows: tokens streamed through registers ---------------------------------------------
 // Block (split, session * kv head * row tile): NR rows (8 or 16) of one kv
@@ -521,24 +550,22 @@ __global__ void __launch_bounds__(256) tree_attn_merge_kernel(const __grid_const
 // Block: a share of the call's (session, kv head, 128-row tile, token tile)
 // units, in that order, so that sessions of any lengths load the SMs evenly;
 // a (row tile)'s token tiles that fall to several blocks meet in the merge.
-//   warps 0-3   softmax: thread r owns row r (TMEM lane r)
-//   warp 4      issues the MMAs
-//   warps 5-12  read codes and convert them to f16 tiles in shared memory
+//   warps 0-7   softmax: thread (half, r) owns half of row r's tokens (TMEM
+//               lane r)
+//   warp 8      issues the MMAs
+//   warps 9-15  read codes and convert them to f16 tiles in shared memory
 // S = Q K^T and O += P V with Q and P as the A operand in TMEM, so shared
 // memory carries only what K and V need: 64 KB written and 64 KB read a tile
 // of 16384 elements each, against 1024 cycles of MMA.  A tile is 64 tokens at
 // head_dim 256, else 128: TMEM then holds O [DP], two S [BT] (P overwrites
 // its S) and Q [DP / 2 columns].
 //   K tile: tokens as rows of 128-byte swizzled lines, 64 dimensions a chunk
-//           (K-major).  Its codes take their exponent relative to the tile's
-//           largest on the way (exact until 2^-24 of it), which leaves one
-//           factor a tile for the scores.  Not so in a tile that some row does
-//           not see whole: what lies in rows that it does not see, which may
-//           be anything, would set that factor; the scores there take each
-//           token's own.
-//   V tile: the same bytes read as the transposed operand (N-major), its
-//           exponents in the weights (see kHead).
-constexpr int kTileWarps = 13, kTileThreads = kTileWarps * 32, kConvThreads = 256, kTileRows = 128;
+//           (K-major).
+//   V tile: the same bytes read as the transposed operand (N-major).
+// The tokens' factors stay out of the tiles: the key's multiplies the score,
+// the value's the weight, both in f32 (see kHead).
+constexpr int kSoftThreads = 256, kMmaWarp = 8, kConvThreads = 224, kTileRows = 128;
+constexpr int kTileThreads = kSoftThreads + 32 + kConvThreads;
 constexpr int kErrTileWait = 503;
 
 template <int DP>
@@ -546,8 +573,10 @@ struct TileShape {
   static constexpr int BT = DP == 256 ? 64 : 128, ST = 3, META = 8;
   static constexpr uint32_t kBytes = BT * DP * 2;
   static constexpr uint32_t kTmemO = 0, kTmemS = DP, kTmemQ = DP + 2 * BT;
-  static constexpr int kPieces = BT * DP / 16 / kConvThreads;  // 16-byte pieces of codes a thread and tile
-  static constexpr size_t smem = 1024 + 2 * ST * (size_t)kBytes + META * BT * 12;
+  static constexpr int kPieces = (BT * DP / 16 + kConvThreads - 1) / kConvThreads;  // 16-byte pieces of codes a thread and tile
+  static constexpr int kQPitch = 40;  // f16 elements of a staged query row's 32 columns: rows on distinct banks
+  static constexpr size_t smem = 1024 + 2 * ST * (size_t)kBytes + META * BT * 8 + kSoftThreads * kQPitch * 2;
+
 };
 
 // Token tiles of session b (0: none of its nodes is there).
@@ -568,24 +597,22 @@ __device__ __forceinline__ long long units_before(const TreeArgs &a, int b, int 
 
 struct Segment {
   int b, kvh, rt, j0, j1, pos, total;
-  bool whole;
 };
 
 // A block's units, one segment (token tiles [j0, j1) of one row tile) at a time.
 struct Walk {
   int b, tiles, row_tiles;
-  long long rem, left;
+  int rem, left;
   __device__ __forceinline__ bool next(const TreeArgs &a, int BT, Segment &s) {
     if (left <= 0) return false;
     const int items = a.kv_heads * row_tiles;
-    while (rem >= (long long)items * tiles) {
-      rem -= (long long)items * tiles;
+    while (rem >= items * tiles) {
+      rem -= items * tiles;
       tiles = session_tiles(a, ++b, BT);
     }
-    const int item = (int)(rem / tiles);
-    s.j0 = (int)(rem % tiles);
-    const int n = (int)min(left, (long long)(tiles - s.j0));
-    s.whole = n == tiles;
+    const int item = rem / tiles;
+    s.j0 = rem % tiles;
+    const int n = min(left, tiles - s.j0);
     left -= n;
     rem += n;
     s.b = b;
@@ -604,6 +631,15 @@ __device__ __forceinline__ void give_up(int *error, volatile int *abort) {
   if (error) atomicCAS(error, 0, kErrTileWait);
 }
 
+// Codes pass by once: they leave L1 to what is used again.
+__device__ __forceinline__ uint4 load_once(const uint8_t *p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -617,55 +653,91 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 
-// One row of S [BT] from TMEM: y = s * f + the value's exponent; returns the
-// largest y.  WEIGH: also the weights 2^(y + base) as f16 pairs in p and their
-// sum without the exponents in l.  OPEN: a tile that not every row sees whole.
-template <int BT, bool OPEN, bool WEIGH>
-__device__ __forceinline__ float softmax_pass(uint32_t s_tmem, const float4 *meta, const float *kf, float f, float base,
-                                              const Sight &sight, int t0, int pos, int total, bool tree,
-                                              uint32_t (&p)[BT / 2], uint64_t &l) {
+// Half a row of S (NT tokens from TMEM column s_tmem, factors fac: two keys',
+// two values' of each pair): weights e = 2^(s * kf * f + base), their sums in l,
+// e * vf as f16 pairs in p; returns the largest e * vf.  OPEN: a tile that not
+// every row sees whole, only its tokens `seen`.
+template <int NT, bool OPEN>
+__device__ __forceinline__ float weigh_pass(uint32_t s_tmem, const float4 *fac, float f, float base, uint64_t seen,
+                                            uint32_t (&p)[NT / 2], uint64_t &l) {
   const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
-  float mx = -INFINITY;
+  float mx[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int c = 0; c < BT / 32; ++c) {
-    uint32_t r[32];
-    tmem_ld32(s_tmem + c * 32, r);
+  for (int c = 0; c < NT / 16; ++c) {
+    uint32_t r[16];
+    tmem_ld16(s_tmem + c * 16, r);
     tmem_ld_wait(r);
 #pragma unroll
-    for (int e = 0; e < 32; e += 2) {
-      const float4 mt = meta[(c * 32 + e) / 2];  // exponents, then their inverse powers
-      float s0 = __uint_as_float(r[e]), s1 = __uint_as_float(r[e + 1]);
+    for (int e = 0; e < 16; e += 2) {
+      const float4 ft = fac[(c * 16 + e) / 2];
+      const uint64_t x = mul2(pack2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), pack2(ft.x, ft.y));
+      float e0, e1, w0, w1;
+      unpack2(fma2(x, f2, b2), e0, e1);
+      e0 = exp2_approx(e0);
+      e1 = exp2_approx(e1);
       if (OPEN) {
-        s0 *= kf[c * 32 + e];
-        s1 *= kf[c * 32 + e + 1];
+        if (!(seen >> (c * 16 + e) & 1)) e0 = 0.0f;
+        if (!(seen >> (c * 16 + e + 1) & 1)) e1 = 0.0f;
       }
-      uint64_t y = fma2(pack2(s0, s1), f2, pack2(mt.x, mt.y));
-      float y0, y1;
-      unpack2(y, y0, y1);
-      if (OPEN) {
-        const int t = t0 + c * 32 + e;
-        if (t >= total || !sight.sees(t, pos, tree)) y0 = -INFINITY;
-        if (t + 1 >= total || !sight.sees(t + 1, pos, tree)) y1 = -INFINITY;
-        y = pack2(y0, y1);
-      }
-      mx = fmaxf(mx, fmaxf(y0, y1));
-      if (WEIGH) {
-        float p0, p1;
-        unpack2(add2(y, b2), p0, p1);
-        p0 = exp2_approx(p0);
-        p1 = exp2_approx(p1);
-        l = fma2(pack2(p0, p1), pack2(mt.z, mt.w), l);
-        p[(c * 32 + e) / 2] = pack_f16x2(p0, p1);
-      }
+      const uint64_t e2 = pack2(e0, e1);
+      l = add2(l, e2);
+      unpack2(mul2(e2, pack2(ft.z, ft.w)), w0, w1);
+      mx[(e >> 1) & 1] = fmaxf(mx[(e >> 1) & 1], fmaxf(w0, w1));
+      p[(c * 16 + e) / 2] = pack_f16x2(w0, w1);
+    }
+  }
+  return fmaxf(mx[0], mx[1]);
+}
+
+// The largest y = s * kf * f + log2(vf) of the same tokens.
+template <int NT>
+__device__ __forceinline__ float max_pass(uint32_t s_tmem, const float4 *fac, float f, uint64_t seen) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < NT / 16; ++c) {
+    uint32_t r[16];
+    tmem_ld16(s_tmem + c * 16, r);
+    tmem_ld_wait(r);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float4 ft = fac[(c * 16 + e) / 2];
+      const float v = (float)((int)(__float_as_uint(e & 1 ? ft.w : ft.z) >> 23) - 127);
+      const float y = fmaf(__uint_as_float(r[e]) * (e & 1 ? ft.y : ft.x), f, v);
+      if (seen >> (c * 16 + e) & 1) mx = fmaxf(mx, y);
     }
   }
   return mx;
+}
+
+// The converting threads meet.
+__device__ __forceinline__ void conv_sync() { asm volatile("bar.sync 1, 224;" ::: "memory"); }
+// All of the softmax threads: meet / meet and learn whether any says yes.
+__device__ __forceinline__ void soft_sync() {
+  tc_fence_before();
+  asm volatile("bar.sync 2, 256;" ::: "memory");
+  tc_fence_after();
+}
+__device__ __forceinline__ bool soft_any(bool v) {
+  int r;
+  tc_fence_before();
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.or.pred q, 2, 256, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((int)v)
+      : "memory");
+  tc_fence_after();
+  return r != 0;
 }
 
 template <int DP>
@@ -675,15 +747,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_attn_tile_kernel(const _
   constexpr int BT = Sh::BT, ST = Sh::ST, META = Sh::META;
   extern __shared__ uint8_t raw_sm[];
   __shared__ uint64_t kfull[ST], kempty[ST], vfull[ST], vempty[ST], sfull[2], pready[2], metafull[META], qready, drain;
-  __shared__ int kref_s[META];
+  __shared__ float mx_s[2][kTileRows];
   __shared__ uint32_t tmem_s;
-  __shared__ int abort_word, never_s, b_s, tiles_s;
-  __shared__ long long rem_s, left_s;
+  __shared__ int abort_word, never_s;
+  __shared__ Walk walk_s, soft_walk_s;
+  __shared__ Segment seg_s;
+  __shared__ bool more_s;
+  __shared__ uint64_t sight_s[kTileRows];
   volatile int *abort_s = &abort_word;
   uint8_t *sK = reinterpret_cast<uint8_t *>(((uintptr_t)raw_sm + 1023) & ~(uintptr_t)1023);
   uint8_t *sV = sK + ST * Sh::kBytes;
-  float4 *meta_s = reinterpret_cast<float4 *>(sV + ST * Sh::kBytes);  // [META][BT / 2]
-  float *kf_s = reinterpret_cast<float *>(meta_s + META * (BT / 2));   // [META][BT], open tiles only
+  float4 *fac_s = reinterpret_cast<float4 *>(sV + ST * Sh::kBytes);  // [META][BT / 2]
+  __half *q_s = reinterpret_cast<__half *>(fac_s + META * (BT / 2));  // [8 warps][32][kQPitch]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rows = a.nodes * a.group, row_tiles = (rows + kTileRows - 1) / kTileRows, D = a.head_dim;
   const bool tree = a.parents != nullptr;
@@ -717,13 +792,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_attn_tile_kernel(const _
         before += __shfl_sync(0xffffffffu, sum, 31);
       }
     if (lane == 0) {
-      b_s = b;
-      tiles_s = u1 > u0 ? session_tiles(a, b, BT) : 1;
-      rem_s = u0 - before;
-      left_s = u1 - u0;
+      walk_s = soft_walk_s = Walk{b, u1 > u0 ? session_tiles(a, b, BT) : 1, row_tiles, (int)(u0 - before),
+                                  (int)(u1 - u0)};
     }
   }
-  if (warp == 4) {
+  if (warp == kMmaWarp) {
     if (lane == 0) {
       for (int i = 0; i < ST; ++i) {
         mbar_init(&kfull[i], kConvThreads / 32);
@@ -733,10 +806,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_attn_tile_kernel(const _
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&sfull[i], 1);
-        mbar_init(&pready[i], 4);
+        mbar_init(&pready[i], 8);
       }
       for (int i = 0; i < META; ++i) mbar_init(&metafull[i], 1);
-      mbar_init(&qready, 4);
+      mbar_init(&qready, 8);
       mbar_init(&drain, 1);
       abort_word = never_s = 0;
       fence_barrier_init();
@@ -748,187 +821,212 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_attn_tile_kernel(const _
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_s;
-  Walk walk{b_s, tiles_s, row_tiles, rem_s, left_s};
-  Segment sg;
 
-  if (warp < 4) {
+  if (warp < 8) {
     // ---- softmax ----
-    const uint32_t my = tmem + ((uint32_t)(warp * 32) << 16);
+    constexpr int NT = BT / 2;
+    const int quad = warp & 3, half = warp >> 2, r_own = quad * 32 + lane;
+    const uint32_t my = tmem_s + ((uint32_t)(quad * 32) << 16);
+    __half *stage = q_s + (size_t)warp * 32 * Sh::kQPitch;
     uint32_t g = 0;  // tiles so far
+    // After a wait that ran out this role goes on to its end without waiting
+    // (the results are void): its warps meet at barriers.
     bool ok = true;
-    for (int seg = 0; ok && walk.next(a, BT, sg); ++seg) {
-      const int row = sg.rt * kTileRows + tid, n = row / a.group, h = sg.kvh * a.group + row % a.group;
-      const bool in = row < rows;
-      const Sight sight = sight_of(a, sg.b, in ? n : a.nodes, sg.pos);
-      const size_t node = (size_t)sg.b * a.nodes + n;
-      float m = -INFINITY, fac;
-      uint64_t l2 = 0;
-      {  // the row's query, scaled into f16, to TMEM
-        const size_t at = node * a.q_pitch + (size_t)h * a.q_head;
-        auto piece = [&](int d, float(&x)[8]) {
-          if (!in || d >= D) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-          } else if (!a.q_vec) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = load_q(a, at + d + i);
-          } else if (a.q_bf16) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) + at + d);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              x[2 * i] = __uint_as_float(w[i] << 16);
-              x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            }
-          } else {
-            const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at + d);
-            const float4 u = p[0], v = p[1];
-            x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-            x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
-          }
-        };
-        float amax = 0.0f;
-        for (int d = 0; d < D; d += 8) {
-          float x[8];
-          piece(d, x);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
-        }
-        const int e = q_exponent(amax);
-        const float inv = pow2i(-e);
-        fac = pow2i(e) * a.scale_log2;
-        for (int d = 0; d < D; d += 64) {
-          uint32_t w[32];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float x[8];
-            piece(d + 8 * j, x);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[4 * j + i] = pack_f16x2(x[2 * i] * inv, x[2 * i + 1] * inv);
-          }
-          tmem_st32(my + Sh::kTmemQ + d / 2, w);
-        }
-        tmem_st_wait();
+    // The walk and what a segment needs once lie in shared memory: the loop
+    // over its tiles wants the registers.
+    for (int seg = 0;; ++seg) {
+      if (tid == 0) {
+        Walk w = soft_walk_s;
+        Segment next;
+        more_s = w.next(a, BT, next);
+        soft_walk_s = w;
+        seg_s = next;
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&qready);
-      for (int j = sg.j0; j < sg.j1; ++j, ++g) {
-        const int t0 = j * BT;
-        const bool open = t0 + BT > sg.pos;
-        ok = mbar_wait(&sfull[g & 1], (g >> 1) & 1, abort_s) && mbar_wait(&metafull[g % META], (g / META) & 1, abort_s);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) {
-          give_up(a.error, abort_s);
-          break;
-        }
-        tc_fence_after();
-        const uint32_t s_tmem = my + Sh::kTmemS + (g & 1) * BT;
-        const float4 *meta = meta_s + (size_t)(g % META) * (BT / 2);
-        const float *kf = kf_s + (size_t)(g % META) * BT;
-        const float f = fac * pow2i(kref_s[g % META]);
-        uint32_t p[BT / 2];
-        const uint64_t l_old = l2;
-        bool grow = true;
-        float mx;
-        if (j > sg.j0) {  // with the maximum so far; again where it has grown too much
-          const float base = m == -INFINITY ? 0.0f : kHead - m;
-          mx = open ? softmax_pass<BT, true, true>(s_tmem, meta, kf, f, base, sight, t0, sg.pos, sg.total, tree, p, l2)
-                    : softmax_pass<BT, false, true>(s_tmem, meta, kf, f, base, sight, t0, sg.pos, sg.total, tree, p, l2);
-          grow = mx > m + kLag || (m == -INFINITY && mx > m);
-          grow = __any_sync(0xffffffffu, grow);
-        } else {
-          mx = open ? softmax_pass<BT, true, false>(s_tmem, meta, kf, f, 0.0f, sight, t0, sg.pos, sg.total, tree, p, l2)
-                    : softmax_pass<BT, false, false>(s_tmem, meta, kf, f, 0.0f, sight, t0, sg.pos, sg.total, tree, p, l2);
-        }
-        if (grow) {
-          const float mn = fmaxf(m, mx);
-          const float old = m == -INFINITY ? 0.0f : exp2_approx(m - mn);
-          m = mn;
-          l2 = fma2(l_old, pack2(old, old), 0);
-          if (j > sg.j0) {  // O of the tiles before takes the new maximum, once they are in it
-            const uint32_t q = g - 1;
-            ok = __all_sync(0xffffffffu, mbar_wait(&vempty[q % ST], (q / ST) & 1, abort_s));
-            if (!ok) {
-              give_up(a.error, abort_s);
-              break;
-            }
-            tc_fence_after();
-            for (int d = 0; d < D; d += 32) {
-              uint32_t r[32];
-              tmem_ld32(my + Sh::kTmemO + d, r);
-              tmem_ld_wait(r);
+      soft_sync();
+      if (!more_s) break;
+      const int j0 = seg_s.j0, j1 = seg_s.j1, pos = seg_s.pos;
+      {
+        const int row = seg_s.rt * kTileRows + r_own;
+        const Sight sight = sight_of(a, seg_s.b, row < rows ? row / a.group : a.nodes, pos);
+        if (half == 0) sight_s[r_own] = tree ? sight.bits : (uint64_t)max(sight.upto, 0);
+      }
+      float m = kLowest;
+      uint64_t l2 = 0;
+      // Queries: 32 columns of the warp's 32 rows at a time, four rows a load
+      // (8 lanes, four columns each), the halves taking the columns' chunks in
+      // turn; as f16 through shared memory to the rows' TMEM lanes.  They are
+      // taken as they are where every row's largest magnitude lies well
+      // inside f16's range, else again with each row's power of two.
+      const int r_sub = lane >> 3, c_sub = 4 * (lane & 7);
+      long long at[8];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * old);
-              tmem_st32(my + Sh::kTmemO + d, r);
+      for (int i = 0; i < 8; ++i) {
+        const int r = seg_s.rt * kTileRows + quad * 32 + 4 * i + r_sub, n = r / a.group;
+        at[i] = r < rows ? ((long long)seg_s.b * a.nodes + n) * a.q_pitch +
+                               (long long)(seg_s.kvh * a.group + (r - n * a.group)) * a.q_head + c_sub
+                         : -1;
+      }
+      int qe = 0;
+      for (int round = 0; round < 2; ++round) {
+        float am[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) am[i] = 0.0f;
+        for (int d = 32 * half; d < D; d += 64) {
+          float4 x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (at[i] < 0 || d + c_sub >= D) continue;
+            const size_t o = (size_t)at[i] + d;
+            if (!a.q_vec) {
+              x[i] = make_float4(load_q(a, o), load_q(a, o + 1), load_q(a, o + 2), load_q(a, o + 3));
+            } else if (a.q_bf16) {
+              const uint2 v = *reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(a.q) + o);
+              x[i] = make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u),
+                                 __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+            } else {
+              x[i] = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + o);
             }
           }
-          const float base = m == -INFINITY ? 0.0f : kHead - m;
-          if (open)
-            softmax_pass<BT, true, true>(s_tmem, meta, kf, f, base, sight, t0, sg.pos, sg.total, tree, p, l2);
-          else
-            softmax_pass<BT, false, true>(s_tmem, meta, kf, f, base, sight, t0, sg.pos, sg.total, tree, p, l2);
-        }
 #pragma unroll
-        for (int i = 0; i < BT / 64; ++i) tmem_st32(s_tmem + 32 * i, p + 32 * i);
+          for (int i = 0; i < 8; ++i) {
+            am[i] = fmaxf(am[i], fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+            const float f = pow2i(-__shfl_sync(0xffffffffu, qe, 4 * i + r_sub));
+            *reinterpret_cast<uint2 *>(stage + (4 * i + r_sub) * Sh::kQPitch + c_sub) =
+                make_uint2(pack_f16x2(x[i].x * f, x[i].y * f), pack_f16x2(x[i].z * f, x[i].w * f));
+          }
+          __syncwarp();
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(stage + lane * Sh::kQPitch + 8 * i);
+            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+          }
+          tmem_st16(my + Sh::kTmemQ + d / 2, w);
+          __syncwarp();
+        }
+        if (round) break;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+          for (int o = 4; o > 0; o >>= 1) am[i] = fmaxf(am[i], __shfl_xor_sync(0xffffffffu, am[i], o));
+          if ((lane & 7) == 0) mx_s[half][quad * 32 + 4 * i + r_sub] = am[i];
+        }
+        soft_sync();
+        const float big = fmaxf(mx_s[0][r_own], mx_s[1][r_own]);
+        if (!soft_any(big != 0.0f && !(big >= 0x1p-3f && big < 0x1p15f))) break;
+        qe = q_exponent(big);
+      }
+      const float f = pow2i(qe) * a.scale_log2;
+      tmem_st_wait();
+      soft_sync();
+      if (lane == 0) mbar_arrive(&qready);
+      for (int j = j0; j < j1; ++j, ++g) {
+        const int t0 = j * BT;
+        const bool open = t0 + BT > pos;
+        if (ok)
+          ok = mbar_wait(&sfull[g & 1], (g >> 1) & 1, abort_s) &&
+               mbar_wait(&metafull[g % META], (g / META) & 1, abort_s);
+        if (!ok) give_up(a.error, abort_s);
+        __syncwarp();
+        tc_fence_after();
+        const uint32_t s_tmem = my + Sh::kTmemS + (g & 1) * BT + half * NT;
+        const float4 *fac = fac_s + ((size_t)(g % META) * BT + half * NT) / 2;
+        uint64_t seen = ~0ull;
+        if (open) {
+          const uint64_t b = sight_s[r_own];
+          seen = Sight{(int)b, b}.seen64(t0 + half * NT, pos, tree);
+        }
+        uint32_t p[NT / 2];
+        // With the maximum so far; where a weight has outgrown it (and for a
+        // segment's first tile) the maximum is raised and the weights taken
+        // again, once.
+        uint64_t l_new;
+        for (bool raise = j == j0;;) {
+          if (raise) {
+            mx_s[half][r_own] = max_pass<NT>(s_tmem, fac, f, seen);
+            soft_sync();
+            // (a row that has seen nothing yet keeps a floor that no score is under)
+            const float mn = fmaxf(m, fmaxf(mx_s[0][r_own], mx_s[1][r_own]));
+            const float old = exp2_approx(m - mn);
+            m = mn;
+            l2 = mul2(l2, pack2(old, old));
+            if (j > j0) {  // O of the tiles before takes the new maximum, once they are in it
+              const uint32_t q = g - 1;
+              if (ok) ok = mbar_wait(&vempty[q % ST], (q / ST) & 1, abort_s);
+              if (!ok) give_up(a.error, abort_s);
+              __syncwarp();
+              tc_fence_after();
+#pragma unroll 1
+              for (int d = 16 * half; d < D; d += 32) {
+                uint32_t r[16];
+                tmem_ld16(my + Sh::kTmemO + d, r);
+                tmem_ld_wait(r);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * old);
+                tmem_st16(my + Sh::kTmemO + d, r);
+              }
+            }
+          }
+          l_new = l2;
+          const float mx = open ? weigh_pass<NT, true>(s_tmem, fac, f, kHead - m, seen, p, l_new)
+                                : weigh_pass<NT, false>(s_tmem, fac, f, kHead - m, seen, p, l_new);
+          if (raise) {
+            soft_sync();
+            break;
+          }
+          raise = soft_any(mx > kMost);
+          if (!raise) break;
+        }
+        l2 = l_new;
+        // P goes over the S that both halves have read, by the barriers above
+        const uint32_t p_tmem = my + Sh::kTmemS + (g & 1) * BT + half * (NT / 2);
+        if constexpr (NT == 64)
+          tmem_st32(p_tmem, p);
+        else
+          tmem_st16(p_tmem, p);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&pready[g & 1]);
       }
-      if (!ok) break;
       float l0, l1;
       unpack2(l2, l0, l1);
-      const float l = l0 + l1;
-      if (sg.j1 > sg.j0) {
+      const size_t slot = (size_t)blockIdx.x * 2 + (seg ? 1 : 0);
+      mx_s[half][r_own] = l0 + l1;
+      soft_sync();
+      if (half == 0)
+        a.part_ml[slot * kTileRows + r_own] =
+            make_float2(j1 > j0 ? fmaxf(m, kLowest) : -INFINITY, mx_s[0][r_own] + mx_s[1][r_own]);
+      if (j1 > j0) {
         const uint32_t q = g - 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(&vempty[q % ST], (q / ST) & 1, abort_s));
-        if (!ok) {
-          give_up(a.error, abort_s);
-          break;
-        }
+        if (ok) ok = mbar_wait(&vempty[q % ST], (q / ST) & 1, abort_s);
+        if (!ok) give_up(a.error, abort_s);
+        __syncwarp();
         tc_fence_after();
-      }
-      const size_t slot = ((size_t)blockIdx.x * 2 + (seg ? 1 : 0)) * kTileRows + tid;
-      if (!sg.whole) a.part_ml[slot] = make_float2(sg.j1 > sg.j0 ? m : -INFINITY, l);
-      const bool there = sight.upto >= 0;
-      const float inv = there ? 1.0f / l : 0.0f;
-      for (int d = 0; d < D && sg.j1 > sg.j0; d += 32) {
-        uint32_t r[32];
-        tmem_ld32(my + Sh::kTmemO + d, r);
-        tmem_ld_wait(r);
-        if (!sg.whole) {
-          float4 *o = reinterpret_cast<float4 *>(a.part + slot * D + d);
+        // four columns of 128 rows lie together: a warp stores 512 bytes
+        float4 *o = reinterpret_cast<float4 *>(a.part) + slot * (kTileRows * (size_t)D / 4) + r_own;
+        for (int d = 32 * half; d < D; d += 64) {
+          uint32_t r[32];
+          tmem_ld32(my + Sh::kTmemO + d, r);
+          tmem_ld_wait(r);
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             if (d + 4 * i < D)
-              o[i] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]),
-                                 __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
-        } else if (in) {
-          float x[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = there ? __uint_as_float(r[i]) * inv : 0.0f;
-          if (a.gate && there) {
-            const float *gt = a.gate + node * a.gate_pitch + (size_t)h * a.gate_head + d;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (d + i < D) x[i] /= 1.0f + expf(-gt[i]);
-          }
-          uint4 *o = reinterpret_cast<uint4 *>(a.out + (node * a.q_heads + h) * D + d);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (d + 8 * i < D)
-              o[i] = make_uint4(pack_bf16x2(x[8 * i], x[8 * i + 1]), pack_bf16x2(x[8 * i + 2], x[8 * i + 3]),
-                                pack_bf16x2(x[8 * i + 4], x[8 * i + 5]), pack_bf16x2(x[8 * i + 6], x[8 * i + 7]));
+              o[(size_t)(d / 4 + i) * kTileRows] =
+                  make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]),
+                              __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
         }
       }
-      tc_fence_before();  // O is read: the next segment's products may overwrite it
+      soft_sync();  // O and mx_s are read: the next segment may overwrite them
     }
-  } else if (warp == 4) {
+  } else if (warp == kMmaWarp) {
     // ---- MMA issue ----
     if (lane == 0) {
       const uint32_t idesc_s = idesc_f16(128, BT, false), idesc_o = idesc_f16(128, D, true);
+      const uint32_t tmem = tmem_s;
+      Walk walk = walk_s;
+      Segment sg;
       uint32_t g = 0;
       bool ok = true;
       auto scores = [&](uint32_t i) {
@@ -973,89 +1071,71 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_attn_tile_kernel(const _
     __syncwarp();
   } else {
     // ---- codes to f16 tiles ----
-    const int ct = tid - 5 * 32, cw = ct >> 5;
+    const int ct = tid - kSoftThreads - 32, cw = ct >> 5;
     constexpr int P = Sh::kPieces, X = BT / 32;
     const int per = D / 16;  // pieces a token
+    const uint32_t pitch = (uint32_t)(a.kv_heads * D);
     int tok[P];
     uint32_t src[P], dst[P];
-    bool flip = false;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       const int idx = i * kConvThreads + ct;
       tok[i] = idx / per;
-      const int ch = idx % per;
-      src[i] = (uint32_t)ch * 16;
+      const int ch = idx - tok[i] * per;
       // the lanes of odd chunks write their second half first, so that eight
-      // lanes' 16-byte stores fall on all banks
+      // lanes' 16-byte stores fall on all banks (bit 31 of src)
       const int first = (ch >> 2) & 1;
-      flip = first;
+      src[i] = (uint32_t)tok[i] * pitch + (uint32_t)ch * 16;
       dst[i] = (uint32_t)((ch >> 2) * (BT * 128) + tok[i] * 128 + (((2 * (ch & 3) + first) ^ (tok[i] & 7)) * 16));
+      if (first) dst[i] |= 1u << 31;
       if (tok[i] >= BT) tok[i] = 1 << 30;
-      if (flip) src[i] |= 1u << 31;
     }
-    Walk ahead = walk;
+    Walk ahead = walk_s;
     Segment na;
-    int jn = 0;
     bool more = ahead.next(a, BT, na);
     while (more && na.j1 <= na.j0) more = ahead.next(a, BT, na);
-    jn = more ? na.j0 : 0;
+    int jn = more ? na.j0 : 0;
     uint4 kb[P], vb[P];
-    uint32_t xk[P], xa[X], xv[X];
-    auto load_k = [&]() {
-      const size_t row = (size_t)na.b * a.max_seq + jn * BT;
-      const uint8_t *e = a.k_exp + row * a.kv_heads + na.kvh;
-      const uint8_t *c = a.k_codes + (row * a.kv_heads + na.kvh) * D;
-      const int live = na.total - jn * BT;
+    uint32_t xk[X], xv[X];
+    auto load = [&](const uint8_t *codes, uint4(&r)[P]) {
+      const uint8_t *c = codes + (((size_t)na.b * a.max_seq + (size_t)jn * BT) * a.kv_heads + na.kvh) * D;
+      const int live = min(BT, na.total - jn * BT);
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const bool in = tok[i] < live && tok[i] < BT;
-        kb[i] = in ? __ldg(reinterpret_cast<const uint4 *>(c + (size_t)tok[i] * a.kv_heads * D + (src[i] & 0x7fffffffu)))
-                   : make_uint4(0, 0, 0, 0);
-        xk[i] = in ? e[(size_t)tok[i] * a.kv_heads] : 0;
-      }
+      for (int i = 0; i < P; ++i)
+        r[i] = tok[i] < live ? load_once(c + src[i]) : make_uint4(0, 0, 0, 0);
+    };
+    auto load_exps = [&]() {
+      const size_t row = ((size_t)na.b * a.max_seq + (size_t)jn * BT) * a.kv_heads + na.kvh;
+      const int live = na.total - jn * BT;
 #pragma unroll
       for (int i = 0; i < X; ++i) {
         const int t = lane + 32 * i;
-        xa[i] = t < live ? e[(size_t)t * a.kv_heads] : 0;
-      }
-      if (cw == 0) {
-        const uint8_t *ev = a.v_exp + row * a.kv_heads + na.kvh;
-#pragma unroll
-        for (int i = 0; i < X; ++i) {
-          const int t = lane + 32 * i;
-          xv[i] = t < live ? ev[(size_t)t * a.kv_heads] : 127;
-        }
+        xk[i] = t < live ? a.k_exp[row + (size_t)t * a.kv_heads] : 127;
+        xv[i] = t < live ? a.v_exp[row + (size_t)t * a.kv_heads] : 127;
       }
     };
-    auto load_v = [&]() {
-      const size_t row = (size_t)na.b * a.max_seq + jn * BT;
-      const uint8_t *c = a.v_codes + (row * a.kv_heads + na.kvh) * D;
-      const int live = na.total - jn * BT;
+    auto store = [&](uint8_t *stage, const uint4(&v)[P]) {
 #pragma unroll
-      for (int i = 0; i < P; ++i)
-        vb[i] = tok[i] < live && tok[i] < BT
-                    ? __ldg(reinterpret_cast<const uint4 *>(c + (size_t)tok[i] * a.kv_heads * D + (src[i] & 0x7fffffffu)))
-                    : make_uint4(0, 0, 0, 0);
-    };
-    auto store = [&](uint8_t *stage, int i, uint4 v, __half2 f, bool scaled) {
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-      uint32_t o[8];
+      for (int i = 0; i < P; ++i) {
+        if (tok[i] >= BT) continue;
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        uint32_t o[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        o[k] = e4m3x2_to_f16x2((uint16_t)(w[k >> 1] >> (16 * (k & 1))));
-        if (scaled) {
-          const __half2 x = __hmul2(*reinterpret_cast<__half2 *>(&o[k]), f);
-          o[k] = *reinterpret_cast<const uint32_t *>(&x);
+        for (int k = 0; k < 4; ++k) {
+          o[2 * k] = e4m3x2_to_f16x2((uint16_t)w[k]);
+          o[2 * k + 1] = e4m3x2_to_f16x2((uint16_t)(w[k] >> 16));
         }
+        const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+        const bool fl = dst[i] >> 31;
+        uint8_t *to = stage + (dst[i] & 0x7fffffffu);
+        *reinterpret_cast<uint4 *>(to) = fl ? hi : lo;
+        *reinterpret_cast<uint4 *>(stage + ((dst[i] & 0x7fffffffu) ^ 16)) = fl ? lo : hi;
       }
-      const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
-      const bool fl = src[i] >> 31;
-      *reinterpret_cast<uint4 *>(stage + dst[i]) = fl ? hi : lo;
-      *reinterpret_cast<uint4 *>(stage + (dst[i] ^ 16)) = fl ? lo : hi;
     };
     if (more) {
-      load_k();
-      load_v();
+      load(a.k_codes, kb);
+      load(a.v_codes, vb);
+      if (cw == 0) load_exps();
     }
     // After a wait that ran out this role goes on to its end without waiting
     // (the results are void): its warps meet at a barrier in open tiles.
@@ -1063,27 +1143,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_attn_tile_kernel(const _
     for (uint32_t g = 0; more; ++g) {
       const int st = g % ST;
       const bool open = (jn + 1) * BT > na.pos;
-      // what the softmax needs of this tile's tokens
-      int ref = 0;
-#pragma unroll
-      for (int i = 0; i < X; ++i) ref = max(ref, (int)xa[i]);
-      ref = open ? 0 : min(kKv8MaxExp, max(kKv8MinExp, (int)__reduce_max_sync(0xffffffffu, (unsigned)ref) - 127));
-      float *mt = reinterpret_cast<float *>(meta_s + (size_t)(g % META) * (BT / 2));
+      float *ft = reinterpret_cast<float *>(fac_s + (size_t)(g % META) * (BT / 2));
       if (g >= ST && ok) ok = mbar_wait(&kempty[st], ((g / ST) - 1) & 1, abort_s);
-      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) give_up(a.error, abort_s);
+      __syncwarp();
       if (cw == 0) {
 #pragma unroll
         for (int i = 0; i < X; ++i) {
           const int t = lane + 32 * i;
-          const float ve = kv8_value_exponent(xv[i]);
-          mt[(t >> 1) * 4 + (t & 1)] = ve;
-          mt[(t >> 1) * 4 + 2 + (t & 1)] = pow2i(-(int)ve);
-          if (open) kf_s[(g % META) * BT + t] = kv8_factor(xa[i]);
+          ft[(t >> 1) * 4 + (t & 1)] = kv8_factor(xk[i]);
+          ft[(t >> 1) * 4 + 2 + (t & 1)] = pow2i((int)kv8_value_exponent(xv[i]));
         }
-        if (lane == 0) kref_s[g % META] = ref;
       }
       if (open) {  // values that are not a number: zero in the product, and the token's score NaN for those who see it
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        conv_sync();
 #pragma unroll
         for (int i = 0; i < P; ++i) {
           uint32_t w[4] = {vb[i].x, vb[i].y, vb[i].z, vb[i].w}, any = 0;
@@ -1094,108 +1167,118 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_attn_tile_kernel(const _
             any |= bad;
           }
           vb[i] = make_uint4(w[0], w[1], w[2], w[3]);
-          if (any && tok[i] < BT) mt[(tok[i] >> 1) * 4 + (tok[i] & 1)] = __int_as_float(0x7fc00000);
+          if (any && tok[i] < BT) ft[(tok[i] >> 1) * 4 + (tok[i] & 1)] = __int_as_float(0x7fc00000);
         }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        conv_sync();
       }
       __syncwarp();
       if (cw == 0 && lane == 0) mbar_arrive(&metafull[g % META]);
-      uint8_t *stage = sK + st * Sh::kBytes;
-#pragma unroll
-      for (int i = 0; i < P; ++i)
-        if (tok[i] < BT)
-          store(stage, i, kb[i], __float2half2_rn(pow2i(open ? 0 : max(-30, min(0, (int)xk[i] - 127 - ref)))), true);
+      store(sK + st * Sh::kBytes, kb);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&kfull[st]);
       // the next tile's keys are on their way while this one's values are stored
-      const bool last = jn + 1 >= na.j1;
-      if (last) {
+      if (jn + 1 >= na.j1) {
         more = ahead.next(a, BT, na);
         while (more && na.j1 <= na.j0) more = ahead.next(a, BT, na);
         jn = more ? na.j0 : 0;
       } else {
         ++jn;
       }
-      if (more) load_k();
+      if (more) {
+        load(a.k_codes, kb);
+        if (cw == 0) load_exps();
+      }
       if (g >= ST && ok) ok = mbar_wait(&vempty[st], ((g / ST) - 1) & 1, abort_s);
-      ok = __all_sync(0xffffffffu, ok);
-      stage = sV + st * Sh::kBytes;
-#pragma unroll
-      for (int i = 0; i < P; ++i)
-        if (tok[i] < BT) store(stage, i, vb[i], __half2(), false);
+      if (!ok) give_up(a.error, abort_s);
+      __syncwarp();
+      store(sV + st * Sh::kBytes, vb);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&vfull[st]);
-      if (more) load_v();
+      if (more) load(a.v_codes, vb);
     }
-    if (!ok) give_up(a.error, abort_s);
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 4) {
+  if (warp == kMmaWarp) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem_s, 512);
   }
 }
 
-// The blocks that share a row's tokens meet, in order: one warp a (session,
-// node, query head).  Rows of one block are written already; rows of nodes
-// that are not there become zeros.
-__global__ void __launch_bounds__(256) tree_attn_tile_merge_kernel(const __grid_constant__ TreeArgs a, int BT,
-                                                                   int grid, int count) {
+// The blocks that share a row tile's tokens meet, in order, with the gate:
+// block (16 rows of a row tile, 64 columns); thread (row, four columns, one of
+// four shares of the blocks).  Rows of nodes that are not there become zeros.
+constexpr int kMergeThreads = 1024, kMergeShares = 4;
+__global__ void __launch_bounds__(kMergeThreads, 1) tree_attn_tile_merge_kernel(const __grid_constant__ TreeArgs a,
+                                                                             int BT, int grid) {
   pdl_enter();
-  const int lane = threadIdx.x & 31, i = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (i >= count) return;
-  const int h = i % a.q_heads, node = i / a.q_heads, b = node / a.nodes, n = node % a.nodes, D = a.head_dim;
-  const int kvh = h / a.group, row = n * a.group + h % a.group;
-  const int row_tiles = (a.nodes * a.group + kTileRows - 1) / kTileRows, items = a.kv_heads * row_tiles;
-  const int d = lane * 8;
-  uint4 *out = reinterpret_cast<uint4 *>(a.out + ((size_t)node * a.q_heads + h) * D + d);
+  __shared__ float4 acc_s[kMergeShares - 1][256];
+  __shared__ float2 ml_s[kMergeShares - 1][256];
+  const int tid = threadIdx.x, share = tid >> 8, t = tid & 255, D = a.head_dim;
+  const int rows = a.nodes * a.group, row_tiles = (rows + kTileRows - 1) / kTileRows, items = a.kv_heads * row_tiles;
+  const int item = blockIdx.x / (kTileRows / 16), r = blockIdx.x % (kTileRows / 16) * 16 + (t & 15);
+  const int b = item / items, kvh = item % items / row_tiles, row = item % row_tiles * kTileRows + r;
+  const int d = blockIdx.y * 64 + 4 * (t >> 4);
+  const bool live = row < rows && d < D;
+  const int n = row / a.group, h = kvh * a.group + row % a.group;
   const int tiles = session_tiles(a, b, BT);
-  if (tiles == 0 || sight_of(a, b, n, a.positions[b]).upto < 0) {
-    if (d < D) *out = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  const long long before = units_before(a, b, BT, items), units = units_before(a, a.batch, BT, items);
-  const long long blocks = min((long long)grid, units);
-  const long long ua = before + (long long)(kvh * row_tiles + row / kTileRows) * tiles, ub = ua + tiles;
-  const int c0 = (int)(((ua + 1) * blocks - 1) / units), c1 = (int)((ub * blocks - 1) / units);
-  if (c0 == c1) return;
-  // the block that the row tile begins in holds it as its last segment, unless it begins there
-  const int first = units * c0 / blocks < ua ? 1 : 0;
-  auto slot = [&](int c) { return ((size_t)c * 2 + (c == c0 ? first : 0)) * kTileRows + row % kTileRows; };
   float m = -INFINITY, l = 0.0f;
-  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, a.part_ml[slot(c)].x);
-  m = warp_max(m);
-  float acc[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (tiles > 0) {
+    const long long before = units_before(a, b, BT, items), units = units_before(a, a.batch, BT, items);
+    const long long blocks = min((long long)grid, units);
+    const long long ua = before + (long long)(item % items) * tiles, ub = ua + tiles;
+    const int c0 = (int)(((ua + 1) * blocks - 1) / units), c1 = (int)((ub * blocks - 1) / units);
+    // the block that the row tile begins in holds it as a later segment, unless it begins there
+    const int first = units * c0 / blocks < ua ? 1 : 0;
+    const float4 *part = reinterpret_cast<const float4 *>(a.part);
 #pragma unroll 4
-  for (int c = c0; c <= c1; ++c) {
-    const size_t s = slot(c);
-    const float2 v = a.part_ml[s];
-    if (v.x == -INFINITY) continue;
-    const float f = exp2_approx(v.x - m);
-    l = fmaf(v.y, f, l);
-    if (d < D) {
-      const float4 *p = reinterpret_cast<const float4 *>(a.part + s * D + d);
-      const float4 x = p[0], z = p[1];
-      acc[0] = fmaf(x.x, f, acc[0]); acc[1] = fmaf(x.y, f, acc[1]);
-      acc[2] = fmaf(x.z, f, acc[2]); acc[3] = fmaf(x.w, f, acc[3]);
-      acc[4] = fmaf(z.x, f, acc[4]); acc[5] = fmaf(z.y, f, acc[5]);
-      acc[6] = fmaf(z.z, f, acc[6]); acc[7] = fmaf(z.w, f, acc[7]);
+    for (int c = c0 + share; c <= c1; c += kMergeShares) {
+      const size_t slot = (size_t)c * 2 + (c == c0 ? first : 0);
+      const float2 v = a.part_ml[slot * kTileRows + r];
+      if (v.x == -INFINITY || !live) continue;
+      const float4 x = part[slot * (kTileRows * (size_t)D / 4) + (size_t)(d / 4) * kTileRows + r];
+      const float mn = fmaxf(m, v.x), fo = exp2_approx(m - mn), fn = exp2_approx(v.x - mn);
+      l = l * fo + v.y * fn;
+      acc.x = acc.x * fo + x.x * fn;
+      acc.y = acc.y * fo + x.y * fn;
+      acc.z = acc.z * fo + x.z * fn;
+      acc.w = acc.w * fo + x.w * fn;
+      m = mn;
     }
   }
-  if (d >= D) return;
+  if (share > 0) {
+    acc_s[share - 1][t] = acc;
+    ml_s[share - 1][t] = make_float2(m, l);
+  }
+  __syncthreads();
+  if (share > 0) return;
+  const bool there = tiles > 0 && sight_of(a, b, row < rows ? n : a.nodes, a.positions[b]).upto >= 0;
+  if (!live) return;
+  for (int i = 0; i < kMergeShares - 1; ++i) {
+    const float2 v = ml_s[i][t];
+    if (v.x == -INFINITY) continue;
+    const float4 x = acc_s[i][t];
+    const float mn = fmaxf(m, v.x), fo = m == -INFINITY ? 0.0f : exp2_approx(m - mn), fn = exp2_approx(v.x - mn);
+    l = l * fo + v.y * fn;
+    acc.x = acc.x * fo + x.x * fn;
+    acc.y = acc.y * fo + x.y * fn;
+    acc.z = acc.z * fo + x.z * fn;
+    acc.w = acc.w * fo + x.w * fn;
+    m = mn;
+  }
+  const size_t node = (size_t)b * a.nodes + n;
+  float o[4] = {acc.x, acc.y, acc.z, acc.w};
   const float inv = 1.0f / l;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    acc[k] *= inv;
-    if (a.gate) acc[k] /= 1.0f + expf(-a.gate[(size_t)node * a.gate_pitch + (size_t)h * a.gate_head + d + k]);
+  for (int i = 0; i < 4; ++i) {
+    o[i] = there ? o[i] * inv : 0.0f;
+    if (there && a.gate) o[i] /= 1.0f + expf(-a.gate[node * a.gate_pitch + (size_t)h * a.gate_head + d + i]);
   }
-  *out = make_uint4(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]), pack_bf16x2(acc[4], acc[5]),
-                    pack_bf16x2(acc[6], acc[7]));
+  *reinterpret_cast<uint2 *>(a.out + (node * a.q_heads + h) * D + d) =
+      make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
 }
 
 // How a call is cut.  tiles: the tcgen05 kernel, `blocks` of them; else rows a
@@ -1203,7 +1286,7 @@ __global__ void __launch_bounds__(256) tree_attn_tile_merge_kernel(const __grid_
 struct Plan {
   bool tiles;
   int rows_tile, splits, blocks, BT;
-  size_t items;
+  size_t items, units;
 };
 
 Plan plan_for(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, size_t head_dim, size_t max_seq) {
@@ -1214,6 +1297,7 @@ Plan plan_for(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, size_
     p.BT = head_dim > 128 ? 64 : 128;
     p.items = batch * kv_heads * ((rows + kTileRows - 1) / kTileRows);
     const size_t most = p.items * ((max_seq + p.BT - 1) / p.BT);
+    p.units = most;
     p.blocks = (int)std::min<size_t>(sm_count(), most);
     return p;
   }
@@ -1243,8 +1327,9 @@ int run_tiles(const TreeArgs &a, const Plan &p, cudaStream_t s) {
   cudaError_t e = launch_pdl(tree_attn_tile_kernel<DP>, dim3((unsigned)p.blocks), kTileThreads, smem, s, a);
   if (e != cudaSuccess) return cuda_fail(e, "tree_attn_tile_kernel");
   FPB_LAUNCH_CHECK("tree_attn_tile_kernel");
-  const int count = a.batch * a.nodes * a.q_heads;
-  e = launch_pdl(tree_attn_tile_merge_kernel, dim3((unsigned)((count + 7) / 8)), 256, 0, s, a, p.BT, p.blocks, count);
+  e = launch_pdl(tree_attn_tile_merge_kernel,
+                 dim3((unsigned)(p.items * (kTileRows / 16)), (unsigned)((a.head_dim + 63) / 64)), kMergeThreads, 0, s, a,
+                 p.BT, p.blocks);
   if (e != cudaSuccess) return cuda_fail(e, "tree_attn_tile_merge_kernel");
   FPB_LAUNCH_CHECK("tree_attn_tile_merge_kernel");
   return FPB_OK;
@@ -1311,8 +1396,9 @@ extern "C" int fpb_tree_attn(const void *q, int q_dtype, size_t q_pitch, size_t 
   if (workspace_bytes < need)
     return fail(FPB_ERR_WORKSPACE, "fpb_tree_attn: workspace %zu < %zu bytes", workspace_bytes, need);
   const Plan p = plan_for(batch, nodes, q_heads, kv_heads, head_dim, max_seq);
-  if (p.items > 65535 || batch * nodes * q_heads > 0x7fffffff)
-    return fail(FPB_ERR_SHAPE, "fpb_tree_attn: %zu tiles of rows in one call (at most 65535)", p.items);
+  if (p.items > 65535 || p.units > 0x7fffffff)
+    return fail(FPB_ERR_SHAPE, "fpb_tree_attn: %zu tiles of rows in one call (at most 65535, and 2^31 with their tiles "
+                "of tokens)", p.items);
   TreeArgs a{};
   a.q = q;
   a.gate = gate;
