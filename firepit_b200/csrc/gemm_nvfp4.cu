@@ -969,6 +969,22 @@ int encode_rows_u8(CUtensorMap *map, const void *base, uint64_t rows, uint64_t r
   return FPB_OK;
 }
 
+int encode_cache_u8(CUtensorMap *map, const void *base, uint64_t batch, uint64_t max_seq, uint64_t kv_heads,
+                    uint64_t head_dim, uint32_t box_bytes, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(FPB_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[4] = {head_dim, kv_heads, max_seq, batch};
+  cuuint64_t strides[3] = {head_dim, head_dim * kv_heads, head_dim * kv_heads * max_seq};
+  cuuint32_t box[4] = {box_bytes, 1, box_rows, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void *>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FPB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return FPB_OK;
+}
+
 bool encode_store_map(CUtensorMap *map, void *y, bool bf16, uint64_t rows, uint64_t cols, uint64_t ld,
                       uint32_t box_rows, uint32_t box_cols) {
   EncodeTiledFn fn = encode_fn();

@@ -10,6 +10,12 @@ namespace fpb {
 // 128-byte swizzle; out-of-range elements read as zero.  FPB status.
 int encode_rows_u8(CUtensorMap *map, const void *base, uint64_t rows, uint64_t row_bytes, uint32_t box_rows);
 
+// 8-bit cache codes [batch, max_seq, kv_heads, head_dim] read in boxes of
+// box_bytes (64 or 128, swizzled over as many) x 1 head x box_rows tokens;
+// out-of-range elements read as zero.  FPB status.
+int encode_cache_u8(CUtensorMap *map, const void *base, uint64_t batch, uint64_t max_seq, uint64_t kv_heads,
+                    uint64_t head_dim, uint32_t box_bytes, uint32_t box_rows);
+
 // Output map for the GEMM epilogues' tiled stores: y [rows, cols] (bf16 or
 // f32, row pitch ld elements), boxes of box_cols x box_rows (box_cols 0: 128
 // bytes); 128-byte boxes use the 128-byte swizzle, narrower ones none.

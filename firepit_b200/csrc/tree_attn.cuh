@@ -1,0 +1,135 @@
+// What the attention kernels over the 8-bit cache share: the call's arguments,
+// what a row sees, the scaling of queries and weights.
+#pragma once
+#include "kv8.cuh"
+
+namespace fpb {
+
+struct TreeArgs {
+  const void *q;
+  const float *gate;
+  const uint8_t *k_codes, *v_codes, *k_exp, *v_exp;
+  const int32_t *positions, *parents;
+  long long q_pitch, q_head, gate_pitch, gate_head;  // elements
+  int batch, nodes, q_heads, kv_heads, group, head_dim, max_seq, q_bf16, q_vec, splits;
+  float scale_log2;  // scale * log2(e): scores and maxima are held in powers of two
+  __nv_bfloat16 *out;
+  float *part;     // [session, kv head, row tile][split][row][head_dim] numerators
+  float2 *part_ml; // [session, kv head, row tile][split][row] maximum, sum
+  int2 *shares;    // (tiles) [session, kv head, row tile] first slot, last block
+  int *error;
+};
+
+// What a row (node n's query head) sees: rows before `pos`, then the tree
+// rows of `bits` (a tree), or the first `upto` of them (a chain); upto < 0:
+// the node is not there.
+struct Sight {
+  int upto;
+  uint64_t bits;
+  // Which of the 64 rows from t0 on it sees.
+  __device__ __forceinline__ uint64_t seen64(int t0, int pos, bool tree) const {
+    const int k = pos - t0;  // rows of the context among them
+    if (!tree) {
+      const int c = k + max(upto, 0);
+      return c >= 64 ? ~0ull : c <= 0 ? 0ull : (1ull << c) - 1;
+    }
+    if (k >= 64) return ~0ull;
+    if (k > 0) return ((1ull << k) - 1) | bits << k;
+    return k > -64 ? bits >> -k : 0ull;
+  }
+  __device__ __forceinline__ bool sees(int t, int pos, bool tree) const {
+    const int j = t - pos;
+    if (j < 0) return true;
+    return tree ? j < kTreeMaxNodes && (bits >> j & 1) : j < upto;
+  }
+};
+
+// The tree is walked through the warp's registers: all 32 lanes call this, each
+// with its own node (n >= nodes: none).
+__device__ __forceinline__ Sight sight_of(const TreeArgs &a, int b, int n, int pos) {
+  Sight s{-1, 0};
+  const bool in = n < a.nodes;
+  const bool inside = pos >= 0 && pos < a.max_seq - n;
+  if (in && !inside && a.error) atomicCAS(a.error, 0, kErrPosition);
+  if (!a.parents) {
+    if (in && inside) s.upto = n + 1;
+    return s;
+  }
+  const int32_t *par = a.parents + (size_t)b * a.nodes;
+  const int lane = threadIdx.x & 31;
+  const int p0 = lane < a.nodes ? par[lane] : -2, p1 = lane + 32 < a.nodes ? par[lane + 32] : -2;
+  const int root = __shfl_sync(0xffffffffu, p0, 0);  // (by every lane, outside the conditions)
+  bool there = in && inside && root == -1;
+  bool going = there && n > 0;
+  int j = in ? n : 0;
+  while (__any_sync(0xffffffffu, going)) {
+    const int lo = __shfl_sync(0xffffffffu, p0, j & 31), hi = __shfl_sync(0xffffffffu, p1, j & 31);
+    const int p = j < 32 ? lo : hi;
+    if (going) {
+      if (p < 0 || p >= j) {
+        if (p >= j && a.error) atomicCAS(a.error, 0, kErrParent);
+        there = going = false;
+      } else {
+        s.bits |= 1ull << j;
+        j = p;
+        going = j > 0;
+      }
+    }
+  }
+  if (there) {
+    s.upto = n + 1;
+    s.bits |= 1;
+  } else {
+    s.bits = 0;
+  }
+  return s;
+}
+
+// Rows of the cache that this session's nodes can see (0: none).
+__device__ __forceinline__ int seen_rows(const TreeArgs &a, int pos, int last_node) {
+  if (pos < 0 || pos >= a.max_seq) return 0;
+  return min(pos + last_node + 1, a.max_seq);
+}
+
+__device__ __forceinline__ float load_q(const TreeArgs &a, size_t at) {
+  return a.q_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(a.q)[at])
+                  : static_cast<const float *>(a.q)[at];
+}
+
+// Power of two that takes a query row into f16: its largest magnitude to
+// [2^8, 2^9), so that f16's 11 bits hold down to 2^-22 of it (f16 products
+// round at 2^-11; the scores' f32 sums and the factor are exact in it).
+__device__ __forceinline__ int q_exponent(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  if (u < 0x00800000u || u >= 0x7f800000u) return 0;  // zero, subnormal, infinite
+  return max(-118, (int)(u >> 23) - 127 - 8);
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Weights are held as 2^(y - m + kHead), y the score (in powers of two) plus
+// the value vector's own exponent: f16 then holds a weight down to 2^-32 of
+// the row's largest, and the exponent costs no multiplication.  The maximum
+// may lag by kLag before the sums are rescaled (weights up to 2^(kHead + kLag)).
+constexpr float kHead = 7.0f, kLag = 8.0f, kMost = 32768.0f, kLowest = -1e30f;
+
+// The tcgen05 kernel (tree_attn_tile.cu): token tiles of BT rows, `blocks` of
+// them, their partial results and the items' shares of them in the workspace.
+struct TilePlan {
+  int BT, blocks;
+  size_t items, units;  // units: a bound
+};
+TilePlan tile_plan(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, size_t head_dim, size_t max_seq);
+size_t tile_workspace_bytes(const TilePlan &p, size_t head_dim);
+int run_tree_tiles(TreeArgs a, const TilePlan &p, void *workspace, cudaStream_t s);
+
+}  // namespace fpb

@@ -1,0 +1,866 @@
+// Tree attention for many rows a key/value head: 128-row tiles on tcgen05.
+//
+// A block takes a share of the call's (session, kv head, row tile, token tile)
+// units, in that order, so that sessions of any lengths load the SMs evenly.
+// Token tiles of one row tile that fall to several blocks meet in the merge.
+//   warps 0-15   softmax: thread (part, r) owns a quarter of row r's tokens
+//                (TMEM lane r); the four warps of a 32-row quad keep step
+//   warp 16      issues the MMAs
+//   warp 17      brings the codes to shared memory by TMA, two tiles ahead
+//   warps 18-25  convert them to f16 tiles
+// S = Q K^T and O += P V, with Q and P as the A operand in TMEM: shared memory
+// carries only what K and V need.  A tile is 64 tokens at head_dim 256, else
+// 128; TMEM then holds O [DP], two S [BT] (P overwrites its S) and Q [DP / 2
+// columns].
+//   K tile: tokens as rows of 128-byte swizzled lines, 64 dimensions a chunk
+//           (K-major).
+//   V tile: the same bytes read as the transposed operand (N-major).
+// The tokens' factors stay out of the tiles: the key's multiplies the score,
+// the value's the weight, both in f32 (see kHead).
+#include <algorithm>
+#include <mutex>
+#include <vector>
+
+#include "sm100.cuh"
+#include "tma_host.cuh"
+#include "tree_attn.cuh"
+
+namespace fpb {
+namespace {
+
+using namespace sm100;
+
+constexpr int kParts = 4, kSoftWarps = 4 * kParts, kSoftThreads = kSoftWarps * 32, kConvWarps = 8, kTileRows = 128;
+constexpr int kMmaWarp = kSoftWarps, kLoadWarp = kMmaWarp + 1, kConvWarp = kLoadWarp + 1;
+constexpr int kTileThreads = (kConvWarp + kConvWarps) * 32;
+constexpr int kErrTileWait = 503;
+
+template <int DP>
+struct TileShape {
+  static constexpr int BT = DP == 256 ? 64 : 128;
+  static constexpr int ST = 2, RAW = 2, META = 4;  // f16 stages, stages of codes, of factors (at least ST + 2)
+  static constexpr uint32_t kBytes = BT * DP * 2, kRawBytes = BT * DP;
+  static constexpr uint32_t kTmemO = 0, kTmemS = DP, kTmemQ = DP + 2 * BT;
+  static constexpr int kPieces = BT * DP / 16 / (kConvWarps * 32);  // 16-byte pieces of codes a thread and tile
+  static constexpr int kBox = DP == 64 ? 64 : 128, kBoxes = DP / kBox;
+};
+
+struct Segment {
+  int b, kvh, rt, item, j0, j1, pos, total;
+  bool ends;
+};
+
+// A block's units, one segment (token tiles [j0, j1) of one row tile) at a time.
+struct Walk {
+  int b, tiles, row_tiles, rem, left;
+  __device__ __forceinline__ bool next(const TreeArgs &a, int BT, Segment &s);
+};
+
+constexpr int kQPitch = 40;  // f16 elements of a staged query row's 32 columns: rows on distinct banks
+
+// Fixed part of the block's shared memory; the stages follow, 1024-byte aligned.
+struct TileShared {
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], rkfull[2], rvfull[2], rkempty[2], rvempty[2], sfull[2], pready[2],
+      metafull[4], qready, drain;
+  Walk walk, soft_walk;
+  Segment seg;
+  uint32_t tmem;
+  int abort, never, more;
+  float red[kParts][kTileRows];  // maxima, then sums, of the rows' parts
+  uint64_t sight[kTileRows];     // a tree: the bits; a chain: the limit
+  float4 fac[4][64];             // [META][pair of tokens]: two keys' factors, two values'
+  __align__(16) __half q[2 * 4 * 32 * kQPitch];
+};
+
+// Token tiles of session b (0: none of its nodes is there).
+__device__ __forceinline__ int session_tiles(const TreeArgs &a, int b, int BT) {
+  if (a.parents && a.parents[(size_t)b * a.nodes] != -1) return 0;
+  return (seen_rows(a, a.positions[b], a.nodes - 1) + BT - 1) / BT;
+}
+
+__device__ __forceinline__ bool Walk::next(const TreeArgs &a, int BT, Segment &s) {
+  if (left <= 0) return false;
+  const int items = a.kv_heads * row_tiles;
+  while (rem >= items * tiles) {
+    rem -= items * tiles;
+    tiles = session_tiles(a, ++b, BT);
+  }
+  const int item = rem / tiles;
+  s.j0 = rem % tiles;
+  const int n = min(left, tiles - s.j0);
+  s.ends = s.j0 + n == tiles;
+  left -= n;
+  rem += n;
+  s.b = b;
+  s.item = b * items + item;
+  s.kvh = item / row_tiles;
+  s.rt = item % row_tiles;
+  s.pos = a.positions[b];
+  // a chain's row tile ends at its last node's own row
+  s.total = seen_rows(a, s.pos, min(a.nodes - 1, (s.rt * kTileRows + kTileRows - 1) / a.group));
+  s.j1 = min(s.j0 + n, (s.total + BT - 1) / BT);
+  return true;
+}
+
+__device__ __forceinline__ void give_up(int *error, volatile int *abort) {
+  *abort = 1;
+  if (error) atomicCAS(error, 0, kErrTileWait);
+}
+
+// Packed pairs of f32.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Barriers of the roles: a quad's softmax warps (ids 1-4), the converting
+// warps (5), all of the softmax (6).  TMEM accesses are ordered across them.
+__device__ __forceinline__ void quad_sync(int quad) {
+  tc_fence_before();
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + quad), "n"(kParts * 32) : "memory");
+  tc_fence_after();
+}
+__device__ __forceinline__ bool quad_any(int quad, bool v) {
+  int r;
+  tc_fence_before();
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((int)v), "r"(1 + quad), "n"(kParts * 32)
+      : "memory");
+  tc_fence_after();
+  return r != 0;
+}
+__device__ __forceinline__ void conv_sync() { asm volatile("bar.sync 5, %0;" ::"n"(kConvWarps * 32) : "memory"); }
+__device__ __forceinline__ void soft_sync() {
+  tc_fence_before();
+  asm volatile("bar.sync 6, %0;" ::"n"(kSoftThreads) : "memory");
+  tc_fence_after();
+}
+
+// A part of a row of S (NT tokens from TMEM column s_tmem, factors fac: two
+// keys', two values' of each pair): weights e = 2^(s * kf * f + base), their
+// sums in l, e * vf as f16 pairs in p; returns the largest e * vf.  OPEN: a
+// tile that not every row sees whole, only its tokens `seen`.
+template <int NT, bool OPEN>
+__device__ __forceinline__ float weigh_pass(uint32_t s_tmem, const float4 *fac, float f, float base, uint64_t seen,
+                                            uint32_t (&p)[NT / 2], uint64_t &l) {
+  const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
+  float mx[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int c = 0; c < NT / 16; ++c) {
+    uint32_t r[16];
+    tmem_ld16(s_tmem + c * 16, r);
+    tmem_ld_wait(r);
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+      const float4 ft = fac[(c * 16 + e) / 2];
+      const uint64_t x = mul2(pack2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), pack2(ft.x, ft.y));
+      float e0, e1, w0, w1;
+      unpack2(fma2(x, f2, b2), e0, e1);
+      e0 = exp2_approx(e0);
+      e1 = exp2_approx(e1);
+      if (OPEN) {
+        if (!(seen >> (c * 16 + e) & 1)) e0 = 0.0f;
+        if (!(seen >> (c * 16 + e + 1) & 1)) e1 = 0.0f;
+      }
+      const uint64_t e2 = pack2(e0, e1);
+      l = add2(l, e2);
+      unpack2(mul2(e2, pack2(ft.z, ft.w)), w0, w1);
+      mx[(e >> 1) & 1] = fmaxf(mx[(e >> 1) & 1], fmaxf(w0, w1));
+      p[(c * 16 + e) / 2] = pack_f16x2(w0, w1);
+    }
+  }
+  return fmaxf(mx[0], mx[1]);
+}
+
+// What happens seldom stays out of line, so that the loop over tiles keeps its
+// registers.
+template <int NT>
+__device__ __noinline__ float weigh_open(uint32_t s_tmem, const float4 *fac, float f, float base, uint64_t seen,
+                                         uint32_t *p, uint64_t *l) {
+  uint32_t q[NT / 2];
+  uint64_t sum = *l;
+  const float mx = weigh_pass<NT, true>(s_tmem, fac, f, base, seen, q, sum);
+#pragma unroll
+  for (int i = 0; i < NT / 2; ++i) p[i] = q[i];
+  *l = sum;
+  return mx;
+}
+
+// The row's maximum raised by this tile's scores (y = s * kf * f + log2(vf)),
+// and O of the tiles before rescaled to it; returns the new maximum and the
+// factor of what was summed before.
+template <int DP, int NT>
+__device__ __noinline__ float2 raise_max(TileShared *sh, uint32_t s_tmem, uint32_t o_tmem, const float4 *fac, float f,
+                                         uint64_t seen, float m, int D, bool sums) {
+  const int quad = (threadIdx.x >> 5) & 3, part = threadIdx.x >> 7, r_own = threadIdx.x & 127;
+  float mx = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < NT / 16; ++c) {
+    uint32_t r[16];
+    tmem_ld16(s_tmem + c * 16, r);
+    tmem_ld_wait(r);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float4 ft = fac[(c * 16 + e) / 2];
+      const float v = (float)((int)(__float_as_uint(e & 1 ? ft.w : ft.z) >> 23) - 127);
+      const float y = fmaf(__uint_as_float(r[e]) * (e & 1 ? ft.y : ft.x), f, v);
+      if (seen >> (c * 16 + e) & 1) mx = fmaxf(mx, y);
+    }
+  }
+  sh->red[part][r_own] = mx;
+  quad_sync(quad);
+  float mn = m;  // (a row that has seen nothing yet keeps its floor)
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) mn = fmaxf(mn, sh->red[i][r_own]);
+  const float old = exp2_approx(m - mn);
+  if (sums) {
+#pragma unroll 1
+    for (int d = 16 * part; d < D; d += 16 * kParts) {
+      uint32_t r[16];
+      tmem_ld16(o_tmem + d, r);
+      tmem_ld_wait(r);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * old);
+      tmem_st16(o_tmem + d, r);
+    }
+    tmem_st_wait();
+  }
+  quad_sync(quad);  // red is read
+  return make_float2(mn, old);
+}
+
+// A quad's 32 queries to TMEM as f16: 32 columns at a time, four rows a load
+// (8 lanes, four columns each), two warps taking the columns' chunks in turn,
+// through shared memory to the rows' lanes.  They are taken as they are where
+// every row's largest magnitude lies well inside f16's range, else again with
+// each row's power of two.  Returns the row's factor of the scores.
+__device__ __noinline__ float load_queries(const TreeArgs &a, TileShared *sh, uint32_t q_tmem) {
+  const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3, part = threadIdx.x >> 7, r_own = threadIdx.x & 127;
+  const int rows = a.nodes * a.group, D = a.head_dim;
+  __half *stage = sh->q + (size_t)(part * 4 + quad) * 32 * kQPitch;  // parts 0 and 1
+  const int r_sub = lane >> 3, c_sub = 4 * (lane & 7);
+  int qe = 0;
+  for (int round = 0; round < 2; ++round) {
+    if (part < 2) {
+      float am[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) am[i] = 0.0f;
+      for (int d = 32 * part; d < D; d += 64) {
+#pragma unroll
+        for (int i0 = 0; i0 < 8; i0 += 4) {
+          float4 x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = sh->seg.rt * kTileRows + quad * 32 + 4 * (i0 + i) + r_sub;
+            x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (r >= rows || d + c_sub >= D) continue;
+            const int n = r / a.group;
+            const size_t o = ((size_t)sh->seg.b * a.nodes + n) * a.q_pitch +
+                             (size_t)(sh->seg.kvh * a.group + (r - n * a.group)) * a.q_head + d + c_sub;
+            if (!a.q_vec) {
+              x[i] = make_float4(load_q(a, o), load_q(a, o + 1), load_q(a, o + 2), load_q(a, o + 3));
+            } else if (a.q_bf16) {
+              const uint2 v = *reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(a.q) + o);
+              x[i] = make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u),
+                                 __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+            } else {
+              x[i] = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + o);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 4 * (i0 + i) + r_sub;
+            am[i0 + i] = fmaxf(am[i0 + i],
+                               fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+            const float f = pow2i(-__shfl_sync(0xffffffffu, qe, r));
+            *reinterpret_cast<uint2 *>(stage + r * kQPitch + c_sub) =
+                make_uint2(pack_f16x2(x[i].x * f, x[i].y * f), pack_f16x2(x[i].z * f, x[i].w * f));
+          }
+        }
+        __syncwarp();
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 v = *reinterpret_cast<const uint4 *>(stage + lane * kQPitch + 8 * i);
+          w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+        }
+        tmem_st16(q_tmem + d / 2, w);
+        __syncwarp();
+      }
+      tmem_st_wait();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) am[i] = fmaxf(am[i], __shfl_xor_sync(0xffffffffu, am[i], o));
+        if (round == 0 && (lane & 7) == 0) sh->red[part][quad * 32 + 4 * i + r_sub] = am[i];
+      }
+    }
+    quad_sync(quad);
+    if (round) break;
+    const float big = fmaxf(sh->red[0][r_own], sh->red[1][r_own]);
+    if (!quad_any(quad, big != 0.0f && !(big >= 0x1p-3f && big < 0x1p15f))) break;
+    qe = q_exponent(big);
+  }
+  return pow2i(qe) * a.scale_log2;
+}
+
+// This block's share of the units, warp 0.
+__device__ __noinline__ void share_out(const TreeArgs &a, TileShared *sh, int BT, int row_tiles) {
+  const int lane = threadIdx.x & 31, items = a.kv_heads * row_tiles;
+  int all = 0;
+  for (int i = lane; i < a.batch; i += 32) all += session_tiles(a, i, BT);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+  const int units = all * items, blocks = min((int)gridDim.x, units);
+  int u0 = 0, u1 = 0;
+  if ((int)blockIdx.x < blocks) {
+    u0 = (int)((long long)units * blockIdx.x / blocks);
+    u1 = (int)((long long)units * (blockIdx.x + 1) / blocks);
+  }
+  int b = 0, before = 0;  // the session that holds unit u0, and the units before it
+  if (u1 > u0)
+    for (int i0 = 0; i0 < a.batch; i0 += 32) {
+      const int n = i0 + lane < a.batch ? session_tiles(a, i0 + lane, BT) * items : 0;
+      int sum = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, before + sum > u0);
+      const int k = past ? __ffs(past) - 1 : 31;
+      const int held = __shfl_sync(0xffffffffu, past ? sum - n : sum, k);
+      before += held;
+      if (past) {
+        b = i0 + k;
+        break;
+      }
+    }
+  if (lane == 0)
+    sh->walk = sh->soft_walk = Walk{b, u1 > u0 ? session_tiles(a, b, BT) : 1, row_tiles, u0 - before, u1 - u0};
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    tree_attn_tile_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap k_map,
+                          const __grid_constant__ CUtensorMap v_map) {
+  pdl_enter();
+  using Sh = TileShape<DP>;
+  constexpr int BT = Sh::BT, ST = Sh::ST, RAW = Sh::RAW, META = Sh::META;
+  extern __shared__ uint8_t raw_sm[];
+  uint8_t *const base_sm = raw_sm + (-smem_u32(raw_sm) & 1023);
+  TileShared *const sh = reinterpret_cast<TileShared *>(base_sm);
+  uint8_t *const sK = base_sm + (sizeof(TileShared) + 1023) / 1024 * 1024, *const sV = sK + ST * Sh::kBytes;
+  uint8_t *const rK = sV + ST * Sh::kBytes, *const rV = rK + RAW * Sh::kRawBytes;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const bool tree = a.parents != nullptr;
+  if (warp == 0) {
+    share_out(a, sh, BT, (a.nodes * a.group + kTileRows - 1) / kTileRows);
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sh->kfull[i], kConvWarps);
+        mbar_init(&sh->vfull[i], kConvWarps);
+        mbar_init(&sh->kempty[i], 1);
+        mbar_init(&sh->vempty[i], 1);
+        mbar_init(&sh->rkfull[i], 1);
+        mbar_init(&sh->rvfull[i], 1);
+        mbar_init(&sh->rkempty[i], kConvWarps);
+        mbar_init(&sh->rvempty[i], kConvWarps);
+        mbar_init(&sh->sfull[i], 1);
+        mbar_init(&sh->pready[i], kSoftWarps);
+      }
+      for (int i = 0; i < META; ++i) mbar_init(&sh->metafull[i], 1);
+      mbar_init(&sh->qready, kSoftWarps);
+      mbar_init(&sh->drain, 1);
+      sh->abort = sh->never = 0;
+      fence_barrier_init();
+    }
+    __syncwarp();
+    tmem_alloc(&sh->tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  volatile int *const abort_s = &sh->abort;
+
+  if (warp < kSoftWarps) {
+    // ---- softmax ----
+    constexpr int NT = BT / kParts;
+    const int quad = warp & 3, part = warp >> 2, r_own = quad * 32 + lane;
+    const uint32_t my = sh->tmem + ((uint32_t)(quad * 32) << 16);
+    uint32_t g = 0;  // tiles so far
+    // After a wait that ran out this role goes on to its end without waiting
+    // (the results are void): its warps meet at barriers.
+    bool ok = true;
+    // The walk, and what a segment needs once, lie in shared memory: the loop
+    // over its tiles wants the registers.
+    for (int seg = 0;; ++seg) {
+      if (tid == 0) {
+        Walk w = sh->soft_walk;
+        Segment next;
+        sh->more = w.next(a, BT, next);
+        sh->soft_walk = w;
+        sh->seg = next;
+      }
+      soft_sync();
+      if (!sh->more) break;
+      const int j0 = sh->seg.j0, j1 = sh->seg.j1, pos = sh->seg.pos;
+      if (part == 0) {
+        const int row = sh->seg.rt * kTileRows + r_own;
+        const Sight s = sight_of(a, sh->seg.b, row < a.nodes * a.group ? row / a.group : a.nodes, pos);
+        sh->sight[r_own] = tree ? s.bits : (uint64_t)max(s.upto, 0);
+      }
+      const float f = load_queries(a, sh, my + Sh::kTmemQ);
+      if (lane == 0) mbar_arrive(&sh->qready);
+      float m = kLowest;
+      uint64_t l2 = 0;
+      for (int j = j0; j < j1; ++j, ++g) {
+        if (ok)
+          ok = mbar_wait(&sh->sfull[g & 1], (g >> 1) & 1, abort_s) &&
+               mbar_wait(&sh->metafull[g % META], (g / META) & 1, abort_s);
+        if (!ok) give_up(a.error, abort_s);
+        __syncwarp();
+        tc_fence_after();
+        const uint32_t s_tmem = my + Sh::kTmemS + (g & 1) * BT + part * NT;
+        const float4 *fac = sh->fac[g % META] + part * NT / 2;
+        const bool open = (j + 1) * BT > pos;
+        uint64_t seen = ~0ull;
+        if (open) {
+          const uint64_t b = sh->sight[r_own];
+          seen = Sight{(int)b, b}.seen64(j * BT + part * NT, pos, tree);
+        }
+        // With the maximum so far; where a weight has outgrown it (and for a
+        // segment's first tile) the maximum is raised and the weights taken
+        // again, once.
+        uint32_t p[NT / 2];
+        uint64_t l_new;
+        for (bool raise = j == j0;;) {
+          if (raise) {
+            if (j > j0) {
+              if (ok) ok = mbar_wait(&sh->vempty[(g - 1) % ST], ((g - 1) / ST) & 1, abort_s);
+              if (!ok) give_up(a.error, abort_s);
+              __syncwarp();
+              tc_fence_after();
+            }
+            const float2 r = raise_max<DP, NT>(sh, s_tmem, my + Sh::kTmemO, fac, f, seen, m, a.head_dim, j > j0);
+            m = r.x;
+            l2 = mul2(l2, pack2(r.y, r.y));
+          }
+          l_new = l2;
+          float mx;
+          if (open) {
+            uint32_t q[NT / 2];
+            uint64_t l = l2;
+            mx = weigh_open<NT>(s_tmem, fac, f, kHead - m, seen, q, &l);
+#pragma unroll
+            for (int i = 0; i < NT / 2; ++i) p[i] = q[i];
+            l_new = l;
+          } else {
+            mx = weigh_pass<NT, false>(s_tmem, fac, f, kHead - m, seen, p, l_new);
+          }
+          const bool more = quad_any(quad, mx > kMost);
+          if (raise || !more) break;
+          raise = true;
+        }
+        l2 = l_new;
+        // P goes over the S that all of the quad's parts have read, by the barrier above
+        const uint32_t p_tmem = my + Sh::kTmemS + (g & 1) * BT + part * (NT / 2);
+        if constexpr (NT == 32)
+          tmem_st16(p_tmem, p);
+        else
+          tmem_st8(p_tmem, p);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->pready[g & 1]);
+      }
+      float l0, l1;
+      unpack2(l2, l0, l1);
+      const size_t slot = (size_t)blockIdx.x * 2 + (seg ? 1 : 0);
+      sh->red[part][r_own] = l0 + l1;
+      quad_sync(quad);
+      if (part == 0) {
+        float l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) l += sh->red[i][r_own];
+        a.part_ml[slot * kTileRows + r_own] = make_float2(j1 > j0 ? m : -INFINITY, l);
+        // whose slots hold the row tile: from its first block's to its last's
+        if (r_own == 0 && j0 == 0) a.shares[sh->seg.item].x = (int)slot;
+        if (r_own == 0 && sh->seg.ends) a.shares[sh->seg.item].y = (int)blockIdx.x;
+      }
+      if (j1 > j0) {
+        if (ok) ok = mbar_wait(&sh->vempty[(g - 1) % ST], ((g - 1) / ST) & 1, abort_s);
+        if (!ok) give_up(a.error, abort_s);
+        __syncwarp();
+        tc_fence_after();
+        // four columns of 128 rows lie together: a warp stores 512 bytes
+        const int D = a.head_dim;
+        float4 *o = reinterpret_cast<float4 *>(a.part) + slot * (kTileRows * (size_t)D / 4) + r_own;
+        for (int d = 16 * part; d < D; d += 16 * kParts) {
+          uint32_t r[16];
+          tmem_ld16(my + Sh::kTmemO + d, r);
+          tmem_ld_wait(r);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            o[(size_t)(d / 4 + i) * kTileRows] =
+                make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]), __uint_as_float(r[4 * i + 2]),
+                            __uint_as_float(r[4 * i + 3]));
+        }
+      }
+      soft_sync();  // O, red and the segment are read: the next may overwrite them
+    }
+  } else if (warp == kMmaWarp) {
+    // ---- MMA issue ----
+    if (lane == 0) {
+      const int D = a.head_dim;
+      const uint32_t idesc_s = idesc_f16(128, BT, false), idesc_o = idesc_f16(128, D, true), tmem = sh->tmem;
+      Walk walk = sh->walk;
+      Segment sg;
+      uint32_t g = 0;
+      bool ok = true;
+      auto scores = [&](uint32_t i) {
+        const int st = i % ST;
+        ok = ok && mbar_wait(&sh->kfull[st], (i / ST) & 1, abort_s);
+        // S of tile i lies where P of tile i - 2 was: its product is done
+        if (ok && i >= 2) ok = mbar_wait(&sh->vempty[(i - 2) % ST], ((i - 2) / ST) & 1, abort_s);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t base = smem_u32(sK + st * Sh::kBytes);
+        for (int k = 0; k < D / 16; ++k)
+          mma_f16_ts(tmem + Sh::kTmemS + (i & 1) * BT, tmem + Sh::kTmemQ + 8 * k,
+                     smem_desc(base + (k >> 2) * (BT * 128) + (k & 3) * 32, 16, 1024, 2), idesc_s, k > 0);
+        tc_commit(&sh->sfull[i & 1]);
+        tc_commit(&sh->kempty[st]);
+      };
+      for (int seg = 0; ok && walk.next(a, BT, sg); ++seg) {
+        ok = mbar_wait(&sh->qready, seg & 1, abort_s);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t g0 = g, g1 = g + max(0, sg.j1 - sg.j0);
+        if (g1 > g0) scores(g0);
+        for (; ok && g < g1; ++g) {
+          if (g + 1 < g1) scores(g + 1);
+          const int st = g % ST;
+          ok = ok && mbar_wait(&sh->vfull[st], (g / ST) & 1, abort_s) &&
+               mbar_wait(&sh->pready[g & 1], (g >> 1) & 1, abort_s);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t base = smem_u32(sV + st * Sh::kBytes);
+#pragma unroll
+          for (int k = 0; k < BT / 16; ++k)
+            mma_f16_ts(tmem + Sh::kTmemO, tmem + Sh::kTmemS + (g & 1) * BT + 8 * k,
+                       smem_desc(base + k * 2048, BT * 128, 1024, 2), idesc_o, g > g0 || k > 0);
+          tc_commit(&sh->vempty[st]);
+        }
+      }
+      if (!ok) {  // what was issued ends before its TMEM is given back
+        give_up(a.error, abort_s);
+        tc_commit(&sh->drain);
+        mbar_wait(&sh->drain, 0, &sh->never);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kLoadWarp) {
+    // ---- codes to shared memory ----
+    if (lane == 0) {
+      Walk walk = sh->walk;
+      Segment sg;
+      uint32_t g = 0;
+      bool ok = true;
+      const int boxes = (a.head_dim + Sh::kBox - 1) / Sh::kBox;
+      while (ok && walk.next(a, BT, sg)) {
+        for (int j = sg.j0; ok && j < sg.j1; ++j, ++g) {
+          const int st = g % RAW;
+          auto fetch = [&](const CUtensorMap *map, uint8_t *to, uint64_t *full, uint64_t *empty) {
+            if (g >= RAW && ok) ok = mbar_wait(empty, ((g / RAW) - 1) & 1, abort_s);
+            if (!ok) return;
+            mbar_arrive_expect_tx(full, (uint32_t)boxes * (BT * Sh::kBox));
+            for (int x = 0; x < boxes; ++x)
+              tma_load_4d(to + x * (BT * Sh::kBox), map, x * Sh::kBox, sg.kvh, j * BT, sg.b, full);
+          };
+          fetch(&k_map, rK + st * Sh::kRawBytes, &sh->rkfull[st], &sh->rkempty[st]);
+          fetch(&v_map, rV + st * Sh::kRawBytes, &sh->rvfull[st], &sh->rvempty[st]);
+        }
+      }
+      if (!ok) give_up(a.error, abort_s);
+      // the copies in flight land before the block ends
+      for (uint32_t i = g > RAW ? g - RAW : 0; i < g; ++i) {
+        mbar_wait(&sh->rkfull[i % RAW], (i / RAW) & 1, &sh->never);
+        mbar_wait(&sh->rvfull[i % RAW], (i / RAW) & 1, &sh->never);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- codes to f16 tiles ----
+    // A warp takes 64 bytes of eight tokens at a time (lane % 8 the token, lane
+    // / 8 the 16-byte piece): eight lanes' 16-byte accesses then fall on all
+    // banks on both sides, and a thread's pieces lie at one distance.
+    const int cw = warp - kConvWarp;
+    constexpr int P = Sh::kPieces, X = BT / 32, kStep = BT / P;
+    const int ch = (cw % (DP / 64)) * 4 + (lane >> 3), t_own = cw / (DP / 64) * 8 + (lane & 7);
+    const uint32_t src = DP == 64 ? t_own * 64 + ((ch ^ ((t_own >> 1) & 3)) * 16)
+                                  : (ch >> 3) * (BT * 128) + t_own * 128 + (((ch & 7) ^ (t_own & 7)) * 16);
+    const uint32_t dst = (ch >> 2) * (BT * 128) + t_own * 128 + (((2 * (ch & 3)) ^ (t_own & 7)) * 16);
+    Walk walk = sh->walk;
+    Segment sg;
+    bool more = false;
+    int j = 0;
+    auto enter = [&]() {  // the next segment that is not empty
+      do more = walk.next(a, BT, sg);
+      while (more && sg.j1 <= sg.j0);
+      j = more ? sg.j0 : 0;
+    };
+    enter();
+    uint32_t xk[X], xv[X];
+    auto load_exps = [&]() {
+      const size_t row = ((size_t)sg.b * a.max_seq + (size_t)j * BT) * a.kv_heads + sg.kvh;
+      const int live = sg.total - j * BT;
+#pragma unroll
+      for (int i = 0; i < X; ++i) {
+        const int t = lane + 32 * i;
+        xk[i] = t < live ? a.k_exp[row + (size_t)t * a.kv_heads] : 127;
+        xv[i] = t < live ? a.v_exp[row + (size_t)t * a.kv_heads] : 127;
+      }
+    };
+    auto fetch = [&](const uint8_t *stage, uint4(&v)[P]) {
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        v[i] = *reinterpret_cast<const uint4 *>(stage + src + i * kStep * (DP == 64 ? 64 : 128));
+    };
+    auto store = [&](uint8_t *stage, const uint4(&v)[P]) {
+      uint8_t *to = stage + dst, *and_to = stage + (dst ^ 16);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        uint32_t o[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          o[2 * k] = e4m3x2_to_f16x2((uint16_t)w[k]);
+          o[2 * k + 1] = e4m3x2_to_f16x2((uint16_t)(w[k] >> 16));
+        }
+        *reinterpret_cast<uint4 *>(to + i * kStep * 128) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4 *>(and_to + i * kStep * 128) = make_uint4(o[4], o[5], o[6], o[7]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    if (more && cw == 0) load_exps();
+    // After a wait that ran out this role goes on to its end without waiting
+    // (the results are void): its warps meet at a barrier in open tiles.
+    bool ok = true;
+    auto wait = [&](uint64_t *bar, uint32_t phase) {
+      if (ok) ok = mbar_wait(bar, phase & 1, abort_s);
+      if (!ok) give_up(a.error, abort_s);
+      __syncwarp();
+    };
+    for (uint32_t g = 0; more; ++g) {
+      const int st = g % ST, rs = g % RAW;
+      const bool open = (j + 1) * BT > sg.pos;
+      float *ft = reinterpret_cast<float *>(sh->fac[g % META]);
+      uint4 kb[P], vb[P];
+      wait(&sh->rkfull[rs], g / RAW);
+      fetch(rK + rs * Sh::kRawBytes, kb);
+      if (g >= ST) wait(&sh->kempty[st], g / ST - 1);
+      if (cw == 0) {
+#pragma unroll
+        for (int i = 0; i < X; ++i) {
+          const int t = lane + 32 * i;
+          ft[(t >> 1) * 4 + (t & 1)] = kv8_factor(xk[i]);
+          ft[(t >> 1) * 4 + 2 + (t & 1)] = pow2i((int)kv8_value_exponent(xv[i]));
+        }
+      }
+      if (open) {  // values that are not a number: zero in the product, and the token's score NaN for those who see it
+        wait(&sh->rvfull[rs], g / RAW);
+        fetch(rV + rs * Sh::kRawBytes, vb);
+        conv_sync();
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          uint32_t w[4] = {vb[i].x, vb[i].y, vb[i].z, vb[i].w}, any = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t bad = __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            w[k] &= ~bad;
+            any |= bad;
+          }
+          vb[i] = make_uint4(w[0], w[1], w[2], w[3]);
+          const int t = t_own + i * kStep;
+          if (any) ft[(t >> 1) * 4 + (t & 1)] = __int_as_float(0x7fc00000);
+        }
+        conv_sync();
+      }
+      __syncwarp();
+      if (cw == 0 && lane == 0) mbar_arrive(&sh->metafull[g % META]);
+      store(sK + st * Sh::kBytes, kb);
+      if (lane == 0) {
+        mbar_arrive(&sh->kfull[st]);
+        mbar_arrive(&sh->rkempty[rs]);
+      }
+      if (!open) {
+        wait(&sh->rvfull[rs], g / RAW);
+        fetch(rV + rs * Sh::kRawBytes, vb);
+      }
+      if (++j >= sg.j1) enter();
+      if (more && cw == 0) load_exps();
+      if (g >= ST) wait(&sh->vempty[st], g / ST - 1);
+      store(sV + st * Sh::kBytes, vb);
+      if (lane == 0) {
+        mbar_arrive(&sh->vfull[st]);
+        mbar_arrive(&sh->rvempty[rs]);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(sh->tmem, 512);
+  }
+}
+
+// The blocks that share a row tile's tokens meet, in order, with the gate:
+// block (16 rows of a row tile, 64 columns); thread (row, four columns, share
+// of the blocks).  Rows of nodes that are not there become zeros.
+constexpr int kMergeShares = 4;
+__global__ void __launch_bounds__(1024, 1) tree_attn_tile_merge_kernel(const __grid_constant__ TreeArgs a, int BT) {
+  pdl_enter();
+  __shared__ float4 acc_s[kMergeShares - 1][256];
+  __shared__ float2 ml_s[kMergeShares - 1][256];
+  const int t = threadIdx.x, share = threadIdx.y, D = a.head_dim;
+  const int rows = a.nodes * a.group, row_tiles = (rows + kTileRows - 1) / kTileRows, items = a.kv_heads * row_tiles;
+  const int item = blockIdx.x / (kTileRows / 16), r = blockIdx.x % (kTileRows / 16) * 16 + (t & 15);
+  const int b = item / items, kvh = item % items / row_tiles, row = item % row_tiles * kTileRows + r;
+  if (item % row_tiles * kTileRows + (r & ~15) >= rows) return;
+  const int d = blockIdx.y * 64 + 4 * (t >> 4);
+  const bool live = row < rows && d < D;
+  const int n = row / a.group, h = kvh * a.group + row % a.group;
+  const bool some = session_tiles(a, b, BT) > 0;
+  float m = -INFINITY, l = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto add = [&](float2 v, float4 x) {
+    const float mn = fmaxf(m, v.x), fo = exp2_approx(m - mn), fn = exp2_approx(v.x - mn);
+    l = l * fo + v.y * fn;
+    acc.x = acc.x * fo + x.x * fn;
+    acc.y = acc.y * fo + x.y * fn;
+    acc.z = acc.z * fo + x.z * fn;
+    acc.w = acc.w * fo + x.w * fn;
+    m = mn;
+  };
+  if (some) {
+    const int2 from = a.shares[item];  // its first slot, its last block
+    const float4 *part = reinterpret_cast<const float4 *>(a.part) + (size_t)(live ? d / 4 : 0) * kTileRows + r;
+    const int c0 = from.x >> 1;
+#pragma unroll 4
+    for (int c = c0 + share; c <= from.y; c += blockDim.y) {
+      const size_t slot = c == c0 ? from.x : c * 2;
+      const float2 v = a.part_ml[slot * kTileRows + r];
+      const float4 x = part[slot * (kTileRows * (size_t)D / 4)];
+      if (v.x != -INFINITY) add(v, x);
+    }
+  }
+  if (blockDim.y > 1) {
+    if (share > 0) {
+      acc_s[share - 1][t] = acc;
+      ml_s[share - 1][t] = make_float2(m, l);
+    }
+    __syncthreads();
+    if (share > 0) return;
+    for (int i = 0; i < (int)blockDim.y - 1; ++i)
+      if (ml_s[i][t].x != -INFINITY) add(ml_s[i][t], acc_s[i][t]);
+  }
+  const bool there = sight_of(a, b, row < rows ? n : a.nodes, a.positions[b]).upto >= 0 && some;
+  if (!live) return;
+  const size_t node = (size_t)b * a.nodes + n;
+  float o[4] = {acc.x, acc.y, acc.z, acc.w};
+  const float inv = 1.0f / l;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    o[i] = there ? o[i] * inv : 0.0f;
+    if (there && a.gate) o[i] /= 1.0f + expf(-a.gate[node * a.gate_pitch + (size_t)h * a.gate_head + d + i]);
+  }
+  *reinterpret_cast<uint2 *>(a.out + (node * a.q_heads + h) * D + d) =
+      make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+}
+
+template <int DP>
+int launch(const TreeArgs &a, const TilePlan &p, cudaStream_t s) {
+  using Sh = TileShape<DP>;
+  constexpr size_t smem =
+      1023 + (sizeof(TileShared) + 1023) / 1024 * 1024 + 2 * (size_t)Sh::ST * Sh::kBytes + 2 * (size_t)Sh::RAW * Sh::kRawBytes;
+  static_assert(smem <= 227 * 1024);
+  {
+    static std::mutex mu;
+    static std::vector<int> done;
+    int dev = 0;
+    FPB_CUDA_TRY(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lock(mu);
+    if (std::find(done.begin(), done.end(), dev) == done.end()) {
+      FPB_CUDA_TRY(cudaFuncSetAttribute(tree_attn_tile_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)smem));
+      done.push_back(dev);
+    }
+  }
+  CUtensorMap k_map, v_map;
+  if (int st = encode_cache_u8(&k_map, a.k_codes, a.batch, a.max_seq, a.kv_heads, a.head_dim, Sh::kBox, Sh::BT))
+    return st;
+  if (int st = encode_cache_u8(&v_map, a.v_codes, a.batch, a.max_seq, a.kv_heads, a.head_dim, Sh::kBox, Sh::BT))
+    return st;
+  cudaError_t e =
+      launch_pdl(tree_attn_tile_kernel<DP>, dim3((unsigned)p.blocks), kTileThreads, smem, s, a, k_map, v_map);
+  if (e != cudaSuccess) return cuda_fail(e, "tree_attn_tile_kernel");
+  FPB_LAUNCH_CHECK("tree_attn_tile_kernel");
+  // a row tile's blocks in one thread's loop while they are few
+  const unsigned shares = (size_t)p.blocks > 16 * p.items ? kMergeShares : 1;
+  e = launch_pdl(tree_attn_tile_merge_kernel,
+                 dim3((unsigned)(p.items * (kTileRows / 16)), (unsigned)((a.head_dim + 63) / 64)), dim3(256, shares), 0, s,
+                 a, p.BT);
+  if (e != cudaSuccess) return cuda_fail(e, "tree_attn_tile_merge_kernel");
+  FPB_LAUNCH_CHECK("tree_attn_tile_merge_kernel");
+  return FPB_OK;
+}
+
+}  // namespace
+
+TilePlan tile_plan(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, size_t head_dim, size_t max_seq) {
+  TilePlan p;
+  p.BT = head_dim > 128 ? 64 : 128;
+  p.items = batch * kv_heads * ((nodes * (q_heads / kv_heads) + kTileRows - 1) / kTileRows);
+  p.units = p.items * ((max_seq + p.BT - 1) / p.BT);
+  p.blocks = (int)std::min<size_t>(sm_count(), p.units);
+  return p;
+}
+
+size_t tile_workspace_bytes(const TilePlan &p, size_t head_dim) {
+  return (size_t)p.blocks * 2 * kTileRows * (head_dim + 2) * sizeof(float) + p.items * sizeof(int2);
+}
+
+int run_tree_tiles(TreeArgs a, const TilePlan &p, void *workspace, cudaStream_t s) {
+  a.part = static_cast<float *>(workspace);
+  a.part_ml = reinterpret_cast<float2 *>(a.part + (size_t)p.blocks * 2 * kTileRows * a.head_dim);
+  a.shares = reinterpret_cast<int2 *>(a.part_ml + (size_t)p.blocks * 2 * kTileRows);
+  return a.head_dim <= 64 ? launch<64>(a, p, s) : a.head_dim <= 128 ? launch<128>(a, p, s) : launch<256>(a, p, s);
+}
+
+}  // namespace fpb
