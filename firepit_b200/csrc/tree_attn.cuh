@@ -16,7 +16,13 @@ struct TreeArgs {
   __nv_bfloat16 *out;
   float *part;     // [session, kv head, row tile][split][row][head_dim] numerators
   float2 *part_ml; // [session, kv head, row tile][split][row] maximum, sum
-  int2 *shares;    // (tiles) [session, kv head, row tile] first slot, last block
+  // for the tiles: queries as f16, their factors, what each node sees [session,
+  // 64], [session, kv head, row tile] first slot and last block, blocks' shares
+  uint4 *q16;
+  float *q_fac;
+  uint64_t *sights;
+  int2 *shares;
+  void *walks;
   int *error;
 };
 
@@ -126,7 +132,7 @@ constexpr float kHead = 7.0f, kLag = 8.0f, kMost = 32768.0f, kLowest = -1e30f;
 // them, their partial results and the items' shares of them in the workspace.
 struct TilePlan {
   int BT, blocks;
-  size_t items, units;  // units: a bound
+  size_t batch, items, units;  // units: a bound
 };
 TilePlan tile_plan(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, size_t head_dim, size_t max_seq);
 size_t tile_workspace_bytes(const TilePlan &p, size_t head_dim);

@@ -56,8 +56,6 @@ struct Walk {
   __device__ __forceinline__ bool next(const TreeArgs &a, int BT, Segment &s);
 };
 
-constexpr int kQPitch = 40;  // f16 elements of a staged query row's 32 columns: rows on distinct banks
-
 // Fixed part of the block's shared memory; the stages follow, 1024-byte aligned.
 struct TileShared {
   uint64_t kfull[2], kempty[2], vfull[2], vempty[2], rkfull[2], rvfull[2], rkempty[2], rvempty[2], sfull[2], pready[2],
@@ -69,7 +67,6 @@ struct TileShared {
   float red[kParts][kTileRows];  // maxima, then sums, of the rows' parts
   uint64_t sight[kTileRows];     // a tree: the bits; a chain: the limit
   float4 fac[4][64];             // [META][pair of tokens]: two keys' factors, two values'
-  __align__(16) __half q[2 * 4 * 32 * kQPitch];
 };
 
 // Token tiles of session b (0: none of its nodes is there).
@@ -250,95 +247,76 @@ __device__ __noinline__ float2 raise_max(TileShared *sh, uint32_t s_tmem, uint32
   return make_float2(mn, old);
 }
 
-// A quad's 32 queries to TMEM as f16: 32 columns at a time, four rows a load
-// (8 lanes, four columns each), two warps taking the columns' chunks in turn,
-// through shared memory to the rows' lanes.  They are taken as they are where
-// every row's largest magnitude lies well inside f16's range, else again with
-// each row's power of two.  Returns the row's factor of the scores.
-__device__ __noinline__ float load_queries(const TreeArgs &a, TileShared *sh, uint32_t q_tmem) {
-  const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3, part = threadIdx.x >> 7, r_own = threadIdx.x & 127;
-  const int rows = a.nodes * a.group, D = a.head_dim;
-  __half *stage = sh->q + (size_t)(part * 4 + quad) * 32 * kQPitch;  // parts 0 and 1
-  const int r_sub = lane >> 3, c_sub = 4 * (lane & 7);
-  int qe = 0;
-  for (int round = 0; round < 2; ++round) {
-    if (part < 2) {
-      float am[8];
+// What the tile kernel reads at its start, made by blocks of 32 rows of a row
+// tile (eight warps): the queries as f16 in the order of its TMEM stores
+// [item][eight columns][128 rows], each row scaled by a power of two into f16's
+// range, with the factor of its scores; what each node sees; each block's
+// share of the units.
+constexpr int kPrepRows = 32;
+__global__ void __launch_bounds__(256) tree_attn_prep_kernel(const __grid_constant__ TreeArgs a, int BT, int blocks) {
+  pdl_enter();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = a.head_dim;
+  const int rows = a.nodes * a.group, row_tiles = (rows + kTileRows - 1) / kTileRows, items = a.kv_heads * row_tiles;
+  const int item = blockIdx.x / (kTileRows / kPrepRows), r0 = blockIdx.x % (kTileRows / kPrepRows) * kPrepRows + warp * 4;
+  const int b = item / items, kvh = item % items / row_tiles, row0 = item % row_tiles * kTileRows + r0;
+  const int col = lane * 8;
+  float x[4][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) am[i] = 0.0f;
-      for (int d = 32 * part; d < D; d += 64) {
+  for (int i = 0; i < 4; ++i) {
+    const int row = row0 + i, n = row / a.group;
 #pragma unroll
-        for (int i0 = 0; i0 < 8; i0 += 4) {
-          float4 x[4];
+    for (int k = 0; k < 8; ++k) x[i][k] = 0.0f;
+    if (row >= rows || col >= D) continue;
+    const size_t at = ((size_t)b * a.nodes + n) * a.q_pitch + (size_t)(kvh * a.group + (row - n * a.group)) * a.q_head + col;
+    if (!a.q_vec) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = sh->seg.rt * kTileRows + quad * 32 + 4 * (i0 + i) + r_sub;
-            x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (r >= rows || d + c_sub >= D) continue;
-            const int n = r / a.group;
-            const size_t o = ((size_t)sh->seg.b * a.nodes + n) * a.q_pitch +
-                             (size_t)(sh->seg.kvh * a.group + (r - n * a.group)) * a.q_head + d + c_sub;
-            if (!a.q_vec) {
-              x[i] = make_float4(load_q(a, o), load_q(a, o + 1), load_q(a, o + 2), load_q(a, o + 3));
-            } else if (a.q_bf16) {
-              const uint2 v = *reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(a.q) + o);
-              x[i] = make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u),
-                                 __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
-            } else {
-              x[i] = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + o);
-            }
-          }
+      for (int k = 0; k < 8; ++k) x[i][k] = load_q(a, at + k);
+    } else if (a.q_bf16) {
+      const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) + at);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = 4 * (i0 + i) + r_sub;
-            am[i0 + i] = fmaxf(am[i0 + i],
-                               fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
-            const float f = pow2i(-__shfl_sync(0xffffffffu, qe, r));
-            *reinterpret_cast<uint2 *>(stage + r * kQPitch + c_sub) =
-                make_uint2(pack_f16x2(x[i].x * f, x[i].y * f), pack_f16x2(x[i].z * f, x[i].w * f));
-          }
-        }
-        __syncwarp();
-        uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4 v = *reinterpret_cast<const uint4 *>(stage + lane * kQPitch + 8 * i);
-          w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-        }
-        tmem_st16(q_tmem + d / 2, w);
-        __syncwarp();
+      for (int k = 0; k < 4; ++k) {
+        x[i][2 * k] = __uint_as_float(w[k] << 16);
+        x[i][2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
       }
-      tmem_st_wait();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) am[i] = fmaxf(am[i], __shfl_xor_sync(0xffffffffu, am[i], o));
-        if (round == 0 && (lane & 7) == 0) sh->red[part][quad * 32 + 4 * i + r_sub] = am[i];
-      }
+    } else {
+      const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at);
+      const float4 u = p[0], v = p[1];
+      x[i][0] = u.x; x[i][1] = u.y; x[i][2] = u.z; x[i][3] = u.w;
+      x[i][4] = v.x; x[i][5] = v.y; x[i][6] = v.z; x[i][7] = v.w;
     }
-    quad_sync(quad);
-    if (round) break;
-    const float big = fmaxf(sh->red[0][r_own], sh->red[1][r_own]);
-    if (!quad_any(quad, big != 0.0f && !(big >= 0x1p-3f && big < 0x1p15f))) break;
-    qe = q_exponent(big);
   }
-  return pow2i(qe) * a.scale_log2;
-}
-
-// This block's share of the units, warp 0.
-__device__ __noinline__ void share_out(const TreeArgs &a, TileShared *sh, int BT, int row_tiles) {
-  const int lane = threadIdx.x & 31, items = a.kv_heads * row_tiles;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float amax = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(x[i][k]));
+    const int e = q_exponent(warp_max(amax));
+    const float f = pow2i(-e);
+    if (col < D)
+      a.q16[((size_t)item * (D / 8) + lane) * kTileRows + r0 + i] =
+          make_uint4(pack_f16x2(x[i][0] * f, x[i][1] * f), pack_f16x2(x[i][2] * f, x[i][3] * f),
+                     pack_f16x2(x[i][4] * f, x[i][5] * f), pack_f16x2(x[i][6] * f, x[i][7] * f));
+    if (lane == 0) a.q_fac[(size_t)item * kTileRows + r0 + i] = pow2i(e) * a.scale_log2;
+  }
+  // a session's first row tile: its nodes' sights
+  if (a.parents && item % items == 0 && r0 < 2 * 4 && warp < 2) {
+    const Sight s = sight_of(a, b, warp * 32 + lane, a.positions[b]);
+    if (warp * 32 + lane < a.nodes) a.sights[(size_t)b * kTreeMaxNodes + warp * 32 + lane] = s.bits;
+  }
+  const int c = blockIdx.x * 8 + warp;  // the block whose share this warp finds
+  if (c >= blocks) return;
   int all = 0;
   for (int i = lane; i < a.batch; i += 32) all += session_tiles(a, i, BT);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-  const int units = all * items, blocks = min((int)gridDim.x, units);
+  const int units = all * items, live = min(blocks, units);
   int u0 = 0, u1 = 0;
-  if ((int)blockIdx.x < blocks) {
-    u0 = (int)((long long)units * blockIdx.x / blocks);
-    u1 = (int)((long long)units * (blockIdx.x + 1) / blocks);
+  if (c < live) {
+    u0 = (int)((long long)units * c / live);
+    u1 = (int)((long long)units * (c + 1) / live);
   }
-  int b = 0, before = 0;  // the session that holds unit u0, and the units before it
+  int s = 0, before = 0;  // the session that holds unit u0, and the units before it
   if (u1 > u0)
     for (int i0 = 0; i0 < a.batch; i0 += 32) {
       const int n = i0 + lane < a.batch ? session_tiles(a, i0 + lane, BT) * items : 0;
@@ -350,34 +328,28 @@ __device__ __noinline__ void share_out(const TreeArgs &a, TileShared *sh, int BT
       }
       const unsigned past = __ballot_sync(0xffffffffu, before + sum > u0);
       const int k = past ? __ffs(past) - 1 : 31;
-      const int held = __shfl_sync(0xffffffffu, past ? sum - n : sum, k);
-      before += held;
+      before += __shfl_sync(0xffffffffu, past ? sum - n : sum, k);
       if (past) {
-        b = i0 + k;
+        s = i0 + k;
         break;
       }
     }
-  if (lane == 0)
-    sh->walk = sh->soft_walk = Walk{b, u1 > u0 ? session_tiles(a, b, BT) : 1, row_tiles, u0 - before, u1 - u0};
+  if (lane == 0) static_cast<Walk *>(a.walks)[c] = Walk{s, u1 > u0 ? session_tiles(a, s, BT) : 1, row_tiles, u0 - before, u1 - u0};
 }
 
 template <int DP>
 __global__ void __launch_bounds__(kTileThreads, 1)
     tree_attn_tile_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap k_map,
                           const __grid_constant__ CUtensorMap v_map) {
-  pdl_enter();
   using Sh = TileShape<DP>;
   constexpr int BT = Sh::BT, ST = Sh::ST, RAW = Sh::RAW, META = Sh::META;
-  extern __shared__ uint8_t raw_sm[];
-  uint8_t *const base_sm = raw_sm + (-smem_u32(raw_sm) & 1023);
-  TileShared *const sh = reinterpret_cast<TileShared *>(base_sm);
-  uint8_t *const sK = base_sm + (sizeof(TileShared) + 1023) / 1024 * 1024, *const sV = sK + ST * Sh::kBytes;
+  extern __shared__ __align__(1024) uint8_t raw_sm[];
+  TileShared *const sh = reinterpret_cast<TileShared *>(raw_sm);
+  uint8_t *const sK = raw_sm + (sizeof(TileShared) + 1023) / 1024 * 1024, *const sV = sK + ST * Sh::kBytes;
   uint8_t *const rK = sV + ST * Sh::kBytes, *const rV = rK + RAW * Sh::kRawBytes;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool tree = a.parents != nullptr;
-  if (warp == 0) {
-    share_out(a, sh, BT, (a.nodes * a.group + kTileRows - 1) / kTileRows);
-  } else if (warp == kMmaWarp) {
+  if (warp == kMmaWarp) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&sh->kfull[i], kConvWarps);
@@ -401,16 +373,26 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     tmem_alloc(&sh->tmem, 512);
     tmem_relinquish();
   }
+  pdl_enter();
+  if (tid == 0) sh->walk = sh->soft_walk = static_cast<const Walk *>(a.walks)[blockIdx.x];
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   volatile int *const abort_s = &sh->abort;
+  // (an allocation of all of TMEM's columns begins at 0, and this block's
+  // shared memory on 1024 bytes: the addresses below are then constants)
+  if (sh->tmem != 0 || (smem_u32(raw_sm) & 1023)) {
+    if (tid == 0) give_up(a.error, abort_s);
+    __syncthreads();
+    if (warp == kMmaWarp) tmem_dealloc(sh->tmem, 512);
+    return;
+  }
 
   if (warp < kSoftWarps) {
     // ---- softmax ----
     constexpr int NT = BT / kParts;
     const int quad = warp & 3, part = warp >> 2, r_own = quad * 32 + lane;
-    const uint32_t my = sh->tmem + ((uint32_t)(quad * 32) << 16);
+    const uint32_t my = (uint32_t)(quad * 32) << 16;
     uint32_t g = 0;  // tiles so far
     // After a wait that ran out this role goes on to its end without waiting
     // (the results are void): its warps meet at barriers.
@@ -428,12 +410,35 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       soft_sync();
       if (!sh->more) break;
       const int j0 = sh->seg.j0, j1 = sh->seg.j1, pos = sh->seg.pos;
-      if (part == 0) {
-        const int row = sh->seg.rt * kTileRows + r_own;
-        const Sight s = sight_of(a, sh->seg.b, row < a.nodes * a.group ? row / a.group : a.nodes, pos);
-        sh->sight[r_own] = tree ? s.bits : (uint64_t)max(s.upto, 0);
+      const float f = a.q_fac[(size_t)sh->seg.item * kTileRows + r_own];
+      {
+        // 16 columns of the row at a time; a warp's loads are 512 bytes together
+        const uint4 *q = a.q16 + (size_t)sh->seg.item * (a.head_dim / 8) * kTileRows + r_own;
+        constexpr int kQ = DP / 16 / kParts;
+        uint4 v[kQ][2];
+#pragma unroll
+        for (int i = 0; i < kQ; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            v[i][k] = (i * kParts + part) * 16 < a.head_dim ? q[(size_t)((i * kParts + part) * 2 + k) * kTileRows]
+                                                            : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < kQ; ++i) {
+          const uint32_t w[8] = {v[i][0].x, v[i][0].y, v[i][0].z, v[i][0].w, v[i][1].x, v[i][1].y, v[i][1].z, v[i][1].w};
+          tmem_st8(my + Sh::kTmemQ + (i * kParts + part) * 8, w);
+        }
       }
-      const float f = load_queries(a, sh, my + Sh::kTmemQ);
+      if (part == 0) {
+        const int n = (sh->seg.rt * kTileRows + r_own) / a.group;
+        uint64_t s = 0;
+        if (tree)
+          s = n < a.nodes ? a.sights[(size_t)sh->seg.b * kTreeMaxNodes + n] : 0;
+        else if (n < a.nodes && pos >= 0 && pos < a.max_seq - n)
+          s = n + 1;
+        sh->sight[r_own] = s;
+      }
+      tmem_st_wait();
+      quad_sync(quad);
       if (lane == 0) mbar_arrive(&sh->qready);
       float m = kLowest;
       uint64_t l2 = 0;
@@ -534,53 +539,67 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
   } else if (warp == kMmaWarp) {
     // ---- MMA issue ----
-    if (lane == 0) {
-      const int D = a.head_dim;
-      const uint32_t idesc_s = idesc_f16(128, BT, false), idesc_o = idesc_f16(128, D, true), tmem = sh->tmem;
-      Walk walk = sh->walk;
-      Segment sg;
-      uint32_t g = 0;
-      bool ok = true;
-      auto scores = [&](uint32_t i) {
-        const int st = i % ST;
-        ok = ok && mbar_wait(&sh->kfull[st], (i / ST) & 1, abort_s);
-        // S of tile i lies where P of tile i - 2 was: its product is done
-        if (ok && i >= 2) ok = mbar_wait(&sh->vempty[(i - 2) % ST], ((i - 2) / ST) & 1, abort_s);
-        if (!ok) return;
-        tc_fence_after();
-        const uint32_t base = smem_u32(sK + st * Sh::kBytes);
-        for (int k = 0; k < D / 16; ++k)
-          mma_f16_ts(tmem + Sh::kTmemS + (i & 1) * BT, tmem + Sh::kTmemQ + 8 * k,
-                     smem_desc(base + (k >> 2) * (BT * 128) + (k & 3) * 32, 16, 1024, 2), idesc_s, k > 0);
+    // The whole warp keeps the loop, so that what it computes is known to be
+    // the warp's; one lane issues.
+    const bool leader = elect_one();
+    const int D = a.head_dim;
+    const uint32_t idesc_s = idesc_f16(128, BT, false), idesc_o = idesc_f16(128, D, true);
+    Walk walk = sh->walk;
+    Segment sg;
+    uint32_t g = 0;
+    bool ok = true;
+    auto scores = [&](uint32_t i) {
+      const uint32_t st = i % ST;
+      ok = ok && mbar_wait(&sh->kfull[st], (i / ST) & 1, abort_s);
+      // S of tile i lies where P of tile i - 2 was: its product is done
+      if (ok && i >= 2) ok = mbar_wait(&sh->vempty[(i - 2) % ST], ((i - 2) / ST) & 1, abort_s);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      tc_fence_after();
+      const uint64_t desc = smem_desc(smem_u32(sK) + st * Sh::kBytes, 16, 1024, 2);
+      const uint32_t to = Sh::kTmemS + (i & 1) * BT;
+      if (leader) {
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+          if (16 * k < D)
+            mma_f16_ts(to, Sh::kTmemQ + 8 * k, desc + (((k >> 2) * (BT * 128) + (k & 3) * 32) >> 4), idesc_s, k > 0);
         tc_commit(&sh->sfull[i & 1]);
         tc_commit(&sh->kempty[st]);
-      };
-      for (int seg = 0; ok && walk.next(a, BT, sg); ++seg) {
-        ok = mbar_wait(&sh->qready, seg & 1, abort_s);
+      }
+      __syncwarp();
+    };
+    for (int seg = 0; ok && walk.next(a, BT, sg); ++seg) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh->qready, seg & 1, abort_s));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t g0 = g, g1 = g + max(0, sg.j1 - sg.j0);
+      if (g1 > g0) scores(g0);
+      for (; ok && g < g1; ++g) {
+        if (g + 1 < g1) scores(g + 1);
+        const uint32_t st = g % ST;
+        ok = ok && mbar_wait(&sh->vfull[st], (g / ST) & 1, abort_s) &&
+             mbar_wait(&sh->pready[g & 1], (g >> 1) & 1, abort_s);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t g0 = g, g1 = g + max(0, sg.j1 - sg.j0);
-        if (g1 > g0) scores(g0);
-        for (; ok && g < g1; ++g) {
-          if (g + 1 < g1) scores(g + 1);
-          const int st = g % ST;
-          ok = ok && mbar_wait(&sh->vfull[st], (g / ST) & 1, abort_s) &&
-               mbar_wait(&sh->pready[g & 1], (g >> 1) & 1, abort_s);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t base = smem_u32(sV + st * Sh::kBytes);
+        const uint64_t desc = smem_desc(smem_u32(sV) + st * Sh::kBytes, BT * 128, 1024, 2);
+        const uint32_t from = Sh::kTmemS + (g & 1) * BT;
+        if (leader) {
 #pragma unroll
           for (int k = 0; k < BT / 16; ++k)
-            mma_f16_ts(tmem + Sh::kTmemO, tmem + Sh::kTmemS + (g & 1) * BT + 8 * k,
-                       smem_desc(base + k * 2048, BT * 128, 1024, 2), idesc_o, g > g0 || k > 0);
+            mma_f16_ts(Sh::kTmemO, from + 8 * k, desc + (k * 2048 >> 4), idesc_o, g > g0 || k > 0);
           tc_commit(&sh->vempty[st]);
         }
+        __syncwarp();
       }
-      if (!ok) {  // what was issued ends before its TMEM is given back
+    }
+    if (!ok) {  // what was issued ends before its TMEM is given back
+      if (leader) {
         give_up(a.error, abort_s);
         tc_commit(&sh->drain);
-        mbar_wait(&sh->drain, 0, &sh->never);
       }
+      __syncwarp();
+      mbar_wait(&sh->drain, 0, &sh->never);
     }
     __syncwarp();
   } else if (warp == kLoadWarp) {
@@ -790,8 +809,9 @@ __global__ void __launch_bounds__(1024, 1) tree_attn_tile_merge_kernel(const __g
     for (int i = 0; i < (int)blockDim.y - 1; ++i)
       if (ml_s[i][t].x != -INFINITY) add(ml_s[i][t], acc_s[i][t]);
   }
-  const bool there = sight_of(a, b, row < rows ? n : a.nodes, a.positions[b]).upto >= 0 && some;
   if (!live) return;
+  const int pos = a.positions[b];
+  const bool there = some && (a.parents ? a.sights[(size_t)b * kTreeMaxNodes + n] != 0 : pos >= 0 && pos < a.max_seq - n);
   const size_t node = (size_t)b * a.nodes + n;
   float o[4] = {acc.x, acc.y, acc.z, acc.w};
   const float inv = 1.0f / l;
@@ -808,7 +828,7 @@ template <int DP>
 int launch(const TreeArgs &a, const TilePlan &p, cudaStream_t s) {
   using Sh = TileShape<DP>;
   constexpr size_t smem =
-      1023 + (sizeof(TileShared) + 1023) / 1024 * 1024 + 2 * (size_t)Sh::ST * Sh::kBytes + 2 * (size_t)Sh::RAW * Sh::kRawBytes;
+      (sizeof(TileShared) + 1023) / 1024 * 1024 + 2 * (size_t)Sh::ST * Sh::kBytes + 2 * (size_t)Sh::RAW * Sh::kRawBytes;
   static_assert(smem <= 227 * 1024);
   {
     static std::mutex mu;
@@ -827,7 +847,11 @@ int launch(const TreeArgs &a, const TilePlan &p, cudaStream_t s) {
     return st;
   if (int st = encode_cache_u8(&v_map, a.v_codes, a.batch, a.max_seq, a.kv_heads, a.head_dim, Sh::kBox, Sh::BT))
     return st;
-  cudaError_t e =
+  cudaError_t e = launch_pdl(tree_attn_prep_kernel, dim3((unsigned)(p.items * (kTileRows / kPrepRows))), 256, 0, s, a, p.BT,
+                             p.blocks);
+  if (e != cudaSuccess) return cuda_fail(e, "tree_attn_prep_kernel");
+  FPB_LAUNCH_CHECK("tree_attn_prep_kernel");
+  e =
       launch_pdl(tree_attn_tile_kernel<DP>, dim3((unsigned)p.blocks), kTileThreads, smem, s, a, k_map, v_map);
   if (e != cudaSuccess) return cuda_fail(e, "tree_attn_tile_kernel");
   FPB_LAUNCH_CHECK("tree_attn_tile_kernel");
@@ -846,20 +870,39 @@ int launch(const TreeArgs &a, const TilePlan &p, cudaStream_t s) {
 TilePlan tile_plan(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, size_t head_dim, size_t max_seq) {
   TilePlan p;
   p.BT = head_dim > 128 ? 64 : 128;
+  p.batch = batch;
   p.items = batch * kv_heads * ((nodes * (q_heads / kv_heads) + kTileRows - 1) / kTileRows);
   p.units = p.items * ((max_seq + p.BT - 1) / p.BT);
-  p.blocks = (int)std::min<size_t>(sm_count(), p.units);
+  // (a prep block of eight warps finds eight shares: never more blocks than that)
+  p.blocks = (int)std::min({(size_t)sm_count(), p.units, p.items * (kTileRows / kPrepRows) * 8});
   return p;
 }
 
-size_t tile_workspace_bytes(const TilePlan &p, size_t head_dim) {
-  return (size_t)p.blocks * 2 * kTileRows * (head_dim + 2) * sizeof(float) + p.items * sizeof(int2);
+// The workspace: queries, partial results, sums, sights, factors, shares.
+static size_t lay_out(TreeArgs *a, const TilePlan &p, size_t head_dim, void *workspace) {
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 15) / 16 * 16;
+    return static_cast<uint8_t *>(workspace) + here;
+  };
+  TreeArgs unused{};
+  if (!a) a = &unused;
+  const size_t slots = (size_t)p.blocks * 2 * kTileRows;
+  a->q16 = reinterpret_cast<uint4 *>(take(p.items * kTileRows * head_dim * 2));
+  a->part = reinterpret_cast<float *>(take(slots * head_dim * 4));
+  a->part_ml = reinterpret_cast<float2 *>(take(slots * sizeof(float2)));
+  a->sights = reinterpret_cast<uint64_t *>(take(p.batch * kTreeMaxNodes * 8));
+  a->q_fac = reinterpret_cast<float *>(take(p.items * kTileRows * 4));
+  a->shares = reinterpret_cast<int2 *>(take(p.items * sizeof(int2)));
+  a->walks = take((size_t)p.blocks * sizeof(Walk));
+  return at;
 }
 
+size_t tile_workspace_bytes(const TilePlan &p, size_t head_dim) { return lay_out(nullptr, p, head_dim, nullptr); }
+
 int run_tree_tiles(TreeArgs a, const TilePlan &p, void *workspace, cudaStream_t s) {
-  a.part = static_cast<float *>(workspace);
-  a.part_ml = reinterpret_cast<float2 *>(a.part + (size_t)p.blocks * 2 * kTileRows * a.head_dim);
-  a.shares = reinterpret_cast<int2 *>(a.part_ml + (size_t)p.blocks * 2 * kTileRows);
+  lay_out(&a, p, a.head_dim, workspace);
   return a.head_dim <= 64 ? launch<64>(a, p, s) : a.head_dim <= 128 ? launch<128>(a, p, s) : launch<256>(a, p, s);
 }
 
