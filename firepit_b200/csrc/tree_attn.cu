@@ -8,6 +8,8 @@
 #include <mutex>
 #include <vector>
 
+#include "sm100.cuh"
+#include "tma_host.cuh"
 #include "tree_attn.cuh"
 
 namespace fpb {
@@ -21,11 +23,14 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// ---- few rows: tokens streamed through registers ---------------------------------------------
-// Block (split, session * kv head * row tile): NR rows (8 or 16) of one kv
-// head, four warps that take steps of 16 tokens in turn, all on their own:
-// codes go from memory to registers to the tensor cores with no shared memory
-// between.
+using namespace sm100;
+
+// ---- few rows: warps that stream tokens on their own -------------------------------------------
+// Block (split, session * kv head): NR rows (8 or 16) of one kv head, four
+// warps that take steps of 16 tokens in turn.  Each warp has its own ring of
+// kRowsStages steps of codes, filled by TMA (128-byte swizzle: its 16-byte
+// reads fall on distinct banks), so that 24 KB a warp are on their way however
+// long a step takes; nothing is shared between the warps before the end.
 //  S = Q K^T   m16n8k16, the rows as M (NR = 8 leaves half of it zero).  The
 //              order of the summed dimension is free as long as both sides
 //              agree, so a lane's 16-byte piece of a key (16 dimensions) is
@@ -35,40 +40,74 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
 //              permutes of two tokens' pieces before the conversion.
 // Each e4m3 is converted to f16 (exact); the key's factor goes to the score,
 // the value's to the weight's exponent.
-constexpr int kRowsThreads = 128, kRowsWarps = 4;
+constexpr int kRowsThreads = 128, kRowsWarps = 4, kRowsStages = 3;
+constexpr int kErrRowsWait = 503;
 
 template <int DP, int NR>
 struct RowsShape {
   static constexpr bool kQShared = NR * DP > 16 * 128;  // 64 registers of queries are too many beside 128 of sums
   static constexpr int kQPitch = DP + 8;                // f16 elements: 16-byte reads of eight rows on distinct banks
-  static constexpr size_t smem = (size_t)kRowsWarps * NR * (DP + 2) * 4;
+  static constexpr int kBox = DP == 64 ? 64 : 128, kBoxes = DP / kBox;
+  static constexpr uint32_t kStage = 2 * 16 * DP;  // a step's codes, keys then values
+  static constexpr size_t kRing = (size_t)kRowsWarps * kRowsStages * kStage;
+  static constexpr size_t kEnd = (size_t)kRowsWarps * NR * (DP + 2) * 4;  // the warps' results, over the ring
+  static constexpr size_t kQueries = (size_t)NR * kQPitch * 2;
+  static constexpr size_t smem = 1023 + (kRing > kEnd ? kRing : kEnd) + kQueries;
 };
 
 template <int DP, int NR>
-__global__ void __launch_bounds__(kRowsThreads, 2) tree_attn_rows_kernel(const __grid_constant__ TreeArgs a) {
-  pdl_enter();
+__global__ void __launch_bounds__(kRowsThreads, 2)
+    tree_attn_rows_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap k_map,
+                          const __grid_constant__ CUtensorMap v_map) {
   using Sh = RowsShape<DP, NR>;
   constexpr int kPieces = DP / 64, kVPieces = DP >= 128 ? DP / 128 : 1, kVBytes = DP >= 128 ? 16 : 8;
   constexpr int kMT = DP / 16, kNT = NR / 8;
-  extern __shared__ __align__(16) float sm[];  // queries (f16) first, then the warps' results
+  extern __shared__ uint8_t raw_sm[];
+  uint8_t *const ring = raw_sm + (-smem_u32(raw_sm) & 1023);  // the swizzle goes by the address
+  float *const sm = reinterpret_cast<float *>(ring);  // at the end: the warps' results
+  __half *const qs = reinterpret_cast<__half *>(ring + (Sh::kRing > Sh::kEnd ? Sh::kRing : Sh::kEnd));
+  __shared__ uint64_t full[kRowsWarps][kRowsStages];
+  __shared__ int abort_s;
   __shared__ float m_s[kRowsWarps][NR], l_s[kRowsWarps][NR];
   __shared__ float fac_s[NR];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, c = lane & 3;
-  const int rows = a.nodes * a.group, tiles = (rows + NR - 1) / NR;
-  const int item = blockIdx.y, tile = item % tiles, bk = item / tiles;
-  const int b = bk / a.kv_heads, kvh = bk % a.kv_heads, D = a.head_dim;
+  const int rows = a.nodes * a.group;
+  const int item = blockIdx.y, b = item / a.kv_heads, kvh = item % a.kv_heads, D = a.head_dim;
+  if (lane == 0) {
+    for (int i = 0; i < kRowsStages; ++i) mbar_init(&full[w][i], 1);
+    if (w == 0) abort_s = 0;
+    fence_barrier_init();
+  }
+  __syncwarp();
+  pdl_enter();
   const int pos = a.positions[b];
   const bool tree = a.parents != nullptr;
-  const int last = min(a.nodes - 1, (tile * NR + NR - 1) / a.group);
-  const int total = seen_rows(a, pos, last);
+  const int total = seen_rows(a, pos, a.nodes - 1);
   // this split's tokens, in whole steps
   const int steps = (total + 15) / 16, per = (steps + a.splits - 1) / a.splits;
   const int s0 = blockIdx.x * per, s1 = min(steps, s0 + per);
 
+  // the ring's first steps are on their way before anything else
+  const int first = s0 + w, boxes = (D + Sh::kBox - 1) / Sh::kBox;
+  uint8_t *const mine_ring = ring + (size_t)w * kRowsStages * Sh::kStage;
+  auto fetch = [&](int i) {  // the warp's i-th step, one lane
+    uint8_t *to = mine_ring + (i % kRowsStages) * Sh::kStage;
+    uint64_t *bar = &full[w][i % kRowsStages];
+    const int t0 = (first + i * kRowsWarps) * 16;
+    mbar_arrive_expect_tx(bar, 2u * boxes * (16 * Sh::kBox));
+    for (int x = 0; x < boxes; ++x) {
+      tma_load_4d(to + x * (16 * Sh::kBox), &k_map, x * Sh::kBox, kvh, t0, b, bar);
+      tma_load_4d(to + Sh::kStage / 2 + x * (16 * Sh::kBox), &v_map, x * Sh::kBox, kvh, t0, b, bar);
+    }
+  };
+  const int count = first < s1 ? (s1 - first + kRowsWarps - 1) / kRowsWarps : 0;
+  if (lane == 0)
+    for (int i = 0; i < min(count, kRowsStages); ++i) fetch(i);
+  __syncwarp();
+
   // queries: a warp takes rows w, w + 4, ...; eight columns a lane
-  __half *qs = reinterpret_cast<__half *>(sm);
   for (int r = w; r < NR; r += kRowsWarps) {
-    const int row = tile * NR + r, n = row / a.group, h = kvh * a.group + row % a.group;
+    const int row = r, n = row / a.group, h = kvh * a.group + row % a.group;
     float x[8];
     float amax = 0.0f;
 #pragma unroll
@@ -97,7 +136,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) tree_attn_rows_kernel(const _
   float fac[kNT];
 #pragma unroll
   for (int i = 0; i < kNT; ++i) {
-    const int row = tile * NR + g + 8 * i;
+    const int row = g + 8 * i;
     sight[i] = sight_of(a, b, row < rows ? row / a.group : a.nodes, pos);
     fac[i] = fac_s[g + 8 * i];
   }
@@ -116,45 +155,10 @@ __global__ void __launch_bounds__(kRowsThreads, 2) tree_attn_rows_kernel(const _
         }
   }
 
-  const size_t pitch = (size_t)a.kv_heads * D;
-  const uint8_t *kc = a.k_codes + ((size_t)b * a.max_seq * a.kv_heads + kvh) * D;
-  const uint8_t *vc = a.v_codes + ((size_t)b * a.max_seq * a.kv_heads + kvh) * D;
   const uint8_t *ex = (lane < 16 ? a.k_exp : a.v_exp) + (size_t)b * a.max_seq * a.kv_heads + kvh;
-  uint4 kr[2][kPieces];
-  uint32_t vr[4][kVPieces][kVBytes / 4];
-  uint32_t xr = 0;
-  auto load_k = [&](int step) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int t = step * 16 + 8 * u + g;
-#pragma unroll
-      for (int p = 0; p < kPieces; ++p) {
-        const int d = 64 * p + 16 * c;
-        kr[u][p] = t < total && d < D ? __ldg(reinterpret_cast<const uint4 *>(kc + (size_t)t * pitch + d))
-                                      : make_uint4(0, 0, 0, 0);
-      }
-    }
+  auto load_exp = [&](int step) -> uint32_t {
     const int t = step * 16 + (lane & 15);
-    xr = t < total ? ex[(size_t)t * a.kv_heads] : 127;
-  };
-  auto load_v = [&](int step) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = step * 16 + 2 * c + (i & 1) + 8 * (i >> 1);
-#pragma unroll
-      for (int p = 0; p < kVPieces; ++p) {
-        const int d = 128 * p + kVBytes * g;
-        if constexpr (kVBytes == 16) {
-          const uint4 v = t < total && d < D ? __ldg(reinterpret_cast<const uint4 *>(vc + (size_t)t * pitch + d))
-                                             : make_uint4(0, 0, 0, 0);
-          vr[i][p][0] = v.x; vr[i][p][1] = v.y; vr[i][p][2] = v.z; vr[i][p][3] = v.w;
-        } else {
-          const uint2 v = t < total && d < D ? __ldg(reinterpret_cast<const uint2 *>(vc + (size_t)t * pitch + d))
-                                             : make_uint2(0, 0);
-          vr[i][p][0] = v.x; vr[i][p][1] = v.y;
-        }
-      }
-    }
+    return t < total ? ex[(size_t)t * a.kv_heads] : 127;
   };
 
   float acc[kMT][kNT][4];
@@ -170,12 +174,17 @@ __global__ void __launch_bounds__(kRowsThreads, 2) tree_attn_rows_kernel(const _
     m[i] = -INFINITY;
     l[i] = 0.0f;
   }
-  int step = s0 + w;
-  if (step < s1) {
-    load_k(step);
-    load_v(step);
-  }
-  for (; step < s1; step += kRowsWarps) {
+  uint32_t xr = count > 0 ? load_exp(first) : 127;
+  bool ok = true;
+  for (int i = 0; i < count; ++i) {
+    const int step = first + i * kRowsWarps;
+    const uint8_t *kst = mine_ring + (i % kRowsStages) * Sh::kStage, *vst = kst + Sh::kStage / 2;
+    if (ok) ok = mbar_wait(&full[w][i % kRowsStages], (i / kRowsStages) & 1, &abort_s);
+    if (!ok && a.error) {  // (a wait that ran out: the results are void, but the loop ends)
+      *(volatile int *)&abort_s = 1;
+      atomicCAS(a.error, 0, kErrRowsWait);
+    }
+    __syncwarp();
     // scores of 16 tokens: s[u] tokens 8 u + 2 c, 2 c + 1 of row g (and g + 8)
     float s[2][4];
 #pragma unroll
@@ -206,7 +215,10 @@ __global__ void __launch_bounds__(kRowsThreads, 2) tree_attn_rows_kernel(const _
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const uint32_t kw[4] = {kr[u][p].x, kr[u][p].y, kr[u][p].z, kr[u][p].w};
+        const int at = DP == 64 ? (8 * u + g) * 64 + ((c ^ ((g >> 1) & 3)) * 16)
+                                : (p >> 1) * 2048 + (8 * u + g) * 128 + (((4 * (p & 1) + c) ^ g) * 16);
+        const uint4 kv = *reinterpret_cast<const uint4 *>(kst + at);
+        const uint32_t kw[4] = {kv.x, kv.y, kv.z, kv.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           mma_f16(s[u], q0[2 * j], q1[2 * j], q0[2 * j + 1], q1[2 * j + 1], e4m3x2_to_f16x2((uint16_t)kw[j]),
@@ -216,7 +228,22 @@ __global__ void __launch_bounds__(kRowsThreads, 2) tree_attn_rows_kernel(const _
     const uint32_t xb = xr;
     const int t0 = step * 16;
     const bool open = t0 + 16 > pos;  // warp-uniform: the tree's rows, or the end
-    if (step + kRowsWarps < s1) load_k(step + kRowsWarps);
+    if (i + 1 < count) xr = load_exp(step + kRowsWarps);
+    uint32_t vr[4][kVPieces][kVBytes / 4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int row = 2 * c + (t & 1) + 8 * (t >> 1);
+#pragma unroll
+      for (int p = 0; p < kVPieces; ++p) {
+        if constexpr (kVBytes == 16) {
+          const uint4 v = *reinterpret_cast<const uint4 *>(vst + p * 2048 + row * 128 + ((g ^ (row & 7)) * 16));
+          vr[t][p][0] = v.x; vr[t][p][1] = v.y; vr[t][p][2] = v.z; vr[t][p][3] = v.w;
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2 *>(vst + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) * 16) + (g & 1) * 8);
+          vr[t][p][0] = v.x; vr[t][p][1] = v.y;
+        }
+      }
+    }
     uint32_t nan[4] = {0, 0, 0, 0};
     if (open) {  // a value vector that some row does not see must not reach it through 0 * NaN
 #pragma unroll
@@ -311,8 +338,15 @@ __global__ void __launch_bounds__(kRowsThreads, 2) tree_attn_rows_kernel(const _
                   e4m3x2_to_f16x2((uint16_t)z1), e4m3x2_to_f16x2((uint16_t)(z1 >> 16)), pb[i][0], pb[i][1]);
         }
       }
-    if (step + kRowsWarps < s1) load_v(step + kRowsWarps);
+    __syncwarp();  // the stage is read
+    if (lane == 0 && i + kRowsStages < count) fetch(i + kRowsStages);
+    __syncwarp();
   }
+  if (!ok)  // copies still in flight land before the block ends
+    for (int i = 0; i < kRowsStages; ++i) {
+      int never = 0;
+      for (uint32_t k = 0; k < 2; ++k) mbar_wait(&full[w][i], k, &never);
+    }
 
   // the warps' results meet: maxima, then sums over one maximum in warp order
 #pragma unroll
@@ -341,7 +375,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) tree_attn_rows_kernel(const _
         }
   __syncthreads();
   for (int r = w; r < NR; r += kRowsWarps) {
-    const int row = tile * NR + r;
+    const int row = r;
     if (row >= rows) break;
     float mt = -INFINITY, f[kRowsWarps], lt = 0.0f;
 #pragma unroll
@@ -442,15 +476,15 @@ Plan plan_for(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, size_
   p.rows_tile = rows <= 8 ? 8 : 16;
   p.items = batch * kv_heads;
   // two blocks an SM; at least 64 tokens a split (a step for each warp)
-  const size_t want = ((size_t)sm_count() * 2 + p.items - 1) / p.items;
+  const size_t want = std::max<size_t>(1, (size_t)sm_count() * 2 / p.items);  // one wave
   p.splits = (int)std::max<size_t>(1, std::min(want, (max_seq + 63) / 64));
   return p;
 }
 
 template <int DP, int NR>
 int run_rows(const TreeArgs &a, const Plan &p, cudaStream_t s) {
-  constexpr size_t smem = std::max(RowsShape<DP, NR>::smem, (size_t)NR * RowsShape<DP, NR>::kQPitch * 2);
-  if (smem > 40 * 1024) {
+  using Sh = RowsShape<DP, NR>;
+  {
     static std::mutex mu;
     static std::vector<int> done;
     int dev = 0;
@@ -458,12 +492,15 @@ int run_rows(const TreeArgs &a, const Plan &p, cudaStream_t s) {
     std::lock_guard<std::mutex> lock(mu);
     if (std::find(done.begin(), done.end(), dev) == done.end()) {
       FPB_CUDA_TRY(cudaFuncSetAttribute(tree_attn_rows_kernel<DP, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        (int)smem));
+                                        (int)Sh::smem));
       done.push_back(dev);
     }
   }
+  CUtensorMap k_map, v_map;
+  if (int st = encode_cache_u8(&k_map, a.k_codes, a.batch, a.max_seq, a.kv_heads, a.head_dim, Sh::kBox, 16)) return st;
+  if (int st = encode_cache_u8(&v_map, a.v_codes, a.batch, a.max_seq, a.kv_heads, a.head_dim, Sh::kBox, 16)) return st;
   cudaError_t e = launch_pdl(tree_attn_rows_kernel<DP, NR>, dim3((unsigned)p.splits, (unsigned)p.items), kRowsThreads,
-                             smem, s, a);
+                             Sh::smem, s, a, k_map, v_map);
   if (e != cudaSuccess) return cuda_fail(e, "tree_attn_rows_kernel");
   FPB_LAUNCH_CHECK("tree_attn_rows_kernel");
   return FPB_OK;
