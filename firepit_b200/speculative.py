@@ -24,28 +24,42 @@ from .gemv import ShapeError
 TREE_MAX_NODES = 64
 
 
-def _empty(stream, device, dtype, *shape):
+class _Torch:
+    """torch and what the calls need of it, looked up once (a decode step's
+    calls take a few microseconds each)."""
+
+    module = None
+
+    @classmethod
+    def load(cls):
+        import torch
+        cls.f32, cls.bf16, cls.i32, cls.u8 = torch.float32, torch.bfloat16, torch.int32, torch.uint8
+        cls.codes = {torch.float32: N.FPB_F32, torch.bfloat16: N.FPB_BF16}
+        cls.raw_stream = staticmethod(torch._C._cuda_getCurrentRawStream) if hasattr(
+            torch._C, "_cuda_getCurrentRawStream") else staticmethod(
+                lambda index: torch.cuda.current_stream(index).cuda_stream)
+        cls.module = torch
+
+
+def _empty(stream, like, dtype, *shape):
     """Memory of the stream that will write it: torch hands memory out in the
     order of the stream it was asked for on."""
-    import torch
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
+    torch = _Torch.module
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=like.device)):
+        return like.new_empty(shape, dtype=dtype)
 
 
-def _handle(stream, device) -> int:
-    import torch
-    return torch.cuda.current_stream(device).cuda_stream if stream is None else stream
+def _handle(stream, like) -> int:
+    return _Torch.raw_stream(like.get_device()) if stream is None else stream
 
 
 def _code(t) -> int:
-    import torch
-    if t.dtype == torch.float32:
-        return N.FPB_F32
-    if t.dtype == torch.bfloat16:
-        return N.FPB_BF16
-    raise ShapeError(f"expected float32 or bfloat16, got {t.dtype}")
+    code = _Torch.codes.get(t.dtype)
+    if code is None:
+        raise ShapeError(f"expected float32 or bfloat16, got {t.dtype}")
+    return code
 
 
 def _ptr(t):
@@ -66,8 +80,7 @@ def _rows(t, what: str, batch: int, nodes: int) -> int:
 
 
 def _ints(t, what: str, *shape):
-    import torch
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype is not _Torch.i32 or t.shape != shape or not t.is_contiguous():
         raise ShapeError(f"{what}: contiguous int32 {list(shape)} expected, got {t.dtype} {list(t.shape)}")
 
 
@@ -89,13 +102,15 @@ class Kv8Cache:
     v_exp: object
 
     def __post_init__(self):
-        import torch
+        if _Torch.module is None:
+            _Torch.load()
         k = self.k
         if k.dim() != 4 or k.shape[3] % 16 or not 0 < k.shape[3] <= 256:
             raise ShapeError(f"cache: [batch, max_seq, kv_heads, head_dim % 16 == 0 <= 256] expected, got "
                              f"{list(k.shape)}")
-        for t, shape in ((k, k.shape), (self.v, k.shape), (self.k_exp, k.shape[:3]), (self.v_exp, k.shape[:3])):
-            if t.dtype != torch.uint8 or t.shape != shape or not t.is_contiguous() or t.device != k.device:
+        u8, full = _Torch.u8, k.shape
+        for t, shape in ((k, full), (self.v, full), (self.k_exp, full[:3]), (self.v_exp, full[:3])):
+            if t.dtype is not u8 or t.shape != shape or not t.is_contiguous() or t.device != k.device:
                 raise ShapeError("cache: contiguous uint8 codes of one shape and exponents [batch, max_seq, kv_heads] "
                                  "on one device expected")
 
@@ -136,7 +151,7 @@ def kv8_append(cache: Kv8Cache, positions, k, v, q=None, parents=None, q_gamma=N
         if hk > 1 and t.stride(2) != d:
             raise ShapeError(f"kv8_append: {what}'s heads must be contiguous")
     for g in (q_gamma, k_gamma):
-        if g is not None and (tuple(g.shape) != (d,) or _code(g) != N.FPB_F32 or not g.is_contiguous()):
+        if g is not None and (g.shape != (d,) or _code(g) != N.FPB_F32 or not g.is_contiguous()):
             raise ShapeError(f"kv8_append: gammas [{d}] f32 expected")
     hq, q_pitch, q_head, out_code = 0, 0, 0, N.FPB_F32
     if q is not None:
@@ -146,8 +161,8 @@ def kv8_append(cache: Kv8Cache, positions, k, v, q=None, parents=None, q_gamma=N
         hq, q_pitch = q.shape[2], _rows(q, "q", b, n)
         q_head = q.stride(2) if hq > 1 else d
         if q_out is None:
-            q_out = _empty(stream, q.device, q.dtype, b, n, hq, d)
-        elif tuple(q_out.shape) != (b, n, hq, d) or not q_out.is_contiguous():
+            q_out = _empty(stream, q, q.dtype, b, n, hq, d)
+        elif q_out.shape != (b, n, hq, d) or not q_out.is_contiguous():
             raise ShapeError(f"kv8_append: q_out [{b}, {n}, {hq}, {d}] contiguous expected")
         out_code = _code(q_out)
     elif q_out is not None:
@@ -155,26 +170,24 @@ def kv8_append(cache: Kv8Cache, positions, k, v, q=None, parents=None, q_gamma=N
     N.call("fpb_kv8_append", _ptr(q), q_pitch, q_head, k.data_ptr(), _rows(k, "k", b, n), v.data_ptr(),
            _rows(v, "v", b, n), _code(k), _ptr(q_gamma), _ptr(k_gamma), positions.data_ptr(), _ptr(parents), b, n, hq,
            hk, d, rotary_dim, theta, eps, s, _ptr(q_out), out_code, cache.k.data_ptr(), cache.v.data_ptr(),
-           cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), _handle(stream, k.device))
+           cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), _handle(stream, k))
     return q_out
 
 
 def kv8_read(cache: Kv8Cache, begin, count: int, dtype=None, stream=None):
     """(k, v) [batch, count, kv_heads, head_dim] as the values that rows
     [begin, begin + count) stand for; begin: an int, or int32 [batch]."""
-    import torch
     b, s, hk, d = cache.shape
-    dtype = torch.float32 if dtype is None else dtype
+    dtype = _Torch.f32 if dtype is None else dtype
     begins = None
     if not isinstance(begin, int):
         _ints(begin, "begin", b)
         begins, begin = begin.data_ptr(), 0
     if count < 1 or begin < 0:
         raise ShapeError(f"kv8_read: rows [{begin}, +{count})")
-    k = _empty(stream, cache.k.device, dtype, b, count, hk, d)
-    v = _empty(stream, cache.k.device, dtype, b, count, hk, d)
+    k, v = _empty(stream, cache.k, dtype, 2, b, count, hk, d).unbind(0)
     N.call("fpb_kv8_read", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), b,
-           s, hk, d, begins, begin, count, k.data_ptr(), v.data_ptr(), _code(k), _handle(stream, cache.k.device))
+           s, hk, d, begins, begin, count, k.data_ptr(), v.data_ptr(), _code(k), _handle(stream, cache.k))
     return k, v
 
 
@@ -185,7 +198,7 @@ def kv8_keep(cache: Kv8Cache, positions, path, stream=None) -> None:
     _ints(positions, "positions", b)
     _ints(path, "path", b, path.shape[-1])
     N.call("fpb_kv8_keep", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), b, s,
-           hk, d, positions.data_ptr(), path.data_ptr(), path.shape[1], _handle(stream, cache.k.device))
+           hk, d, positions.data_ptr(), path.data_ptr(), path.shape[1], _handle(stream, cache.k))
 
 
 def tree_attention_workspace_bytes(cache: Kv8Cache, nodes: int, q_heads: int) -> int:
@@ -201,7 +214,6 @@ def tree_attention(q, cache: Kv8Cache, positions, parents=None, gate=None, scale
     q f32 or bf16, any row and head pitch; scale default 1 / sqrt(head_dim);
     ``workspace``: uint8 of ``tree_attention_workspace_bytes`` (allocated where
     None)."""
-    import torch
     b, s, hk, d = cache.shape
     if q.dim() != 4 or q.shape[0] != b or q.shape[3] != d or q.shape[2] % hk:
         raise ShapeError(f"tree_attention: q [{b}, nodes, a multiple of {hk}, {d}] expected, got {list(q.shape)}")
@@ -210,20 +222,20 @@ def tree_attention(q, cache: Kv8Cache, positions, parents=None, gate=None, scale
     _ints(positions, "positions", b)
     gate_pitch = gate_head = 0
     if gate is not None:
-        if gate.shape != q.shape or gate.dtype != torch.float32:
+        if gate.shape != q.shape or gate.dtype is not _Torch.f32:
             raise ShapeError(f"tree_attention: gate f32 {list(q.shape)} expected")
         gate_pitch, gate_head = _rows(gate, "gate", b, n), gate.stride(2) if hq > 1 else d
     if out is None:
-        out = _empty(stream, q.device, torch.bfloat16, b, n, hq, d)
-    elif out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
+        out = _empty(stream, q, _Torch.bf16, b, n, hq, d)
+    elif out.shape != q.shape or out.dtype is not _Torch.bf16 or not out.is_contiguous():
         raise ShapeError("tree_attention: out bf16 of q's shape, contiguous, expected")
     if workspace is None:
-        workspace = _empty(stream, q.device, torch.uint8, tree_attention_workspace_bytes(cache, n, hq))
+        workspace = _empty(stream, q, _Torch.u8, N.lib.fpb_tree_attn_workspace_bytes(b, n, hq, hk, d, s))
     N.call("fpb_tree_attn", q.data_ptr(), _code(q), _rows(q, "q", b, n), q.stride(2) if hq > 1 else d,
            cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), positions.data_ptr(),
            _ptr(parents), _ptr(gate), gate_pitch, gate_head, b, n, hq, hk, d, s,
            1.0 / math.sqrt(d) if scale is None else scale, workspace.data_ptr(), workspace.numel(), out.data_ptr(),
-           _handle(stream, q.device))
+           _handle(stream, q))
     return out
 
 
@@ -236,7 +248,8 @@ def tree_verify(logits, tokens, parents=None, temperature: float = 0.0, accept=N
     variates decide, and draft [batch, nodes, vocab] f32 (None: certain drafts)
     holds the probabilities that each node's children were drawn from.  Emitted
     tokens are then distributed as the target's."""
-    import torch
+    if _Torch.module is None:
+        _Torch.load()
     if logits.dim() != 3:
         raise ShapeError(f"tree_verify: logits [batch, nodes, vocab] expected, got {list(logits.shape)}")
     b, n, vocab = logits.shape
@@ -248,22 +261,22 @@ def tree_verify(logits, tokens, parents=None, temperature: float = 0.0, accept=N
     if temperature != 0.0:
         if accept is None or noise is None:
             raise ShapeError("tree_verify: a temperature above 0 needs accept and noise")
-        if accept.dtype != torch.float32 or tuple(accept.shape) != (b, n) or not accept.is_contiguous():
+        if accept.dtype is not _Torch.f32 or accept.shape != (b, n) or not accept.is_contiguous():
             raise ShapeError(f"tree_verify: accept f32 [{b}, {n}] expected")
-        if noise.dtype != torch.float32 or tuple(noise.shape) != (b, vocab) or (vocab > 1 and noise.stride(1) != 1):
+        if noise.dtype is not _Torch.f32 or noise.shape != (b, vocab) or (vocab > 1 and noise.stride(1) != 1):
             raise ShapeError(f"tree_verify: noise f32 [{b}, {vocab}] expected")
         noise_pitch = noise.stride(0) if b > 1 else vocab
         if draft is not None:
-            if draft.dtype != torch.float32 or draft.shape != logits.shape:
+            if draft.dtype is not _Torch.f32 or draft.shape != logits.shape:
                 raise ShapeError(f"tree_verify: draft f32 {list(logits.shape)} expected")
             draft_pitch = _pitch(draft, "draft")
     else:
         accept = noise = draft = None
-    words = _empty(stream, logits.device, torch.int32, b * (n + 2))
-    path, count, nxt = words[:b * n].view(b, n), words[b * n:b * (n + 1)], words[b * (n + 1):]
+    path = _empty(stream, logits, _Torch.i32, b, n)
+    count, nxt = _empty(stream, logits, _Torch.i32, 2, b).unbind(0)
     N.call("fpb_tree_verify", logits.data_ptr(), _code(logits), _pitch(logits, "logits"), _ptr(draft), draft_pitch,
            tokens.data_ptr(), _ptr(parents), _ptr(accept), _ptr(noise), noise_pitch, b, n, vocab, temperature,
-           path.data_ptr(), count.data_ptr(), nxt.data_ptr(), _handle(stream, logits.device))
+           path.data_ptr(), count.data_ptr(), nxt.data_ptr(), _handle(stream, logits))
     return path, count, nxt
 
 
