@@ -23,14 +23,15 @@ namespace {
 
 constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32, kVerifyCluster = 8;
 constexpr int kVerifyMaxSlice = 55296;  // f32 of shared memory a CTA: 216 KB
+constexpr int kBatch = 5;               // 16-byte loads a thread has under way
 
 struct VerifyArgs {
   const void *logits;
   const float *draft, *accept, *noise;
   const int32_t *tokens, *parents;
   long long logits_pitch, draft_pitch, noise_pitch;  // elements between rows
-  int nodes, vocab, slice;
-  float temperature;
+  int nodes, vocab, slice, vec;  // vec: every row and slice begins on 16 bytes
+  float scale_log2;  // log2(e) / temperature; 0: greedy
   int32_t *path, *count, *next;
   int *error;
 };
@@ -45,28 +46,88 @@ __device__ __forceinline__ int dsmem_load_int(const int *p, unsigned rank) {
   return __float_as_int(dsmem_load(reinterpret_cast<const float *>(p), rank));
 }
 
+__device__ __forceinline__ float pow2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Calls f(i, x[N]) for the N = 16 / sizeof(T) elements from i on, for all of
+// row[0, len), loads in batches; the tail, and rows that do not begin on 16
+// bytes, one element (f(i, x, 1)) at a time.
+template <typename T, typename F>
+__device__ __forceinline__ void for_row(const T *row, int len, bool vec, F f) {
+  constexpr int N = 16 / sizeof(T);
+  const int whole = vec ? len / N * N : 0;
+  for (int i0 = threadIdx.x * N; i0 < whole; i0 += kBatch * kVerifyThreads * N) {
+    uint4 v[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int i = i0 + k * kVerifyThreads * N;
+      v[k] = i < whole ? __ldg(reinterpret_cast<const uint4 *>(row + i)) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int i = i0 + k * kVerifyThreads * N;
+      if (i >= whole) break;
+      const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+      float x[N];
+      if constexpr (N == 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(w[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[2 * j] = __uint_as_float(w[j] << 16);
+          x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        }
+      }
+      f(i, x, N);
+    }
+  }
+  for (int i = whole + threadIdx.x; i < len; i += kVerifyThreads) {
+    const float x[1] = {static_cast<float>(row[i])};
+    f(i, x, 1);
+  }
+}
+
+// `bytes` from p on (a row's slice, both multiples of 16) to L2.
+__device__ __forceinline__ void to_l2(const void *p, int bytes) {
+  if (bytes > 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
+
 // Block (cluster of kVerifyCluster CTAs) per session: CTA `rank` owns the
 // vocabulary's slice [rank * slice, +slice) and keeps what is left of the
 // node's distribution there in shared memory, so that a refused child's pass
-// over the vocabulary does not go to memory for it again, and rows of nodes
-// off the path are never read.  Every CTA takes the same walk: the values a
-// decision needs come through distributed shared memory.
+// over the vocabulary does not go to memory for it again.  Every CTA takes the
+// same walk: the values a decision needs come through distributed shared
+// memory, one exchange a node.  The walk is bound by the latency of its steps:
+// the rows that the next step may want (the children's logits, the node's
+// draft, the noise) are sent to L2 while the node's own is worked on.
 template <typename T>
 __global__ void __launch_bounds__(kVerifyThreads) tree_verify_kernel(const __grid_constant__ VerifyArgs a) {
   pdl_enter();
-  extern __shared__ float r[];  // [slice]: exp(l / T - max), or what is left of it
+  extern __shared__ __align__(16) float r[];  // [slice]: exp(l / T - the slice's maximum), or what is left of it
   __shared__ int par[kTreeMaxNodes], tok[kTreeMaxNodes], refused[kTreeMaxNodes];
-  __shared__ float acc[kTreeMaxNodes], red[kVerifyWarps], out_v[2];
+  __shared__ float acc[kTreeMaxNodes], q_tok[kTreeMaxNodes], red[kVerifyWarps], red2[kVerifyWarps];
+  __shared__ float out_v[2], out_s[2], scale_s[kVerifyCluster];
   __shared__ int red_i[kVerifyWarps], out_i[2];
   const unsigned rank = cluster_ctarank(), ctas = cluster_nctarank();
   const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int v0 = (int)rank * a.slice, len = max(0, min(a.vocab - v0, a.slice));
+  const bool greedy = a.scale_log2 == 0.0f;
+  auto logits_of = [&](int n) { return static_cast<const T *>(a.logits) + ((size_t)b * a.nodes + n) * a.logits_pitch + v0; };
+  const float *noise = greedy ? nullptr : a.noise + (size_t)b * a.noise_pitch + v0;
+  const int l_bytes = a.vec ? len * (int)sizeof(T) / 16 * 16 : 0, f_bytes = a.vec ? len / 4 * 16 : 0;
   for (int i = tid; i < a.nodes; i += kVerifyThreads) {
-    par[i] = a.parents ? a.parents[(size_t)b * a.nodes + i] : i - 1;
-    tok[i] = a.tokens[(size_t)b * a.nodes + i];
+    const int p = a.parents ? a.parents[(size_t)b * a.nodes + i] : i - 1, x = a.tokens[(size_t)b * a.nodes + i];
+    par[i] = p;
+    tok[i] = x;
     acc[i] = a.accept ? a.accept[(size_t)b * a.nodes + i] : 0.0f;
+    q_tok[i] = a.draft && p >= 0 && p < i && x >= 0 && x < a.vocab
+                   ? a.draft[((size_t)b * a.nodes + p) * a.draft_pitch + x] : 1.0f;
     if (rank == 0) a.path[(size_t)b * a.nodes + i] = -1;
-    if (rank == 0 && a.error && i > 0 && par[i] >= i) atomicCAS(a.error, 0, kErrParent);
+    if (rank == 0 && a.error && i > 0 && p >= i) atomicCAS(a.error, 0, kErrParent);
   }
   __syncthreads();
   if (par[0] != -1) {  // no tree in this session
@@ -76,27 +137,19 @@ __global__ void __launch_bounds__(kVerifyThreads) tree_verify_kernel(const __gri
     }
     return;
   }
-  int flip = 0;
-  // Sum, or best, over the cluster; the slots alternate, so that one round's
-  // reads may overlap the next round's write.
-  auto cluster_sum = [&](float v) {
+  if (tid == 0 && !greedy) to_l2(noise, f_bytes);
+  int flip = 0;  // the slots alternate, so that one round's reads may overlap the next round's write
+  auto block_sum = [&](float v) {  // of the block, for thread 0
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane == 0) red2[warp] = v;
     __syncthreads();
-    if (lane == 0) red[warp] = v;
-    __syncthreads();
-    if (tid == 0) {
-      float t = 0.0f;
-      for (int w = 0; w < kVerifyWarps; ++w) t += red[w];
-      out_v[flip] = t;
-    }
-    cluster_sync();
     float t = 0.0f;
-    for (unsigned c = 0; c < ctas; ++c) t += dsmem_load(&out_v[flip], c);
-    flip ^= 1;
+    if (tid == 0)
+      for (int w = 0; w < kVerifyWarps; ++w) t += red2[w];
     return t;
   };
-  auto cluster_best = [&](Best x) {
+  auto block_best = [&](Best x) {  // of the block, for every thread
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       Best y{__shfl_xor_sync(0xffffffffu, x.v, o), __shfl_xor_sync(0xffffffffu, x.i, o)};
@@ -108,46 +161,63 @@ __global__ void __launch_bounds__(kVerifyThreads) tree_verify_kernel(const __gri
       red_i[warp] = x.i;
     }
     __syncthreads();
-    if (tid == 0) {
-      for (int w = 1; w < kVerifyWarps; ++w) x = better(x, Best{red[w], red_i[w]});
-      out_v[flip] = x.v;
-      out_i[flip] = x.i;
-    }
-    cluster_sync();
-    Best t{-INFINITY, 0x7fffffff};
-    for (unsigned c = 0; c < ctas; ++c)
-      t = better(t, Best{dsmem_load(&out_v[flip], c), dsmem_load_int(&out_i[flip], c)});
-    flip ^= 1;
-    return t;
+    x = Best{red[0], red_i[0]};
+    for (int w = 1; w < kVerifyWarps; ++w) x = better(x, Best{red[w], red_i[w]});
+    return x;
   };
-  const bool greedy = a.temperature == 0.0f;
   int node = 0, taken = 0, next = 0;
   while (true) {
     if (rank == 0 && tid == 0) a.path[(size_t)b * a.nodes + taken] = node;
     ++taken;
-    // the node's row: maximum (of finite logits), then exponentials and their sum
-    const T *row = static_cast<const T *>(a.logits) + ((size_t)b * a.nodes + node) * a.logits_pitch + v0;
-    Best top{-INFINITY, 0x7fffffff};
-    for (int i = tid; i < len; i += kVerifyThreads) {
-      const float l = static_cast<float>(row[i]);
-      const float x = isfinite(l) ? l : -INFINITY;
-      if (!greedy) r[i] = x / a.temperature;
-      if (x > top.v) top = Best{x, v0 + i};
+    if (a.vec && warp == 0) {
+      for (int c = node + 1 + lane; c < a.nodes; c += 32)
+        if (par[c] == node) to_l2(logits_of(c), l_bytes);
+      if (lane == 0 && a.draft) to_l2(a.draft + ((size_t)b * a.nodes + node) * a.draft_pitch + v0, f_bytes);
     }
-    top = cluster_best(top);
-    float left = 0.0f;
+    // the slice's maximum (of finite logits), then exponentials by it and their sum
+    Best top{-INFINITY, 0x7fffffff};
+    for_row(logits_of(node), len, a.vec, [&](int i, const float *x, int n) {
+      for (int k = 0; k < n; ++k) {
+        const float y = isfinite(x[k]) ? x[k] : -INFINITY;
+        if (!greedy) r[i + k] = y;
+        if (y > top.v) top = Best{y, v0 + i + k};
+      }
+    });
+    top = block_best(top);
+    float s = 0.0f;
     if (!greedy) {
-      const float m = top.v / a.temperature;
-      float s = 0.0f;
+#pragma unroll 4
       for (int i = tid; i < len; i += kVerifyThreads) {
-        const float e = r[i] == -INFINITY ? 0.0f : expf(r[i] - m);
+        const float y = r[i], e = y == -INFINITY ? 0.0f : pow2((y - top.v) * a.scale_log2);
         r[i] = e;
         s += e;
       }
-      left = cluster_sum(s);
+      s = block_sum(s);
     }
+    if (tid == 0) {
+      out_v[flip] = top.v;
+      out_i[flip] = top.i;
+      out_s[flip] = s;
+    }
+    cluster_sync();
+    // the slices' factors to one maximum, and the whole sum
+    float left = 0.0f;
+    Best all{-INFINITY, 0x7fffffff};
+    for (unsigned c = 0; c < ctas; ++c)
+      all = better(all, Best{dsmem_load(&out_v[flip], c), dsmem_load_int(&out_i[flip], c)});
+    if (!greedy) {
+      for (unsigned c = 0; c < ctas; ++c) {
+        const float mc = dsmem_load(&out_v[flip], c);
+        const float f = mc == -INFINITY ? 0.0f : pow2((mc - all.v) * a.scale_log2);
+        left = fmaf(dsmem_load(&out_s[flip], c), f, left);
+        if (tid == 0) scale_s[c] = f;
+      }
+      __syncthreads();
+    }
+    flip ^= 1;
+    float own = greedy ? 0.0f : scale_s[rank];  // of this slice's r
     int child = -1, rejected = 0;
-    const float *q = a.draft ? a.draft + ((size_t)b * a.nodes + node) * a.draft_pitch : nullptr;
+    const float *q = a.draft ? a.draft + ((size_t)b * a.nodes + node) * a.draft_pitch + v0 : nullptr;
     for (int c = node + 1; c < a.nodes; ++c) {
       if (par[c] != node) continue;
       const int x = tok[c];
@@ -156,28 +226,47 @@ __global__ void __launch_bounds__(kVerifyThreads) tree_verify_kernel(const __gri
         continue;
       }
       if (greedy) {
-        if (x == top.i) {
+        if (x == all.i) {
           child = c;
           break;
         }
         continue;
       }
-      float rx = dsmem_load(&r[x % a.slice], (unsigned)(x / a.slice));
+      float rx = fmaxf(dsmem_load(&r[x % a.slice], (unsigned)(x / a.slice)), 0.0f) * scale_s[x / a.slice];
       if (q) {
-        if (acc[c] * q[x] * left < rx) {
+        if (acc[c] * q_tok[c] * left < rx) {
           child = c;
           break;
         }
         cluster_sync();  // every CTA has read rx
-        const float inv = 1.0f / left;
-        float s = 0.0f;
-        for (int i = tid; i < len; i += kVerifyThreads) s += fmaxf(r[i] * inv - q[v0 + i], 0.0f);
-        s = cluster_sum(s);
-        if (s > 0.0f) {  // else the draft covers all that was left: it stays
-          for (int i = tid; i < len; i += kVerifyThreads) r[i] = fmaxf(r[i] * inv - q[v0 + i], 0.0f);
-          left = s;
-          cluster_sync();  // the new values are there for the next child
+        // What is left over, with its sign: whoever reads r takes it as at
+        // least 0, and what it was can be had back.
+        const float inv = own / left;
+        float z = 0.0f;
+        for_row(q, len, a.vec, [&](int i, const float *y, int n) {
+          for (int k = 0; k < n; ++k) {
+            const float d = fmaf(fmaxf(r[i + k], 0.0f), inv, -y[k]);
+            r[i + k] = d;
+            z += fmaxf(d, 0.0f);
+          }
+        });
+        z = block_sum(z);
+        if (tid == 0) out_s[flip] = z;
+        cluster_sync();  // also: the new values are there for the next child
+        z = 0.0f;
+        for (unsigned k = 0; k < ctas; ++k) z += dsmem_load(&out_s[flip], k);
+        flip ^= 1;
+        left = z;
+        if (!(z > 0.0f)) {  // the draft covers all that was left: it stays
+          for_row(q, len, a.vec, [&](int i, const float *y, int n) {
+            for (int k = 0; k < n; ++k) r[i + k] += y[k];
+          });
+          left = 1.0f;
+          cluster_sync();
         }
+        own = 1.0f;
+        if (tid < (int)ctas) scale_s[tid] = 1.0f;
+        __syncthreads();
       } else {
         for (int j = 0; j < rejected; ++j)
           if (refused[j] == x) rx = 0.0f;
@@ -198,7 +287,7 @@ __global__ void __launch_bounds__(kVerifyThreads) tree_verify_kernel(const __gri
       continue;
     }
     if (greedy) {
-      next = top.i == 0x7fffffff ? 0 : top.i;
+      next = all.i == 0x7fffffff ? 0 : all.i;
       break;
     }
     cluster_sync();
@@ -206,12 +295,21 @@ __global__ void __launch_bounds__(kVerifyThreads) tree_verify_kernel(const __gri
       if (refused[j] >= v0 && refused[j] < v0 + len) r[refused[j] - v0] = 0.0f;
     __syncthreads();
     Best pick{-1.0f, 0x7fffffff};
-    const float *e = a.noise + (size_t)b * a.noise_pitch + v0;
-    for (int i = tid; i < len; i += kVerifyThreads) {
-      const float w = r[i] / e[i];
-      if (w > pick.v) pick = Best{w, v0 + i};
+    for_row(noise, len, a.vec, [&](int i, const float *e, int n) {
+      for (int k = 0; k < n; ++k) {
+        const float w = fmaxf(r[i + k], 0.0f) * own / e[k];
+        if (w > pick.v) pick = Best{w, v0 + i + k};
+      }
+    });
+    pick = block_best(pick);
+    if (tid == 0) {
+      out_v[flip] = pick.v;
+      out_i[flip] = pick.i;
     }
-    pick = cluster_best(pick);
+    cluster_sync();
+    pick = Best{-1.0f, 0x7fffffff};
+    for (unsigned c = 0; c < ctas; ++c)
+      pick = better(pick, Best{dsmem_load(&out_v[flip], c), dsmem_load_int(&out_i[flip], c)});
     next = pick.i == 0x7fffffff ? 0 : pick.i;
     break;
   }
@@ -282,11 +380,15 @@ extern "C" int fpb_tree_verify(const void *logits, int logits_dtype, size_t logi
   a.nodes = (int)nodes;
   a.vocab = (int)vocab;
   a.slice = (int)((vocab + kVerifyCluster - 1) / kVerifyCluster + 7) / 8 * 8;
-  a.temperature = temperature;
+  a.scale_log2 = greedy ? 0.0f : (float)(1.4426950408889634 / (double)temperature);
   a.path = path;
   a.count = count;
   a.next = next;
   a.error = device_error_ptr();
+  const size_t el = logits_dtype == FPB_F32 ? 4 : 2;
+  auto lies = [](const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && bytes % 16 == 0; };
+  a.vec = lies(logits, logits_pitch * el) && (greedy || lies(noise, noise_pitch * 4)) &&
+          (!a.draft || lies(draft, draft_pitch * 4));
   const size_t smem = greedy ? 0 : (size_t)a.slice * sizeof(float);
   return logits_dtype == FPB_F32 ? run_verify<float>(a, batch, smem, as_stream(stream))
                                  : run_verify<__nv_bfloat16>(a, batch, smem, as_stream(stream));

@@ -816,7 +816,8 @@ int fpb_tree_attn(const void *q, int q_dtype, size_t q_pitch, size_t q_head_pitc
  * Writes path [batch, nodes] (the accepted nodes, 0 first, then -1), count
  * [batch] (their number) and next [batch] (the token after them); a session
  * with no tree: count 0, next -1.  nodes <= 64, vocab <= 442368
- * (FPB_ERR_UNSUPPORTED above).  One launch; rows off the path are not read. */
+ * (FPB_ERR_UNSUPPORTED above).  One launch; of the tree's rows only the path's and
+ * its nodes' children's are touched. */
 int fpb_tree_verify(const void *logits, int logits_dtype, size_t logits_pitch, const float *draft, size_t draft_pitch,
                     const int32_t *tokens, const int32_t *parents, const float *accept, const float *noise,
                     size_t noise_pitch, size_t batch, size_t nodes, size_t vocab, float temperature, int32_t *path,
