@@ -24,6 +24,7 @@ namespace {
 constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32, kVerifyCluster = 8;
 constexpr int kVerifyMaxSlice = 55296;  // f32 of shared memory a CTA: 216 KB
 constexpr int kBatch = 5;               // 16-byte loads a thread has under way
+constexpr int kHold = 40;               // logits a thread keeps in registers between a slice's maximum and its powers
 
 struct VerifyArgs {
   const void *logits;
@@ -42,8 +43,26 @@ struct Best {
 };
 __device__ __forceinline__ Best better(Best a, Best b) { return b.v > a.v || (b.v == a.v && b.i < a.i) ? b : a; }
 
-__device__ __forceinline__ int dsmem_load_int(const int *p, unsigned rank) {
-  return __float_as_int(dsmem_load(reinterpret_cast<const float *>(p), rank));
+// Stores v at this CTA's shared-memory address p, in cluster CTA `rank`.
+__device__ __forceinline__ void dsmem_store(float *p, unsigned rank, float v) {
+  unsigned local = (unsigned)__cvta_generic_to_shared(p), remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
+}
+
+// Over the cluster, each lane holding CTA lane % 8's value (every lane gets the
+// same bits: the pairs are added alike everywhere).
+static_assert(kVerifyCluster == 8);
+__device__ __forceinline__ float over_ctas_sum(float v) {
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ Best over_ctas_best(Best x) {
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1)
+    x = better(x, Best{__shfl_xor_sync(0xffffffffu, x.v, o), __shfl_xor_sync(0xffffffffu, x.i, o)});
+  return x;
 }
 
 __device__ __forceinline__ float pow2(float x) {
@@ -52,11 +71,12 @@ __device__ __forceinline__ float pow2(float x) {
   return y;
 }
 
-// Calls f(i, x[N]) for the N = 16 / sizeof(T) elements from i on, for all of
-// row[0, len), loads in batches; the tail, and rows that do not begin on 16
-// bytes, one element (f(i, x, 1)) at a time.
-template <typename T, typename F>
-__device__ __forceinline__ void for_row(const T *row, int len, bool vec, F f) {
+// Calls f(x, r) for every element x of row[0, len) with its r (read before and
+// written back after where KEEP): loads in batches, shared memory 16 bytes at a
+// time; the tail, and rows that do not begin on 16 bytes, element by element.
+// The element's index is passed third.
+template <bool KEEP, typename T, typename F>
+__device__ __forceinline__ void for_row(const T *row, int len, bool vec, float *r, F f) {
   constexpr int N = 16 / sizeof(T);
   const int whole = vec ? len / N * N : 0;
   for (int i0 = threadIdx.x * N; i0 < whole; i0 += kBatch * kVerifyThreads * N) {
@@ -82,12 +102,22 @@ __device__ __forceinline__ void for_row(const T *row, int len, bool vec, F f) {
           x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
         }
       }
-      f(i, x, N);
+#pragma unroll
+      for (int j = 0; j < N; j += 4) {
+        float4 *at = reinterpret_cast<float4 *>(r + i + j);
+        float4 y = r ? *at : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        f(x[j], y.x, i + j);
+        f(x[j + 1], y.y, i + j + 1);
+        f(x[j + 2], y.z, i + j + 2);
+        f(x[j + 3], y.w, i + j + 3);
+        if (KEEP && r) *at = y;
+      }
     }
   }
   for (int i = whole + threadIdx.x; i < len; i += kVerifyThreads) {
-    const float x[1] = {static_cast<float>(row[i])};
-    f(i, x, 1);
+    float y = r ? r[i] : 0.0f;
+    f(static_cast<float>(row[i]), y, i);
+    if (KEEP && r) r[i] = y;
   }
 }
 
@@ -100,19 +130,23 @@ __device__ __forceinline__ void to_l2(const void *p, int bytes) {
 // vocabulary's slice [rank * slice, +slice) and keeps what is left of the
 // node's distribution there in shared memory, so that a refused child's pass
 // over the vocabulary does not go to memory for it again.  Every CTA takes the
-// same walk: the values a decision needs come through distributed shared
-// memory, one exchange a node.  The walk is bound by the latency of its steps:
-// the rows that the next step may want (the children's logits, the node's
-// draft, the noise) are sent to L2 while the node's own is worked on.
+// same walk: each pushes what a decision needs (its slice's maximum and sum,
+// the children's weights that it owns) into every CTA's shared memory, and one
+// cluster barrier a step makes it known.  The walk is bound by the latency of
+// its steps: the rows that the next step may want (the children's logits, the
+// node's draft, the noise) are sent to L2 while the node's own is worked on.
 template <typename T>
-__global__ void __launch_bounds__(kVerifyThreads) tree_verify_kernel(const __grid_constant__ VerifyArgs a) {
+__global__ void __launch_bounds__(kVerifyThreads, 1) tree_verify_kernel(const __grid_constant__ VerifyArgs a) {
   pdl_enter();
-  extern __shared__ __align__(16) float r[];  // [slice]: exp(l / T - the slice's maximum), or what is left of it
+  extern __shared__ __align__(16) float r[];  // [slice]: 2^((l - slice's maximum) scale), or what is left of it
   __shared__ int par[kTreeMaxNodes], tok[kTreeMaxNodes], refused[kTreeMaxNodes];
   __shared__ float acc[kTreeMaxNodes], q_tok[kTreeMaxNodes], red[kVerifyWarps], red2[kVerifyWarps];
-  __shared__ float out_v[2], out_s[2], scale_s[kVerifyCluster];
-  __shared__ int red_i[kVerifyWarps], out_i[2];
-  const unsigned rank = cluster_ctarank(), ctas = cluster_nctarank();
+  __shared__ int red_i[kVerifyWarps];
+  // what the CTAs tell one another; the halves alternate, so that one step's
+  // reads may overlap the next one's stores
+  __shared__ float got_v[2][kVerifyCluster], got_i[2][kVerifyCluster], got_s[2][kVerifyCluster],
+      got_r[2][kTreeMaxNodes], scale_s[kVerifyCluster];
+  const unsigned rank = cluster_ctarank(), peer = threadIdx.x % kVerifyCluster;
   const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int v0 = (int)rank * a.slice, len = max(0, min(a.vocab - v0, a.slice));
   const bool greedy = a.scale_log2 == 0.0f;
@@ -137,34 +171,52 @@ __global__ void __launch_bounds__(kVerifyThreads) tree_verify_kernel(const __gri
     }
     return;
   }
+  cluster_sync();  // every CTA of the cluster runs: its shared memory may be stored to
   if (tid == 0 && !greedy) to_l2(noise, f_bytes);
-  int flip = 0;  // the slots alternate, so that one round's reads may overlap the next round's write
-  auto block_sum = [&](float v) {  // of the block, for thread 0
+  int flip = 0;
+  auto block_sum = [&](float v) {  // of the block, for every thread; all threads meet
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
     if (lane == 0) red2[warp] = v;
     __syncthreads();
-    float t = 0.0f;
-    if (tid == 0)
-      for (int w = 0; w < kVerifyWarps; ++w) t += red2[w];
+    float t = red2[lane % kVerifyWarps];
+#pragma unroll
+    for (int o = kVerifyWarps / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     return t;
   };
-  auto block_best = [&](Best x) {  // of the block, for every thread
+  auto block_best = [&](Best x) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      Best y{__shfl_xor_sync(0xffffffffu, x.v, o), __shfl_xor_sync(0xffffffffu, x.i, o)};
-      x = better(x, y);
-    }
-    __syncthreads();
+    for (int o = 16; o > 0; o >>= 1)
+      x = better(x, Best{__shfl_xor_sync(0xffffffffu, x.v, o), __shfl_xor_sync(0xffffffffu, x.i, o)});
     if (lane == 0) {
       red[warp] = x.v;
       red_i[warp] = x.i;
     }
     __syncthreads();
-    x = Best{red[0], red_i[0]};
-    for (int w = 1; w < kVerifyWarps; ++w) x = better(x, Best{red[w], red_i[w]});
+    x = Best{red[lane % kVerifyWarps], red_i[lane % kVerifyWarps]};
+#pragma unroll
+    for (int o = kVerifyWarps / 2; o > 0; o >>= 1)
+      x = better(x, Best{__shfl_xor_sync(0xffffffffu, x.v, o), __shfl_xor_sync(0xffffffffu, x.i, o)});
     return x;
   };
+  // To every CTA: this slice's maximum and sum, and of the children of `node`
+  // past `from` the weights that lie here (thread (child, peer); r complete).
+  auto tell = [&](int node, int from, Best top, float s) {
+    if (tid < kVerifyCluster) {
+      dsmem_store(&got_v[flip][rank], peer, top.v);
+      dsmem_store(&got_i[flip][rank], peer, __int_as_float(top.i));
+      dsmem_store(&got_s[flip][rank], peer, s);
+    }
+    const int c = tid / kVerifyCluster;
+    if (!greedy && c > from && c < a.nodes && par[c] == node) {
+      const int x = tok[c] - v0;
+      if (x >= 0 && x < len) dsmem_store(&got_r[flip][c], peer, r[x]);
+    }
+    cluster_sync();
+    flip ^= 1;
+  };
+  static_assert(kTreeMaxNodes * kVerifyCluster <= kVerifyThreads);
   int node = 0, taken = 0, next = 0;
   while (true) {
     if (rank == 0 && tid == 0) a.path[(size_t)b * a.nodes + taken] = node;
@@ -174,47 +226,77 @@ __global__ void __launch_bounds__(kVerifyThreads) tree_verify_kernel(const __gri
         if (par[c] == node) to_l2(logits_of(c), l_bytes);
       if (lane == 0 && a.draft) to_l2(a.draft + ((size_t)b * a.nodes + node) * a.draft_pitch + v0, f_bytes);
     }
-    // the slice's maximum (of finite logits), then exponentials by it and their sum
+    // the slice's maximum (of finite logits), then powers by it and their sum
     Best top{-INFINITY, 0x7fffffff};
-    for_row(logits_of(node), len, a.vec, [&](int i, const float *x, int n) {
-      for (int k = 0; k < n; ++k) {
-        const float y = isfinite(x[k]) ? x[k] : -INFINITY;
-        if (!greedy) r[i + k] = y;
-        if (y > top.v) top = Best{y, v0 + i + k};
-      }
-    });
-    top = block_best(top);
     float s = 0.0f;
-    if (!greedy) {
-#pragma unroll 4
-      for (int i = tid; i < len; i += kVerifyThreads) {
-        const float y = r[i], e = y == -INFINITY ? 0.0f : pow2((y - top.v) * a.scale_log2);
-        r[i] = e;
-        s += e;
+    constexpr int N = 16 / sizeof(T), kLoads = kHold / N;
+    if (!greedy && a.vec && len % N == 0 && len <= kHold * kVerifyThreads) {  // the slice in registers between the two
+      const T *row = logits_of(node);
+      uint4 v[kLoads];
+      float m = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k) {
+        const int i = (k * kVerifyThreads + tid) * N;
+        // past the slice: NaN, which counts as -inf
+        v[k] = i < len ? __ldg(reinterpret_cast<const uint4 *>(row + i)) : make_uint4(~0u, ~0u, ~0u, ~0u);
+      }
+      auto value = [&](int k, int j) {
+        const uint32_t w = N == 4 ? (j == 0 ? v[k].x : j == 1 ? v[k].y : j == 2 ? v[k].z : v[k].w)
+                                  : (j < 2 ? v[k].x : j < 4 ? v[k].y : j < 6 ? v[k].z : v[k].w);
+        const float x = __uint_as_float(N == 4 ? w : j & 1 ? w & 0xffff0000u : w << 16);
+        return fabsf(x) <= 3.402823466e38f ? x : -INFINITY;
+      };
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k)
+#pragma unroll
+        for (int j = 0; j < N; ++j) m = fmaxf(m, value(k, j));
+      top = block_best(Best{m, 0});
+      const float bias = top.v == -INFINITY ? 0.0f : -top.v * a.scale_log2;
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k) {
+        const int i = (k * kVerifyThreads + tid) * N;
+        if (i >= len) break;
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+          float4 e;
+          e.x = pow2(fmaf(value(k, j), a.scale_log2, bias));
+          e.y = pow2(fmaf(value(k, j + 1), a.scale_log2, bias));
+          e.z = pow2(fmaf(value(k, j + 2), a.scale_log2, bias));
+          e.w = pow2(fmaf(value(k, j + 3), a.scale_log2, bias));
+          s += (e.x + e.y) + (e.z + e.w);
+          *reinterpret_cast<float4 *>(r + i + j) = e;
+        }
       }
       s = block_sum(s);
+    } else {
+      for_row<true>(logits_of(node), len, a.vec, greedy ? nullptr : r, [&](float x, float &y, int i) {
+        y = isfinite(x) ? x : -INFINITY;
+        if (y > top.v) top = Best{y, v0 + i};
+      });
+      top = block_best(top);
+      if (!greedy) {
+        const float bias = top.v == -INFINITY ? 0.0f : -top.v * a.scale_log2;
+#pragma unroll 4
+        for (int i = tid; i < len; i += kVerifyThreads) {
+          const float e = pow2(fmaf(r[i], a.scale_log2, bias));
+          r[i] = e;
+          s += e;
+        }
+        s = block_sum(s);
+      }
     }
-    if (tid == 0) {
-      out_v[flip] = top.v;
-      out_i[flip] = top.i;
-      out_s[flip] = s;
-    }
-    cluster_sync();
+    tell(node, node, top, s);
     // the slices' factors to one maximum, and the whole sum
     float left = 0.0f;
-    Best all{-INFINITY, 0x7fffffff};
-    for (unsigned c = 0; c < ctas; ++c)
-      all = better(all, Best{dsmem_load(&out_v[flip], c), dsmem_load_int(&out_i[flip], c)});
+    const float mc = got_v[flip ^ 1][peer];
+    const Best all = over_ctas_best(Best{mc, __float_as_int(got_i[flip ^ 1][peer])});
     if (!greedy) {
-      for (unsigned c = 0; c < ctas; ++c) {
-        const float mc = dsmem_load(&out_v[flip], c);
-        const float f = mc == -INFINITY ? 0.0f : pow2((mc - all.v) * a.scale_log2);
-        left = fmaf(dsmem_load(&out_s[flip], c), f, left);
-        if (tid == 0) scale_s[c] = f;
-      }
+      const float f = mc == -INFINITY ? 0.0f : pow2((mc - all.v) * a.scale_log2);
+      left = over_ctas_sum(got_s[flip ^ 1][peer] * f);
+      __syncthreads();  // the node before is done with the factors
+      if (tid < kVerifyCluster) scale_s[tid] = f;
       __syncthreads();
     }
-    flip ^= 1;
     float own = greedy ? 0.0f : scale_s[rank];  // of this slice's r
     int child = -1, rejected = 0;
     const float *q = a.draft ? a.draft + ((size_t)b * a.nodes + node) * a.draft_pitch + v0 : nullptr;
@@ -232,40 +314,32 @@ __global__ void __launch_bounds__(kVerifyThreads) tree_verify_kernel(const __gri
         }
         continue;
       }
-      float rx = fmaxf(dsmem_load(&r[x % a.slice], (unsigned)(x / a.slice)), 0.0f) * scale_s[x / a.slice];
+      float rx = fmaxf(got_r[flip ^ 1][c], 0.0f) * scale_s[x / a.slice];
       if (q) {
         if (acc[c] * q_tok[c] * left < rx) {
           child = c;
           break;
         }
-        cluster_sync();  // every CTA has read rx
         // What is left over, with its sign: whoever reads r takes it as at
         // least 0, and what it was can be had back.
         const float inv = own / left;
         float z = 0.0f;
-        for_row(q, len, a.vec, [&](int i, const float *y, int n) {
-          for (int k = 0; k < n; ++k) {
-            const float d = fmaf(fmaxf(r[i + k], 0.0f), inv, -y[k]);
-            r[i + k] = d;
-            z += fmaxf(d, 0.0f);
-          }
+        for_row<true>(q, len, a.vec, r, [&](float x, float &y, int) {
+          y = fmaf(fmaxf(y, 0.0f), inv, -x);
+          z += fmaxf(y, 0.0f);
         });
-        z = block_sum(z);
-        if (tid == 0) out_s[flip] = z;
-        cluster_sync();  // also: the new values are there for the next child
-        z = 0.0f;
-        for (unsigned k = 0; k < ctas; ++k) z += dsmem_load(&out_s[flip], k);
-        flip ^= 1;
+        tell(node, c, top, block_sum(z));
+        z = over_ctas_sum(got_s[flip ^ 1][peer]);
         left = z;
         if (!(z > 0.0f)) {  // the draft covers all that was left: it stays
-          for_row(q, len, a.vec, [&](int i, const float *y, int n) {
-            for (int k = 0; k < n; ++k) r[i + k] += y[k];
-          });
+          for_row<true>(q, len, a.vec, r, [&](float x, float &y, int) { y += x; });
+          __syncthreads();
+          tell(node, c, top, 0.0f);
           left = 1.0f;
-          cluster_sync();
         }
         own = 1.0f;
-        if (tid < (int)ctas) scale_s[tid] = 1.0f;
+        __syncthreads();
+        if (tid < kVerifyCluster) scale_s[tid] = 1.0f;
         __syncthreads();
       } else {
         for (int j = 0; j < rejected; ++j)
@@ -282,42 +356,32 @@ __global__ void __launch_bounds__(kVerifyThreads) tree_verify_kernel(const __gri
       }
     }
     if (child >= 0) {
-      cluster_sync();  // reads of r are done before the next row overwrites it
       node = child;
+      __syncthreads();  // r is read
       continue;
     }
     if (greedy) {
       next = all.i == 0x7fffffff ? 0 : all.i;
       break;
     }
-    cluster_sync();
     for (int j = tid; j < rejected; j += kVerifyThreads)
       if (refused[j] >= v0 && refused[j] < v0 + len) r[refused[j] - v0] = 0.0f;
     __syncthreads();
     Best pick{-1.0f, 0x7fffffff};
-    for_row(noise, len, a.vec, [&](int i, const float *e, int n) {
-      for (int k = 0; k < n; ++k) {
-        const float w = fmaxf(r[i + k], 0.0f) * own / e[k];
-        if (w > pick.v) pick = Best{w, v0 + i + k};
-      }
+    for_row<false>(noise, len, a.vec, r, [&](float e, float &y, int i) {
+      const float w = fmaxf(y, 0.0f) * own / e;
+      if (w > pick.v) pick = Best{w, v0 + i};
     });
-    pick = block_best(pick);
-    if (tid == 0) {
-      out_v[flip] = pick.v;
-      out_i[flip] = pick.i;
-    }
-    cluster_sync();
-    pick = Best{-1.0f, 0x7fffffff};
-    for (unsigned c = 0; c < ctas; ++c)
-      pick = better(pick, Best{dsmem_load(&out_v[flip], c), dsmem_load_int(&out_i[flip], c)});
+    tell(a.nodes, a.nodes, block_best(pick), 0.0f);
+    pick = over_ctas_best(Best{got_v[flip ^ 1][peer], __float_as_int(got_i[flip ^ 1][peer])});
     next = pick.i == 0x7fffffff ? 0 : pick.i;
     break;
   }
+  // (nothing is stored to another CTA after its last barrier)
   if (rank == 0 && tid == 0) {
     a.count[b] = taken;
     a.next[b] = next;
   }
-  cluster_sync();  // no CTA leaves while its slots may still be read
 }
 
 template <typename T>
