@@ -9,14 +9,14 @@
 namespace fpb {
 namespace {
 
-constexpr int kAppendThreads = 256, kMaxHalf = 128;
+constexpr int kAppendThreads = 256, kMaxHalf = 128, kMaxSpan = 4;
 
 struct AppendArgs {
   const void *q, *k, *v;
   long long q_pitch, q_head, k_pitch, v_pitch;  // elements
   const float *q_gamma, *k_gamma;
   const int32_t *positions, *parents;
-  int nodes, q_heads, kv_heads, head_dim, rotary_dim, max_seq, vec;
+  int rows, span, nodes, q_heads, kv_heads, head_dim, rotary_dim, max_seq, vec;
   float inv_d, eps;
   void *q_out;
   int q_out_bf16;
@@ -25,33 +25,44 @@ struct AppendArgs {
   uint64_t turn[kMaxHalf];  // theta^(-i / half) / (2 pi) of a turn, in units of 2^-64
 };
 
-// Eight consecutive elements as f32.
+// Eight consecutive elements as they lie; their f32 values.
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, bool vec, float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
+struct Eight {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T *p, bool vec) {
     if (vec) {
-      const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-      x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
     } else {
+      uint32_t *o = reinterpret_cast<uint32_t *>(w);
+      if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = p[i];
-    }
-  } else {
-    if (vec) {
-      const uint4 a = *reinterpret_cast<const uint4 *>(p);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+        for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(p[i]);
+      } else {
+        const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        for (int i = 0; i < 4; ++i) o[i] = h[2 * i] | (uint32_t)h[2 * i + 1] << 16;
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __bfloat162float(p[i]);
     }
   }
-}
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void values(float (&x)[8]) const {
+    const uint32_t *o = reinterpret_cast<const uint32_t *>(w);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(o[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(o[i] << 16);
+        x[2 * i + 1] = __uint_as_float(o[i] & 0xffff0000u);
+      }
+    }
+  }
+};
 
 // Two values -> two e4m3 codes (RNE, satfinite; NaN stays NaN), a in the low byte.
 __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
@@ -60,9 +71,9 @@ __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
   return out;
 }
 
-// One token's heads: block (row, part) takes every gridDim.y-th group of
-// heads of row b * nodes + n, LG lanes a head vector, eight elements a lane
-// (LG * 8 >= head_dim).
+// Some tokens' heads: block (x, part) takes the `span` rows from x * span on
+// (row b * nodes + n: a token) and of their heads every gridDim.y-th group, LG
+// lanes a head vector, eight elements a lane (LG * 8 >= head_dim).
 //  norm    x * rsqrt(mean x^2 + eps) * gamma, f32
 //  rotate  dimensions i and i + half by (position + depth) * theta^(-i/half).
 //          The turn is taken as a 64-bit fraction, an exact product of whole
@@ -75,47 +86,85 @@ __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
 template <typename T, int LG>
 __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const __grid_constant__ AppendArgs a) {
   pdl_enter();
-  __shared__ float cs[kMaxHalf], sn[kMaxHalf];
+  __shared__ float2 turn_s[kMaxSpan][kMaxHalf];  // cosine, sine
   __shared__ float xs[kAppendThreads / LG][LG * 8];
-  __shared__ int depth_s;
-  const int row = blockIdx.x, b = row / a.nodes, n = row % a.nodes;
+  __shared__ int depth_s[kMaxSpan], pos_s[kMaxSpan];
+  __shared__ size_t to_s[kMaxSpan];  // the rows' places in the cache, in rows
   const int tid = threadIdx.x, lane = tid % LG, item = tid / LG;
-  const int pos = a.positions[b];
-  if (tid == 0) {
+  constexpr int kItems = kAppendThreads / LG;
+  const int row0 = blockIdx.x * a.span, span = min(a.span, a.rows - row0);
+  const int D = a.head_dim, c0 = lane * 8, heads = a.q_heads + 2 * a.kv_heads, half = a.rotary_dim / 2;
+  // a head's elements are asked for one head ahead, the first before the sines
+  Eight<T> raw;
+  auto ask = [&](int rl, int h) {
+    raw.zero();
+    if (rl >= span || c0 >= D) return;
+    const size_t row = row0 + rl;
+    const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + a.kv_heads;
+    const T *src = is_q   ? static_cast<const T *>(a.q) + row * a.q_pitch + (size_t)h * a.q_head
+                   : is_k ? static_cast<const T *>(a.k) + row * a.k_pitch + (size_t)(h - a.q_heads) * D
+                          : static_cast<const T *>(a.v) + row * a.v_pitch + (size_t)(h - a.q_heads - a.kv_heads) * D;
+    raw.load(src + c0, a.vec);
+  };
+  int rl = 0, h = blockIdx.y * kItems + item;
+  while (h >= heads) {
+    h -= heads;
+    ++rl;
+  }
+  ask(rl, h);
+  if (tid < span) {
+    const int row = row0 + tid, b = row / a.nodes, n = row - b * a.nodes, pos = a.positions[b];
     bool bad = false;
-    int d = tree_depth(a.parents ? a.parents + (size_t)b * a.nodes : nullptr, n, &bad);
+    int depth = tree_depth(a.parents ? a.parents + (size_t)b * a.nodes : nullptr, n, &bad);
     if (bad && a.error) atomicCAS(a.error, 0, kErrParent);
-    if (d >= 0 && (pos < 0 || pos >= a.max_seq - n)) {
+    if (depth >= 0 && (pos < 0 || pos >= a.max_seq - n)) {
       if (a.error) atomicCAS(a.error, 0, kErrPosition);
-      d = -1;
+      depth = -1;
     }
-    depth_s = d;
+    depth_s[tid] = depth;
+    pos_s[tid] = pos;
+    to_s[tid] = (size_t)b * a.max_seq + pos + n;
   }
   __syncthreads();
-  const int depth = depth_s, half = a.rotary_dim / 2;
-  if (depth >= 0)
-    for (int i = tid; i < half; i += kAppendThreads) {
-      const uint64_t turn = a.turn[i] * (uint64_t)(uint32_t)(pos + depth);
+  if (half > 0) {
+    for (int i = tid; i < span * half; i += kAppendThreads) {
+      const int r = i / half, c = i - r * half;
+      const uint64_t turn = a.turn[c] * (uint64_t)(uint32_t)(pos_s[r] + max(depth_s[r], 0));
       const float t = (float)(int32_t)(uint32_t)(turn >> 32) * 0x1p-31f;  // half turns, in [-1, 1]
-      sincospif(t, &sn[i], &cs[i]);
+      float2 cs;
+      sincospif(t, &cs.y, &cs.x);
+      turn_s[r][c] = cs;
     }
-  __syncthreads();
-  const int D = a.head_dim, c0 = lane * 8, heads = a.q_heads + 2 * a.kv_heads;
-  constexpr int kItems = kAppendThreads / LG;
-  for (int h0 = blockIdx.y * kItems; h0 < heads; h0 += gridDim.y * kItems) {
-    const int h = h0 + item;
-    const bool live = h < heads && c0 < D;
-    const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + a.kv_heads;
-    const int kvh = is_q ? 0 : h - a.q_heads - (is_k ? 0 : a.kv_heads);
-    float x[8];
+    __syncthreads();
+  }
+  // The sines of a lane's columns serve all of a row's heads: in registers, with
+  // 1 and 0 past the rotated dimensions.
+  const bool lanes_turn = half > 0 && half % 8 == 0, low = c0 < half;
+  const int partner = (tid & 31) + (c0 >= 2 * half ? 0 : low ? half / 8 : -half / 8);
+  int turned = -1;
+  float cs[8], sn[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-    if (live && depth >= 0) {
-      const T *src = is_q ? static_cast<const T *>(a.q) + (size_t)row * a.q_pitch + (size_t)h * a.q_head
-                   : is_k ? static_cast<const T *>(a.k) + (size_t)row * a.k_pitch + (size_t)kvh * D
-                          : static_cast<const T *>(a.v) + (size_t)row * a.v_pitch + (size_t)kvh * D;
-      load8(src + c0, a.vec, x);
+  for (int i = 0; i < 8; ++i) {
+    cs[i] = 1.0f;
+    sn[i] = 0.0f;
+  }
+  // (the loop ends together for the whole block: its warps' lanes shuffle)
+  const int total = span * heads;
+  for (int i0 = blockIdx.y * kItems; i0 < total; i0 += gridDim.y * kItems) {
+    const int depth = rl < span ? depth_s[rl] : -1;
+    const size_t row = row0 + rl;
+    const bool live = rl < span && c0 < D;
+    const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + a.kv_heads;
+    const int kvh = is_q ? 0 : h - a.q_heads - (is_k ? 0 : a.kv_heads), here = h, at = min(rl, span - 1);
+    float x[8];
+    if (depth < 0) raw.zero();  // rows of nodes that are not there: zeros
+    raw.values(x);
+    h += gridDim.y * kItems;
+    while (h >= heads) {
+      h -= heads;
+      ++rl;
     }
+    ask(rl, h);
     const float *gamma = is_q ? a.q_gamma : is_k ? a.k_gamma : nullptr;
     float ss = 0.0f;
 #pragma unroll
@@ -124,23 +173,42 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const __grid
     for (int o = LG / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     if (gamma && live) {
       const float scale = __frsqrt_rn(fmaf(ss, a.inv_d, a.eps));
-      float g[8];
-      load8(gamma + c0, true, g);
+      const float4 g0 = __ldg(reinterpret_cast<const float4 *>(gamma + c0)),
+                   g1 = __ldg(reinterpret_cast<const float4 *>(gamma + c0) + 1);
+      const float g[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = x[i] * scale * g[i];
     }
-    if (half > 0) {
+    if (lanes_turn) {  // the partners of a lane's eight lie in one lane
+      if (at != turned && c0 < 2 * half) {
+        const float2 *t = &turn_s[at][low ? c0 : c0 - half];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) xs[item][c0 + i] = x[i];
+        for (int i = 0; i < 8; ++i) {
+          cs[i] = t[i].x;
+          sn[i] = low ? -t[i].y : t[i].y;
+        }
+        turned = at;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float y = __shfl_sync(0xffffffffu, x[i], partner);
+        if (is_q || is_k) x[i] = fmaf(y, sn[i], x[i] * cs[i]);
+      }
+    } else if (half > 0) {
+      const bool turns = live && (is_q || is_k) && c0 < 2 * half;
+      if (turns) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) xs[item][c0 + i] = x[i];
+      }
       __syncwarp();
-      if (live && (is_q || is_k) && depth >= 0) {
+      if (turns) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int c = c0 + i;
           if (c < half)
-            x[i] = x[i] * cs[c] - xs[item][c + half] * sn[c];
+            x[i] = x[i] * turn_s[at][c].x - xs[item][c + half] * turn_s[at][c].y;
           else if (c < 2 * half)
-            x[i] = x[i] * cs[c - half] + xs[item][c - half] * sn[c - half];
+            x[i] = x[i] * turn_s[at][c - half].x + xs[item][c - half] * turn_s[at][c - half].y;
         }
       }
       __syncwarp();
@@ -151,8 +219,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const __grid
 #pragma unroll
     for (int o = LG / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if (!live) continue;
-    if (is_q) {  // rows of nodes that are not there: zeros
-      const size_t o = ((size_t)row * a.q_heads + h) * D + c0;
+    if (is_q) {
+      const size_t o = (row * a.q_heads + here) * D + c0;
       if (a.q_out_bf16) {
         uint4 w;
         w.x = pack_bf16x2(x[0], x[1]);
@@ -168,7 +236,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const __grid
     } else if (depth >= 0) {
       const int e = kv8_exponent(amax);
       const float inv = pow2i(-e);
-      const size_t vec = ((size_t)b * a.max_seq + pos + n) * a.kv_heads + kvh;
+      const size_t vec = to_s[at] * a.kv_heads + kvh;
       uint2 w;
       w.x = e4m3x2(x[0] * inv, x[1] * inv) | e4m3x2(x[2] * inv, x[3] * inv) << 16;
       w.y = e4m3x2(x[4] * inv, x[5] * inv) | e4m3x2(x[6] * inv, x[7] * inv) << 16;
@@ -280,16 +348,18 @@ int check_cache(const char *name, const void *kc, const void *vc, const void *ke
 }
 
 template <typename T>
-int run_append(const AppendArgs &a, size_t rows, cudaStream_t s) {
+int run_append(AppendArgs a, size_t rows, cudaStream_t s) {
   const int lanes = a.head_dim / 8;
   const int lg = lanes <= 8 ? 8 : lanes <= 16 ? 16 : 32;
   const int heads = a.q_heads + 2 * a.kv_heads, per = kAppendThreads / lg;
-  // One pass over the heads a block while that leaves fewer than four blocks
-  // an SM; beyond, a block takes all of its token's heads and makes the
-  // token's sines once.
+  // Few rows: one group of heads a block.  Beyond four blocks an SM a block
+  // takes all of a row's heads, and of four rows from sixteen blocks an SM on:
+  // the rows' positions and sines are then made for all of them at once
+  // (2 x 4096 tokens of 48 heads: 97 us with one row a block).
   const int parts = (heads + per - 1) / per;
-  const int want = (int)std::min<size_t>(parts, std::max<size_t>(1, (size_t)sm_count() * 4 / rows));
-  const dim3 grid((unsigned)rows, (unsigned)want);
+  a.span = rows >= (size_t)sm_count() * 16 ? kMaxSpan : 1;
+  const size_t want = std::min<size_t>(parts, std::max<size_t>(1, (size_t)sm_count() * 4 / rows));
+  const dim3 grid((unsigned)((rows + a.span - 1) / a.span), (unsigned)want);
   cudaError_t e = lg == 8    ? launch_pdl(kv8_append_kernel<T, 8>, grid, kAppendThreads, 0, s, a)
                   : lg == 16 ? launch_pdl(kv8_append_kernel<T, 16>, grid, kAppendThreads, 0, s, a)
                              : launch_pdl(kv8_append_kernel<T, 32>, grid, kAppendThreads, 0, s, a);
@@ -339,6 +409,7 @@ extern "C" int fpb_kv8_append(const void *q, size_t q_pitch, size_t q_head_pitch
   a.k_gamma = k_gamma;
   a.positions = positions;
   a.parents = parents;
+  a.rows = (int)(batch * nodes);
   a.nodes = (int)nodes;
   a.q_heads = (int)q_heads;
   a.kv_heads = (int)kv_heads;
@@ -356,8 +427,10 @@ extern "C" int fpb_kv8_append(const void *q, size_t q_pitch, size_t q_head_pitch
   a.v_exp = v_exp;
   a.error = device_error_ptr();
   const int half = (int)rotary_dim / 2;
-  for (int i = 0; i < half; ++i)  // at most 2^64 / (2 pi)
-    a.turn[i] = (uint64_t)(powl((long double)theta, -(long double)i / half) / (2.0L * M_PIl) * 0x1p64L);
+  // theta^(-i / half) by products of 64-bit mantissas: off by i * 2^-63 of itself at most
+  const long double ratio = half ? powl((long double)theta, -1.0L / half) : 0.0L;
+  long double turn = 0x1p64L / (2.0L * M_PIl);
+  for (int i = 0; i < half; ++i, turn *= ratio) a.turn[i] = (uint64_t)turn;
   cudaStream_t s = as_stream(stream);
   return dtype == FPB_F32 ? run_append<float>(a, batch * nodes, s) : run_append<__nv_bfloat16>(a, batch * nodes, s);
 }
