@@ -11,6 +11,11 @@ N(0, 0.02) (each expert and each matrix its own global), activations f32,
 GEMV inputs bf16; the decode step for a batch of sessions is one CUDA graph;
 the prompt runs through the same decode step, one token per step.
 
+``Decoder(..., kv8=True)`` keeps the attention layers' keys and values in the
+8-bit cache (firepit_b200/speculative.py).  ``SpeculativeDecoder`` runs a tree
+of drafted tokens a session through a model of full-attention layers in one
+step and keeps the path that the model accepts.
+
 Multi-GPU: ``replicas`` — every GPU holds the whole model and decodes its own
 sessions (no exchange).
 """
@@ -203,19 +208,25 @@ class HybridModel:
 class Decoder:
     """Greedy decoding of `batch` sessions on one GPU: ``step()`` issues one
     decode step (all layers, LM head, argmax) on the current stream;
-    ``capture()`` records it as a CUDA graph."""
+    ``capture()`` records it as a CUDA graph.  kv8: the attention layers' caches
+    in 8 bits (a quarter of the f32 caches' bytes; head_dim a multiple of 16)."""
 
-    def __init__(self, model: HybridModel, batch: int, max_seq: int, history_len: int = 0):
+    nodes = 1  # rows a session
+    parents = None
+
+    def __init__(self, model: HybridModel, batch: int, max_seq: int, history_len: int = 0, kv8: bool = False):
         import torch
+
+        from .speculative import Kv8Cache
         self.model, self.cfg = model, model.cfg
-        c, dev, B = model.cfg, model.device, batch
-        self.batch, self.max_seq = batch, max_seq
+        c, dev, B = model.cfg, model.device, batch * self.nodes
+        self.sessions, self.batch, self.max_seq, self.kv8 = batch, B, max_seq, kv8
         f32 = dict(dtype=torch.float32, device=dev)
         i32 = dict(dtype=torch.int32, device=dev)
         bf = dict(dtype=torch.bfloat16, device=dev)
         h = c.hidden
         self.tokens = torch.zeros(B, **i32)
-        self.positions = torch.zeros(B, **i32)
+        self.positions = torch.zeros(batch, **i32)
         self.step_ctr = torch.zeros(2, **i32)
         self.history_len = history_len
         self.history = torch.zeros(B, max(1, history_len), **i32)
@@ -234,8 +245,9 @@ class Decoder:
         self.vp = torch.zeros(B, c.kv_heads * c.head_dim, **f32)
         self.q_rot = torch.zeros(B, c.q_heads, c.head_dim, **f32)
         self.attn = torch.zeros(B, c.q_heads * c.head_dim, **bf)
-        self.attn_ws = torch.empty(int(N.lib.fpb_attn_decode_workspace_bytes(B, c.q_heads, c.head_dim, max_seq, 32)),
-                                   dtype=torch.uint8, device=dev)
+        ws = int(N.lib.fpb_tree_attn_workspace_bytes(batch, self.nodes, c.q_heads, c.kv_heads, c.head_dim, max_seq)
+                 if kv8 else N.lib.fpb_attn_decode_workspace_bytes(B, c.q_heads, c.head_dim, max_seq, 32))
+        self.attn_ws = torch.empty(ws, dtype=torch.uint8, device=dev)
         self.logits_r = torch.zeros(B, c.route_rows, **f32)  # router logits, then the gate logit
         self.gate = torch.zeros(B, **f32)
         self.ids = torch.zeros(B, c.slots, **i32)
@@ -258,8 +270,9 @@ class Decoder:
         self.gdn = {}
         for i, L in enumerate(model.layers):
             if L["kind"] == "attention":
-                shape = (B, max_seq, c.kv_heads, c.head_dim)
-                self.kv[i] = (torch.zeros(shape, **f32), torch.zeros(shape, **f32))
+                shape = (batch, max_seq, c.kv_heads, c.head_dim)
+                self.kv[i] = Kv8Cache.zeros(*shape, device=dev) if kv8 else (torch.zeros(shape, **f32),
+                                                                             torch.zeros(shape, **f32))
             else:
                 self.gdn[i] = (torch.zeros(B, c.conv_dim, c.conv_kernel - 1, **f32),
                                torch.zeros(B, c.value_heads, c.key_head_dim, c.value_head_dim, **f32))
@@ -307,6 +320,39 @@ class Decoder:
         else:
             N.call("fpb_nvfp4_gemv_batched", b._segs, len(members), N.FPB_BF16, N.FPB_F32, self.batch, sh)
 
+    def _attend(self, i, L, sh: int) -> None:
+        """Attention layer i from its projections to self.attn: head norms,
+        rotation and cache append, then the attention with its output gate."""
+        c, B, eps, BF = self.cfg, self.batch, self.cfg.eps, N.FPB_BF16
+        if self.kv8:
+            kv, D, par = self.kv[i], c.head_dim, None if self.parents is None else self.parents.data_ptr()
+            N.call("fpb_kv8_append", self.qg.data_ptr(), self.qg.shape[1], 2 * D, self.kp.data_ptr(), self.kp.shape[1],
+                   self.vp.data_ptr(), self.vp.shape[1], N.FPB_F32, L["q_norm"].data_ptr(), L["k_norm"].data_ptr(),
+                   self.positions.data_ptr(), par, self.sessions, self.nodes, c.q_heads, c.kv_heads, D, c.rotary_dim,
+                   c.rope_theta, eps, self.max_seq, self.q_rot.data_ptr(), N.FPB_F32, kv.k.data_ptr(), kv.v.data_ptr(),
+                   kv.k_exp.data_ptr(), kv.v_exp.data_ptr(), sh)
+            N.call("fpb_tree_attn", self.q_rot.data_ptr(), N.FPB_F32, c.q_heads * D, D, kv.k.data_ptr(),
+                   kv.v.data_ptr(), kv.k_exp.data_ptr(), kv.v_exp.data_ptr(), self.positions.data_ptr(), par,
+                   self.qg.data_ptr() + 4 * D, self.qg.shape[1], 2 * D, self.sessions, self.nodes, c.q_heads,
+                   c.kv_heads, D, self.max_seq, 1.0 / math.sqrt(D), self.attn_ws.data_ptr(), self.attn_ws.numel(),
+                   self.attn.data_ptr(), sh)
+            return
+        kc, vc = self.kv[i]
+        N.call("fpb_attn_prepare", self.qg.data_ptr(), self.qg.shape[1], self.kp.data_ptr(), self.kp.shape[1],
+               self.vp.data_ptr(), self.vp.shape[1], L["q_norm"].data_ptr(), L["k_norm"].data_ptr(),
+               self.positions.data_ptr(), B, c.q_heads, c.kv_heads, c.head_dim, c.rotary_dim, c.rope_theta, eps,
+               self.max_seq, self.q_rot.data_ptr(), kc.data_ptr(), vc.data_ptr(), sh)
+        N.call("fpb_attn_decode", self.q_rot.data_ptr(), kc.data_ptr(), vc.data_ptr(), self.positions.data_ptr(),
+               self.qg.data_ptr(), self.qg.shape[1], B, c.q_heads, c.kv_heads, c.head_dim, self.max_seq, 32,
+               1.0 / math.sqrt(c.head_dim), self.attn_ws.data_ptr(), self.attn_ws.numel(),
+               self.attn.data_ptr(), BF, sh)
+
+    def _sample(self, sh: int) -> None:
+        """The next tokens from self.logits, and the sessions' positions."""
+        N.call("fpb_argmax_advance", self.logits.data_ptr(), self.batch, self.cfg.vocab, self.tokens.data_ptr(),
+               self.positions.data_ptr(), self.history.data_ptr() if self.history_len else None, self.history_len,
+               self.step_ctr.data_ptr(), sh)
+
     def step(self, sh: int) -> None:
         """One decode step of every session on stream handle sh."""
         m, c, B = self.model, self.cfg, self.batch
@@ -341,15 +387,7 @@ class Decoder:
             else:
                 self._gemv(("attn", i), [(L["w_qg"], self.qg), (L["w_k"], self.kp), (L["w_v"], self.vp)],
                            self.normed, sh)
-                kc, vc = self.kv[i]
-                N.call("fpb_attn_prepare", self.qg.data_ptr(), self.qg.shape[1], self.kp.data_ptr(), self.kp.shape[1],
-                       self.vp.data_ptr(), self.vp.shape[1], L["q_norm"].data_ptr(), L["k_norm"].data_ptr(),
-                       self.positions.data_ptr(), B, c.q_heads, c.kv_heads, c.head_dim, c.rotary_dim, c.rope_theta, eps,
-                       self.max_seq, self.q_rot.data_ptr(), kc.data_ptr(), vc.data_ptr(), sh)
-                N.call("fpb_attn_decode", self.q_rot.data_ptr(), kc.data_ptr(), vc.data_ptr(), self.positions.data_ptr(),
-                       self.qg.data_ptr(), self.qg.shape[1], B, c.q_heads, c.kv_heads, c.head_dim, self.max_seq, 32,
-                       1.0 / math.sqrt(c.head_dim), self.attn_ws.data_ptr(), self.attn_ws.numel(),
-                       self.attn.data_ptr(), BF, sh)
+                self._attend(i, L, sh)
                 self._gemv(("attn_out", i), [(L["w_o"], self.delta)], self.attn, sh)
             # post norm: resid[1 - cur] = resid[cur] + delta, normed = RMSNorm
             N.call("fpb_rms_norm", self.resid[cur].data_ptr(), F32, h, self.delta.data_ptr(),
@@ -410,9 +448,7 @@ class Decoder:
                    self.logits.data_ptr(), F32, self.ws_x.data_ptr(), self.ws_x.numel(), sh)
         else:
             self._gemv(("lm_head",), [(m.lm_head, self.logits)], self.normed, sh)
-        N.call("fpb_argmax_advance", self.logits.data_ptr(), B, c.vocab, self.tokens.data_ptr(),
-               self.positions.data_ptr(), self.history.data_ptr() if self.history_len else None, self.history_len,
-               self.step_ctr.data_ptr(), sh)
+        self._sample(sh)
 
     def capture(self):
         """Records one decode step as a CUDA graph (every code path run once
@@ -429,9 +465,9 @@ class Decoder:
         """Clears the sessions: positions, caches, recurrent states, history."""
         for t in (self.tokens, self.positions, self.step_ctr, self.history):
             t.zero_()
-        for kc, vc in self.kv.values():
-            kc.zero_()
-            vc.zero_()
+        for kv in self.kv.values():
+            for t in (kv,) if self.kv8 else kv:
+                t.zero_()
         for cs, rs in self.gdn.values():
             cs.zero_()
             rs.zero_()
@@ -448,3 +484,136 @@ class Decoder:
     def generate(self, steps: int) -> None:
         for _ in range(steps):
             self.graph.replay()
+
+
+class SpeculativeDecoder(Decoder):
+    """Speculative decoding of `sessions` sessions over the 8-bit cache, on a
+    model whose layers are all full attention (a recurrent layer's state cannot
+    hold the branches of a tree; full_attention_interval 1).
+
+    A step takes `nodes` rows a session: ``tokens`` [sessions, nodes] with the
+    last emitted token first, and ``parents`` (-2: no such node).  It appends,
+    attends and verifies the tree, moves the accepted path's rows together,
+    advances the positions by ``count`` and makes ``next`` the new first token;
+    ``emitted`` [sessions, nodes] holds the tokens that the step added, -1 after
+    them.  temperature 0: greedy; above it ``accept`` [sessions, nodes] and
+    ``noise`` [sessions, vocab] hold the step's random numbers (``draw``) and
+    ``draft``, where set, the drafts' probabilities.  sessions * nodes <= 16
+    (the decode GEMVs' rows)."""
+
+    def __init__(self, model: HybridModel, sessions: int, nodes: int, max_seq: int, temperature: float = 0.0):
+        import torch
+
+        from .gemv import ShapeError
+        c, dev = model.cfg, model.device
+        if not all(c.is_attention(i) for i in range(c.layers)):
+            raise ShapeError("speculative decoding needs full attention in every layer (full_attention_interval 1)")
+        if sessions < 1 or nodes < 1 or sessions * nodes > 16:
+            raise ShapeError(f"speculative decoding: {sessions} sessions x {nodes} nodes, at most 16 rows")
+        if nodes > max_seq:
+            raise ShapeError(f"speculative decoding: {nodes} nodes in a cache of {max_seq} rows")
+        self.nodes = nodes
+        super().__init__(model, sessions, max_seq, kv8=True)
+        i32 = dict(dtype=torch.int32, device=dev)
+        self.temperature = temperature
+        self.tree = self.tokens.view(sessions, nodes)
+        self.parents = torch.full((sessions, nodes), -2, **i32)
+        self.parents[:, 0] = -1
+        self.path = torch.zeros(sessions, nodes, **i32)
+        self.count = torch.zeros(sessions, **i32)
+        self.next = torch.zeros(sessions, **i32)
+        self.emitted = torch.full((sessions, nodes), -1, **i32)
+        self.at = torch.arange(nodes, **i32)
+        self.draft = None
+        self.accept = self.noise = None
+        if temperature > 0.0:
+            self.accept = torch.zeros(sessions, nodes, device=dev)
+            self.noise = torch.ones(sessions, c.vocab, device=dev)
+
+    def reset(self) -> None:
+        super().reset()
+        self.parents.fill_(-2)
+        self.parents[:, 0] = -1
+
+    def draw(self, generator=None) -> None:
+        """New random numbers for the next step."""
+        self.accept.uniform_(generator=generator)
+        self.noise.exponential_(generator=generator).clamp_(min=1e-20)
+
+    def _sample(self, sh: int) -> None:
+        import torch
+        c, S, n = self.cfg, self.sessions, self.nodes
+        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        N.call("fpb_tree_verify", self.logits.data_ptr(), N.FPB_F32, c.vocab, ptr(self.draft), c.vocab,
+               self.tokens.data_ptr(), self.parents.data_ptr(), ptr(self.accept), ptr(self.noise), c.vocab, S, n,
+               c.vocab, self.temperature, self.path.data_ptr(), self.count.data_ptr(), self.next.data_ptr(), sh)
+        for kv in self.kv.values():
+            N.call("fpb_kv8_keep", kv.k.data_ptr(), kv.v.data_ptr(), kv.k_exp.data_ptr(), kv.v_exp.data_ptr(), S,
+                   self.max_seq, c.kv_heads, c.head_dim, self.positions.data_ptr(), self.path.data_ptr(), n, sh)
+        # the accepted drafts, then the token after them
+        taken = torch.gather(self.tree, 1, self.path.clamp(min=0).long()).roll(-1, 1)
+        left = self.count[:, None] - 1 - self.at
+        self.emitted.copy_(torch.where(left > 0, taken, torch.where(left == 0, self.next[:, None], -1)))
+        self.positions.add_(self.count)
+        self.tree[:, 0].copy_(self.next)
+
+    def feed(self, tokens) -> None:
+        """Runs known tokens [sessions, n] (device int32) through the model,
+        `nodes` of them a step (teacher forcing); their rows join the cache."""
+        import torch
+        sh = torch.cuda.current_stream(self.model.device).cuda_stream
+        for t in range(0, tokens.shape[1], self.nodes):
+            part = tokens[:, t:t + self.nodes]
+            m = part.shape[1]
+            self.tree[:, :m].copy_(part)
+            self.parents.copy_(torch.where(self.at < m, self.at - 1, -2).expand_as(self.parents))
+            before = self.positions.clone()
+            self.step(sh)  # (what the verification keeps of a chain lies where it is)
+            self.positions.copy_(before.add_(m))
+
+    def generate(self, prompt, new_tokens: int, drafter) -> list[list[int]]:
+        """Appends at least `new_tokens` tokens to each session's prompt
+        [sessions, length]; drafter(history: list[int], nodes) -> (tokens,
+        parents) proposes each step's tree after its first node (lists of at
+        most nodes - 1 entries; a parent is 0 for the first node, k for the
+        k-th drafted token).  Returns the new tokens of each session."""
+        import torch
+
+        from .gemv import ShapeError
+        if prompt.shape[1] + new_tokens + 2 * self.nodes > self.max_seq:
+            raise ShapeError(f"generate: {prompt.shape[1]} + {new_tokens} tokens and two steps' nodes in a cache of "
+                             f"{self.max_seq} rows")
+        self.reset()
+        if prompt.shape[1] > 1:
+            self.feed(prompt[:, :-1])
+        self.tree[:, 0].copy_(prompt[:, -1])
+        sh = torch.cuda.current_stream(self.model.device).cuda_stream
+        history = prompt.cpu().tolist()
+        start = [len(h) for h in history]
+        while min(len(h) - n for h, n in zip(history, start)) < new_tokens:
+            tok, par = self.tree.cpu(), torch.full((self.sessions, self.nodes), -2, dtype=torch.int32)
+            par[:, 0] = -1
+            for s, h in enumerate(history):
+                drafts, up = drafter(h, self.nodes)
+                k = min(len(drafts), self.nodes - 1)
+                tok[s, 1:1 + k] = torch.tensor(drafts[:k], dtype=torch.int32)
+                par[s, 1:1 + k] = torch.tensor(up[:k], dtype=torch.int32)
+            self.tree.copy_(tok)
+            self.parents.copy_(par)
+            if self.temperature > 0.0:
+                self.draw()
+            self.step(sh)
+            for h, e in zip(history, self.emitted.cpu().tolist()):
+                h.extend(t for t in e if t >= 0)
+        return [h[n:] for h, n in zip(history, start)]
+
+
+def lookup_drafts(history: list[int], nodes: int, match: int = 2):
+    """A drafter for ``SpeculativeDecoder.generate``: the tokens that followed
+    the latest earlier occurrence of the last `match` tokens, as a chain."""
+    key = history[-match:]
+    for i in range(len(history) - match - 1, -1, -1):
+        if history[i:i + match] == key:
+            drafts = history[i + match:i + match + nodes - 1]
+            return drafts, list(range(len(drafts)))
+    return [], []

@@ -119,3 +119,19 @@ def test_speculative_oracle_agrees_with_the_formats():
     codes, exps = R.quantise(x[None])
     assert exps[0] == 127
     assert [int(c) for c in codes[0]] == [N.lib.fpb_f32_to_e4m3(float(v)) for v in x]
+
+
+def test_speculative_decoder_refuses_what_it_cannot_run():
+    torch = pytest.importorskip("torch")
+    from types import SimpleNamespace
+
+    from firepit_b200.model import HybridConfig, SpeculativeDecoder, lookup_drafts
+    full = SimpleNamespace(cfg=HybridConfig(layers=2, full_attention_interval=1), device=torch.device("cpu"))
+    hybrid = SimpleNamespace(cfg=HybridConfig(layers=4), device=torch.device("cpu"))
+    for model, sessions, nodes, max_seq in ((hybrid, 1, 4, 64), (full, 0, 4, 64), (full, 1, 0, 64), (full, 2, 9, 64),
+                                            (full, 1, 8, 7)):
+        with pytest.raises(F.ShapeError):
+            SpeculativeDecoder(model, sessions, nodes, max_seq)
+    assert lookup_drafts([1, 2, 3, 4, 1, 2], 3) == ([3, 4], [0, 1])
+    assert lookup_drafts([1, 2, 3], 3) == ([], [])
+    assert lookup_drafts([5], 3) == ([], [])
