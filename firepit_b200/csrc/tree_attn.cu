@@ -47,7 +47,7 @@ template <int DP, int NR>
 struct RowsShape {
   static constexpr bool kQShared = NR * DP > 16 * 128;  // 64 registers of queries are too many beside 128 of sums
   static constexpr int kQPitch = DP + 8;                // f16 elements: 16-byte reads of eight rows on distinct banks
-  static constexpr int kBox = DP == 64 ? 64 : 128, kBoxes = DP / kBox;
+  static constexpr int kBox = DP == 64 ? 64 : 128;
   static constexpr uint32_t kStage = 2 * 16 * DP;  // a step's codes, keys then values
   static constexpr size_t kRing = (size_t)kRowsWarps * kRowsStages * kStage;
   static constexpr size_t kEnd = (size_t)kRowsWarps * NR * (DP + 2) * 4;  // the warps' results, over the ring

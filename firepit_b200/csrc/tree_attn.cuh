@@ -17,12 +17,11 @@ struct TreeArgs {
   float *part;     // [session, kv head, row tile][split][row][head_dim] numerators
   float2 *part_ml; // [session, kv head, row tile][split][row] maximum, sum
   // for the tiles: queries as f16, their factors, what each node sees [session,
-  // 64], [session, kv head, row tile] first slot and last block, blocks' shares
+  // 64], [session, kv head, row tile] first slot and last block
   uint4 *q16;
   float *q_fac;
   uint64_t *sights;
   int2 *shares;
-  void *walks;
   int *error;
 };
 

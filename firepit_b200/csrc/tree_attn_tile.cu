@@ -42,7 +42,7 @@ struct TileShape {
   static constexpr uint32_t kBytes = BT * DP * 2, kRawBytes = BT * DP;
   static constexpr uint32_t kTmemO = 0, kTmemS = DP, kTmemQ = DP + 2 * BT;
   static constexpr int kPieces = BT * DP / 16 / (kConvWarps * 32);  // 16-byte pieces of codes a thread and tile
-  static constexpr int kBox = DP == 64 ? 64 : 128, kBoxes = DP / kBox;
+  static constexpr int kBox = DP == 64 ? 64 : 128;
 };
 
 struct Segment {
@@ -164,27 +164,27 @@ __device__ __forceinline__ float weigh_pass(uint32_t s_tmem, const float4 *fac, 
   const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
   float mx[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int c = 0; c < NT / 16; ++c) {
-    uint32_t r[16];
-    tmem_ld16(s_tmem + c * 16, r);
+  for (int c = 0; c < NT / 8; ++c) {
+    uint32_t r[8];
+    tmem_ld8(s_tmem + c * 8, r);
     tmem_ld_wait(r);
 #pragma unroll
-    for (int e = 0; e < 16; e += 2) {
-      const float4 ft = fac[(c * 16 + e) / 2];
+    for (int e = 0; e < 8; e += 2) {
+      const float4 ft = fac[(c * 8 + e) / 2];
       const uint64_t x = mul2(pack2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), pack2(ft.x, ft.y));
       float e0, e1, w0, w1;
       unpack2(fma2(x, f2, b2), e0, e1);
       e0 = exp2_approx(e0);
       e1 = exp2_approx(e1);
       if (OPEN) {
-        if (!(seen >> (c * 16 + e) & 1)) e0 = 0.0f;
-        if (!(seen >> (c * 16 + e + 1) & 1)) e1 = 0.0f;
+        if (!(seen >> (c * 8 + e) & 1)) e0 = 0.0f;
+        if (!(seen >> (c * 8 + e + 1) & 1)) e1 = 0.0f;
       }
       const uint64_t e2 = pack2(e0, e1);
       l = add2(l, e2);
       unpack2(mul2(e2, pack2(ft.z, ft.w)), w0, w1);
       mx[(e >> 1) & 1] = fmaxf(mx[(e >> 1) & 1], fmaxf(w0, w1));
-      p[(c * 16 + e) / 2] = pack_f16x2(w0, w1);
+      p[(c * 8 + e) / 2] = pack_f16x2(w0, w1);
     }
   }
   return fmaxf(mx[0], mx[1]);
@@ -250,10 +250,9 @@ __device__ __noinline__ float2 raise_max(TileShared *sh, uint32_t s_tmem, uint32
 // What the tile kernel reads at its start, made by blocks of 32 rows of a row
 // tile (eight warps): the queries as f16 in the order of its TMEM stores
 // [item][eight columns][128 rows], each row scaled by a power of two into f16's
-// range, with the factor of its scores; what each node sees; each block's
-// share of the units.
+// range, with the factor of its scores; what each node sees.
 constexpr int kPrepRows = 32;
-__global__ void __launch_bounds__(256) tree_attn_prep_kernel(const __grid_constant__ TreeArgs a, int BT, int blocks) {
+__global__ void __launch_bounds__(256) tree_attn_prep_kernel(const __grid_constant__ TreeArgs a) {
   pdl_enter();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = a.head_dim;
   const int rows = a.nodes * a.group, row_tiles = (rows + kTileRows - 1) / kTileRows, items = a.kv_heads * row_tiles;
@@ -304,17 +303,21 @@ __global__ void __launch_bounds__(256) tree_attn_prep_kernel(const __grid_consta
     const Sight s = sight_of(a, b, warp * 32 + lane, a.positions[b]);
     if (warp * 32 + lane < a.nodes) a.sights[(size_t)b * kTreeMaxNodes + warp * 32 + lane] = s.bits;
   }
-  const int c = blockIdx.x * 8 + warp;  // the block whose share this warp finds
-  if (c >= blocks) return;
+}
+
+// This block's share of the units, one warp.
+__device__ __noinline__ void share_out(const TreeArgs &a, TileShared *sh, int BT) {
+  const int lane = threadIdx.x & 31, row_tiles = (a.nodes * a.group + kTileRows - 1) / kTileRows;
+  const int items = a.kv_heads * row_tiles;
   int all = 0;
   for (int i = lane; i < a.batch; i += 32) all += session_tiles(a, i, BT);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-  const int units = all * items, live = min(blocks, units);
+  const int units = all * items, blocks = min((int)gridDim.x, units);
   int u0 = 0, u1 = 0;
-  if (c < live) {
-    u0 = (int)((long long)units * c / live);
-    u1 = (int)((long long)units * (c + 1) / live);
+  if ((int)blockIdx.x < blocks) {
+    u0 = (int)((long long)units * blockIdx.x / blocks);
+    u1 = (int)((long long)units * (blockIdx.x + 1) / blocks);
   }
   int s = 0, before = 0;  // the session that holds unit u0, and the units before it
   if (u1 > u0)
@@ -334,7 +337,8 @@ __global__ void __launch_bounds__(256) tree_attn_prep_kernel(const __grid_consta
         break;
       }
     }
-  if (lane == 0) static_cast<Walk *>(a.walks)[c] = Walk{s, u1 > u0 ? session_tiles(a, s, BT) : 1, row_tiles, u0 - before, u1 - u0};
+  if (lane == 0)
+    sh->walk = sh->soft_walk = Walk{s, u1 > u0 ? session_tiles(a, s, BT) : 1, row_tiles, u0 - before, u1 - u0};
 }
 
 template <int DP>
@@ -349,7 +353,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint8_t *const rK = sV + ST * Sh::kBytes, *const rV = rK + RAW * Sh::kRawBytes;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool tree = a.parents != nullptr;
-  if (warp == kMmaWarp) {
+  // The tile kernel starts beside the prep kernel, which has by then waited
+  // for whatever came before: only what the prep kernel itself writes is waited
+  // for, by the softmax.
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (warp == 0) {
+    share_out(a, sh, BT);
+  } else if (warp == kMmaWarp) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&sh->kfull[i], kConvWarps);
@@ -373,8 +383,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     tmem_alloc(&sh->tmem, 512);
     tmem_relinquish();
   }
-  pdl_enter();
-  if (tid == 0) sh->walk = sh->soft_walk = static_cast<const Walk *>(a.walks)[blockIdx.x];
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -397,6 +405,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     // After a wait that ran out this role goes on to its end without waiting
     // (the results are void): its warps meet at barriers.
     bool ok = true;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     // The walk, and what a segment needs once, lie in shared memory: the loop
     // over its tiles wants the registers.
     for (int seg = 0;; ++seg) {
@@ -757,34 +766,51 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     tc_fence_after();
     tmem_dealloc(sh->tmem, 512);
   }
+  // (a block without a share too: when this grid has ended, so has the prep grid)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // The blocks that share a row tile's tokens meet, in order, with the gate:
-// block (16 rows of a row tile, 64 columns); thread (row, four columns, share
-// of the blocks).  Rows of nodes that are not there become zeros.
+// block (16 rows of a row tile, 128 columns); thread (row, eight columns, share
+// of the blocks).  Rows of nodes that are not there become zeros.  What the
+// tile kernel does not write is read before it is waited for.
 constexpr int kMergeShares = 4;
 __global__ void __launch_bounds__(1024, 1) tree_attn_tile_merge_kernel(const __grid_constant__ TreeArgs a, int BT) {
-  pdl_enter();
-  __shared__ float4 acc_s[kMergeShares - 1][256];
+  __shared__ float4 acc_s[kMergeShares - 1][2][256];
   __shared__ float2 ml_s[kMergeShares - 1][256];
   const int t = threadIdx.x, share = threadIdx.y, D = a.head_dim;
   const int rows = a.nodes * a.group, row_tiles = (rows + kTileRows - 1) / kTileRows, items = a.kv_heads * row_tiles;
   const int item = blockIdx.x / (kTileRows / 16), r = blockIdx.x % (kTileRows / 16) * 16 + (t & 15);
   const int b = item / items, kvh = item % items / row_tiles, row = item % row_tiles * kTileRows + r;
-  if (item % row_tiles * kTileRows + (r & ~15) >= rows) return;
-  const int d = blockIdx.y * 64 + 4 * (t >> 4);
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (item % row_tiles * kTileRows + (r & ~15) >= rows) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
+  const int d = blockIdx.y * 128 + 8 * (t >> 4);
   const bool live = row < rows && d < D;
-  const int n = row / a.group, h = kvh * a.group + row % a.group;
+  const int n = row / a.group, h = kvh * a.group + row % a.group, pos = a.positions[b];
+  const size_t node = (size_t)b * a.nodes + n;
   const bool some = session_tiles(a, b, BT) > 0;
+  float gate[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) gate[i] = 1.0f;
+  if (live && a.gate && share == 0) {
+    const float *g = a.gate + node * a.gate_pitch + (size_t)h * a.gate_head + d;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) gate[i] = 1.0f + expf(-g[i]);
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   float m = -INFINITY, l = 0.0f;
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  auto add = [&](float2 v, float4 x) {
+  float acc[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
+  auto add = [&](float2 v, float4 x, float4 y) {
     const float mn = fmaxf(m, v.x), fo = exp2_approx(m - mn), fn = exp2_approx(v.x - mn);
+    const float z[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
     l = l * fo + v.y * fn;
-    acc.x = acc.x * fo + x.x * fn;
-    acc.y = acc.y * fo + x.y * fn;
-    acc.z = acc.z * fo + x.z * fn;
-    acc.w = acc.w * fo + x.w * fn;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = acc[i] * fo + z[i] * fn;
     m = mn;
   };
   if (some) {
@@ -795,33 +821,30 @@ __global__ void __launch_bounds__(1024, 1) tree_attn_tile_merge_kernel(const __g
     for (int c = c0 + share; c <= from.y; c += blockDim.y) {
       const size_t slot = c == c0 ? from.x : c * 2;
       const float2 v = a.part_ml[slot * kTileRows + r];
-      const float4 x = part[slot * (kTileRows * (size_t)D / 4)];
-      if (v.x != -INFINITY) add(v, x);
+      const float4 *p = part + slot * (kTileRows * (size_t)D / 4);
+      const float4 x = p[0], y = p[kTileRows];
+      if (v.x != -INFINITY) add(v, x, y);
     }
   }
   if (blockDim.y > 1) {
     if (share > 0) {
-      acc_s[share - 1][t] = acc;
+      acc_s[share - 1][0][t] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      acc_s[share - 1][1][t] = make_float4(acc[4], acc[5], acc[6], acc[7]);
       ml_s[share - 1][t] = make_float2(m, l);
     }
     __syncthreads();
     if (share > 0) return;
     for (int i = 0; i < (int)blockDim.y - 1; ++i)
-      if (ml_s[i][t].x != -INFINITY) add(ml_s[i][t], acc_s[i][t]);
+      if (ml_s[i][t].x != -INFINITY) add(ml_s[i][t], acc_s[i][0][t], acc_s[i][1][t]);
   }
   if (!live) return;
-  const int pos = a.positions[b];
   const bool there = some && (a.parents ? a.sights[(size_t)b * kTreeMaxNodes + n] != 0 : pos >= 0 && pos < a.max_seq - n);
-  const size_t node = (size_t)b * a.nodes + n;
-  float o[4] = {acc.x, acc.y, acc.z, acc.w};
   const float inv = 1.0f / l;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    o[i] = there ? o[i] * inv : 0.0f;
-    if (there && a.gate) o[i] /= 1.0f + expf(-a.gate[node * a.gate_pitch + (size_t)h * a.gate_head + d + i]);
-  }
-  *reinterpret_cast<uint2 *>(a.out + (node * a.q_heads + h) * D + d) =
-      make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+  for (int i = 0; i < 8; ++i) acc[i] = there ? acc[i] * inv / gate[i] : 0.0f;
+  *reinterpret_cast<uint4 *>(a.out + (node * a.q_heads + h) * D + d) =
+      make_uint4(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]), pack_bf16x2(acc[4], acc[5]),
+                 pack_bf16x2(acc[6], acc[7]));
 }
 
 template <int DP>
@@ -847,8 +870,7 @@ int launch(const TreeArgs &a, const TilePlan &p, cudaStream_t s) {
     return st;
   if (int st = encode_cache_u8(&v_map, a.v_codes, a.batch, a.max_seq, a.kv_heads, a.head_dim, Sh::kBox, Sh::BT))
     return st;
-  cudaError_t e = launch_pdl(tree_attn_prep_kernel, dim3((unsigned)(p.items * (kTileRows / kPrepRows))), 256, 0, s, a, p.BT,
-                             p.blocks);
+  cudaError_t e = launch_pdl(tree_attn_prep_kernel, dim3((unsigned)(p.items * (kTileRows / kPrepRows))), 256, 0, s, a);
   if (e != cudaSuccess) return cuda_fail(e, "tree_attn_prep_kernel");
   FPB_LAUNCH_CHECK("tree_attn_prep_kernel");
   e =
@@ -858,7 +880,7 @@ int launch(const TreeArgs &a, const TilePlan &p, cudaStream_t s) {
   // a row tile's blocks in one thread's loop while they are few
   const unsigned shares = (size_t)p.blocks > 16 * p.items ? kMergeShares : 1;
   e = launch_pdl(tree_attn_tile_merge_kernel,
-                 dim3((unsigned)(p.items * (kTileRows / 16)), (unsigned)((a.head_dim + 63) / 64)), dim3(256, shares), 0, s,
+                 dim3((unsigned)(p.items * (kTileRows / 16)), (unsigned)((a.head_dim + 127) / 128)), dim3(256, shares), 0, s,
                  a, p.BT);
   if (e != cudaSuccess) return cuda_fail(e, "tree_attn_tile_merge_kernel");
   FPB_LAUNCH_CHECK("tree_attn_tile_merge_kernel");
@@ -873,12 +895,11 @@ TilePlan tile_plan(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, 
   p.batch = batch;
   p.items = batch * kv_heads * ((nodes * (q_heads / kv_heads) + kTileRows - 1) / kTileRows);
   p.units = p.items * ((max_seq + p.BT - 1) / p.BT);
-  // (a prep block of eight warps finds eight shares: never more blocks than that)
-  p.blocks = (int)std::min({(size_t)sm_count(), p.units, p.items * (kTileRows / kPrepRows) * 8});
+  p.blocks = (int)std::min<size_t>(sm_count(), p.units);
   return p;
 }
 
-// The workspace: queries, partial results, sums, sights, factors, shares.
+// The workspace: queries, partial results, sums, sights, factors, items' shares.
 static size_t lay_out(TreeArgs *a, const TilePlan &p, size_t head_dim, void *workspace) {
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -895,7 +916,6 @@ static size_t lay_out(TreeArgs *a, const TilePlan &p, size_t head_dim, void *wor
   a->sights = reinterpret_cast<uint64_t *>(take(p.batch * kTreeMaxNodes * 8));
   a->q_fac = reinterpret_cast<float *>(take(p.items * kTileRows * 4));
   a->shares = reinterpret_cast<int2 *>(take(p.items * sizeof(int2)));
-  a->walks = take((size_t)p.blocks * sizeof(Walk));
   return at;
 }
 

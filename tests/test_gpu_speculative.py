@@ -237,6 +237,22 @@ def test_tree_attention(F, torch, b, n, hq, hk, d, s, pos, q_dtype):
     _check_attention(F, torch, rng, cache, pos, _tree(rng, b, n), n, hq, q_dtype)
 
 
+@pytest.mark.parametrize("tree", [False, True])
+def test_many_sessions_of_any_length_share_the_gpu(F, torch, tree):
+    """More sessions than a warp has lanes, from one token to some hundreds;
+    with trees, fifty are not there, the first forty among them."""
+    rng = np.random.default_rng(14)
+    b, n, s = 75, 20, 640
+    cache = _cache(F, torch, rng, b, s, 1, 32)
+    pos = rng.integers(0, s - n + 1, b).astype(np.int32)
+    pos[::7] = 0
+    par = _tree(rng, b, n) if tree else None
+    if tree:
+        par[:40, 0] = par[50:60, 0] = -2
+    _check_attention(F, torch, rng, cache, pos.tolist(), par, n, 2)
+    assert F.device_error(reset=True) == 0
+
+
 @pytest.mark.parametrize("n,pos", [(1, 0), (70, 0), (200, 57)])
 def test_chain_attention_is_causal(F, torch, n, pos):
     """parents None: a prompt's chunk, longer than a tree may be."""
