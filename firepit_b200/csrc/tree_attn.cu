@@ -23,58 +23,91 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// An 8 x 8 matrix of f16 pairs (lane 4 r + c: row r, columns 2 c and 2 c + 1), transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
 using namespace sm100;
 
 // ---- few rows: warps that stream tokens on their own -------------------------------------------
 // Block (split, session * kv head): NR rows (8 or 16) of one kv head, four
 // warps that take steps of 16 tokens in turn.  Each warp has its own ring of
-// kRowsStages steps of codes, filled by TMA (128-byte swizzle: its 16-byte
+// kStages steps of codes, filled by TMA (128-byte swizzle: its 16-byte
 // reads fall on distinct banks), so that 24 KB a warp are on their way however
 // long a step takes; nothing is shared between the warps before the end.
-//  S = Q K^T   m16n8k16, the rows as M (NR = 8 leaves half of it zero).  The
-//              order of the summed dimension is free as long as both sides
-//              agree, so a lane's 16-byte piece of a key (16 dimensions) is
-//              its operand of four instructions as it lies.
-//  O^T = V^T P^T  the dimensions as M, the rows as N: P^T's operand is S's
-//              result as it lies.  V's needs pairs of tokens in a word: byte
-//              permutes of two tokens' pieces before the conversion.
+//  S^T = K Q^T  m16n8k16, the tokens as M, the rows as N.  The order of the
+//               summed dimension is free as long as both sides agree, so a
+//               lane's 16-byte piece of a key (16 dimensions) is its operand
+//               of four instructions as it lies.
+//  O^T = V^T P^T  the dimensions as M, the rows as N: P^T's operand is S^T's
+//               result, transposed eight by eight.  V's needs pairs of tokens
+//               in a word: byte permutes of two tokens' pieces before the
+//               conversion.
+// Row i of an operand of eight is token token_at(i), and piece i of a value
+// piece_at(i): a quarter of a warp then reads 16 bytes from all of the banks.
 // Each e4m3 is converted to f16 (exact); the key's factor goes to the score,
 // the value's to the weight's exponent.
-constexpr int kRowsThreads = 128, kRowsWarps = 4, kRowsStages = 3;
+constexpr int kRowsThreads = 128, kRowsWarps = 4;
 constexpr int kErrRowsWait = 503;
+
+// Blocks an SM.  Their registers would allow three at 256 columns and eight
+// rows, and four at fewer columns, but more splits cost the merge what they
+// gain (1 x 30000, 256 columns: 20.7 us with two, 23.7 with three; 8 x 8192, 64
+// columns, 16 rows: 19.7 us with two, 17.7 with three, 18.3 with four).
+constexpr int rows_blocks(int DP) { return DP == 256 ? 2 : 3; }
 
 template <int DP, int NR>
 struct RowsShape {
+  static constexpr int kBlocks = rows_blocks(DP), kStages = 3;
   static constexpr bool kQShared = NR * DP > 16 * 128;  // 64 registers of queries are too many beside 128 of sums
   static constexpr int kQPitch = DP + 8;                // f16 elements: 16-byte reads of eight rows on distinct banks
   static constexpr int kBox = DP == 64 ? 64 : 128;
   static constexpr uint32_t kStage = 2 * 16 * DP;  // a step's codes, keys then values
-  static constexpr size_t kRing = (size_t)kRowsWarps * kRowsStages * kStage;
+  static constexpr size_t kRing = (size_t)kRowsWarps * kStages * kStage;
   static constexpr size_t kEnd = (size_t)kRowsWarps * NR * (DP + 2) * 4;  // the warps' results, over the ring
   static constexpr size_t kQueries = (size_t)NR * kQPitch * 2;
   static constexpr size_t smem = 1023 + (kRing > kEnd ? kRing : kEnd) + kQueries;
 };
 
+// Steps of a split: what the call's splits share of a session's, in whole
+// rounds of a block's warps; a session of few tokens leaves splits unused.
+__device__ __forceinline__ int steps_a_split(int steps, int splits) {
+  return ((steps + splits - 1) / splits + kRowsWarps - 1) / kRowsWarps * kRowsWarps;
+}
+
+template <int DP>
+__device__ __forceinline__ int token_at(int i) {
+  return DP == 64 ? i ^ ((i >> 1) & 1) : (i >> 1) | (i & 1) << 2;
+}
+template <int DP>
+__device__ __forceinline__ int piece_at(int i) {
+  return DP == 64 ? i : token_at<DP>(i);
+}
+
 template <int DP, int NR>
-__global__ void __launch_bounds__(kRowsThreads, 2)
+__global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
     tree_attn_rows_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap k_map,
                           const __grid_constant__ CUtensorMap v_map) {
   using Sh = RowsShape<DP, NR>;
-  constexpr int kPieces = DP / 64, kVPieces = DP >= 128 ? DP / 128 : 1, kVBytes = DP >= 128 ? 16 : 8;
+  constexpr int kStages = Sh::kStages, kPieces = DP / 64, kVPieces = DP >= 128 ? DP / 128 : 1, kVBytes = DP >= 128 ? 16 : 8;
   constexpr int kMT = DP / 16, kNT = NR / 8;
   extern __shared__ uint8_t raw_sm[];
   uint8_t *const ring = raw_sm + (-smem_u32(raw_sm) & 1023);  // the swizzle goes by the address
   float *const sm = reinterpret_cast<float *>(ring);  // at the end: the warps' results
   __half *const qs = reinterpret_cast<__half *>(ring + (Sh::kRing > Sh::kEnd ? Sh::kRing : Sh::kEnd));
-  __shared__ uint64_t full[kRowsWarps][kRowsStages];
+  __shared__ uint64_t full[kRowsWarps][kStages];
   __shared__ int abort_s;
   __shared__ float m_s[kRowsWarps][NR], l_s[kRowsWarps][NR];
   __shared__ float fac_s[NR];
+  __shared__ Sight sight_s[NR];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, c = lane & 3;
   const int rows = a.nodes * a.group;
   const int item = blockIdx.y, b = item / a.kv_heads, kvh = item % a.kv_heads, D = a.head_dim;
   if (lane == 0) {
-    for (int i = 0; i < kRowsStages; ++i) mbar_init(&full[w][i], 1);
+    for (int i = 0; i < kStages; ++i) mbar_init(&full[w][i], 1);
     if (w == 0) abort_s = 0;
     fence_barrier_init();
   }
@@ -84,15 +117,16 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   const bool tree = a.parents != nullptr;
   const int total = seen_rows(a, pos, a.nodes - 1);
   // this split's tokens, in whole steps
-  const int steps = (total + 15) / 16, per = (steps + a.splits - 1) / a.splits;
+  const int steps = (total + 15) / 16, per = steps_a_split(steps, a.splits);
   const int s0 = blockIdx.x * per, s1 = min(steps, s0 + per);
+  if (blockIdx.x > 0 && s0 >= steps) return;
 
   // the ring's first steps are on their way before anything else
   const int first = s0 + w, boxes = (D + Sh::kBox - 1) / Sh::kBox;
-  uint8_t *const mine_ring = ring + (size_t)w * kRowsStages * Sh::kStage;
+  uint8_t *const mine_ring = ring + (size_t)w * kStages * Sh::kStage;
   auto fetch = [&](int i) {  // the warp's i-th step, one lane
-    uint8_t *to = mine_ring + (i % kRowsStages) * Sh::kStage;
-    uint64_t *bar = &full[w][i % kRowsStages];
+    uint8_t *to = mine_ring + (i % kStages) * Sh::kStage;
+    uint64_t *bar = &full[w][i % kStages];
     const int t0 = (first + i * kRowsWarps) * 16;
     mbar_arrive_expect_tx(bar, 2u * boxes * (16 * Sh::kBox));
     for (int x = 0; x < boxes; ++x) {
@@ -102,7 +136,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   };
   const int count = first < s1 ? (s1 - first + kRowsWarps - 1) / kRowsWarps : 0;
   if (lane == 0)
-    for (int i = 0; i < min(count, kRowsStages); ++i) fetch(i);
+    for (int i = 0; i < min(count, kStages); ++i) fetch(i);
   __syncwarp();
 
   // queries: a warp takes rows w, w + 4, ...; eight columns a lane
@@ -130,17 +164,18 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     }
     if (lane == 0) fac_s[r] = pow2i(e) * a.scale_log2;
   }
-  __syncthreads();
-  // the lane's rows of S: g and, with 16 rows, g + 8
-  Sight sight[kNT];
-  float fac[kNT];
-#pragma unroll
-  for (int i = 0; i < kNT; ++i) {
-    const int row = g + 8 * i;
-    sight[i] = sight_of(a, b, row < rows ? row / a.group : a.nodes, pos);
-    fac[i] = fac_s[g + 8 * i];
+  if (w == 0) {
+    const Sight s = sight_of(a, b, lane < rows ? lane / a.group : a.nodes, pos);
+    if (lane < NR) sight_s[lane] = s;
   }
-  // Q operands of piece p: row's dimensions 64 p + 16 c + [0, 16)
+  __syncthreads();
+  // the lane's rows: 2 c, 2 c + 1 and, with 16 rows, those + 8
+  float fac[kNT][2];
+#pragma unroll
+  for (int i = 0; i < kNT; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) fac[i][e] = fac_s[8 * i + 2 * c + e];
+  // Q operands of piece p: row g (+ 8 i)'s dimensions 64 p + 16 c + [0, 16)
   uint32_t qr[Sh::kQShared ? 1 : kPieces * kNT * 8];
   if constexpr (!Sh::kQShared) {
 #pragma unroll
@@ -155,10 +190,17 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
         }
   }
 
-  const uint8_t *ex = (lane < 16 ? a.k_exp : a.v_exp) + (size_t)b * a.max_seq * a.kv_heads + kvh;
-  auto load_exp = [&](int step) -> uint32_t {
-    const int t = step * 16 + (lane & 15);
-    return t < total ? ex[(size_t)t * a.kv_heads] : 127;
+  // the exponents of the lane's tokens, token_at(g) and that + 8
+  const int own = token_at<DP>(g);
+  const size_t ex0 = (size_t)b * a.max_seq * a.kv_heads + kvh;
+  auto load_exps = [&](int step, uint32_t(&x)[4]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int t = step * 16 + own + 8 * h;
+      const size_t at = ex0 + (size_t)t * a.kv_heads;
+      x[h] = t < total ? a.k_exp[at] : 127;
+      x[2 + h] = t < total ? a.v_exp[at] : 127;
+    }
   };
 
   float acc[kMT][kNT][4];
@@ -168,158 +210,169 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     for (int j = 0; j < kNT; ++j)
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[i][j][k] = 0.0f;
-  float m[kNT], l[kNT];
+  float m[kNT][2], l[kNT][2];
 #pragma unroll
-  for (int i = 0; i < kNT; ++i) {
-    m[i] = -INFINITY;
-    l[i] = 0.0f;
-  }
-  uint32_t xr = count > 0 ? load_exp(first) : 127;
+  for (int i = 0; i < kNT; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      m[i][e] = -INFINITY;
+      l[i][e] = 0.0f;
+    }
+  uint32_t xr[4] = {127, 127, 127, 127};
+  if (count > 0) load_exps(first, xr);
   bool ok = true;
   for (int i = 0; i < count; ++i) {
     const int step = first + i * kRowsWarps;
-    const uint8_t *kst = mine_ring + (i % kRowsStages) * Sh::kStage, *vst = kst + Sh::kStage / 2;
-    if (ok) ok = mbar_wait(&full[w][i % kRowsStages], (i / kRowsStages) & 1, &abort_s);
+    const uint8_t *kst = mine_ring + (i % kStages) * Sh::kStage, *vst = kst + Sh::kStage / 2;
+    if (ok) ok = mbar_wait(&full[w][i % kStages], (i / kStages) & 1, &abort_s);
     if (!ok && a.error) {  // (a wait that ran out: the results are void, but the loop ends)
       *(volatile int *)&abort_s = 1;
       atomicCAS(a.error, 0, kErrRowsWait);
     }
     __syncwarp();
-    // scores of 16 tokens: s[u] tokens 8 u + 2 c, 2 c + 1 of row g (and g + 8)
-    float s[2][4];
+    // scores of 16 tokens: s[i][.][2 h + e] token token_at(g) + 8 h, row 2 c + e + 8 i,
+    // with eight rows in two sums that do not wait for one another
+    constexpr int kChains = NR == 8 ? 2 : 1;
+    float s[kNT][kChains][4];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int i = 0; i < kNT; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s[u][k] = 0.0f;
+      for (int u = 0; u < kChains; ++u)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[i][u][k] = 0.0f;
 #pragma unroll
     for (int p = 0; p < kPieces; ++p) {
-      uint32_t q0[8], q1[8];
+      uint32_t kw[2][4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) q1[j] = 0;
-      if constexpr (Sh::kQShared) {
+      for (int h = 0; h < 2; ++h) {
+        const int at = DP == 64 ? (8 * h + own) * 64 + ((c ^ ((own >> 1) & 3)) * 16)
+                                : (p >> 1) * 2048 + (8 * h + own) * 128 + (((4 * (p & 1) + c) ^ own) * 16);
+        const uint4 kv = *reinterpret_cast<const uint4 *>(kst + at);
+        kw[h][0] = kv.x; kw[h][1] = kv.y; kw[h][2] = kv.z; kw[h][3] = kv.w;
+      }
+      uint32_t q[kNT][8];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint4 v = *reinterpret_cast<const uint4 *>(qs + g * Sh::kQPitch + 64 * p + 16 * c + 8 * j);
-          q0[4 * j] = v.x; q0[4 * j + 1] = v.y; q0[4 * j + 2] = v.z; q0[4 * j + 3] = v.w;
-          if constexpr (NR == 16) {
-            const uint4 y = *reinterpret_cast<const uint4 *>(qs + (g + 8) * Sh::kQPitch + 64 * p + 16 * c + 8 * j);
-            q1[4 * j] = y.x; q1[4 * j + 1] = y.y; q1[4 * j + 2] = y.z; q1[4 * j + 3] = y.w;
+      for (int i = 0; i < kNT; ++i) {
+        if constexpr (Sh::kQShared) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(qs + (g + 8 * i) * Sh::kQPitch + 64 * p + 16 * c + 8 * j);
+            q[i][4 * j] = v.x; q[i][4 * j + 1] = v.y; q[i][4 * j + 2] = v.z; q[i][4 * j + 3] = v.w;
           }
-        }
-      } else {
+        } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          q0[j] = qr[p * kNT * 8 + j];
-          if constexpr (NR == 16) q1[j] = qr[(p * kNT + 1) * 8 + j];
+          for (int j = 0; j < 8; ++j) q[i][j] = qr[(p * kNT + i) * 8 + j];
         }
       }
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int at = DP == 64 ? (8 * u + g) * 64 + ((c ^ ((g >> 1) & 3)) * 16)
-                                : (p >> 1) * 2048 + (8 * u + g) * 128 + (((4 * (p & 1) + c) ^ g) * 16);
-        const uint4 kv = *reinterpret_cast<const uint4 *>(kst + at);
-        const uint32_t kw[4] = {kv.x, kv.y, kv.z, kv.w};
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)kw[0][j]), a1 = e4m3x2_to_f16x2((uint16_t)kw[1][j]),
+                       a2 = e4m3x2_to_f16x2((uint16_t)(kw[0][j] >> 16)), a3 = e4m3x2_to_f16x2((uint16_t)(kw[1][j] >> 16));
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          mma_f16(s[u], q0[2 * j], q1[2 * j], q0[2 * j + 1], q1[2 * j + 1], e4m3x2_to_f16x2((uint16_t)kw[j]),
-                  e4m3x2_to_f16x2((uint16_t)(kw[j] >> 16)));
+        for (int i = 0; i < kNT; ++i) mma_f16(s[i][j % kChains], a0, a1, a2, a3, q[i][2 * j], q[i][2 * j + 1]);
       }
     }
-    const uint32_t xb = xr;
+    if constexpr (kChains == 2) {
+#pragma unroll
+      for (int i = 0; i < kNT; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[i][0][k] += s[i][1][k];
+    }
     const int t0 = step * 16;
     const bool open = t0 + 16 > pos;  // warp-uniform: the tree's rows, or the end
-    if (i + 1 < count) xr = load_exp(step + kRowsWarps);
+    float kf[2], ve[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      kf[h] = kv8_factor(xr[h]);
+      ve[h] = kv8_value_exponent(xr[2 + h]);
+    }
+    if (i + 1 < count) load_exps(step + kRowsWarps, xr);
     uint32_t vr[4][kVPieces][kVBytes / 4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const int row = 2 * c + (t & 1) + 8 * (t >> 1);
+      const int row = token_at<DP>(2 * c + (t & 1)) + 8 * (t >> 1), at = piece_at<DP>(g);
 #pragma unroll
       for (int p = 0; p < kVPieces; ++p) {
         if constexpr (kVBytes == 16) {
-          const uint4 v = *reinterpret_cast<const uint4 *>(vst + p * 2048 + row * 128 + ((g ^ (row & 7)) * 16));
+          const uint4 v = *reinterpret_cast<const uint4 *>(vst + p * 2048 + row * 128 + ((at ^ (row & 7)) * 16));
           vr[t][p][0] = v.x; vr[t][p][1] = v.y; vr[t][p][2] = v.z; vr[t][p][3] = v.w;
         } else {
-          const uint2 v = *reinterpret_cast<const uint2 *>(vst + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) * 16) + (g & 1) * 8);
+          const uint2 v = *reinterpret_cast<const uint2 *>(vst + row * 64 + (((at >> 1) ^ ((row >> 1) & 3)) * 16) + (at & 1) * 8);
           vr[t][p][0] = v.x; vr[t][p][1] = v.y;
         }
       }
     }
-    uint32_t nan[4] = {0, 0, 0, 0};
+    bool nan[2] = {false, false};  // of the lane's tokens
     if (open) {  // a value vector that some row does not see must not reach it through 0 * NaN
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int t = 0; t < 4; ++t) {
+        uint32_t any = 0;
 #pragma unroll
         for (int p = 0; p < kVPieces; ++p)
 #pragma unroll
           for (int j = 0; j < kVBytes / 4; ++j) {
-            const uint32_t bad = __vcmpeq4(vr[i][p][j] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-            vr[i][p][j] &= ~bad;
-            nan[i] |= bad;
+            const uint32_t bad = __vcmpeq4(vr[t][p][j] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            vr[t][p][j] &= ~bad;
+            any |= bad;
           }
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) nan[i] |= __shfl_xor_sync(0xffffffffu, nan[i], o);
+        // operand row 2 c + t % 2 (+ 8) lies over the lanes of this c
+        const uint32_t lanes = __ballot_sync(0xffffffffu, any != 0) & (0x11111111u << (g >> 1));
+        if ((g & 1) == (t & 1) && lanes) nan[t >> 1] = true;
       }
     }
-    // y = score + the value's exponent, and the rows' maxima
-    float y[kNT][4], ve[4], mx[kNT];
-#pragma unroll
-    for (int i = 0; i < kNT; ++i) mx[i] = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int u = k >> 1, e = k & 1, tl = 8 * u + 2 * c + e, t = t0 + tl;
-      const float kf = kv8_factor(__shfl_sync(0xffffffffu, xb, tl));
-      ve[k] = kv8_value_exponent(__shfl_sync(0xffffffffu, xb, 16 + tl));
-#pragma unroll
-      for (int i = 0; i < kNT; ++i) {
-        float v = fmaf(s[u][2 * i + e], kf * fac[i], ve[k]);
-        if (open) {
-          if (nan[k]) v = __int_as_float(0x7fc00000);
-          if (t >= total || !sight[i].sees(t, pos, tree)) v = -INFINITY;
-        }
-        y[i][k] = v;
-        mx[i] = fmaxf(mx[i], v);
-      }
-    }
+    // y = score + the value's exponent
+    float y[kNT][2][2];  // row, token
     bool grow = false;
 #pragma unroll
-    for (int i = 0; i < kNT; ++i) {
-      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-      grow |= mx[i] > m[i] + kLag || (m[i] == -INFINITY && mx[i] > m[i]);
-    }
-    if (__any_sync(0xffffffffu, grow)) {
-      float old[kNT];
+    for (int i = 0; i < kNT; ++i)
 #pragma unroll
-      for (int i = 0; i < kNT; ++i) {
-        const float mn = fmaxf(m[i], mx[i]);
-        old[i] = m[i] == -INFINITY ? 0.0f : exp2_approx(m[i] - mn);
-        l[i] *= old[i];
-        m[i] = mn;
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v = fmaf(s[i][0][2 * h + e], kf[h] * fac[i][e], ve[h]);
+          if (open) {
+            const int t = t0 + own + 8 * h;
+            if (nan[h]) v = __int_as_float(0x7fc00000);
+            if (t >= total || !sight_s[8 * i + 2 * c + e].sees(t, pos, tree)) v = -INFINITY;
+          }
+          y[i][e][h] = v;
+        }
+        grow |= fmaxf(y[i][e][0], y[i][e][1]) > m[i][e] + kLag;
       }
+    if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-      for (int j = 0; j < kNT; ++j)  // the sums hold rows 2 c, 2 c + 1 (+ 8 j): their factors are lanes 8 c and 8 c + 4's
+      for (int i = 0; i < kNT; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float f = __shfl_sync(0xffffffffu, old[j], 8 * c + 4 * e);
+          float mn = fmaxf(m[i][e], fmaxf(y[i][e][0], y[i][e][1]));
 #pragma unroll
-          for (int i = 0; i < kMT; ++i) {
-            acc[i][j][e] *= f;
-            acc[i][j][2 + e] *= f;
+          for (int o = 4; o < 32; o <<= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+          const float old = m[i][e] == -INFINITY ? 0.0f : exp2_approx(m[i][e] - mn);
+          l[i][e] *= old;
+          m[i][e] = mn;
+#pragma unroll
+          for (int k = 0; k < kMT; ++k) {
+            acc[k][i][e] *= old;
+            acc[k][i][2 + e] *= old;
           }
         }
     }
     uint32_t pb[kNT][2];
+    const float vi[2] = {pow2i(-(int)ve[0]), pow2i(-(int)ve[1])};
 #pragma unroll
     for (int i = 0; i < kNT; ++i) {
-      const float base = m[i] == -INFINITY ? 0.0f : kHead - m[i];
-      float p[4];
+      float p[2][2];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        p[k] = exp2_approx(y[i][k] + base);
-        l[i] = fmaf(p[k], pow2i(-(int)ve[k]), l[i]);
+      for (int e = 0; e < 2; ++e) {
+        const float base = m[i][e] == -INFINITY ? 0.0f : kHead - m[i][e];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          p[e][h] = exp2_approx(y[i][e][h] + base);
+          l[i][e] = fmaf(p[e][h], vi[h], l[i][e]);
+        }
       }
-      pb[i][0] = pack_f16x2(p[0], p[1]);
-      pb[i][1] = pack_f16x2(p[2], p[3]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) pb[i][h] = transposed(pack_f16x2(p[0][h], p[1][h]));
     }
 #pragma unroll
     for (int p = 0; p < kVPieces; ++p)
@@ -339,25 +392,27 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
         }
       }
     __syncwarp();  // the stage is read
-    if (lane == 0 && i + kRowsStages < count) fetch(i + kRowsStages);
+    if (lane == 0 && i + kStages < count) fetch(i + kStages);
     __syncwarp();
   }
   if (!ok)  // copies still in flight land before the block ends
-    for (int i = 0; i < kRowsStages; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       int never = 0;
       for (uint32_t k = 0; k < 2; ++k) mbar_wait(&full[w][i], k, &never);
     }
 
   // the warps' results meet: maxima, then sums over one maximum in warp order
 #pragma unroll
-  for (int i = 0; i < kNT; ++i) {
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    if (c == 0) {
-      m_s[w][g + 8 * i] = m[i];
-      l_s[w][g + 8 * i] = l[i];
+  for (int i = 0; i < kNT; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], o);
+      if (g == 0) {
+        m_s[w][8 * i + 2 * c + e] = m[i][e];
+        l_s[w][8 * i + 2 * c + e] = l[i][e];
+      }
     }
-  }
   __syncthreads();  // also: every warp is done with the queries that `sm` held
   float *mine = sm + (size_t)w * NR * (DP + 2);
 #pragma unroll
@@ -368,7 +423,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
       for (int i = 0; i < kNT; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int mt = (p * kVBytes / 4 + j) * 2, d = 128 * p + kVBytes * g + 4 * j;
+          const int mt = (p * kVBytes / 4 + j) * 2, d = 128 * p + kVBytes * piece_at<DP>(g) + 4 * j;
           float *o = mine + (size_t)(8 * i + 2 * c + e) * (DP + 2) + d;
           *reinterpret_cast<float2 *>(o) = make_float2(acc[mt][i][e], acc[mt][i][2 + e]);
           *reinterpret_cast<float2 *>(o + 2) = make_float2(acc[mt + 1][i][e], acc[mt + 1][i][2 + e]);
@@ -386,7 +441,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
       lt += l_s[x][r] * f[x];
     }
     const int n = row / a.group, h = kvh * a.group + row % a.group;
-    const bool there = sight_of(a, b, n, pos).upto >= 0;
+    const bool there = sight_s[r].upto >= 0;
     for (int d = lane * 2; d < D; d += 64) {
       float2 o = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -415,50 +470,71 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   }
 }
 
-// The splits of a row meet: one warp a (session, node, query head), the
-// splits in order.
-__global__ void __launch_bounds__(256) tree_attn_merge_kernel(const __grid_constant__ TreeArgs a, int NR, int count) {
-  pdl_enter();
-  const int lane = threadIdx.x & 31, i = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (i >= count) return;
-  const int h = i % a.q_heads, node = i / a.q_heads, b = node / a.nodes, n = node % a.nodes, D = a.head_dim;
-  const int kvh = h / a.group, row = n * a.group + h % a.group;
-  const int tiles = (a.nodes * a.group + NR - 1) / NR;
-  const size_t item = ((size_t)b * a.kv_heads + kvh) * tiles + row / NR;
-  const int r = row % NR, pos = a.positions[b];
+// The splits of a row (session, node, query head) meet, in order: blockDim.y
+// warps a row and 128 columns share them, four columns a lane.  What the rows
+// kernel does not write is read before it is waited for.
+constexpr int kMergeWarps = 16;
+__global__ void __launch_bounds__(kMergeWarps * 32, 2) tree_attn_merge_kernel(const __grid_constant__ TreeArgs a, int NR,
+                                                                            int count) {
+  __shared__ float4 acc_s[kMergeWarps][32];
+  __shared__ float l_s[kMergeWarps];
+  const int lane = threadIdx.x, share = threadIdx.y, shares = blockDim.y, w = threadIdx.z * shares + share;
+  const int i = blockIdx.x * blockDim.z + threadIdx.z, d = blockIdx.y * 128 + lane * 4, D = a.head_dim;
+  const bool in = i < count;
+  const int h = i % a.q_heads, node = in ? i / a.q_heads : 0, b = node / a.nodes, n = node % a.nodes;
+  const int kvh = h / a.group, r = n * a.group + h % a.group, pos = a.positions[b];
+  const size_t slot0 = ((size_t)b * a.kv_heads + kvh) * a.splits * NR + r;
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int steps = (seen_rows(a, pos, a.nodes - 1) + 15) / 16, per = max(1, steps_a_split(steps, a.splits));
+  const int splits = max(1, (steps + per - 1) / per);
   const bool there = sight_of(a, b, n, pos).upto >= 0;
-  const float2 *ml = a.part_ml + item * a.splits * NR + r;
-  float m = -INFINITY, l = 0.0f;
-  for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, ml[(size_t)s * NR].x);
-  m = warp_max(m);
-  float acc[8];
+  float gate[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (there && a.gate && d < D && share == 0) {
+    const float *g = a.gate + (size_t)node * a.gate_pitch + (size_t)h * a.gate_head + d;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
-  const int d = lane * 8;
-  for (int s = 0; s < a.splits; ++s) {
+    for (int k = 0; k < 4; ++k) gate[k] = expf(-g[k]);
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const float2 *ml = a.part_ml + slot0;
+  float m = -INFINITY, l = 0.0f;
+  for (int s = lane; s < splits; s += 32) m = fmaxf(m, ml[(size_t)s * NR].x);
+  m = warp_max(m);
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto add = [&](float4 x, float f) {
+    acc.x = fmaf(x.x, f, acc.x);
+    acc.y = fmaf(x.y, f, acc.y);
+    acc.z = fmaf(x.z, f, acc.z);
+    acc.w = fmaf(x.w, f, acc.w);
+  };
+  const float *part = a.part + slot0 * D + (d < D ? d : 0);
+#pragma unroll 4
+  for (int s = share; s < splits; s += shares) {
     const float2 v = ml[(size_t)s * NR];
+    const float4 x = *reinterpret_cast<const float4 *>(part + (size_t)s * NR * D);
     const float f = v.x == -INFINITY ? 0.0f : exp2_approx(v.x - m);
     l = fmaf(v.y, f, l);
-    if (d < D && f != 0.0f) {
-      const float4 *p = reinterpret_cast<const float4 *>(a.part + ((item * a.splits + s) * NR + r) * D + d);
-      const float4 x = p[0], z = p[1];
-      acc[0] = fmaf(x.x, f, acc[0]); acc[1] = fmaf(x.y, f, acc[1]);
-      acc[2] = fmaf(x.z, f, acc[2]); acc[3] = fmaf(x.w, f, acc[3]);
-      acc[4] = fmaf(z.x, f, acc[4]); acc[5] = fmaf(z.y, f, acc[5]);
-      acc[6] = fmaf(z.z, f, acc[6]); acc[7] = fmaf(z.w, f, acc[7]);
+    add(x, f);
+  }
+  if (shares > 1) {
+    if (share > 0) {
+      acc_s[w][lane] = acc;
+      if (lane == 0) l_s[w] = l;
+    }
+    __syncthreads();
+    if (share > 0) return;
+    for (int k = w + 1; k < w + shares; ++k) {
+      add(acc_s[k][lane], 1.0f);
+      l += l_s[k];
     }
   }
-  if (d >= D) return;
-  const float inv = 1.0f / l;
+  if (!in || d >= D) return;
+  const float inv = there ? 1.0f / l : 0.0f;
+  const float x[4] = {acc.x, acc.y, acc.z, acc.w};
+  float o[4];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    acc[k] = there ? acc[k] * inv : 0.0f;
-    if (there && a.gate)
-      acc[k] /= 1.0f + expf(-a.gate[(size_t)node * a.gate_pitch + (size_t)h * a.gate_head + d + k]);
-  }
-  *reinterpret_cast<uint4 *>(a.out + ((size_t)node * a.q_heads + h) * D + d) =
-      make_uint4(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]), pack_bf16x2(acc[4], acc[5]),
-                 pack_bf16x2(acc[6], acc[7]));
+  for (int k = 0; k < 4; ++k) o[k] = there ? x[k] * inv / (1.0f + gate[k]) : 0.0f;
+  *reinterpret_cast<uint2 *>(a.out + ((size_t)node * a.q_heads + h) * D + d) =
+      make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
 }
 
 // How a call of few rows is cut: rows a tile, tiles, splits of the tokens.
@@ -470,13 +546,14 @@ struct Plan {
 // Rows a key/value head from which the tcgen05 kernel takes over.
 bool wants_tiles(size_t nodes, size_t q_heads, size_t kv_heads) { return nodes * (q_heads / kv_heads) > 16; }
 
-Plan plan_for(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, size_t max_seq) {
+Plan plan_for(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, size_t head_dim, size_t max_seq) {
   Plan p{};
   const size_t rows = nodes * (q_heads / kv_heads);
   p.rows_tile = rows <= 8 ? 8 : 16;
   p.items = batch * kv_heads;
-  // two blocks an SM; at least 64 tokens a split (a step for each warp)
-  const size_t want = std::max<size_t>(1, (size_t)sm_count() * 2 / p.items);  // one wave
+  // one wave of blocks; at least 64 tokens a split (a step for each warp)
+  const size_t resident = (size_t)sm_count() * rows_blocks(head_dim <= 128 ? 128 : 256);
+  const size_t want = std::max<size_t>(1, resident / p.items);
   p.splits = (int)std::max<size_t>(1, std::min(want, (max_seq + 63) / 64));
   return p;
 }
@@ -518,7 +595,7 @@ extern "C" size_t fpb_tree_attn_workspace_bytes(size_t batch, size_t nodes, size
   if (batch == 0 || nodes == 0 || kv_heads == 0 || q_heads == 0 || q_heads % kv_heads) return 16;
   if (wants_tiles(nodes, q_heads, kv_heads))
     return tile_workspace_bytes(tile_plan(batch, nodes, q_heads, kv_heads, head_dim, max_seq), head_dim);
-  const Plan p = plan_for(batch, nodes, q_heads, kv_heads, max_seq);
+  const Plan p = plan_for(batch, nodes, q_heads, kv_heads, head_dim, max_seq);
   return p.splits == 1 ? 16 : p.items * p.splits * p.rows_tile * (head_dim + 2) * sizeof(float);
 }
 
@@ -578,7 +655,7 @@ extern "C" int fpb_tree_attn(const void *q, int q_dtype, size_t q_pitch, size_t 
                   "tiles of tokens)", p.items);
     return run_tree_tiles(a, p, workspace, s);
   }
-  const Plan p = plan_for(batch, nodes, q_heads, kv_heads, max_seq);
+  const Plan p = plan_for(batch, nodes, q_heads, kv_heads, head_dim, max_seq);
   if (p.items > 65535) return fail(FPB_ERR_SHAPE, "fpb_tree_attn: %zu key/value heads in one call", p.items);
   a.splits = p.splits;
   a.part = static_cast<float *>(workspace);
@@ -589,8 +666,15 @@ extern "C" int fpb_tree_attn(const void *q, int q_dtype, size_t q_pitch, size_t 
                                    : (few ? run_rows<256, 8>(a, p, s) : run_rows<256, 16>(a, p, s));
   if (st || p.splits == 1) return st;
   const int count = (int)(batch * nodes * q_heads);
-  cudaError_t e = launch_pdl(tree_attn_merge_kernel, dim3((unsigned)((count + 7) / 8)), 256, 0, s, a, p.rows_tile,
-                             count);
+  // as many warps a row as it has splits, while all of them run at once
+  const unsigned halves = head_dim > 128 ? 2 : 1;
+  unsigned shares = 1;
+  while (shares < (unsigned)kMergeWarps && 2 * shares <= (unsigned)p.splits &&
+         2 * shares * halves * (size_t)count <= (size_t)sm_count() * 16)
+    shares *= 2;
+  const unsigned per = std::max(1u, 8 / shares);
+  cudaError_t e = launch_pdl(tree_attn_merge_kernel, dim3((unsigned)((count + per - 1) / per), halves),
+                             dim3(32, shares, per), 0, s, a, p.rows_tile, count);
   if (e != cudaSuccess) return cuda_fail(e, "tree_attn_merge_kernel");
   FPB_LAUNCH_CHECK("tree_attn_merge_kernel");
   return FPB_OK;
