@@ -247,6 +247,55 @@ __device__ __noinline__ float2 raise_max(TileShared *sh, uint32_t s_tmem, uint32
   return make_float2(mn, old);
 }
 
+// O of a row tile's share to its slot: four columns of 128 rows lie together, so
+// that a warp stores 512 bytes.
+__device__ __noinline__ void write_part(const TreeArgs &a, size_t slot, uint32_t o_tmem) {
+  const int part = threadIdx.x >> 7, r_own = threadIdx.x & 127, D = a.head_dim;
+  float4 *o = reinterpret_cast<float4 *>(a.part) + slot * (kTileRows * (size_t)D / 4) + r_own;
+  for (int d = 16 * part; d < D; d += 16 * kParts) {
+    uint32_t r[16];
+    tmem_ld16(o_tmem + d, r);
+    tmem_ld_wait(r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      o[(size_t)(d / 4 + i) * kTileRows] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]),
+                                                       __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
+  }
+}
+
+// The same to `out`, divided by the row's sum, with the gate.
+__device__ __noinline__ void write_rows(const TreeArgs &a, TileShared *sh, uint32_t o_tmem) {
+  const int part = threadIdx.x >> 7, r_own = threadIdx.x & 127, D = a.head_dim;
+  const int row = sh->seg.rt * kTileRows + r_own, n = row / a.group, h = sh->seg.kvh * a.group + row % a.group;
+  const size_t node = (size_t)sh->seg.b * a.nodes + n;
+  const bool live = n < a.nodes, there = sh->sight[r_own] != 0;
+  float l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) l += sh->red[i][r_own];
+  const float inv = 1.0f / l;
+  __nv_bfloat16 *o = a.out + (node * a.q_heads + h) * D;
+  const float *gate = a.gate ? a.gate + node * a.gate_pitch + (size_t)h * a.gate_head : nullptr;
+#pragma unroll 1
+  for (int d = 16 * part; d < D; d += 16 * kParts) {
+    uint32_t r[16];
+    tmem_ld16(o_tmem + d, r);
+    tmem_ld_wait(r);
+    if (live) {
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        x[i] = there ? __uint_as_float(r[i]) * inv : 0.0f;
+        if (there && gate) x[i] /= 1.0f + expf(-gate[d + i]);
+      }
+      uint4 *to = reinterpret_cast<uint4 *>(o + d);
+      to[0] = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+      to[1] = make_uint4(pack_bf16x2(x[8], x[9]), pack_bf16x2(x[10], x[11]), pack_bf16x2(x[12], x[13]),
+                         pack_bf16x2(x[14], x[15]));
+    }
+    __syncwarp();
+  }
+}
+
 // What the tile kernel reads at its start, made by blocks of 32 rows of a row
 // tile (eight warps): the queries as f16 in the order of its TMEM stores
 // [item][eight columns][128 rows], each row scaled by a power of two into f16's
@@ -513,36 +562,31 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       float l0, l1;
       unpack2(l2, l0, l1);
+      // A row tile that this block has whole is finished here.  Of the others a
+      // block has two at most: the end of one (slot 0) and the start of another.
+      const bool whole = j0 == 0 && sh->seg.ends;
       const size_t slot = (size_t)blockIdx.x * 2 + (seg ? 1 : 0);
       sh->red[part][r_own] = l0 + l1;
       quad_sync(quad);
-      if (part == 0) {
+      if (part == 0 && !whole) {
         float l = 0.0f;
 #pragma unroll
         for (int i = 0; i < kParts; ++i) l += sh->red[i][r_own];
         a.part_ml[slot * kTileRows + r_own] = make_float2(j1 > j0 ? m : -INFINITY, l);
-        // whose slots hold the row tile: from its first block's to its last's
-        if (r_own == 0 && j0 == 0) a.shares[sh->seg.item].x = (int)slot;
-        if (r_own == 0 && sh->seg.ends) a.shares[sh->seg.item].y = (int)blockIdx.x;
+      }
+      if (tid == 0) {  // whose slots hold the row tile: from its first block's to its last's
+        if (j0 == 0) a.shares[sh->seg.item].x = whole ? -1 : (int)slot;
+        if (sh->seg.ends) a.shares[sh->seg.item].y = (int)blockIdx.x;
       }
       if (j1 > j0) {
         if (ok) ok = mbar_wait(&sh->vempty[(g - 1) % ST], ((g - 1) / ST) & 1, abort_s);
         if (!ok) give_up(a.error, abort_s);
         __syncwarp();
         tc_fence_after();
-        // four columns of 128 rows lie together: a warp stores 512 bytes
-        const int D = a.head_dim;
-        float4 *o = reinterpret_cast<float4 *>(a.part) + slot * (kTileRows * (size_t)D / 4) + r_own;
-        for (int d = 16 * part; d < D; d += 16 * kParts) {
-          uint32_t r[16];
-          tmem_ld16(my + Sh::kTmemO + d, r);
-          tmem_ld_wait(r);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            o[(size_t)(d / 4 + i) * kTileRows] =
-                make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]), __uint_as_float(r[4 * i + 2]),
-                            __uint_as_float(r[4 * i + 3]));
-        }
+        if (whole)
+          write_rows(a, sh, my + Sh::kTmemO);
+        else
+          write_part(a, slot, my + Sh::kTmemO);
       }
       soft_sync();  // O, red and the segment are read: the next may overwrite them
     }
@@ -772,7 +816,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
 // The blocks that share a row tile's tokens meet, in order, with the gate:
 // block (16 rows of a row tile, 128 columns); thread (row, eight columns, share
-// of the blocks).  Rows of nodes that are not there become zeros.  What the
+// of the blocks).  Rows of nodes that are not there become zeros, and those of
+// sessions that no block has.  What the
 // tile kernel does not write is read before it is waited for.
 constexpr int kMergeShares = 4;
 __global__ void __launch_bounds__(1024, 1) tree_attn_tile_merge_kernel(const __grid_constant__ TreeArgs a, int BT) {
@@ -813,8 +858,9 @@ __global__ void __launch_bounds__(1024, 1) tree_attn_tile_merge_kernel(const __g
     for (int i = 0; i < 8; ++i) acc[i] = acc[i] * fo + z[i] * fn;
     m = mn;
   };
+  const int2 from = some ? a.shares[item] : make_int2(0, -1);  // its first slot, its last block
+  if (from.x < 0) return;                                      // one block had it whole
   if (some) {
-    const int2 from = a.shares[item];  // its first slot, its last block
     const float4 *part = reinterpret_cast<const float4 *>(a.part) + (size_t)(live ? d / 4 : 0) * kTileRows + r;
     const int c0 = from.x >> 1;
 #pragma unroll 4

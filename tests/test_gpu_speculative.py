@@ -253,6 +253,20 @@ def test_many_sessions_of_any_length_share_the_gpu(F, torch, tree):
     assert F.device_error(reset=True) == 0
 
 
+@pytest.mark.parametrize("tree,d,gate", [(False, 32, True), (True, 128, False), (True, 208, True)])
+def test_more_heads_and_sessions_than_blocks(F, torch, tree, d, gate):
+    """Three hundred key heads with a tile or two of tokens each: a block
+    takes several of them whole."""
+    rng = np.random.default_rng(15)
+    b, n, hk, s = 75, 5, 4, 150
+    cache = _cache(F, torch, rng, b, s, hk, d)
+    pos = rng.integers(0, s - n + 1, b)
+    par = _tree(rng, b, n) if tree else None
+    if tree:
+        par[20:30, 0] = -2
+    _check_attention(F, torch, rng, cache, pos.tolist(), par, n, 16, gate=gate)
+
+
 @pytest.mark.parametrize("n,pos", [(1, 0), (70, 0), (200, 57)])
 def test_chain_attention_is_causal(F, torch, n, pos):
     """parents None: a prompt's chunk, longer than a tree may be."""
