@@ -47,12 +47,14 @@ struct TileShape {
 
 struct Segment {
   int b, kvh, rt, item, j0, j1, pos, total;
-  bool ends;
+  bool starts, ends;
 };
 
 // A block's units, one segment (token tiles [j0, j1) of one row tile) at a time.
+// A row tile counts for `skip` units more than it has token tiles: what a block
+// spends on taking up another one.
 struct Walk {
-  int b, tiles, row_tiles, rem, left;
+  int b, units, skip, row_tiles, rem, left;
   __device__ __forceinline__ bool next(const TreeArgs &a, int BT, Segment &s);
 };
 
@@ -69,23 +71,30 @@ struct TileShared {
   float4 fac[4][64];             // [META][pair of tokens]: two keys' factors, two values'
 };
 
+constexpr int kTakeUp = 3;  // token tiles that taking up another row tile costs as much as
+
 // Token tiles of session b (0: none of its nodes is there).
 __device__ __forceinline__ int session_tiles(const TreeArgs &a, int b, int BT) {
   if (a.parents && a.parents[(size_t)b * a.nodes] != -1) return 0;
   return (seen_rows(a, a.positions[b], a.nodes - 1) + BT - 1) / BT;
 }
 
+__device__ __forceinline__ int session_units(const TreeArgs &a, int b, int BT, int skip) {
+  const int tiles = session_tiles(a, b, BT);
+  return tiles ? tiles + skip : 0;
+}
+
 __device__ __forceinline__ bool Walk::next(const TreeArgs &a, int BT, Segment &s) {
   if (left <= 0) return false;
   const int items = a.kv_heads * row_tiles;
-  while (rem >= items * tiles) {
-    rem -= items * tiles;
-    tiles = session_tiles(a, ++b, BT);
+  while (rem >= items * units) {
+    rem -= items * units;
+    units = session_units(a, ++b, BT, skip);
   }
-  const int item = rem / tiles;
-  s.j0 = rem % tiles;
-  const int n = min(left, tiles - s.j0);
-  s.ends = s.j0 + n == tiles;
+  const int item = rem / units, u0 = rem % units, n = min(left, units - u0);
+  s.starts = u0 == 0;
+  s.ends = u0 + n == units;
+  s.j0 = max(0, u0 - skip);
   left -= n;
   rem += n;
   s.b = b;
@@ -95,7 +104,7 @@ __device__ __forceinline__ bool Walk::next(const TreeArgs &a, int BT, Segment &s
   s.pos = a.positions[b];
   // a chain's row tile ends at its last node's own row
   s.total = seen_rows(a, s.pos, min(a.nodes - 1, (s.rt * kTileRows + kTileRows - 1) / a.group));
-  s.j1 = min(s.j0 + n, (s.total + BT - 1) / BT);
+  s.j1 = min(u0 + n - skip, (s.total + BT - 1) / BT);
   return true;
 }
 
@@ -299,12 +308,23 @@ __device__ __noinline__ void write_rows(const TreeArgs &a, TileShared *sh, uint3
 // What the tile kernel reads at its start, made by blocks of 32 rows of a row
 // tile (eight warps): the queries as f16 in the order of its TMEM stores
 // [item][eight columns][128 rows], each row scaled by a power of two into f16's
-// range, with the factor of its scores; what each node sees.
+// range, with the factor of its scores; what each node sees (a block a session).
 constexpr int kPrepRows = 32;
 __global__ void __launch_bounds__(256) tree_attn_prep_kernel(const __grid_constant__ TreeArgs a) {
   pdl_enter();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = a.head_dim;
   const int rows = a.nodes * a.group, row_tiles = (rows + kTileRows - 1) / kTileRows, items = a.kv_heads * row_tiles;
+  if ((int)blockIdx.x >= a.batch * items * (kTileRows / kPrepRows)) {  // the blocks past the rows': a session's sights
+    if (warp >= kTreeMaxNodes / 32) return;
+    const int b = blockIdx.x - a.batch * items * (kTileRows / kPrepRows), n = warp * 32 + lane, pos = a.positions[b];
+    if (a.parents) {
+      const Sight s = sight_of(a, b, n, pos);
+      if (n < a.nodes) a.sights[(size_t)b * kTreeMaxNodes + n] = s.bits;
+    } else if (n == 0 && (pos < 0 || pos > a.max_seq - a.nodes) && a.error) {
+      atomicCAS(a.error, 0, kErrPosition);
+    }
+    return;
+  }
   const int item = blockIdx.x / (kTileRows / kPrepRows), r0 = blockIdx.x % (kTileRows / kPrepRows) * kPrepRows + warp * 4;
   const int b = item / items, kvh = item % items / row_tiles, row0 = item % row_tiles * kTileRows + r0;
   const int col = lane * 8;
@@ -347,22 +367,25 @@ __global__ void __launch_bounds__(256) tree_attn_prep_kernel(const __grid_consta
                      pack_f16x2(x[i][4] * f, x[i][5] * f), pack_f16x2(x[i][6] * f, x[i][7] * f));
     if (lane == 0) a.q_fac[(size_t)item * kTileRows + r0 + i] = pow2i(e) * a.scale_log2;
   }
-  // a session's first row tile: its nodes' sights
-  if (a.parents && item % items == 0 && r0 < 2 * 4 && warp < 2) {
-    const Sight s = sight_of(a, b, warp * 32 + lane, a.positions[b]);
-    if (warp * 32 + lane < a.nodes) a.sights[(size_t)b * kTreeMaxNodes + warp * 32 + lane] = s.bits;
-  }
 }
 
 // This block's share of the units, one warp.
 __device__ __noinline__ void share_out(const TreeArgs &a, TileShared *sh, int BT) {
   const int lane = threadIdx.x & 31, row_tiles = (a.nodes * a.group + kTileRows - 1) / kTileRows;
   const int items = a.kv_heads * row_tiles;
-  int all = 0;
-  for (int i = lane; i < a.batch; i += 32) all += session_tiles(a, i, BT);
+  int all = 0, there = 0;
+  for (int i = lane; i < a.batch; i += 32) {
+    const int tiles = session_tiles(a, i, BT);
+    all += tiles;
+    there += tiles > 0;
+  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-  const int units = all * items, blocks = min((int)gridDim.x, units);
+  for (int o = 16; o > 0; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    there += __shfl_xor_sync(0xffffffffu, there, o);
+  }
+  const int skip = all * items >= 8 * (int)gridDim.x ? kTakeUp : 0;  // (few units: all of a block's belong together)
+  const int units = (all + there * skip) * items, blocks = min((int)gridDim.x, units);
   int u0 = 0, u1 = 0;
   if ((int)blockIdx.x < blocks) {
     u0 = (int)((long long)units * blockIdx.x / blocks);
@@ -371,7 +394,7 @@ __device__ __noinline__ void share_out(const TreeArgs &a, TileShared *sh, int BT
   int s = 0, before = 0;  // the session that holds unit u0, and the units before it
   if (u1 > u0)
     for (int i0 = 0; i0 < a.batch; i0 += 32) {
-      const int n = i0 + lane < a.batch ? session_tiles(a, i0 + lane, BT) * items : 0;
+      const int n = i0 + lane < a.batch ? session_units(a, i0 + lane, BT, skip) * items : 0;
       int sum = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -387,7 +410,8 @@ __device__ __noinline__ void share_out(const TreeArgs &a, TileShared *sh, int BT
       }
     }
   if (lane == 0)
-    sh->walk = sh->soft_walk = Walk{s, u1 > u0 ? session_tiles(a, s, BT) : 1, row_tiles, u0 - before, u1 - u0};
+    sh->walk = sh->soft_walk =
+        Walk{s, u1 > u0 ? session_units(a, s, BT, skip) : 1, skip, row_tiles, u0 - before, u1 - u0};
 }
 
 template <int DP>
@@ -469,6 +493,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (!sh->more) break;
       const int j0 = sh->seg.j0, j1 = sh->seg.j1, pos = sh->seg.pos;
       const float f = a.q_fac[(size_t)sh->seg.item * kTileRows + r_own];
+      uint64_t sight = 0;
+      if (part == 0) {
+        const int n = (sh->seg.rt * kTileRows + r_own) / a.group;
+        if (tree)
+          sight = n < a.nodes ? a.sights[(size_t)sh->seg.b * kTreeMaxNodes + n] : 0;
+        else if (n < a.nodes && pos >= 0 && pos < a.max_seq - n)
+          sight = n + 1;
+      }
       {
         // 16 columns of the row at a time; a warp's loads are 512 bytes together
         const uint4 *q = a.q16 + (size_t)sh->seg.item * (a.head_dim / 8) * kTileRows + r_own;
@@ -486,15 +518,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tmem_st8(my + Sh::kTmemQ + (i * kParts + part) * 8, w);
         }
       }
-      if (part == 0) {
-        const int n = (sh->seg.rt * kTileRows + r_own) / a.group;
-        uint64_t s = 0;
-        if (tree)
-          s = n < a.nodes ? a.sights[(size_t)sh->seg.b * kTreeMaxNodes + n] : 0;
-        else if (n < a.nodes && pos >= 0 && pos < a.max_seq - n)
-          s = n + 1;
-        sh->sight[r_own] = s;
-      }
+      if (part == 0) sh->sight[r_own] = sight;
       tmem_st_wait();
       quad_sync(quad);
       if (lane == 0) mbar_arrive(&sh->qready);
@@ -564,7 +588,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       unpack2(l2, l0, l1);
       // A row tile that this block has whole is finished here.  Of the others a
       // block has two at most: the end of one (slot 0) and the start of another.
-      const bool whole = j0 == 0 && sh->seg.ends;
+      const bool whole = sh->seg.starts && sh->seg.ends;
       const size_t slot = (size_t)blockIdx.x * 2 + (seg ? 1 : 0);
       sh->red[part][r_own] = l0 + l1;
       quad_sync(quad);
@@ -575,7 +599,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         a.part_ml[slot * kTileRows + r_own] = make_float2(j1 > j0 ? m : -INFINITY, l);
       }
       if (tid == 0) {  // whose slots hold the row tile: from its first block's to its last's
-        if (j0 == 0) a.shares[sh->seg.item].x = whole ? -1 : (int)slot;
+        if (sh->seg.starts) a.shares[sh->seg.item].x = whole ? -1 : (int)slot;
         if (sh->seg.ends) a.shares[sh->seg.item].y = (int)blockIdx.x;
       }
       if (j1 > j0) {
@@ -916,7 +940,7 @@ int launch(const TreeArgs &a, const TilePlan &p, cudaStream_t s) {
     return st;
   if (int st = encode_cache_u8(&v_map, a.v_codes, a.batch, a.max_seq, a.kv_heads, a.head_dim, Sh::kBox, Sh::BT))
     return st;
-  cudaError_t e = launch_pdl(tree_attn_prep_kernel, dim3((unsigned)(p.items * (kTileRows / kPrepRows))), 256, 0, s, a);
+  cudaError_t e = launch_pdl(tree_attn_prep_kernel, dim3((unsigned)(p.items * (kTileRows / kPrepRows) + p.batch)), 256, 0, s, a);
   if (e != cudaSuccess) return cuda_fail(e, "tree_attn_prep_kernel");
   FPB_LAUNCH_CHECK("tree_attn_prep_kernel");
   e =
@@ -940,8 +964,8 @@ TilePlan tile_plan(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, 
   p.BT = head_dim > 128 ? 64 : 128;
   p.batch = batch;
   p.items = batch * kv_heads * ((nodes * (q_heads / kv_heads) + kTileRows - 1) / kTileRows);
-  p.units = p.items * ((max_seq + p.BT - 1) / p.BT);
-  p.blocks = (int)std::min<size_t>(sm_count(), p.units);
+  p.units = p.items * ((max_seq + p.BT - 1) / p.BT + kTakeUp);
+  p.blocks = (int)std::min<size_t>(sm_count(), p.items * ((max_seq + p.BT - 1) / p.BT));
   return p;
 }
 

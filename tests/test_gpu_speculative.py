@@ -267,6 +267,17 @@ def test_more_heads_and_sessions_than_blocks(F, torch, tree, d, gate):
     _check_attention(F, torch, rng, cache, pos.tolist(), par, n, 16, gate=gate)
 
 
+@pytest.mark.parametrize("n", [3, 20])
+def test_attention_of_positions_outside_the_cache(F, torch, n):
+    rng = np.random.default_rng(16)
+    cache = _cache(F, torch, rng, 5, 90, 1, 32)
+    q = _dev(torch, rng.standard_normal((5, n, 2, 32)).astype(np.float32))
+    out = F.tree_attention(q, cache, _dev(torch, np.array([-1, 90, 1 << 30, 88, 0], np.int32)), None)
+    live = (out != 0).any(-1).any(-1).cpu().numpy()
+    assert not live[:3].any() and live[3].tolist() == [True] * 2 + [False] * (n - 2) and live[4].all()
+    assert F.device_error(reset=True) == 502
+
+
 @pytest.mark.parametrize("n,pos", [(1, 0), (70, 0), (200, 57)])
 def test_chain_attention_is_causal(F, torch, n, pos):
     """parents None: a prompt's chunk, longer than a tree may be."""
