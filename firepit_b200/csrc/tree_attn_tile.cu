@@ -71,7 +71,7 @@ struct TileShared {
   float4 fac[4][64];             // [META][pair of tokens]: two keys' factors, two values'
 };
 
-constexpr int kTakeUp = 3;  // token tiles that taking up another row tile costs as much as
+constexpr int kTakeUp = 320;  // tokens that taking up another row tile costs as much as
 
 // Token tiles of session b (0: none of its nodes is there).
 __device__ __forceinline__ int session_tiles(const TreeArgs &a, int b, int BT) {
@@ -384,7 +384,7 @@ __device__ __noinline__ void share_out(const TreeArgs &a, TileShared *sh, int BT
     all += __shfl_xor_sync(0xffffffffu, all, o);
     there += __shfl_xor_sync(0xffffffffu, there, o);
   }
-  const int skip = all * items >= 8 * (int)gridDim.x ? kTakeUp : 0;  // (few units: all of a block's belong together)
+  const int skip = all * items >= 8 * (int)gridDim.x ? kTakeUp / BT : 0;  // (few units: all of a block's belong together)
   const int units = (all + there * skip) * items, blocks = min((int)gridDim.x, units);
   int u0 = 0, u1 = 0;
   if ((int)blockIdx.x < blocks) {
@@ -948,7 +948,7 @@ int launch(const TreeArgs &a, const TilePlan &p, cudaStream_t s) {
   if (e != cudaSuccess) return cuda_fail(e, "tree_attn_tile_kernel");
   FPB_LAUNCH_CHECK("tree_attn_tile_kernel");
   // a row tile's blocks in one thread's loop while they are few
-  const unsigned shares = (size_t)p.blocks > 16 * p.items ? kMergeShares : 1;
+  const unsigned shares = (size_t)p.blocks > 16 * p.items ? kMergeShares : (size_t)p.blocks > 8 * p.items ? 2 : 1;
   e = launch_pdl(tree_attn_tile_merge_kernel,
                  dim3((unsigned)(p.items * (kTileRows / 16)), (unsigned)((a.head_dim + 127) / 128)), dim3(256, shares), 0, s,
                  a, p.BT);
@@ -964,7 +964,7 @@ TilePlan tile_plan(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, 
   p.BT = head_dim > 128 ? 64 : 128;
   p.batch = batch;
   p.items = batch * kv_heads * ((nodes * (q_heads / kv_heads) + kTileRows - 1) / kTileRows);
-  p.units = p.items * ((max_seq + p.BT - 1) / p.BT + kTakeUp);
+  p.units = p.items * ((max_seq + p.BT - 1) / p.BT + kTakeUp / p.BT);
   p.blocks = (int)std::min<size_t>(sm_count(), p.items * ((max_seq + p.BT - 1) / p.BT));
   return p;
 }
