@@ -133,19 +133,23 @@ __device__ __forceinline__ void to_l2(const void *p, int bytes) {
 // same walk: each pushes what a decision needs (its slice's maximum and sum,
 // the children's weights that it owns) into every CTA's shared memory, and one
 // cluster barrier a step makes it known.  The walk is bound by the latency of
-// its steps: the rows that the next step may want (the children's logits, the
-// node's draft, the noise) are sent to L2 while the node's own is worked on.
+// its steps: the rows that the next step may want (the children's logits, at
+// the start the noise) are sent to L2 while the node's own is worked on.  (The
+// node's draft row as well: 62 us instead of 59 where drafts are refused.)  Two
+// CTAs an SM, since a cluster's eight have to lie in one part of the GPU: with
+// one, 16 clusters do not run at once (16 sessions of 9 drafts, all taken,
+// 151936 tokens: 79 us, with two 57).
 template <typename T>
-__global__ void __launch_bounds__(kVerifyThreads, 1) tree_verify_kernel(const __grid_constant__ VerifyArgs a) {
+__global__ void __launch_bounds__(kVerifyThreads, 2) tree_verify_kernel(const __grid_constant__ VerifyArgs a) {
   pdl_enter();
   extern __shared__ __align__(16) float r[];  // [slice]: 2^((l - slice's maximum) scale), or what is left of it
-  __shared__ int par[kTreeMaxNodes], tok[kTreeMaxNodes], refused[kTreeMaxNodes];
+  __shared__ int par[kTreeMaxNodes], tok[kTreeMaxNodes], owner[kTreeMaxNodes], refused[kTreeMaxNodes];
   __shared__ float acc[kTreeMaxNodes], q_tok[kTreeMaxNodes], red[kVerifyWarps], red2[kVerifyWarps];
   __shared__ int red_i[kVerifyWarps];
   // what the CTAs tell one another; the halves alternate, so that one step's
   // reads may overlap the next one's stores
   __shared__ float got_v[2][kVerifyCluster], got_i[2][kVerifyCluster], got_s[2][kVerifyCluster],
-      got_r[2][kTreeMaxNodes], scale_s[kVerifyCluster];
+      got_r[2][kTreeMaxNodes];
   const unsigned rank = cluster_ctarank(), peer = threadIdx.x % kVerifyCluster;
   const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int v0 = (int)rank * a.slice, len = max(0, min(a.vocab - v0, a.slice));
@@ -157,6 +161,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) tree_verify_kernel(const __
     const int p = a.parents ? a.parents[(size_t)b * a.nodes + i] : i - 1, x = a.tokens[(size_t)b * a.nodes + i];
     par[i] = p;
     tok[i] = x;
+    owner[i] = x / a.slice;
     acc[i] = a.accept ? a.accept[(size_t)b * a.nodes + i] : 0.0f;
     q_tok[i] = a.draft && p >= 0 && p < i && x >= 0 && x < a.vocab
                    ? a.draft[((size_t)b * a.nodes + p) * a.draft_pitch + x] : 1.0f;
@@ -174,10 +179,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) tree_verify_kernel(const __
   cluster_sync();  // every CTA of the cluster runs: its shared memory may be stored to
   if (tid == 0 && !greedy) to_l2(noise, f_bytes);
   int flip = 0;
-  auto block_sum = [&](float v) {  // of the block, for every thread; all threads meet
+  auto block_sum = [&](float v) {  // of the block, for every thread; all threads meet (and in `tell` before the next)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
     if (lane == 0) red2[warp] = v;
     __syncthreads();
     float t = red2[lane % kVerifyWarps];
@@ -221,16 +225,20 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) tree_verify_kernel(const __
   while (true) {
     if (rank == 0 && tid == 0) a.path[(size_t)b * a.nodes + taken] = node;
     ++taken;
-    if (a.vec && warp == 0) {
+    auto prefetch = [&]() {  // what the next step may want (by the last warp, with its own loads under way)
+      if (!a.vec || warp != kVerifyWarps - 1) return;
       for (int c = node + 1 + lane; c < a.nodes; c += 32)
         if (par[c] == node) to_l2(logits_of(c), l_bytes);
-      if (lane == 0 && a.draft) to_l2(a.draft + ((size_t)b * a.nodes + node) * a.draft_pitch + v0, f_bytes);
-    }
+    };
     // the slice's maximum (of finite logits), then powers by it and their sum
     Best top{-INFINITY, 0x7fffffff};
     float s = 0.0f;
     constexpr int N = 16 / sizeof(T), kLoads = kHold / N;
-    if (!greedy && a.vec && len % N == 0 && len <= kHold * kVerifyThreads) {  // the slice in registers between the two
+    // The slice stays in registers between the two where it fills at least half of
+    // them, else it goes through shared memory (12 sessions, 9 drafts taken, f32:
+    // 96000 tokens 36 us in registers, 41 through shared memory; 32000 29 and 28).
+    constexpr int kAll = kHold * kVerifyThreads;
+    if (!greedy && a.vec && len % N == 0 && a.slice <= kAll && a.slice * 2 >= kAll) {
       const T *row = logits_of(node);
       uint4 v[kLoads];
       float m = -INFINITY;
@@ -240,6 +248,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) tree_verify_kernel(const __
         // past the slice: NaN, which counts as -inf
         v[k] = i < len ? __ldg(reinterpret_cast<const uint4 *>(row + i)) : make_uint4(~0u, ~0u, ~0u, ~0u);
       }
+      prefetch();
       auto value = [&](int k, int j) {
         const uint32_t w = N == 4 ? (j == 0 ? v[k].x : j == 1 ? v[k].y : j == 2 ? v[k].z : v[k].w)
                                   : (j < 2 ? v[k].x : j < 4 ? v[k].y : j < 6 ? v[k].z : v[k].w);
@@ -269,6 +278,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) tree_verify_kernel(const __
       }
       s = block_sum(s);
     } else {
+      prefetch();
       for_row<true>(logits_of(node), len, a.vec, greedy ? nullptr : r, [&](float x, float &y, int i) {
         y = isfinite(x) ? x : -INFINITY;
         if (y > top.v) top = Best{y, v0 + i};
@@ -287,17 +297,13 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) tree_verify_kernel(const __
     }
     tell(node, node, top, s);
     // the slices' factors to one maximum, and the whole sum
-    float left = 0.0f;
+    float left = 0.0f, factor = 0.0f;  // of CTA `peer`'s r
     const float mc = got_v[flip ^ 1][peer];
     const Best all = over_ctas_best(Best{mc, __float_as_int(got_i[flip ^ 1][peer])});
     if (!greedy) {
-      const float f = mc == -INFINITY ? 0.0f : pow2((mc - all.v) * a.scale_log2);
-      left = over_ctas_sum(got_s[flip ^ 1][peer] * f);
-      __syncthreads();  // the node before is done with the factors
-      if (tid < kVerifyCluster) scale_s[tid] = f;
-      __syncthreads();
+      factor = mc == -INFINITY ? 0.0f : pow2((mc - all.v) * a.scale_log2);
+      left = over_ctas_sum(got_s[flip ^ 1][peer] * factor);
     }
-    float own = greedy ? 0.0f : scale_s[rank];  // of this slice's r
     int child = -1, rejected = 0;
     const float *q = a.draft ? a.draft + ((size_t)b * a.nodes + node) * a.draft_pitch + v0 : nullptr;
     for (int c = node + 1; c < a.nodes; ++c) {
@@ -314,7 +320,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) tree_verify_kernel(const __
         }
         continue;
       }
-      float rx = fmaxf(got_r[flip ^ 1][c], 0.0f) * scale_s[x / a.slice];
+      float rx = fmaxf(got_r[flip ^ 1][c], 0.0f) * __shfl_sync(0xffffffffu, factor, owner[c]);
       if (q) {
         if (acc[c] * q_tok[c] * left < rx) {
           child = c;
@@ -322,7 +328,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) tree_verify_kernel(const __
         }
         // What is left over, with its sign: whoever reads r takes it as at
         // least 0, and what it was can be had back.
-        const float inv = own / left;
+        const float inv = __shfl_sync(0xffffffffu, factor, rank) / left;
         float z = 0.0f;
         for_row<true>(q, len, a.vec, r, [&](float x, float &y, int) {
           y = fmaf(fmaxf(y, 0.0f), inv, -x);
@@ -337,10 +343,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) tree_verify_kernel(const __
           tell(node, c, top, 0.0f);
           left = 1.0f;
         }
-        own = 1.0f;
-        __syncthreads();
-        if (tid < kVerifyCluster) scale_s[tid] = 1.0f;
-        __syncthreads();
+        factor = 1.0f;
       } else {
         for (int j = 0; j < rejected; ++j)
           if (refused[j] == x) rx = 0.0f;
@@ -368,8 +371,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) tree_verify_kernel(const __
       if (refused[j] >= v0 && refused[j] < v0 + len) r[refused[j] - v0] = 0.0f;
     __syncthreads();
     Best pick{-1.0f, 0x7fffffff};
+    const float own = __shfl_sync(0xffffffffu, factor, rank);
     for_row<false>(noise, len, a.vec, r, [&](float e, float &y, int i) {
-      const float w = fmaxf(y, 0.0f) * own / e;
+      const float w = __fdividef(fmaxf(y, 0.0f) * own, e);
       if (w > pick.v) pick = Best{w, v0 + i};
     });
     tell(a.nodes, a.nodes, block_best(pick), 0.0f);
