@@ -35,9 +35,9 @@ using namespace sm100;
 // ---- few rows: warps that stream tokens on their own -------------------------------------------
 // Block (split, session * kv head): NR rows (8 or 16) of one kv head, four
 // warps that take steps of 16 tokens in turn.  Each warp has its own ring of
-// kStages steps of codes, filled by TMA (128-byte swizzle: its 16-byte
-// reads fall on distinct banks), so that 24 KB a warp are on their way however
-// long a step takes; nothing is shared between the warps before the end.
+// kStages steps of codes, filled by TMA, so that up to 24 KB a warp are on their
+// way however long a step takes; nothing is shared between the warps before the
+// end.
 //  S^T = K Q^T  m16n8k16, the tokens as M, the rows as N.  The order of the
 //               summed dimension is free as long as both sides agree, so a
 //               lane's 16-byte piece of a key (16 dimensions) is its operand
@@ -50,6 +50,15 @@ using namespace sm100;
 // piece_at(i): a quarter of a warp then reads 16 bytes from all of the banks.
 // Each e4m3 is converted to f16 (exact); the key's factor goes to the score,
 // the value's to the weight's exponent.
+// The tokens as M, not the rows: eight rows take half as many instructions, and
+// a token's exponents belong to one lane (8 x 8192 tokens x 2 heads x 256, 16
+// rows: 27.5 us against 32 with the rows as M).
+// Meant to be bound by the cache's bytes; what it takes is the start (positions,
+// then the first codes: 3 us), its steps' latency (480 instructions of which a
+// third depend on the one before, eight warps an SM by their registers), and 4
+// us of the splits' results and their merge.  16 x 1 node x 16 heads (2 kv) x
+// 256, 8192 tokens: 32.5 us, 3.7 TB/s; 8 sessions of 8 rows 21.5 us, of which
+// 14 (4.8 TB/s) grow with the length.
 constexpr int kRowsThreads = 128, kRowsWarps = 4;
 constexpr int kErrRowsWait = 503;
 
@@ -73,7 +82,9 @@ struct RowsShape {
 };
 
 // Steps of a split: what the call's splits share of a session's, in whole
-// rounds of a block's warps; a session of few tokens leaves splits unused.
+// rounds of a block's warps; a session of few tokens leaves splits unused (1000
+// tokens in a cache of 32768: 7.8 us, 9.1 with 63 splits of one step; elsewhere
+// alike).
 __device__ __forceinline__ int steps_a_split(int steps, int splits) {
   return ((steps + splits - 1) / splits + kRowsWarps - 1) / kRowsWarps * kRowsWarps;
 }
@@ -472,7 +483,8 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
 
 // The splits of a row (session, node, query head) meet, in order: blockDim.y
 // warps a row and 128 columns share them, four columns a lane.  What the rows
-// kernel does not write is read before it is waited for.
+// kernel does not write is read before it is waited for.  Bound by the latency
+// of two reads in a row (maxima, then values, in L2).
 constexpr int kMergeWarps = 16;
 __global__ void __launch_bounds__(kMergeWarps * 32, 2) tree_attn_merge_kernel(const __grid_constant__ TreeArgs a, int NR,
                                                                             int count) {
@@ -543,15 +555,19 @@ struct Plan {
   size_t items;
 };
 
-// Rows a key/value head from which the tcgen05 kernel takes over.
+// Past 16 rows a key/value head the tcgen05 kernel takes over, which takes 128 of
+// them in the time of 17.  Up to 16 it is the slower one: 16 rows x 256 columns,
+// 8 x 8192 tokens 47 us here 27.5, 1 x 30000 36 and 22, 64 x 1000 51 and 28.
 bool wants_tiles(size_t nodes, size_t q_heads, size_t kv_heads) { return nodes * (q_heads / kv_heads) > 16; }
 
 Plan plan_for(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, size_t head_dim, size_t max_seq) {
   Plan p{};
   const size_t rows = nodes * (q_heads / kv_heads);
+  // (eight rows as 16: 25.9 us instead of 21.5 at 8 x 8192 x 256, 9.0 instead of 7.7 at 1 x 1000)
   p.rows_tile = rows <= 8 ? 8 : 16;
   p.items = batch * kv_heads;
-  // one wave of blocks; at least 64 tokens a split (a step for each warp)
+  // One wave of blocks; at least 64 tokens a split, a step for each warp (1 x 1000
+  // tokens: 7.8 us, with 128 tokens 8.7, with 256 11.1).
   const size_t resident = (size_t)sm_count() * rows_blocks(head_dim <= 128 ? 128 : 256);
   const size_t want = std::max<size_t>(1, resident / p.items);
   p.splits = (int)std::max<size_t>(1, std::min(want, (max_seq + 63) / 64));
@@ -666,7 +682,9 @@ extern "C" int fpb_tree_attn(const void *q, int q_dtype, size_t q_pitch, size_t 
                                    : (few ? run_rows<256, 8>(a, p, s) : run_rows<256, 16>(a, p, s));
   if (st || p.splits == 1) return st;
   const int count = (int)(batch * nodes * q_heads);
-  // as many warps a row as it has splits, while all of them run at once
+  // As many warps a row as it has splits, while all of them run at once (whole
+  // calls, one warp a row and shared: 1 x 30000 28.5 and 16.9 us, 8 x 8192 with 16
+  // rows 29.3 and 27.5; shared past what runs at once: 31).
   const unsigned halves = head_dim > 128 ? 2 : 1;
   unsigned shares = 1;
   while (shares < (unsigned)kMergeWarps && 2 * shares <= (unsigned)p.splits &&

@@ -17,6 +17,17 @@
 //   V tile: the same bytes read as the transposed operand (N-major).
 // The tokens' factors stay out of the tiles: the key's multiplies the score,
 // the value's the weight, both in f32 (see kHead).
+// Neither the cache's bytes nor the tensor cores bound it.  A unit takes 2800
+// cycles at 128 tokens and 128 columns, of which the two products' instructions
+// need 1300, the conversion of its 32768 codes and the 16384 powers about 900
+// (converters' pipe), the 0.6 MB through shared memory 1300: each role waits
+// for the one before it for a part of its time, two units in the ring or four,
+// one softmax group or two alike.  Issue slots 52% busy, tensor cores 32%.
+//   8 sessions x 16 nodes x 16 heads (2 kv) x 256, 16384 tokens: 61 us with its
+//     two helpers; 2.05 TB/s of the cache, 440 TFLOP/s
+//   4 x 61 x 32 (4) x 128, 30011 tokens: 192 us, 500 TFLOP/s
+// Before the first products the block spends 8 us (start, shares, queries), at
+// its end 4 us on the 64 to 128 KB of its partial result.
 #include <algorithm>
 #include <mutex>
 #include <vector>
@@ -51,10 +62,13 @@ struct Segment {
 };
 
 // A block's units, one segment (token tiles [j0, j1) of one row tile) at a time.
-// A row tile counts for `skip` units more than it has token tiles: what a block
-// spends on taking up another one.
+// A row tile counts for kTakeUp / BT units more than it has token tiles, what a
+// block spends on taking up another one (its end's and the next one's queries,
+// first scores: 7 us, five tiles of 64 tokens at 256 columns).  8 x 16 nodes at
+// 16384: 64.8 us, 68.5 without.
+constexpr int kTakeUp = 320;  // tokens
 struct Walk {
-  int b, units, skip, row_tiles, rem, left;
+  int b, units, row_tiles, rem, left;
   __device__ __forceinline__ bool next(const TreeArgs &a, int BT, Segment &s);
 };
 
@@ -71,25 +85,23 @@ struct TileShared {
   float4 fac[4][64];             // [META][pair of tokens]: two keys' factors, two values'
 };
 
-constexpr int kTakeUp = 320;  // tokens that taking up another row tile costs as much as
-
 // Token tiles of session b (0: none of its nodes is there).
 __device__ __forceinline__ int session_tiles(const TreeArgs &a, int b, int BT) {
   if (a.parents && a.parents[(size_t)b * a.nodes] != -1) return 0;
   return (seen_rows(a, a.positions[b], a.nodes - 1) + BT - 1) / BT;
 }
 
-__device__ __forceinline__ int session_units(const TreeArgs &a, int b, int BT, int skip) {
+__device__ __forceinline__ int session_units(const TreeArgs &a, int b, int BT) {
   const int tiles = session_tiles(a, b, BT);
-  return tiles ? tiles + skip : 0;
+  return tiles ? tiles + kTakeUp / BT : 0;
 }
 
 __device__ __forceinline__ bool Walk::next(const TreeArgs &a, int BT, Segment &s) {
   if (left <= 0) return false;
-  const int items = a.kv_heads * row_tiles;
+  const int items = a.kv_heads * row_tiles, skip = kTakeUp / BT;
   while (rem >= items * units) {
     rem -= items * units;
-    units = session_units(a, ++b, BT, skip);
+    units = session_units(a, ++b, BT);
   }
   const int item = rem / units, u0 = rem % units, n = min(left, units - u0);
   s.starts = u0 == 0;
@@ -309,6 +321,9 @@ __device__ __noinline__ void write_rows(const TreeArgs &a, TileShared *sh, uint3
 // tile (eight warps): the queries as f16 in the order of its TMEM stores
 // [item][eight columns][128 rows], each row scaled by a power of two into f16's
 // range, with the factor of its scores; what each node sees (a block a session).
+// A kernel of its own since several blocks read a row's queries (here once, 128
+// KB a row tile), and a row's factor needs all of its columns: 2 us, most of it
+// hidden behind the tile kernel's own start.
 constexpr int kPrepRows = 32;
 __global__ void __launch_bounds__(256) tree_attn_prep_kernel(const __grid_constant__ TreeArgs a) {
   pdl_enter();
@@ -373,19 +388,11 @@ __global__ void __launch_bounds__(256) tree_attn_prep_kernel(const __grid_consta
 __device__ __noinline__ void share_out(const TreeArgs &a, TileShared *sh, int BT) {
   const int lane = threadIdx.x & 31, row_tiles = (a.nodes * a.group + kTileRows - 1) / kTileRows;
   const int items = a.kv_heads * row_tiles;
-  int all = 0, there = 0;
-  for (int i = lane; i < a.batch; i += 32) {
-    const int tiles = session_tiles(a, i, BT);
-    all += tiles;
-    there += tiles > 0;
-  }
+  int all = 0;
+  for (int i = lane; i < a.batch; i += 32) all += session_units(a, i, BT);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-    there += __shfl_xor_sync(0xffffffffu, there, o);
-  }
-  const int skip = all * items >= 8 * (int)gridDim.x ? kTakeUp / BT : 0;  // (few units: all of a block's belong together)
-  const int units = (all + there * skip) * items, blocks = min((int)gridDim.x, units);
+  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+  const int units = all * items, blocks = min((int)gridDim.x, units);
   int u0 = 0, u1 = 0;
   if ((int)blockIdx.x < blocks) {
     u0 = (int)((long long)units * blockIdx.x / blocks);
@@ -394,7 +401,7 @@ __device__ __noinline__ void share_out(const TreeArgs &a, TileShared *sh, int BT
   int s = 0, before = 0;  // the session that holds unit u0, and the units before it
   if (u1 > u0)
     for (int i0 = 0; i0 < a.batch; i0 += 32) {
-      const int n = i0 + lane < a.batch ? session_units(a, i0 + lane, BT, skip) * items : 0;
+      const int n = i0 + lane < a.batch ? session_units(a, i0 + lane, BT) * items : 0;
       int sum = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -410,8 +417,7 @@ __device__ __noinline__ void share_out(const TreeArgs &a, TileShared *sh, int BT
       }
     }
   if (lane == 0)
-    sh->walk = sh->soft_walk =
-        Walk{s, u1 > u0 ? session_units(a, s, BT, skip) : 1, skip, row_tiles, u0 - before, u1 - u0};
+    sh->walk = sh->soft_walk = Walk{s, u1 > u0 ? session_units(a, s, BT) : 1, row_tiles, u0 - before, u1 - u0};
 }
 
 template <int DP>
@@ -839,14 +845,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 }
 
 // The blocks that share a row tile's tokens meet, in order, with the gate:
-// block (16 rows of a row tile, 128 columns); thread (row, eight columns, share
-// of the blocks).  Rows of nodes that are not there become zeros, and those of
-// sessions that no block has.  What the
-// tile kernel does not write is read before it is waited for.
-constexpr int kMergeShares = 4;
-__global__ void __launch_bounds__(1024, 1) tree_attn_tile_merge_kernel(const __grid_constant__ TreeArgs a, int BT) {
-  __shared__ float4 acc_s[kMergeShares - 1][2][256];
-  __shared__ float2 ml_s[kMergeShares - 1][256];
+// block (16 rows of a row tile, blockDim.x / 2 columns); thread (row, eight
+// columns, share of the blocks).  Rows of nodes that are not there become zeros,
+// and those of sessions that no block has.  What the tile kernel does not write
+// is read before it is waited for.  Bound by the latency of two reads in a row
+// (whose slots, then their values, in L2): 5 us for 21 MB of 148 blocks.
+constexpr int kMergeThreads = 1024;
+__global__ void __launch_bounds__(kMergeThreads, 1) tree_attn_tile_merge_kernel(const __grid_constant__ TreeArgs a, int BT) {
+  __shared__ float4 acc_s[2][kMergeThreads];
+  __shared__ float2 ml_s[kMergeThreads];
   const int t = threadIdx.x, share = threadIdx.y, D = a.head_dim;
   const int rows = a.nodes * a.group, row_tiles = (rows + kTileRows - 1) / kTileRows, items = a.kv_heads * row_tiles;
   const int item = blockIdx.x / (kTileRows / 16), r = blockIdx.x % (kTileRows / 16) * 16 + (t & 15);
@@ -856,7 +863,7 @@ __global__ void __launch_bounds__(1024, 1) tree_attn_tile_merge_kernel(const __g
     asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
-  const int d = blockIdx.y * 128 + 8 * (t >> 4);
+  const int d = blockIdx.y * (blockDim.x / 2) + 8 * (t >> 4);
   const bool live = row < rows && d < D;
   const int n = row / a.group, h = kvh * a.group + row % a.group, pos = a.positions[b];
   const size_t node = (size_t)b * a.nodes + n;
@@ -897,15 +904,16 @@ __global__ void __launch_bounds__(1024, 1) tree_attn_tile_merge_kernel(const __g
     }
   }
   if (blockDim.y > 1) {
+    const int at = share * blockDim.x + t;
     if (share > 0) {
-      acc_s[share - 1][0][t] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      acc_s[share - 1][1][t] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-      ml_s[share - 1][t] = make_float2(m, l);
+      acc_s[0][at] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      acc_s[1][at] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      ml_s[at] = make_float2(m, l);
     }
     __syncthreads();
     if (share > 0) return;
-    for (int i = 0; i < (int)blockDim.y - 1; ++i)
-      if (ml_s[i][t].x != -INFINITY) add(ml_s[i][t], acc_s[i][0][t], acc_s[i][1][t]);
+    for (int i = at + blockDim.x; i < (int)(blockDim.x * blockDim.y); i += blockDim.x)
+      if (ml_s[i].x != -INFINITY) add(ml_s[i], acc_s[0][i], acc_s[1][i]);
   }
   if (!live) return;
   const bool there = some && (a.parents ? a.sights[(size_t)b * kTreeMaxNodes + n] != 0 : pos >= 0 && pos < a.max_seq - n);
@@ -947,11 +955,16 @@ int launch(const TreeArgs &a, const TilePlan &p, cudaStream_t s) {
       launch_pdl(tree_attn_tile_kernel<DP>, dim3((unsigned)p.blocks), kTileThreads, smem, s, a, k_map, v_map);
   if (e != cudaSuccess) return cuda_fail(e, "tree_attn_tile_kernel");
   FPB_LAUNCH_CHECK("tree_attn_tile_kernel");
-  // a row tile's blocks in one thread's loop while they are few
-  const unsigned shares = (size_t)p.blocks > 16 * p.items ? kMergeShares : (size_t)p.blocks > 8 * p.items ? 2 : 1;
+  // A row tile's blocks in one thread's loop while they are few, else shared, by
+  // narrower blocks of more shares where they are many and the row tiles few
+  // (whole calls; 74 blocks a row tile: 16 shares 22.4 us, 4 shares 31, none 66;
+  // 18: 4 shares 57 us, 16 shares 69, none 65; 9: 2 shares 65 us, 4 shares 67,
+  // none 68; 4: none 202 us, 2 shares 205, 4 shares 211).
+  const size_t each = p.blocks / p.items;
+  const unsigned shares = each > 32 ? 16 : each > 16 ? 4 : each > 8 ? 2 : 1, cols = shares == 16 ? 32 : 128;
   e = launch_pdl(tree_attn_tile_merge_kernel,
-                 dim3((unsigned)(p.items * (kTileRows / 16)), (unsigned)((a.head_dim + 127) / 128)), dim3(256, shares), 0, s,
-                 a, p.BT);
+                 dim3((unsigned)(p.items * (kTileRows / 16)), (unsigned)((a.head_dim + cols - 1) / cols)),
+                 dim3(2 * cols, shares), 0, s, a, p.BT);
   if (e != cudaSuccess) return cuda_fail(e, "tree_attn_tile_merge_kernel");
   FPB_LAUNCH_CHECK("tree_attn_tile_merge_kernel");
   return FPB_OK;
