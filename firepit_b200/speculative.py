@@ -45,10 +45,10 @@ def _empty(stream, like, dtype, *shape):
     """Memory of the stream that will write it: torch hands memory out in the
     order of the stream it was asked for on."""
     if stream is None:
-        return like.new_empty(shape, dtype=dtype)
+        return like.new_empty(*shape, dtype=dtype)
     torch = _Torch.module
     with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=like.device)):
-        return like.new_empty(shape, dtype=dtype)
+        return like.new_empty(*shape, dtype=dtype)
 
 
 def _handle(stream, like) -> int:
@@ -185,7 +185,7 @@ def kv8_read(cache: Kv8Cache, begin, count: int, dtype=None, stream=None):
         begins, begin = begin.data_ptr(), 0
     if count < 1 or begin < 0:
         raise ShapeError(f"kv8_read: rows [{begin}, +{count})")
-    k, v = _empty(stream, cache.k, dtype, 2, b, count, hk, d).unbind(0)
+    k, v = _empty(stream, cache.k, dtype, b, count, hk, d), _empty(stream, cache.k, dtype, b, count, hk, d)
     N.call("fpb_kv8_read", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), b,
            s, hk, d, begins, begin, count, k.data_ptr(), v.data_ptr(), _code(k), _handle(stream, cache.k))
     return k, v
@@ -273,7 +273,7 @@ def tree_verify(logits, tokens, parents=None, temperature: float = 0.0, accept=N
     else:
         accept = noise = draft = None
     path = _empty(stream, logits, _Torch.i32, b, n)
-    count, nxt = _empty(stream, logits, _Torch.i32, 2, b).unbind(0)
+    count, nxt = _empty(stream, logits, _Torch.i32, b), _empty(stream, logits, _Torch.i32, b)
     N.call("fpb_tree_verify", logits.data_ptr(), _code(logits), _pitch(logits, "logits"), _ptr(draft), draft_pitch,
            tokens.data_ptr(), _ptr(parents), _ptr(accept), _ptr(noise), noise_pitch, b, n, vocab, temperature,
            path.data_ptr(), count.data_ptr(), nxt.data_ptr(), _handle(stream, logits))
