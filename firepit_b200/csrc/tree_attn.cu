@@ -35,9 +35,10 @@ using namespace sm100;
 // ---- few rows: warps that stream tokens on their own -------------------------------------------
 // Block (split, session * kv head): NR rows (8 or 16) of one kv head, four
 // warps that take steps of 16 tokens in turn.  Each warp has its own ring of
-// kStages steps of codes, filled by TMA, so that up to 24 KB a warp are on their
-// way however long a step takes; nothing is shared between the warps before the
-// end.
+// kStages steps of codes, filled by TMA, so that up to 16 KB a warp are on their
+// way however long a step takes (three stages: 21.4 us instead of 20.9 at 8 x
+// 8192 x 256, 56.4 instead of 52.5 at 8 x 65536 x 128); nothing is shared between
+// the warps before the end.
 //  S^T = K Q^T  m16n8k16, the tokens as M, the rows as N.  The order of the
 //               summed dimension is free as long as both sides agree, so a
 //               lane's 16-byte piece of a key (16 dimensions) is its operand
@@ -53,12 +54,11 @@ using namespace sm100;
 // The tokens as M, not the rows: eight rows take half as many instructions, and
 // a token's exponents belong to one lane (8 x 8192 tokens x 2 heads x 256, 16
 // rows: 27.5 us against 32 with the rows as M).
-// Meant to be bound by the cache's bytes; what it takes is the start (positions,
-// then the first codes: 3 us), its steps' latency (480 instructions of which a
-// third depend on the one before, eight warps an SM by their registers), and 4
-// us of the splits' results and their merge.  16 x 1 node x 16 heads (2 kv) x
-// 256, 8192 tokens: 32.5 us, 3.7 TB/s; 8 sessions of 8 rows 21.5 us, of which
-// 14 (4.8 TB/s) grow with the length.
+// Long caches are bound by their bytes (from 8 x 16384 to 8 x 32768 tokens, 8 rows
+// x 256: 134 MB more in 20 us, 6.7 TB/s), shorter ones by some 11 us besides:
+// the launches, the start (positions, then the first codes), the last steps'
+// latency, the splits' results and their merge.  16 x 1 node x 16 heads (2 kv) x
+// 256, 8192 tokens: 32 us, 3.7 TB/s.
 constexpr int kRowsThreads = 128, kRowsWarps = 4;
 constexpr int kErrRowsWait = 503;
 
@@ -70,7 +70,7 @@ constexpr int rows_blocks(int DP) { return DP == 256 ? 2 : 3; }
 
 template <int DP, int NR>
 struct RowsShape {
-  static constexpr int kBlocks = rows_blocks(DP), kStages = 3;
+  static constexpr int kBlocks = rows_blocks(DP), kStages = 2;
   static constexpr bool kQShared = NR * DP > 16 * 128;  // 64 registers of queries are too many beside 128 of sums
   static constexpr int kQPitch = DP + 8;                // f16 elements: 16-byte reads of eight rows on distinct banks
   static constexpr int kBox = DP == 64 ? 64 : 128;
