@@ -185,31 +185,34 @@ __device__ __forceinline__ float weigh_pass(uint32_t s_tmem, const float4 *fac, 
   const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
   float mx[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int c = 0; c < NT / 8; ++c) {
-    uint32_t r[8];
-    tmem_ld8(s_tmem + c * 8, r);
+  for (int c = 0; c < NT / 16; ++c) {
+    uint32_t r[16];
+    tmem_ld16(s_tmem + c * 16, r);
     tmem_ld_wait(r);
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const float4 ft = fac[(c * 8 + e) / 2];
+    for (int e = 0; e < 16; e += 2) {
+      const float4 ft = fac[(c * 16 + e) / 2];
       const uint64_t x = mul2(pack2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), pack2(ft.x, ft.y));
       float e0, e1, w0, w1;
       unpack2(fma2(x, f2, b2), e0, e1);
       e0 = exp2_approx(e0);
       e1 = exp2_approx(e1);
       if (OPEN) {
-        if (!(seen >> (c * 8 + e) & 1)) e0 = 0.0f;
-        if (!(seen >> (c * 8 + e + 1) & 1)) e1 = 0.0f;
+        if (!(seen >> (c * 16 + e) & 1)) e0 = 0.0f;
+        if (!(seen >> (c * 16 + e + 1) & 1)) e1 = 0.0f;
       }
       const uint64_t e2 = pack2(e0, e1);
       l = add2(l, e2);
       unpack2(mul2(e2, pack2(ft.z, ft.w)), w0, w1);
       mx[(e >> 1) & 1] = fmaxf(mx[(e >> 1) & 1], fmaxf(w0, w1));
-      p[(c * 8 + e) / 2] = pack_f16x2(w0, w1);
+      p[(c * 16 + e) / 2] = pack_f16x2(w0, w1);
     }
   }
   return fmaxf(mx[0], mx[1]);
 }
+
+// Bytes of four codes that are not a number.
+__device__ __forceinline__ uint32_t not_numbers(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 
 // What happens seldom stays out of line, so that the loop over tiles keeps its
 // registers.
@@ -752,6 +755,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       for (int i = 0; i < P; ++i)
         v[i] = *reinterpret_cast<const uint4 *>(stage + src + i * kStep * (DP == 64 ? 64 : 128));
     };
+    // (one tile's pieces are held at a time: with both, spilled registers cost 4 x
+    // 61 at 30011 188 us instead of 177)
     auto store = [&](uint8_t *stage, const uint4(&v)[P]) {
       uint8_t *to = stage + dst, *and_to = stage + (dst ^ 16);
 #pragma unroll
@@ -782,10 +787,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const int st = g % ST, rs = g % RAW;
       const bool open = (j + 1) * BT > sg.pos;
       float *ft = reinterpret_cast<float *>(sh->fac[g % META]);
-      uint4 kb[P], vb[P];
+      uint4 cb[P];
       wait(&sh->rkfull[rs], g / RAW);
-      fetch(rK + rs * Sh::kRawBytes, kb);
-      if (g >= ST) wait(&sh->kempty[st], g / ST - 1);
       if (cw == 0) {
 #pragma unroll
         for (int i = 0; i < X; ++i) {
@@ -796,38 +799,40 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       if (open) {  // values that are not a number: zero in the product, and the token's score NaN for those who see it
         wait(&sh->rvfull[rs], g / RAW);
-        fetch(rV + rs * Sh::kRawBytes, vb);
         conv_sync();
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < P; ++i) {
-          uint32_t w[4] = {vb[i].x, vb[i].y, vb[i].z, vb[i].w}, any = 0;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t bad = __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-            w[k] &= ~bad;
-            any |= bad;
-          }
-          vb[i] = make_uint4(w[0], w[1], w[2], w[3]);
+          const uint4 v = *reinterpret_cast<const uint4 *>(rV + rs * Sh::kRawBytes + src + i * kStep * (DP == 64 ? 64 : 128));
           const int t = t_own + i * kStep;
-          if (any) ft[(t >> 1) * 4 + (t & 1)] = __int_as_float(0x7fc00000);
+          if (not_numbers(v.x) | not_numbers(v.y) | not_numbers(v.z) | not_numbers(v.w))
+            ft[(t >> 1) * 4 + (t & 1)] = __int_as_float(0x7fc00000);
         }
         conv_sync();
       }
       __syncwarp();
       if (cw == 0 && lane == 0) mbar_arrive(&sh->metafull[g % META]);
-      store(sK + st * Sh::kBytes, kb);
+      fetch(rK + rs * Sh::kRawBytes, cb);
+      if (g >= ST) wait(&sh->kempty[st], g / ST - 1);
+      store(sK + st * Sh::kBytes, cb);
       if (lane == 0) {
         mbar_arrive(&sh->kfull[st]);
         mbar_arrive(&sh->rkempty[rs]);
       }
-      if (!open) {
-        wait(&sh->rvfull[rs], g / RAW);
-        fetch(rV + rs * Sh::kRawBytes, vb);
+      if (!open) wait(&sh->rvfull[rs], g / RAW);
+      fetch(rV + rs * Sh::kRawBytes, cb);
+      if (open) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          cb[i].x &= ~not_numbers(cb[i].x);
+          cb[i].y &= ~not_numbers(cb[i].y);
+          cb[i].z &= ~not_numbers(cb[i].z);
+          cb[i].w &= ~not_numbers(cb[i].w);
+        }
       }
       if (++j >= sg.j1) enter();
       if (more && cw == 0) load_exps();
       if (g >= ST) wait(&sh->vempty[st], g / ST - 1);
-      store(sV + st * Sh::kBytes, vb);
+      store(sV + st * Sh::kBytes, cb);
       if (lane == 0) {
         mbar_arrive(&sh->vfull[st]);
         mbar_arrive(&sh->rvempty[rs]);
