@@ -17,15 +17,14 @@
 //   V tile: the same bytes read as the transposed operand (N-major).
 // The tokens' factors stay out of the tiles: the key's multiplies the score,
 // the value's the weight, both in f32 (see kHead).
-// Neither the cache's bytes nor the tensor cores bound it.  A unit takes 2800
-// cycles at 128 tokens and 128 columns, of which the two products' instructions
-// need 1300, the conversion of its 32768 codes and the 16384 powers about 900
-// (converters' pipe), the 0.6 MB through shared memory 1300: each role waits
-// for the one before it for a part of its time, two units in the ring or four,
-// one softmax group or two alike.  Issue slots 52% busy, tensor cores 32%.
-//   8 sessions x 16 nodes x 16 heads (2 kv) x 256, 16384 tokens: 61 us with its
-//     two helpers; 2.05 TB/s of the cache, 440 TFLOP/s
-//   4 x 61 x 32 (4) x 128, 30011 tokens: 192 us, 500 TFLOP/s
+// Neither the cache's bytes nor the tensor cores bound it.  A unit of 128 tokens
+// and 128 columns takes 2600 cycles, of which the two products need 1280, the
+// softmax's and the converters' instructions 1350 issue cycles a scheduler, and
+// shared memory about 1800 (copies in, converters' reads and writes, operands,
+// factors).  Issue slots 51% busy, tensor cores 33%.
+//   8 sessions x 16 nodes x 16 heads (2 kv) x 256, 16384 tokens: 60 us with its
+//     two helpers; 2.1 TB/s of the cache, 450 TFLOP/s
+//   4 x 61 x 32 (4) x 128, 30011 tokens: 180 us, 530 TFLOP/s
 // Before the first products the block spends 8 us (start, shares, queries), at
 // its end 4 us on the 64 to 128 KB of its partial result.
 #include <algorithm>
