@@ -9,7 +9,7 @@
 namespace fpb {
 namespace {
 
-constexpr int kAppendThreads = 256, kMaxHalf = 128, kMaxSpan = 4;
+constexpr int kAppendThreads = 128, kMaxHalf = 128, kMaxSpan = 2;
 
 struct AppendArgs {
   const void *q, *k, *v;
@@ -73,7 +73,9 @@ __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
 
 // Some tokens' heads: block (x, part) takes the `span` rows from x * span on
 // (row b * nodes + n: a token) and of their heads every gridDim.y-th group, LG
-// lanes a head vector, eight elements a lane (LG * 8 >= head_dim).
+// lanes a head vector, two pieces of eight elements a lane (LG * 16 >= head_dim).
+// Where the rotated dimensions' halves come in eights, a lane's second piece
+// holds the partners of its first.
 //  norm    x * rsqrt(mean x^2 + eps) * gamma, f32
 //  rotate  dimensions i and i + half by (position + depth) * theta^(-i/half).
 //          The turn is taken as a 64-bit fraction, an exact product of whole
@@ -81,32 +83,40 @@ __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
 //          is off by position * 2^-24 radians, 0.002 at position 32768.
 //          The token's cosines and sines are made once for its heads.
 //  write   q' as given, k' and v as codes and exponents at row position + n
-// A decode step is bound by latency (loads of the positions, then sines: 3.3 us
-// for 8 x 1 x 48 heads x 128), a prompt by instructions: 2 x 4096 x 48 heads x
-// 128, bf16, takes 71 us for 235 MB (3.3 TB/s), 270 instructions for a warp's
-// two head vectors.
+// A decode step is bound by latency (loads of the positions, then sines: 3.5 us
+// for 8 x 1 x 20 heads x 256), a prompt by instructions and their latency: 2 x
+// 4096 x 48 heads x 128, bf16, takes 48 us for 185 MB (3.9 TB/s).  Sixteen
+// elements a lane, not eight: a vector's sums, addresses and index take as many
+// instructions for either (71 us), and partners in one lane need no shuffles.
+// Blocks of four warps, seven an SM (of eight warps 56 us; eight an SM 50, fewer
+// than seven 49).
 template <typename T, int LG>
-__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 7) kv8_append_kernel(const __grid_constant__ AppendArgs a) {
   pdl_enter();
   __shared__ float2 turn_s[kMaxSpan][kMaxHalf];  // cosine, sine
-  __shared__ float xs[kAppendThreads / LG][LG * 8];
+  __shared__ float xs[kAppendThreads / LG][LG * 16];
   __shared__ int depth_s[kMaxSpan], pos_s[kMaxSpan];
   __shared__ size_t to_s[kMaxSpan];  // the rows' places in the cache, in rows
   const int tid = threadIdx.x, lane = tid % LG, item = tid / LG;
   constexpr int kItems = kAppendThreads / LG;
   const int row0 = blockIdx.x * a.span, span = min(a.span, a.rows - row0);
-  const int D = a.head_dim, c0 = lane * 8, heads = a.q_heads + 2 * a.kv_heads, half = a.rotary_dim / 2;
+  const int D = a.head_dim, heads = a.q_heads + 2 * a.kv_heads, half = a.rotary_dim / 2;
+  const int turning = half % 8 == 0 ? half / 8 : 0;  // lanes whose pieces are partners
+  const bool turns = lane < turning;
+  const int c0 = turns ? 8 * lane : 16 * lane, col[2] = {c0, turns ? c0 + half : c0 + 8};  // (16 turning = 2 half)
   // a head's elements are asked for one head ahead, the first before the sines
-  Eight<T> raw;
+  Eight<T> raw[2];
   auto ask = [&](int rl, int h) {
-    raw.zero();
+    raw[0].zero();
+    raw[1].zero();
     if (rl >= span || c0 >= D) return;
     const size_t row = row0 + rl;
     const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + a.kv_heads;
     const T *src = is_q   ? static_cast<const T *>(a.q) + row * a.q_pitch + (size_t)h * a.q_head
                    : is_k ? static_cast<const T *>(a.k) + row * a.k_pitch + (size_t)(h - a.q_heads) * D
                           : static_cast<const T *>(a.v) + row * a.v_pitch + (size_t)(h - a.q_heads - a.kv_heads) * D;
-    raw.load(src + c0, a.vec);
+    raw[0].load(src + col[0], a.vec);
+    raw[1].load(src + col[1], a.vec);
   };
   int rl = 0, h = blockIdx.y * kItems + item;
   while (h >= heads) {
@@ -139,17 +149,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const __grid
     }
     __syncthreads();
   }
-  // The sines of a lane's columns serve all of a row's heads: in registers, with
-  // 1 and 0 past the rotated dimensions.
-  const bool lanes_turn = half > 0 && half % 8 == 0, low = c0 < half;
-  const int partner = (tid & 31) + (c0 >= 2 * half ? 0 : low ? half / 8 : -half / 8);
-  int turned = -1;
+  int turned = -1;  // the row whose cosines and sines the lane holds: they serve all of its heads
   float cs[8], sn[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    cs[i] = 1.0f;
-    sn[i] = 0.0f;
-  }
   // (the loop ends together for the whole block: its warps' lanes shuffle)
   const int total = span * heads;
   for (int i0 = blockIdx.y * kItems; i0 < total; i0 += gridDim.y * kItems) {
@@ -158,9 +159,12 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const __grid
     const bool live = rl < span && c0 < D;
     const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + a.kv_heads;
     const int kvh = is_q ? 0 : h - a.q_heads - (is_k ? 0 : a.kv_heads), here = h, at = min(rl, span - 1);
-    float x[8];
-    if (depth < 0) raw.zero();  // rows of nodes that are not there: zeros
-    raw.values(x);
+    float x[2][8];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (depth < 0) raw[j].zero();  // rows of nodes that are not there: zeros
+      raw[j].values(x[j]);
+    }
     h += gridDim.y * kItems;
     while (h >= heads) {
       h -= heads;
@@ -170,79 +174,96 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const __grid
     const float *gamma = is_q ? a.q_gamma : is_k ? a.k_gamma : nullptr;
     float ss = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = fmaf(x[j][i], x[j][i], ss);
 #pragma unroll
     for (int o = LG / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     if (gamma && live) {
       const float scale = __frsqrt_rn(fmaf(ss, a.inv_d, a.eps));
-      const float4 g0 = __ldg(reinterpret_cast<const float4 *>(gamma + c0)),
-                   g1 = __ldg(reinterpret_cast<const float4 *>(gamma + c0) + 1);
-      const float g[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * scale * g[i];
+      for (int j = 0; j < 2; ++j) {
+        const float4 g0 = __ldg(reinterpret_cast<const float4 *>(gamma + col[j])),
+                     g1 = __ldg(reinterpret_cast<const float4 *>(gamma + col[j]) + 1);
+        const float g[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[j][i] = x[j][i] * scale * g[i];
+      }
     }
-    if (lanes_turn) {  // the partners of a lane's eight lie in one lane
-      if (at != turned && c0 < 2 * half) {
-        const float2 *t = &turn_s[at][low ? c0 : c0 - half];
+    if (turning) {
+      if (turns && (is_q || is_k)) {
+        if (at != turned) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            cs[i] = turn_s[at][c0 + i].x;
+            sn[i] = turn_s[at][c0 + i].y;
+          }
+          turned = at;
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          cs[i] = t[i].x;
-          sn[i] = low ? -t[i].y : t[i].y;
+          const float u = x[0][i], v = x[1][i];
+          x[0][i] = fmaf(-v, sn[i], u * cs[i]);
+          x[1][i] = fmaf(u, sn[i], v * cs[i]);
         }
-        turned = at;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float y = __shfl_sync(0xffffffffu, x[i], partner);
-        if (is_q || is_k) x[i] = fmaf(y, sn[i], x[i] * cs[i]);
       }
     } else if (half > 0) {
-      const bool turns = live && (is_q || is_k) && c0 < 2 * half;
-      if (turns) {
+      const bool rotates = live && (is_q || is_k) && c0 < 2 * half;
+      if (rotates) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) xs[item][c0 + i] = x[i];
+        for (int i = 0; i < 16; ++i) xs[item][c0 + i] = x[i >> 3][i & 7];
       }
       __syncwarp();
-      if (turns) {
+      if (rotates) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 16; ++i) {
           const int c = c0 + i;
+          float &v = x[i >> 3][i & 7];
           if (c < half)
-            x[i] = x[i] * turn_s[at][c].x - xs[item][c + half] * turn_s[at][c].y;
+            v = v * turn_s[at][c].x - xs[item][c + half] * turn_s[at][c].y;
           else if (c < 2 * half)
-            x[i] = x[i] * turn_s[at][c - half].x + xs[item][c - half] * turn_s[at][c - half].y;
+            v = v * turn_s[at][c - half].x + xs[item][c - half] * turn_s[at][c - half].y;
         }
       }
       __syncwarp();
     }
     float amax = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[j][i]));
 #pragma unroll
     for (int o = LG / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if (!live) continue;
     if (is_q) {
-      const size_t o = (row * a.q_heads + here) * D + c0;
-      if (a.q_out_bf16) {
-        uint4 w;
-        w.x = pack_bf16x2(x[0], x[1]);
-        w.y = pack_bf16x2(x[2], x[3]);
-        w.z = pack_bf16x2(x[4], x[5]);
-        w.w = pack_bf16x2(x[6], x[7]);
-        *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(a.q_out) + o) = w;
-      } else {
-        float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(a.q_out) + o);
-        dst[0] = make_float4(x[0], x[1], x[2], x[3]);
-        dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+      const size_t head = (row * a.q_heads + here) * D;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const size_t o = head + col[j];
+        const float *y = x[j];
+        if (a.q_out_bf16) {
+          *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(a.q_out) + o) =
+              make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
+                         pack_bf16x2(y[6], y[7]));
+        } else {
+          float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(a.q_out) + o);
+          dst[0] = make_float4(y[0], y[1], y[2], y[3]);
+          dst[1] = make_float4(y[4], y[5], y[6], y[7]);
+        }
       }
     } else if (depth >= 0) {
       const int e = kv8_exponent(amax);
       const float inv = pow2i(-e);
       const size_t vec = to_s[at] * a.kv_heads + kvh;
-      uint2 w;
-      w.x = e4m3x2(x[0] * inv, x[1] * inv) | e4m3x2(x[2] * inv, x[3] * inv) << 16;
-      w.y = e4m3x2(x[4] * inv, x[5] * inv) | e4m3x2(x[6] * inv, x[7] * inv) << 16;
-      *reinterpret_cast<uint2 *>((is_k ? a.k_codes : a.v_codes) + vec * D + c0) = w;
+      uint8_t *codes = (is_k ? a.k_codes : a.v_codes) + vec * D;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float *y = x[j];
+        uint2 w;
+        w.x = e4m3x2(y[0] * inv, y[1] * inv) | e4m3x2(y[2] * inv, y[3] * inv) << 16;
+        w.y = e4m3x2(y[4] * inv, y[5] * inv) | e4m3x2(y[6] * inv, y[7] * inv) << 16;
+        *reinterpret_cast<uint2 *>(codes + col[j]) = w;
+      }
       if (lane == 0) (is_k ? a.k_exp : a.v_exp)[vec] = (uint8_t)(e + 127);
     }
   }
@@ -353,22 +374,22 @@ int check_cache(const char *name, const void *kc, const void *vc, const void *ke
 
 template <typename T>
 int run_append(AppendArgs a, size_t rows, cudaStream_t s) {
-  const int lanes = a.head_dim / 8;
-  const int lg = lanes <= 8 ? 8 : lanes <= 16 ? 16 : 32;
+  const int lanes = a.head_dim / 16;
+  const int lg = lanes <= 4 ? 4 : lanes <= 8 ? 8 : 16;
   const int heads = a.q_heads + 2 * a.kv_heads, per = kAppendThreads / lg;
-  // Few rows: one group of heads a block (8 rows of 48 heads 3.3 us, with all
-  // heads in a block 4.6).  Beyond four blocks an SM a block takes all of a row's
-  // heads (1024 rows 12.2 us, with a group a block 18.4), and of four rows from
-  // sixteen blocks an SM on: the rows' positions and sines are then made for all
-  // of them at once (8192 rows 71 us, with one row a block 80; 512 rows 11.8
-  // with four, 7.8 with one; 2048 rows 23 either way).
+  // Few rows: one group of heads a block (8 rows of 20 heads x 256 3.4 us, with
+  // all heads in a block 4.8).  Beyond eight blocks an SM a block takes all of a
+  // row's heads (1024 rows of 48 heads x 128 10.6 us, with a group a block 12),
+  // and of two rows from sixteen rows an SM on: the rows' positions and sines are
+  // then made for both at once (8192 rows 49 us, with one row a block 53, with
+  // four 52; 2048 rows 17 with one, 18 with two).
   const int parts = (heads + per - 1) / per;
   a.span = rows >= (size_t)sm_count() * 16 ? kMaxSpan : 1;
-  const size_t want = std::min<size_t>(parts, std::max<size_t>(1, (size_t)sm_count() * 4 / rows));
+  const size_t want = std::min<size_t>(parts, std::max<size_t>(1, (size_t)sm_count() * 8 / rows));
   const dim3 grid((unsigned)((rows + a.span - 1) / a.span), (unsigned)want);
-  cudaError_t e = lg == 8    ? launch_pdl(kv8_append_kernel<T, 8>, grid, kAppendThreads, 0, s, a)
-                  : lg == 16 ? launch_pdl(kv8_append_kernel<T, 16>, grid, kAppendThreads, 0, s, a)
-                             : launch_pdl(kv8_append_kernel<T, 32>, grid, kAppendThreads, 0, s, a);
+  cudaError_t e = lg == 4   ? launch_pdl(kv8_append_kernel<T, 4>, grid, kAppendThreads, 0, s, a)
+                  : lg == 8 ? launch_pdl(kv8_append_kernel<T, 8>, grid, kAppendThreads, 0, s, a)
+                            : launch_pdl(kv8_append_kernel<T, 16>, grid, kAppendThreads, 0, s, a);
   if (e != cudaSuccess) return cuda_fail(e, "kv8_append_kernel");
   FPB_LAUNCH_CHECK("kv8_append_kernel");
   return FPB_OK;
