@@ -239,11 +239,12 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) tree_verify_kernel(const __
     Best top{-INFINITY, 0x7fffffff};
     float s = 0.0f;
     constexpr int N = 16 / sizeof(T), kLoads = kHold / N;
-    // The slice stays in registers between the two where it fills at least half of
-    // them, else it goes through shared memory (12 sessions, 9 drafts taken, f32:
-    // 96000 tokens 36 us in registers, 41 through shared memory; 32000 29 and 28).
+    // The slice is read at once, and stays in registers between the two, where it
+    // fills at least half of them; else it is read in batches and goes through
+    // shared memory (12 sessions, 9 drafts taken, f32: 96000 tokens 36 us in
+    // registers, 41 else; 32000 29 and 28; greedy, 16 x 9 and 151936 40.5 and 42).
     constexpr int kAll = kHold * kVerifyThreads;
-    if (!greedy && a.vec && len % N == 0 && a.slice <= kAll && a.slice * 2 >= kAll) {
+    if (a.vec && len % N == 0 && a.slice <= kAll && a.slice * 2 >= kAll) {
       const T *row = logits_of(node);
       uint4 v[kLoads];
       float m = -INFINITY;
@@ -260,28 +261,41 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) tree_verify_kernel(const __
         const float x = __uint_as_float(N == 4 ? w : j & 1 ? w & 0xffff0000u : w << 16);
         return fabsf(x) <= 3.402823466e38f ? x : -INFINITY;
       };
+      if (greedy) {
 #pragma unroll
-      for (int k = 0; k < kLoads; ++k)
+        for (int k = 0; k < kLoads; ++k)
 #pragma unroll
-        for (int j = 0; j < N; ++j) m = fmaxf(m, value(k, j));
-      top = block_best(Best{m, 0});
-      const float bias = top.v == -INFINITY ? 0.0f : -top.v * a.scale_log2;
+          for (int j = 0; j < N; ++j) {
+            const float x = value(k, j);
+            if (x > top.v) top = Best{x, v0 + (k * kVerifyThreads + tid) * N + j};
+          }
+      } else {
 #pragma unroll
-      for (int k = 0; k < kLoads; ++k) {
-        const int i = (k * kVerifyThreads + tid) * N;
-        if (i >= len) break;
+        for (int k = 0; k < kLoads; ++k)
 #pragma unroll
-        for (int j = 0; j < N; j += 4) {
-          float4 e;
-          e.x = pow2(fmaf(value(k, j), a.scale_log2, bias));
-          e.y = pow2(fmaf(value(k, j + 1), a.scale_log2, bias));
-          e.z = pow2(fmaf(value(k, j + 2), a.scale_log2, bias));
-          e.w = pow2(fmaf(value(k, j + 3), a.scale_log2, bias));
-          s += (e.x + e.y) + (e.z + e.w);
-          *reinterpret_cast<float4 *>(r + i + j) = e;
-        }
+          for (int j = 0; j < N; ++j) m = fmaxf(m, value(k, j));
+        top.v = m;
       }
-      s = block_sum(s);
+      top = block_best(top);
+      const float bias = top.v == -INFINITY ? 0.0f : -top.v * a.scale_log2;
+      if (!greedy) {
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k) {
+          const int i = (k * kVerifyThreads + tid) * N;
+          if (i >= len) break;
+#pragma unroll
+          for (int j = 0; j < N; j += 4) {
+            float4 e;
+            e.x = pow2(fmaf(value(k, j), a.scale_log2, bias));
+            e.y = pow2(fmaf(value(k, j + 1), a.scale_log2, bias));
+            e.z = pow2(fmaf(value(k, j + 2), a.scale_log2, bias));
+            e.w = pow2(fmaf(value(k, j + 3), a.scale_log2, bias));
+            s += (e.x + e.y) + (e.z + e.w);
+            *reinterpret_cast<float4 *>(r + i + j) = e;
+          }
+        }
+        s = block_sum(s);
+      }
     } else {
       prefetch();
       for_row<true>(logits_of(node), len, a.vec, greedy ? nullptr : r, [&](float x, float &y, int i) {
