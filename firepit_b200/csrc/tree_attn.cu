@@ -150,29 +150,29 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
     for (int i = 0; i < min(count, kStages); ++i) fetch(i);
   __syncwarp();
 
-  // queries: a warp takes rows w, w + 4, ...; eight columns a lane
-  for (int r = w; r < NR; r += kRowsWarps) {
-    const int row = r, n = row / a.group, h = kvh * a.group + row % a.group;
-    float x[8];
+  // queries: a warp takes rows w, w + 4, ...; eight columns a lane, all rows' asked for at once
+  constexpr int kMine = NR / kRowsWarps;
+  float x[kMine][8];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int row = w + i * kRowsWarps, n = row / a.group, col = lane * 8;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[i][k] = 0.0f;
+    if (row < rows && col < D)
+      load_q8(a, ((size_t)b * a.nodes + n) * a.q_pitch + (size_t)(kvh * a.group + row - n * a.group) * a.q_head + col, x[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int r = w + i * kRowsWarps;
     float amax = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int col = lane * 8 + i;
-      x[i] = row < rows && col < D
-                 ? load_q(a, ((size_t)b * a.nodes + n) * a.q_pitch + (size_t)h * a.q_head + col) : 0.0f;
-      amax = fmaxf(amax, fabsf(x[i]));
-    }
-    amax = warp_max(amax);
-    const int e = q_exponent(amax);
+    for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(x[i][k]));
+    const int e = q_exponent(warp_max(amax));
     const float f = pow2i(-e);
-    if (lane * 8 < DP) {
-      uint4 o;
-      o.x = pack_f16x2(x[0] * f, x[1] * f);
-      o.y = pack_f16x2(x[2] * f, x[3] * f);
-      o.z = pack_f16x2(x[4] * f, x[5] * f);
-      o.w = pack_f16x2(x[6] * f, x[7] * f);
-      *reinterpret_cast<uint4 *>(qs + r * Sh::kQPitch + lane * 8) = o;
-    }
+    if (lane * 8 < DP)
+      *reinterpret_cast<uint4 *>(qs + r * Sh::kQPitch + lane * 8) =
+          make_uint4(pack_f16x2(x[i][0] * f, x[i][1] * f), pack_f16x2(x[i][2] * f, x[i][3] * f),
+                     pack_f16x2(x[i][4] * f, x[i][5] * f), pack_f16x2(x[i][6] * f, x[i][7] * f));
     if (lane == 0) fac_s[r] = pow2i(e) * a.scale_log2;
   }
   if (w == 0) {
@@ -232,10 +232,10 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
   uint32_t xr[4] = {127, 127, 127, 127};
   if (count > 0) load_exps(first, xr);
   bool ok = true;
-  for (int i = 0; i < count; ++i) {
-    const int step = first + i * kRowsWarps;
-    const uint8_t *kst = mine_ring + (i % kStages) * Sh::kStage, *vst = kst + Sh::kStage / 2;
-    if (ok) ok = mbar_wait(&full[w][i % kStages], (i / kStages) & 1, &abort_s);
+  for (int at_step = 0; at_step < count; ++at_step) {
+    const int step = first + at_step * kRowsWarps;
+    const uint8_t *kst = mine_ring + (at_step % kStages) * Sh::kStage, *vst = kst + Sh::kStage / 2;
+    if (ok) ok = mbar_wait(&full[w][at_step % kStages], (at_step / kStages) & 1, &abort_s);
     if (!ok && a.error) {  // (a wait that ran out: the results are void, but the loop ends)
       *(volatile int *)&abort_s = 1;
       atomicCAS(a.error, 0, kErrRowsWait);
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
       kf[h] = kv8_factor(xr[h]);
       ve[h] = kv8_value_exponent(xr[2 + h]);
     }
-    if (i + 1 < count) load_exps(step + kRowsWarps, xr);
+    if (at_step + 1 < count) load_exps(step + kRowsWarps, xr);
     uint32_t vr[4][kVPieces][kVBytes / 4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
         }
       }
     __syncwarp();  // the stage is read
-    if (lane == 0 && i + kStages < count) fetch(i + kStages);
+    if (lane == 0 && at_step + kStages < count) fetch(at_step + kStages);
     __syncwarp();
   }
   if (!ok)  // copies still in flight land before the block ends

@@ -101,6 +101,27 @@ __device__ __forceinline__ float load_q(const TreeArgs &a, size_t at) {
                   : static_cast<const float *>(a.q)[at];
 }
 
+// Eight elements of q from `at` on (a multiple of 8).
+__device__ __forceinline__ void load_q8(const TreeArgs &a, size_t at, float (&x)[8]) {
+  if (!a.q_vec) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = load_q(a, at + k);
+  } else if (a.q_bf16) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) + at);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      x[2 * k] = __uint_as_float(w[k] << 16);
+      x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+    }
+  } else {
+    const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at);
+    const float4 u = p[0], v = p[1];
+    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+    x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+  }
+}
+
 // Power of two that takes a query row into f16: its largest magnitude to
 // [2^8, 2^9), so that f16's 11 bits hold down to 2^-22 of it (f16 products
 // round at 2^-11; the scores' f32 sums and the factor are exact in it).

@@ -86,8 +86,8 @@ struct TileShared {
 
 // Token tiles of session b (0: none of its nodes is there).
 __device__ __forceinline__ int session_tiles(const TreeArgs &a, int b, int BT) {
-  if (a.parents && a.parents[(size_t)b * a.nodes] != -1) return 0;
-  return (seen_rows(a, a.positions[b], a.nodes - 1) + BT - 1) / BT;
+  const int root = a.parents ? a.parents[(size_t)b * a.nodes] : -1, pos = a.positions[b];  // (both asked for at once)
+  return root == -1 ? (seen_rows(a, pos, a.nodes - 1) + BT - 1) / BT : 0;
 }
 
 __device__ __forceinline__ int session_units(const TreeArgs &a, int b, int BT) {
@@ -352,24 +352,7 @@ __global__ void __launch_bounds__(256) tree_attn_prep_kernel(const __grid_consta
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[i][k] = 0.0f;
     if (row >= rows || col >= D) continue;
-    const size_t at = ((size_t)b * a.nodes + n) * a.q_pitch + (size_t)(kvh * a.group + (row - n * a.group)) * a.q_head + col;
-    if (!a.q_vec) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[i][k] = load_q(a, at + k);
-    } else if (a.q_bf16) {
-      const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) + at);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        x[i][2 * k] = __uint_as_float(w[k] << 16);
-        x[i][2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-      }
-    } else {
-      const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at);
-      const float4 u = p[0], v = p[1];
-      x[i][0] = u.x; x[i][1] = u.y; x[i][2] = u.z; x[i][3] = u.w;
-      x[i][4] = v.x; x[i][5] = v.y; x[i][6] = v.z; x[i][7] = v.w;
-    }
+    load_q8(a, ((size_t)b * a.nodes + n) * a.q_pitch + (size_t)(kvh * a.group + row - n * a.group) * a.q_head + col, x[i]);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
