@@ -150,6 +150,21 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
     for (int i = 0; i < min(count, kStages); ++i) fetch(i);
   __syncwarp();
 
+  // the exponents of the lane's tokens, token_at(g) and that + 8
+  const int own = token_at<DP>(g);
+  const size_t ex0 = (size_t)b * a.max_seq * a.kv_heads + kvh;
+  auto load_exps = [&](int step, uint32_t(&x)[4]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int t = step * 16 + own + 8 * h;
+      const size_t at = ex0 + (size_t)t * a.kv_heads;
+      x[h] = t < total ? a.k_exp[at] : 127;
+      x[2 + h] = t < total ? a.v_exp[at] : 127;
+    }
+  };
+  uint32_t xr[4] = {127, 127, 127, 127};
+  if (count > 0) load_exps(first, xr);
+
   // queries: a warp takes rows w, w + 4, ...; eight columns a lane, all rows' asked for at once
   constexpr int kMine = NR / kRowsWarps;
   float x[kMine][8];
@@ -160,6 +175,10 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
     for (int k = 0; k < 8; ++k) x[i][k] = 0.0f;
     if (row < rows && col < D)
       load_q8(a, ((size_t)b * a.nodes + n) * a.q_pitch + (size_t)(kvh * a.group + row - n * a.group) * a.q_head + col, x[i]);
+  }
+  if (w == 0) {
+    const Sight s = sight_of(a, b, lane < rows ? lane / a.group : a.nodes, pos);
+    if (lane < NR) sight_s[lane] = s;
   }
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
@@ -174,10 +193,6 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
           make_uint4(pack_f16x2(x[i][0] * f, x[i][1] * f), pack_f16x2(x[i][2] * f, x[i][3] * f),
                      pack_f16x2(x[i][4] * f, x[i][5] * f), pack_f16x2(x[i][6] * f, x[i][7] * f));
     if (lane == 0) fac_s[r] = pow2i(e) * a.scale_log2;
-  }
-  if (w == 0) {
-    const Sight s = sight_of(a, b, lane < rows ? lane / a.group : a.nodes, pos);
-    if (lane < NR) sight_s[lane] = s;
   }
   __syncthreads();
   // the lane's rows: 2 c, 2 c + 1 and, with 16 rows, those + 8
@@ -201,19 +216,6 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
         }
   }
 
-  // the exponents of the lane's tokens, token_at(g) and that + 8
-  const int own = token_at<DP>(g);
-  const size_t ex0 = (size_t)b * a.max_seq * a.kv_heads + kvh;
-  auto load_exps = [&](int step, uint32_t(&x)[4]) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int t = step * 16 + own + 8 * h;
-      const size_t at = ex0 + (size_t)t * a.kv_heads;
-      x[h] = t < total ? a.k_exp[at] : 127;
-      x[2 + h] = t < total ? a.v_exp[at] : 127;
-    }
-  };
-
   float acc[kMT][kNT][4];
 #pragma unroll
   for (int i = 0; i < kMT; ++i)
@@ -229,8 +231,6 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
       m[i][e] = -INFINITY;
       l[i][e] = 0.0f;
     }
-  uint32_t xr[4] = {127, 127, 127, 127};
-  if (count > 0) load_exps(first, xr);
   bool ok = true;
   for (int at_step = 0; at_step < count; ++at_step) {
     const int step = first + at_step * kRowsWarps;
