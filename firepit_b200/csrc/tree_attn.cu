@@ -53,12 +53,12 @@ using namespace sm100;
 // the value's to the weight's exponent.
 // The tokens as M, not the rows: eight rows take half as many instructions, and
 // a token's exponents belong to one lane (8 x 8192 tokens x 2 heads x 256, 16
-// rows: 27.5 us against 32 with the rows as M).
+// rows: 27.9 us against 32 with the rows as M; 24.5 now).
 // Long caches are bound by their bytes (from 8 x 16384 to 8 x 32768 tokens, 8 rows
-// x 256: 134 MB more in 20 us, 6.7 TB/s), shorter ones by some 11 us besides:
+// x 256: 134 MB more in 20 us, 6.7 TB/s), shorter ones by some 10 us besides:
 // the launches, the start (positions, then the first codes), the last steps'
 // latency, the splits' results and their merge.  16 x 1 node x 16 heads (2 kv) x
-// 256, 8192 tokens: 32 us, 3.7 TB/s.
+// 256, 8192 tokens: 30.4 us, 3.9 TB/s.
 constexpr int kRowsThreads = 128, kRowsWarps = 4;
 constexpr int kErrRowsWait = 503;
 
@@ -557,7 +557,7 @@ struct Plan {
 
 // Past 16 rows a key/value head the tcgen05 kernel takes over, which takes 128 of
 // them in the time of 17.  Up to 16 it is the slower one: 16 rows x 256 columns,
-// 8 x 8192 tokens 47 us here 27.5, 1 x 30000 36 and 22, 64 x 1000 51 and 28.
+// 8 x 8192 tokens 47 us, here 24.5, 1 x 30000 36 and 22, 64 x 1000 51 and 28.
 bool wants_tiles(size_t nodes, size_t q_heads, size_t kv_heads) { return nodes * (q_heads / kv_heads) > 16; }
 
 Plan plan_for(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, size_t head_dim, size_t max_seq) {

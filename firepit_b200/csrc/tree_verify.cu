@@ -127,10 +127,10 @@ __device__ __forceinline__ void to_l2(const void *p, int bytes) {
 }
 
 // Bytes: the visited nodes' logits once, once more per refused draft the draft's
-// row, the noise.  Measured: 16 sessions x 9 drafts drawn, 151936 tokens, f32
-// logits 33 us (the 83 MB of its walks at 2.5 TB/s), 8 x 32 tree 15.5 us, 2 x 5
-// greedy 14 us.  A step takes 4 us: maximum 1.6, powers 0.7, sums 0.3, the
-// cluster's barrier 0.8, decisions 0.5.
+// row, the noise.  Measured, 151936 tokens: 16 sessions x 9 drafts drawn, bf16
+// logits, 33 to 39 us by its walks (83 MB at 2.1 to 2.5 TB/s), 8 x 32 tree 15 us,
+// 2 x 5 greedy 14 to 16.  A step takes 4 us: maximum 1.6, powers 0.7, sums 0.3,
+// the cluster's barrier 0.8, decisions 0.5; a greedy one 3.
 // Block (cluster of kVerifyCluster CTAs) per session: CTA `rank` owns the
 // vocabulary's slice [rank * slice, +slice) and keeps what is left of the
 // node's distribution there in shared memory, so that a refused child's pass
