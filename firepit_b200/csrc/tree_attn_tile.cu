@@ -483,7 +483,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       soft_sync();
       if (!sh->more) break;
       const int j0 = sh->seg.j0, j1 = sh->seg.j1, pos = sh->seg.pos;
-      const float f = a.q_fac[(size_t)sh->seg.item * kTileRows + r_own];
+      // Only a segment with tiles takes up queries: what it then waits for (its
+      // last product) shows that the MMA warp has seen this phase of qready, and
+      // so the next may complete.  Nothing would wait in one without (what a
+      // block has of a row tile may lie in its take-up or past its last row).
+      const bool tiles = j1 > j0;
+      const float f = tiles ? a.q_fac[(size_t)sh->seg.item * kTileRows + r_own] : 0.0f;
       uint64_t sight = 0;
       if (part == 0) {
         const int n = (sh->seg.rt * kTileRows + r_own) / a.group;
@@ -492,7 +497,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         else if (n < a.nodes && pos >= 0 && pos < a.max_seq - n)
           sight = n + 1;
       }
-      {
+      if (tiles) {
         // 16 columns of the row at a time; a warp's loads are 512 bytes together
         const uint4 *q = a.q16 + (size_t)sh->seg.item * (a.head_dim / 8) * kTileRows + r_own;
         constexpr int kQ = DP / 16 / kParts;
@@ -512,7 +517,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (part == 0) sh->sight[r_own] = sight;
       tmem_st_wait();
       quad_sync(quad);
-      if (lane == 0) mbar_arrive(&sh->qready);
+      if (tiles && lane == 0) mbar_arrive(&sh->qready);
       float m = kLowest;
       uint64_t l2 = 0;
       for (int j = j0; j < j1; ++j, ++g) {
@@ -587,13 +592,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         float l = 0.0f;
 #pragma unroll
         for (int i = 0; i < kParts; ++i) l += sh->red[i][r_own];
-        a.part_ml[slot * kTileRows + r_own] = make_float2(j1 > j0 ? m : -INFINITY, l);
+        a.part_ml[slot * kTileRows + r_own] = make_float2(tiles ? m : -INFINITY, l);
       }
       if (tid == 0) {  // whose slots hold the row tile: from its first block's to its last's
         if (sh->seg.starts) a.shares[sh->seg.item].x = whole ? -1 : (int)slot;
         if (sh->seg.ends) a.shares[sh->seg.item].y = (int)blockIdx.x;
       }
-      if (j1 > j0) {
+      if (tiles) {
         if (ok) ok = mbar_wait(&sh->vempty[(g - 1) % ST], ((g - 1) / ST) & 1, abort_s);
         if (!ok) give_up(a.error, abort_s);
         __syncwarp();
@@ -636,12 +641,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       __syncwarp();
     };
-    for (int seg = 0; ok && walk.next(a, BT, sg); ++seg) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&sh->qready, seg & 1, abort_s));
+    for (uint32_t taken = 0; ok && walk.next(a, BT, sg);) {
+      if (sg.j1 <= sg.j0) continue;
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh->qready, taken++ & 1, abort_s));
       if (!ok) break;
       tc_fence_after();
-      const uint32_t g0 = g, g1 = g + max(0, sg.j1 - sg.j0);
-      if (g1 > g0) scores(g0);
+      const uint32_t g0 = g, g1 = g + (sg.j1 - sg.j0);
+      scores(g0);
       for (; ok && g < g1; ++g) {
         if (g + 1 < g1) scores(g + 1);
         const uint32_t st = g % ST;

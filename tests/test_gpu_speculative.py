@@ -534,3 +534,15 @@ def test_verified_tokens_are_distributed_as_the_target(F, torch, drawn):
     freq = np.bincount(first, minlength=V) / b
     assert (np.abs(freq - p) <= 5 * np.sqrt(p * (1 - p) / b)).all(), (freq, p)
     assert (path[:, 1] > 0).mean() > 0.3
+
+
+# ---- chains of several row tiles ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("b,n,hq,hk,d,s,pos", [
+    (2, 300, 8, 8, 256, 600, [0, 0]), (3, 260, 15, 5, 192, 500, [0, 77, 200]), (2, 333, 8, 4, 256, 700, [1, 300])])
+def test_chains_whose_blocks_hold_segments_without_tiles(F, torch, b, n, hq, hk, d, s, pos):
+    """Row tiles that end before their session's last tile of tokens, cut so that
+    blocks hold segments without any tile before others: in the first and third
+    sixteen blocks have two of them in a row, in the second seven."""
+    rng = np.random.default_rng(n)
+    cache = _cache(F, torch, rng, b, s, hk, d)
+    _check_attention(F, torch, rng, cache, pos, None, n, hq, gate=False)
