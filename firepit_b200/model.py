@@ -496,7 +496,8 @@ class SpeculativeDecoder(Decoder):
     attends and verifies the tree, moves the accepted path's rows together,
     advances the positions by ``count`` and makes ``next`` the new first token;
     ``emitted`` [sessions, nodes] holds the tokens that the step added, -1 after
-    them.  temperature 0: greedy; above it ``accept`` [sessions, nodes] and
+    them.  A session whose parents begin with -2 sits a step out: nothing of it
+    changes.  temperature 0: greedy; above it ``accept`` [sessions, nodes] and
     ``noise`` [sessions, vocab] hold the step's random numbers (``draw``) and
     ``draft``, where set, the drafts' probabilities.  sessions * nodes <= 16
     (the decode GEMVs' rows)."""
@@ -555,7 +556,8 @@ class SpeculativeDecoder(Decoder):
         left = self.count[:, None] - 1 - self.at
         self.emitted.copy_(torch.where(left > 0, taken, torch.where(left == 0, self.next[:, None], -1)))
         self.positions.add_(self.count)
-        self.tree[:, 0].copy_(self.next)
+        # (a session without a tree has no next token: it keeps its own, which the next step may embed)
+        self.tree[:, 0].copy_(torch.where(self.count > 0, self.next, self.tree[:, 0]))
 
     def feed(self, tokens) -> None:
         """Runs known tokens [sessions, n] (device int32) through the model,

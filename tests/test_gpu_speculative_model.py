@@ -222,3 +222,31 @@ def test_sampled_generation_is_a_graph_too(torch, model):
         outs.append(got)
     assert outs[0] == outs[1]
     _no_error()
+
+
+def test_a_session_without_a_tree_keeps_its_place(torch, model):
+    """A session whose node 0 is absent for a step: no token, no row, no error,
+    and it goes on after it as if the step had not been."""
+    from firepit_b200.model import SpeculativeDecoder
+    sh = torch.cuda.current_stream().cuda_stream
+    runs = []
+    for parked in (False, True):
+        dec = SpeculativeDecoder(model, 2, 4, 64)
+        dec.feed(torch.tensor([[3, 14, 15], [92, 65, 35]], dtype=torch.int32, device="cuda"))
+        dec.tree[:, 0] = torch.tensor([7, 8], dtype=torch.int32)
+        dec.parents.copy_(torch.tensor([[-1, -2, -2, -2]] * 2, dtype=torch.int32))
+        if parked:
+            dec.parents[1, 0] = -2
+            dec.step(sh)
+            assert dec.count.tolist() == [1, 0] and dec.positions.tolist() == [4, 3]
+            assert dec.emitted[1].tolist() == [-1] * 4 and dec.tree[1, 0].item() == 8
+            dec.parents[1, 0], dec.parents[0, 0] = -1, -2
+        else:
+            dec.parents[0, 0] = -2
+        got = []
+        for _ in range(4):
+            dec.step(sh)
+            got.append(dec.emitted[1, 0].item())
+        runs.append((got, dec.positions[1].item()))
+    assert runs[0] == runs[1] and min(runs[0][0]) >= 0
+    _no_error()
