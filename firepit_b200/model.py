@@ -578,9 +578,14 @@ class SpeculativeDecoder(Decoder):
         [sessions, length]; drafter(history: list[int], nodes) -> (tokens,
         parents) proposes each step's tree after its first node (lists of at
         most nodes - 1 entries; a parent is 0 for the first node, k for the
-        k-th drafted token).  Returns the new tokens of each session."""
+        k-th drafted token).  A session that has its tokens sits the other
+        sessions' steps out, so none goes more than `nodes` rows past them.
+        Returns the new tokens of each session; a device error, which would
+        make them doubtful, is raised (and left for ``device_error`` to
+        read)."""
         import torch
 
+        from .gemm import device_error
         from .gemv import ShapeError
         if prompt.shape[1] + new_tokens + 2 * self.nodes > self.max_seq:
             raise ShapeError(f"generate: {prompt.shape[1]} + {new_tokens} tokens and two steps' nodes in a cache of "
@@ -594,8 +599,10 @@ class SpeculativeDecoder(Decoder):
         start = [len(h) for h in history]
         while min(len(h) - n for h, n in zip(history, start)) < new_tokens:
             tok, par = self.tree.cpu(), torch.full((self.sessions, self.nodes), -2, dtype=torch.int32)
-            par[:, 0] = -1
             for s, h in enumerate(history):
+                if len(h) - start[s] >= new_tokens:
+                    continue
+                par[s, 0] = -1
                 drafts, up = drafter(h, self.nodes)
                 k = min(len(drafts), self.nodes - 1)
                 tok[s, 1:1 + k] = torch.tensor(drafts[:k], dtype=torch.int32)
@@ -607,6 +614,9 @@ class SpeculativeDecoder(Decoder):
             self.step(sh)
             for h, e in zip(history, self.emitted.cpu().tolist()):
                 h.extend(t for t in e if t >= 0)
+        error = device_error(reset=False)
+        if error:
+            raise RuntimeError(f"generate: device error {error}")
         return [h[n:] for h, n in zip(history, start)]
 
 

@@ -250,3 +250,43 @@ def test_a_session_without_a_tree_keeps_its_place(torch, model):
         runs.append((got, dec.positions[1].item()))
     assert runs[0] == runs[1] and min(runs[0][0]) >= 0
     _no_error()
+
+
+@pytest.mark.parametrize("fast", [0, 1])
+def test_generation_of_sessions_that_advance_unevenly(torch, model, fast):
+    """One session's drafts are all taken and the other's none, in the smallest
+    cache that is accepted: every returned token is greedy decoding's."""
+    from firepit_b200.model import SpeculativeDecoder
+    new, nodes = 40, 8
+    prompt = torch.tensor([[4, 8, 15, 16, 23, 42, 4, 8], [1, 2, 3, 1, 2, 3, 1, 2]], dtype=torch.int32, device="cuda")
+    want = SpeculativeDecoder(model, 2, nodes, 128).generate(prompt, new + nodes, lambda h, n: ([], []))
+    dec = SpeculativeDecoder(model, 2, nodes, prompt.shape[1] + new + 2 * nodes)
+    start, line = prompt[fast].tolist(), prompt[fast].tolist() + want[fast]
+    asked = [0, 0]
+
+    def drafter(history, n):
+        mine = history[:len(start)] == start
+        asked[0 if mine else 1] += 1
+        drafts = line[len(history):len(history) + n - 1] if mine else [(history[-1] + 1) % 512] * (n - 1)
+        return drafts, list(range(len(drafts)))
+
+    got = dec.generate(prompt, new, drafter)
+    assert len(got[fast]) >= new and len(got[1 - fast]) >= new
+    for g, w in zip(got, want):
+        assert len(g) <= len(w) and g == w[:len(g)]
+    assert asked[0] <= new // nodes + 2 and asked[1] > new // 2  # a session that has its tokens is not drafted for
+    assert max(dec.positions.tolist()) <= prompt.shape[1] + new + nodes
+    _no_error()
+
+
+def test_generation_reports_a_device_error(torch, model):
+    """What a kernel records while tokens are made is raised, not left behind."""
+    import firepit_b200 as F
+    from firepit_b200.model import SpeculativeDecoder
+    prompt = torch.tensor([[1, 2, 3]], dtype=torch.int32, device="cuda")
+    dec = SpeculativeDecoder(model, 1, 4, 64)
+    with pytest.raises(RuntimeError, match="50[145]"):
+        dec.generate(prompt, 4, lambda h, n: ([5], [3]))  # node 1's parent is a later node
+    assert F.device_error(reset=True) == 504
+    assert len(dec.generate(prompt, 4, lambda h, n: ([], []))[0]) >= 4
+    _no_error()
