@@ -551,13 +551,17 @@ class SpeculativeDecoder(Decoder):
         for kv in self.kv.values():
             N.call("fpb_kv8_keep", kv.k.data_ptr(), kv.v.data_ptr(), kv.k_exp.data_ptr(), kv.v_exp.data_ptr(), S,
                    self.max_seq, c.kv_heads, c.head_dim, self.positions.data_ptr(), self.path.data_ptr(), n, sh)
-        # the accepted drafts, then the token after them
-        taken = torch.gather(self.tree, 1, self.path.clamp(min=0).long()).roll(-1, 1)
-        left = self.count[:, None] - 1 - self.at
-        self.emitted.copy_(torch.where(left > 0, taken, torch.where(left == 0, self.next[:, None], -1)))
-        self.positions.add_(self.count)
-        # (a session without a tree has no next token: it keeps its own, which the next step may embed)
-        self.tree[:, 0].copy_(torch.where(self.count > 0, self.next, self.tree[:, 0]))
+        # the steps on the results, behind the kernels on their stream
+        now = torch.cuda.current_stream(self.model.device)
+        with torch.cuda.stream(now if now.cuda_stream == sh else
+                               torch.cuda.ExternalStream(sh, device=self.model.device)):
+            # the accepted drafts, then the token after them
+            taken = torch.gather(self.tree, 1, self.path.clamp(min=0).long()).roll(-1, 1)
+            left = self.count[:, None] - 1 - self.at
+            self.emitted.copy_(torch.where(left > 0, taken, torch.where(left == 0, self.next[:, None], -1)))
+            self.positions.add_(self.count)
+            # (a session without a tree has no next token: it keeps its own, which the next step may embed)
+            self.tree[:, 0].copy_(torch.where(self.count > 0, self.next, self.tree[:, 0]))
 
     def feed(self, tokens) -> None:
         """Runs known tokens [sessions, n] (device int32) through the model,

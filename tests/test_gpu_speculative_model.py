@@ -290,3 +290,32 @@ def test_generation_reports_a_device_error(torch, model):
     assert F.device_error(reset=True) == 504
     assert len(dec.generate(prompt, 4, lambda h, n: ([], []))[0]) >= 4
     _no_error()
+
+
+def test_a_step_keeps_to_its_stream(torch, model):
+    """Steps on a side stream that still has work ahead of them, issued while
+    torch's current stream is another: the results are those of the current
+    stream's, once the side stream alone is done."""
+    from firepit_b200.model import SpeculativeDecoder
+    tree = torch.tensor([[7, 8, 9, 10], [11, 12, 13, 14]], dtype=torch.int32, device="cuda")
+    par = torch.tensor([[-1, 0, 0, 1]] * 2, dtype=torch.int32, device="cuda")
+    runs = []
+    for side in (None, torch.cuda.Stream()):
+        dec = SpeculativeDecoder(model, 2, 4, 64)
+        dec.feed(torch.tensor([[3, 14, 15], [92, 65, 35]], dtype=torch.int32, device="cuda"))
+        got, stream = [], side or torch.cuda.current_stream()
+        for _ in range(3):
+            dec.tree[:, 1:].copy_(tree[:, 1:])
+            dec.parents.copy_(par)
+            torch.cuda.synchronize()
+            if side:
+                with torch.cuda.stream(side):  # some milliseconds of work ahead of the step
+                    big = torch.zeros(1 << 28, device="cuda")
+                    for _ in range(20):
+                        big.add_(1.0)
+            dec.step(stream.cuda_stream)
+            stream.synchronize()
+            got.append((dec.emitted.tolist(), dec.positions.tolist(), dec.tree[:, 0].tolist()))
+        runs.append(got)
+    assert runs[0] == runs[1]
+    _no_error()
