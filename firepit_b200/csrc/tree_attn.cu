@@ -291,11 +291,12 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
     }
     const int t0 = step * 16;
     const bool open = t0 + 16 > pos;  // warp-uniform: the tree's rows, or the end
-    float kf[2], ve[2];
+    float kf[2], ve[2], vf[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       kf[h] = kv8_factor(xr[h]);
       ve[h] = kv8_value_exponent(xr[2 + h]);
+      vf[h] = pow2i((int)ve[h] - kSpread);
     }
     if (at_step + 1 < count) load_exps(step + kRowsWarps, xr);
     uint32_t vr[4][kVPieces][kVBytes / 4];
@@ -331,8 +332,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
         if ((g & 1) == (t & 1) && lanes) nan[t >> 1] = true;
       }
     }
-    // y = score + the value's exponent
-    float y[kNT][2][2];  // row, token
+    float y[kNT][2][2];  // scores: row, token
     bool grow = false;
 #pragma unroll
     for (int i = 0; i < kNT; ++i)
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float v = fmaf(s[i][0][2 * h + e], kf[h] * fac[i][e], ve[h]);
+          float v = s[i][0][2 * h + e] * (kf[h] * fac[i][e]);
           if (open) {
             const int t = t0 + own + 8 * h;
             if (nan[h]) v = __int_as_float(0x7fc00000);
@@ -348,18 +348,18 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
           }
           y[i][e][h] = v;
         }
-        grow |= fmaxf(y[i][e][0], y[i][e][1]) > m[i][e] + kLag;
+        grow |= fmaxf(y[i][e][0] + ve[0], y[i][e][1] + ve[1]) > m[i][e] + kLag;
       }
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
       for (int i = 0; i < kNT; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float mn = fmaxf(m[i][e], fmaxf(y[i][e][0], y[i][e][1]));
+          float mn = fmaxf(m[i][e], fmaxf(y[i][e][0] + ve[0], y[i][e][1] + ve[1]));
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-          const float old = m[i][e] == -INFINITY ? 0.0f : exp2_approx(m[i][e] - mn);
-          l[i][e] *= old;
+          const float by = m[i][e] == -INFINITY ? -INFINITY : m[i][e] - mn, old = exp2_approx(by);
+          l[i][e] = sum_to(l[i][e], by);
           m[i][e] = mn;
 #pragma unroll
           for (int k = 0; k < kMT; ++k) {
@@ -369,17 +369,17 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
         }
     }
     uint32_t pb[kNT][2];
-    const float vi[2] = {pow2i(-(int)ve[0]), pow2i(-(int)ve[1])};
 #pragma unroll
     for (int i = 0; i < kNT; ++i) {
       float p[2][2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float base = m[i][e] == -INFINITY ? 0.0f : kHead - m[i][e];
+        const float base = m[i][e] == -INFINITY ? 0.0f : kHead + kSpread - m[i][e];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          p[e][h] = exp2_approx(y[i][e][h] + base);
-          l[i][e] = fmaf(p[e][h], vi[h], l[i][e]);
+          const float x = exp2_approx(y[i][e][h] + base);
+          l[i][e] = fmaf(x, kSumScale, l[i][e]);
+          p[e][h] = x * vf[h];
         }
       }
 #pragma unroll
@@ -448,8 +448,9 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
     for (int x = 0; x < kRowsWarps; ++x) mt = fmaxf(mt, m_s[x][r]);
 #pragma unroll
     for (int x = 0; x < kRowsWarps; ++x) {
-      f[x] = m_s[x][r] == -INFINITY ? 0.0f : exp2_approx(m_s[x][r] - mt);
-      lt += l_s[x][r] * f[x];
+      const float by = m_s[x][r] == -INFINITY ? -INFINITY : m_s[x][r] - mt;
+      f[x] = exp2_approx(by);
+      lt += sum_to(l_s[x][r], by);
     }
     const int n = row / a.group, h = kvh * a.group + row % a.group;
     const bool there = sight_s[r].upto >= 0;
@@ -465,7 +466,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
         *reinterpret_cast<float2 *>(a.part + (((size_t)item * a.splits + blockIdx.x) * NR + r) * D + d) = o;
       } else {
         const size_t node = (size_t)b * a.nodes + n;
-        const float inv = there ? 1.0f / lt : 0.0f;
+        const float inv = there ? kSumBack / lt : 0.0f;
         o.x = there ? o.x * inv : 0.0f;
         o.y = there ? o.y * inv : 0.0f;
         if (a.gate && there) {
@@ -523,9 +524,9 @@ __global__ void __launch_bounds__(kMergeWarps * 32, 2) tree_attn_merge_kernel(co
   for (int s = share; s < splits; s += shares) {
     const float2 v = ml[(size_t)s * NR];
     const float4 x = *reinterpret_cast<const float4 *>(part + (size_t)s * NR * D);
-    const float f = v.x == -INFINITY ? 0.0f : exp2_approx(v.x - m);
-    l = fmaf(v.y, f, l);
-    add(x, f);
+    const float by = v.x == -INFINITY ? -INFINITY : v.x - m;
+    l += sum_to(v.y, by);
+    add(x, exp2_approx(by));
   }
   if (shares > 1) {
     if (share > 0) {
@@ -540,7 +541,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32, 2) tree_attn_merge_kernel(co
     }
   }
   if (!in || d >= D) return;
-  const float inv = there ? 1.0f / l : 0.0f;
+  const float inv = there ? kSumBack / l : 0.0f;
   const float x[4] = {acc.x, acc.y, acc.z, acc.w};
   float o[4];
 #pragma unroll

@@ -144,9 +144,26 @@ __device__ __forceinline__ float exp2_approx(float x) {
 
 // Weights are held as 2^(y - m + kHead), y the score (in powers of two) plus
 // the value vector's own exponent: f16 then holds a weight down to 2^-32 of
-// the row's largest, and the exponent costs no multiplication.  The maximum
-// may lag by kLag before the sums are rescaled (weights up to 2^(kHead + kLag)).
+// the row's largest.  The maximum may lag by kLag before the sums are rescaled
+// (weights up to 2^(kHead + kLag)).
 constexpr float kHead = 7.0f, kLag = 8.0f, kMost = 32768.0f, kLowest = -1e30f;
+// Their sum takes them without the values' exponents v, which lie within [-100,
+// 120]: a value's size is no part of its weight.  Since m >= y + v - kLag for
+// every score y, 2^(y - m + kHead) could reach 2^115, and the largest be 2^-113;
+// times 2^kSpread that becomes 2^126 and 2^-102, so that no weight overflows and
+// none is lost that is above 2^-24 of the largest.  The value's factor takes
+// 2^kSpread back, and the sum is held times kSumScale (2^20 weights fit), what
+// 1 / sum has to be multiplied by kSumBack for.
+constexpr int kSpread = 11;
+constexpr float kSumScale = 0x1p-20f, kSumBack = 0x1p-9f;
+static_assert(kSumScale / kSumBack == 1.0f / (1 << kSpread));
+// A sum of weights taken from one maximum to another that is `by` (<= 0) higher.
+// Two maxima may lie 220 and more apart, where the factor is no f32 but the
+// sum's two ends are: it goes by halves.
+__device__ __forceinline__ float sum_to(float l, float by) {
+  const float half = exp2_approx(0.5f * by);
+  return l * half * half;
+}
 
 // The tcgen05 kernel (tree_attn_tile.cu): token tiles of BT rows, `blocks` of
 // them, their partial results and the items' shares of them in the workspace.

@@ -143,11 +143,6 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 
 // Barriers of the roles: a quad's softmax warps (ids 1-4), the converting
 // warps (5), all of the softmax (6).  TMEM accesses are ordered across them.
@@ -175,13 +170,13 @@ __device__ __forceinline__ void soft_sync() {
 }
 
 // A part of a row of S (NT tokens from TMEM column s_tmem, factors fac: two
-// keys', two values' of each pair): weights e = 2^(s * kf * f + base), their
-// sums in l, e * vf as f16 pairs in p; returns the largest e * vf.  OPEN: a
+// keys', two values' of each pair): weights e = 2^(s * kf * f + base), kSumScale
+// of their sums in l, e * vf as f16 pairs in p; returns the largest e * vf.  OPEN: a
 // tile that not every row sees whole, only its tokens `seen`.
 template <int NT, bool OPEN>
 __device__ __forceinline__ float weigh_pass(uint32_t s_tmem, const float4 *fac, float f, float base, uint64_t seen,
                                             uint32_t (&p)[NT / 2], uint64_t &l) {
-  const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
+  const uint64_t f2 = pack2(f, f), b2 = pack2(base, base), k2 = pack2(kSumScale, kSumScale);
   float mx[2] = {0.0f, 0.0f};
 #pragma unroll
   for (int c = 0; c < NT / 16; ++c) {
@@ -201,7 +196,7 @@ __device__ __forceinline__ float weigh_pass(uint32_t s_tmem, const float4 *fac, 
         if (!(seen >> (c * 16 + e + 1) & 1)) e1 = 0.0f;
       }
       const uint64_t e2 = pack2(e0, e1);
-      l = add2(l, e2);
+      l = fma2(e2, k2, l);
       unpack2(mul2(e2, pack2(ft.z, ft.w)), w0, w1);
       mx[(e >> 1) & 1] = fmaxf(mx[(e >> 1) & 1], fmaxf(w0, w1));
       p[(c * 16 + e) / 2] = pack_f16x2(w0, w1);
@@ -228,8 +223,8 @@ __device__ __noinline__ float weigh_open(uint32_t s_tmem, const float4 *fac, flo
 }
 
 // The row's maximum raised by this tile's scores (y = s * kf * f + log2(vf)),
-// and O of the tiles before rescaled to it; returns the new maximum and the
-// factor of what was summed before.
+// and O of the tiles before rescaled to it; returns the new maximum and what
+// it is above the old one, negated.
 template <int DP, int NT>
 __device__ __noinline__ float2 raise_max(TileShared *sh, uint32_t s_tmem, uint32_t o_tmem, const float4 *fac, float f,
                                          uint64_t seen, float m, int D, bool sums) {
@@ -243,7 +238,7 @@ __device__ __noinline__ float2 raise_max(TileShared *sh, uint32_t s_tmem, uint32
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const float4 ft = fac[(c * 16 + e) / 2];
-      const float v = (float)((int)(__float_as_uint(e & 1 ? ft.w : ft.z) >> 23) - 127);
+      const float v = (float)((int)(__float_as_uint(e & 1 ? ft.w : ft.z) >> 23) - 127 + kSpread);
       const float y = fmaf(__uint_as_float(r[e]) * (e & 1 ? ft.y : ft.x), f, v);
       if (seen >> (c * 16 + e) & 1) mx = fmaxf(mx, y);
     }
@@ -267,7 +262,7 @@ __device__ __noinline__ float2 raise_max(TileShared *sh, uint32_t s_tmem, uint32
     tmem_st_wait();
   }
   quad_sync(quad);  // red is read
-  return make_float2(mn, old);
+  return make_float2(mn, m - mn);
 }
 
 // O of a row tile's share to its slot: four columns of 128 rows lie together, so
@@ -295,7 +290,7 @@ __device__ __noinline__ void write_rows(const TreeArgs &a, TileShared *sh, uint3
   float l = 0.0f;
 #pragma unroll
   for (int i = 0; i < kParts; ++i) l += sh->red[i][r_own];
-  const float inv = 1.0f / l;
+  const float inv = kSumBack / l;
   __nv_bfloat16 *o = a.out + (node * a.q_heads + h) * D;
   const float *gate = a.gate ? a.gate + node * a.gate_pitch + (size_t)h * a.gate_head : nullptr;
 #pragma unroll 1
@@ -550,19 +545,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
             const float2 r = raise_max<DP, NT>(sh, s_tmem, my + Sh::kTmemO, fac, f, seen, m, a.head_dim, j > j0);
             m = r.x;
-            l2 = mul2(l2, pack2(r.y, r.y));
+            const float half = exp2_approx(0.5f * r.y);  // (as sum_to)
+            l2 = mul2(mul2(l2, pack2(half, half)), pack2(half, half));
           }
           l_new = l2;
           float mx;
           if (open) {
             uint32_t q[NT / 2];
             uint64_t l = l2;
-            mx = weigh_open<NT>(s_tmem, fac, f, kHead - m, seen, q, &l);
+            mx = weigh_open<NT>(s_tmem, fac, f, kHead + kSpread - m, seen, q, &l);
 #pragma unroll
             for (int i = 0; i < NT / 2; ++i) p[i] = q[i];
             l_new = l;
           } else {
-            mx = weigh_pass<NT, false>(s_tmem, fac, f, kHead - m, seen, p, l_new);
+            mx = weigh_pass<NT, false>(s_tmem, fac, f, kHead + kSpread - m, seen, p, l_new);
           }
           const bool more = quad_any(quad, mx > kMost);
           if (raise || !more) break;
@@ -782,7 +778,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int i = 0; i < X; ++i) {
           const int t = lane + 32 * i;
           ft[(t >> 1) * 4 + (t & 1)] = kv8_factor(xk[i]);
-          ft[(t >> 1) * 4 + 2 + (t & 1)] = pow2i((int)kv8_value_exponent(xv[i]));
+          ft[(t >> 1) * 4 + 2 + (t & 1)] = pow2i((int)kv8_value_exponent(xv[i]) - kSpread);
         }
       }
       if (open) {  // values that are not a number: zero in the product, and the token's score NaN for those who see it
@@ -877,7 +873,7 @@ __global__ void __launch_bounds__(kMergeThreads, 1) tree_attn_tile_merge_kernel(
   auto add = [&](float2 v, float4 x, float4 y) {
     const float mn = fmaxf(m, v.x), fo = exp2_approx(m - mn), fn = exp2_approx(v.x - mn);
     const float z[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-    l = l * fo + v.y * fn;
+    l = sum_to(l, m - mn) + sum_to(v.y, v.x - mn);
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = acc[i] * fo + z[i] * fn;
     m = mn;
@@ -910,7 +906,7 @@ __global__ void __launch_bounds__(kMergeThreads, 1) tree_attn_tile_merge_kernel(
   }
   if (!live) return;
   const bool there = some && (a.parents ? a.sights[(size_t)b * kTreeMaxNodes + n] != 0 : pos >= 0 && pos < a.max_seq - n);
-  const float inv = 1.0f / l;
+  const float inv = kSumBack / l;
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = there ? acc[i] * inv / gate[i] : 0.0f;
   *reinterpret_cast<uint4 *>(a.out + (node * a.q_heads + h) * D + d) =

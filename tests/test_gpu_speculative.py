@@ -546,3 +546,33 @@ def test_chains_whose_blocks_hold_segments_without_tiles(F, torch, b, n, hq, hk,
     rng = np.random.default_rng(n)
     cache = _cache(F, torch, rng, b, s, hk, d)
     _check_attention(F, torch, rng, cache, pos, None, n, hq, gate=False)
+
+
+# ---- the softmax's sum apart from the values' exponents ---------------------------------------------------------
+@pytest.mark.parametrize("hq", [2, 24])  # both kernels
+@pytest.mark.parametrize("e0,e1", [(66, -83), (-83, 66), (125, -98), (-98, 125), (-98, -98), (125, 125)])
+def test_a_weight_counts_whatever_its_value_s_size(F, torch, hq, e0, e1):
+    """Equal scores: the output is the mean of the values, though one of them is
+    2^149 or 2^223 times the other."""
+    rng = np.random.default_rng(21)
+    d = 64
+    v = rng.standard_normal((1, 4, 1, d))
+    v *= (2.0 ** np.array([e0, e1, e1, e0]))[None, :, None, None]
+    (kc, ke), (vc, ve) = R.quantise(np.zeros((1, 4, 1, d))), R.quantise(v)
+    cache = F.Kv8Cache(*(_dev(torch, x) for x in (kc, vc, ke, ve)))
+    _check_attention(F, torch, rng, cache, [1], np.array([[-1, 0, 1]], np.int32), 3, hq, gate=False)
+
+
+@pytest.mark.parametrize("n,hq", [(3, 2), (3, 24)])
+def test_attention_over_the_whole_range_of_exponents(F, torch, n, hq):
+    """Value vectors 2^-105 to 2^124 in size over several tiles, in descending,
+    ascending and random order."""
+    rng = np.random.default_rng(22)
+    s, d = 700, 64
+    size = rng.integers(-105, 125, s)
+    for order in (np.sort(size), np.sort(size)[::-1], size):
+        k = rng.standard_normal((1, s, 1, d)) * 0.5
+        v = rng.standard_normal((1, s, 1, d)) * (2.0 ** order)[None, :, None, None]
+        (kc, ke), (vc, ve) = R.quantise(k), R.quantise(v)
+        cache = F.Kv8Cache(*(_dev(torch, x) for x in (kc, vc, ke, ve)))
+        _check_attention(F, torch, rng, cache, [s - n], _tree(rng, 1, n), n, hq, gate=False)
