@@ -576,3 +576,19 @@ def test_attention_over_the_whole_range_of_exponents(F, torch, n, hq):
         (kc, ke), (vc, ve) = R.quantise(k), R.quantise(v)
         cache = F.Kv8Cache(*(_dev(torch, x) for x in (kc, vc, ke, ve)))
         _check_attention(F, torch, rng, cache, [s - n], _tree(rng, 1, n), n, hq, gate=False)
+
+
+@pytest.mark.parametrize("hq", [2, 24])  # both kernels
+@pytest.mark.parametrize("size", [120, -100])
+def test_keys_of_any_size_against_queries_of_the_other(F, torch, hq, size):
+    """Keys of about 2^120 and queries of about 2^-100, and the other way round:
+    the scores are ordinary numbers, what they are made of is not."""
+    rng = np.random.default_rng(28)
+    s, d, n = 200, 64, 3
+    k = rng.standard_normal((1, s, 1, d)) * 2.0 ** size
+    v = rng.standard_normal((1, s, 1, d))
+    (kc, ke), (vc, ve) = R.quantise(k), R.quantise(v)
+    cache = F.Kv8Cache(*(_dev(torch, x) for x in (kc, vc, ke, ve)))
+    other = -100 if size == 120 else 110
+    _check_attention(F, torch, rng, cache, [s - n], _tree(rng, 1, n), n, hq, amp=2.0 ** other,
+                     scale=2.0 ** -(size + other) / 8)
