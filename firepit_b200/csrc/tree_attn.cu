@@ -352,6 +352,20 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
       }
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        uint32_t any = 0;
+#pragma unroll
+        for (int p = 0; p < kVPieces; ++p)
+#pragma unroll
+          for (int j = 0; j < kVBytes / 4; ++j) any |= vr[t][p][j];
+        // operand row 2 c + t % 2 (+ 8) lies over the lanes of this c
+        const uint32_t lanes = __ballot_sync(0xffffffffu, (any & 0x7f7f7f7fu) != 0) & (0x11111111u << (g >> 1));
+        if ((g & 1) == (t & 1) && !lanes) {
+          ve[t >> 1] = kZeroExp;
+          vf[t >> 1] = 0.0f;
+        }
+      }
+#pragma unroll
       for (int i = 0; i < kNT; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {

@@ -157,6 +157,11 @@ constexpr float kHead = 7.0f, kLag = 8.0f, kMost = 32768.0f, kLowest = -1e30f;
 constexpr int kSpread = 11;
 constexpr float kSumScale = 0x1p-20f, kSumBack = 0x1p-9f;
 static_assert(kSumScale / kSumBack == 1.0f / (1 << kSpread));
+// A zero value vector adds to the sum only: it takes part in the maximum as
+// one of the smallest exponent, so that a large weight of its own (a row that
+// the model rests attention on) does not push what the others give out of f16.
+// Found where a maximum is about to be raised, from the codes.
+constexpr float kZeroExp = kKv8MinExp;
 // A sum of weights taken from one maximum to another that is `by` (<= 0) higher.
 // Two maxima may lie 220 and more apart, where the factor is no f32 but the
 // sum's two ends are: it goes by halves.

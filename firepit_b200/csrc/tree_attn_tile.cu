@@ -228,13 +228,29 @@ __device__ __noinline__ float weigh_open(uint32_t s_tmem, const float4 *fac, flo
   return mx;
 }
 
-// The row's maximum raised by this tile's scores (y = s * kf * f + log2(vf)),
-// and O of the tiles before rescaled to it; returns the new maximum and what
-// it is above the old one, negated.
+// The row's maximum raised by the scores of this tile's NT tokens from t0 on (y
+// = s * kf * f + the value's exponent) where they are above it by more than the
+// lag, and O of the tiles before rescaled to it; returns the new maximum and what
+// it is above the old one, negated.  Zero values' factors become those of
+// kZeroExp, for every quad of rows: whether another one takes this tile's weights
+// before or after that, its maximum is raised by the same values (hence by the
+// lag and a half: whatever is above that has a weight above kMost).
 template <int DP, int NT>
-__device__ __noinline__ float2 raise_max(TileShared *sh, uint32_t s_tmem, uint32_t o_tmem, const float4 *fac, float f,
-                                         uint64_t seen, float m, int D, bool sums) {
-  const int quad = (threadIdx.x >> 5) & 3, part = threadIdx.x >> 7, r_own = threadIdx.x & 127;
+__device__ __noinline__ float2 raise_max(const TreeArgs &a, TileShared *sh, uint32_t s_tmem, uint32_t o_tmem,
+                                         const float4 *fac, float f, uint64_t seen, float m, int t0, bool sums) {
+  const int quad = (threadIdx.x >> 5) & 3, part = threadIdx.x >> 7, r_own = threadIdx.x & 127, lane = threadIdx.x & 31;
+  const int D = a.head_dim;
+  if (lane < NT && t0 + lane < sh->seg.total) {  // a lane a token, whose first codes mostly tell
+    const uint4 *v = reinterpret_cast<const uint4 *>(
+        a.v_codes + (((size_t)sh->seg.b * a.max_seq + t0 + lane) * a.kv_heads + sh->seg.kvh) * D);
+    bool zero = true;
+    for (int i = 0; zero && i < D / 16; ++i) {
+      const uint4 x = __ldg(v + i);
+      zero = ((x.x | x.y | x.z | x.w) & 0x7f7f7f7fu) == 0;
+    }
+    if (zero) const_cast<float *>(&fac[lane >> 1].z)[lane & 1] = pow2i((int)kZeroExp - kSpread);
+  }
+  __syncwarp();
   float mx = -INFINITY;
 #pragma unroll 1
   for (int c = 0; c < NT / 16; ++c) {
@@ -254,6 +270,7 @@ __device__ __noinline__ float2 raise_max(TileShared *sh, uint32_t s_tmem, uint32
   float mn = m;  // (a row that has seen nothing yet keeps its floor)
 #pragma unroll
   for (int i = 0; i < kParts; ++i) mn = fmaxf(mn, sh->red[i][r_own]);
+  if (mn <= m + (kLag + 0.5f)) mn = m;
   const float old = exp2_approx(m - mn);
   if (sums) {
 #pragma unroll 1
@@ -550,7 +567,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               __syncwarp();
               tc_fence_after();
             }
-            const float2 r = raise_max<DP, NT>(sh, s_tmem, my + Sh::kTmemO, fac, f, seen, m, a.head_dim, j > j0);
+            const float2 r = raise_max<DP, NT>(a, sh, s_tmem, my + Sh::kTmemO, fac, f, seen, m, j * BT + part * NT, j > j0);
             m = r.x;
             const float half = exp2_approx(0.5f * r.y);  // (as sum_to)
             l2 = mul2(mul2(l2, pack2(half, half)), pack2(half, half));

@@ -592,3 +592,35 @@ def test_keys_of_any_size_against_queries_of_the_other(F, torch, hq, size):
     other = -100 if size == 120 else 110
     _check_attention(F, torch, rng, cache, [s - n], _tree(rng, 1, n), n, hq, amp=2.0 ** other,
                      scale=2.0 ** -(size + other) / 8)
+
+
+# ---- zero value vectors ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("hq", [1, 4, 24])  # eight and sixteen rows a tile, the tcgen05 kernel
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("size", [1.0, 1e-7, 1e-20])
+@pytest.mark.parametrize("zeros", [(0,), (3, 150, 151, 399), (401, 402), (70, 401), tuple(range(400))])
+def test_zero_values_with_the_largest_scores(F, torch, hq, d, size, zeros):
+    """Rows whose value is zero take nearly all of the weight: what the others
+    give keeps its bits.  Scores: queries of ones and keys of a constant, so that
+    a zero row's is 24 and another's within [0, 1].  Bars as above, the weights'
+    relative to the sum that the exact weights have."""
+    rng = np.random.default_rng(23)
+    s, pos, n = 404, 400, 4
+    a = rng.random(s)
+    a[list(zeros)] = 24.0
+    k = np.repeat(a[:, None], d, 1) / math.sqrt(d)
+    v = rng.standard_normal((s, d)) * size
+    v[list(zeros)] = rng.choice([0.0, -0.0], (len(zeros), d))
+    (kc, ke), (vc, ve) = R.quantise(k), R.quantise(v)
+    cache = F.Kv8Cache(*(_dev(torch, x[None, :, None]) for x in (kc, vc, ke, ve)))
+    q = torch.ones(1, n, hq, d, device="cuda")
+    par = np.array([[-1, 0, 1, 1]], np.int32)
+    outs = [F.tree_attention(q, cache, _dev(torch, np.array([pos], np.int32)), _dev(torch, par)) for _ in range(3)]
+    assert all(torch.equal(o, outs[0]) for o in outs)
+    got = _host(outs[0])
+    k, v = R.values(kc, ke), R.values(vc, ve)
+    for j, line in enumerate(R.ancestors(par[0])):
+        rows = list(range(pos)) + [pos + i for i in line]
+        o, pv, sabs = R.attend(np.ones(d), k[rows], v[rows], 1 / math.sqrt(d))
+        bound = (2 * 2.0 ** -11 * sabs + 2.0 ** -11 + 2.0 ** -16) * pv
+        assert (np.abs(got[0, j] - o) <= bound + 2.0 ** -8 * np.abs(o)).all(), (j, got[0, j, 0, :4], o[:4])
