@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
       m[i][e] = -INFINITY;
       l[i][e] = 0.0f;
     }
-  bool ok = true;
+  bool ok = true, nan = false;  // nan: a NaN among the lane's values of open steps
   for (int at_step = 0; at_step < count; ++at_step) {
     const int step = first + at_step * kRowsWarps;
     const uint8_t *kst = mine_ring + (at_step % kStages) * Sh::kStage, *vst = kst + Sh::kStage / 2;
@@ -314,11 +314,10 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
         }
       }
     }
-    bool nan[2] = {false, false};  // of the lane's tokens
     if (open) {  // a value vector that some row does not see must not reach it through 0 * NaN
+      uint32_t any = 0;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        uint32_t any = 0;
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int p = 0; p < kVPieces; ++p)
 #pragma unroll
@@ -327,10 +326,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
             vr[t][p][j] &= ~bad;
             any |= bad;
           }
-        // operand row 2 c + t % 2 (+ 8) lies over the lanes of this c
-        const uint32_t lanes = __ballot_sync(0xffffffffu, any != 0) & (0x11111111u << (g >> 1));
-        if ((g & 1) == (t & 1) && lanes) nan[t >> 1] = true;
-      }
+      nan |= any != 0;
     }
     float y[kNT][2][2];  // scores: row, token
     bool grow = false;
@@ -343,7 +339,6 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
           float v = s[i][0][2 * h + e] * (kf[h] * fac[i][e]);
           if (open) {
             const int t = t0 + own + 8 * h;
-            if (nan[h]) v = __int_as_float(0x7fc00000);
             if (t >= total || !sight_s[8 * i + 2 * c + e].sees(t, pos, tree)) v = -INFINITY;
           }
           y[i][e][h] = v;
@@ -424,6 +419,31 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<DP, NR>::kBlocks))
     for (int i = 0; i < kStages; ++i) {
       int never = 0;
       for (uint32_t k = 0; k < 2; ++k) mbar_wait(&full[w][i], k, &never);
+    }
+
+  // Those who see a value with NaN codes have NaN in its columns (the lane's:
+  // whichever lane has met one, all look).
+  if (__any_sync(0xffffffffu, nan))
+    for (int t = max(s0 * 16, pos / 16 * 16); t < min(s1 * 16, total); ++t) {
+      if ((t / 16 - first) % kRowsWarps) continue;  // another warp's step
+      const uint8_t *v = a.v_codes + (((size_t)b * a.max_seq + t) * a.kv_heads + kvh) * D;
+#pragma unroll
+      for (int p = 0; p < kVPieces; ++p)
+#pragma unroll
+        for (int j = 0; j < kVBytes / 4; ++j) {
+          const int d = 128 * p + kVBytes * piece_at<DP>(g) + 4 * j, mt = (p * kVBytes / 4 + j) * 2;
+          const uint32_t w = d < D ? __ldg(reinterpret_cast<const uint32_t *>(v + d)) : 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if ((w >> (8 * k) & 0x7f) == 0x7f) {
+#pragma unroll
+              for (int i = 0; i < kNT; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if (sight_s[8 * i + 2 * c + e].sees(t, pos, tree))
+                    acc[mt + (k >> 1)][i][2 * (k & 1) + e] = __int_as_float(0x7fc00000);
+            }
+        }
     }
 
   // the warps' results meet: maxima, then sums over one maximum in warp order

@@ -84,7 +84,7 @@ struct TileShared {
   Walk walk, soft_walk;
   Segment seg;
   uint32_t tmem;
-  int abort, never, more;
+  int abort, never, more, nan;  // nan: there has been a NaN among the values of an open tile
   float red[kParts][kTileRows];  // maxima, then sums, of the rows' parts
   uint64_t sight[kTileRows];     // a tree: the bits; a chain: the limit
   float4 fac[4][64];             // [META][pair of tokens]: two keys' factors, two values'
@@ -288,15 +288,40 @@ __device__ __noinline__ float2 raise_max(const TreeArgs &a, TileShared *sh, uint
   return make_float2(mn, m - mn);
 }
 
+// Columns [d, d + 16) of the row r_own's result: NaN where a value that it sees
+// in the segment's open tiles holds one.  (Past a NaN the block does this for each
+// of its segments.)
+__device__ __noinline__ void put_nan(const TreeArgs &a, const TileShared *sh, int BT, int r_own, int d, uint32_t *r) {
+  const Segment &s = sh->seg;
+  const uint64_t sight = sh->sight[r_own];
+  for (int t = max(s.j0, s.pos / BT) * BT; t < min(s.j1 * BT, s.total); ++t) {
+    if (!Sight{(int)sight, sight}.sees(t, s.pos, a.parents != nullptr)) continue;
+    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(
+        a.v_codes + (((size_t)s.b * a.max_seq + t) * a.kv_heads + s.kvh) * a.head_dim + d));
+    const uint32_t w[4] = {not_numbers(v.x), not_numbers(v.y), not_numbers(v.z), not_numbers(v.w)};
+    for (int i = 0; i < 16; ++i)
+      if (w[i >> 2] >> (8 * (i & 3)) & 1) r[i] = 0x7fc00000u;
+  }
+}
+
 // O of a row tile's share to its slot: four columns of 128 rows lie together, so
 // that a warp stores 512 bytes.
-__device__ __noinline__ void write_part(const TreeArgs &a, size_t slot, uint32_t o_tmem) {
+__device__ __noinline__ void write_part(const TreeArgs &a, const TileShared *sh, int BT, size_t slot, uint32_t o_tmem) {
   const int part = threadIdx.x >> 7, r_own = threadIdx.x & 127, D = a.head_dim;
   float4 *o = reinterpret_cast<float4 *>(a.part) + slot * (kTileRows * (size_t)D / 4) + r_own;
   for (int d = 16 * part; d < D; d += 16 * kParts) {
     uint32_t r[16];
     tmem_ld16(o_tmem + d, r);
     tmem_ld_wait(r);
+    if (sh->nan) {
+      uint32_t x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = r[i];
+      put_nan(a, sh, BT, r_own, d, x);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) r[i] = x[i];
+    }
+    __syncwarp();
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       o[(size_t)(d / 4 + i) * kTileRows] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]),
@@ -305,7 +330,7 @@ __device__ __noinline__ void write_part(const TreeArgs &a, size_t slot, uint32_t
 }
 
 // The same to `out`, divided by the row's sum, with the gate.
-__device__ __noinline__ void write_rows(const TreeArgs &a, TileShared *sh, uint32_t o_tmem) {
+__device__ __noinline__ void write_rows(const TreeArgs &a, const TileShared *sh, int BT, uint32_t o_tmem) {
   const int part = threadIdx.x >> 7, r_own = threadIdx.x & 127, D = a.head_dim;
   const int row = sh->seg.rt * kTileRows + r_own, n = row / a.group, h = sh->seg.kvh * a.group + row % a.group;
   const size_t node = (size_t)sh->seg.b * a.nodes + n;
@@ -321,6 +346,15 @@ __device__ __noinline__ void write_rows(const TreeArgs &a, TileShared *sh, uint3
     uint32_t r[16];
     tmem_ld16(o_tmem + d, r);
     tmem_ld_wait(r);
+    if (sh->nan) {
+      uint32_t y[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] = r[i];
+      put_nan(a, sh, BT, r_own, d, y);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) r[i] = y[i];
+    }
+    __syncwarp();
     if (live) {
       float x[16];
 #pragma unroll
@@ -459,7 +493,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       for (int i = 0; i < META; ++i) mbar_init(&sh->metafull[i], 1);
       mbar_init(&sh->qready, kSoftWarps);
       mbar_init(&sh->drain, 1);
-      sh->abort = sh->never = 0;
+      sh->abort = sh->never = sh->nan = 0;
       fence_barrier_init();
     }
     __syncwarp();
@@ -624,9 +658,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         __syncwarp();
         tc_fence_after();
         if (whole)
-          write_rows(a, sh, my + Sh::kTmemO);
+          write_rows(a, sh, BT, my + Sh::kTmemO);
         else
-          write_part(a, slot, my + Sh::kTmemO);
+          write_part(a, sh, BT, slot, my + Sh::kTmemO);
       }
       soft_sync();  // O, red and the segment are read: the next may overwrite them
     }
@@ -805,15 +839,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           ft[(t >> 1) * 4 + 2 + (t & 1)] = pow2i((int)kv8_value_exponent(xv[i]) - kSpread);
         }
       }
-      if (open) {  // values that are not a number: zero in the product, and the token's score NaN for those who see it
+      if (open) {  // values that are not a number: zero in the product, and told to the softmax ahead of the tile
         wait(&sh->rvfull[rs], g / RAW);
-        conv_sync();
 #pragma unroll 1
         for (int i = 0; i < P; ++i) {
           const uint4 v = *reinterpret_cast<const uint4 *>(rV + rs * Sh::kRawBytes + src + i * kStep * (DP == 64 ? 64 : 128));
-          const int t = t_own + i * kStep;
-          if (not_numbers(v.x) | not_numbers(v.y) | not_numbers(v.z) | not_numbers(v.w))
-            ft[(t >> 1) * 4 + (t & 1)] = __int_as_float(0x7fc00000);
+          if (not_numbers(v.x) | not_numbers(v.y) | not_numbers(v.z) | not_numbers(v.w)) sh->nan = 1;
         }
         conv_sync();
       }

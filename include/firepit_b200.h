@@ -793,7 +793,8 @@ int fpb_kv8_keep(uint8_t *k_codes, uint8_t *v_codes, uint8_t *k_exp, uint8_t *v_
  * head_dim] bf16 = softmax(scale q . k) v, times sigmoid(gate) where gate
  * [batch * nodes rows of gate_pitch, heads of gate_head_pitch] f32 is given.
  * Rows of the cache that a node does not see never reach its output, whatever
- * they hold. */
+ * they hold; a NaN among the values of one that it sees makes that column NaN,
+ * one among the keys the whole output. */
 size_t fpb_tree_attn_workspace_bytes(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, size_t head_dim,
                                      size_t max_seq);
 int fpb_tree_attn(const void *q, int q_dtype, size_t q_pitch, size_t q_head_pitch, const uint8_t *k_codes,

@@ -624,3 +624,33 @@ def test_zero_values_with_the_largest_scores(F, torch, hq, d, size, zeros):
         o, pv, sabs = R.attend(np.ones(d), k[rows], v[rows], 1 / math.sqrt(d))
         bound = (2 * 2.0 ** -11 * sabs + 2.0 ** -11 + 2.0 ** -16) * pv
         assert (np.abs(got[0, j] - o) <= bound + 2.0 ** -8 * np.abs(o)).all(), (j, got[0, j, 0, :4], o[:4])
+
+
+# ---- NaN among the values -------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("hq", [2, 8, 48])  # both kernels
+@pytest.mark.parametrize("d", [48, 64, 128, 256])
+@pytest.mark.parametrize("tree", [True, False])
+def test_a_nan_code_reaches_its_column_alone(F, torch, hq, d, tree):
+    """A NaN among the codes of a value makes that column NaN for the nodes that
+    see its row, in the context as in the tree, and nothing else."""
+    rng = np.random.default_rng(24)
+    s, pos, n, hk = 300, 290, 4, 2
+    clean = _cache(F, torch, rng, 1, s, hk, d)
+    dirty = F.Kv8Cache(*(getattr(clean, x).clone() for x in ("k", "v", "k_exp", "v_exp")))
+    par = np.array([[-1, 0, 0, 1]], np.int32) if tree else None
+    lines = _lines(par, 1, n)[0]
+    at = [(7, 3), (7, 17), (289, 0), (pos + 1, 5), (pos + 1, d - 1), (pos + 2, 31), (pos + 3, 14)]
+    want = np.zeros((n, d), bool)
+    for row, col in at:
+        dirty.v[0, row, 1, col] = 0x7f if col % 2 else 0xff
+        for j in range(n):
+            want[j, col] |= row < pos or row - pos in lines[j]
+    q = _dev(torch, rng.standard_normal((1, n, hq, d)).astype(np.float32))
+    where, par = _dev(torch, np.array([pos], np.int32)), None if par is None else _dev(torch, par)
+    a, b = (F.tree_attention(q, c, where, par)[0] for c in (clean, dirty))
+    nan = torch.isnan(b).cpu().numpy()
+    assert not nan[:, :hq // 2].any() and torch.equal(a[:, :hq // 2], b[:, :hq // 2])
+    for h in range(hq // 2, hq):
+        assert np.array_equal(nan[:, h], want), h
+    # elsewhere the outputs are the clean ones, but for the codes that a NaN has replaced
+    assert torch.equal(torch.where(torch.isnan(b), 0.0, b), torch.where(torch.isnan(b), 0.0, a))
