@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kAppendThreads, 7) kv8_append_kernel(const __g
       for (int i = 0; i < 8; ++i) ss = fmaf(x[j][i], x[j][i], ss);
 #pragma unroll
     for (int o = LG / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (gamma && live) {
+    if (gamma && live && depth >= 0) {  // (a norm of zeros with eps 0 would be NaN)
       const float scale = __frsqrt_rn(fmaf(ss, a.inv_d, a.eps));
 #pragma unroll
       for (int j = 0; j < 2; ++j) {

@@ -654,3 +654,18 @@ def test_a_nan_code_reaches_its_column_alone(F, torch, hq, d, tree):
         assert np.array_equal(nan[:, h], want), h
     # elsewhere the outputs are the clean ones, but for the codes that a NaN has replaced
     assert torch.equal(torch.where(torch.isnan(b), 0.0, b), torch.where(torch.isnan(b), 0.0, a))
+
+
+# ---- absent nodes ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("eps", [0.0, 1e-6])
+def test_append_of_absent_nodes_gives_zeros_at_any_eps(F, torch, eps):
+    rng = np.random.default_rng(25)
+    d = 64
+    q, k = (_dev(torch, rng.standard_normal((1, 4, 2, d)).astype(np.float32)) for _ in range(2))
+    ones = torch.ones(d, device="cuda")
+    cache = F.Kv8Cache.zeros(1, 8, 2, d)
+    got = F.kv8_append(cache, torch.zeros(1, dtype=torch.int32, device="cuda"), k, k, q=q,
+                       parents=_dev(torch, np.array([[-1, -2, 0, 1]], np.int32)), q_gamma=ones, k_gamma=ones, eps=eps,
+                       rotary_dim=32)
+    assert not got[0, [1, 3]].any() and torch.isfinite(got).all() and (got[0, [0, 2]] != 0).any(-1).all()
+    assert not cache.k[0, [1, 3]].any() and cache.k[0, [0, 2]].any()
