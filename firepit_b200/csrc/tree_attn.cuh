@@ -50,21 +50,22 @@ struct Sight {
 };
 
 // The tree is walked through the warp's registers: all 32 lanes call this, each
-// with its own node (n >= nodes: none).
+// with its own node (n >= nodes: none).  A row outside the cache is an error of a
+// node that would be there.
 __device__ __forceinline__ Sight sight_of(const TreeArgs &a, int b, int n, int pos) {
   Sight s{-1, 0};
   const bool in = n < a.nodes;
   const bool inside = pos >= 0 && pos < a.max_seq - n;
-  if (in && !inside && a.error) atomicCAS(a.error, 0, kErrPosition);
   if (!a.parents) {
     if (in && inside) s.upto = n + 1;
+    if (in && !inside && a.error) atomicCAS(a.error, 0, kErrPosition);
     return s;
   }
   const int32_t *par = a.parents + (size_t)b * a.nodes;
   const int lane = threadIdx.x & 31;
   const int p0 = lane < a.nodes ? par[lane] : -2, p1 = lane + 32 < a.nodes ? par[lane + 32] : -2;
   const int root = __shfl_sync(0xffffffffu, p0, 0);  // (by every lane, outside the conditions)
-  bool there = in && inside && root == -1;
+  bool there = in && root == -1;
   bool going = there && n > 0;
   int j = in ? n : 0;
   while (__any_sync(0xffffffffu, going)) {
@@ -80,6 +81,10 @@ __device__ __forceinline__ Sight sight_of(const TreeArgs &a, int b, int n, int p
         going = j > 0;
       }
     }
+  }
+  if (there && !inside) {
+    there = false;
+    if (a.error) atomicCAS(a.error, 0, kErrPosition);
   }
   if (there) {
     s.upto = n + 1;

@@ -669,3 +669,22 @@ def test_append_of_absent_nodes_gives_zeros_at_any_eps(F, torch, eps):
                        rotary_dim=32)
     assert not got[0, [1, 3]].any() and torch.isfinite(got).all() and (got[0, [0, 2]] != 0).any(-1).all()
     assert not cache.k[0, [1, 3]].any() and cache.k[0, [0, 2]].any()
+
+
+@pytest.mark.parametrize("hq", [2, 24])  # both kernels
+def test_absent_nodes_past_the_cache_are_no_error(F, torch, hq):
+    """Only a node that is there can lie outside the cache: the slots that a tree
+    leaves empty at the end of its cache, and a session without a tree at any
+    position, record nothing."""
+    rng = np.random.default_rng(26)
+    s, n, d = 40, 4, 32
+    cache = _cache(F, torch, rng, 3, s, 1, d)
+    par = np.array([[-1, 0, -2, -2], [-2, -2, -2, -2], [-1, 0, 1, 2]], np.int32)
+    got = _check_attention(F, torch, rng, cache, [s - 2, 7, s - n], par, n, hq)
+    assert got[0, :2].any(-1).all() and F.device_error(reset=True) == 0
+    q = _dev(torch, rng.standard_normal((3, n, hq, d)).astype(np.float32))
+    out = F.tree_attention(q, cache, _dev(torch, np.array([s - 2, -5, s - n], np.int32)), _dev(torch, par))
+    assert not out[1].any() and F.device_error(reset=True) == 0
+    par[0, 2] = 0  # node 2 is there now, and outside
+    out = F.tree_attention(q, cache, _dev(torch, np.array([s - 2, 7, s - n], np.int32)), _dev(torch, par))
+    assert out[0, :2].any() and not out[0, 2:].any() and F.device_error(reset=True) == 502
