@@ -38,6 +38,7 @@ class _Torch:
         cls.raw_stream = staticmethod(torch._C._cuda_getCurrentRawStream) if hasattr(
             torch._C, "_cuda_getCurrentRawStream") else staticmethod(
                 lambda index: torch.cuda.current_stream(index).cuda_stream)
+        cls.current_device = staticmethod(getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device))
         cls.module = torch
 
 
@@ -53,6 +54,17 @@ def _empty(stream, like, dtype, *shape):
 
 def _handle(stream, like) -> int:
     return _Torch.raw_stream(like.get_device()) if stream is None else stream
+
+
+def _on_device(what: str, like, *tensors) -> None:
+    """A call's tensors lie on the current CUDA device: their addresses are what
+    the kernels get."""
+    device = like.get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise ShapeError(f"{what}: tensors on {like.device} and {t.device}")
+    if device < 0 or device != _Torch.current_device():
+        raise ShapeError(f"{what}: tensors on {like.device}, which is not the current CUDA device")
 
 
 def _code(t) -> int:
@@ -160,13 +172,14 @@ def kv8_append(cache: Kv8Cache, positions, k, v, q=None, parents=None, q_gamma=N
                              f"{q.dtype}")
         hq, q_pitch = q.shape[2], _rows(q, "q", b, n)
         q_head = q.stride(2) if hq > 1 else d
-        if q_out is None:
-            q_out = _empty(stream, q, q.dtype, b, n, hq, d)
-        elif q_out.shape != (b, n, hq, d) or not q_out.is_contiguous():
+        if q_out is not None and (q_out.shape != (b, n, hq, d) or not q_out.is_contiguous()):
             raise ShapeError(f"kv8_append: q_out [{b}, {n}, {hq}, {d}] contiguous expected")
-        out_code = _code(q_out)
+        out_code = _code(q if q_out is None else q_out)
     elif q_out is not None:
         raise ShapeError("kv8_append: q_out without q")
+    _on_device("kv8_append", cache.k, positions, k, v, q, parents, q_gamma, k_gamma, q_out)
+    if q is not None and q_out is None:
+        q_out = _empty(stream, q, q.dtype, b, n, hq, d)
     N.call("fpb_kv8_append", _ptr(q), q_pitch, q_head, k.data_ptr(), _rows(k, "k", b, n), v.data_ptr(),
            _rows(v, "v", b, n), _code(k), _ptr(q_gamma), _ptr(k_gamma), positions.data_ptr(), _ptr(parents), b, n, hq,
            hk, d, rotary_dim, theta, eps, s, _ptr(q_out), out_code, cache.k.data_ptr(), cache.v.data_ptr(),
@@ -179,12 +192,13 @@ def kv8_read(cache: Kv8Cache, begin, count: int, dtype=None, stream=None):
     [begin, begin + count) stand for; begin: an int, or int32 [batch]."""
     b, s, hk, d = cache.shape
     dtype = _Torch.f32 if dtype is None else dtype
-    begins = None
+    begins = where = None
     if not isinstance(begin, int):
         _ints(begin, "begin", b)
-        begins, begin = begin.data_ptr(), 0
+        where, begins, begin = begin, begin.data_ptr(), 0
     if count < 1 or begin < 0:
         raise ShapeError(f"kv8_read: rows [{begin}, +{count})")
+    _on_device("kv8_read", cache.k, where)
     k, v = _empty(stream, cache.k, dtype, b, count, hk, d), _empty(stream, cache.k, dtype, b, count, hk, d)
     N.call("fpb_kv8_read", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), b,
            s, hk, d, begins, begin, count, k.data_ptr(), v.data_ptr(), _code(k), _handle(stream, cache.k))
@@ -197,6 +211,7 @@ def kv8_keep(cache: Kv8Cache, positions, path, stream=None) -> None:
     b, s, hk, d = cache.shape
     _ints(positions, "positions", b)
     _ints(path, "path", b, path.shape[-1])
+    _on_device("kv8_keep", cache.k, positions, path)
     N.call("fpb_kv8_keep", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), b, s,
            hk, d, positions.data_ptr(), path.data_ptr(), path.shape[1], _handle(stream, cache.k))
 
@@ -225,10 +240,13 @@ def tree_attention(q, cache: Kv8Cache, positions, parents=None, gate=None, scale
         if gate.shape != q.shape or gate.dtype is not _Torch.f32:
             raise ShapeError(f"tree_attention: gate f32 {list(q.shape)} expected")
         gate_pitch, gate_head = _rows(gate, "gate", b, n), gate.stride(2) if hq > 1 else d
+    if out is not None and (out.shape != q.shape or out.dtype is not _Torch.bf16 or not out.is_contiguous()):
+        raise ShapeError("tree_attention: out bf16 of q's shape, contiguous, expected")
+    if workspace is not None and (workspace.dtype is not _Torch.u8 or not workspace.is_contiguous()):
+        raise ShapeError("tree_attention: workspace contiguous uint8 expected")
+    _on_device("tree_attention", cache.k, q, positions, parents, gate, out, workspace)
     if out is None:
         out = _empty(stream, q, _Torch.bf16, b, n, hq, d)
-    elif out.shape != q.shape or out.dtype is not _Torch.bf16 or not out.is_contiguous():
-        raise ShapeError("tree_attention: out bf16 of q's shape, contiguous, expected")
     if workspace is None:
         workspace = _empty(stream, q, _Torch.u8, N.lib.fpb_tree_attn_workspace_bytes(b, n, hq, hk, d, s))
     N.call("fpb_tree_attn", q.data_ptr(), _code(q), _rows(q, "q", b, n), q.stride(2) if hq > 1 else d,
@@ -272,6 +290,7 @@ def tree_verify(logits, tokens, parents=None, temperature: float = 0.0, accept=N
             draft_pitch = _pitch(draft, "draft")
     else:
         accept = noise = draft = None
+    _on_device("tree_verify", logits, tokens, parents, accept, noise, draft)
     path = _empty(stream, logits, _Torch.i32, b, n)
     count, nxt = _empty(stream, logits, _Torch.i32, b), _empty(stream, logits, _Torch.i32, b)
     N.call("fpb_tree_verify", logits.data_ptr(), _code(logits), _pitch(logits, "logits"), _ptr(draft), draft_pitch,

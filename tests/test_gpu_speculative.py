@@ -688,3 +688,30 @@ def test_absent_nodes_past_the_cache_are_no_error(F, torch, hq):
     par[0, 2] = 0  # node 2 is there now, and outside
     out = F.tree_attention(q, cache, _dev(torch, np.array([s - 2, 7, s - n], np.int32)), _dev(torch, par))
     assert out[0, :2].any() and not out[0, 2:].any() and F.device_error(reset=True) == 502
+
+
+def test_wrappers_refuse_tensors_of_another_device(F, torch):
+    """One argument at a time on the host, the others on the GPU: refused before
+    anything is launched."""
+    cache = F.Kv8Cache.zeros(2, 32, 2, 64)
+    z = dict(device="cuda")
+    pos, par = torch.zeros(2, dtype=torch.int32, **z), torch.zeros(2, 4, dtype=torch.int32, **z)
+    q, kv, ones = torch.zeros(2, 4, 6, 64, **z), torch.zeros(2, 4, 2, 64, **z), torch.ones(64, **z)
+    lg, unit = torch.zeros(2, 4, 10, **z), torch.ones(2, 10, **z)
+    ws = torch.zeros(F.tree_attention_workspace_bytes(cache, 4, 6), dtype=torch.uint8, **z)
+    calls = [
+        (F.kv8_append, dict(positions=pos, k=kv, v=kv, q=q, parents=par, q_gamma=ones, k_gamma=ones, q_out=q.clone())),
+        (F.kv8_read, dict(begin=pos, count=4)),
+        (F.kv8_keep, dict(positions=pos, path=par)),
+        (F.tree_attention, dict(q=q, positions=pos, parents=par, gate=q, out=q.bfloat16(), workspace=ws)),
+        (F.tree_verify, dict(logits=lg, tokens=par, parents=par, accept=lg[..., 0].contiguous(), noise=unit, draft=lg)),
+    ]
+    launches = F.launch_count()
+    for call, args in calls:
+        own = dict(temperature=1.0) if call is F.tree_verify else dict(cache=cache)
+        for name, t in args.items():
+            if torch.is_tensor(t):
+                with pytest.raises(F.ShapeError, match="cpu"):
+                    call(**own, **dict(args, **{name: t.cpu()}))
+                    pytest.fail(f"{call.__name__}: {name} was taken")
+    assert F.launch_count() == launches

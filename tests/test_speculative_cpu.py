@@ -135,3 +135,27 @@ def test_speculative_decoder_refuses_what_it_cannot_run():
     assert lookup_drafts([1, 2, 3, 4, 1, 2], 3) == ([3, 4], [0, 1])
     assert lookup_drafts([1, 2, 3], 3) == ([], [])
     assert lookup_drafts([5], 3) == ([], [])
+
+
+def test_speculative_wrappers_check_devices():
+    """Tensors that are right in every other way, but not on a CUDA device: no
+    address of theirs reaches a kernel."""
+    torch = pytest.importorskip("torch")
+    cache = F.Kv8Cache.zeros(2, 32, 2, 64, device="cpu")
+    pos = torch.zeros(2, dtype=torch.int32)
+    par = torch.zeros(2, 4, dtype=torch.int32)
+    q, kv, gamma = torch.zeros(2, 4, 6, 64), torch.zeros(2, 4, 2, 64), torch.ones(64)
+    logits, unit = torch.zeros(2, 4, 10), torch.ones(2, 10)
+    ws = torch.zeros(F.tree_attention_workspace_bytes(cache, 4, 6), dtype=torch.uint8)
+    for call in (lambda: F.kv8_append(cache, pos, kv, kv, q=q, parents=par, q_gamma=gamma, k_gamma=gamma),
+                 lambda: F.kv8_append(cache, pos, kv, kv),
+                 lambda: F.kv8_read(cache, pos, 4), lambda: F.kv8_read(cache, 0, 4),
+                 lambda: F.kv8_keep(cache, pos, par),
+                 lambda: F.tree_attention(q, cache, pos, par, gate=q), lambda: F.tree_attention(q, cache, pos),
+                 lambda: F.tree_attention(q, cache, pos, par, out=q.bfloat16(), workspace=ws),
+                 lambda: F.tree_verify(logits, par, par),
+                 lambda: F.tree_verify(logits, par, par, 1.0, torch.zeros(2, 4), unit, draft=logits)):
+        with pytest.raises(F.ShapeError, match="device"):
+            call()
+    with pytest.raises(F.ShapeError, match="workspace"):
+        F.tree_attention(q, cache, pos, par, workspace=ws.float())
