@@ -525,11 +525,30 @@ class SpeculativeDecoder(Decoder):
         self.next = torch.zeros(sessions, **i32)
         self.emitted = torch.full((sessions, nodes), -1, **i32)
         self.at = torch.arange(nodes, **i32)
-        self.draft = None
+        self._draft = None
         self.accept = self.noise = None
         if temperature > 0.0:
             self.accept = torch.zeros(sessions, nodes, device=dev)
             self.noise = torch.ones(sessions, c.vocab, device=dev)
+
+    @property
+    def draft(self):
+        """The probabilities [sessions, nodes, vocab] f32 that each node's children
+        are drawn from (None: certain drafts).  A step reads the tensor that it
+        was issued or captured with, so setting another one drops ``graph``."""
+        return self._draft
+
+    @draft.setter
+    def draft(self, value) -> None:
+        from .gemv import ShapeError
+        shape = (self.sessions, self.nodes, self.cfg.vocab)
+        if value is not None and (value.shape != shape or value.dtype != self.logits.dtype or
+                                  not value.is_contiguous() or value.device != self.logits.device):
+            raise ShapeError(f"draft: contiguous f32 {list(shape)} on {self.logits.device} expected, got {value.dtype} "
+                             f"{list(value.shape)} on {value.device}")
+        if value is not self._draft:
+            self.__dict__.pop("graph", None)
+        self._draft = value
 
     def reset(self) -> None:
         super().reset()

@@ -319,3 +319,49 @@ def test_a_step_keeps_to_its_stream(torch, model):
         runs.append(got)
     assert runs[0] == runs[1]
     _no_error()
+
+
+def test_a_step_with_drawn_drafts(torch, model):
+    """``draft`` through the decoder: the walk is the definition's on the step's own
+    logits, eager and captured; what does not fit is refused, and a step captured
+    with other probabilities is dropped."""
+    import firepit_b200 as F
+    from firepit_b200.model import SpeculativeDecoder
+    from oracle import speculative as R
+    vocab, par = model.cfg.vocab, [[-1, 0, 0, 1], [-1, 0, 1, 1]]
+    dec = SpeculativeDecoder(model, 2, 4, 64, temperature=0.9)
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    sh, draft = torch.cuda.current_stream().cuda_stream, torch.empty(2, 4, vocab, device="cuda")
+    for bad in (draft[:, :3], draft[..., 1:], draft.double(), draft.cpu(), draft[:1]):
+        with pytest.raises(F.ShapeError):
+            dec.draft = bad
+    assert dec.draft is None
+    dec.step(sh)
+    dec.capture()
+    dec.draft = draft
+    assert not hasattr(dec, "graph")
+    dec.step(sh)
+    dec.capture()
+    dec.draft = draft  # the same: the captured step stays
+    dec.reset()
+    dec.feed(torch.tensor([[1, 2, 3], [4, 5, 6]], dtype=torch.int32, device="cuda"))
+    lengths = set()
+    for k in range(8):
+        dec.draw(gen)
+        # flat and peaked drafts by turns; the children drawn from their parents' rows
+        draft.copy_(torch.softmax(torch.randn(2, 4, vocab, generator=gen, device="cuda") * (k % 4), -1))
+        dec.parents.copy_(torch.tensor(par, dtype=torch.int32))
+        up = dec.parents.clamp(min=0).long()
+        drawn = torch.multinomial(draft.view(8, vocab), 4, True, generator=gen).view(2, 4, 4)
+        dec.tree[:, 1:] = torch.gather(drawn.permute(0, 2, 1), 2, up[..., None]).squeeze(2)[:, 1:].int()
+        tokens = dec.tree.cpu().numpy().copy()
+        dec.graph.replay() if k % 2 else dec.step(sh)
+        logits, q = dec.logits.view(2, 4, vocab).cpu().numpy(), draft.cpu().numpy()
+        for s in range(2):
+            path, token = R.verify(logits[s], tokens[s], par[s], dec.temperature, dec.accept[s].cpu().numpy(),
+                                   dec.noise[s].cpu().numpy(), q[s])
+            assert dec.path[s].tolist() == path + [-1] * (4 - len(path)) and dec.next[s].item() == token
+            assert dec.tree[s, 0].item() == token
+            lengths.add(len(path))
+    assert len(lengths) > 1
+    _no_error()
