@@ -596,6 +596,16 @@ class SpeculativeDecoder(Decoder):
             self.step(sh)  # (what the verification keeps of a chain lies where it is)
             self.positions.copy_(before.add_(m))
 
+    def prefill(self, prompt) -> None:
+        """Takes the prompt [sessions, length] (device int32) up to where the next
+        step emits the first token after it: the rows of all but its last token
+        join the cache, and that one is each session's first node."""
+        if prompt.shape[1] > 1:
+            self.feed(prompt[:, :-1])
+        self.tree[:, 0].copy_(prompt[:, -1])
+        self.parents.fill_(-2)
+        self.parents[:, 0] = -1
+
     def generate(self, prompt, new_tokens: int, drafter) -> list[list[int]]:
         """Appends at least `new_tokens` tokens to each session's prompt
         [sessions, length]; drafter(history: list[int], nodes) -> (tokens,
@@ -614,9 +624,7 @@ class SpeculativeDecoder(Decoder):
             raise ShapeError(f"generate: {prompt.shape[1]} + {new_tokens} tokens and two steps' nodes in a cache of "
                              f"{self.max_seq} rows")
         self.reset()
-        if prompt.shape[1] > 1:
-            self.feed(prompt[:, :-1])
-        self.tree[:, 0].copy_(prompt[:, -1])
+        self.prefill(prompt)
         sh = torch.cuda.current_stream(self.model.device).cuda_stream
         history = prompt.cpu().tolist()
         start = [len(h) for h in history]

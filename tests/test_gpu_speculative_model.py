@@ -365,3 +365,35 @@ def test_a_step_with_drawn_drafts(torch, model):
             lengths.add(len(path))
     assert len(lengths) > 1
     _no_error()
+
+
+@pytest.mark.parametrize("length", [1, 4, 5, 9])
+def test_prefill_leads_to_the_first_token(torch, model, length):
+    """The decoder's prefill on the speculative one: chunks of four rows, whole or
+    not, and a prompt of one token; the steps after it emit greedy decoding's
+    tokens, with what an earlier step left in the tree."""
+    from firepit_b200.model import Decoder, SpeculativeDecoder
+    prompt = torch.tensor([[7, 1, 9, 30, 2, 8, 8, 1, 3], [4, 8, 15, 16, 23, 42, 4, 8, 5]], dtype=torch.int32,
+                          device="cuda")[:, :length].contiguous()
+    plain = Decoder(model, 2, 64, history_len=8, kv8=True)
+    plain.capture()
+    plain.reset()
+    plain.prefill(prompt)
+    first = plain.tokens.tolist()
+    plain.generate(3)
+    want = [[f] + h[:3] for f, h in zip(first, plain.history.tolist())]
+    dec = SpeculativeDecoder(model, 2, 4, 64)
+    sh = torch.cuda.current_stream().cuda_stream
+    dec.tree.fill_(77)
+    dec.parents.copy_(torch.tensor([[-1, 0, 0, 0]] * 2, dtype=torch.int32))
+    dec.step(sh)
+    dec.positions.zero_()
+    dec.prefill(prompt)
+    assert dec.positions.tolist() == [length - 1] * 2
+    got = []
+    for _ in range(4):
+        dec.step(sh)
+        assert dec.count.tolist() == [1, 1]
+        got.append(dec.emitted[:, 0].tolist())
+    assert [list(g) for g in zip(*got)] == want
+    _no_error()
