@@ -715,3 +715,37 @@ def test_wrappers_refuse_tensors_of_another_device(F, torch):
                     call(**own, **dict(args, **{name: t.cpu()}))
                     pytest.fail(f"{call.__name__}: {name} was taken")
     assert F.launch_count() == launches
+
+
+# ---- offsets past 32 bits -------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("hq", [4, 40])  # both kernels
+def test_attention_and_moves_past_32_bits(F, torch, hq):
+    """The last session of a cache of over 2^32 codes, its rows at the end: the
+    own row's score is large and positive, so that the output is that row's value;
+    then a path that moves rows there."""
+    b, s, hk, d = 5, 1 << 21, 2, 256
+    cache = F.Kv8Cache.zeros(b, s, hk, d)
+    rng = np.random.default_rng(27)
+    pos = np.array([3, 0, 0, 0, s - 300], np.int32)
+    kv = _dev(torch, rng.standard_normal((b, 3, 2, hk, d)).astype(np.float32))
+    k, v = kv[:, :, 0], kv[:, :, 1]
+    par = _dev(torch, np.array([[-1, 0, 0]] * b, np.int32))
+    where = _dev(torch, pos)
+    F.kv8_append(cache, where, k, v, parents=par)
+    held_k, held_v = F.kv8_read(cache, where, 3)
+    # zero keys score 0, the own one 20 |k|^2 / 16 of about 300, another node's some 80 at most beside it
+    q = 20.0 * k.repeat_interleave(hq // hk, 2)
+    score = torch.einsum("bihd,bjhd->bhij", q, held_k.repeat_interleave(hq // hk, 2)) / 16
+    own = score.diagonal(dim1=2, dim2=3)
+    assert float(own.min()) > 60 + float((score - torch.diag_embed(own)).max())
+    out = F.tree_attention(q, cache, where, par).float()
+    want = held_v.repeat_interleave(hq // hk, 2)
+    # the other weights are below 2^21 e^-60, the own one is 1 but for its own f16's 2^-11 and bf16's 2^-8
+    assert bool(((out - want).abs() <= (2.0 ** -11 + 2.0 ** -8) * want.abs() + 1e-12).all())
+    before = {x: getattr(cache, x)[4, s - 300:s - 296].clone() for x in ("k", "v", "k_exp", "v_exp")}
+    F.kv8_keep(cache, where, _dev(torch, np.array([[0, 2, -1]] * b, np.int32)))
+    for x, old in before.items():
+        now = getattr(cache, x)[4, s - 300:s - 296]
+        assert torch.equal(now[[0, 2, 3]], old[[0, 2, 3]]) and torch.equal(now[1], old[2]), x
+        assert x.endswith("exp") or not torch.equal(old[1], old[2])
+    del cache
