@@ -22,9 +22,12 @@
 // softmax's and the converters' instructions 1350 issue cycles a scheduler, and
 // shared memory about 1800 (copies in, converters' reads and writes, operands,
 // factors).  Issue slots 51% busy, tensor cores 33%.
-//   8 sessions x 16 nodes x 16 heads (2 kv) x 256, 16384 tokens: 59.5 us with its
-//     two helpers; 2.1 TB/s of the cache, 455 TFLOP/s
-//   4 x 61 x 32 (4) x 128, 30011 tokens: 178 us, 540 TFLOP/s
+//   8 sessions x 16 nodes x 16 heads (2 kv) x 256, 16384 tokens: 61 us with its
+//     two helpers; 2.05 TB/s of the cache, 443 TFLOP/s
+//   4 x 61 x 32 (4) x 128, 30011 tokens: 183 us, 525 TFLOP/s
+//   a prompt's chunk of 2048 rows x 16 heads (2 kv) x 256: 163 us from position 0
+//     (211 TFLOP/s: a row tile's share counts its session's tiles, of which it
+//     sees half), 436 us from 8192 (710 TFLOP/s)
 // Before the first products the block spends 8 us (start, shares, queries), at
 // its end 4 us on the 64 to 128 KB of its partial result.
 #include <algorithm>

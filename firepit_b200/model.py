@@ -584,7 +584,8 @@ class SpeculativeDecoder(Decoder):
 
     def feed(self, tokens) -> None:
         """Runs known tokens [sessions, n] (device int32) through the model,
-        `nodes` of them a step (teacher forcing); their rows join the cache."""
+        `nodes` of them a step (teacher forcing); their rows join the cache.  The
+        steps are whole ones, issued one by one: what they verify is not used."""
         import torch
         sh = torch.cuda.current_stream(self.model.device).cuda_stream
         for t in range(0, tokens.shape[1], self.nodes):
@@ -611,7 +612,9 @@ class SpeculativeDecoder(Decoder):
         [sessions, length]; drafter(history: list[int], nodes) -> (tokens,
         parents) proposes each step's tree after its first node (lists of at
         most nodes - 1 entries; a parent is 0 for the first node, k for the
-        k-th drafted token).  A session that has its tokens sits the other
+        k-th drafted token); they count as certain unless ``draft`` holds what
+        they were drawn from.  The steps are issued one by one, not replayed, and
+        above temperature 0 take torch's default generator.  A session that has its tokens sits the other
         sessions' steps out, so none goes more than `nodes` rows past them.
         Returns the new tokens of each session; a device error, which would
         make them doubtful, is raised (and left for ``device_error`` to

@@ -10,8 +10,9 @@ The reference has none of these: its cache is f32 (attention.rs:6-30) and its
 greedy decode takes one token a step (generation.rs:34-42).
 
 A tree is ``parents`` [batch, nodes] int32: -1 for node 0, an earlier node for
-the others, -2 for a node that is not there.  Every call only enqueues work on
-``stream`` (default: the current one); the outputs it allocates belong to it.
+the others, -2 for a node that is not there.  A call's tensors lie on the current
+CUDA device.  Every call only enqueues work on ``stream`` (default: the current
+one); the outputs it allocates belong to it.
 """
 from __future__ import annotations
 
@@ -226,7 +227,9 @@ def tree_attention(q, cache: Kv8Cache, positions, parents=None, gate=None, scale
     """out [batch, nodes, q_heads, head_dim] bf16: each node's attention over
     the rows before its session's position, its ancestors and itself (already
     appended), times sigmoid(gate) where a gate (f32, q's shape) is given.
-    q f32 or bf16, any row and head pitch; scale default 1 / sqrt(head_dim);
+    q f32 or bf16, any row and head pitch, rounded to f16 for the products (each
+    row scaled by a power of two), as the weights are; scale default 1 /
+    sqrt(head_dim);
     ``workspace``: uint8 of ``tree_attention_workspace_bytes`` (allocated where
     None)."""
     b, s, hk, d = cache.shape

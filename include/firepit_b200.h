@@ -794,7 +794,13 @@ int fpb_kv8_keep(uint8_t *k_codes, uint8_t *v_codes, uint8_t *k_exp, uint8_t *v_
  * [batch * nodes rows of gate_pitch, heads of gate_head_pitch] f32 is given.
  * Rows of the cache that a node does not see never reach its output, whatever
  * they hold; a NaN among the values of one that it sees makes that column NaN,
- * one among the keys the whole output. */
+ * one among the keys the whole output.
+ * The products are of f16 with f32 sums: q, f32 too, is rounded to f16's 11 bits
+ * (its row scaled by a power of two), the codes are exact, the softmax's weights
+ * are rounded to 11 bits beside a sum of f32 ones.  Against 64 bits the bf16
+ * output is off by up to 4 % more than that of a form in 32 bits.  batch * nodes
+ * at most 65535 (a longer prompt goes in several calls), batch * kv_heads and the
+ * tiles of 128 rows too. */
 size_t fpb_tree_attn_workspace_bytes(size_t batch, size_t nodes, size_t q_heads, size_t kv_heads, size_t head_dim,
                                      size_t max_seq);
 int fpb_tree_attn(const void *q, int q_dtype, size_t q_pitch, size_t q_head_pitch, const uint8_t *k_codes,
@@ -817,8 +823,9 @@ int fpb_tree_attn(const void *q, int q_dtype, size_t q_pitch, size_t q_head_pitc
  * Writes path [batch, nodes] (the accepted nodes, 0 first, then -1), count
  * [batch] (their number) and next [batch] (the token after them); a session
  * with no tree: count 0, next -1.  nodes <= 64, vocab <= 442368
- * (FPB_ERR_UNSUPPORTED above).  One launch; of the tree's rows only the path's and
- * its nodes' children's are touched. */
+ * (FPB_ERR_UNSUPPORTED above).  The powers and the draw's quotients are f32 to
+ * 2^-22 of themselves.  One launch; of the tree's rows only the path's and its
+ * nodes' children's are touched. */
 int fpb_tree_verify(const void *logits, int logits_dtype, size_t logits_pitch, const float *draft, size_t draft_pitch,
                     const int32_t *tokens, const int32_t *parents, const float *accept, const float *noise,
                     size_t noise_pitch, size_t batch, size_t nodes, size_t vocab, float temperature, int32_t *path,
