@@ -21,7 +21,7 @@
 // and 128 columns takes 2600 cycles, of which the two products need 1280, the
 // softmax's and the converters' instructions 1350 issue cycles a scheduler, and
 // shared memory about 1800 (copies in, converters' reads and writes, operands,
-// factors).  Issue slots 51% busy, tensor cores 33%.
+// factors).  Issue slots 54% busy, tensor cores 33%.
 //   8 sessions x 16 nodes x 16 heads (2 kv) x 256, 16384 tokens: 61 us with its
 //     two helpers; 2.05 TB/s of the cache, 443 TFLOP/s
 //   4 x 61 x 32 (4) x 128, 30011 tokens: 183 us, 525 TFLOP/s
