@@ -153,11 +153,11 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // (weights up to 2^(kHead + kLag)).
 constexpr float kHead = 7.0f, kLag = 8.0f, kMost = 32768.0f, kLowest = -1e30f;
 // Their sum takes them without the values' exponents v, which lie within [-100,
-// 120]: a value's size is no part of its weight.  Since m >= y + v - kLag for
-// every score y, 2^(y - m + kHead) could reach 2^115, and the largest be 2^-113;
-// times 2^kSpread that becomes 2^126 and 2^-102, so that no weight overflows and
-// none is lost that is above 2^-24 of the largest.  The value's factor takes
-// 2^kSpread back, and the sum is held times kSumScale (2^20 weights fit), what
+// 120]: a value's size is no part of its weight.  Since m >= y + v - kLag (in the
+// tiles a half less) for every score y, 2^(y - m + kHead) could reach 2^115.5, and
+// the largest be 2^-113; times 2^kSpread that becomes 2^126.5 and 2^-102, so that
+// no weight overflows and none is lost that is above 2^-24 of the largest.  The
+// value's factor takes 2^kSpread back, and the sum is held times kSumScale (2^20 weights fit), what
 // 1 / sum has to be multiplied by kSumBack for.
 constexpr int kSpread = 11;
 constexpr float kSumScale = 0x1p-20f, kSumBack = 0x1p-9f;
