@@ -26,6 +26,8 @@ from .fp8 import (Fp8Gemm, Fp8GroupedGemmView, Fp8Matrix, Fp8Scaling, HostFp8Mat
                   fp8_grouped_gemm_q, fp8_grouped_gemm_view, quantize_fp8)
 from .speculative import (TREE_MAX_NODES, Kv8Cache, kv8_append, kv8_keep, kv8_read, tree_attention,
                           tree_attention_workspace_bytes, tree_verify)
+from .paged import (PagedCache, PageMap, PageTables, page_extend, page_truncate, paged_append, paged_attention,
+                    paged_attention_workspace_bytes, sample)
 from .checkpoint import (Checkpoint, CheckpointError, Fp8Config, HostBf16Weight, ModelOptConfig, Quantization,
                          SafetensorsFile, WeightFormat, check_companions, load_experts, load_weight, stack_weights,
                          verify_formats)

@@ -201,6 +201,14 @@ SIGNATURES: dict[str, tuple] = {
     "fpb_tree_attn": (i32, [vp, i32, sz, sz, vp, vp, vp, vp, vp, vp, vp, sz, sz, sz, sz, sz, sz, sz, sz, C.c_float, vp,
                             sz, vp, vp]),
     "fpb_tree_verify": (i32, [vp, i32, sz, vp, sz, vp, vp, vp, vp, sz, sz, sz, sz, C.c_float, vp, vp, vp, vp]),
+    "fpb_page_extend": (i32, [vp, sz, sz, sz, vp, vp, vp, vp, sz, sz, sz, i32, vp, vp, vp, vp, vp]),
+    "fpb_page_truncate": (i32, [vp, sz, sz, sz, vp, vp, vp, vp, sz, sz, vp]),
+    "fpb_paged_append": (i32, [vp, sz, sz, vp, sz, vp, sz, i32, vp, vp, vp, vp, sz, sz, sz, sz, sz, C.c_float, C.c_float,
+                               vp, i32, vp, vp, i32, sz, sz, sz, sz, sz, vp]),
+    "fpb_paged_attn_workspace_bytes": (sz, [sz, sz, sz, sz]),
+    "fpb_paged_attn": (i32, [vp, i32, sz, sz, vp, vp, i32, sz, sz, sz, sz, sz, vp, sz, sz, vp, vp, sz, sz, sz, sz, sz,
+                             sz, C.c_float, vp, sz, vp, i32, vp]),
+    "fpb_sample": (i32, [vp, i32, sz, vp, vp, vp, vp, vp, sz, sz, sz, vp, vp, vp]),
     "fpb_comm_available": (i32, []),
     "fpb_comm_version": (i32, [C.POINTER(i32)]),
     "fpb_comm_unique_id": (i32, [vp]),

@@ -1,10 +1,13 @@
 // The 8-bit key/value cache of speculative decoding: the step that norms,
 // rotates and quantises new tokens into it, its read-back, and the move of an
-// accepted path's rows.  The formats are in kv8.cuh.
+// accepted path's rows; and the same step into the paged cache.  The formats are
+// in kv8.cuh and paged.cuh.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kv8.cuh"
+#include "paged.cuh"
 
 namespace fpb {
 namespace {
@@ -21,6 +24,9 @@ struct AppendArgs {
   void *q_out;
   int q_out_bf16;
   uint8_t *k_codes, *v_codes, *k_exp, *v_exp;
+  void *k_pages, *v_pages;  // the paged cache instead, with a slot and a position a row
+  const int32_t *slots;
+  PageShape page;
   int *error;
   uint64_t turn[kMaxHalf];  // theta^(-i / half) / (2 pi) of a turn, in units of 2^-64
 };
@@ -64,6 +70,16 @@ struct Eight {
   }
 };
 
+// Eight values to eight consecutive elements (16-byte aligned).
+__device__ __forceinline__ void store8(__nv_bfloat16 *p, const float (&y)[8]) {
+  *reinterpret_cast<uint4 *>(p) =
+      make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+}
+__device__ __forceinline__ void store8(float *p, const float (&y)[8]) {
+  reinterpret_cast<float4 *>(p)[0] = make_float4(y[0], y[1], y[2], y[3]);
+  reinterpret_cast<float4 *>(p)[1] = make_float4(y[4], y[5], y[6], y[7]);
+}
+
 // Two values -> two e4m3 codes (RNE, satfinite; NaN stays NaN), a in the low byte.
 __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
   uint16_t out;
@@ -82,7 +98,8 @@ __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
 //          numbers, and reduced before it is rounded to f32: an f32 product
 //          is off by position * 2^-24 radians, 0.002 at position 32768.
 //          The token's cosines and sines are made once for its heads.
-//  write   q' as given, k' and v as codes and exponents at row position + n
+//  write   q' as given, k' and v as codes and exponents at row position + n, or
+//          (C float or bfloat16) as elements of the pages at the row's slot
 // A decode step is bound by latency (loads of the positions, then sines: 3.5 us
 // for 8 x 1 x 20 heads x 256), a prompt by instructions and their latency: 2 x
 // 4096 x 48 heads x 128, bf16, takes 48 us for 185 MB (3.9 TB/s).  Sixteen
@@ -90,13 +107,14 @@ __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
 // instructions for either (71 us), and partners in one lane need no shuffles.
 // Blocks of four warps, seven an SM (of eight warps 56 us; eight an SM 50, fewer
 // than seven 49).
-template <typename T, int LG>
+template <typename T, int LG, typename C>
 __global__ void __launch_bounds__(kAppendThreads, 7) kv8_append_kernel(const __grid_constant__ AppendArgs a) {
   pdl_enter();
+  constexpr bool kCodes = std::is_same<C, uint8_t>::value;
   __shared__ float2 turn_s[kMaxSpan][kMaxHalf];  // cosine, sine
   __shared__ float xs[kAppendThreads / LG][LG * 16];
   __shared__ int depth_s[kMaxSpan], pos_s[kMaxSpan];
-  __shared__ size_t to_s[kMaxSpan];  // the rows' places in the cache, in rows
+  __shared__ size_t to_s[kMaxSpan];  // the rows' places in the cache, in rows (of pages: in elements)
   const int tid = threadIdx.x, lane = tid % LG, item = tid / LG;
   constexpr int kItems = kAppendThreads / LG;
   const int row0 = blockIdx.x * a.span, span = min(a.span, a.rows - row0);
@@ -125,17 +143,31 @@ __global__ void __launch_bounds__(kAppendThreads, 7) kv8_append_kernel(const __g
   }
   ask(rl, h);
   if (tid < span) {
-    const int row = row0 + tid, b = row / a.nodes, n = row - b * a.nodes, pos = a.positions[b];
-    bool bad = false;
-    int depth = tree_depth(a.parents ? a.parents + (size_t)b * a.nodes : nullptr, n, &bad);
-    if (bad && a.error) atomicCAS(a.error, 0, kErrParent);
-    if (depth >= 0 && (pos < 0 || pos >= a.max_seq - n)) {
-      if (a.error) atomicCAS(a.error, 0, kErrPosition);
-      depth = -1;
+    const int row = row0 + tid;
+    int depth, pos;
+    if constexpr (kCodes) {
+      const int b = row / a.nodes, n = row - b * a.nodes;
+      pos = a.positions[b];
+      bool bad = false;
+      depth = tree_depth(a.parents ? a.parents + (size_t)b * a.nodes : nullptr, n, &bad);
+      if (bad && a.error) atomicCAS(a.error, 0, kErrParent);
+      if (depth >= 0 && (pos < 0 || pos >= a.max_seq - n)) {
+        if (a.error) atomicCAS(a.error, 0, kErrPosition);
+        depth = -1;
+      }
+      to_s[tid] = (size_t)b * a.max_seq + pos + n;
+    } else {
+      const int slot = a.slots[row], page = slot / a.page.page_size;
+      pos = a.positions[row];
+      depth = slot < 0 ? -1 : 0;
+      if (depth == 0 && (page >= a.page.pages || pos < 0)) {
+        if (a.error) atomicCAS(a.error, 0, pos < 0 ? kErrPosition : kErrPage);
+        depth = -1;
+      }
+      to_s[tid] = page * a.page.page_pitch + (slot - page * a.page.page_size) * a.page.row_pitch;
     }
     depth_s[tid] = depth;
     pos_s[tid] = pos;
-    to_s[tid] = (size_t)b * a.max_seq + pos + n;
   }
   __syncthreads();
   if (half > 0) {
@@ -228,29 +260,29 @@ __global__ void __launch_bounds__(kAppendThreads, 7) kv8_append_kernel(const __g
       __syncwarp();
     }
     float amax = 0.0f;
+    if constexpr (kCodes) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[j][i]));
+        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[j][i]));
 #pragma unroll
-    for (int o = LG / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      for (int o = LG / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    }
     if (!live) continue;
     if (is_q) {
       const size_t head = (row * a.q_heads + here) * D;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const size_t o = head + col[j];
-        const float *y = x[j];
-        if (a.q_out_bf16) {
-          *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(a.q_out) + o) =
-              make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
-                         pack_bf16x2(y[6], y[7]));
-        } else {
-          float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(a.q_out) + o);
-          dst[0] = make_float4(y[0], y[1], y[2], y[3]);
-          dst[1] = make_float4(y[4], y[5], y[6], y[7]);
-        }
+        if (a.q_out_bf16)
+          store8(static_cast<__nv_bfloat16 *>(a.q_out) + head + col[j], x[j]);
+        else
+          store8(static_cast<float *>(a.q_out) + head + col[j], x[j]);
       }
+    } else if (depth >= 0 && !kCodes) {
+      C *to = static_cast<C *>(is_k ? a.k_pages : a.v_pages) + to_s[at] + kvh * a.page.head_pitch;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if constexpr (!kCodes) store8(to + col[j], x[j]);
     } else if (depth >= 0) {
       const int e = kv8_exponent(amax);
       const float inv = pow2i(-e);
@@ -373,7 +405,50 @@ int check_cache(const char *name, const void *kc, const void *vc, const void *ke
   return FPB_OK;
 }
 
-template <typename T>
+// The projections' part of an append's arguments, checked.
+int append_args(const char *name, AppendArgs &a, const void *q, size_t q_pitch, size_t q_head_pitch, const void *k,
+                size_t k_pitch, const void *v, size_t v_pitch, int dtype, const float *q_gamma, const float *k_gamma,
+                const int32_t *positions, size_t rows, size_t q_heads, size_t kv_heads, size_t head_dim,
+                size_t rotary_dim, float theta, float eps, void *q_out, int q_out_dtype) {
+  if (rotary_dim % 2 || rotary_dim > head_dim || (rotary_dim && !(theta >= 1.0f && std::isfinite(theta))))
+    return fail(FPB_ERR_SHAPE, "%s: rotary_dim %zu (even, at most head_dim), theta %g (at least 1)", name, rotary_dim,
+                (double)theta);
+  if (k_pitch < kv_heads * head_dim || v_pitch < kv_heads * head_dim || (q && q_head_pitch < head_dim))
+    return fail(FPB_ERR_SHAPE, "%s: pitch", name);
+  const size_t el = dtype == FPB_F32 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % el ||
+      (q && !aligned16(q_out)) || (q_gamma && !aligned16(q_gamma)) || (k_gamma && !aligned16(k_gamma)))
+    return fail(FPB_ERR_INVALID_ARGUMENT, "%s: alignment (q_out and the gammas: 16 bytes)", name);
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_pitch = (long long)q_pitch;
+  a.q_head = (long long)q_head_pitch;
+  a.k_pitch = (long long)k_pitch;
+  a.v_pitch = (long long)v_pitch;
+  a.q_gamma = q_gamma;
+  a.k_gamma = k_gamma;
+  a.positions = positions;
+  a.rows = (int)rows;
+  a.q_heads = (int)q_heads;
+  a.kv_heads = (int)kv_heads;
+  a.head_dim = (int)head_dim;
+  a.rotary_dim = (int)rotary_dim;
+  a.vec = aligned16(q) && aligned16(k) && aligned16(v) && (q_pitch | q_head_pitch | k_pitch | v_pitch) * el % 16 == 0;
+  a.inv_d = 1.0f / (float)head_dim;
+  a.eps = eps;
+  a.q_out = q_out;
+  a.q_out_bf16 = q_out_dtype == FPB_BF16;
+  a.error = device_error_ptr();
+  const int half = (int)rotary_dim / 2;
+  // theta^(-i / half) by products of 64-bit mantissas: off by i * 2^-63 of itself at most
+  const long double ratio = half ? powl((long double)theta, -1.0L / half) : 0.0L;
+  long double turn = 0x1p64L / (2.0L * M_PIl);
+  for (int i = 0; i < half; ++i, turn *= ratio) a.turn[i] = (uint64_t)turn;
+  return FPB_OK;
+}
+
+template <typename T, typename C>
 int run_append(AppendArgs a, size_t rows, cudaStream_t s) {
   const int lanes = a.head_dim / 16;
   const int lg = lanes <= 4 ? 4 : lanes <= 8 ? 8 : 16;
@@ -388,9 +463,9 @@ int run_append(AppendArgs a, size_t rows, cudaStream_t s) {
   a.span = rows >= (size_t)sm_count() * 16 ? kMaxSpan : 1;
   const size_t want = std::min<size_t>(parts, std::max<size_t>(1, (size_t)sm_count() * 8 / rows));
   const dim3 grid((unsigned)((rows + a.span - 1) / a.span), (unsigned)want);
-  cudaError_t e = lg == 4   ? launch_pdl(kv8_append_kernel<T, 4>, grid, kAppendThreads, 0, s, a)
-                  : lg == 8 ? launch_pdl(kv8_append_kernel<T, 8>, grid, kAppendThreads, 0, s, a)
-                            : launch_pdl(kv8_append_kernel<T, 16>, grid, kAppendThreads, 0, s, a);
+  cudaError_t e = lg == 4   ? launch_pdl(kv8_append_kernel<T, 4, C>, grid, kAppendThreads, 0, s, a)
+                  : lg == 8 ? launch_pdl(kv8_append_kernel<T, 8, C>, grid, kAppendThreads, 0, s, a)
+                            : launch_pdl(kv8_append_kernel<T, 16, C>, grid, kAppendThreads, 0, s, a);
   if (e != cudaSuccess) return cuda_fail(e, "kv8_append_kernel");
   FPB_LAUNCH_CHECK("kv8_append_kernel");
   return FPB_OK;
@@ -416,51 +491,54 @@ extern "C" int fpb_kv8_append(const void *q, size_t q_pitch, size_t q_head_pitch
   if (nodes == 0 || nodes > max_seq || batch * nodes > 0x7fffffff || q_heads > 65535 ||
       (parents && nodes > (size_t)kTreeMaxNodes))
     return fail(FPB_ERR_SHAPE, "fpb_kv8_append: nodes %zu (a tree has at most %d)", nodes, kTreeMaxNodes);
-  if (rotary_dim % 2 || rotary_dim > head_dim || (rotary_dim && !(theta >= 1.0f && std::isfinite(theta))))
-    return fail(FPB_ERR_SHAPE, "fpb_kv8_append: rotary_dim %zu (even, at most head_dim), theta %g (at least 1)",
-                rotary_dim, (double)theta);
-  if (k_pitch < kv_heads * head_dim || v_pitch < kv_heads * head_dim || (q && q_head_pitch < head_dim))
-    return fail(FPB_ERR_SHAPE, "fpb_kv8_append: pitch");
-  const size_t el = dtype == FPB_F32 ? 4 : 2;
-  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % el ||
-      (q && !aligned16(q_out)) || (q_gamma && !aligned16(q_gamma)) || (k_gamma && !aligned16(k_gamma)))
-    return fail(FPB_ERR_INVALID_ARGUMENT, "fpb_kv8_append: alignment (q_out and the gammas: 16 bytes)");
   AppendArgs a{};
-  a.q = q;
-  a.k = k;
-  a.v = v;
-  a.q_pitch = (long long)q_pitch;
-  a.q_head = (long long)q_head_pitch;
-  a.k_pitch = (long long)k_pitch;
-  a.v_pitch = (long long)v_pitch;
-  a.q_gamma = q_gamma;
-  a.k_gamma = k_gamma;
-  a.positions = positions;
+  if (int st = append_args("fpb_kv8_append", a, q, q_pitch, q_head_pitch, k, k_pitch, v, v_pitch, dtype, q_gamma,
+                           k_gamma, positions, batch * nodes, q_heads, kv_heads, head_dim, rotary_dim, theta, eps,
+                           q_out, q_out_dtype))
+    return st;
   a.parents = parents;
-  a.rows = (int)(batch * nodes);
   a.nodes = (int)nodes;
-  a.q_heads = (int)q_heads;
-  a.kv_heads = (int)kv_heads;
-  a.head_dim = (int)head_dim;
-  a.rotary_dim = (int)rotary_dim;
   a.max_seq = (int)max_seq;
-  a.vec = aligned16(q) && aligned16(k) && aligned16(v) && (q_pitch | q_head_pitch | k_pitch | v_pitch) * el % 16 == 0;
-  a.inv_d = 1.0f / (float)head_dim;
-  a.eps = eps;
-  a.q_out = q_out;
-  a.q_out_bf16 = q_out_dtype == FPB_BF16;
   a.k_codes = k_codes;
   a.v_codes = v_codes;
   a.k_exp = k_exp;
   a.v_exp = v_exp;
-  a.error = device_error_ptr();
-  const int half = (int)rotary_dim / 2;
-  // theta^(-i / half) by products of 64-bit mantissas: off by i * 2^-63 of itself at most
-  const long double ratio = half ? powl((long double)theta, -1.0L / half) : 0.0L;
-  long double turn = 0x1p64L / (2.0L * M_PIl);
-  for (int i = 0; i < half; ++i, turn *= ratio) a.turn[i] = (uint64_t)turn;
   cudaStream_t s = as_stream(stream);
-  return dtype == FPB_F32 ? run_append<float>(a, batch * nodes, s) : run_append<__nv_bfloat16>(a, batch * nodes, s);
+  return dtype == FPB_F32 ? run_append<float, uint8_t>(a, batch * nodes, s)
+                          : run_append<__nv_bfloat16, uint8_t>(a, batch * nodes, s);
+}
+
+extern "C" int fpb_paged_append(const void *q, size_t q_pitch, size_t q_head_pitch, const void *k, size_t k_pitch,
+                                const void *v, size_t v_pitch, int dtype, const float *q_gamma, const float *k_gamma,
+                                const int32_t *slots, const int32_t *positions, size_t rows, size_t q_heads,
+                                size_t kv_heads, size_t head_dim, size_t rotary_dim, float theta, float eps,
+                                void *q_out, int q_out_dtype, void *k_pages, void *v_pages, int page_dtype,
+                                size_t pages, size_t page_size, size_t page_pitch, size_t row_pitch,
+                                size_t head_pitch, void *stream) {
+  if (!k || !v || !slots || !positions || (q_heads != 0) != (q != nullptr) || (q != nullptr) != (q_out != nullptr))
+    return fail(FPB_ERR_INVALID_ARGUMENT, "fpb_paged_append: null pointer (q, q_out and q_heads go together)");
+  if (int st = check_pages("fpb_paged_append", k_pages, v_pages, page_dtype, pages, page_size, page_pitch, row_pitch,
+                           head_pitch, kv_heads, head_dim))
+    return st;
+  if ((dtype != FPB_F32 && dtype != FPB_BF16) || (q && q_out_dtype != FPB_F32 && q_out_dtype != FPB_BF16))
+    return fail(FPB_ERR_INVALID_ARGUMENT, "fpb_paged_append: dtype");
+  if (rows == 0 || rows > 0x7fffffff || q_heads > 65535)
+    return fail(FPB_ERR_SHAPE, "fpb_paged_append: %zu rows, %zu query heads", rows, q_heads);
+  AppendArgs a{};
+  if (int st = append_args("fpb_paged_append", a, q, q_pitch, q_head_pitch, k, k_pitch, v, v_pitch, dtype, q_gamma,
+                           k_gamma, positions, rows, q_heads, kv_heads, head_dim, rotary_dim, theta, eps, q_out,
+                           q_out_dtype))
+    return st;
+  a.nodes = 1;
+  a.slots = slots;
+  a.k_pages = k_pages;
+  a.v_pages = v_pages;
+  a.page = PageShape{(int)pages, (int)page_size, (long long)page_pitch, (long long)row_pitch, (long long)head_pitch};
+  cudaStream_t s = as_stream(stream);
+  if (page_dtype == FPB_F32)
+    return dtype == FPB_F32 ? run_append<float, float>(a, rows, s) : run_append<__nv_bfloat16, float>(a, rows, s);
+  return dtype == FPB_F32 ? run_append<float, __nv_bfloat16>(a, rows, s)
+                          : run_append<__nv_bfloat16, __nv_bfloat16>(a, rows, s);
 }
 
 extern "C" int fpb_kv8_read(const uint8_t *k_codes, const uint8_t *v_codes, const uint8_t *k_exp,

@@ -1,0 +1,313 @@
+// The paged cache's book-keeping on the device: block tables and slot maps from
+// the requests' lengths, and pages given back.  paged.cuh has the layout.
+//
+// The free pages are a stack, free[0, n).  With the requests' new pages counted
+// through in order of request and page (an exclusive prefix sum over requests),
+// the i-th takes free[n - 1 - i].  Giving back puts the i-th of them at free[n + F
+// - 1 - i], F their number, so that what a step took and gave back leaves the
+// stack as it was.
+#include <algorithm>
+#include <mutex>
+#include <vector>
+
+#include "paged.cuh"
+
+namespace fpb {
+namespace {
+
+constexpr int kPageThreads = 1024, kPageWarps = kPageThreads / 32, kPageCluster = 8, kPageMaxBatch = 16384;
+
+struct PageArgs {
+  int32_t *table, *lengths, *free, *free_count;
+  const int32_t *change;  // new tokens, or new lengths
+  long long pitch;        // elements between the table's rows
+  int batch, max_pages, pages, page_size;
+  int rows, width, vec;  // width: rows a request where they are padded, 0 where they are packed
+  int32_t *slots, *positions, *requests, *starts;
+  int *error;
+};
+
+__device__ __forceinline__ void page_error(const PageArgs &a, int code) {
+  if (a.error) atomicCAS(a.error, 0, code);
+}
+
+__device__ __forceinline__ int pages_of(int tokens, int page_size) {
+  return tokens / page_size + (tokens % page_size != 0);
+}
+
+// Sum of the values before this thread's, and of all of them in *total; the
+// whole block calls this.
+__device__ __forceinline__ long long before(long long v, long long *total, long long *sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // the sums of the call before are read
+  if (lane == 31) sums[warp] = x;
+  __syncthreads();
+  long long s = lane < kPageWarps ? sums[lane] : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += y;
+  }
+  *total = __shfl_sync(0xffffffffu, s, 31);
+  const long long mine = __shfl_sync(0xffffffffu, s, warp == 0 ? 0 : warp - 1);
+  return x - v + (warp == 0 ? 0 : mine);
+}
+
+// The last i in [0, n) with at[i] <= x (at[0] <= x).
+__device__ __forceinline__ int last_at(const int *at, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (at[mid] <= x)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// One cluster: each CTA scans all requests for itself, then they share the rows
+// and the new pages.  A request is served whole (its rows fit, its table and the
+// pool have the pages) or not at all.
+__global__ void __launch_bounds__(kPageThreads) page_extend_kernel(const __grid_constant__ PageArgs a) {
+  pdl_enter();
+  extern __shared__ int page_sm[];
+  int *row0 = page_sm, *off = row0 + a.batch + 1, *len = off + a.batch + 1;  // len -1: not served
+  __shared__ long long sums[kPageWarps];
+  __shared__ int used_s;
+  const int tid = threadIdx.x, rank = (int)cluster_ctarank(), ctas = (int)cluster_nctarank();
+  if (tid == 0) used_s = 0;
+  int free_n = *a.free_count;
+  if (free_n < 0 || free_n > a.pages) {
+    if (tid == 0) page_error(a, kErrLength);
+    free_n = 0;
+  }
+  const long long most = (long long)a.max_pages * a.page_size;
+  long long rows_before = 0, pages_before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kPageThreads) {
+    const int b = b0 + tid;
+    const bool in = b < a.batch;
+    const int n = in ? a.lengths[b] : 0, c = in ? a.change[b] : 0;
+    const bool bad = n < 0 || c < 0 || n > most;
+    if (bad) page_error(a, kErrLength);
+    const long long count = max(c, 0);
+    long long total, first;
+    if (a.width) {
+      first = (long long)b * a.width;
+      total = 0;
+    } else {
+      first = rows_before + before(count, &total, sums);
+    }
+    bool served = in && !bad && n + count <= most && (a.width ? count <= a.width : first + count <= a.rows);
+    const long long need = served ? pages_of(n + (int)count, a.page_size) - pages_of(n, a.page_size) : 0;
+    long long taken;
+    const long long at = pages_before + before(need, &taken, sums);
+    served = served && (need == 0 || at + need <= free_n);
+    if (served && need > 0) atomicMax(&used_s, (int)(at + need));
+    if (in) {
+      row0[b] = (int)min(first, (long long)a.rows);
+      off[b] = (int)min(at, (long long)free_n);
+      len[b] = served ? n : -1;
+    }
+    rows_before += total;
+    pages_before += taken;
+  }
+  // (a request that is not served for want of pages keeps its place in the sum:
+  // those after it that need any are not served either, so the pages used are the
+  // stack's first ones)
+  if (tid == 0) {
+    row0[a.batch] = a.width ? a.rows : (int)min(rows_before, (long long)a.rows);
+    off[a.batch] = (int)min(pages_before, (long long)free_n);
+  }
+  cluster_sync();  // every CTA has read the state
+  const int used = used_s;
+  if (rank == 0) {
+    for (int b = tid; b < a.batch; b += kPageThreads)
+      if (len[b] >= 0) a.lengths[b] = len[b] + a.change[b];
+    if (a.starts)
+      for (int b = tid; b <= a.batch; b += kPageThreads) a.starts[b] = row0[b];
+    if (tid == 0 && used > 0) *a.free_count = free_n - used;
+  }
+  const int threads = ctas * kPageThreads, me = rank * kPageThreads + tid;
+  for (int i = me; i < used; i += threads) {
+    const int b = last_at(off, a.batch, i);
+    const int page = a.free[free_n - 1 - i];
+    if (page < 0 || page >= a.pages) page_error(a, kErrPage);
+    a.table[b * a.pitch + pages_of(len[b], a.page_size) + i - off[b]] = page;
+  }
+  // four rows a thread
+  for (int r0 = me * 4; r0 < a.rows; r0 += threads * 4) {
+    int slot[4], pos[4], req[4];
+    int b = a.width ? r0 / a.width : last_at(row0, a.batch, r0);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = r0 + k;
+      slot[k] = pos[k] = req[k] = -1;
+      if (r >= a.rows) break;
+      while (b + 1 < a.batch && row0[b + 1] <= r) ++b;
+      const int i = r - row0[b], n = len[b];
+      if (n < 0 || i >= (a.width ? a.change[b] : row0[b + 1] - row0[b])) continue;
+      const int t = n + i, p = t / a.page_size, held = pages_of(n, a.page_size);
+      const int page = p < held ? a.table[b * a.pitch + p] : a.free[free_n - 1 - (off[b] + p - held)];
+      pos[k] = t;
+      req[k] = b;
+      if (page < 0 || page >= a.pages)
+        page_error(a, kErrPage);
+      else
+        slot[k] = page * a.page_size + t - p * a.page_size;
+    }
+    if (a.vec && r0 + 4 <= a.rows) {
+      *reinterpret_cast<int4 *>(a.slots + r0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+      *reinterpret_cast<int4 *>(a.positions + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+      if (a.requests) *reinterpret_cast<int4 *>(a.requests + r0) = make_int4(req[0], req[1], req[2], req[3]);
+    } else {
+      for (int k = 0; k < 4 && r0 + k < a.rows; ++k) {
+        a.slots[r0 + k] = slot[k];
+        a.positions[r0 + k] = pos[k];
+        if (a.requests) a.requests[r0 + k] = req[k];
+      }
+    }
+  }
+}
+
+// Likewise: each CTA scans the requests, all share the pages.
+__global__ void __launch_bounds__(kPageThreads) page_truncate_kernel(const __grid_constant__ PageArgs a) {
+  pdl_enter();
+  extern __shared__ int page_sm[];
+  int *off = page_sm, *kept = off + a.batch + 1;  // kept: pages that the request keeps
+  __shared__ long long sums[kPageWarps];
+  const int tid = threadIdx.x, rank = (int)cluster_ctarank(), ctas = (int)cluster_nctarank();
+  const int free_n = *a.free_count;
+  const long long most = (long long)a.max_pages * a.page_size;
+  long long back = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kPageThreads) {
+    const int b = b0 + tid;
+    const bool in = b < a.batch;
+    const int n = in ? a.lengths[b] : 0, to = in ? a.change[b] : -1;
+    const bool bad = n < 0 || n > most, cut = !bad && to >= 0 && to < n;
+    if (bad) page_error(a, kErrLength);
+    const int keeps = cut ? pages_of(to, a.page_size) : 0;
+    const long long given = cut ? pages_of(n, a.page_size) - keeps : 0;
+    long long total;
+    const long long at = back + before(given, &total, sums);
+    if (in) {
+      off[b] = (int)min(at, (long long)a.pages);
+      kept[b] = cut ? keeps : -1;
+    }
+    back += total;
+  }
+  if (tid == 0) off[a.batch] = (int)min(back, (long long)a.pages);
+  cluster_sync();  // every CTA has read the state
+  if (free_n < 0 || back > a.pages - free_n) {  // more than the pool can have: nothing is taken back
+    if (tid == 0) page_error(a, kErrLength);
+    return;
+  }
+  if (rank == 0) {
+    for (int b = tid; b < a.batch; b += kPageThreads)
+      if (kept[b] >= 0) a.lengths[b] = a.change[b];
+    if (tid == 0 && back > 0) *a.free_count = free_n + (int)back;
+  }
+  for (int i = rank * kPageThreads + tid; i < (int)back; i += ctas * kPageThreads) {
+    const int b = last_at(off, a.batch, i);
+    int32_t *entry = a.table + b * a.pitch + kept[b] + i - off[b];
+    const int page = *entry;
+    if (page < 0 || page >= a.pages) page_error(a, kErrPage);
+    a.free[free_n + (int)back - 1 - i] = page;
+    *entry = -1;
+  }
+}
+
+int check_tables(const char *name, const PageArgs &a, size_t table_pitch, size_t batch, size_t max_pages,
+                 size_t pages, size_t page_size) {
+  if (!a.table || !a.lengths || !a.change || !a.free || !a.free_count)
+    return fail(FPB_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
+  if (batch == 0 || batch > (size_t)kPageMaxBatch || max_pages == 0 || pages == 0 || page_size == 0 ||
+      pages > 0x7fffffffu / page_size || max_pages > 0x7fffffffu / page_size || table_pitch < max_pages ||
+      table_pitch >> 38)
+    return fail(FPB_ERR_SHAPE, "%s: batch %zu (at most %d), tables of %zu pages (pitch %zu), pool of %zu x %zu rows "
+                "(both fewer than 2^31 rows)", name, batch, kPageMaxBatch, max_pages, table_pitch, pages, page_size);
+  return FPB_OK;
+}
+
+// One cluster; one CTA where a step has few rows and pages.
+int launch_pages(void (*kernel)(PageArgs), const char *name, const PageArgs &a, size_t work, size_t smem,
+                 cudaStream_t s) {
+  {
+    static std::mutex mu;
+    static std::vector<int> done;
+    int dev = 0;
+    FPB_CUDA_TRY(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lock(mu);
+    if (std::find(done.begin(), done.end(), dev) == done.end()) {
+      for (auto k : {page_extend_kernel, page_truncate_kernel})
+        FPB_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          (int)(3 * (kPageMaxBatch + 1) * sizeof(int))));
+      done.push_back(dev);
+    }
+  }
+  const unsigned ctas = work > 4 * kPageThreads ? kPageCluster : 1;
+  cudaError_t e = launch_pdl_cluster(kernel, ctas, kPageThreads, smem, s, ctas, a);
+  if (e != cudaSuccess) return cuda_fail(e, name);
+  FPB_LAUNCH_CHECK(name);
+  return FPB_OK;
+}
+
+PageArgs page_args(int32_t *table, size_t table_pitch, size_t batch, size_t max_pages, int32_t *lengths,
+                   const int32_t *change, int32_t *free_pages, int32_t *free_count, size_t pages, size_t page_size) {
+  PageArgs a{};
+  a.table = table;
+  a.pitch = (long long)table_pitch;
+  a.batch = (int)batch;
+  a.max_pages = (int)max_pages;
+  a.lengths = lengths;
+  a.change = change;
+  a.free = free_pages;
+  a.free_count = free_count;
+  a.pages = (int)pages;
+  a.page_size = (int)page_size;
+  return a;
+}
+
+}  // namespace
+}  // namespace fpb
+
+using namespace fpb;
+
+extern "C" int fpb_page_extend(int32_t *table, size_t table_pitch, size_t batch, size_t max_pages, int32_t *lengths,
+                               const int32_t *counts, int32_t *free_pages, int32_t *free_count, size_t pages,
+                               size_t page_size, size_t rows, int padded, int32_t *slots, int32_t *positions,
+                               int32_t *requests, int32_t *starts, void *stream) {
+  PageArgs a = page_args(table, table_pitch, batch, max_pages, lengths, counts, free_pages, free_count, pages,
+                         page_size);
+  if (int st = check_tables("fpb_page_extend", a, table_pitch, batch, max_pages, pages, page_size)) return st;
+  if (!slots || !positions) return fail(FPB_ERR_INVALID_ARGUMENT, "fpb_page_extend: null pointer");
+  if (rows == 0 || rows > 0x7ffffff0 || (padded && rows % batch))
+    return fail(FPB_ERR_SHAPE, "fpb_page_extend: %zu rows (padded: a multiple of the batch, %zu)", rows, batch);
+  a.rows = (int)rows;
+  a.width = padded ? (int)(rows / batch) : 0;
+  a.slots = slots;
+  a.positions = positions;
+  a.requests = requests;
+  a.starts = starts;
+  a.vec = aligned_to(slots, 16) && aligned_to(positions, 16) && aligned_to(requests, 16);
+  a.error = device_error_ptr();
+  return launch_pages(page_extend_kernel, "page_extend_kernel", a, rows, 3 * (batch + 1) * sizeof(int),
+                      as_stream(stream));
+}
+
+extern "C" int fpb_page_truncate(int32_t *table, size_t table_pitch, size_t batch, size_t max_pages, int32_t *lengths,
+                                 const int32_t *new_lengths, int32_t *free_pages, int32_t *free_count, size_t pages,
+                                 size_t page_size, void *stream) {
+  PageArgs a = page_args(table, table_pitch, batch, max_pages, lengths, new_lengths, free_pages, free_count, pages,
+                         page_size);
+  if (int st = check_tables("fpb_page_truncate", a, table_pitch, batch, max_pages, pages, page_size)) return st;
+  a.error = device_error_ptr();
+  return launch_pages(page_truncate_kernel, "page_truncate_kernel", a, std::min(batch * max_pages, pages),
+                      2 * (batch + 1) * sizeof(int), as_stream(stream));
+}

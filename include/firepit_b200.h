@@ -831,6 +831,86 @@ int fpb_tree_verify(const void *logits, int logits_dtype, size_t logits_pitch, c
                     size_t noise_pitch, size_t batch, size_t nodes, size_t vocab, float temperature, int32_t *path,
                     int32_t *count, int32_t *next, void *stream);
 
+/* ---- serving over a paged key/value cache --------------------------------------
+ * No reference counterpart (each of its sessions owns a contiguous f32 cache and
+ * decodes greedily, attention.rs:6-30, generation.rs:34-42).  Requests of any
+ * length share a pool of pages.
+ *
+ * Pages: k_pages, v_pages [pages, page_size, kv_heads, head_dim] f32 or bf16, with
+ * pitches in elements between pages, rows and heads (the same for both; a multiple
+ * of 16 bytes, as the addresses are; head_dim contiguous, a multiple of 16 up to
+ * 256), so that the pages may also be laid out heads first, or with keys and
+ * values in one allocation.  pages * page_size below 2^31; any page_size (the
+ * attention reads whole tiles where it is a multiple of 16).
+ * Table: table [batch rows of table_pitch, max_pages] int32; token t of request b
+ * lies in row t % page_size of page table[b][t / page_size]; its slot is page *
+ * page_size + row.  A request of n tokens holds its table's first ceil(n /
+ * page_size) entries.  Pool: free_pages [pages] int32, a stack of the *free_count
+ * pages that nobody holds.
+ * Device errors (fpb_device_error): 502 a negative position at a slot, 503 a wait
+ * inside a kernel ran out (the results are not to be used), 506 a slot or an entry
+ * of the table or the pool outside the pages (nothing is read or written there),
+ * 507 a length, count or pool size out of range (such a request counts as absent). */
+/* The requests take pages for counts[b] further tokens, in order of request: new
+ * entries of the table, lengths += counts, and the stack's top goes down.  A
+ * request is served whole or not at all: one whose tokens the pool, its table or
+ * the rows cannot hold keeps its length (and once the pool falls short, so do the
+ * requests after it that need pages).
+ * Each new token has a row: rows follow one another in order of request (packed;
+ * rows of requests that are not served stay in their place), or (padded) request b
+ * has rows [b, b + 1) * rows / batch.  slots, positions, requests [rows]: the
+ * token's slot, its position and its request, -1 in rows without one; starts [batch
+ * + 1]: each request's first row.  requests and starts may be NULL.  batch at most
+ * 16384.  One launch. */
+int fpb_page_extend(int32_t *table, size_t table_pitch, size_t batch, size_t max_pages, int32_t *lengths,
+                    const int32_t *counts, int32_t *free_pages, int32_t *free_count, size_t pages, size_t page_size,
+                    size_t rows, int padded, int32_t *slots, int32_t *positions, int32_t *requests, int32_t *starts,
+                    void *stream);
+/* Cuts requests to new_lengths[b] tokens (negative, or not below the present
+ * length: as it was; 0: done) and gives the pages back, so that what fpb_page_extend
+ * took and this gives back leaves the stack as it was.  Entries given back become -1. */
+int fpb_page_truncate(int32_t *table, size_t table_pitch, size_t batch, size_t max_pages, int32_t *lengths,
+                      const int32_t *new_lengths, int32_t *free_pages, int32_t *free_count, size_t pages,
+                      size_t page_size, void *stream);
+/* fpb_kv8_append's norms and rotation, row r by positions[r], with k and v written
+ * at slots[r] in the pages' type.  Rows of a negative slot hold no token: nothing
+ * is written for them and their q_out is zeros.  No two rows may have one slot. */
+int fpb_paged_append(const void *q, size_t q_pitch, size_t q_head_pitch, const void *k, size_t k_pitch, const void *v,
+                     size_t v_pitch, int dtype, const float *q_gamma, const float *k_gamma, const int32_t *slots,
+                     const int32_t *positions, size_t rows, size_t q_heads, size_t kv_heads, size_t head_dim,
+                     size_t rotary_dim, float theta, float eps, void *q_out, int q_out_dtype, void *k_pages,
+                     void *v_pages, int page_dtype, size_t pages, size_t page_size, size_t page_pitch,
+                     size_t row_pitch, size_t head_pitch, void *stream);
+/* Attention of one token a session over the first lengths[b] tokens of its pages:
+ * q [batch rows of q_pitch, q_heads of q_head_pitch] f32 or bf16, query head h reads
+ * kv head h / (q_heads / kv_heads); out [batch, q_heads * head_dim] f32 or bf16 =
+ * softmax(scale q . k) v, times sigmoid(gate) where gate [batch rows of gate_pitch,
+ * heads of gate_head_pitch] f32 is given.  A session of length 0 gets zeros.  Rows
+ * behind its last token never reach an output, whatever they hold; a token whose
+ * page is outside the pool counts as not there.  batch at most 16384. */
+size_t fpb_paged_attn_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads, size_t head_dim);
+int fpb_paged_attn(const void *q, int q_dtype, size_t q_pitch, size_t q_head_pitch, const void *k_pages,
+                   const void *v_pages, int page_dtype, size_t pages, size_t page_size, size_t page_pitch,
+                   size_t row_pitch, size_t head_pitch, const int32_t *table, size_t table_pitch, size_t max_pages,
+                   const int32_t *lengths, const float *gate, size_t gate_pitch, size_t gate_head_pitch, size_t batch,
+                   size_t q_heads, size_t kv_heads, size_t head_dim, float scale, void *workspace,
+                   size_t workspace_bytes, void *out, int out_dtype, void *stream);
+/* The next tokens [batch] from logits [batch rows of logits_pitch, vocab] (f32 or
+ * bf16; non-finite ones count as -inf).  With w = exp((l - max l) / T) a row's
+ * tokens are ordered by logit, falling, ties by index, and each filter keeps a first
+ * part of that order: top_k the first k (0 or below: all), top_p the shortest part
+ * whose weights reach p of what top_k kept (1 or above: all; at least one token),
+ * min_p those with w >= min_p (0 or below: all; above 1: as 1).  The token is
+ * argmax w / noise over what is kept (noise [batch rows of noise_pitch, vocab] f32,
+ * exponential variates, positive), which draws from w; ties go to the lowest index.
+ * temperature [batch] (NULL: 1; held within [1e-6, 1e6]): 0 or below takes the first
+ * token; top_k, top_p, min_p [batch] (NULL: none).  A row without a finite logit
+ * gives -1.  logprobs [batch] (NULL: not wanted): the log of the token's weight among
+ * what is kept (greedy: 0).  vocab up to 442368. */
+int fpb_sample(const void *logits, int logits_dtype, size_t logits_pitch, const float *temperature,
+               const int32_t *top_k, const float *top_p, const float *min_p, const float *noise, size_t noise_pitch,
+               size_t batch, size_t vocab, int32_t *tokens, float *logprobs, void *stream);
+
 /* ---- collectives (NCCL) ------------------------------------------------------
  * The reference runs on one GPU and has no collectives.  These are the
  * exchange steps of the multi-GPU paths: the all-gather of each rank's output
