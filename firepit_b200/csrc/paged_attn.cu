@@ -4,88 +4,805 @@
 //   out = sum_t softmax(s)_t v_t, times sigmoid(gate) where a gate is given.
 #include <algorithm>
 #include <cmath>
+#include <mutex>
+#include <vector>
 
 #include "paged.cuh"
+#include "sm100.cuh"
+#include "tma_host.cuh"
 
 namespace fpb {
 namespace {
 
+using namespace sm100;
+
 struct PagedArgs {
-  const void *q, *k, *v;
+  const void *q;
   const float *gate;
   const int32_t *table, *lengths;
   long long q_pitch, q_head, gate_pitch, gate_head, table_pitch;  // elements
-  PageShape page;
-  int batch, q_heads, kv_heads, group, head_dim, max_pages, q_bf16;
+  int batch, q_heads, kv_heads, group, head_dim, max_pages, pages, page_size, q_bf16, q_vec;
+  int box;     // tokens of a copy: the largest power of two that divides the page size, up to a step's
+  int tiles;   // row tiles of a kv head's query heads
+  int slots;   // blocks that the GPU has room for
+  int waves;   // 0: as many blocks as there is room for; else shares of 1 / (waves * slots) of the steps, and the rest
   float scale_log2;  // scale * log2(e): scores and maxima are held in powers of two
   void *out;
   int out_bf16;
+  float *part;      // [slot][row][head_dim] numerators
+  float2 *part_ml;  // [slot][row] maximum, sum
+  int2 *shares;     // [session, kv head, row tile] first slot, number of slots (1: nothing to merge)
   int *error;
 };
 
-template <typename T>
-__device__ __forceinline__ float value(const T *p, size_t i) {
-  if constexpr (sizeof(T) == 4)
-    return p[i];
-  else
-    return __bfloat162float(p[i]);
+constexpr int kPagedThreads = 128, kPagedWarps = 4, kPagedMaxBatch = 4096, kPagedWaves = 4;
+constexpr int kErrPagedWait = 503;
+// The maximum may lag by kLag (powers of two) before the sums are rescaled, and
+// weights are held as 2^(y - m - kBack): 2^20 of them times a value of the type's
+// largest then stay within f32, and weights down to 2^-98 of the largest count.
+constexpr float kLag = 8.0f, kBack = 28.0f;
+
+__device__ __forceinline__ float pow2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// One warp a query head: the tokens one by one, the maximum and sum running.
-template <typename T>
-__global__ void __launch_bounds__(128) paged_attn_kernel(const __grid_constant__ PagedArgs a) {
-  pdl_enter();
-  const int lane = threadIdx.x & 31, item = blockIdx.x * 4 + (threadIdx.x >> 5), D = a.head_dim;
-  if (item >= a.batch * a.q_heads) return;
-  const int b = item / a.q_heads, h = item % a.q_heads, kvh = h / a.group;
-  int n = a.lengths[b];
-  const long long most = (long long)a.max_pages * a.page.page_size;
-  if (n < 0 || n > most) {
-    if (lane == 0 && a.error) atomicCAS(a.error, 0, kErrLength);
-    n = 0;
-  }
-  float q[8], acc[8], m = -INFINITY, l = 0.0f;
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Four 8 x 8 matrices of bf16, transposed; lane 8 i + r holds the address of row r of matrix i.
+__device__ __forceinline__ void load_transposed(uint32_t (&x)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+               : "r"(addr)
+               : "memory");
+}
+
+// An 8 x 8 matrix of 16-bit pairs (lane 4 r + c: row r, columns 2 c and 2 c + 1), transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// (lo, hi) as bf16 pairs, and what the rounding left of them.
+__device__ __forceinline__ uint32_t split_bf16x2(float lo, float hi, uint32_t *rest) {
+  const uint32_t x = pack_bf16x2(lo, hi);
+  *rest = pack_bf16x2(lo - __uint_as_float(x << 16), hi - __uint_as_float(x & 0xffff0000u));
+  return x;
+}
+
+__device__ __forceinline__ float load_q(const PagedArgs &a, int b, int h, int d) {
+  const size_t at = (size_t)b * a.q_pitch + (size_t)h * a.q_head + d;
+  return a.q_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(a.q)[at]) : static_cast<const float *>(a.q)[at];
+}
+
+// Eight elements of a query from column d on (a multiple of 8); zeros where `there` is false.
+__device__ __forceinline__ void load_q8(const PagedArgs &a, int b, int h, int d, bool there, float (&x)[8]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int d = lane + 32 * i;
-    const size_t at = (size_t)b * a.q_pitch + (size_t)h * a.q_head + d;
-    q[i] = d < D ? (a.q_bf16 ? value(static_cast<const __nv_bfloat16 *>(a.q), at) : value(static_cast<const float *>(a.q), at))
-                 : 0.0f;
-    acc[i] = 0.0f;
-  }
-  for (int t = 0; t < n; ++t) {
-    const int p = t / a.page.page_size, page = a.table[b * a.table_pitch + p];
-    if (page < 0 || page >= a.page.pages) {
-      if (lane == 0 && a.error) atomicCAS(a.error, 0, kErrPage);
-      continue;
+  for (int k = 0; k < 8; ++k) x[k] = 0.0f;
+  if (!there) return;
+  const size_t at = (size_t)b * a.q_pitch + (size_t)h * a.q_head + d;
+  if (!a.q_vec) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = load_q(a, b, h, d + k);
+  } else if (a.q_bf16) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) + at);
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      x[2 * k] = __uint_as_float(u[k] << 16);
+      x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
     }
-    const size_t at = page * a.page.page_pitch + (t - p * a.page.page_size) * a.page.row_pitch + kvh * a.page.head_pitch;
-    float s = 0.0f;
+  } else {
+    const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at);
+    const float4 u = p[0], v = p[1];
+    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+    x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+  }
+}
+
+// N columns of head h from d on: the numerators x over the sum l, gated.  No token:
+// zeros.
+template <int N>
+__device__ __forceinline__ void store_out(const PagedArgs &a, int b, int h, int d, const float (&x)[N], float l) {
+  const size_t at = ((size_t)b * a.q_heads + h) * a.head_dim + d;
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  float o[N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < D) s = fmaf(q[i], value(static_cast<const T *>(a.k), at + lane + 32 * i), s);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    s *= a.scale_log2;
-    const float mn = fmaxf(m, s), old = m == -INFINITY ? 0.0f : exp2f(m - mn), w = exp2f(s - (mn == -INFINITY ? 0.0f : mn));
-    m = mn;
-    l = fmaf(l, old, w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < D) acc[i] = fmaf(acc[i], old, w * value(static_cast<const T *>(a.v), at + lane + 32 * i));
+  for (int k = 0; k < N; ++k) {
+    o[k] = l != 0.0f ? x[k] * inv : 0.0f;
+    if (a.gate && l != 0.0f) o[k] /= 1.0f + expf(-a.gate[(size_t)b * a.gate_pitch + (size_t)h * a.gate_head + d + k]);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int d = lane + 32 * i;
-    if (d >= D) break;
-    float o = l != 0.0f ? acc[i] / l : 0.0f;
-    if (a.gate && n > 0) o /= 1.0f + expf(-a.gate[(size_t)b * a.gate_pitch + (size_t)h * a.gate_head + d]);
-    const size_t at = ((size_t)b * a.q_heads + h) * D + d;
+  for (int k = 0; k < N; k += 2) {
     if (a.out_bf16)
-      static_cast<__nv_bfloat16 *>(a.out)[at] = __float2bfloat16_rn(o);
+      *reinterpret_cast<uint32_t *>(static_cast<__nv_bfloat16 *>(a.out) + at + k) = pack_bf16x2(o[k], o[k + 1]);
     else
-      static_cast<float *>(a.out)[at] = o;
+      *reinterpret_cast<float2 *>(static_cast<float *>(a.out) + at + k) = make_float2(o[k], o[k + 1]);
   }
+}
+
+// Operand row i of eight is token token_at(i) of its eight: a quarter of a warp
+// then reads 16 bytes from all of the banks.
+__device__ __forceinline__ int token_at(int i) { return (i >> 1) | (i & 1) << 2; }
+
+template <typename T, int DP, int NR>
+struct PagedShape {
+  static constexpr bool kHalf = sizeof(T) == 2;
+  static constexpr int kTok = kHalf ? 16 : 8;                       // tokens of a step
+  static constexpr int kCols = 128 / (int)sizeof(T), kBoxes = DP / kCols;  // a copy's columns; copies side by side
+  static constexpr uint32_t kPart = kTok * DP * sizeof(T);          // a step's keys, or its values
+  static constexpr int kBlocks = DP == 256 ? 2 : 3;                 // an SM
+  static constexpr int kParts = (DP == 256 ? 3 : DP == 128 ? 4 : 6) - (NR == 16);  // of a warp's ring
+  static constexpr bool kQShared = NR == 16 && DP >= 128;           // too many registers of queries beside those of sums
+  static constexpr int kQPitch = DP + 32;                           // bf16 elements: 16-byte reads of eight rows on distinct banks
+  static constexpr int kEndPitch = DP + 4;
+  static constexpr size_t kRing = (size_t)kPagedWarps * kParts * kPart;
+  static constexpr size_t kEnd = (size_t)kPagedWarps * NR * kEndPitch * 4;  // the warps' results, over the ring
+  static constexpr size_t kPlan = (size_t)kPagedMaxBatch * 4;               // the sessions' steps, over the ring
+  static constexpr size_t kOver = kRing > kEnd ? kRing : kEnd;
+  static constexpr size_t kQueries = kHalf ? (size_t)2 * NR * kQPitch * 2 : (size_t)kPagedWarps * 64 * 4;
+  static constexpr size_t smem = 1023 + kOver + kQueries;
+  static_assert(kPlan <= kOver && kBlocks * (smem + 3 * 1024) <= 228 * 1024);
+};
+
+// What a block does: steps [first, first + count) of a session's kv head and row tile.
+struct PagedShare {
+  int b, kvh, tile, length, first, count, part, parts, slot;
+};
+
+// The sessions' steps are cut into shares of S, each session's evenly, and the
+// shares numbered in order of session, kv head, part and row tile.  Every block
+// finds its own: false where there is none.  `steps` [batch] in shared memory.
+// One wave: the smallest S whose shares the GPU has room for at once, among 32
+// between total / slots, which is below it, and total / (slots - items), whose
+// shares fit: each item rounds up by less than one.
+template <int TOK>
+__device__ __forceinline__ bool paged_share(const PagedArgs &a, int *steps, PagedShare *out) {
+  __shared__ unsigned long long sum_s[kPagedWarps];
+  __shared__ int alive_s[kPagedWarps], blocks_s[kPagedWarps][32], found_s[4];
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const long long most = (long long)a.max_pages * a.page_size;
+  unsigned long long sum = 0;
+  int alive = 0;
+  for (int b = tid; b < a.batch; b += kPagedThreads) {
+    int n = a.lengths[b];
+    if (n < 0 || n > most) {
+      if (blockIdx.x == 0 && a.error) atomicCAS(a.error, 0, kErrLength);
+      n = 0;
+    }
+    const int s = n / TOK + (n % TOK != 0);
+    steps[b] = s;
+    sum += s;
+    alive += s > 0;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    alive += __shfl_xor_sync(0xffffffffu, alive, o);
+  }
+  if (lane == 0) {
+    sum_s[w] = sum;
+    alive_s[w] = alive;
+  }
+  if (tid == 0) found_s[0] = -1;
+  __syncthreads();
+  sum = 0;
+  alive = 0;
+#pragma unroll
+  for (int i = 0; i < kPagedWarps; ++i) {
+    sum += sum_s[i];
+    alive += alive_s[i];
+  }
+  const int heads = a.kv_heads * a.tiles;
+  const unsigned long long work = sum * heads;
+  if (work == 0) return false;
+  constexpr int kLeast = kPagedWarps;  // a step a warp
+  int S;
+  if (a.waves) {
+    S = (int)min((work + (unsigned long long)a.waves * a.slots - 1) / ((unsigned long long)a.waves * a.slots),
+                 (unsigned long long)0x7fffffff);
+  } else {
+    const int items = alive * heads;
+    const int lo = (int)((work + a.slots - 1) / a.slots), hi = (int)((work + a.slots - items - 1) / (a.slots - items));
+    const int trial = max(kLeast, lo + (int)((long long)(hi - lo) * lane / 31));
+    int n = 0;
+    for (int b = w; b < a.batch; b += kPagedWarps) n += (steps[b] + trial - 1) / trial;
+    blocks_s[w][lane] = n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < kPagedWarps; ++i) n += blocks_s[i][lane];
+    const uint32_t fits = __ballot_sync(0xffffffffu, n * heads <= a.slots);
+    S = __shfl_sync(0xffffffffu, trial, __ffs(fits) - 1);
+  }
+  S = max(S, kLeast);
+  // the session of this block, and the slots of split sessions before it
+  int blocks0 = 0, slots0 = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kPagedThreads) {
+    const int b = b0 + tid, n = b < a.batch ? (steps[b] + S - 1) / S : 0;
+    int blocks = n * heads, slots = n > 1 ? blocks : 0, x = blocks, y = slots;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) {
+        x += u;
+        y += v;
+      }
+    }
+    __syncthreads();  // (the words below are read)
+    if (lane == 31) {
+      blocks_s[w][0] = x;
+      blocks_s[w][1] = y;
+    }
+    __syncthreads();
+    int before = blocks0, slots_before = slots0;
+#pragma unroll
+    for (int i = 0; i < kPagedWarps; ++i) {
+      if (i < w) {
+        before += blocks_s[i][0];
+        slots_before += blocks_s[i][1];
+      }
+      blocks0 += blocks_s[i][0];
+      slots0 += blocks_s[i][1];
+    }
+    before += x - blocks;
+    slots_before += y - slots;
+    if ((int)blockIdx.x >= before && (int)blockIdx.x < before + blocks) {
+      found_s[0] = b;
+      found_s[1] = before;
+      found_s[2] = slots_before;
+      found_s[3] = n;
+    }
+    __syncthreads();
+    if (found_s[0] >= 0 || (int)blockIdx.x < blocks0) break;
+  }
+  const int b = found_s[0];
+  if (b < 0) return false;
+  const int n = found_s[3], at = (int)blockIdx.x - found_s[1], tile = at % a.tiles, part = at / a.tiles % n;
+  out->b = b;
+  out->tile = tile;
+  out->part = part;
+  out->parts = n;
+  out->kvh = at / a.tiles / n;
+  out->length = a.lengths[b];
+  const int total = steps[b];
+  out->first = (int)((long long)total * part / n);
+  out->count = (int)((long long)total * (part + 1) / n) - out->first;
+  out->slot = found_s[2] + (out->kvh * a.tiles + tile) * n + part;
+  __syncthreads();  // `steps` is read
+  return true;
+}
+
+template <typename T, int DP, int NR>
+__global__ void __launch_bounds__(kPagedThreads, (PagedShape<T, DP, NR>::kBlocks))
+    paged_attn_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ CUtensorMap k_map,
+                      const __grid_constant__ CUtensorMap v_map) {
+  using Sh = PagedShape<T, DP, NR>;
+  constexpr int kTok = Sh::kTok, kParts = Sh::kParts, kNT = NR / 8;
+  extern __shared__ uint8_t raw_sm[];
+  uint8_t *const ring = raw_sm + (-smem_u32(raw_sm) & 1023);  // the swizzle goes by the address
+  float *const sm = reinterpret_cast<float *>(ring);          // at the end: the warps' results
+  __shared__ uint64_t full[kPagedWarps][kParts];
+  __shared__ int abort_s;
+  __shared__ float m_s[kPagedWarps][NR], l_s[kPagedWarps][NR];
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, D = a.head_dim;
+  if (lane == 0) {
+    for (int i = 0; i < kParts; ++i) mbar_init(&full[w][i], 1);
+    if (w == 0) abort_s = 0;
+    fence_barrier_init();
+  }
+  __syncwarp();
+  pdl_enter();
+  PagedShare me;
+  if (!paged_share<kTok>(a, reinterpret_cast<int *>(ring), &me)) return;
+  fence_proxy_async_smem();  // the plan's words lie where the first copies go
+  __syncthreads();
+  if (tid == 0 && me.part == 0)
+    a.shares[(size_t)(me.b * a.kv_heads + me.kvh) * a.tiles + me.tile] = make_int2(me.slot, me.parts);
+
+  // A warp takes steps w, w + 4, ... of the share; part 2 i of its ring's sequence
+  // is its i-th step's keys, part 2 i + 1 its values.
+  const int count = w < me.count ? (me.count - w + kPagedWarps - 1) / kPagedWarps : 0;
+  uint8_t *const mine = ring + (size_t)w * kParts * Sh::kPart;
+  const int boxes = kTok / a.box;  // copies of a step one below another: lane i's begins at token i * box
+  const int32_t *const table = a.table + me.b * a.table_pitch;
+  auto token0 = [&](int i) { return (me.first + w + i * kPagedWarps) * kTok; };
+  auto look_up = [&](int i) {  // the page of the lane's copy in step i
+    const int t = token0(i) + lane * a.box;
+    return lane < boxes && i < count && t < me.length ? table[t / a.page_size] : -1;
+  };
+  int page = -1, next_page = look_up(0);
+  bool wrong = false;  // a page outside the pool was met
+  auto fetch = [&](int j) {
+    const int i = j >> 1, t = token0(i) + lane * a.box;
+    if (!(j & 1)) {
+      page = next_page;
+      next_page = look_up(i + 1);
+    }
+    const bool there = lane < boxes && t < me.length, good = there && page >= 0 && page < a.pages;
+    const uint32_t all = __ballot_sync(0xffffffffu, good);
+    if (__any_sync(0xffffffffu, there && !good)) {
+      wrong = true;
+      if (lane == 0 && a.error) atomicCAS(a.error, 0, kErrPage);
+    }
+    uint64_t *bar = &full[w][j % kParts];
+    if (lane == 0) mbar_arrive_expect_tx(bar, __popc(all) * a.box * 128 * Sh::kBoxes);
+    __syncwarp();
+    if (good) {
+      uint8_t *to = mine + (j % kParts) * Sh::kPart + lane * a.box * 128;
+      const CUtensorMap *map = j & 1 ? &v_map : &k_map;
+      const int row = t % a.page_size;
+#pragma unroll
+      for (int x = 0; x < Sh::kBoxes; ++x)
+        tma_load_4d(to + x * (kTok * 128), map, x * Sh::kCols, me.kvh, row, page, bar);
+    }
+    __syncwarp();
+  };
+  for (int j = 0; j < min(2 * count, kParts); ++j) fetch(j);
+
+  const int head0 = me.kvh * a.group + me.tile * NR, rows = min(NR, a.group - me.tile * NR);
+  bool ok = true;
+  auto wait = [&](int j) {
+    if (ok) ok = mbar_wait(&full[w][j % kParts], (j / kParts) & 1, &abort_s);
+    if (!ok) {  // (a wait that ran out: the results are void, but the loop ends)
+      *(volatile int *)&abort_s = 1;
+      if (a.error) atomicCAS(a.error, 0, kErrPagedWait);
+    }
+    __syncwarp();
+    ok = __all_sync(0xffffffffu, ok);
+  };
+  int asked = min(2 * count, kParts);
+  auto done = [&](int j) {  // part j is read: its place takes a later one
+    __syncwarp();
+    if (ok && j + kParts < 2 * count) {
+      fetch(j + kParts);
+      asked = j + kParts + 1;
+    }
+  };
+  // whether token t of the session is one, with its page in the pool
+  auto token_there = [&](int t) {
+    if (t >= me.length) return false;
+    if (!wrong) return true;
+    const int p = table[t / a.page_size];
+    return p >= 0 && p < a.pages;
+  };
+  // tokens of a step that are not there: their values become zeros, since a
+  // weight of 0 does not hide a NaN
+  auto clear_values = [&](uint8_t *part, int t0) {
+    for (int r = 0; r < kTok; ++r) {
+      if (token_there(t0 + r)) continue;
+      for (int i = lane; i < Sh::kBoxes * 8; i += 32)
+        *reinterpret_cast<uint4 *>(part + (i >> 3) * (kTok * 128) + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+    }
+    fence_proxy_async_smem();  // (the next copy into it comes behind these)
+    __syncwarp();
+  };
+
+  // copies still in flight land before their memory is used otherwise
+  auto finish = [&]() {
+    if (!ok)
+      for (int j = max(0, asked - kParts); j < asked; ++j) {
+        int never = 0;
+        mbar_wait(&full[w][j % kParts], (j / kParts) & 1, &never);
+      }
+    __syncthreads();
+  };
+
+  if constexpr (Sh::kHalf) {
+    const int g = lane >> 2, c = lane & 3, own = token_at(g);
+    __nv_bfloat16 *const qs = reinterpret_cast<__nv_bfloat16 *>(ring + Sh::kOver);  // [high, low][row][kQPitch]
+    constexpr int kPieces = DP / 32, kMT = DP / 16, kMine = NR / kPagedWarps, kChains = NR == 8 ? 4 : 2;
+    const bool low = !a.q_bf16;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int r = w + i * kPagedWarps, col = lane * 8;
+      float x[8];
+      load_q8(a, me.b, head0 + r, col, r < rows && col < D, x);
+      if (col < DP) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) hi[k] = split_bf16x2(x[2 * k], x[2 * k + 1], &lo[k]);
+        *reinterpret_cast<uint4 *>(qs + r * Sh::kQPitch + col) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4 *>(qs + (NR + r) * Sh::kQPitch + col) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+    }
+    __syncthreads();
+    // Q operands of piece p: row g (+ 8 i)'s dimensions 32 p + 8 c + [0, 8)
+    auto query = [&](int part, int i, int p) {
+      return *reinterpret_cast<const uint4 *>(qs + (part * NR + g + 8 * i) * Sh::kQPitch + 32 * p + 8 * c);
+    };
+    uint4 qr[Sh::kQShared ? 1 : 2 * kNT * kPieces];
+    if constexpr (!Sh::kQShared) {
+#pragma unroll
+      for (int part = 0; part < 2; ++part)
+#pragma unroll
+        for (int i = 0; i < kNT; ++i)
+#pragma unroll
+          for (int p = 0; p < kPieces; ++p) qr[(part * kNT + i) * kPieces + p] = query(part, i, p);
+    }
+    float acc[kMT][kNT][4], m[kNT][2], l[kNT][2];
+#pragma unroll
+    for (int i = 0; i < kNT; ++i) {
+#pragma unroll
+      for (int k = 0; k < kMT; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[k][i][e] = 0.0f;
+      m[i][0] = m[i][1] = -INFINITY;
+      l[i][0] = l[i][1] = 0.0f;
+    }
+    for (int at = 0; at < count; ++at) {
+      const int t0 = token0(at);
+      const uint8_t *kst = mine + (2 * at) % kParts * Sh::kPart;
+      wait(2 * at);
+      // scores of 16 tokens: s[i][.][2 h + e] token own + 8 h, row 2 c + e + 8 i, in sums
+      // that do not wait for one another
+      float s[kNT][kChains][4];
+#pragma unroll
+      for (int i = 0; i < kNT; ++i)
+#pragma unroll
+        for (int u = 0; u < kChains; ++u)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s[i][u][k] = 0.0f;
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) {
+        const uint8_t *row = kst + (p >> 1) * (kTok * 128) + own * 128 + ((4 * (p & 1) + c) ^ own) * 16;
+        const uint4 u = *reinterpret_cast<const uint4 *>(row), v = *reinterpret_cast<const uint4 *>(row + 8 * 128);
+#pragma unroll
+        for (int i = 0; i < kNT; ++i) {
+          const uint4 q = Sh::kQShared ? query(0, i, p) : qr[Sh::kQShared ? 0 : i * kPieces + p];
+          mma_bf16(s[i][0], u.x, v.x, u.y, v.y, q.x, q.y);
+          mma_bf16(s[i][1], u.z, v.z, u.w, v.w, q.z, q.w);
+          if (low) {
+            const uint4 r = Sh::kQShared ? query(1, i, p) : qr[Sh::kQShared ? 0 : (kNT + i) * kPieces + p];
+            mma_bf16(s[i][kChains - 2], u.x, v.x, u.y, v.y, r.x, r.y);
+            mma_bf16(s[i][kChains - 1], u.z, v.z, u.w, v.w, r.z, r.w);
+          }
+        }
+      }
+      done(2 * at);
+      const bool open = t0 + kTok > me.length || wrong;
+      float y[kNT][2][2];  // scores: row, token
+      bool grow = false;
+#pragma unroll
+      for (int i = 0; i < kNT; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float x = s[i][0][2 * h + e] + s[i][1][2 * h + e];
+            if (kChains == 4) x += s[i][kChains - 2][2 * h + e] + s[i][kChains - 1][2 * h + e];
+            y[i][e][h] = x * a.scale_log2;
+            if (open && !token_there(t0 + own + 8 * h)) y[i][e][h] = -INFINITY;
+          }
+          grow |= fmaxf(y[i][e][0], y[i][e][1]) > m[i][e] + kLag;
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int i = 0; i < kNT; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mn = fmaxf(m[i][e], fmaxf(y[i][e][0], y[i][e][1]));
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+            const float old = m[i][e] == -INFINITY ? 0.0f : pow2(m[i][e] - mn);
+            l[i][e] *= old;
+            m[i][e] = mn;
+#pragma unroll
+            for (int k = 0; k < kMT; ++k) {
+              acc[k][i][e] *= old;
+              acc[k][i][2 + e] *= old;
+            }
+          }
+      }
+      uint32_t ph[kNT][2], pl[kNT][2];
+#pragma unroll
+      for (int i = 0; i < kNT; ++i) {
+        const float base[2] = {m[i][0] == -INFINITY ? 0.0f : -kBack - m[i][0],
+                               m[i][1] == -INFINITY ? 0.0f : -kBack - m[i][1]};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float p0 = pow2(y[i][0][h] + base[0]), p1 = pow2(y[i][1][h] + base[1]);
+          l[i][0] += p0;
+          l[i][1] += p1;
+          uint32_t rest;
+          const uint32_t x = split_bf16x2(p0, p1, &rest);
+          ph[i][h] = transposed(x);
+          pl[i][h] = transposed(rest);
+        }
+      }
+      uint8_t *vst = mine + (2 * at + 1) % kParts * Sh::kPart;
+      wait(2 * at + 1);
+      if (open) clear_values(vst, t0);
+      const int vrow = token_at(lane & 7), half = (lane >> 3) & 1;
+      const uint32_t v0 = smem_u32(vst) + (vrow + 8 * (lane >> 4)) * 128;
+#pragma unroll
+      for (int k = 0; k < kMT; ++k) {
+        uint32_t x[4];
+        load_transposed(x, v0 + (k >> 2) * (kTok * 128) + ((2 * (k & 3) + half) ^ vrow) * 16);
+#pragma unroll
+        for (int i = 0; i < kNT; ++i) {
+          mma_bf16(acc[k][i], x[0], x[1], x[2], x[3], ph[i][0], ph[i][1]);
+          mma_bf16(acc[k][i], x[0], x[1], x[2], x[3], pl[i][0], pl[i][1]);
+        }
+      }
+      done(2 * at + 1);
+    }
+#pragma unroll
+    for (int i = 0; i < kNT; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], o);
+        if (g == 0) {
+          m_s[w][8 * i + 2 * c + e] = m[i][e];
+          l_s[w][8 * i + 2 * c + e] = l[i][e];
+        }
+      }
+    finish();
+    float *mine_f = sm + (size_t)w * NR * Sh::kEndPitch;
+#pragma unroll
+    for (int k = 0; k < kMT; ++k)
+#pragma unroll
+      for (int i = 0; i < kNT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          mine_f[(8 * i + 2 * c + (e & 1)) * Sh::kEndPitch + 16 * k + g + 8 * (e >> 1)] = acc[k][i][e];
+  } else {
+    constexpr int kPer = DP / 32;  // columns a lane: 2, or fours 128 apart
+    auto column = [&](int j) { return kPer == 2 ? 2 * lane + j : (j >> 2) * 128 + 4 * lane + (j & 3); };
+    float *const ps = reinterpret_cast<float *>(ring + Sh::kOver) + w * 64;  // [token][row] weights
+    const int row = lane & 7, tok = lane >> 3;
+    float q[8][kPer], acc[8][kPer], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        q[r][j] = r < rows && column(j) < D ? load_q(a, me.b, head0 + r, column(j)) : 0.0f;
+        acc[r][j] = 0.0f;
+      }
+    auto load_row = [&](const uint8_t *part, int t, float (&x)[kPer]) {
+#pragma unroll
+      for (int j = 0; j < kPer; j += 4) {
+        const int d = column(j);
+        const uint8_t *p = part + (d >> 5) * (kTok * 128) + t * 128 + ((((d & 31) >> 2) ^ t) * 16);
+        if constexpr (kPer == 2) {
+          const float2 v = *reinterpret_cast<const float2 *>(p + (d & 3) * 4);
+          x[0] = v.x;
+          x[1] = v.y;
+        } else {
+          const float4 v = *reinterpret_cast<const float4 *>(p);
+          x[j] = v.x;
+          x[j + 1] = v.y;
+          x[j + 2] = v.z;
+          x[j + 3] = v.w;
+        }
+      }
+    };
+    for (int at = 0; at < count; ++at) {
+      const int t0 = token0(at);
+      const uint8_t *kst = mine + (2 * at) % kParts * Sh::kPart;
+      wait(2 * at);
+      float y[2];  // scores of tokens tok and tok + 4, the lane's row
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float v[32];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          float x[kPer];
+          load_row(kst, 4 * u + t, x);
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            float s = q[r][0] * x[0];
+#pragma unroll
+            for (int j = 1; j < kPer; ++j) s = fmaf(q[r][j], x[j], s);
+            v[8 * t + r] = s;
+          }
+        }
+        // 32 sums over the warp, one to a lane
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+          for (int i = 0; i < o; ++i) {
+            const float keep = lane & o ? v[i + o] : v[i], send = lane & o ? v[i] : v[i + o];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+          }
+        y[u] = v[0] * a.scale_log2;
+      }
+      done(2 * at);
+      const bool open = t0 + kTok > me.length || wrong;
+      if (open) {
+        if (!token_there(t0 + tok)) y[0] = -INFINITY;
+        if (!token_there(t0 + tok + 4)) y[1] = -INFINITY;
+      }
+      if (__any_sync(0xffffffffu, fmaxf(y[0], y[1]) > m + kLag)) {
+        float mn = fmaxf(m, fmaxf(y[0], y[1]));
+        mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 8));
+        mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 16));
+        const float old = m == -INFINITY ? 0.0f : pow2(m - mn);
+        l *= old;
+        m = mn;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const float f = __shfl_sync(0xffffffffu, old, r);
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) acc[r][j] *= f;
+        }
+      }
+      const float base = m == -INFINITY ? 0.0f : -kBack - m;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float p = pow2(y[u] + base);
+        l += p;
+        ps[(4 * u + tok) * 8 + row] = p;
+      }
+      uint8_t *vst = mine + (2 * at + 1) % kParts * Sh::kPart;
+      wait(2 * at + 1);  // (the warp meets: the weights are there)
+      if (open) clear_values(vst, t0);
+#pragma unroll
+      for (int t = 0; t < kTok; ++t) {
+        float x[kPer];
+        load_row(vst, t, x);
+        const float4 u = *reinterpret_cast<const float4 *>(ps + 8 * t), v = *reinterpret_cast<const float4 *>(ps + 8 * t + 4);
+        const float p[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) acc[r][j] = fmaf(p[r], x[j], acc[r][j]);
+      }
+      done(2 * at + 1);
+    }
+    l += __shfl_xor_sync(0xffffffffu, l, 8);
+    l += __shfl_xor_sync(0xffffffffu, l, 16);
+    if (lane < 8) {
+      m_s[w][lane] = m;
+      l_s[w][lane] = l;
+    }
+    finish();
+    float *mine_f = sm + (size_t)w * NR * Sh::kEndPitch;
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) mine_f[r * Sh::kEndPitch + column(j)] = acc[r][j];
+  }
+  __syncthreads();
+  // the warps' results meet: maxima, then sums over one maximum in warp order
+  for (int r = w; r < rows; r += kPagedWarps) {
+    float top = -INFINITY, f[kPagedWarps], sum = 0.0f;
+#pragma unroll
+    for (int x = 0; x < kPagedWarps; ++x) top = fmaxf(top, m_s[x][r]);
+#pragma unroll
+    for (int x = 0; x < kPagedWarps; ++x) {
+      f[x] = m_s[x][r] == -INFINITY ? 0.0f : pow2(m_s[x][r] - top);
+      sum = fmaf(l_s[x][r], f[x], sum);
+    }
+    const size_t to = (size_t)me.slot * NR + r;
+    for (int d = lane * 2; d < D; d += 64) {
+      float2 o = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int x = 0; x < kPagedWarps; ++x) {
+        const float2 v = *reinterpret_cast<const float2 *>(sm + ((size_t)x * NR + r) * Sh::kEndPitch + d);
+        o.x = fmaf(v.x, f[x], o.x);
+        o.y = fmaf(v.y, f[x], o.y);
+      }
+      if (me.parts > 1) {
+        *reinterpret_cast<float2 *>(a.part + to * D + d) = o;
+      } else {
+        const float x[2] = {o.x, o.y};
+        store_out<2>(a, me.b, head0 + r, d, x, sum);
+      }
+    }
+    if (me.parts > 1 && lane == 0) a.part_ml[to] = make_float2(top, sum);
+  }
+}
+
+// The shares of a row (session and query head) meet, in order: blockDim.y warps a
+// row and 128 columns share them, four columns a lane.  A session without tokens
+// gets its zeros here.
+constexpr int kMergeWarps = 16;
+__global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __grid_constant__ PagedArgs a, int NR,
+                                                                      int count) {
+  __shared__ float4 acc_s[kMergeWarps][32];
+  __shared__ float l_s[kMergeWarps];
+  const int lane = threadIdx.x, share = threadIdx.y, shares = blockDim.y, w = threadIdx.z * shares + share;
+  const int i = blockIdx.x * blockDim.z + threadIdx.z, d = blockIdx.y * 128 + lane * 4, D = a.head_dim;
+  const bool in = i < count;
+  const int h = in ? i % a.q_heads : 0, b = in ? i / a.q_heads : 0, kvh = h / a.group, in_group = h % a.group;
+  const int tile = in_group / NR, r = in_group % NR;
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int n = a.lengths[b];
+  const bool none = n <= 0 || n > (long long)a.max_pages * a.page_size;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  int2 mine = make_int2(0, 0);
+  if (in && !none) mine = a.shares[(size_t)(b * a.kv_heads + kvh) * a.tiles + tile];
+  const int parts = mine.y > 1 ? mine.y : 0;
+  const float2 *ml = a.part_ml + (size_t)mine.x * NR + r;
+  float top = -INFINITY, l = 0.0f;
+  for (int s = lane; s < parts; s += 32) top = fmaxf(top, ml[(size_t)s * NR].x);
+  top = warp_max(top);
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto add = [&](float4 x, float f) {
+    acc.x = fmaf(x.x, f, acc.x);
+    acc.y = fmaf(x.y, f, acc.y);
+    acc.z = fmaf(x.z, f, acc.z);
+    acc.w = fmaf(x.w, f, acc.w);
+  };
+  const float *part = a.part + ((size_t)mine.x * NR + r) * D + (d < D ? d : 0);
+#pragma unroll 4
+  for (int s = share; s < parts; s += shares) {
+    const float2 v = ml[(size_t)s * NR];
+    const float4 x = *reinterpret_cast<const float4 *>(part + (size_t)s * NR * D);
+    const float f = v.x == -INFINITY ? 0.0f : pow2(v.x - top);
+    l = fmaf(v.y, f, l);
+    add(x, f);
+  }
+  if (shares > 1) {
+    if (share > 0) {
+      acc_s[w][lane] = acc;
+      if (lane == 0) l_s[w] = l;
+    }
+    __syncthreads();
+    if (share > 0) return;
+    for (int k = w + 1; k < w + shares; ++k) {
+      add(acc_s[k][lane], 1.0f);
+      l += l_s[k];
+    }
+  }
+  if (!in || d >= D || mine.y == 1) return;
+  const float x[4] = {acc.x, acc.y, acc.z, acc.w};
+  store_out<4>(a, b, h, d, x, l);
+}
+
+// How a call is cut.
+struct Plan {
+  int rows, tiles, slots, waves;
+  size_t blocks, parts;
+};
+
+template <typename T, int DP, int NR>
+int run_paged(const PagedArgs &a, const Plan &p, const CUtensorMap &k_map, const CUtensorMap &v_map, cudaStream_t s) {
+  using Sh = PagedShape<T, DP, NR>;
+  {
+    static std::mutex mu;
+    static std::vector<int> done;
+    int dev = 0;
+    FPB_CUDA_TRY(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lock(mu);
+    if (std::find(done.begin(), done.end(), dev) == done.end()) {
+      FPB_CUDA_TRY(cudaFuncSetAttribute(paged_attn_kernel<T, DP, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)Sh::smem));
+      done.push_back(dev);
+    }
+  }
+  cudaError_t e = launch_pdl(paged_attn_kernel<T, DP, NR>, (unsigned)p.blocks, kPagedThreads, Sh::smem, s, a, k_map, v_map);
+  if (e != cudaSuccess) return cuda_fail(e, "paged_attn_kernel");
+  FPB_LAUNCH_CHECK("paged_attn_kernel");
+  return FPB_OK;
+}
+
+Plan plan_for(size_t batch, size_t q_heads, size_t kv_heads, size_t head_dim, bool f32) {
+  Plan p{};
+  const size_t group = q_heads / kv_heads;
+  p.rows = group <= 8 || f32 ? 8 : 16;
+  p.tiles = (int)((group + p.rows - 1) / p.rows);
+  p.slots = sm_count() * (head_dim > 128 ? 2 : 3);
+  const size_t items = batch * kv_heads * p.tiles;
+  p.waves = 2 * items <= (size_t)p.slots ? 0 : kPagedWaves;
+  // an item that is cut has more than S steps, so at most twice its steps / S shares
+  p.blocks = p.waves ? (size_t)p.waves * p.slots + items : p.slots;
+  p.parts = p.waves ? (size_t)2 * p.waves * p.slots : p.slots;
+  return p;
+}
+
+size_t workspace_for(const Plan &p, size_t batch, size_t kv_heads, size_t head_dim) {
+  return p.parts * p.rows * (head_dim + 2) * sizeof(float) + batch * kv_heads * p.tiles * sizeof(int2);
 }
 
 }  // namespace
@@ -94,8 +811,10 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const __grid_constant__
 using namespace fpb;
 
 extern "C" size_t fpb_paged_attn_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads, size_t head_dim) {
-  (void)batch; (void)q_heads; (void)kv_heads; (void)head_dim;
-  return 16;
+  if (batch == 0 || kv_heads == 0 || q_heads == 0 || q_heads % kv_heads) return 16;
+  const size_t a = workspace_for(plan_for(batch, q_heads, kv_heads, head_dim, false), batch, kv_heads, head_dim),
+               b = workspace_for(plan_for(batch, q_heads, kv_heads, head_dim, true), batch, kv_heads, head_dim);
+  return std::max(a, b);
 }
 
 extern "C" int fpb_paged_attn(const void *q, int q_dtype, size_t q_pitch, size_t q_head_pitch, const void *k_pages,
@@ -112,10 +831,10 @@ extern "C" int fpb_paged_attn(const void *q, int q_dtype, size_t q_pitch, size_t
   if (int st = check_pages("fpb_paged_attn", k_pages, v_pages, page_dtype, pages, page_size, page_pitch, row_pitch,
                            head_pitch, kv_heads, head_dim))
     return st;
-  if (batch == 0 || batch > 16384 || q_heads == 0 || q_heads % kv_heads || q_heads > 65535 || max_pages == 0 ||
+  if (batch == 0 || batch > (size_t)kPagedMaxBatch || q_heads == 0 || q_heads % kv_heads || q_heads > 65535 || max_pages == 0 ||
       max_pages > 0x7fffffffu / page_size || table_pitch < max_pages || table_pitch >> 38)
-    return fail(FPB_ERR_SHAPE, "fpb_paged_attn: batch %zu (at most 16384), heads %zu / %zu, tables of %zu pages (pitch "
-                "%zu)", batch, q_heads, kv_heads, max_pages, table_pitch);
+    return fail(FPB_ERR_SHAPE, "fpb_paged_attn: batch %zu (at most %d), heads %zu / %zu, tables of %zu pages (pitch "
+                "%zu)", batch, kPagedMaxBatch, q_heads, kv_heads, max_pages, table_pitch);
   if (q_head_pitch < head_dim || (gate && gate_head_pitch < head_dim) || !std::isfinite(scale))
     return fail(FPB_ERR_SHAPE, "fpb_paged_attn: pitches or scale");
   if (!aligned_to(workspace, 16) || !aligned_to(out, 16) || !aligned_to(q, q_dtype == FPB_F32 ? 4 : 2) ||
@@ -124,10 +843,11 @@ extern "C" int fpb_paged_attn(const void *q, int q_dtype, size_t q_pitch, size_t
   const size_t need = fpb_paged_attn_workspace_bytes(batch, q_heads, kv_heads, head_dim);
   if (workspace_bytes < need)
     return fail(FPB_ERR_WORKSPACE, "fpb_paged_attn: workspace %zu < %zu bytes", workspace_bytes, need);
+  const bool f32 = page_dtype == FPB_F32;
+  const Plan p = plan_for(batch, q_heads, kv_heads, head_dim, f32);
+  if (p.blocks > 0x7fffffff) return fail(FPB_ERR_SHAPE, "fpb_paged_attn: %zu blocks", p.blocks);
   PagedArgs a{};
   a.q = q;
-  a.k = k_pages;
-  a.v = v_pages;
   a.gate = gate;
   a.table = table;
   a.lengths = lengths;
@@ -136,22 +856,56 @@ extern "C" int fpb_paged_attn(const void *q, int q_dtype, size_t q_pitch, size_t
   a.gate_pitch = (long long)gate_pitch;
   a.gate_head = (long long)gate_head_pitch;
   a.table_pitch = (long long)table_pitch;
-  a.page = PageShape{(int)pages, (int)page_size, (long long)page_pitch, (long long)row_pitch, (long long)head_pitch};
   a.batch = (int)batch;
   a.q_heads = (int)q_heads;
   a.kv_heads = (int)kv_heads;
   a.group = (int)(q_heads / kv_heads);
   a.head_dim = (int)head_dim;
   a.max_pages = (int)max_pages;
+  a.pages = (int)pages;
+  a.page_size = (int)page_size;
   a.q_bf16 = q_dtype == FPB_BF16;
+  a.q_vec = aligned_to(q, 16) && (q_pitch | q_head_pitch) * (a.q_bf16 ? 2 : 4) % 16 == 0;
+  a.box = f32 ? 8 : 16;
+  while (page_size % a.box) a.box /= 2;
+  a.tiles = p.tiles;
+  a.slots = p.slots;
+  a.waves = p.waves;
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
   a.out = out;
   a.out_bf16 = out_dtype == FPB_BF16;
+  a.part = static_cast<float *>(workspace);
+  a.part_ml = reinterpret_cast<float2 *>(a.part + p.parts * p.rows * head_dim);
+  a.shares = reinterpret_cast<int2 *>(a.part_ml + p.parts * p.rows);
   a.error = device_error_ptr();
-  const unsigned blocks = (unsigned)((batch * q_heads + 3) / 4);
-  cudaError_t e = page_dtype == FPB_F32 ? launch_pdl(paged_attn_kernel<float>, blocks, 128, 0, as_stream(stream), a)
-                                        : launch_pdl(paged_attn_kernel<__nv_bfloat16>, blocks, 128, 0, as_stream(stream), a);
-  if (e != cudaSuccess) return cuda_fail(e, "paged_attn_kernel");
-  FPB_LAUNCH_CHECK("paged_attn_kernel");
+  CUtensorMap k_map, v_map;
+  if (int st = encode_pages(&k_map, k_pages, !f32, head_dim, kv_heads, page_size, pages, head_pitch, row_pitch,
+                            page_pitch, (uint32_t)a.box))
+    return st;
+  if (int st = encode_pages(&v_map, v_pages, !f32, head_dim, kv_heads, page_size, pages, head_pitch, row_pitch,
+                            page_pitch, (uint32_t)a.box))
+    return st;
+  cudaStream_t s = as_stream(stream);
+  using bf = __nv_bfloat16;
+  const bool few = p.rows == 8;
+  int st;
+  if (f32)
+    st = head_dim <= 64    ? run_paged<float, 64, 8>(a, p, k_map, v_map, s)
+         : head_dim <= 128 ? run_paged<float, 128, 8>(a, p, k_map, v_map, s)
+                           : run_paged<float, 256, 8>(a, p, k_map, v_map, s);
+  else
+    st = head_dim <= 64    ? (few ? run_paged<bf, 64, 8>(a, p, k_map, v_map, s) : run_paged<bf, 64, 16>(a, p, k_map, v_map, s))
+         : head_dim <= 128 ? (few ? run_paged<bf, 128, 8>(a, p, k_map, v_map, s) : run_paged<bf, 128, 16>(a, p, k_map, v_map, s))
+                           : (few ? run_paged<bf, 256, 8>(a, p, k_map, v_map, s) : run_paged<bf, 256, 16>(a, p, k_map, v_map, s));
+  if (st) return st;
+  const int count = (int)(batch * q_heads);
+  const unsigned halves = head_dim > 128 ? 2 : 1;
+  unsigned shares = 1;  // warps a row: as many as run at once
+  while (shares < (unsigned)kMergeWarps && 2 * shares * halves * (size_t)count <= (size_t)sm_count() * 16) shares *= 2;
+  const unsigned per = std::max(1u, 8 / shares);
+  cudaError_t e = launch_pdl(paged_merge_kernel, dim3((unsigned)((count + per - 1) / per), halves), dim3(32, shares, per),
+                             0, s, a, p.rows, count);
+  if (e != cudaSuccess) return cuda_fail(e, "paged_merge_kernel");
+  FPB_LAUNCH_CHECK("paged_merge_kernel");
   return FPB_OK;
 }
