@@ -10,167 +10,648 @@
 // distributed as w.
 #include <algorithm>
 #include <cmath>
+#include <mutex>
+#include <vector>
 
 #include "common.cuh"
 
 namespace fpb {
 namespace {
 
-constexpr int kSampleThreads = 1024, kSampleWarps = kSampleThreads / 32;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kCluster = 8;
+constexpr int kMaxSlice = 49152;  // f32 of shared memory a CTA: 192 KB
+constexpr int kBatch = 5;         // 16-byte loads a thread has under way
+constexpr int kBins = 256, kPerOctave = 8;  // bins of a histogram: an eighth of a power of two each, the last one the rest
+constexpr int kList = 2048;       // tokens that one CTA orders
 
 struct SampleArgs {
   const void *logits;
   const float *temperature, *top_p, *min_p, *noise;
   const int32_t *top_k;
   long long logits_pitch, noise_pitch;  // elements between rows
-  int vocab;
+  int vocab, slice, vec, noise_vec;     // vec: every slice begins on 16 bytes
   int32_t *tokens;
   float *logprobs;
 };
 
-// Order of f32 values as that of whole numbers (-inf above 0).
+struct Best {
+  float v;
+  int i;
+};
+__device__ __forceinline__ Best better(Best a, Best b) { return b.v > a.v || (b.v == a.v && b.i < a.i) ? b : a; }
+
+__device__ __forceinline__ float pow2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Order of f32 values as that of whole numbers, and back.
 __device__ __forceinline__ uint32_t ordered(float x) {
   const uint32_t u = __float_as_uint(x);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float unordered(uint32_t u) {
+  return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
+}
+
+__device__ __forceinline__ uint32_t peer_address(const void *p, unsigned rank) {
+  const uint32_t local = (uint32_t)__cvta_generic_to_shared(p);
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+  return remote;
+}
+__device__ __forceinline__ void peer_store(const void *p, unsigned rank, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_address(p, rank)), "r"(v) : "memory");
+}
+__device__ __forceinline__ void peer_store(const void *p, unsigned rank, unsigned long long v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer_address(p, rank)), "l"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t peer_load(const uint32_t *p, unsigned rank) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer_address(p, rank)) : "memory");
+  return v;
+}
 
 template <typename V>
-__device__ __forceinline__ V block_sum(V v, V *red) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ V warp_total(V v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if (lane == 0) red[warp] = v;
-  __syncthreads();
-  V t = red[lane];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-  return t;
+  return v;
 }
 
-struct Pick {
-  double v;
-  int i;
+struct Shared {
+  unsigned long long list[kList];  // of the first CTA: tokens to be ordered, (falling logit, index) as one number
+  uint32_t hist[3][kBins];         // tokens; their weights' sum, low and high part
+  uint32_t got[2][4][kCluster];    // what the CTAs tell one another; the halves alternate, so that one exchange's
+                                   // reads may overlap the next one's stores
+  double sums[kWarps];
+  uint32_t counts[kWarps];
+  Best best[kWarps];
+  float pick_x;
+  int border, n_before, n_in;      // where a histogram reaches its target: the bin, tokens before and in it
+  double s_before;
+  int gathered;
+  uint32_t cut_key, cut_index;
 };
 
-__device__ __forceinline__ Pick block_best(Pick x, Pick *red) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto meet = [&]() {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const double v = __shfl_xor_sync(0xffffffffu, x.v, o);
-      const int i = __shfl_xor_sync(0xffffffffu, x.i, o);
-      if (v > x.v || (v == x.v && i < x.i)) x = Pick{v, i};
-    }
-  };
-  meet();
-  __syncthreads();
-  if (lane == 0) red[warp] = x;
-  __syncthreads();
-  x = red[lane];
-  meet();
-  return x;
-}
-
-// One block a row.  What is kept is {key above `key`} and, at `key`, the indices
-// up to `last`; both are found bit by bit, a pass over the row each.
 template <typename T>
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_constant__ SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
+  // every CTA of the cluster runs, before its shared memory is stored to
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   pdl_enter();
-  __shared__ double red[kSampleWarps];
-  __shared__ Pick red_p[kSampleWarps];
-  const int b = blockIdx.x, tid = threadIdx.x;
-  const T *row = static_cast<const T *>(a.logits) + (size_t)b * a.logits_pitch;
-  const float *noise = a.noise + (size_t)b * a.noise_pitch;
-  auto logit = [&](int i) {
-    const float x = static_cast<float>(row[i]);
-    return fabsf(x) <= 3.402823466e38f ? x : -INFINITY;
-  };
-  Pick top{-INFINITY, 0x7fffffff};
-  for (int i = tid; i < a.vocab; i += kSampleThreads) {
-    const float x = logit(i);
-    if (x > top.v) top = Pick{x, i};
-  }
-  top = block_best(top, red_p);
+  extern __shared__ __align__(16) float xs[];  // the slice's logits
+  __shared__ Shared sh;
+  const unsigned rank = cluster_ctarank();
+  const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int v0 = (int)rank * a.slice, len = max(0, min(a.vocab - v0, a.slice)), padded = (len + 3) / 4 * 4;
+  const T *row = static_cast<const T *>(a.logits) + (size_t)b * a.logits_pitch + v0;
+  const float *noise = a.noise + (size_t)b * a.noise_pitch + v0;
   const float t = a.temperature ? a.temperature[b] : 1.0f;
-  if (top.i == 0x7fffffff || !(t > 0.0f)) {
-    if (tid == 0) {
+  const bool greedy = !(t > 0.0f);
+  const int k = a.top_k ? a.top_k[b] : 0;
+  const float p = a.top_p ? a.top_p[b] : 1.0f, m = a.min_p ? a.min_p[b] : 0.0f;
+  const bool by_k = k > 0 && k < a.vocab, by_p = p < 1.0f;
+  const float least = m > 0.0f ? fminf(m, 1.0f) : 0.0f;
+  if (!greedy && !by_k && !by_p && least == 0.0f && a.noise_vec && tid == 0 && len >= 4)  // all of its noise is wanted
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(noise), "r"(len / 4 * 16) : "memory");
+
+  // the slice to shared memory, and its first largest logit
+  Best top{-INFINITY, 0x7fffffff};
+  auto take = [&](float x, int i) {
+    x = fabsf(x) <= 3.402823466e38f ? x : -INFINITY;
+    if (x > top.v) top = Best{x, v0 + i};
+    return x;
+  };
+  {
+    constexpr int N = 16 / sizeof(T);
+    const int whole = a.vec ? len / N * N : 0;
+    for (int i0 = tid * N; i0 < whole; i0 += kBatch * kThreads * N) {
+      uint4 v[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = i0 + j * kThreads * N;
+        v[j] = i < whole ? __ldg(reinterpret_cast<const uint4 *>(row + i)) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = i0 + j * kThreads * N;
+        if (i >= whole) break;
+        const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+        if constexpr (N == 4) {
+          float4 y;
+          y.x = take(__uint_as_float(w[0]), i);
+          y.y = take(__uint_as_float(w[1]), i + 1);
+          y.z = take(__uint_as_float(w[2]), i + 2);
+          y.w = take(__uint_as_float(w[3]), i + 3);
+          *reinterpret_cast<float4 *>(xs + i) = y;
+        } else {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            float4 y;
+            y.x = take(__uint_as_float(w[2 * q] << 16), i + 4 * q);
+            y.y = take(__uint_as_float(w[2 * q] & 0xffff0000u), i + 4 * q + 1);
+            y.z = take(__uint_as_float(w[2 * q + 1] << 16), i + 4 * q + 2);
+            y.w = take(__uint_as_float(w[2 * q + 1] & 0xffff0000u), i + 4 * q + 3);
+            *reinterpret_cast<float4 *>(xs + i + 4 * q) = y;
+          }
+        }
+      }
+    }
+    for (int i = whole + tid; i < padded; i += kThreads) xs[i] = i < len ? take(static_cast<float>(row[i]), i) : -INFINITY;
+  }
+  auto block_best = [&](Best x) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      x = better(x, Best{__shfl_xor_sync(0xffffffffu, x.v, o), __shfl_xor_sync(0xffffffffu, x.i, o)});
+    if (lane == 0) sh.best[warp] = x;
+    __syncthreads();
+    x = sh.best[lane % kWarps];
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1)
+      x = better(x, Best{__shfl_xor_sync(0xffffffffu, x.v, o), __shfl_xor_sync(0xffffffffu, x.i, o)});
+    return x;
+  };
+  auto block_sum = [&](double v) {
+    v = warp_total(v);
+    __syncthreads();  // (the sums before are read)
+    if (lane == 0) sh.sums[warp] = v;
+    __syncthreads();
+    v = sh.sums[lane % kWarps];
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  };
+  int flip = 0;
+  auto tell = [&](uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+    if (tid < kCluster) {
+      peer_store(&sh.got[flip][0][rank], tid, w0);
+      peer_store(&sh.got[flip][1][rank], tid, w1);
+      peer_store(&sh.got[flip][2][rank], tid, w2);
+      peer_store(&sh.got[flip][3][rank], tid, w3);
+    }
+    cluster_sync();
+    flip ^= 1;
+  };
+  auto heard = [&](int word, int from) { return sh.got[flip ^ 1][word][from]; };
+  auto best_of_all = [&]() {
+    Best x{__uint_as_float(heard(0, lane % kCluster)), (int)heard(1, lane % kCluster)};
+#pragma unroll
+    for (int o = kCluster / 2; o > 0; o >>= 1)
+      x = better(x, Best{__shfl_xor_sync(0xffffffffu, x.v, o), __shfl_xor_sync(0xffffffffu, x.i, o)});
+    return x;
+  };
+  top = block_best(top);
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  tell(__float_as_uint(top.v), (uint32_t)top.i, 0, 0);
+  top = best_of_all();
+  if (greedy || top.i == 0x7fffffff) {
+    if (rank == 0 && tid == 0) {
       a.tokens[b] = top.i == 0x7fffffff ? -1 : top.i;
       if (a.logprobs) a.logprobs[b] = top.i == 0x7fffffff ? -INFINITY : 0.0f;
     }
     return;
   }
-  const double inv = 1.0 / (double)fminf(fmaxf(t, 1e-6f), 1e6f), best = top.v;
-  uint32_t key = ordered(-INFINITY);  // (not kept itself)
-  int last = -1;
-  auto weight = [&](float x) { return exp(((double)x - best) * inv); };
-  auto kept = [&](float x, int i) {
-    const uint32_t u = ordered(x);
-    return u > key || (u == key && i <= last);
+  const float temp = fminf(fmaxf(t, 1e-6f), 1e6f), per = 1.4426950408889634f / temp, largest = top.v;
+  auto depth = [&](float x) { return (largest - x) * per; };  // w = 2^-depth
+  // What is kept so far: logits above `cut` (ordered), and those of it up to index
+  // `cut_index`.
+  uint32_t cut = 0, cut_index = 0;
+  auto kept = [&](uint32_t u, int i) { return u > cut || (u == cut && (uint32_t)(v0 + i) <= cut_index); };
+  // f(x, i) for every finite logit of the slice
+  auto for_slice = [&](auto f) {
+    for (int i = tid * 4; i < len; i += kThreads * 4) {
+      const float4 x = *reinterpret_cast<const float4 *>(xs + i);
+      if (x.x > -INFINITY) f(x.x, i);
+      if (x.y > -INFINITY) f(x.y, i + 1);
+      if (x.z > -INFINITY) f(x.z, i + 2);
+      if (x.w > -INFINITY) f(x.w, i + 3);
+    }
   };
-  // Shortens what is kept to the first part whose sum of f reaches `target`.
-  auto cut = [&](double target, auto f) {
-    uint32_t k = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t trial = k | 1u << bit;
-      double s = 0.0;
-      for (int i = tid; i < a.vocab; i += kSampleThreads) {
-        const float x = logit(i);
-        if (ordered(x) >= trial && kept(x, i)) s += f(x);
-      }
-      if (block_sum(s, red) >= target) k = trial;
-    }
-    int lo = 0, hi = a.vocab - 1;  // the first index at which the sum is reached
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      double s = 0.0;
-      for (int i = tid; i < a.vocab; i += kSampleThreads) {
-        const float x = logit(i);
-        const uint32_t u = ordered(x);
-        if ((u > k || (u == k && i <= mid)) && kept(x, i)) s += f(x);
-      }
-      if (block_sum(s, red) >= target)
-        hi = mid;
-      else
-        lo = mid + 1;
-    }
-    key = k;
-    last = lo;
-  };
-  const int k = a.top_k ? a.top_k[b] : 0;
-  if (k > 0 && k < a.vocab) {
-    double n = 0.0;
-    for (int i = tid; i < a.vocab; i += kSampleThreads) n += kept(logit(i), i);
-    if (block_sum(n, red) > k) cut((double)k, [](float) { return 1.0; });
-  }
-  const float p = a.top_p ? a.top_p[b] : 1.0f;
-  if (p < 1.0f) {
-    double s = 0.0;
-    for (int i = tid; i < a.vocab; i += kSampleThreads) {
-      const float x = logit(i);
-      if (kept(x, i)) s += weight(x);
-    }
-    s = block_sum(s, red);
-    cut(fmax((double)p * s, 1e-300), weight);
-  }
-  const float m = a.min_p ? a.min_p[b] : 0.0f;
-  const double floor_w = m > 0.0f ? (double)fminf(m, 1.0f) : 0.0;
-  Pick pick{-INFINITY, 0x7fffffff};
-  double s = 0.0;
-  for (int i = tid; i < a.vocab; i += kSampleThreads) {
-    const float x = logit(i);
-    const double w = weight(x);
-    if (!kept(x, i) || w < floor_w) continue;
-    s += w;
-    const double v = w / (double)noise[i];
-    if (v > pick.v) pick = Pick{v, i};
-  }
-  s = block_sum(s, red);
-  pick = block_best(pick, red_p);
-  if (tid == 0) {
+  // the row's token and its log probability, of weights that sum to s
+  auto answer = [&](Best pick, float x, double s) {
     a.tokens[b] = pick.i;
-    if (a.logprobs) a.logprobs[b] = (float)(((double)logit(pick.i) - best) * inv - log(s));
+    if (a.logprobs) a.logprobs[b] = (float)(((double)x - (double)largest) / (double)temp - log(s));
+  };
+
+  // Weights go to a histogram as whole numbers, relative to the bin's largest, so
+  // that their sum does not depend on the order: 31 bits in two parts of 16 and 15
+  // (49152 of them fit 32 bits).
+  auto count_in = [&](int bin, float u, bool weigh) {
+    atomicAdd(&sh.hist[0][bin], 1u);
+    if (weigh) {
+      const uint32_t f = (uint32_t)__float2uint_rn(u * 0x1p31f);
+      atomicAdd(&sh.hist[1][bin], f & 0xffffu);
+      atomicAdd(&sh.hist[2][bin], f >> 16);
+    }
+  };
+  auto clear_hist = [&]() {
+    for (int i = tid; i < 3 * kBins; i += kThreads) (&sh.hist[0][0])[i] = 0;
+    __syncthreads();
+  };
+  // Over the cluster's histograms (scale(bin): what a bin's weights are relative
+  // to): the first bin at which the running count, or sum, reaches the target, with
+  // what lies before it; `base`: tokens of the CTAs before this one up to and with
+  // that bin, and in it.  sum: all bins'.  Every CTA finds the same.
+  int base_through = 0, base_in = 0;
+  double sum_all = 0.0;
+  auto find_border = [&](bool weigh, double target_share, double extra, double given_target, double n0, double s0,
+                         auto scale) {
+    uint32_t c = 0, below = 0;
+    unsigned long long s = 0;
+    if (tid < kBins) {
+#pragma unroll
+      for (int r = 0; r < kCluster; ++r) {
+        const uint32_t x = peer_load(&sh.hist[0][tid], r);
+        if (r < (int)rank) below += x;
+        c += x;
+        if (weigh) s += peer_load(&sh.hist[1][tid], r) + ((unsigned long long)peer_load(&sh.hist[2][tid], r) << 16);
+      }
+    }
+    double v = weigh && tid < kBins ? (double)s * 0x1p-31 * scale(tid) : 0.0;
+    // running count and sum over the bins
+    uint32_t n = c;
+    double run = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, n, o);
+      const double y = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) {
+        n += x;
+        run += y;
+      }
+    }
+    __syncthreads();
+    if (lane == 31) {
+      sh.counts[warp] = n;
+      sh.sums[warp] = run;
+    }
+    if (tid == 0) sh.border = -1;
+    __syncthreads();
+    double s_at = s0, s_total = 0.0;
+    uint32_t n_at = 0;
+#pragma unroll
+    for (int i = 0; i < kBins / 32; ++i) {
+      if (i < warp) {
+        n_at += sh.counts[i];
+        s_at += sh.sums[i];
+      }
+      s_total += sh.sums[i];
+    }
+    sum_all = s_total + extra;
+    const double target = weigh ? (target_share >= 0.0 ? target_share * sum_all : given_target) : given_target;
+    if (tid < kBins && c > 0) {
+      if ((weigh ? s_at + run : n0 + n_at + n) >= target) atomicMax(&sh.border, kBins - 1 - tid);  // the first of them
+    }
+    __syncthreads();
+    const int border = sh.border < 0 ? -1 : kBins - 1 - sh.border;
+    if (tid == border) {
+      sh.n_before = (int)(n_at + n - c);
+      sh.n_in = (int)c;
+      sh.s_before = s_at + run - v;
+    }
+    // tokens that CTAs before this one have up to the border
+    uint32_t through = tid <= border ? below : 0, in = tid == border ? below : 0;
+    through = warp_total(through);
+    in = warp_total(in);
+    __syncthreads();
+    if (lane == 0) {
+      sh.counts[warp] = through;
+      sh.best[warp].i = (int)in;
+    }
+    if (tid == 0) sh.gathered = 0;
+    __syncthreads();
+    base_through = base_in = 0;
+#pragma unroll
+    for (int i = 0; i < kBins / 32; ++i) {
+      base_through += sh.counts[i];
+      base_in += sh.best[i].i;
+    }
+    return border;
+  };
+  // A token of the slice to the first CTA's list.
+  auto gather = [&](float x, int i, int base) {
+    const int at = base + atomicAdd(&sh.gathered, 1);
+    peer_store(&sh.list[at], 0, (unsigned long long)~ordered(x) << 32 | (uint32_t)(v0 + i));
+  };
+  // The first n of the list in order (the first CTA).
+  auto sort_list = [&](int n) {
+    int size = 2;
+    while (size < n) size *= 2;
+    for (int i = n + tid; i < size; i += kThreads) sh.list[i] = ~0ull;
+    __syncthreads();
+    for (int run = 2; run <= size; run *= 2)
+      for (int step = run / 2; step > 0; step /= 2) {
+        for (int i = tid; i < size / 2; i += kThreads) {
+          const int lo = (i / step) * 2 * step + i % step, hi = lo + step;
+          const unsigned long long x = sh.list[lo], y = sh.list[hi];
+          if ((x > y) == ((lo & run) == 0)) {
+            sh.list[lo] = y;
+            sh.list[hi] = x;
+          }
+        }
+        __syncthreads();
+      }
+  };
+  constexpr int kMine = kList / kThreads;
+  // Four of the ordered list a thread: their logits and weights, and the weights'
+  // sum before the first of them.
+  auto list_sums = [&](int n, float (&x)[kMine], float (&w)[kMine]) {
+    double mine = 0.0;
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      const int i = tid * kMine + j;
+      x[j] = i < n ? unordered(~(uint32_t)(sh.list[i] >> 32)) : -INFINITY;
+      w[j] = i < n ? pow2(-depth(x[j])) : 0.0f;
+      mine += w[j];
+    }
+    double run = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += y;
+    }
+    __syncthreads();
+    if (lane == 31) sh.sums[warp] = run;
+    __syncthreads();
+    double before = run - mine;
+    for (int i = 0; i < warp; ++i) before += sh.sums[i];
+    return before;
+  };
+
+  for (int which = 0; which < 2; ++which) {
+    const bool weigh = which == 1;
+    if (!(weigh ? by_p : by_k)) continue;
+    // Tokens this far down can be no part of top-p's: all of them together, each
+    // below (1 - p) / vocab of the largest weight, are less than 1 - p of the sum.
+    const float deepest = log2f((float)a.vocab / (1.0f - fmaxf(p, 0.0f))) + 1.0f;
+    clear_hist();
+    float rest = 0.0f;
+    for_slice([&](float x, int i) {
+      if (!kept(ordered(x), i)) return;
+      const float d = depth(x);
+      if (weigh && d > deepest) {
+        rest += pow2(-d);
+        return;
+      }
+      const int bin = (int)fminf(d * kPerOctave, (float)(kBins - 1));
+      count_in(bin, weigh ? pow2((float)bin / kPerOctave - d) : 0.0f, weigh);
+    });
+    double extra = 0.0;
+    if (weigh) extra = block_sum((double)rest);
+    tell((uint32_t)__float_as_uint((float)extra), 0, 0, 0);
+    extra = 0.0;
+    if (weigh)
+      for (int r = 0; r < kCluster; ++r) extra += (double)__uint_as_float(heard(0, r));
+    int border = find_border(weigh, weigh ? (double)fmaxf(p, 0.0f) : -1.0, extra, (double)k, 0.0, 0.0,
+                             [&](int bin) { return exp2(-(double)bin / kPerOctave); });
+    const double whole = sum_all, target = weigh ? (double)fmaxf(p, 0.0f) * whole : (double)k;
+    if (border < 0) {  // all that is there is kept
+      cluster_sync();  // the histograms are read
+      continue;
+    }
+    int n_before = sh.n_before, n_in = sh.n_in;
+    double s_before = sh.s_before;
+    if (n_before + n_in <= kList) {
+      // what may be kept fits one CTA, which does the rest
+      const int n = n_before + n_in;
+      for_slice([&](float x, int i) {
+        if (!kept(ordered(x), i)) return;
+        const float d = depth(x);
+        if ((!weigh || d <= deepest) && (int)fminf(d * kPerOctave, (float)(kBins - 1)) <= border)
+          gather(x, i, base_through);
+      });
+      cluster_sync();
+      if (rank != 0) return;
+      sort_list(n);
+      float x[kMine], w[kMine];
+      double before = list_sums(n, x, w);
+      const int most = weigh ? n : min(n, k);
+      double sum = whole;
+      if (!weigh) {
+        double s = 0.0;
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) s += tid * kMine + j < most ? w[j] : 0.0f;
+        sum = block_sum(s);
+      }
+      Best pick{-1.0f, top.i};
+      double s = 0.0;
+#pragma unroll
+      for (int j = 0; j < kMine; ++j) {
+        const int i = tid * kMine + j;
+        if (i < most && (i == 0 || !by_p || before < (double)p * sum) && w[j] >= least) {
+          const int token = (int)(uint32_t)sh.list[i];
+          s += w[j];
+          pick = better(pick, Best{__fdividef(w[j], a.noise[(size_t)b * a.noise_pitch + token]), token});
+        }
+        before += w[j];
+      }
+      s = block_sum(s);
+      pick = block_best(pick);
+#pragma unroll
+      for (int j = 0; j < kMine; ++j) {
+        const int i = tid * kMine + j;
+        if (i < most && (int)(uint32_t)sh.list[i] == pick.i) answer(pick, x[j], s);
+      }
+      return;
+    }
+    // Else the border itself is found, in the border's bin alone: by ever finer
+    // histograms of the ordered logits until its tokens fit the list or are equal.
+    uint32_t lo = 0xffffffffu, hi = 0;
+    for_slice([&](float x, int i) {
+      const uint32_t u = ordered(x);
+      if (!kept(u, i)) return;
+      const float d = depth(x);
+      if ((weigh && d > deepest) || (int)fminf(d * kPerOctave, (float)(kBins - 1)) != border) return;
+      lo = min(lo, u);
+      hi = max(hi, u);
+    });
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    __syncthreads();
+    if (lane == 0) {
+      sh.counts[warp] = lo;
+      sh.best[warp].i = (int)hi;
+    }
+    __syncthreads();
+    lo = __reduce_min_sync(0xffffffffu, sh.counts[lane % kWarps]);
+    hi = __reduce_max_sync(0xffffffffu, (uint32_t)sh.best[lane % kWarps].i);
+    tell(lo, hi, 0, 0);
+    lo = __reduce_min_sync(0xffffffffu, heard(0, lane % kCluster));
+    hi = __reduce_max_sync(0xffffffffu, heard(1, lane % kCluster));
+    while (n_in > kList && lo < hi) {
+      const int shift = max(0, 32 - __clz((int)(hi - lo)) - 8);
+      const float d0 = depth(unordered(hi));
+      cluster_sync();  // the histograms are read
+      clear_hist();
+      for_slice([&](float x, int i) {
+        const uint32_t u = ordered(x);
+        if (u < lo || u > hi || !kept(u, i)) return;
+        count_in((int)((hi - u) >> shift), weigh ? pow2(d0 - depth(x)) : 0.0f, weigh);
+      });
+      cluster_sync();
+      const double scale = exp2(-(double)d0);
+      border = find_border(weigh, -1.0, 0.0, target, (double)n_before, s_before, [&](int) { return scale; });
+      if (border < 0) {  // (rounding has the whole bin short of the target: it is kept whole)
+        hi = lo;
+        n_before += n_in;
+        n_in = 0;
+        break;
+      }
+      n_before += sh.n_before;
+      n_in = sh.n_in;
+      s_before = sh.s_before;
+      hi -= (uint32_t)border << shift;
+      if (hi - lo >= 1u << shift) lo = hi - ((1u << shift) - 1);
+    }
+    if (n_in == 0) {
+      cut = lo;
+      cut_index = 0xffffffffu;
+    } else if (lo < hi || n_in <= kList) {
+      __syncthreads();
+      for_slice([&](float x, int i) {
+        const uint32_t u = ordered(x);
+        if (u >= lo && u <= hi && kept(u, i)) gather(x, i, base_in);
+      });
+      cluster_sync();
+      if (rank == 0) {
+        sort_list(n_in);
+        float x[kMine], w[kMine];
+        double run = s_before + list_sums(n_in, x, w);
+        if (tid == 0) sh.border = n_in - 1;
+        __syncthreads();
+        if (!weigh) {
+          if (tid == 0) sh.border = min(n_in - 1, k - 1 - n_before);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kMine; ++j) {
+            run += w[j];
+            if (tid * kMine + j < n_in && run >= target) atomicMin(&sh.border, tid * kMine + j);
+          }
+        }
+        __syncthreads();
+        const unsigned long long last = sh.list[sh.border];
+        if (tid < kCluster) {
+          peer_store(&sh.cut_key, tid, (uint32_t)~(uint32_t)(last >> 32));
+          peer_store(&sh.cut_index, tid, (uint32_t)last);
+        }
+      }
+      cluster_sync();
+      cut = sh.cut_key;
+      cut_index = sh.cut_index;
+    } else {
+      // equal logits: as many of them as are wanted, by index
+      const double each = (double)pow2(-depth(unordered(lo)));
+      int wanted = weigh ? (int)fmin(fmax(ceil((target - s_before) / each), 1.0), (double)n_in) : k - n_before;
+      wanted = max(1, min(wanted, n_in));
+      const int chunk = (len + kThreads - 1) / kThreads, i0 = min(len, tid * chunk), i1 = min(len, i0 + chunk);
+      int mine = 0;
+      for (int i = i0; i < i1; ++i) mine += ordered(xs[i]) == lo && kept(lo, i);
+      int run = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += y;
+      }
+      __syncthreads();
+      if (lane == 31) sh.counts[warp] = run;
+      __syncthreads();
+      int before = run - mine, all = 0;
+      for (int i = 0; i < kWarps; ++i) {
+        if (i < warp) before += sh.counts[i];
+        all += sh.counts[i];
+      }
+      tell((uint32_t)all, 0, 0, 0);
+      for (int r = 0; r < (int)rank; ++r) before += heard(0, r);
+      if (before < wanted && before + mine >= wanted) {
+        int n = before, i = i0;
+        for (;; ++i)
+          if (ordered(xs[i]) == lo && kept(lo, i) && ++n == wanted) break;
+        for (int r = 0; r < kCluster; ++r) peer_store(&sh.cut_index, r, (uint32_t)(v0 + i));
+      }
+      cluster_sync();
+      cut = lo;
+      cut_index = sh.cut_index;
+    }
+    cluster_sync();  // what the CTAs told one another here is read
   }
+
+  // the race over what is kept
+  Best pick{-1.0f, top.i};
+  float pick_x = largest;
+  double s = 0.0;
+  float part = 0.0f;
+  int terms = 0;
+  auto race = [&](float x, int i, float e) {
+    const float w = pow2(-depth(x));
+    part += w;
+    const float v = __fdividef(w, e);
+    if (v > pick.v) {
+      pick = Best{v, v0 + i};
+      pick_x = x;
+    }
+  };
+  const bool all = !by_k && !by_p && least == 0.0f && a.noise_vec;
+  for (int i = tid * 4; i < len; i += kThreads * 4) {
+    const float4 x = *reinterpret_cast<const float4 *>(xs + i);
+    const float y[4] = {x.x, x.y, x.z, x.w};
+    if (all && i + 4 <= len) {
+      const float4 e = __ldg(reinterpret_cast<const float4 *>(noise + i));
+      const float f[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (y[j] > -INFINITY) race(y[j], i + j, f[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (y[j] > -INFINITY && kept(ordered(y[j]), i + j) && pow2(-depth(y[j])) >= least)
+          race(y[j], i + j, __ldg(noise + i + j));
+    }
+    if (++terms == 8) {  // (short f32 sums: 32 terms)
+      s += part;
+      part = 0.0f;
+      terms = 0;
+    }
+  }
+  s = block_sum(s + (double)part);
+  const Best mine = pick;
+  pick = block_best(pick);
+  if (mine.i == pick.i) sh.pick_x = pick_x;
+  __syncthreads();
+  const unsigned long long bits = __double_as_longlong(s);
+  if (tid < kCluster) peer_store(&sh.list[rank], tid, bits);
+  tell(__float_as_uint(pick.v), (uint32_t)pick.i, __float_as_uint(sh.pick_x), 0);
+  pick = best_of_all();
+  if (rank == 0 && tid == 0) {
+    s = 0.0;
+    float x = 0.0f;
+    for (int r = 0; r < kCluster; ++r) {
+      s += __longlong_as_double(sh.list[r]);
+      if ((int)heard(1, r) == pick.i) x = __uint_as_float(heard(2, r));
+    }
+    answer(pick, x, s);
+  }
+}
+
+template <typename T>
+int run_sample(const SampleArgs &a, size_t batch, cudaStream_t s) {
+  {
+    static std::mutex mu;
+    static std::vector<int> done;
+    int dev = 0;
+    FPB_CUDA_TRY(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lock(mu);
+    if (std::find(done.begin(), done.end(), dev) == done.end()) {
+      FPB_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)(kMaxSlice * sizeof(float))));
+      done.push_back(dev);
+    }
+  }
+  cudaError_t e = launch_pdl_cluster(sample_kernel<T>, dim3(kCluster, (unsigned)batch), kThreads,
+                                     (size_t)a.slice * sizeof(float), s, kCluster, a);
+  if (e != cudaSuccess) return cuda_fail(e, "sample_kernel");
+  FPB_LAUNCH_CHECK("sample_kernel");
+  return FPB_OK;
 }
 
 }  // namespace
@@ -185,9 +666,9 @@ extern "C" int fpb_sample(const void *logits, int logits_dtype, size_t logits_pi
   if (!logits || !noise || !tokens) return fail(FPB_ERR_INVALID_ARGUMENT, "fpb_sample: null pointer");
   if (logits_dtype != FPB_F32 && logits_dtype != FPB_BF16)
     return fail(FPB_ERR_INVALID_ARGUMENT, "fpb_sample: dtype");
-  if (batch == 0 || batch > 65535 || vocab == 0 || vocab > 442368 || logits_pitch < vocab || noise_pitch < vocab ||
+  if (batch == 0 || batch > 65535 || vocab == 0 || vocab > (size_t)kMaxSlice * kCluster || logits_pitch < vocab || noise_pitch < vocab ||
       (logits_pitch | noise_pitch) >> 38)
-    return fail(FPB_ERR_SHAPE, "fpb_sample: batch %zu, vocab %zu (at most 442368), pitches", batch, vocab);
+    return fail(FPB_ERR_SHAPE, "fpb_sample: batch %zu, vocab %zu (at most %d), pitches", batch, vocab, kMaxSlice * kCluster);
   if (reinterpret_cast<uintptr_t>(logits) % (logits_dtype == FPB_F32 ? 4 : 2) ||
       reinterpret_cast<uintptr_t>(noise) % 4)
     return fail(FPB_ERR_INVALID_ARGUMENT, "fpb_sample: alignment");
@@ -203,10 +684,10 @@ extern "C" int fpb_sample(const void *logits, int logits_dtype, size_t logits_pi
   a.vocab = (int)vocab;
   a.tokens = tokens;
   a.logprobs = logprobs;
-  cudaError_t e = logits_dtype == FPB_F32
-                      ? launch_pdl(sample_kernel<float>, (unsigned)batch, kSampleThreads, 0, as_stream(stream), a)
-                      : launch_pdl(sample_kernel<__nv_bfloat16>, (unsigned)batch, kSampleThreads, 0, as_stream(stream), a);
-  if (e != cudaSuccess) return cuda_fail(e, "sample_kernel");
-  FPB_LAUNCH_CHECK("sample_kernel");
-  return FPB_OK;
+  a.slice = (int)((vocab + kCluster - 1) / kCluster + 7) / 8 * 8;
+  auto lies = [](const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && bytes % 16 == 0; };
+  a.vec = lies(logits, logits_pitch * (logits_dtype == FPB_F32 ? 4 : 2));
+  a.noise_vec = lies(noise, noise_pitch * 4);
+  return logits_dtype == FPB_F32 ? run_sample<float>(a, batch, as_stream(stream))
+                                 : run_sample<__nv_bfloat16>(a, batch, as_stream(stream));
 }

@@ -906,7 +906,7 @@ int fpb_paged_attn(const void *q, int q_dtype, size_t q_pitch, size_t q_head_pit
  * temperature [batch] (NULL: 1; held within [1e-6, 1e6]): 0 or below takes the first
  * token; top_k, top_p, min_p [batch] (NULL: none).  A row without a finite logit
  * gives -1.  logprobs [batch] (NULL: not wanted): the log of the token's weight among
- * what is kept (greedy: 0).  vocab up to 442368. */
+ * what is kept (greedy: 0).  vocab up to 393216. */
 int fpb_sample(const void *logits, int logits_dtype, size_t logits_pitch, const float *temperature,
                const int32_t *top_k, const float *top_p, const float *min_p, const float *noise, size_t noise_pitch,
                size_t batch, size_t vocab, int32_t *tokens, float *logprobs, void *stream);

@@ -84,7 +84,7 @@ def test_sample_checks_arguments():
                dict(logits=f + 1, dtype=1)):
         assert sample(**kw) == bad, kw
     for kw in (dict(batch=0), dict(batch=65536), dict(vocab=0), dict(pitch=99), dict(noise_pitch=99),
-               dict(vocab=442369, pitch=442369, noise_pitch=442369), dict(pitch=1 << 40)):
+               dict(vocab=393217, pitch=393217, noise_pitch=393217), dict(pitch=1 << 40)):
         assert sample(**kw) == shape, kw
 
 
