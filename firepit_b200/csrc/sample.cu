@@ -20,9 +20,16 @@ namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kCluster = 8;
 constexpr int kMaxSlice = 49152;  // f32 of shared memory a CTA: 192 KB
-constexpr int kBatch = 5;         // 16-byte loads a thread has under way
-constexpr int kBins = 256, kPerOctave = 8;  // bins of a histogram: an eighth of a power of two each, the last one the rest
-constexpr int kList = 2048;       // tokens that one CTA orders
+constexpr int kBatch = 5;         // 16-byte loads a thread has under way (f32 logits: twice as many)
+constexpr int kBins = 256;        // bins of a histogram
+constexpr int kList = kThreads;   // tokens that one CTA orders
+constexpr int kLargest = kWarps * kCluster;  // warps of a cluster, each with its largest logit
+// What the k-th largest of the warps' 128 largest logits reaches is, with logits in
+// no order, -128 ln(1 - k / 128) tokens: for 120 of them 355, for 96 177.
+constexpr int kDirect = 120, kDirectSum = 96;
+constexpr int kLists = 16;  // at most: one, and for each of two filters one and 32 / 8 finer ones
+
+constexpr float kLowest = -3.402823466e38f;
 
 struct SampleArgs {
   const void *logits;
@@ -64,13 +71,27 @@ __device__ __forceinline__ uint32_t peer_address(const void *p, unsigned rank) {
 __device__ __forceinline__ void peer_store(const void *p, unsigned rank, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_address(p, rank)), "r"(v) : "memory");
 }
-__device__ __forceinline__ void peer_store(const void *p, unsigned rank, unsigned long long v) {
-  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer_address(p, rank)), "l"(v) : "memory");
-}
-__device__ __forceinline__ uint32_t peer_load(const uint32_t *p, unsigned rank) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer_address(p, rank)) : "memory");
+__device__ __forceinline__ unsigned long long peer_load(const unsigned long long *p, unsigned rank) {
+  unsigned long long v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(peer_address(p, rank)) : "memory");
   return v;
+}
+__device__ __forceinline__ uint2 peer_load(const uint2 *p, unsigned rank) {
+  uint2 v;
+  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(peer_address(p, rank)) : "memory");
+  return v;
+}
+// cluster_sync() behind code that lanes may leave apart: its barrier counts whole warps.
+__device__ __forceinline__ void meet() {
+  __syncwarp();
+  cluster_sync();
+}
+// *p += v in shared memory where `ok`.
+__device__ __forceinline__ void add_if(bool ok, uint32_t *p, uint32_t v) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q red.shared.add.u32 [%0], %1;\n\t}" ::"r"(
+                   (uint32_t)__cvta_generic_to_shared(p)),
+               "r"(v), "r"((int)ok)
+               : "memory");
 }
 
 template <typename V>
@@ -81,22 +102,103 @@ __device__ __forceinline__ V warp_total(V v) {
 }
 
 struct Shared {
-  unsigned long long list[kList];  // of the first CTA: tokens to be ordered, (falling logit, index) as one number
-  uint32_t hist[3][kBins];         // tokens; their weights' sum, low and high part
+  unsigned long long list[kList];  // tokens to be ordered, (falling logit, index) as one number
+  uint2 hist[kBins];               // x: tokens, or the low part of their weights' sum; y: its high part
   // what the CTAs tell one another; the halves alternate, so that one exchange's
   // reads may overlap the next one's stores
   uint32_t got[2][5][kCluster];
-  float maxima[kCluster * kWarps];  // every warp's largest logit
+  float maxima[kLargest];
   double sums[kWarps];
   uint32_t counts[kWarps];
   Best best[kWarps];
-  int border, n_before, n_in;  // where a histogram reaches its target: the bin, tokens before and in it
+  int border;  // where a histogram reaches its target: the bin, tokens and weights before it, tokens in it
+  uint32_t n_before, n_in;
   double s_before;
-  int gathered[3];  // of the first CTA: tokens in the list, each time anew
-  int sent;         // this CTA's part of the first ones
-  uint32_t cut, cut_index;
-  float bound, pick_x;
+  uint32_t listed[kLists];  // tokens in the list, each time anew
+  float cut;
+  int cut_index;
+  uint32_t bound;
+  float last_sum[kWarps], last_x[kWarps];
 };
+
+// The block's n (<= kList) numbers x, one a thread, in order: the tid-th, or ~0 past
+// them.  All threads.  Bitonic, neighbours up to 16 apart through registers.
+__device__ __noinline__ unsigned long long sorted(Shared &sh, int n, unsigned long long x) {
+  const int tid = threadIdx.x;
+  int size = 32;
+  while (size < n) size *= 2;
+  for (int run = 2; run <= size; run *= 2) {
+    const bool up = (tid & run) == 0;
+    int step = run / 2;
+    for (; step >= 32; step /= 2) {
+      __syncthreads();
+      if (tid < size) sh.list[tid] = x;
+      __syncthreads();
+      if (tid < size) {
+        const unsigned long long y = sh.list[tid ^ step];
+        x = (x < y) == (((tid & step) == 0) == up) ? x : y;
+      }
+    }
+    if (tid < size)
+      for (; step > 0; step /= 2) {
+        const unsigned long long y = __shfl_xor_sync(0xffffffffu, x, step);
+        x = (x < y) == (((tid & step) == 0) == up) ? x : y;
+      }
+  }
+  __syncthreads();
+  return x;
+}
+
+// Over the cluster's histograms: the first bin at which the running count (from n0
+// on), or weight (from s0 on; bin i's whole numbers times 2^-20 and 2^-(i * step)),
+// reaches the target (-1: none), with what lies before it.  Every CTA finds the
+// same.  Two threads a bin, four CTAs' each.
+__device__ __noinline__ int find_border(Shared &sh, bool weigh, double target, uint32_t n0, double s0, float step) {
+  static_assert(kThreads == 2 * kBins && kCluster == 8);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bin = tid >> 1, from = 4 * (tid & 1);
+  uint2 x[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) x[r] = peer_load(&sh.hist[bin], from + r);
+  uint32_t c = x[0].x + x[1].x + x[2].x + x[3].x;
+  unsigned long long f = c + ((unsigned long long)x[0].y + x[1].y + x[2].y + x[3].y << 11);
+  c += __shfl_xor_sync(0xffffffffu, c, 1);
+  f += __shfl_xor_sync(0xffffffffu, f, 1);
+  const bool one = (tid & 1) == 0;
+  if (!one) c = 0;
+  const double v = weigh && one ? (double)f * 0x1p-20 * (double)pow2(-(float)bin * step) : 0.0;
+  // running count and sum over the bins
+  uint32_t n = c;
+  double run = v;
+#pragma unroll
+  for (int o = 2; o < 32; o <<= 1) {
+    const uint32_t u = __shfl_up_sync(0xffffffffu, n, o);
+    const double w = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o && one) {
+      n += u;
+      run += w;
+    }
+  }
+  if (lane == 30) {
+    sh.counts[warp] = n;
+    sh.sums[warp] = run;
+  }
+  if (tid == 0) sh.border = kBins;
+  __syncthreads();
+  for (int i = 0; i < warp; ++i) {
+    n0 += sh.counts[i];
+    s0 += sh.sums[i];
+  }
+  if (one && f > 0 && (weigh ? s0 + run >= target : n0 + n >= (uint32_t)target)) atomicMin(&sh.border, bin);
+  __syncthreads();
+  const int border = sh.border;
+  if (one && bin == border) {
+    sh.n_before = n0 + n - c;
+    sh.n_in = c;
+    sh.s_before = s0 + run - v;
+  }
+  __syncthreads();
+  return border < kBins ? border : -1;
+}
 
 // A cluster of kCluster CTAs a row: CTA `rank` keeps the vocabulary's slice [rank
 // * slice, +slice) in shared memory, so that the row is read once.
@@ -128,54 +230,59 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const bool greedy = !(t > 0.0f), by_k = k > 0 && k < a.vocab, by_p = p < 1.0f;
   const float least = m > 0.0f ? fminf(m, 1.0f) : 0.0f;
   const bool plain = !by_k && !by_p && least == 0.0f;
-  if (!greedy && plain && a.noise_vec && tid == 0 && len >= 4)  // all of its noise is wanted
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(noise), "r"(len / 4 * 16) : "memory");
-  if (tid < 3) sh.gathered[tid] = 0;
-  if (tid == 3) sh.sent = 0;
-
-  // the slice to shared memory, and its first largest logit
-  Best top{-INFINITY, 0x7fffffff};
-  auto take = [&](float x, int i) {
-    x = fabsf(x) <= 3.402823466e38f ? x : -INFINITY;
-    if (x > top.v) top = Best{x, v0 + i};
-    return x;
+  const float temp = fminf(fmaxf(t, 1e-6f), 1e6f), per = 1.4426950408889634f / temp;
+  auto want_noise = [&]() {  // all of the slice's, to L2
+    if (a.noise_vec && tid == 0 && len >= 4)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(noise), "r"(len / 4 * 16) : "memory");
   };
+  if (!greedy && plain) want_noise();
+  if (tid < kLists) sh.listed[tid] = 0;
+  if (tid == 0) sh.bound = 0xffffffffu;
+
+  // The slice to shared memory, and its largest logit: the first of the first four
+  // that hold one.
+  Best top{-INFINITY, 0x7fffffff};
   {
-    constexpr int N = 16 / sizeof(T);
+    constexpr int N = 16 / sizeof(T), kLoads = sizeof(T) == 4 ? 2 * kBatch : kBatch;
+    auto finite = [](float x) { return fabsf(x) <= 3.402823466e38f ? x : -INFINITY; };
+    auto take = [&](float x0, float x1, float x2, float x3, int i) {
+      const float4 y = make_float4(finite(x0), finite(x1), finite(x2), finite(x3));
+      *reinterpret_cast<float4 *>(xs + i) = y;
+      const float most = fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w));
+      if (most > top.v) top = Best{most, i};
+    };
     const int whole = a.vec ? len / N * N : 0;
-    for (int i0 = tid * N; i0 < whole; i0 += kBatch * kThreads * N) {
-      uint4 v[kBatch];
+    for (int i0 = tid * N; i0 < whole; i0 += kLoads * kThreads * N) {
+      uint4 v[kLoads];
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
+      for (int j = 0; j < kLoads; ++j) {
         const int i = i0 + j * kThreads * N;
         v[j] = i < whole ? __ldg(reinterpret_cast<const uint4 *>(row + i)) : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
+      for (int j = 0; j < kLoads; ++j) {
         const int i = i0 + j * kThreads * N;
         if (i >= whole) break;
-        const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
         if constexpr (N == 4) {
-          float4 y;
-          y.x = take(__uint_as_float(w[0]), i);
-          y.y = take(__uint_as_float(w[1]), i + 1);
-          y.z = take(__uint_as_float(w[2]), i + 2);
-          y.w = take(__uint_as_float(w[3]), i + 3);
-          *reinterpret_cast<float4 *>(xs + i) = y;
+          take(__uint_as_float(v[j].x), __uint_as_float(v[j].y), __uint_as_float(v[j].z), __uint_as_float(v[j].w), i);
         } else {
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            float4 y;
-            y.x = take(__uint_as_float(w[2 * q] << 16), i + 4 * q);
-            y.y = take(__uint_as_float(w[2 * q] & 0xffff0000u), i + 4 * q + 1);
-            y.z = take(__uint_as_float(w[2 * q + 1] << 16), i + 4 * q + 2);
-            y.w = take(__uint_as_float(w[2 * q + 1] & 0xffff0000u), i + 4 * q + 3);
-            *reinterpret_cast<float4 *>(xs + i + 4 * q) = y;
-          }
+          take(__uint_as_float(v[j].x << 16), __uint_as_float(v[j].x & 0xffff0000u), __uint_as_float(v[j].y << 16),
+               __uint_as_float(v[j].y & 0xffff0000u), i);
+          take(__uint_as_float(v[j].z << 16), __uint_as_float(v[j].z & 0xffff0000u), __uint_as_float(v[j].w << 16),
+               __uint_as_float(v[j].w & 0xffff0000u), i + 4);
         }
       }
     }
-    for (int i = whole + tid; i < padded; i += kThreads) xs[i] = i < len ? take(static_cast<float>(row[i]), i) : -INFINITY;
+    for (int i = whole + tid * 4; i < padded; i += kThreads * 4) {
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = i + j < len ? static_cast<float>(row[i + j]) : -INFINITY;
+      take(x[0], x[1], x[2], x[3], i);
+    }
+    if (top.i != 0x7fffffff) {  // which of the four
+      const float4 y = *reinterpret_cast<const float4 *>(xs + top.i);
+      top.i += v0 + (y.x == top.v ? 0 : y.y == top.v ? 1 : y.z == top.v ? 2 : 3);
+    }
   }
   auto block_best = [&](Best x) {  // (the warps' own are left in sh.best)
 #pragma unroll
@@ -189,38 +296,46 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       x = better(x, Best{__shfl_xor_sync(0xffffffffu, x.v, o), __shfl_xor_sync(0xffffffffu, x.i, o)});
     return x;
   };
-  auto block_sum = [&](double v) {
+  // Sum over the block: a warp's in f32, those in 64 bits.
+  auto block_sum = [&](float v) {
     v = warp_total(v);
     __syncthreads();  // (the sums before are read)
     if (lane == 0) sh.sums[warp] = v;
     __syncthreads();
-    v = sh.sums[lane % kWarps];
+    double s = 0.0;
 #pragma unroll
-    for (int o = kWarps / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    for (int i = 0; i < kWarps; ++i) s += sh.sums[i];
+    return s;
   };
   int flip = 0;
-  auto tell = [&](uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t w4 = 0) {
-    if (tid < kCluster) {
-      peer_store(&sh.got[flip][4][rank], tid, w4);
-      peer_store(&sh.got[flip][0][rank], tid, w0);
-      peer_store(&sh.got[flip][1][rank], tid, w1);
-      peer_store(&sh.got[flip][2][rank], tid, w2);
-      peer_store(&sh.got[flip][3][rank], tid, w3);
+  auto tell = [&](uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t w4) {
+    if (tid < 5 * kCluster) {
+      const int word = tid / kCluster;
+      peer_store(&sh.got[flip][word][rank], tid % kCluster,
+                 word == 0 ? w0 : word == 1 ? w1 : word == 2 ? w2 : word == 3 ? w3 : w4);
     }
-    cluster_sync();
+    meet();
     flip ^= 1;
   };
-  auto tell_sums = [&](double x, double y, uint32_t n = 0) {
-    const unsigned long long u = __double_as_longlong(x), v = __double_as_longlong(y);
-    tell((uint32_t)u, (uint32_t)(u >> 32), (uint32_t)v, (uint32_t)(v >> 32), n);
+  // (words 0, 1: a logit and its token; 2, 3: a sum; 4: a number)
+  auto tell_best = [&](Best x, double sum, uint32_t n) {
+    const unsigned long long u = __double_as_longlong(sum);
+    tell(__float_as_uint(x.v), (uint32_t)x.i, (uint32_t)u, (uint32_t)(u >> 32), n);
   };
   auto heard = [&](int word, int from) { return sh.got[flip ^ 1][word][from]; };
-  auto heard_sum = [&](int word) {  // over the CTAs, in order
-    double s = 0.0;
-    for (int r = 0; r < kCluster; ++r)
-      s += __longlong_as_double((unsigned long long)heard(word + 1, r) << 32 | heard(word, r));
+  auto heard_double = [&](int from) {
+    return __longlong_as_double((unsigned long long)heard(3, from) << 32 | heard(2, from));
+  };
+  auto over_ctas = [&](double s) {  // each lane with CTA lane % 8's: every lane gets the same
+#pragma unroll
+    for (int o = kCluster / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     return s;
+  };
+  auto heard_sum = [&]() { return over_ctas(heard_double(lane % kCluster)); };
+  auto heard_count = [&]() {
+    uint32_t n = 0;
+    for (int r = 0; r < kCluster; ++r) n += heard(4, r);
+    return n;
   };
   auto best_of_all = [&]() {
     Best x{__uint_as_float(heard(0, lane % kCluster)), (int)heard(1, lane % kCluster)};
@@ -230,11 +345,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     return x;
   };
   top = block_best(top);
+  // for top-p alone: the slice's weights over its largest logit
+  double slice_sum = 0.0;
+  if (by_p && !by_k && !greedy) {
+    const float over = fmaxf(top.v, kLowest);  // (a slice may have no finite logit)
+    float part = 0.0f;
+#pragma unroll 5
+    for (int i = tid * 4; i < len; i += kThreads * 4) {
+      const float4 x = *reinterpret_cast<const float4 *>(xs + i);
+      part += (pow2((x.x - over) * per) + pow2((x.y - over) * per)) + (pow2((x.z - over) * per) + pow2((x.w - over) * per));
+    }
+    slice_sum = block_sum(part);
+  }
+  __syncwarp();
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  static_assert(kWarps * kCluster <= kThreads);
-  if (tid < kWarps * kCluster)
+  static_assert(kLargest <= kThreads);
+  if (tid < kLargest)
     peer_store(&sh.maxima[rank * kWarps + tid / kCluster], tid % kCluster, __float_as_uint(sh.best[tid / kCluster].v));
-  tell(__float_as_uint(top.v), (uint32_t)top.i, 0, 0);
+  tell_best(top, slice_sum, 0);
   top = best_of_all();
   if (greedy || top.i == 0x7fffffff) {
     if (rank == 0 && tid == 0) {
@@ -243,101 +371,70 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
     return;
   }
-  const float temp = fminf(fmaxf(t, 1e-6f), 1e6f), per = 1.4426950408889634f / temp, largest = top.v;
+  const float largest = top.v;
   auto depth = [&](float x) { return (largest - x) * per; };  // w = 2^-depth
-  // What is kept so far: logits above `cut` (ordered), and those of it up to index
+  double whole;  // the weights' sum, for top-p alone
+  {
+    const float theirs = fmaxf(__uint_as_float(heard(0, lane % kCluster)), kLowest);
+    whole = over_ctas(heard_double(lane % kCluster) * (double)pow2(-depth(theirs)));
+  }
+  // What is kept so far: logits above `cut`, and of those equal to it the tokens up to
   // `cut_index`.
-  uint32_t cut = 0, cut_index = 0;
-  auto kept = [&](float x, int i) {
-    const uint32_t u = ordered(x);
-    return u > cut || (u == cut && (uint32_t)(v0 + i) <= cut_index);
-  };
-  // f(x, i) for the slice's logits from `bound` (finite) up
+  float cut = -INFINITY;
+  int cut_index = -1;
+  auto kept = [&](float x, int i) { return x > cut || (x == cut && v0 + i <= cut_index); };
+  // f(x, i) for the slice's logits x[0, 4) from i on where one is `bound` (finite) or
+  // above
   auto for_above = [&](float bound, auto f) {
 #pragma unroll 2
     for (int i = tid * 4; i < len; i += kThreads * 4) {
-      const float4 x = *reinterpret_cast<const float4 *>(xs + i);
-      if (fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)) >= bound) {
-        if (x.x >= bound) f(x.x, i);
-        if (x.y >= bound) f(x.y, i + 1);
-        if (x.z >= bound) f(x.z, i + 2);
-        if (x.w >= bound) f(x.w, i + 3);
-      }
+      const float4 y = *reinterpret_cast<const float4 *>(xs + i);
+      const float x[4] = {y.x, y.y, y.z, y.w};
+      if (fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= bound) f(x, i);
     }
   };
-  constexpr float kLowest = -3.402823466e38f;
   // the row's token and its log probability, of weights that sum to s
   auto answer = [&](int token, float x, double s) {
     a.tokens[b] = token;
     if (a.logprobs) a.logprobs[b] = (float)(((double)x - (double)largest) / (double)temp - log(s));
   };
-  // A token of the slice to the first CTA's list, if it has room.
-  auto gather = [&](float x, int i, int counter) {
-    uint32_t at;
-    asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;"
-                 : "=r"(at)
-                 : "r"(peer_address(&sh.gathered[counter], 0))
-                 : "memory");
-    if (at < (uint32_t)kList) peer_store(&sh.list[at], 0, (unsigned long long)~ordered(x) << 32 | (uint32_t)(v0 + i));
-  };
-  // The first n of the list in order (the first CTA).
-  auto sort_list = [&](int n) {
-    if (n <= kThreads) {  // a token a thread; neighbours through registers
-      int size = 32;
-      while (size < n) size *= 2;
-      unsigned long long x = tid < n ? sh.list[tid] : ~0ull;
-      for (int run = 2; run <= size; run *= 2) {
-        const bool up = (tid & run) == 0;
-        for (int step = run / 2; step > 0; step /= 2) {
-          unsigned long long y;
-          if (step >= 32) {
-            __syncthreads();
-            if (tid < size) sh.list[tid] = x;
-            __syncthreads();
-            y = tid < size ? sh.list[tid ^ step] : x;
-          } else {
-            y = __shfl_xor_sync(0xffffffffu, x, step);
-          }
-          const bool low = (tid & step) == 0;
-          x = (x < y) == (low == up) ? x : y;
-        }
-      }
-      __syncthreads();
-      if (tid < size) sh.list[tid] = x;
-      __syncthreads();
-      return;
-    }
-    int size = 2 * kThreads, bits;
-    while (size < n) size *= 2;
-    for (int i = n + tid; i < size; i += kThreads) sh.list[i] = ~0ull;
-    __syncthreads();
-    for (int run = 2; run <= size; run *= 2)
-      for (bits = 30 - __clz(run); bits >= 0; --bits) {
-        const int step = 1 << bits;
-        for (int i = tid; i < size / 2; i += kThreads) {
-          const int lo = (i >> bits) << (bits + 1) | (i & (step - 1)), hi = lo + step;
-          const unsigned long long x = sh.list[lo], y = sh.list[hi];
-          if ((x > y) == ((lo & run) == 0)) {
-            sh.list[lo] = y;
-            sh.list[hi] = x;
-          }
-        }
-        __syncthreads();
-      }
-  };
-  constexpr int kMine = kList / kThreads;
-  // Four of the ordered list a thread: their logits and weights, and the weights'
-  // sum before the first of them.
-  auto list_sums = [&](int n, float (&x)[kMine], float (&w)[kMine]) {
-    double mine = 0.0;
+  // Lists the slice's logits from `bound` up that are wanted(x, i), as long as there
+  // is room; returns how many the cluster has, with the sum of the weights of this
+  // CTA's told where it is asked for.
+  int lists = 0;
+  auto gather = [&](float bound, bool weigh, auto wanted) {
+    float in = 0.0f;
+    for_above(bound, [&](const float (&x)[4], int i) {
+      uint32_t hits = 0;
 #pragma unroll
-    for (int j = 0; j < kMine; ++j) {
-      const int i = tid * kMine + j;
-      x[j] = i < n ? unordered(~(uint32_t)(sh.list[i] >> 32)) : -INFINITY;
-      w[j] = i < n ? pow2(-depth(x[j])) : 0.0f;
-      mine += w[j];
-    }
-    double run = mine;
+      for (int j = 0; j < 4; ++j) hits |= (uint32_t)((x[j] >= bound) & wanted(x[j], i + j)) << j;
+      if (!hits) return;
+      uint32_t at = atomicAdd(&sh.listed[lists], (uint32_t)__popc(hits));
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (hits >> j & 1) {
+          if (at < (uint32_t)kList) sh.list[at] = (unsigned long long)~ordered(x[j]) << 32 | (uint32_t)(v0 + i + j);
+          ++at;
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(noise + i + j));
+          if (weigh) in += pow2(-depth(x[j]));
+        }
+    });
+    const double mine = weigh ? block_sum(in) : 0.0;
+    __syncthreads();
+    tell_best(Best{0.0f, 0}, mine, sh.listed[lists]);
+    ++lists;
+    return heard_count();
+  };
+  // The lists of the cluster, n in all: its tid-th token, in order of CTA (the first
+  // CTA's threads).
+  auto listed = [&](int n) {
+    int r = 0, at = tid;
+    while (r < kCluster - 1 && at >= (int)heard(4, r)) at -= (int)heard(4, r++);
+    return tid < n ? peer_load(&sh.list[at], r) : ~0ull;
+  };
+  // The running sum of the weights w of the ordered list, without the thread's own.
+  auto before_in_list = [&](float w) {
+    double run = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double y = __shfl_up_sync(0xffffffffu, run, o);
@@ -346,295 +443,190 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     __syncthreads();
     if (lane == 31) sh.sums[warp] = run;
     __syncthreads();
-    double before = run - mine;
+    double before = run - w;
     for (int i = 0; i < warp; ++i) before += sh.sums[i];
     return before;
   };
-  // The answer from a list of n that holds all that may be kept: the first `most` of
-  // it, of them what makes p of `sum` (0: of their own weights).
-  auto finish_list = [&](int n, int most, double sum) {
-    sort_list(n);
-    float x[kMine], w[kMine];
-    double before = list_sums(n, x, w);
-    if (sum == 0.0 && by_p) {
-      double s = 0.0;
-#pragma unroll
-      for (int j = 0; j < kMine; ++j) s += tid * kMine + j < most ? w[j] : 0.0f;
-      sum = block_sum(s);
-    }
-    Best pick{0.0f, top.i};
-    double s = 0.0;
-#pragma unroll
-    for (int j = 0; j < kMine; ++j) {
-      const int i = tid * kMine + j;
-      if (i < most && (i == 0 || !by_p || before < (double)p * sum) && w[j] >= least) {
-        const int token = (int)(uint32_t)sh.list[i];
-        s += w[j];
-        pick = better(pick, Best{__fdividef(w[j], a.noise[(size_t)b * a.noise_pitch + token]), token});
-      }
-      before += w[j];
-    }
-    s = block_sum(s);
-    pick = block_best(pick);
-#pragma unroll
-    for (int j = 0; j < kMine; ++j) {
-      const int i = tid * kMine + j;
-      if (i < most && (int)(uint32_t)sh.list[i] == pick.i) answer(pick.i, x[j], s);
-    }
-  };
 
-  double whole = 0.0;  // the row's weights, where they are known
-  if (by_k ? k <= kWarps * kCluster : by_p) {
-    const int wanted = by_k ? k : kWarps * kCluster;
-    if (tid < kWarps * kCluster) {
-      const float mine = sh.maxima[tid];
+  if (by_k ? k <= kDirect : by_p) {
+    const int wanted = by_k ? k : kDirectSum;
+    {  // The smallest of the warps' largest that fewer than `wanted` of them are above:
+       // four threads each, a quarter of the others.
+      static_assert(kThreads == 4 * kLargest);
+      const float mine = sh.maxima[tid / 4];
       int above = 0;
-#pragma unroll 8
-      for (int i = 0; i < kWarps * kCluster; ++i) {
-        const float x = sh.maxima[i];
-        above += x > mine || (x == mine && i < tid);
+#pragma unroll
+      for (int j = 0; j < kLargest / 16; ++j) {
+        const float4 x = *reinterpret_cast<const float4 *>(sh.maxima + 4 * (4 * j + tid % 4));
+        above += (x.x > mine) + (x.y > mine) + (x.z > mine) + (x.w > mine);
       }
-      if (above == wanted - 1) sh.bound = fmaxf(mine, kLowest);
+      above += __shfl_xor_sync(0xffffffffu, above, 1);
+      above += __shfl_xor_sync(0xffffffffu, above, 2);
+      const uint32_t low = __reduce_min_sync(0xffffffffu, above < wanted ? ordered(mine) : 0xffffffffu);
+      if (lane == 0) atomicMin(&sh.bound, low);
     }
     __syncthreads();
-    const float bound = sh.bound;
-    auto candidate = [&](float x, int i) {
-      gather(x, i, 0);
-      atomicAdd(&sh.sent, 1);
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(noise + i));
-    };
-    if (by_k) {
-      for_above(bound, candidate);
-      __syncthreads();
-      tell_sums(0.0, 0.0, (uint32_t)sh.sent);
-    } else {
-      float part = 0.0f, in = 0.0f;
-      for (int i = tid * 4; i < len; i += kThreads * 4) {
-        const float4 x = *reinterpret_cast<const float4 *>(xs + i);
-        const float w[4] = {pow2(-depth(x.x)), pow2(-depth(x.y)), pow2(-depth(x.z)), pow2(-depth(x.w))};
-        part += (w[0] + w[1]) + (w[2] + w[3]);
-        if (fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)) >= bound) {
-          const float y[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (y[j] >= bound) {
-              candidate(y[j], i + j);
-              in += w[j];
-            }
-        }
-      }
-      const double mine = block_sum((double)part), mine_in = block_sum((double)in);
-      tell_sums(mine, mine_in, (uint32_t)sh.sent);
-      whole = heard_sum(0);
-    }
-    int n = 0;
-    for (int r = 0; r < kCluster; ++r) n += (int)heard(4, r);
+    const uint32_t n = gather(fmaxf(unordered(sh.bound), kLowest), !by_k, [](float, int) { return true; });
     // (a list whose weights make p of the row's but for rounding might be a token short)
-    if (n <= kList && (by_k || heard_sum(2) >= (double)p * whole * (1.0 + 1e-6))) {
-      if (rank == 0) finish_list(n, by_k ? min(n, k) : n, whole);
+    if (n <= (uint32_t)kList && (by_k || heard_sum() >= (double)p * whole * (1.0 + 1e-6))) {
+      unsigned long long mine = rank == 0 ? listed((int)n) : 0;
+      __syncwarp();
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // the lists are read
+      if (rank != 0) {
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        return;
+      }
+      const int most = by_k ? min((int)n, k) : (int)n;
+      mine = sorted(sh, (int)n, mine);
+      const int token = (int)(uint32_t)mine;
+      const float x = tid < most ? unordered(~(uint32_t)(mine >> 32)) : -INFINITY, w = pow2(-depth(x));
+      const float e = tid < most ? __ldg(a.noise + (size_t)b * a.noise_pitch + token) : 1.0f;
+      const double before = by_p ? before_in_list(w) : 0.0;
+      if (by_k && by_p) whole = block_sum(w);
+      const bool in = tid < most && (tid == 0 || !by_p || before < (double)p * whole) && w >= least;
+      const Best pick = block_best(in ? Best{__fdividef(w, e), token} : Best{0.0f, top.i});
+      const double s = block_sum(in ? w : 0.0f);
+      if (tid < most && token == pick.i) answer(token, x, s);
+      __syncwarp();
+      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
       return;
     }
   }
 
-  // Weights go to a histogram as whole numbers, relative to the bin's largest, so
-  // that their sum does not depend on the order: 31 bits in two parts of 16 and 15
-  // (49152 of them fit 32 bits).
-  auto count_in = [&](int bin, float u, bool weigh) {
-    atomicAdd(&sh.hist[0][bin], 1u);
-    if (weigh) {
-      const uint32_t f = (uint32_t)__float2uint_rn(u * 0x1p31f);
-      atomicAdd(&sh.hist[1][bin], f & 0xffffu);
-      atomicAdd(&sh.hist[2][bin], f >> 16);
-    }
+  // Weights go to a histogram as whole numbers, relative to their bin's, so that
+  // their sum does not depend on the order: 22 bits in two parts of 11 (49152 of
+  // them fit 32 bits).  A bin is a nearest whole number: its own add to 1.5 * 2^23
+  // has it in the low bits (conversions take as long as a power).
+  constexpr float kRound = 12582912.0f;
+  auto count_in = [&](bool ok, int bin, float u, bool weigh) {
+    const uint32_t f = __float_as_uint(fmaf(u, 0.125f, 1.0f)) & 0x7fffffu;  // u * 2^20
+    add_if(ok, &sh.hist[bin].x, weigh ? f & 0x7ffu : 1u);
+    add_if(ok && weigh, &sh.hist[bin].y, f >> 11);
   };
   auto clear_hist = [&]() {
-    for (int i = tid; i < 3 * kBins; i += kThreads) (&sh.hist[0][0])[i] = 0;
+    reinterpret_cast<uint32_t *>(sh.hist)[tid] = 0;
     __syncthreads();
   };
-  auto bin_of = [&](float x) { return (int)fminf(depth(x) * kPerOctave, (float)(kBins - 1)); };
-  // Over the cluster's histograms (scale(bin): what a bin's weights are relative
-  // to): the first bin at which the running count, or sum, from n0 and s0 on, reaches
-  // the target (-1: none), with what lies before it.  Every CTA finds the same.
-  auto find_border = [&](bool weigh, double target, double n0, double s0, auto scale) {
-    uint32_t c = 0;
-    unsigned long long s = 0;
-    if (tid < kBins) {
-#pragma unroll
-      for (int r = 0; r < kCluster; ++r) {
-        c += peer_load(&sh.hist[0][tid], r);
-        if (weigh) s += peer_load(&sh.hist[1][tid], r) + ((unsigned long long)peer_load(&sh.hist[2][tid], r) << 16);
-      }
-    }
-    const double v = weigh && tid < kBins ? (double)s * 0x1p-31 * scale(tid) : 0.0;
-    // running count and sum over the bins
-    uint32_t n = c;
-    double run = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t x = __shfl_up_sync(0xffffffffu, n, o);
-      const double y = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) {
-        n += x;
-        run += y;
-      }
-    }
-    __syncthreads();
-    if (lane == 31) {
-      sh.counts[warp] = n;
-      sh.sums[warp] = run;
-    }
-    if (tid == 0) sh.border = -1;
-    __syncthreads();
-    double s_at = s0;
-    uint32_t n_at = 0;
-#pragma unroll
-    for (int i = 0; i < kBins / 32; ++i)
-      if (i < warp) {
-        n_at += sh.counts[i];
-        s_at += sh.sums[i];
-      }
-    if (tid < kBins && c > 0 && (weigh ? s_at + run : n0 + n_at + n) >= target)
-      atomicMax(&sh.border, kBins - 1 - tid);  // the first of them
-    __syncthreads();
-    const int border = sh.border < 0 ? -1 : kBins - 1 - sh.border;
-    if (tid == border) {
-      sh.n_before = (int)(n_at + n - c);
-      sh.n_in = (int)c;
-      sh.s_before = s_at + run - v;
-    }
-    __syncthreads();
-    return border;
-  };
+  static_assert(kThreads == 2 * kBins);
+  if (by_p) want_noise();  // much of it: more is kept than fits the list
 
   for (int which = 0; which < 2; ++which) {
     const bool weigh = which == 1;
     if (!(weigh ? by_p : by_k)) continue;
-    float bound = kLowest;
+    float bound = kLowest, octave = 8.0f;  // bins an octave
     if (weigh) {
-      if (whole == 0.0 || cut) {  // of what top-k kept
+      if (by_k) {  // of what top-k kept
         float part = 0.0f;
-        for_above(kLowest, [&](float x, int i) { part += kept(x, i) ? pow2(-depth(x)) : 0.0f; });
-        tell_sums(block_sum((double)part), 0.0);
-        whole = heard_sum(0);
+        for_above(kLowest, [&](const float (&x)[4], int i) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) part += kept(x[j], i + j) ? pow2(-depth(x[j])) : 0.0f;
+        });
+        tell_best(top, block_sum(part), 0);
+        whole = heard_sum();
       }
       // Tokens this far down can be no part of top-p's: all of them together, each
       // below (1 - p) / vocab of the sum, are less than 1 - p of it.
       const float deepest = log2f((float)a.vocab / ((1.0f - fmaxf(p, 0.0f)) * (float)whole)) + 1.0f;
       bound = fmaxf(largest - deepest / per, kLowest);
+      octave = (float)(kBins - 1) / fmaxf(deepest, 1.0f);
     }
+    const float step = 1.0f / octave;
+    auto bin_of = [&](float x, float *nearest) {
+      const float r = fminf(depth(x) * octave, (float)(kBins - 1)) + kRound;
+      *nearest = r - kRound;
+      return (int)(__float_as_uint(r) & 0x3ffu);
+    };
     clear_hist();
-    for_above(bound, [&](float x, int i) {
-      if (!kept(x, i)) return;
-      const int bin = bin_of(x);
-      count_in(bin, weigh ? pow2((float)bin / kPerOctave - depth(x)) : 0.0f, weigh);
+    for_above(bound, [&](const float (&x)[4], int i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float nearest;
+        const int bin = bin_of(x[j], &nearest);
+        count_in(x[j] >= bound && kept(x[j], i + j), bin, weigh ? pow2(fmaf(nearest, step, -depth(x[j]))) : 0.0f, weigh);
+      }
     });
-    cluster_sync();
+    meet();
     const double target = weigh ? (double)fmaxf(p, 0.0f) * whole : (double)k;
-    int border = find_border(weigh, target, 0.0, 0.0, [&](int bin) { return exp2(-(double)bin / kPerOctave); });
+    const int border = find_border(sh, weigh, target, 0, 0.0, step);
     if (border < 0) {  // all that is there is kept
-      cluster_sync();  // the histograms are read
+      meet();  // the histograms are read
       continue;
     }
-    int n_before = sh.n_before, n_in = sh.n_in;
+    uint32_t n_before = sh.n_before;
     double s_before = sh.s_before;
-    // (no logit of the border's bin is below this: the bin's own end, less rounding)
-    const float deep = border == kBins - 1 ? INFINITY : (float)(border + 1) / kPerOctave;
-    const float near = fmaxf(bound, fmaxf(largest - deep / per * 1.0001f - fabsf(largest) * 1e-6f, kLowest));
-    if (n_before + n_in <= kList) {
-      // what may be kept fits one CTA, which does the rest
-      const int n = n_before + n_in;
-      for_above(near, [&](float x, int i) {
-        if (kept(x, i) && bin_of(x) <= border) gather(x, i, 1 + which);
-      });
-      cluster_sync();
-      if (rank == 0) finish_list(n, weigh ? n : min(n, k), weigh ? whole : 0.0);
-      return;
-    }
-    // Else the border itself is found, in the border's bin alone: by ever finer
-    // histograms of the ordered logits until its tokens fit the list or are equal.
-    uint32_t lo = 0xffffffffu, hi = 0;
-    for_above(near, [&](float x, int i) {
-      if (!kept(x, i) || bin_of(x) != border) return;
-      lo = min(lo, ordered(x));
-      hi = max(hi, ordered(x));
-    });
-    lo = __reduce_min_sync(0xffffffffu, lo);
-    hi = __reduce_max_sync(0xffffffffu, hi);
-    __syncthreads();
-    if (lane == 0) {
-      sh.counts[warp] = lo;
-      sh.best[warp].i = (int)hi;
-    }
-    __syncthreads();
-    lo = __reduce_min_sync(0xffffffffu, sh.counts[lane % kWarps]);
-    hi = __reduce_max_sync(0xffffffffu, (uint32_t)sh.best[lane % kWarps].i);
-    tell(lo, hi, 0, 0);
-    lo = __reduce_min_sync(0xffffffffu, heard(0, lane % kCluster));
-    hi = __reduce_max_sync(0xffffffffu, heard(1, lane % kCluster));
-    while (n_in > kList && lo < hi) {
+    // The logits [lo, hi] of the border's bin, ordered: a bin is a step of a falling
+    // function, whose ends a warp finds 32 at a time.
+    auto first_below = [&](int end) {  // the lowest ordered logit whose bin is below `end`
+      uint32_t at = ordered(bound), above = ordered(largest) + 1;  // in (at - 1, above]
+      while (at < above) {
+        const uint32_t part = (above - at) / 33 + 1, mine = at + lane * part;
+        float nearest;
+        const bool in = mine < above && bin_of(unordered(mine), &nearest) >= end;
+        const int n = __popc(__ballot_sync(0xffffffffu, in));  // the lanes' first n
+        if (n < 32 && at + n * part < above) above = at + n * part;
+        if (n > 0) at = at + (n - 1) * part + 1;
+      }
+      return at;
+    };
+    uint32_t lo = first_below(border + 1), hi = first_below(border) - 1;
+    // By ever finer histograms, until the tokens there fit the list or are equal.
+    bool all_of_it = false;
+    uint32_t n_in = 0;
+    while (true) {
+      const float low = unordered(lo), high = unordered(hi);
+      n_in = gather(low, false, [&](float x, int i) { return x <= high && kept(x, i); });  // (the histograms are read)
+      if (n_in <= (uint32_t)kList || lo == hi) break;
       const int shift = max(0, 32 - __clz((int)(hi - lo)) - 8);
-      const float d0 = depth(unordered(hi));
-      cluster_sync();  // the histograms are read
+      const float d0 = depth(high);
       clear_hist();
-      for_above(near, [&](float x, int i) {
-        const uint32_t u = ordered(x);
-        if (u < lo || u > hi || !kept(x, i)) return;
-        count_in((int)((hi - u) >> shift), weigh ? pow2(d0 - depth(x)) : 0.0f, weigh);
+      for_above(low, [&](const float (&x)[4], int i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          count_in(x[j] >= low && x[j] <= high && kept(x[j], i + j), (int)(min(hi - ordered(x[j]), hi - lo) >> shift),
+                   weigh ? pow2(d0 - depth(x[j])) : 0.0f, weigh);
       });
-      cluster_sync();
-      const double scale = exp2(-(double)d0);
-      border = find_border(weigh, target, (double)n_before, s_before, [&](int) { return scale; });
-      if (border < 0) {  // (rounding has the whole bin short of the target: it is kept whole)
-        hi = lo;
-        n_in = 0;
+      meet();
+      const double scale = (double)pow2(-d0);
+      const int finer = find_border(sh, weigh, weigh ? (target - s_before) / scale : target, weigh ? 0 : n_before, 0.0, 0.0f);
+      if (finer < 0) {  // (rounding has the whole bin short of the target)
+        all_of_it = true;
         break;
       }
-      n_before += sh.n_before;
-      n_in = sh.n_in;
-      s_before = sh.s_before;
-      hi -= (uint32_t)border << shift;
+      n_before = sh.n_before;
+      s_before += weigh ? sh.s_before * scale : 0.0;
+      hi -= (uint32_t)finer << shift;
       if (hi - lo >= 1u << shift) lo = hi - ((1u << shift) - 1);
     }
-    if (n_in == 0) {
-      cut = lo;
-      cut_index = 0xffffffffu;
-    } else if (n_in <= kList) {
-      for_above(near, [&](float x, int i) {
-        const uint32_t u = ordered(x);
-        if (u >= lo && u <= hi && kept(x, i)) gather(x, i, 1 + which);
-      });
-      cluster_sync();
+    if (all_of_it) {
+      cut = unordered(lo);
+      cut_index = 0x7fffffff;
+    } else if (n_in <= (uint32_t)kList) {
       if (rank == 0) {
-        sort_list(n_in);
-        float x[kMine], w[kMine];
-        double run = s_before + list_sums(n_in, x, w);
-        if (tid == 0) sh.border = weigh ? n_in - 1 : min(n_in - 1, k - 1 - n_before);
+        const unsigned long long mine = sorted(sh, (int)n_in, listed((int)n_in));
+        const bool in = tid < (int)n_in;
+        const float x = unordered(~(uint32_t)(mine >> 32)), w = in ? pow2(-depth(x)) : 0.0f;
+        if (tid == 0) sh.border = weigh ? (int)n_in - 1 : min((int)n_in, k - (int)n_before) - 1;
+        const double run = s_before + before_in_list(w) + w;  // (meets)
+        if (weigh && in && run >= target) atomicMin(&sh.border, tid);
         __syncthreads();
-        if (weigh) {
-#pragma unroll
-          for (int j = 0; j < kMine; ++j) {
-            run += w[j];
-            if (tid * kMine + j < n_in && run >= target) atomicMin(&sh.border, tid * kMine + j);
+        if (tid == max(0, sh.border))
+          for (int r = 0; r < kCluster; ++r) {
+            peer_store(&sh.cut, r, __float_as_uint(x));
+            peer_store(&sh.cut_index, r, (uint32_t)mine);
           }
-          __syncthreads();
-        }
-        const unsigned long long last = sh.list[sh.border];
-        if (tid < kCluster) {
-          peer_store(&sh.cut, tid, ~(uint32_t)(last >> 32));
-          peer_store(&sh.cut_index, tid, (uint32_t)last);
-        }
       }
-      cluster_sync();
+      meet();
       cut = sh.cut;
       cut_index = sh.cut_index;
     } else {
       // equal logits: as many of them as are wanted, by index
-      const double each = (double)pow2(-depth(unordered(lo)));
-      int wanted = weigh ? (int)fmin(fmax(ceil((target - s_before) / each), 1.0), (double)n_in) : k - n_before;
-      wanted = max(1, min(wanted, n_in));
+      const float equal = unordered(lo);
+      const double each = (double)pow2(-depth(equal));
+      int wanted = weigh ? (int)fmin(fmax(ceil((target - s_before) / each), 1.0), (double)n_in) : k - (int)n_before;
+      wanted = max(1, min(wanted, (int)n_in));
       const int chunk = (len + kThreads - 1) / kThreads, i0 = min(len, tid * chunk), i1 = min(len, i0 + chunk);
       int mine = 0;
-      for (int i = i0; i < i1; ++i) mine += ordered(xs[i]) == lo && kept(xs[i], i);
+      for (int i = i0; i < i1; ++i) mine += xs[i] == equal && kept(equal, i);
       int run = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -649,94 +641,113 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         if (i < warp) before += sh.counts[i];
         all += sh.counts[i];
       }
-      tell((uint32_t)all, 0, 0, 0);
+      tell((uint32_t)all, 0, 0, 0, 0);
       for (int r = 0; r < (int)rank; ++r) before += heard(0, r);
       if (before < wanted && before + mine >= wanted) {
         int n = before, i = i0;
         for (;; ++i)
-          if (ordered(xs[i]) == lo && kept(xs[i], i) && ++n == wanted) break;
+          if (xs[i] == equal && kept(equal, i) && ++n == wanted) break;
         for (int r = 0; r < kCluster; ++r) peer_store(&sh.cut_index, r, (uint32_t)(v0 + i));
       }
-      cluster_sync();
-      cut = lo;
+      meet();
+      cut = equal;
       cut_index = sh.cut_index;
     }
-    cluster_sync();  // what the CTAs told one another here is read
+    meet();  // what the CTAs told one another here is read
   }
 
   // The race over what is kept: the best of four tokens at a time, and in the end
   // which of a thread's best four it was.
   float best = 0.0f, part = 0.0f;
   int at = -1;
-  if (plain && a.noise_vec) {
-#pragma unroll 2
-    for (int i = tid * 4; i < len; i += kThreads * 4) {
-      const float4 x = *reinterpret_cast<const float4 *>(xs + i);
-      float4 e = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-      if (i + 4 <= len) {
-        e = __ldg(reinterpret_cast<const float4 *>(noise + i));
-      } else {
-        e.x = __ldg(noise + i);
-        if (i + 1 < len) e.y = __ldg(noise + i + 1);
-        if (i + 2 < len) e.z = __ldg(noise + i + 2);
+  const float deep = least > 0.0f ? -log2f(least) : INFINITY;
+  const float bound = fmaxf(fmaxf(cut, largest - deep / per * 1.0001f - fabsf(largest) * 1e-6f), kLowest);
+  auto weight = [&](float x, int i) {  // 0: not kept
+    const float w = pow2(-depth(x));
+    return x >= bound && w >= least && kept(x, i) ? w : 0.0f;
+  };
+  constexpr int kFew = 3;
+  for (int i0 = tid * 4; i0 - lane * 4 < len; i0 += kFew * kThreads * 4) {
+    float4 x[kFew], e[kFew];
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < kFew; ++j) {
+      const int i = i0 + j * kThreads * 4;
+      x[j] = i < len ? *reinterpret_cast<const float4 *>(xs + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      const bool hit = fmaxf(fmaxf(x[j].x, x[j].y), fmaxf(x[j].z, x[j].w)) >= bound;
+      any |= hit;
+      e[j] = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+      if (hit && a.noise_vec && i + 4 <= len) {
+        e[j] = __ldg(reinterpret_cast<const float4 *>(noise + i));
+      } else if (hit) {
+        e[j].x = __ldg(noise + i);
+        if (i + 1 < len) e[j].y = __ldg(noise + i + 1);
+        if (i + 2 < len) e[j].z = __ldg(noise + i + 2);
+        if (i + 3 < len) e[j].w = __ldg(noise + i + 3);
       }
-      const float w[4] = {pow2(-depth(x.x)), pow2(-depth(x.y)), pow2(-depth(x.z)), pow2(-depth(x.w))};
+    }
+    if (!__any_sync(0xffffffffu, any)) continue;
+#pragma unroll
+    for (int j = 0; j < kFew; ++j) {
+      const int i = i0 + j * kThreads * 4;
+      const float w[4] = {weight(x[j].x, i), weight(x[j].y, i + 1), weight(x[j].z, i + 2), weight(x[j].w, i + 3)};
       part += (w[0] + w[1]) + (w[2] + w[3]);
-      const float v = fmaxf(fmaxf(__fdividef(w[0], e.x), __fdividef(w[1], e.y)),
-                            fmaxf(__fdividef(w[2], e.z), __fdividef(w[3], e.w)));
+      const float v = fmaxf(fmaxf(__fdividef(w[0], e[j].x), __fdividef(w[1], e[j].y)),
+                            fmaxf(__fdividef(w[2], e[j].z), __fdividef(w[3], e[j].w)));
       if (v > best) {
         best = v;
         at = i;
       }
     }
-  } else {
-    const float deep = least > 0.0f ? -log2f(least) : INFINITY;
-    const float bound = fmaxf(fmaxf(cut ? unordered(cut) : kLowest, largest - deep / per * 1.0001f - fabsf(largest) * 1e-6f),
-                              kLowest);
-    for_above(bound, [&](float x, int i) {
-      const float w = pow2(-depth(x));
-      if (w < least || !kept(x, i)) return;
-      part += w;
-      const float v = __fdividef(w, __ldg(noise + i));
-      if (v > best) {
-        best = v;
-        at = i & ~3;
-      }
-    });
   }
   Best pick{0.0f, top.i};
   float pick_x = largest;
   if (at >= 0) {
-    pick = Best{-1.0f, 0};
+    pick.v = -1.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int i = at + j;
-      const float x = i < len ? xs[i] : -INFINITY, w = pow2(-depth(x));
-      if (x == -INFINITY || w < least || !kept(x, i)) continue;
-      const float v = __fdividef(w, __ldg(noise + i));
+      const float x = i < len ? xs[i] : -INFINITY, w = weight(x, i);
+      const float v = w > 0.0f ? __fdividef(w, __ldg(noise + i)) : -1.0f;
       if (v > pick.v) {
         pick = Best{v, v0 + i};
         pick_x = x;
       }
     }
   }
-  const double mine_s = block_sum((double)part);
-  const Best mine = pick;
-  pick = block_best(pick);
-  if (mine.i == pick.i) sh.pick_x = pick_x;
+  // the warps' best, with its logit, and sums meet
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const Best y{__shfl_xor_sync(0xffffffffu, pick.v, o), __shfl_xor_sync(0xffffffffu, pick.i, o)};
+    const float y_x = __shfl_xor_sync(0xffffffffu, pick_x, o);
+    const Best z = better(pick, y);
+    if (z.i != pick.i) pick_x = y_x;
+    pick = z;
+  }
+  part = warp_total(part);
   __syncthreads();
-  const unsigned long long bits = __double_as_longlong(mine_s);
-  if (tid < kCluster) peer_store(&sh.list[rank], tid, bits);
-  tell(__float_as_uint(pick.v), (uint32_t)pick.i, __float_as_uint(sh.pick_x), 0);
+  if (lane == 0) {
+    sh.best[warp] = pick;
+    sh.last_x[warp] = pick_x;
+    sh.last_sum[warp] = part;
+  }
+  __syncthreads();
+  double mine_s = 0.0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    const Best z = better(pick, sh.best[i]);
+    if (z.i != pick.i) pick_x = sh.last_x[i];
+    pick = z;
+    mine_s += sh.last_sum[i];
+  }
+  tell_best(pick, mine_s, __float_as_uint(pick_x));
   pick = best_of_all();
+  const double all = heard_sum();
   if (rank == 0 && tid == 0) {
-    double s = 0.0;
     float x = 0.0f;
-    for (int r = 0; r < kCluster; ++r) {
-      s += __longlong_as_double(sh.list[r]);
-      if ((int)heard(1, r) == pick.i) x = __uint_as_float(heard(2, r));
-    }
-    answer(pick.i, x, s);
+    for (int r = 0; r < kCluster; ++r)
+      if ((int)heard(1, r) == pick.i) x = __uint_as_float(heard(4, r));
+    answer(pick.i, x, all);
   }
 }
 
