@@ -53,9 +53,15 @@ __device__ __forceinline__ float pow2(float x) {
   return y;
 }
 
-// Order of f32 values as that of whole numbers, and back.
+__device__ __forceinline__ float inverse(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Order of f32 values as that of whole numbers (the zeros are one), and back.
 __device__ __forceinline__ uint32_t ordered(float x) {
-  const uint32_t u = __float_as_uint(x);
+  const uint32_t u = __float_as_uint(x + 0.0f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float unordered(uint32_t u) {
@@ -76,9 +82,9 @@ __device__ __forceinline__ unsigned long long peer_load(const unsigned long long
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(peer_address(p, rank)) : "memory");
   return v;
 }
-__device__ __forceinline__ uint2 peer_load(const uint2 *p, unsigned rank) {
-  uint2 v;
-  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(peer_address(p, rank)) : "memory");
+__device__ __forceinline__ uint32_t peer_load(const uint32_t *p, unsigned rank) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer_address(p, rank)) : "memory");
   return v;
 }
 // cluster_sync() behind code that lanes may leave apart: its barrier counts whole warps.
@@ -103,7 +109,7 @@ __device__ __forceinline__ V warp_total(V v) {
 
 struct Shared {
   unsigned long long list[kList];  // tokens to be ordered, (falling logit, index) as one number
-  uint2 hist[kBins];               // x: tokens, or the low part of their weights' sum; y: its high part
+  uint32_t hist[kBins];            // tokens, or their weights
   // what the CTAs tell one another; the halves alternate, so that one exchange's
   // reads may overlap the next one's stores
   uint32_t got[2][5][kCluster];
@@ -111,8 +117,8 @@ struct Shared {
   double sums[kWarps];
   uint32_t counts[kWarps];
   Best best[kWarps];
-  int border;  // where a histogram reaches its target: the bin, tokens and weights before it, tokens in it
-  uint32_t n_before, n_in;
+  int border;  // where a histogram reaches its target: the bin, tokens or weights before it
+  uint32_t n_before;
   double s_before;
   uint32_t listed[kLists];  // tokens in the list, each time anew
   float cut;
@@ -150,22 +156,21 @@ __device__ __noinline__ unsigned long long sorted(Shared &sh, int n, unsigned lo
 }
 
 // Over the cluster's histograms: the first bin at which the running count (from n0
-// on), or weight (from s0 on; bin i's whole numbers times 2^-20 and 2^-(i * step)),
+// on), or weight (from s0 on; bin i's numbers times `unit` and 2^-(i * step)),
 // reaches the target (-1: none), with what lies before it.  Every CTA finds the
 // same.  Two threads a bin, four CTAs' each.
-__device__ __noinline__ int find_border(Shared &sh, bool weigh, double target, uint32_t n0, double s0, float step) {
+__device__ __noinline__ int find_border(Shared &sh, bool weigh, double target, uint32_t n0, double s0, double unit,
+                                        float step) {
   static_assert(kThreads == 2 * kBins && kCluster == 8);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bin = tid >> 1, from = 4 * (tid & 1);
-  uint2 x[4];
+  unsigned long long f = 0;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) x[r] = peer_load(&sh.hist[bin], from + r);
-  uint32_t c = x[0].x + x[1].x + x[2].x + x[3].x;
-  unsigned long long f = c + ((unsigned long long)x[0].y + x[1].y + x[2].y + x[3].y << 11);
-  c += __shfl_xor_sync(0xffffffffu, c, 1);
+  for (int r = 0; r < 4; ++r) f += peer_load(&sh.hist[bin], from + r);
   f += __shfl_xor_sync(0xffffffffu, f, 1);
+  uint32_t c = weigh ? 0 : (uint32_t)f;
   const bool one = (tid & 1) == 0;
   if (!one) c = 0;
-  const double v = weigh && one ? (double)f * 0x1p-20 * (double)pow2(-(float)bin * step) : 0.0;
+  const double v = weigh && one ? (double)f * unit * (double)pow2(-(float)bin * step) : 0.0;
   // running count and sum over the bins
   uint32_t n = c;
   double run = v;
@@ -193,7 +198,6 @@ __device__ __noinline__ int find_border(Shared &sh, bool weigh, double target, u
   const int border = sh.border;
   if (one && bin == border) {
     sh.n_before = n0 + n - c;
-    sh.n_in = c;
     sh.s_before = s0 + run - v;
   }
   __syncthreads();
@@ -378,17 +382,39 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     const float theirs = fmaxf(__uint_as_float(heard(0, lane % kCluster)), kLowest);
     whole = over_ctas(heard_double(lane % kCluster) * (double)pow2(-depth(theirs)));
   }
-  // What is kept so far: logits above `cut`, and of those equal to it the tokens up to
-  // `cut_index`.
-  float cut = -INFINITY;
+  // What is kept so far: logits above `cut`, and those equal to it up to the slice's
+  // token `cut_index`.
+  float cut = -INFINITY, above_cut = -INFINITY;
   int cut_index = -1;
-  auto kept = [&](float x, int i) { return x > cut || (x == cut && v0 + i <= cut_index); };
-  // f(x, i) for the slice's logits x[0, 4) from i on where one is `bound` (finite) or
-  // above
+  auto set_cut = [&](float x, int token) {
+    cut = x;
+    above_cut = unordered(ordered(x) + 1);
+    cut_index = token - v0;
+  };
+  auto kept = [&](float x, int i) { return x > cut || (x == cut && i <= cut_index); };
+  // four of the slice's logits; -inf where they are not kept
+  auto load4 = [&](int i) {
+    float4 y = *reinterpret_cast<const float4 *>(xs + i);
+    if (cut > -INFINITY) {
+      const float from = i <= cut_index ? cut : above_cut;
+      y.x = y.x >= from ? y.x : -INFINITY;
+      y.y = y.y >= from ? y.y : -INFINITY;
+      y.z = y.z >= from ? y.z : -INFINITY;
+      y.w = y.w >= from ? y.w : -INFINITY;
+      if (i <= cut_index && cut_index < i + 3) {
+        if (i + 1 > cut_index && y.y == cut) y.y = -INFINITY;
+        if (i + 2 > cut_index && y.z == cut) y.z = -INFINITY;
+        if (y.w == cut) y.w = -INFINITY;
+      }
+    }
+    return y;
+  };
+  // f(x, i) for the slice's kept logits x[0, 4) from i on where one is `bound`
+  // (finite) or above
   auto for_above = [&](float bound, auto f) {
 #pragma unroll 2
     for (int i = tid * 4; i < len; i += kThreads * 4) {
-      const float4 y = *reinterpret_cast<const float4 *>(xs + i);
+      const float4 y = load4(i);
       const float x[4] = {y.x, y.y, y.z, y.w};
       if (fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= bound) f(x, i);
     }
@@ -484,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       const double before = by_p ? before_in_list(w) : 0.0;
       if (by_k && by_p) whole = block_sum(w);
       const bool in = tid < most && (tid == 0 || !by_p || before < (double)p * whole) && w >= least;
-      const Best pick = block_best(in ? Best{__fdividef(w, e), token} : Best{0.0f, top.i});
+      const Best pick = block_best(in ? Best{w * inverse(e), token} : Best{0.0f, top.i});
       const double s = block_sum(in ? w : 0.0f);
       if (tid < most && token == pick.i) answer(token, x, s);
       __syncwarp();
@@ -494,20 +520,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   }
 
   // Weights go to a histogram as whole numbers, relative to their bin's, so that
-  // their sum does not depend on the order: 22 bits in two parts of 11 (49152 of
-  // them fit 32 bits).  A bin is a nearest whole number: its own add to 1.5 * 2^23
-  // has it in the low bits (conversions take as long as a power).
+  // their sum does not depend on the order: as many bits as leave room for the whole
+  // slice in a word (17 for 151936 tokens: off by 2^-18 of themselves at most, so
+  // that top-p's border is to within that of the row's sum).  A bin is a nearest
+  // whole number: added to 1.5 * 2^23 it lies in the low bits, as the weight does
+  // added to 2^23 (conversions take as long as a power, and a word's atomic longer
+  // than the rest: with two words 22 bits are kept and a flat row takes 5 us more).
   constexpr float kRound = 12582912.0f;
+  const float units = fminf(3.5e9f / (float)a.slice, 4.0e6f);
   auto count_in = [&](bool ok, int bin, float u, bool weigh) {
-    const uint32_t f = __float_as_uint(fmaf(u, 0.125f, 1.0f)) & 0x7fffffu;  // u * 2^20
-    add_if(ok, &sh.hist[bin].x, weigh ? f & 0x7ffu : 1u);
-    add_if(ok && weigh, &sh.hist[bin].y, f >> 11);
+    add_if(ok, &sh.hist[bin], weigh ? __float_as_uint(fmaf(u, units, 8388608.0f)) & 0x7fffffu : 1u);
   };
   auto clear_hist = [&]() {
-    reinterpret_cast<uint32_t *>(sh.hist)[tid] = 0;
+    if (tid < kBins) sh.hist[tid] = 0;
     __syncthreads();
   };
-  static_assert(kThreads == 2 * kBins);
   if (by_p) want_noise();  // much of it: more is kept than fits the list
 
   for (int which = 0; which < 2; ++which) {
@@ -517,9 +544,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     if (weigh) {
       if (by_k) {  // of what top-k kept
         float part = 0.0f;
-        for_above(kLowest, [&](const float (&x)[4], int i) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) part += kept(x[j], i + j) ? pow2(-depth(x[j])) : 0.0f;
+        for_above(kLowest, [&](const float (&x)[4], int) {
+          part += (pow2(-depth(x[0])) + pow2(-depth(x[1]))) + (pow2(-depth(x[2])) + pow2(-depth(x[3])));
         });
         tell_best(top, block_sum(part), 0);
         whole = heard_sum();
@@ -537,17 +563,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       return (int)(__float_as_uint(r) & 0x3ffu);
     };
     clear_hist();
-    for_above(bound, [&](const float (&x)[4], int i) {
+    for_above(bound, [&](const float (&x)[4], int) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float nearest;
         const int bin = bin_of(x[j], &nearest);
-        count_in(x[j] >= bound && kept(x[j], i + j), bin, weigh ? pow2(fmaf(nearest, step, -depth(x[j]))) : 0.0f, weigh);
+        count_in(x[j] >= bound, bin, weigh ? pow2(fmaf(nearest, step, -depth(x[j]))) : 0.0f, weigh);
       }
     });
     meet();
     const double target = weigh ? (double)fmaxf(p, 0.0f) * whole : (double)k;
-    const int border = find_border(sh, weigh, target, 0, 0.0, step);
+    const int border = find_border(sh, weigh, target, 0, 0.0, 1.0 / (double)units, step);
     if (border < 0) {  // all that is there is kept
       meet();  // the histograms are read
       continue;
@@ -557,10 +583,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     // The logits [lo, hi] of the border's bin, ordered: a bin is a step of a falling
     // function, whose ends a warp finds 32 at a time.
     auto first_below = [&](int end) {  // the lowest ordered logit whose bin is below `end`
-      uint32_t at = ordered(bound), above = ordered(largest) + 1;  // in (at - 1, above]
+      // (it lies near the bins' border, or at an end; in [at, above])
+      const float near = largest - ((float)end - 0.5f) * step / per, slack = fabsf(near) * 1e-6f + fabsf(largest) * 1e-6f;
+      uint32_t at = ordered(bound), above = ordered(largest) + 1;
+      float nearest;
+      const uint32_t low = ordered(fminf(fmaxf(near - slack, bound), largest)), high = ordered(fminf(fmaxf(near + slack, bound), largest));
+      if (bin_of(unordered(low), &nearest) >= end) at = low; else above = low;
+      if (high >= at && high < above) {
+        if (bin_of(unordered(high), &nearest) >= end) at = high; else above = high;
+      }
       while (at < above) {
-        const uint32_t part = (above - at) / 33 + 1, mine = at + lane * part;
-        float nearest;
+        const uint32_t part = ((above - at) >> 5) + 1, mine = at + lane * part;
         const bool in = mine < above && bin_of(unordered(mine), &nearest) >= end;
         const int n = __popc(__ballot_sync(0xffffffffu, in));  // the lanes' first n
         if (n < 32 && at + n * part < above) above = at + n * part;
@@ -574,20 +607,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     uint32_t n_in = 0;
     while (true) {
       const float low = unordered(lo), high = unordered(hi);
-      n_in = gather(low, false, [&](float x, int i) { return x <= high && kept(x, i); });  // (the histograms are read)
+      n_in = gather(low, false, [&](float x, int) { return x <= high; });  // (the histograms are read)
       if (n_in <= (uint32_t)kList || lo == hi) break;
       const int shift = max(0, 32 - __clz((int)(hi - lo)) - 8);
       const float d0 = depth(high);
       clear_hist();
-      for_above(low, [&](const float (&x)[4], int i) {
+      for_above(low, [&](const float (&x)[4], int) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          count_in(x[j] >= low && x[j] <= high && kept(x[j], i + j), (int)(min(hi - ordered(x[j]), hi - lo) >> shift),
+          count_in(x[j] >= low && x[j] <= high, (int)(min(hi - ordered(x[j]), hi - lo) >> shift),
                    weigh ? pow2(d0 - depth(x[j])) : 0.0f, weigh);
       });
       meet();
       const double scale = (double)pow2(-d0);
-      const int finer = find_border(sh, weigh, weigh ? (target - s_before) / scale : target, weigh ? 0 : n_before, 0.0, 0.0f);
+      const int finer = find_border(sh, weigh, weigh ? (target - s_before) / scale : target, weigh ? 0 : n_before, 0.0,
+                                    1.0 / (double)units, 0.0f);
       if (finer < 0) {  // (rounding has the whole bin short of the target)
         all_of_it = true;
         break;
@@ -598,8 +632,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       if (hi - lo >= 1u << shift) lo = hi - ((1u << shift) - 1);
     }
     if (all_of_it) {
-      cut = unordered(lo);
-      cut_index = 0x7fffffff;
+      set_cut(unordered(lo), 0x7fffffff);
     } else if (n_in <= (uint32_t)kList) {
       if (rank == 0) {
         const unsigned long long mine = sorted(sh, (int)n_in, listed((int)n_in));
@@ -616,8 +649,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           }
       }
       meet();
-      cut = sh.cut;
-      cut_index = sh.cut_index;
+      set_cut(sh.cut, sh.cut_index);
     } else {
       // equal logits: as many of them as are wanted, by index
       const float equal = unordered(lo);
@@ -650,8 +682,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         for (int r = 0; r < kCluster; ++r) peer_store(&sh.cut_index, r, (uint32_t)(v0 + i));
       }
       meet();
-      cut = equal;
-      cut_index = sh.cut_index;
+      set_cut(equal, sh.cut_index);
     }
     meet();  // what the CTAs told one another here is read
   }
@@ -662,9 +693,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   int at = -1;
   const float deep = least > 0.0f ? -log2f(least) : INFINITY;
   const float bound = fmaxf(fmaxf(cut, largest - deep / per * 1.0001f - fabsf(largest) * 1e-6f), kLowest);
-  auto weight = [&](float x, int i) {  // 0: not kept
+  auto weight = [&](float x) {  // 0: not kept
     const float w = pow2(-depth(x));
-    return x >= bound && w >= least && kept(x, i) ? w : 0.0f;
+    return w >= least ? w : 0.0f;
   };
   constexpr int kFew = 3;
   for (int i0 = tid * 4; i0 - lane * 4 < len; i0 += kFew * kThreads * 4) {
@@ -673,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 #pragma unroll
     for (int j = 0; j < kFew; ++j) {
       const int i = i0 + j * kThreads * 4;
-      x[j] = i < len ? *reinterpret_cast<const float4 *>(xs + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      x[j] = i < len ? load4(i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
       const bool hit = fmaxf(fmaxf(x[j].x, x[j].y), fmaxf(x[j].z, x[j].w)) >= bound;
       any |= hit;
       e[j] = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
@@ -690,10 +721,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 #pragma unroll
     for (int j = 0; j < kFew; ++j) {
       const int i = i0 + j * kThreads * 4;
-      const float w[4] = {weight(x[j].x, i), weight(x[j].y, i + 1), weight(x[j].z, i + 2), weight(x[j].w, i + 3)};
+      const float w[4] = {weight(x[j].x), weight(x[j].y), weight(x[j].z), weight(x[j].w)};
       part += (w[0] + w[1]) + (w[2] + w[3]);
-      const float v = fmaxf(fmaxf(__fdividef(w[0], e[j].x), __fdividef(w[1], e[j].y)),
-                            fmaxf(__fdividef(w[2], e[j].z), __fdividef(w[3], e[j].w)));
+      const float v = fmaxf(fmaxf(w[0] * inverse(e[j].x), w[1] * inverse(e[j].y)),
+                            fmaxf(w[2] * inverse(e[j].z), w[3] * inverse(e[j].w)));
       if (v > best) {
         best = v;
         at = i;
@@ -704,14 +735,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   float pick_x = largest;
   if (at >= 0) {
     pick.v = -1.0f;
+    const float4 y = load4(at);
+    const float x[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int i = at + j;
-      const float x = i < len ? xs[i] : -INFINITY, w = weight(x, i);
-      const float v = w > 0.0f ? __fdividef(w, __ldg(noise + i)) : -1.0f;
+      const float w = weight(x[j]), v = w > 0.0f ? w * inverse(__ldg(noise + at + j)) : -1.0f;
       if (v > pick.v) {
-        pick = Best{v, v0 + i};
-        pick_x = x;
+        pick = Best{v, v0 + at + j};
+        pick_x = x[j];
       }
     }
   }
