@@ -118,7 +118,7 @@ struct Shared {
   uint32_t counts[kWarps];
   Best best[kWarps];
   int border;  // where a histogram reaches its target: the bin, tokens or weights before it
-  uint32_t n_before;
+  uint32_t n_before, n_in;  // n_in: tokens in it, or about as many
   double s_before;
   uint32_t listed[kLists];  // tokens in the list, each time anew
   float cut;
@@ -198,6 +198,7 @@ __device__ __noinline__ int find_border(Shared &sh, bool weigh, double target, u
   const int border = sh.border;
   if (one && bin == border) {
     sh.n_before = n0 + n - c;
+    sh.n_in = weigh ? (uint32_t)((double)f * unit) : c;  // (a weight relative to its bin's is about 1)
     sh.s_before = s0 + run - v;
   }
   __syncthreads();
@@ -604,11 +605,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     uint32_t lo = first_below(border + 1), hi = first_below(border) - 1;
     // By ever finer histograms, until the tokens there fit the list or are equal.
     bool all_of_it = false;
-    uint32_t n_in = 0;
+    uint32_t n_in = sh.n_in;
     while (true) {
       const float low = unordered(lo), high = unordered(hi);
-      n_in = gather(low, false, [&](float x, int) { return x <= high; });  // (the histograms are read)
-      if (n_in <= (uint32_t)kList || lo == hi) break;
+      if (n_in <= (uint32_t)kList || lo == hi) {
+        n_in = gather(low, false, [&](float x, int) { return x <= high; });  // (meets: the histograms are read)
+        if (n_in <= (uint32_t)kList || lo == hi) break;
+      } else {
+        meet();
+      }
       const int shift = max(0, 32 - __clz((int)(hi - lo)) - 8);
       const float d0 = depth(high);
       clear_hist();
@@ -627,6 +632,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         break;
       }
       n_before = sh.n_before;
+      n_in = sh.n_in;
       s_before += weigh ? sh.s_before * scale : 0.0;
       hi -= (uint32_t)finer << shift;
       if (hi - lo >= 1u << shift) lo = hi - ((1u << shift) - 1);
