@@ -25,7 +25,7 @@ struct PagedArgs {
   int box;     // tokens of a copy: the largest power of two that divides the page size, up to a step's
   int tiles;   // row tiles of a kv head's query heads
   int slots;   // blocks that the GPU has room for
-  int waves;   // 0: as many blocks as there is room for; else shares of 1 / (waves * slots) of the steps, and the rest
+  int waves;   // 0: no more blocks than that; else shares of 1 / (waves * slots) of the steps
   float scale_log2;  // scale * log2(e): scores and maxima are held in powers of two
   void *out;
   int out_bf16;
@@ -35,7 +35,7 @@ struct PagedArgs {
   int *error;
 };
 
-constexpr int kPagedThreads = 128, kPagedWarps = 4, kPagedMaxBatch = 4096, kPagedWaves = 4;
+constexpr int kPagedMaxBatch = 4096, kPagedWaves = 4;
 constexpr int kErrPagedWait = 503;
 // The maximum may lag by kLag (powers of two) before the sums are rescaled, and
 // weights are held as 2^(y - m - kBack): 2^20 of them times a value of the type's
@@ -133,24 +133,32 @@ __device__ __forceinline__ void store_out(const PagedArgs &a, int b, int h, int 
 // then reads 16 bytes from all of the banks.
 __device__ __forceinline__ int token_at(int i) { return (i >> 1) | (i & 1) << 2; }
 
-template <typename T, int DP, int NR>
+// Blocks of W warps.  Where the calls' blocks are all there at once there is one an
+// SM, of 8 or 12 warps: smaller ones, two or three an SM, leave registers that do
+// not lie together when the kernel before is still there, and an SM then takes one
+// block less (3 x 100003 tokens behind another call 172 us, alone 106).  Where they
+// come one after another small blocks overlap their beginnings and ends.
+constexpr int warps_of(int DP, bool once) { return !once ? 4 : DP == 256 ? 8 : 12; }
+constexpr int blocks_of(int DP, bool once) { return once ? 1 : DP == 256 ? 2 : 3; }
+
+template <typename T, int DP, int NR, bool ONCE>
 struct PagedShape {
   static constexpr bool kHalf = sizeof(T) == 2;
+  static constexpr int W = warps_of(DP, ONCE), kThreads = 32 * W, kBlocks = blocks_of(DP, ONCE);
   static constexpr int kTok = kHalf ? 16 : 8;                       // tokens of a step
   static constexpr int kCols = 128 / (int)sizeof(T), kBoxes = DP / kCols;  // a copy's columns; copies side by side
   static constexpr uint32_t kPart = kTok * DP * sizeof(T);          // a step's keys, or its values
-  static constexpr int kBlocks = DP == 256 ? 2 : 3;                 // an SM
-  static constexpr int kParts = (DP == 256 ? 3 : DP == 128 ? 4 : 6) - (NR == 16);  // of a warp's ring
+  static constexpr int kParts = (DP == 256 ? 3 : DP == 128 ? 4 : 6) - (NR == 16 && !ONCE);  // of a warp's ring
   static constexpr bool kQShared = NR == 16 && DP >= 128;           // too many registers of queries beside those of sums
   static constexpr int kQPitch = DP + 32;                           // bf16 elements: 16-byte reads of eight rows on distinct banks
   static constexpr int kEndPitch = DP + 4;
-  static constexpr size_t kRing = (size_t)kPagedWarps * kParts * kPart;
-  static constexpr size_t kEnd = (size_t)kPagedWarps * NR * kEndPitch * 4;  // the warps' results, over the ring
-  static constexpr size_t kPlan = (size_t)kPagedMaxBatch * 4;               // the sessions' steps, over the ring
+  static constexpr size_t kRing = (size_t)W * kParts * kPart;
+  static constexpr size_t kEnd = (size_t)W * NR * kEndPitch * 4;  // the warps' results, over the ring
+  static constexpr size_t kPlan = (size_t)kPagedMaxBatch * 4;     // the sessions' steps, over the ring
   static constexpr size_t kOver = kRing > kEnd ? kRing : kEnd;
-  static constexpr size_t kQueries = kHalf ? (size_t)2 * NR * kQPitch * 2 : (size_t)kPagedWarps * 64 * 4;
+  static constexpr size_t kQueries = kHalf ? (size_t)2 * NR * kQPitch * 2 : (size_t)W * 64 * 4;
   static constexpr size_t smem = 1023 + kOver + kQueries;
-  static_assert(kPlan <= kOver && kBlocks * (smem + 3 * 1024) <= 228 * 1024);
+  static_assert(kPlan <= kOver && kBlocks * (smem + 4 * 1024) <= 228 * 1024);
 };
 
 // What a block does: steps [first, first + count) of a session's kv head and row tile.
@@ -164,15 +172,73 @@ struct PagedShare {
 // One wave: the smallest S whose shares the GPU has room for at once, among 32
 // between total / slots, which is below it, and total / (slots - items), whose
 // shares fit: each item rounds up by less than one.
+constexpr int kLeast = 4;  // steps of a share, at least
+
+// Up to 32 sessions: every warp finds the share on its own, a session a lane.
 template <int TOK>
+__device__ __forceinline__ bool paged_share_few(const PagedArgs &a, PagedShare *out) {
+  const int lane = threadIdx.x & 31, heads = a.kv_heads * a.tiles;
+  int n = lane < a.batch ? a.lengths[lane] : 0;
+  if (n < 0 || n > (long long)a.max_pages * a.page_size) {
+    if (blockIdx.x == 0 && threadIdx.x < 32 && a.error) atomicCAS(a.error, 0, kErrLength);
+    n = 0;
+  }
+  const int steps = n / TOK + (n % TOK != 0);
+  const uint32_t alive = __ballot_sync(0xffffffffu, steps > 0);
+  unsigned long long work = steps;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
+  work *= heads;
+  if (work == 0) return false;
+  int S;
+  if (a.waves) {
+    const unsigned long long all = (unsigned long long)a.waves * a.slots;
+    S = max(kLeast, (int)min((work + all - 1) / all, 0x7fffffffull));
+  } else {
+    const int items = __popc(alive) * heads;
+    const int lo = (int)((work + a.slots - 1) / a.slots), hi = (int)((work + a.slots - items - 1) / (a.slots - items));
+    const int trial = max(kLeast, lo + (int)((long long)(hi - lo) * lane / 31));
+    int blocks = 0;
+    for (int b = 0; b < a.batch; ++b) blocks += (__shfl_sync(0xffffffffu, steps, b) + trial - 1) / trial;
+    const uint32_t fits = __ballot_sync(0xffffffffu, blocks * heads <= a.slots);
+    S = __shfl_sync(0xffffffffu, trial, __ffs(fits) - 1);
+  }
+  const int parts = (steps + S - 1) / S, blocks = parts * heads, slots = parts > 1 ? blocks : 0;
+  int x = blocks, y = slots;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) {
+      x += u;
+      y += v;
+    }
+  }
+  const uint32_t mine = __ballot_sync(0xffffffffu, (int)blockIdx.x >= x - blocks && (int)blockIdx.x < x);
+  if (!mine) return false;
+  const int b = __ffs(mine) - 1, P = __shfl_sync(0xffffffffu, parts, b), total = __shfl_sync(0xffffffffu, steps, b);
+  const int at = (int)blockIdx.x - __shfl_sync(0xffffffffu, x - blocks, b);
+  out->b = b;
+  out->tile = at % a.tiles;
+  out->part = at / a.tiles % P;
+  out->parts = P;
+  out->kvh = at / a.tiles / P;
+  out->length = __shfl_sync(0xffffffffu, n, b);
+  out->first = (int)((long long)total * out->part / P);
+  out->count = (int)((long long)total * (out->part + 1) / P) - out->first;
+  out->slot = __shfl_sync(0xffffffffu, y - slots, b) + (out->kvh * a.tiles + out->tile) * P + out->part;
+  return true;
+}
+
+template <int TOK, int W>
 __device__ __forceinline__ bool paged_share(const PagedArgs &a, int *steps, PagedShare *out) {
-  __shared__ unsigned long long sum_s[kPagedWarps];
-  __shared__ int alive_s[kPagedWarps], blocks_s[kPagedWarps][32], found_s[4];
+  constexpr int kThreads = 32 * W;
+  __shared__ unsigned long long sum_s[W];
+  __shared__ int alive_s[W], blocks_s[W][32], found_s[4];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const long long most = (long long)a.max_pages * a.page_size;
   unsigned long long sum = 0;
   int alive = 0;
-  for (int b = tid; b < a.batch; b += kPagedThreads) {
+  for (int b = tid; b < a.batch; b += kThreads) {
     int n = a.lengths[b];
     if (n < 0 || n > most) {
       if (blockIdx.x == 0 && a.error) atomicCAS(a.error, 0, kErrLength);
@@ -197,36 +263,35 @@ __device__ __forceinline__ bool paged_share(const PagedArgs &a, int *steps, Page
   sum = 0;
   alive = 0;
 #pragma unroll
-  for (int i = 0; i < kPagedWarps; ++i) {
+  for (int i = 0; i < W; ++i) {
     sum += sum_s[i];
     alive += alive_s[i];
   }
   const int heads = a.kv_heads * a.tiles;
   const unsigned long long work = sum * heads;
   if (work == 0) return false;
-  constexpr int kLeast = kPagedWarps;  // a step a warp
   int S;
   if (a.waves) {
-    S = (int)min((work + (unsigned long long)a.waves * a.slots - 1) / ((unsigned long long)a.waves * a.slots),
-                 (unsigned long long)0x7fffffff);
+    const unsigned long long all = (unsigned long long)a.waves * a.slots;
+    S = (int)min((work + all - 1) / all, 0x7fffffffull);
   } else {
     const int items = alive * heads;
     const int lo = (int)((work + a.slots - 1) / a.slots), hi = (int)((work + a.slots - items - 1) / (a.slots - items));
     const int trial = max(kLeast, lo + (int)((long long)(hi - lo) * lane / 31));
     int n = 0;
-    for (int b = w; b < a.batch; b += kPagedWarps) n += (steps[b] + trial - 1) / trial;
+    for (int b = w; b < a.batch; b += W) n += (steps[b] + trial - 1) / trial;
     blocks_s[w][lane] = n;
     __syncthreads();
     n = 0;
 #pragma unroll
-    for (int i = 0; i < kPagedWarps; ++i) n += blocks_s[i][lane];
+    for (int i = 0; i < W; ++i) n += blocks_s[i][lane];
     const uint32_t fits = __ballot_sync(0xffffffffu, n * heads <= a.slots);
     S = __shfl_sync(0xffffffffu, trial, __ffs(fits) - 1);
   }
   S = max(S, kLeast);
   // the session of this block, and the slots of split sessions before it
   int blocks0 = 0, slots0 = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += kPagedThreads) {
+  for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
     const int b = b0 + tid, n = b < a.batch ? (steps[b] + S - 1) / S : 0;
     int blocks = n * heads, slots = n > 1 ? blocks : 0, x = blocks, y = slots;
 #pragma unroll
@@ -245,7 +310,7 @@ __device__ __forceinline__ bool paged_share(const PagedArgs &a, int *steps, Page
     __syncthreads();
     int before = blocks0, slots_before = slots0;
 #pragma unroll
-    for (int i = 0; i < kPagedWarps; ++i) {
+    for (int i = 0; i < W; ++i) {
       if (i < w) {
         before += blocks_s[i][0];
         slots_before += blocks_s[i][1];
@@ -277,22 +342,23 @@ __device__ __forceinline__ bool paged_share(const PagedArgs &a, int *steps, Page
   out->first = (int)((long long)total * part / n);
   out->count = (int)((long long)total * (part + 1) / n) - out->first;
   out->slot = found_s[2] + (out->kvh * a.tiles + tile) * n + part;
-  __syncthreads();  // `steps` is read
+  fence_proxy_async_smem();  // the words in `steps` lie where the first copies go
+  __syncthreads();
   return true;
 }
 
-template <typename T, int DP, int NR>
-__global__ void __launch_bounds__(kPagedThreads, (PagedShape<T, DP, NR>::kBlocks))
+template <typename T, int DP, int NR, bool ONCE>
+__global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (PagedShape<T, DP, NR, ONCE>::kBlocks))
     paged_attn_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ CUtensorMap k_map,
                       const __grid_constant__ CUtensorMap v_map) {
-  using Sh = PagedShape<T, DP, NR>;
-  constexpr int kTok = Sh::kTok, kParts = Sh::kParts, kNT = NR / 8;
+  using Sh = PagedShape<T, DP, NR, ONCE>;
+  constexpr int W = Sh::W, kTok = Sh::kTok, kParts = Sh::kParts, kNT = NR / 8;
   extern __shared__ uint8_t raw_sm[];
   uint8_t *const ring = raw_sm + (-smem_u32(raw_sm) & 1023);  // the swizzle goes by the address
   float *const sm = reinterpret_cast<float *>(ring);          // at the end: the warps' results
-  __shared__ uint64_t full[kPagedWarps][kParts];
+  __shared__ uint64_t full[W][kParts];
   __shared__ int abort_s;
-  __shared__ float m_s[kPagedWarps][NR], l_s[kPagedWarps][NR];
+  __shared__ float m_s[W][NR], l_s[W][NR];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, D = a.head_dim;
   if (lane == 0) {
     for (int i = 0; i < kParts; ++i) mbar_init(&full[w][i], 1);
@@ -302,19 +368,18 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedShape<T, DP, NR>::kBlocks
   __syncwarp();
   pdl_enter();
   PagedShare me;
-  if (!paged_share<kTok>(a, reinterpret_cast<int *>(ring), &me)) return;
-  fence_proxy_async_smem();  // the plan's words lie where the first copies go
-  __syncthreads();
+  if (!(a.batch <= 32 ? paged_share_few<kTok>(a, &me) : paged_share<kTok, W>(a, reinterpret_cast<int *>(ring), &me)))
+    return;
   if (tid == 0 && me.part == 0)
     a.shares[(size_t)(me.b * a.kv_heads + me.kvh) * a.tiles + me.tile] = make_int2(me.slot, me.parts);
 
   // A warp takes steps w, w + 4, ... of the share; part 2 i of its ring's sequence
   // is its i-th step's keys, part 2 i + 1 its values.
-  const int count = w < me.count ? (me.count - w + kPagedWarps - 1) / kPagedWarps : 0;
+  const int count = w < me.count ? (me.count - w + W - 1) / W : 0;
   uint8_t *const mine = ring + (size_t)w * kParts * Sh::kPart;
   const int boxes = kTok / a.box;  // copies of a step one below another: lane i's begins at token i * box
   const int32_t *const table = a.table + me.b * a.table_pitch;
-  auto token0 = [&](int i) { return (me.first + w + i * kPagedWarps) * kTok; };
+  auto token0 = [&](int i) { return (me.first + w + i * W) * kTok; };
   auto look_up = [&](int i) {  // the page of the lane's copy in step i
     const int t = token0(i) + lane * a.box;
     return lane < boxes && i < count && t < me.length ? table[t / a.page_size] : -1;
@@ -399,14 +464,14 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedShape<T, DP, NR>::kBlocks
   if constexpr (Sh::kHalf) {
     const int g = lane >> 2, c = lane & 3, own = token_at(g);
     __nv_bfloat16 *const qs = reinterpret_cast<__nv_bfloat16 *>(ring + Sh::kOver);  // [high, low][row][kQPitch]
-    constexpr int kPieces = DP / 32, kMT = DP / 16, kMine = NR / kPagedWarps, kChains = NR == 8 ? 4 : 2;
+    constexpr int kPieces = DP / 32, kMT = DP / 16, kMine = (NR + W - 1) / W, kChains = NR == 8 ? 4 : 2;
     const bool low = !a.q_bf16;
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
-      const int r = w + i * kPagedWarps, col = lane * 8;
+      const int r = w + i * W, col = lane * 8;
       float x[8];
       load_q8(a, me.b, head0 + r, col, r < rows && col < D, x);
-      if (col < DP) {
+      if (col < DP && r < NR) {
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) hi[k] = split_bf16x2(x[2 * k], x[2 * k + 1], &lo[k]);
@@ -568,6 +633,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedShape<T, DP, NR>::kBlocks
         q[r][j] = r < rows && column(j) < D ? load_q(a, me.b, head0 + r, column(j)) : 0.0f;
         acc[r][j] = 0.0f;
       }
+    __syncthreads();  // (abort_s)
     auto load_row = [&](const uint8_t *part, int t, float (&x)[kPer]) {
 #pragma unroll
       for (int j = 0; j < kPer; j += 4) {
@@ -674,12 +740,12 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedShape<T, DP, NR>::kBlocks
   }
   __syncthreads();
   // the warps' results meet: maxima, then sums over one maximum in warp order
-  for (int r = w; r < rows; r += kPagedWarps) {
-    float top = -INFINITY, f[kPagedWarps], sum = 0.0f;
+  for (int r = w; r < rows; r += W) {
+    float top = -INFINITY, f[W], sum = 0.0f;
 #pragma unroll
-    for (int x = 0; x < kPagedWarps; ++x) top = fmaxf(top, m_s[x][r]);
+    for (int x = 0; x < W; ++x) top = fmaxf(top, m_s[x][r]);
 #pragma unroll
-    for (int x = 0; x < kPagedWarps; ++x) {
+    for (int x = 0; x < W; ++x) {
       f[x] = m_s[x][r] == -INFINITY ? 0.0f : pow2(m_s[x][r] - top);
       sum = fmaf(l_s[x][r], f[x], sum);
     }
@@ -687,7 +753,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedShape<T, DP, NR>::kBlocks
     for (int d = lane * 2; d < D; d += 64) {
       float2 o = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int x = 0; x < kPagedWarps; ++x) {
+      for (int x = 0; x < W; ++x) {
         const float2 v = *reinterpret_cast<const float2 *>(sm + ((size_t)x * NR + r) * Sh::kEndPitch + d);
         o.x = fmaf(v.x, f[x], o.x);
         o.y = fmaf(v.y, f[x], o.y);
@@ -766,9 +832,9 @@ struct Plan {
   size_t blocks, parts;
 };
 
-template <typename T, int DP, int NR>
-int run_paged(const PagedArgs &a, const Plan &p, const CUtensorMap &k_map, const CUtensorMap &v_map, cudaStream_t s) {
-  using Sh = PagedShape<T, DP, NR>;
+template <typename T, int DP, int NR, bool ONCE>
+int run_shape(const PagedArgs &a, const Plan &p, const CUtensorMap &k_map, const CUtensorMap &v_map, cudaStream_t s) {
+  using Sh = PagedShape<T, DP, NR, ONCE>;
   {
     static std::mutex mu;
     static std::vector<int> done;
@@ -776,15 +842,21 @@ int run_paged(const PagedArgs &a, const Plan &p, const CUtensorMap &k_map, const
     FPB_CUDA_TRY(cudaGetDevice(&dev));
     std::lock_guard<std::mutex> lock(mu);
     if (std::find(done.begin(), done.end(), dev) == done.end()) {
-      FPB_CUDA_TRY(cudaFuncSetAttribute(paged_attn_kernel<T, DP, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      FPB_CUDA_TRY(cudaFuncSetAttribute(paged_attn_kernel<T, DP, NR, ONCE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         (int)Sh::smem));
       done.push_back(dev);
     }
   }
-  cudaError_t e = launch_pdl(paged_attn_kernel<T, DP, NR>, (unsigned)p.blocks, kPagedThreads, Sh::smem, s, a, k_map, v_map);
+  cudaError_t e = launch_pdl(paged_attn_kernel<T, DP, NR, ONCE>, (unsigned)p.blocks, Sh::kThreads, Sh::smem, s, a, k_map,
+                             v_map);
   if (e != cudaSuccess) return cuda_fail(e, "paged_attn_kernel");
   FPB_LAUNCH_CHECK("paged_attn_kernel");
   return FPB_OK;
+}
+
+template <typename T, int DP, int NR>
+int run_paged(const PagedArgs &a, const Plan &p, const CUtensorMap &k_map, const CUtensorMap &v_map, cudaStream_t s) {
+  return p.waves ? run_shape<T, DP, NR, false>(a, p, k_map, v_map, s) : run_shape<T, DP, NR, true>(a, p, k_map, v_map, s);
 }
 
 Plan plan_for(size_t batch, size_t q_heads, size_t kv_heads, size_t head_dim, bool f32) {
@@ -792,9 +864,10 @@ Plan plan_for(size_t batch, size_t q_heads, size_t kv_heads, size_t head_dim, bo
   const size_t group = q_heads / kv_heads;
   p.rows = group <= 8 || f32 ? 8 : 16;
   p.tiles = (int)((group + p.rows - 1) / p.rows);
-  p.slots = sm_count() * (head_dim > 128 ? 2 : 3);
   const size_t items = batch * kv_heads * p.tiles;
-  p.waves = 2 * items <= (size_t)p.slots ? 0 : kPagedWaves;
+  // one wave where half of the blocks at most can be short ones
+  p.waves = 2 * items <= (size_t)sm_count() ? 0 : kPagedWaves;
+  p.slots = sm_count() * blocks_of(head_dim > 128 ? 256 : 128, !p.waves);
   // an item that is cut has more than S steps, so at most twice its steps / S shares
   p.blocks = p.waves ? (size_t)p.waves * p.slots + items : p.slots;
   p.parts = p.waves ? (size_t)2 * p.waves * p.slots : p.slots;
