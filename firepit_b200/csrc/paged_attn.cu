@@ -3,6 +3,8 @@
 // Session b's query heads see the tokens t < lengths[b].  With s_t = scale q . k_t:
 //   out = sum_t softmax(s)_t v_t, times sigmoid(gate) where a gate is given.
 #include <algorithm>
+#include <atomic>
+#include <chrono>
 #include <cmath>
 #include <mutex>
 #include <vector>
@@ -24,6 +26,8 @@ struct PagedArgs {
   int batch, q_heads, kv_heads, group, head_dim, max_pages, pages, page_size, q_bf16, q_vec;
   int box;     // tokens of a copy: the largest power of two that divides the page size, up to a step's
   int tiles;   // row tiles of a kv head's query heads
+  int tok;     // tokens of a step
+  int least;   // steps of a share, at least
   int slots;   // blocks that the GPU has room for
   int waves;   // 0: no more blocks than that; else shares of 1 / (waves * slots) of the steps
   float scale_log2;  // scale * log2(e): scores and maxima are held in powers of two
@@ -31,7 +35,7 @@ struct PagedArgs {
   int out_bf16;
   float *part;      // [slot][row][head_dim] numerators
   float2 *part_ml;  // [slot][row] maximum, sum
-  int2 *shares;     // [session, kv head, row tile] first slot, number of slots (1: nothing to merge)
+  unsigned long long *flags, token;  // [slot]: `token`, this call's own, where the share's results are there
   int *error;
 };
 
@@ -46,6 +50,23 @@ __device__ __forceinline__ float pow2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two f32 in a register pair, and their arithmetic.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  return (uint64_t)__float_as_uint(hi) << 32 | __float_as_uint(lo);
+}
+__device__ __forceinline__ float low_of(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float high_of(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -108,17 +129,18 @@ __device__ __forceinline__ void load_q8(const PagedArgs &a, int b, int h, int d,
   }
 }
 
-// N columns of head h from d on: the numerators x over the sum l, gated.  No token:
-// zeros.
+// N columns of head h from d on: the numerators x over the sum l, times the gate's
+// sigmoid where there is one.  No token: zeros.
 template <int N>
-__device__ __forceinline__ void store_out(const PagedArgs &a, int b, int h, int d, const float (&x)[N], float l) {
+__device__ __forceinline__ void store_out(const PagedArgs &a, int b, int h, int d, const float (&x)[N], float l,
+                                          const float (&gate)[N]) {
   const size_t at = ((size_t)b * a.q_heads + h) * a.head_dim + d;
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;
   float o[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     o[k] = l != 0.0f ? x[k] * inv : 0.0f;
-    if (a.gate && l != 0.0f) o[k] /= 1.0f + expf(-a.gate[(size_t)b * a.gate_pitch + (size_t)h * a.gate_head + d + k]);
+    if (a.gate && l != 0.0f) o[k] /= 1.0f + expf(-gate[k]);
   }
 #pragma unroll
   for (int k = 0; k < N; k += 2) {
@@ -156,7 +178,7 @@ struct PagedShape {
   static constexpr size_t kEnd = (size_t)W * NR * kEndPitch * 4;  // the warps' results, over the ring
   static constexpr size_t kPlan = (size_t)kPagedMaxBatch * 4;     // the sessions' steps, over the ring
   static constexpr size_t kOver = kRing > kEnd ? kRing : kEnd;
-  static constexpr size_t kQueries = kHalf ? (size_t)2 * NR * kQPitch * 2 : (size_t)W * 64 * 4;
+  static constexpr size_t kQueries = kHalf ? (size_t)2 * NR * kQPitch * 2 : (size_t)W * 64 * 8;
   static constexpr size_t smem = 1023 + kOver + kQueries;
   static_assert(kPlan <= kOver && kBlocks * (smem + 4 * 1024) <= 228 * 1024);
 };
@@ -172,38 +194,41 @@ struct PagedShare {
 // One wave: the smallest S whose shares the GPU has room for at once, among 32
 // between total / slots, which is below it, and total / (slots - items), whose
 // shares fit: each item rounds up by less than one.
-constexpr int kLeast = 4;  // steps of a share, at least
+// Up to 32 sessions: every warp finds the shares on its own, a session a lane.
+struct FewPlan {
+  int length, steps, parts;   // of the lane's session
+  int blocks0, slots0;        // blocks, and slots of sessions that are cut, before it
+};
 
-// Up to 32 sessions: every warp finds the share on its own, a session a lane.
-template <int TOK>
-__device__ __forceinline__ bool paged_share_few(const PagedArgs &a, PagedShare *out) {
+// From the lane's session's length.
+__device__ __noinline__ FewPlan few_plan(const PagedArgs &a, int n) {
   const int lane = threadIdx.x & 31, heads = a.kv_heads * a.tiles;
-  int n = lane < a.batch ? a.lengths[lane] : 0;
-  if (n < 0 || n > (long long)a.max_pages * a.page_size) {
-    if (blockIdx.x == 0 && threadIdx.x < 32 && a.error) atomicCAS(a.error, 0, kErrLength);
-    n = 0;
-  }
-  const int steps = n / TOK + (n % TOK != 0);
-  const uint32_t alive = __ballot_sync(0xffffffffu, steps > 0);
-  unsigned long long work = steps;
+  FewPlan p{};
+  if (n < 0 || n > (long long)a.max_pages * a.page_size) n = 0;
+  p.length = n;
+  p.steps = n / a.tok + (n % a.tok != 0);
+  const uint32_t alive = __ballot_sync(0xffffffffu, p.steps > 0);
+  unsigned long long work = p.steps;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
   work *= heads;
-  if (work == 0) return false;
+  if (work == 0) return p;
+  // ceil(work / n); 64-bit quotients take a few hundred cycles
+  auto over = [&](uint32_t n) { return work >> 31 ? (int)min((work + n - 1) / n, 0x7fffffffull) : (int)(((uint32_t)work + n - 1) / n); };
   int S;
   if (a.waves) {
-    const unsigned long long all = (unsigned long long)a.waves * a.slots;
-    S = max(kLeast, (int)min((work + all - 1) / all, 0x7fffffffull));
+    S = max(a.least, over((uint32_t)a.waves * a.slots));
   } else {
-    const int items = __popc(alive) * heads;
-    const int lo = (int)((work + a.slots - 1) / a.slots), hi = (int)((work + a.slots - items - 1) / (a.slots - items));
-    const int trial = max(kLeast, lo + (int)((long long)(hi - lo) * lane / 31));
-    int blocks = 0;
-    for (int b = 0; b < a.batch; ++b) blocks += (__shfl_sync(0xffffffffu, steps, b) + trial - 1) / trial;
+    const int items = __popc(alive) * heads, lo = over(a.slots), hi = over(a.slots - items);
+    const uint32_t trial = max(a.least, lo + (hi - lo >= 31 ? (hi - lo) / 31 * lane + (hi - lo) % 31 * lane / 31 : min(lane, hi - lo)));
+    uint32_t blocks = 0;
+#pragma unroll 4
+    for (int b = 0; b < a.batch; ++b) blocks += ((uint32_t)__shfl_sync(0xffffffffu, p.steps, b) + trial - 1) / trial;
     const uint32_t fits = __ballot_sync(0xffffffffu, blocks * heads <= a.slots);
-    S = __shfl_sync(0xffffffffu, trial, __ffs(fits) - 1);
+    S = __shfl_sync(0xffffffffu, (int)trial, __ffs(fits) - 1);
   }
-  const int parts = (steps + S - 1) / S, blocks = parts * heads, slots = parts > 1 ? blocks : 0;
+  p.parts = (int)(((uint32_t)p.steps + S - 1) / S);
+  const int blocks = p.parts * heads, slots = p.parts > 1 ? blocks : 0;
   int x = blocks, y = slots;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -213,19 +238,28 @@ __device__ __forceinline__ bool paged_share_few(const PagedArgs &a, PagedShare *
       y += v;
     }
   }
-  const uint32_t mine = __ballot_sync(0xffffffffu, (int)blockIdx.x >= x - blocks && (int)blockIdx.x < x);
+  p.blocks0 = x - blocks;
+  p.slots0 = y - slots;
+  return p;
+}
+
+__device__ __forceinline__ bool paged_share_few(const PagedArgs &a, int length, uint32_t *empty, PagedShare *out) {
+  const FewPlan p = few_plan(a, length);
+  *empty = __ballot_sync(0xffffffffu, (int)(threadIdx.x & 31) < a.batch && p.steps == 0);
+  const int x = (int)blockIdx.x - p.blocks0;
+  const uint32_t mine = __ballot_sync(0xffffffffu, x >= 0 && x < p.parts * a.kv_heads * a.tiles);
   if (!mine) return false;
-  const int b = __ffs(mine) - 1, P = __shfl_sync(0xffffffffu, parts, b), total = __shfl_sync(0xffffffffu, steps, b);
-  const int at = (int)blockIdx.x - __shfl_sync(0xffffffffu, x - blocks, b);
+  const int b = __ffs(mine) - 1, P = __shfl_sync(0xffffffffu, p.parts, b), total = __shfl_sync(0xffffffffu, p.steps, b);
+  const int at = __shfl_sync(0xffffffffu, x, b);
   out->b = b;
   out->tile = at % a.tiles;
   out->part = at / a.tiles % P;
   out->parts = P;
   out->kvh = at / a.tiles / P;
-  out->length = __shfl_sync(0xffffffffu, n, b);
+  out->length = __shfl_sync(0xffffffffu, p.length, b);
   out->first = (int)((long long)total * out->part / P);
   out->count = (int)((long long)total * (out->part + 1) / P) - out->first;
-  out->slot = __shfl_sync(0xffffffffu, y - slots, b) + (out->kvh * a.tiles + out->tile) * P + out->part;
+  out->slot = __shfl_sync(0xffffffffu, p.slots0, b) + (out->kvh * a.tiles + out->tile) * P + out->part;
   return true;
 }
 
@@ -277,7 +311,7 @@ __device__ __forceinline__ bool paged_share(const PagedArgs &a, int *steps, Page
   } else {
     const int items = alive * heads;
     const int lo = (int)((work + a.slots - 1) / a.slots), hi = (int)((work + a.slots - items - 1) / (a.slots - items));
-    const int trial = max(kLeast, lo + (int)((long long)(hi - lo) * lane / 31));
+    const int trial = max(a.least, lo + (int)((long long)(hi - lo) * lane / 31));
     int n = 0;
     for (int b = w; b < a.batch; b += W) n += (steps[b] + trial - 1) / trial;
     blocks_s[w][lane] = n;
@@ -288,7 +322,7 @@ __device__ __forceinline__ bool paged_share(const PagedArgs &a, int *steps, Page
     const uint32_t fits = __ballot_sync(0xffffffffu, n * heads <= a.slots);
     S = __shfl_sync(0xffffffffu, trial, __ffs(fits) - 1);
   }
-  S = max(S, kLeast);
+  S = max(S, a.least);
   // the session of this block, and the slots of split sessions before it
   int blocks0 = 0, slots0 = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
@@ -366,25 +400,68 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
     fence_barrier_init();
   }
   __syncwarp();
-  pdl_enter();
+  if (tid == 0) {
+    prefetch_tensormap(&k_map);
+    prefetch_tensormap(&v_map);
+  }
+  // A warp takes steps w, w + W, ... of the share; part 2 i of its ring's sequence is
+  // its i-th step's keys, part 2 i + 1 its values.  A step has copies one below
+  // another: lane i's begins at token i * box.
   PagedShare me;
-  if (!(a.batch <= 32 ? paged_share_few<kTok>(a, &me) : paged_share<kTok, W>(a, reinterpret_cast<int *>(ring), &me)))
-    return;
-  if (tid == 0 && me.part == 0)
-    a.shares[(size_t)(me.b * a.kv_heads + me.kvh) * a.tiles + me.tile] = make_int2(me.slot, me.parts);
-
-  // A warp takes steps w, w + 4, ... of the share; part 2 i of its ring's sequence
-  // is its i-th step's keys, part 2 i + 1 its values.
-  const int count = w < me.count ? (me.count - w + W - 1) / W : 0;
-  uint8_t *const mine = ring + (size_t)w * kParts * Sh::kPart;
-  const int boxes = kTok / a.box;  // copies of a step one below another: lane i's begins at token i * box
-  const int32_t *const table = a.table + me.b * a.table_pitch;
+  int count = 0;
+  const int32_t *table = a.table;
+  const int boxes = kTok / a.box;
   auto token0 = [&](int i) { return (me.first + w + i * W) * kTok; };
   auto look_up = [&](int i) {  // the page of the lane's copy in step i
     const int t = token0(i) + lane * a.box;
-    return lane < boxes && i < count && t < me.length ? table[t / a.page_size] : -1;
+    return lane < boxes && i < count && t < me.length ? __ldcg(table + t / a.page_size) : -1;
   };
-  int page = -1, next_page = look_up(0);
+  auto begin = [&]() {
+    count = w < me.count ? (me.count - w + W - 1) / W : 0;
+    table = a.table + me.b * a.table_pitch;
+  };
+  // Up to 32 sessions: the share is found while the kernel ahead still runs.  What
+  // that one may have changed since is read again behind it, past L1, and the share
+  // found anew if a length is another.
+  const bool few = a.batch <= 32;
+  uint32_t empty = 0;  // sessions without tokens, of up to 32
+  bool any = false;
+  int early = 0, page = -1, next_page = -1;
+  if (few) {
+    early = lane < a.batch ? __ldcg(a.lengths + lane) : 0;
+    any = paged_share_few(a, early, &empty, &me);
+    if (any) {
+      begin();
+      const int t = token0(0) + lane * a.box;
+      if (lane < boxes && t < me.length) asm volatile("prefetch.global.L2 [%0];" ::"l"(table + t / a.page_size));
+    }
+  }
+  pdl_enter();
+  if (few) {
+    const int length = lane < a.batch ? __ldcg(a.lengths + lane) : 0;
+    if (any) next_page = look_up(0);
+    if (blockIdx.x == 0 && w == 0 && (length < 0 || length > (long long)a.max_pages * a.page_size) && a.error)
+      atomicCAS(a.error, 0, kErrLength);
+    if (__any_sync(0xffffffffu, length != early)) {
+      any = paged_share_few(a, length, &empty, &me);
+      if (any) {
+        begin();
+        next_page = look_up(0);
+      }
+    }
+  } else if ((any = paged_share<kTok, W>(a, reinterpret_cast<int *>(ring), &me))) {
+    begin();
+    next_page = look_up(0);
+  }
+  // sessions without tokens: block b writes session b's zeros, and those a grid on
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
+    if (few ? empty >> b & 1 : a.lengths[b] <= 0 || a.lengths[b] > (long long)a.max_pages * a.page_size)
+      for (int i = tid; i < a.q_heads * D / 2; i += Sh::kThreads) {
+        const float zeros[2] = {0.0f, 0.0f};
+        store_out<2>(a, b, 0, 2 * i, zeros, 0.0f, zeros);
+      }
+  if (!any) return;
+  uint8_t *const mine = ring + (size_t)w * kParts * Sh::kPart;
   bool wrong = false;  // a page outside the pool was met
   auto fetch = [&](int j) {
     const int i = j >> 1, t = token0(i) + lane * a.box;
@@ -621,34 +698,32 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
         for (int e = 0; e < 4; ++e)
           mine_f[(8 * i + 2 * c + (e & 1)) * Sh::kEndPitch + 16 * k + g + 8 * (e >> 1)] = acc[k][i][e];
   } else {
-    constexpr int kPer = DP / 32;  // columns a lane: 2, or fours 128 apart
-    auto column = [&](int j) { return kPer == 2 ? 2 * lane + j : (j >> 2) * 128 + 4 * lane + (j & 3); };
-    float *const ps = reinterpret_cast<float *>(ring + Sh::kOver) + w * 64;  // [token][row] weights
+    constexpr int kPairs = DP / 64;  // pairs of columns a lane: one, or twos 128 columns apart
+    auto column = [&](int j) { return kPairs == 1 ? 2 * lane : (j >> 1) * 128 + 4 * lane + 2 * (j & 1); };
+    uint64_t *const ps = reinterpret_cast<uint64_t *>(ring + Sh::kOver) + w * 64;  // [token][row] weights, twice each
     const int row = lane & 7, tok = lane >> 3;
-    float q[8][kPer], acc[8][kPer], m = -INFINITY, l = 0.0f;
+    uint64_t q[8][kPairs], acc[8][kPairs];
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int r = 0; r < 8; ++r)
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        q[r][j] = r < rows && column(j) < D ? load_q(a, me.b, head0 + r, column(j)) : 0.0f;
-        acc[r][j] = 0.0f;
+      for (int j = 0; j < kPairs; ++j) {
+        const bool in = r < rows && column(j) < D;
+        q[r][j] = in ? pair(load_q(a, me.b, head0 + r, column(j)), load_q(a, me.b, head0 + r, column(j) + 1)) : 0;
+        acc[r][j] = 0;
       }
     __syncthreads();  // (abort_s)
-    auto load_row = [&](const uint8_t *part, int t, float (&x)[kPer]) {
+    auto load_row = [&](const uint8_t *part, int t, uint64_t (&x)[kPairs]) {
 #pragma unroll
-      for (int j = 0; j < kPer; j += 4) {
+      for (int j = 0; j < kPairs; j += 2) {
         const int d = column(j);
         const uint8_t *p = part + (d >> 5) * (kTok * 128) + t * 128 + ((((d & 31) >> 2) ^ t) * 16);
-        if constexpr (kPer == 2) {
-          const float2 v = *reinterpret_cast<const float2 *>(p + (d & 3) * 4);
-          x[0] = v.x;
-          x[1] = v.y;
+        if constexpr (kPairs == 1) {
+          x[0] = *reinterpret_cast<const uint64_t *>(p + (d & 3) * 4);
         } else {
-          const float4 v = *reinterpret_cast<const float4 *>(p);
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(p);
           x[j] = v.x;
           x[j + 1] = v.y;
-          x[j + 2] = v.z;
-          x[j + 3] = v.w;
         }
       }
     };
@@ -662,14 +737,14 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
         float v[32];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          float x[kPer];
+          uint64_t x[kPairs];
           load_row(kst, 4 * u + t, x);
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
-            float s = q[r][0] * x[0];
+            uint64_t s = mul2(q[r][0], x[0]);
 #pragma unroll
-            for (int j = 1; j < kPer; ++j) s = fmaf(q[r][j], x[j], s);
-            v[8 * t + r] = s;
+            for (int j = 1; j < kPairs; ++j) s = fma2(q[r][j], x[j], s);
+            v[8 * t + r] = low_of(s) + high_of(s);
           }
         }
         // 32 sums over the warp, one to a lane
@@ -699,7 +774,7 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
         for (int r = 0; r < 8; ++r) {
           const float f = __shfl_sync(0xffffffffu, old, r);
 #pragma unroll
-          for (int j = 0; j < kPer; ++j) acc[r][j] *= f;
+          for (int j = 0; j < kPairs; ++j) acc[r][j] = mul2(acc[r][j], pair(f, f));
         }
       }
       const float base = m == -INFINITY ? 0.0f : -kBack - m;
@@ -707,21 +782,24 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
       for (int u = 0; u < 2; ++u) {
         const float p = pow2(y[u] + base);
         l += p;
-        ps[(4 * u + tok) * 8 + row] = p;
+        ps[(4 * u + tok) * 8 + row] = pair(p, p);
       }
       uint8_t *vst = mine + (2 * at + 1) % kParts * Sh::kPart;
       wait(2 * at + 1);  // (the warp meets: the weights are there)
       if (open) clear_values(vst, t0);
 #pragma unroll
       for (int t = 0; t < kTok; ++t) {
-        float x[kPer];
+        uint64_t x[kPairs];
         load_row(vst, t, x);
-        const float4 u = *reinterpret_cast<const float4 *>(ps + 8 * t), v = *reinterpret_cast<const float4 *>(ps + 8 * t + 4);
-        const float p[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
+        for (int r = 0; r < 8; r += 2) {
+          const ulonglong2 p = *reinterpret_cast<const ulonglong2 *>(ps + 8 * t + r);
 #pragma unroll
-          for (int j = 0; j < kPer; ++j) acc[r][j] = fmaf(p[r], x[j], acc[r][j]);
+          for (int j = 0; j < kPairs; ++j) {
+            acc[r][j] = fma2(p.x, x[j], acc[r][j]);
+            acc[r + 1][j] = fma2(p.y, x[j], acc[r + 1][j]);
+          }
+        }
       }
       done(2 * at + 1);
     }
@@ -736,7 +814,8 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
 #pragma unroll
     for (int r = 0; r < 8; ++r)
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) mine_f[r * Sh::kEndPitch + column(j)] = acc[r][j];
+      for (int j = 0; j < kPairs; ++j)
+        *reinterpret_cast<uint64_t *>(mine_f + r * Sh::kEndPitch + column(j)) = acc[r][j];
   }
   __syncthreads();
   // the warps' results meet: maxima, then sums over one maximum in warp order
@@ -761,74 +840,106 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
       if (me.parts > 1) {
         *reinterpret_cast<float2 *>(a.part + to * D + d) = o;
       } else {
-        const float x[2] = {o.x, o.y};
-        store_out<2>(a, me.b, head0 + r, d, x, sum);
+        const float *g = a.gate ? a.gate + (size_t)me.b * a.gate_pitch + (size_t)(head0 + r) * a.gate_head + d : nullptr;
+        const float x[2] = {o.x, o.y}, gate[2] = {g ? g[0] : 0.0f, g ? g[1] : 0.0f};
+        store_out<2>(a, me.b, head0 + r, d, x, sum, gate);
       }
     }
     if (me.parts > 1 && lane == 0) a.part_ml[to] = make_float2(top, sum);
   }
-}
-
-// The shares of a row (session and query head) meet, in order: blockDim.y warps a
-// row and 128 columns share them, four columns a lane.  A session without tokens
-// gets its zeros here.
-constexpr int kMergeWarps = 16;
-__global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __grid_constant__ PagedArgs a, int NR,
-                                                                      int count) {
-  __shared__ float4 acc_s[kMergeWarps][32];
-  __shared__ float l_s[kMergeWarps];
-  const int lane = threadIdx.x, share = threadIdx.y, shares = blockDim.y, w = threadIdx.z * shares + share;
-  const int i = blockIdx.x * blockDim.z + threadIdx.z, d = blockIdx.y * 128 + lane * 4, D = a.head_dim;
-  const bool in = i < count;
-  const int h = in ? i % a.q_heads : 0, b = in ? i / a.q_heads : 0, kvh = h / a.group, in_group = h % a.group;
-  const int tile = in_group / NR, r = in_group % NR;
-  asm volatile("griddepcontrol.launch_dependents;");
-  const int n = a.lengths[b];
-  const bool none = n <= 0 || n > (long long)a.max_pages * a.page_size;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  int2 mine = make_int2(0, 0);
-  if (in && !none) mine = a.shares[(size_t)(b * a.kv_heads + kvh) * a.tiles + tile];
-  const int parts = mine.y > 1 ? mine.y : 0;
-  const float2 *ml = a.part_ml + (size_t)mine.x * NR + r;
-  float top = -INFINITY, l = 0.0f;
-  for (int s = lane; s < parts; s += 32) top = fmaxf(top, ml[(size_t)s * NR].x);
-  top = warp_max(top);
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  auto add = [&](float4 x, float f) {
-    acc.x = fmaf(x.x, f, acc.x);
-    acc.y = fmaf(x.y, f, acc.y);
-    acc.z = fmaf(x.z, f, acc.z);
-    acc.w = fmaf(x.w, f, acc.w);
-  };
-  const float *part = a.part + ((size_t)mine.x * NR + r) * D + (d < D ? d : 0);
-#pragma unroll 4
-  for (int s = share; s < parts; s += shares) {
-    const float2 v = ml[(size_t)s * NR];
-    const float4 x = *reinterpret_cast<const float4 *>(part + (size_t)s * NR * D);
-    const float f = v.x == -INFINITY ? 0.0f : pow2(v.x - top);
-    l = fmaf(v.y, f, l);
-    add(x, f);
-  }
-  if (shares > 1) {
-    if (share > 0) {
-      acc_s[w][lane] = acc;
-      if (lane == 0) l_s[w] = l;
+  if (me.parts == 1) return;
+  // The shares of an item meet in the block that finds all of them there: each says
+  // so by its flag and then looks at the others', so that the last one does find
+  // them (another that does as well writes the same).  What a flag says is the
+  // call's own number, whatever lay there before; they are cleared for the next use.
+  // (A kernel behind this one for it: 1 x 777 tokens 10.9 us, so 8.)
+  __shared__ int last_s;
+  const int slot0 = me.slot - me.part;
+  __syncthreads();
+  if (w == 0) {
+    if (lane == 0) {
+      __threadfence();
+      *reinterpret_cast<volatile unsigned long long *>(a.flags + me.slot) = a.token;
+      __threadfence();
     }
-    __syncthreads();
-    if (share > 0) return;
-    for (int k = w + 1; k < w + shares; ++k) {
-      add(acc_s[k][lane], 1.0f);
-      l += l_s[k];
+    __syncwarp();
+    bool all = true;
+    for (int i = lane; i < me.parts; i += 32)
+      all &= *reinterpret_cast<volatile unsigned long long *>(a.flags + slot0 + i) == a.token;
+    all = __all_sync(0xffffffffu, all);
+    __threadfence();
+    if (lane == 0) last_s = all;
+  }
+  __syncthreads();
+  if (!last_s) return;
+  const float2 *ml = a.part_ml + (size_t)slot0 * NR;
+  const float *part = a.part + (size_t)slot0 * NR * D;
+  // (a thread's fours of columns, and of eight shares each, are asked for together, and the gates with them)
+  constexpr int kItems = (NR * DP / 4 + Sh::kThreads - 1) / Sh::kThreads, kAtOnce = kItems >= 4 ? 4 : 8;
+  float4 o[kItems], gate[kItems];
+  float top[kItems], sum[kItems];
+  int row[kItems], col[kItems];
+#pragma unroll
+  for (int j = 0; j < kItems; ++j) {
+    const int i = tid + j * Sh::kThreads;
+    row[j] = i / (D / 4);
+    col[j] = (i - row[j] * (D / 4)) * 4;
+    o[j] = gate[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    top[j] = -INFINITY;
+    sum[j] = 0.0f;
+    if (a.gate && row[j] < rows) {
+      const float *g = a.gate + (size_t)me.b * a.gate_pitch + (size_t)(head0 + row[j]) * a.gate_head + col[j];
+      gate[j] = make_float4(g[0], g[1], g[2], g[3]);
     }
   }
-  if (!in || d >= D || mine.y == 1) return;
-  const float x[4] = {acc.x, acc.y, acc.z, acc.w};
-  store_out<4>(a, b, h, d, x, l);
+#pragma unroll 1
+  for (int x0 = 0; x0 < me.parts; x0 += kAtOnce) {
+    float4 v[kItems][kAtOnce];
+    float2 y[kItems][kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kItems; ++j)
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const bool in = x0 + k < me.parts && row[j] < rows;
+        const size_t at = (size_t)(x0 + k) * NR + row[j];
+        v[j][k] = in ? __ldcg(reinterpret_cast<const float4 *>(part + at * D + col[j])) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        y[j][k] = in ? __ldcg(ml + at) : make_float2(-INFINITY, 0.0f);
+      }
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) {
+      float high = top[j];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) high = fmaxf(high, y[j][k].x);
+      const float old = top[j] == -INFINITY ? 0.0f : pow2(top[j] - high);
+      top[j] = high;
+      o[j].x *= old;
+      o[j].y *= old;
+      o[j].z *= old;
+      o[j].w *= old;
+      sum[j] *= old;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const float f = y[j][k].x == -INFINITY ? 0.0f : pow2(y[j][k].x - high);
+        sum[j] = fmaf(y[j][k].y, f, sum[j]);
+        o[j].x = fmaf(v[j][k].x, f, o[j].x);
+        o[j].y = fmaf(v[j][k].y, f, o[j].y);
+        o[j].z = fmaf(v[j][k].z, f, o[j].z);
+        o[j].w = fmaf(v[j][k].w, f, o[j].w);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kItems; ++j) {
+    if (row[j] >= rows) continue;
+    const float x[4] = {o[j].x, o[j].y, o[j].z, o[j].w}, g[4] = {gate[j].x, gate[j].y, gate[j].z, gate[j].w};
+    store_out<4>(a, me.b, head0 + row[j], col[j], x, sum[j], g);
+  }
+  for (int i = tid; i < me.parts; i += Sh::kThreads) a.flags[slot0 + i] = 0;
 }
 
 // How a call is cut.
 struct Plan {
-  int rows, tiles, slots, waves;
+  int rows, tiles, slots, waves, least;
   size_t blocks, parts;
 };
 
@@ -867,6 +978,7 @@ Plan plan_for(size_t batch, size_t q_heads, size_t kv_heads, size_t head_dim, bo
   const size_t items = batch * kv_heads * p.tiles;
   // one wave where half of the blocks at most can be short ones
   p.waves = 2 * items <= (size_t)sm_count() ? 0 : kPagedWaves;
+  p.least = p.waves ? 16 : 4;
   p.slots = sm_count() * blocks_of(head_dim > 128 ? 256 : 128, !p.waves);
   // an item that is cut has more than S steps, so at most twice its steps / S shares
   p.blocks = p.waves ? (size_t)p.waves * p.slots + items : p.slots;
@@ -874,8 +986,19 @@ Plan plan_for(size_t batch, size_t q_heads, size_t kv_heads, size_t head_dim, bo
   return p;
 }
 
-size_t workspace_for(const Plan &p, size_t batch, size_t kv_heads, size_t head_dim) {
-  return p.parts * p.rows * (head_dim + 2) * sizeof(float) + batch * kv_heads * p.tiles * sizeof(int2);
+// A number that no other call has: mixed, so that nothing that happens to lie in a
+// workspace is likely to be it (the mixing is that of splitmix64).
+unsigned long long call_number() {
+  static std::atomic<unsigned long long> calls{(unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count()};
+  unsigned long long x = calls.fetch_add(0x9e3779b97f4a7c15ull);
+  x = (x ^ x >> 30) * 0xbf58476d1ce4e5b9ull;
+  x = (x ^ x >> 27) * 0x94d049bb133111ebull;
+  x ^= x >> 31;
+  return x ? x : 1;
+}
+
+size_t workspace_for(const Plan &p, size_t head_dim) {
+  return p.parts * (p.rows * (head_dim + 2) * sizeof(float) + sizeof(unsigned long long));
 }
 
 }  // namespace
@@ -885,8 +1008,8 @@ using namespace fpb;
 
 extern "C" size_t fpb_paged_attn_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads, size_t head_dim) {
   if (batch == 0 || kv_heads == 0 || q_heads == 0 || q_heads % kv_heads) return 16;
-  const size_t a = workspace_for(plan_for(batch, q_heads, kv_heads, head_dim, false), batch, kv_heads, head_dim),
-               b = workspace_for(plan_for(batch, q_heads, kv_heads, head_dim, true), batch, kv_heads, head_dim);
+  const size_t a = workspace_for(plan_for(batch, q_heads, kv_heads, head_dim, false), head_dim),
+               b = workspace_for(plan_for(batch, q_heads, kv_heads, head_dim, true), head_dim);
   return std::max(a, b);
 }
 
@@ -942,6 +1065,8 @@ extern "C" int fpb_paged_attn(const void *q, int q_dtype, size_t q_pitch, size_t
   a.box = f32 ? 8 : 16;
   while (page_size % a.box) a.box /= 2;
   a.tiles = p.tiles;
+  a.tok = f32 ? 8 : 16;
+  a.least = p.least;
   a.slots = p.slots;
   a.waves = p.waves;
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
@@ -949,7 +1074,8 @@ extern "C" int fpb_paged_attn(const void *q, int q_dtype, size_t q_pitch, size_t
   a.out_bf16 = out_dtype == FPB_BF16;
   a.part = static_cast<float *>(workspace);
   a.part_ml = reinterpret_cast<float2 *>(a.part + p.parts * p.rows * head_dim);
-  a.shares = reinterpret_cast<int2 *>(a.part_ml + p.parts * p.rows);
+  a.flags = reinterpret_cast<unsigned long long *>(a.part_ml + p.parts * p.rows);
+  a.token = call_number();
   a.error = device_error_ptr();
   CUtensorMap k_map, v_map;
   if (int st = encode_pages(&k_map, k_pages, !f32, head_dim, kv_heads, page_size, pages, head_pitch, row_pitch,
@@ -970,15 +1096,5 @@ extern "C" int fpb_paged_attn(const void *q, int q_dtype, size_t q_pitch, size_t
     st = head_dim <= 64    ? (few ? run_paged<bf, 64, 8>(a, p, k_map, v_map, s) : run_paged<bf, 64, 16>(a, p, k_map, v_map, s))
          : head_dim <= 128 ? (few ? run_paged<bf, 128, 8>(a, p, k_map, v_map, s) : run_paged<bf, 128, 16>(a, p, k_map, v_map, s))
                            : (few ? run_paged<bf, 256, 8>(a, p, k_map, v_map, s) : run_paged<bf, 256, 16>(a, p, k_map, v_map, s));
-  if (st) return st;
-  const int count = (int)(batch * q_heads);
-  const unsigned halves = head_dim > 128 ? 2 : 1;
-  unsigned shares = 1;  // warps a row: as many as run at once
-  while (shares < (unsigned)kMergeWarps && 2 * shares * halves * (size_t)count <= (size_t)sm_count() * 16) shares *= 2;
-  const unsigned per = std::max(1u, 8 / shares);
-  cudaError_t e = launch_pdl(paged_merge_kernel, dim3((unsigned)((count + per - 1) / per), halves), dim3(32, shares, per),
-                             0, s, a, p.rows, count);
-  if (e != cudaSuccess) return cuda_fail(e, "paged_merge_kernel");
-  FPB_LAUNCH_CHECK("paged_merge_kernel");
-  return FPB_OK;
+  return st;
 }
