@@ -39,7 +39,7 @@ struct PagedArgs {
   int *error;
 };
 
-constexpr int kPagedMaxBatch = 4096, kPagedWaves = 4;
+constexpr int kPagedMaxBatch = 4096, kPagedWaves = 2;
 constexpr int kErrPagedWait = 503;
 // The maximum may lag by kLag (powers of two) before the sums are rescaled, and
 // weights are held as 2^(y - m - kBack): 2^20 of them times a value of the type's
@@ -194,6 +194,13 @@ struct PagedShare {
 // One wave: the smallest S whose shares the GPU has room for at once, among 32
 // between total / slots, which is below it, and total / (slots - items), whose
 // shares fit: each item rounds up by less than one.
+// Lane 0 lo, lane 31 hi, the others between them, in even ratios but for rounding.
+__device__ __forceinline__ int between(int lo, int hi) {
+  const int lane = threadIdx.x & 31;
+  const float ratio = __log2f((float)hi / (float)lo) * (1.0f / 31.0f);
+  return lane == 31 ? hi : min(hi, (int)((float)lo * exp2f(ratio * lane)));
+}
+
 // Up to 32 sessions: every warp finds the shares on its own, a session a lane.
 struct FewPlan {
   int length, steps, parts;   // of the lane's session
@@ -220,7 +227,7 @@ __device__ __noinline__ FewPlan few_plan(const PagedArgs &a, int n) {
     S = max(a.least, over((uint32_t)a.waves * a.slots));
   } else {
     const int items = __popc(alive) * heads, lo = over(a.slots), hi = over(a.slots - items);
-    const uint32_t trial = max(a.least, lo + (hi - lo >= 31 ? (hi - lo) / 31 * lane + (hi - lo) % 31 * lane / 31 : min(lane, hi - lo)));
+    const uint32_t trial = max(a.least, between(lo, hi));
     uint32_t blocks = 0;
 #pragma unroll 4
     for (int b = 0; b < a.batch; ++b) blocks += ((uint32_t)__shfl_sync(0xffffffffu, p.steps, b) + trial - 1) / trial;
@@ -311,7 +318,7 @@ __device__ __forceinline__ bool paged_share(const PagedArgs &a, int *steps, Page
   } else {
     const int items = alive * heads;
     const int lo = (int)((work + a.slots - 1) / a.slots), hi = (int)((work + a.slots - items - 1) / (a.slots - items));
-    const int trial = max(a.least, lo + (int)((long long)(hi - lo) * lane / 31));
+    const int trial = max(a.least, between(lo, hi));
     int n = 0;
     for (int b = w; b < a.batch; b += W) n += (steps[b] + trial - 1) / trial;
     blocks_s[w][lane] = n;
@@ -978,7 +985,7 @@ Plan plan_for(size_t batch, size_t q_heads, size_t kv_heads, size_t head_dim, bo
   const size_t items = batch * kv_heads * p.tiles;
   // one wave where half of the blocks at most can be short ones
   p.waves = 2 * items <= (size_t)sm_count() ? 0 : kPagedWaves;
-  p.least = p.waves ? 16 : 4;
+  p.least = p.waves ? 64 : 8;
   p.slots = sm_count() * blocks_of(head_dim > 128 ? 256 : 128, !p.waves);
   // an item that is cut has more than S steps, so at most twice its steps / S shares
   p.blocks = p.waves ? (size_t)p.waves * p.slots + items : p.slots;
