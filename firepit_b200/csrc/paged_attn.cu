@@ -52,21 +52,35 @@ __device__ __forceinline__ float pow2(float x) {
   return y;
 }
 
-// Two f32 in a register pair, and their arithmetic.
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  return (uint64_t)__float_as_uint(hi) << 32 | __float_as_uint(lo);
-}
-__device__ __forceinline__ float low_of(uint64_t x) { return __uint_as_float((uint32_t)x); }
-__device__ __forceinline__ float high_of(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+// Two f32 sums at once.
+__device__ __forceinline__ void add2(float &x, float &y, float u, float v) {
   uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"((uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x)), "l"((uint64_t)__float_as_uint(v) << 32 | __float_as_uint(u)));
+  x = __uint_as_float((uint32_t)r);
+  y = __uint_as_float((uint32_t)(r >> 32));
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
+
+__device__ __forceinline__ void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// An f32 as what the tensor cores take of it (11 bits) and the rest of it, of which
+// they take 11 more.  Cut: 2^-20 is lost at most, and 2^-10 the rest's size;
+// nearest: 2^-21 and 2^-11.
+__device__ __forceinline__ void split_cut(uint32_t x, uint32_t *hi, uint32_t *lo) {
+  *hi = x & 0xffffe000u;
+  *lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(*hi));
+}
+__device__ __forceinline__ void split_nearest(float x, uint32_t *hi, uint32_t *lo) {
+  const uint32_t h = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  *hi = h;
+  *lo = __float_as_uint(x - __uint_as_float(h));
 }
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -152,33 +166,38 @@ __device__ __forceinline__ void store_out(const PagedArgs &a, int b, int h, int 
 }
 
 // Operand row i of eight is token token_at(i) of its eight: a quarter of a warp
-// then reads 16 bytes from all of the banks.
-__device__ __forceinline__ int token_at(int i) { return (i >> 1) | (i & 1) << 2; }
+// then reads 16 bytes from all of the banks.  For f32 the values' rows are read by
+// pairs of them too.
+template <typename T>
+__device__ __forceinline__ int token_at(int i) {
+  return sizeof(T) == 2 ? (i >> 1) | (i & 1) << 2 : i & 1 ? ((i - 1) ^ 4) | 1 : i;
+}
 
 // Blocks of W warps.  Where the calls' blocks are all there at once there is one an
 // SM, of 8 or 12 warps: smaller ones, two or three an SM, leave registers that do
 // not lie together when the kernel before is still there, and an SM then takes one
 // block less (3 x 100003 tokens behind another call 172 us, alone 106).  Where they
 // come one after another small blocks overlap their beginnings and ends.
-constexpr int warps_of(int DP, bool once) { return !once ? 4 : DP == 256 ? 8 : 12; }
+constexpr int warps_of(int DP, bool f32, bool once) { return !once ? 4 : DP == 256 && !f32 ? 8 : 12; }
 constexpr int blocks_of(int DP, bool once) { return once ? 1 : DP == 256 ? 2 : 3; }
 
 template <typename T, int DP, int NR, bool ONCE>
 struct PagedShape {
   static constexpr bool kHalf = sizeof(T) == 2;
-  static constexpr int W = warps_of(DP, ONCE), kThreads = 32 * W, kBlocks = blocks_of(DP, ONCE);
+  static constexpr int W = warps_of(DP, !kHalf, ONCE), kThreads = 32 * W, kBlocks = blocks_of(DP, ONCE);
   static constexpr int kTok = kHalf ? 16 : 8;                       // tokens of a step
   static constexpr int kCols = 128 / (int)sizeof(T), kBoxes = DP / kCols;  // a copy's columns; copies side by side
   static constexpr uint32_t kPart = kTok * DP * sizeof(T);          // a step's keys, or its values
-  static constexpr int kParts = (DP == 256 ? 3 : DP == 128 ? 4 : 6) - (NR == 16 && !ONCE);  // of a warp's ring
+  static constexpr int kParts = (DP == 256 ? (kHalf ? 3 : 2) : DP == 128 ? 4 : 6) -
+                                (!ONCE && (NR == 16 || (!kHalf && DP == 128)));  // of a warp's ring
   static constexpr bool kQShared = NR == 16 && DP >= 128;           // too many registers of queries beside those of sums
-  static constexpr int kQPitch = DP + 32;                           // bf16 elements: 16-byte reads of eight rows on distinct banks
+  static constexpr int kQPitch = DP + (kHalf ? 32 : 16);            // elements: 16-byte reads of eight rows on distinct banks
   static constexpr int kEndPitch = DP + 4;
   static constexpr size_t kRing = (size_t)W * kParts * kPart;
   static constexpr size_t kEnd = (size_t)W * NR * kEndPitch * 4;  // the warps' results, over the ring
   static constexpr size_t kPlan = (size_t)kPagedMaxBatch * 4;     // the sessions' steps, over the ring
   static constexpr size_t kOver = kRing > kEnd ? kRing : kEnd;
-  static constexpr size_t kQueries = kHalf ? (size_t)2 * NR * kQPitch * 2 : (size_t)W * 64 * 8;
+  static constexpr size_t kQueries = (size_t)2 * NR * kQPitch * sizeof(T);
   static constexpr size_t smem = 1023 + kOver + kQueries;
   static_assert(kPlan <= kOver && kBlocks * (smem + 4 * 1024) <= 228 * 1024);
 };
@@ -546,7 +565,7 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
   };
 
   if constexpr (Sh::kHalf) {
-    const int g = lane >> 2, c = lane & 3, own = token_at(g);
+    const int g = lane >> 2, c = lane & 3, own = token_at<T>(g);
     __nv_bfloat16 *const qs = reinterpret_cast<__nv_bfloat16 *>(ring + Sh::kOver);  // [high, low][row][kQPitch]
     constexpr int kPieces = DP / 32, kMT = DP / 16, kMine = (NR + W - 1) / W, kChains = NR == 8 ? 4 : 2;
     const bool low = !a.q_bf16;
@@ -670,7 +689,7 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
       uint8_t *vst = mine + (2 * at + 1) % kParts * Sh::kPart;
       wait(2 * at + 1);
       if (open) clear_values(vst, t0);
-      const int vrow = token_at(lane & 7), half = (lane >> 3) & 1;
+      const int vrow = token_at<T>(lane & 7), half = (lane >> 3) & 1;
       const uint32_t v0 = smem_u32(vst) + (vrow + 8 * (lane >> 4)) * 128;
 #pragma unroll
       for (int k = 0; k < kMT; ++k) {
@@ -705,124 +724,128 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
         for (int e = 0; e < 4; ++e)
           mine_f[(8 * i + 2 * c + (e & 1)) * Sh::kEndPitch + 16 * k + g + 8 * (e >> 1)] = acc[k][i][e];
   } else {
-    constexpr int kPairs = DP / 64;  // pairs of columns a lane: one, or twos 128 columns apart
-    auto column = [&](int j) { return kPairs == 1 ? 2 * lane : (j >> 1) * 128 + 4 * lane + 2 * (j & 1); };
-    uint64_t *const ps = reinterpret_cast<uint64_t *>(ring + Sh::kOver) + w * 64;  // [token][row] weights, twice each
-    const int row = lane & 7, tok = lane >> 3;
-    uint64_t q[8][kPairs], acc[8][kPairs];
-    float m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int r = 0; r < 8; ++r)
-#pragma unroll
-      for (int j = 0; j < kPairs; ++j) {
-        const bool in = r < rows && column(j) < D;
-        q[r][j] = in ? pair(load_q(a, me.b, head0 + r, column(j)), load_q(a, me.b, head0 + r, column(j) + 1)) : 0;
-        acc[r][j] = 0;
+    // S = Q K^T with the rows as M (eight of sixteen), eight tokens as N; O^T = V^T P^T
+    // with the dimensions as M, the rows as N: S's result is P^T's operand as it lies.
+    const int g = lane >> 2, c = lane & 3, own = token_at<T>(g);
+    uint32_t *const qs = reinterpret_cast<uint32_t *>(ring + Sh::kOver);  // [high, low][row][kQPitch]
+    constexpr int kBoxes = Sh::kBoxes, kMT = DP / 16;
+    for (int r = w; r < NR; r += W)
+      for (int col = lane; col < DP; col += 32) {
+        const float x = r < rows && col < D ? load_q(a, me.b, head0 + r, col) : 0.0f;
+        split_nearest(x, qs + r * Sh::kQPitch + col, qs + (NR + r) * Sh::kQPitch + col);
       }
-    __syncthreads();  // (abort_s)
-    auto load_row = [&](const uint8_t *part, int t, uint64_t (&x)[kPairs]) {
+    __syncthreads();
+    float acc[kMT][4], m = -INFINITY, l = 0.0f;  // the row g's maximum and sum
 #pragma unroll
-      for (int j = 0; j < kPairs; j += 2) {
-        const int d = column(j);
-        const uint8_t *p = part + (d >> 5) * (kTok * 128) + t * 128 + ((((d & 31) >> 2) ^ t) * 16);
-        if constexpr (kPairs == 1) {
-          x[0] = *reinterpret_cast<const uint64_t *>(p + (d & 3) * 4);
-        } else {
-          const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(p);
-          x[j] = v.x;
-          x[j + 1] = v.y;
-        }
-      }
-    };
+    for (int k = 0; k < kMT; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[k][e] = 0.0f;
+    const int v0 = token_at<T>(2 * c), v1 = token_at<T>(2 * c + 1);
     for (int at = 0; at < count; ++at) {
       const int t0 = token0(at);
       const uint8_t *kst = mine + (2 * at) % kParts * Sh::kPart;
       wait(2 * at);
-      float y[2];  // scores of tokens tok and tok + 4, the lane's row
+      // scores of eight tokens, row g: s[.][0] token v0, s[.][1] v1, in sums that do not
+      // wait for one another
+      float s[4][4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float v[32];
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          uint64_t x[kPairs];
-          load_row(kst, 4 * u + t, x);
+        for (int k = 0; k < 4; ++k) s[u][k] = 0.0f;
 #pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            uint64_t s = mul2(q[r][0], x[0]);
-#pragma unroll
-            for (int j = 1; j < kPairs; ++j) s = fma2(q[r][j], x[j], s);
-            v[8 * t + r] = low_of(s) + high_of(s);
-          }
-        }
-        // 32 sums over the warp, one to a lane
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-          for (int i = 0; i < o; ++i) {
-            const float keep = lane & o ? v[i + o] : v[i], send = lane & o ? v[i] : v[i + o];
-            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-          }
-        y[u] = v[0] * a.scale_log2;
+      for (int p = 0; p < 2 * kBoxes; ++p) {  // sixteen dimensions: the lane's four, 16 p + 4 c
+        const uint4 x = *reinterpret_cast<const uint4 *>(kst + (p >> 1) * (kTok * 128) + own * 128 +
+                                                         ((4 * (p & 1) + c) ^ own) * 16);
+        const uint4 qh = *reinterpret_cast<const uint4 *>(qs + g * Sh::kQPitch + 16 * p + 4 * c);
+        const uint4 ql = *reinterpret_cast<const uint4 *>(qs + (NR + g) * Sh::kQPitch + 16 * p + 4 * c);
+        uint4 hi, lo;
+        split_cut(x.x, &hi.x, &lo.x);
+        split_cut(x.y, &hi.y, &lo.y);
+        split_cut(x.z, &hi.z, &lo.z);
+        split_cut(x.w, &hi.w, &lo.w);
+        mma_tf32(s[0], qh.x, 0, qh.y, 0, hi.x, hi.y);
+        mma_tf32(s[1], qh.z, 0, qh.w, 0, hi.z, hi.w);
+        mma_tf32(s[2], qh.x, 0, qh.y, 0, lo.x, lo.y);
+        mma_tf32(s[3], ql.x, 0, ql.y, 0, hi.x, hi.y);
+        mma_tf32(s[2], qh.z, 0, qh.w, 0, lo.z, lo.w);
+        mma_tf32(s[3], ql.z, 0, ql.w, 0, hi.z, hi.w);
       }
       done(2 * at);
       const bool open = t0 + kTok > me.length || wrong;
-      if (open) {
-        if (!token_there(t0 + tok)) y[0] = -INFINITY;
-        if (!token_there(t0 + tok + 4)) y[1] = -INFINITY;
+      float y[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        y[u] = ((s[0][u] + s[1][u]) + (s[2][u] + s[3][u])) * a.scale_log2;
+        if (open && !token_there(t0 + (u ? v1 : v0))) y[u] = -INFINITY;
       }
       if (__any_sync(0xffffffffu, fmaxf(y[0], y[1]) > m + kLag)) {
         float mn = fmaxf(m, fmaxf(y[0], y[1]));
-        mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 8));
-        mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 16));
+        mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 1));
+        mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 2));
         const float old = m == -INFINITY ? 0.0f : pow2(m - mn);
         l *= old;
         m = mn;
+        const float f0 = __shfl_sync(0xffffffffu, old, 8 * c), f1 = __shfl_sync(0xffffffffu, old, 8 * c + 4);  // rows 2 c, 2 c + 1
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          const float f = __shfl_sync(0xffffffffu, old, r);
-#pragma unroll
-          for (int j = 0; j < kPairs; ++j) acc[r][j] = mul2(acc[r][j], pair(f, f));
+        for (int k = 0; k < kMT; ++k) {
+          acc[k][0] *= f0;
+          acc[k][1] *= f1;
+          acc[k][2] *= f0;
+          acc[k][3] *= f1;
         }
       }
       const float base = m == -INFINITY ? 0.0f : -kBack - m;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float p = pow2(y[u] + base);
-        l += p;
-        ps[(4 * u + tok) * 8 + row] = pair(p, p);
-      }
+      const float p0 = pow2(y[0] + base), p1 = pow2(y[1] + base);
+      l += p0 + p1;
+      uint32_t ph[2], pl[2];
+      split_nearest(p0, &ph[0], &pl[0]);
+      split_nearest(p1, &ph[1], &pl[1]);
       uint8_t *vst = mine + (2 * at + 1) % kParts * Sh::kPart;
-      wait(2 * at + 1);  // (the warp meets: the weights are there)
+      wait(2 * at + 1);
       if (open) clear_values(vst, t0);
+      // (the sums over the steps are kept apart: the tensor cores' own cut what they add)
 #pragma unroll
-      for (int t = 0; t < kTok; ++t) {
-        uint64_t x[kPairs];
-        load_row(vst, t, x);
-#pragma unroll
-        for (int r = 0; r < 8; r += 2) {
-          const ulonglong2 p = *reinterpret_cast<const ulonglong2 *>(ps + 8 * t + r);
-#pragma unroll
-          for (int j = 0; j < kPairs; ++j) {
-            acc[r][j] = fma2(p.x, x[j], acc[r][j]);
-            acc[r + 1][j] = fma2(p.y, x[j], acc[r + 1][j]);
-          }
-        }
+      for (int x = 0; x < kBoxes; ++x) {  // 32 dimensions: the lane's four, 32 x + 4 g
+        const uint8_t *box = vst + x * (kTok * 128);
+        const uint4 u = *reinterpret_cast<const uint4 *>(box + v0 * 128 + (g ^ v0) * 16);
+        const uint4 v = *reinterpret_cast<const uint4 *>(box + v1 * 128 + (g ^ v1) * 16);
+        uint4 uh, ul, vh, vl;
+        split_cut(u.x, &uh.x, &ul.x);
+        split_cut(u.y, &uh.y, &ul.y);
+        split_cut(u.z, &uh.z, &ul.z);
+        split_cut(u.w, &uh.w, &ul.w);
+        split_cut(v.x, &vh.x, &vl.x);
+        split_cut(v.y, &vh.y, &vl.y);
+        split_cut(v.z, &vh.z, &vl.z);
+        split_cut(v.w, &vh.w, &vl.w);
+        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f}, e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        mma_tf32(d, uh.x, uh.y, vh.x, vh.y, ph[0], ph[1]);
+        mma_tf32(e, uh.z, uh.w, vh.z, vh.w, ph[0], ph[1]);
+        mma_tf32(d, ul.x, ul.y, vl.x, vl.y, ph[0], ph[1]);
+        mma_tf32(e, ul.z, ul.w, vl.z, vl.w, ph[0], ph[1]);
+        mma_tf32(d, uh.x, uh.y, vh.x, vh.y, pl[0], pl[1]);
+        mma_tf32(e, uh.z, uh.w, vh.z, vh.w, pl[0], pl[1]);
+        add2(acc[2 * x][0], acc[2 * x][1], d[0], d[1]);
+        add2(acc[2 * x][2], acc[2 * x][3], d[2], d[3]);
+        add2(acc[2 * x + 1][0], acc[2 * x + 1][1], e[0], e[1]);
+        add2(acc[2 * x + 1][2], acc[2 * x + 1][3], e[2], e[3]);
       }
       done(2 * at + 1);
     }
-    l += __shfl_xor_sync(0xffffffffu, l, 8);
-    l += __shfl_xor_sync(0xffffffffu, l, 16);
-    if (lane < 8) {
-      m_s[w][lane] = m;
-      l_s[w][lane] = l;
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (c == 0) {
+      m_s[w][g] = m;
+      l_s[w][g] = l;
     }
     finish();
     float *mine_f = sm + (size_t)w * NR * Sh::kEndPitch;
+    // tile 2 x + h of 16 dimensions: row i < 8 of it is dimension 32 x + 4 i + 2 h, row i + 8 the one after it
 #pragma unroll
-    for (int r = 0; r < 8; ++r)
+    for (int k = 0; k < kMT; ++k)
 #pragma unroll
-      for (int j = 0; j < kPairs; ++j)
-        *reinterpret_cast<uint64_t *>(mine_f + r * Sh::kEndPitch + column(j)) = acc[r][j];
+      for (int e = 0; e < 4; ++e)
+        mine_f[(2 * c + (e & 1)) * Sh::kEndPitch + 32 * (k >> 1) + 4 * g + 2 * (k & 1) + (e >> 1)] = acc[k][e];
   }
   __syncthreads();
   // the warps' results meet: maxima, then sums over one maximum in warp order
