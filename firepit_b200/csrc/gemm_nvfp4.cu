@@ -987,15 +987,15 @@ int encode_cache_u8(CUtensorMap *map, const void *base, uint64_t batch, uint64_t
 
 int encode_pages(CUtensorMap *map, const void *base, bool bf16, uint64_t head_dim, uint64_t kv_heads,
                  uint64_t page_size, uint64_t pages, uint64_t head_pitch, uint64_t row_pitch, uint64_t page_pitch,
-                 uint32_t box_rows) {
+                 uint32_t box_rows, uint32_t pieces) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(FPB_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-  const uint64_t el = bf16 ? 2 : 4;
-  cuuint64_t dims[4] = {head_dim, kv_heads, page_size, pages};
-  cuuint64_t strides[3] = {head_pitch * el, row_pitch * el, page_pitch * el};
-  cuuint32_t box[4] = {(cuuint32_t)(128 / el), 1, box_rows, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4,
+  const uint64_t el = bf16 ? 2 : 4, cols = 128 / el;
+  cuuint64_t dims[5] = {pieces > 1 ? cols : head_dim, page_size, pieces > 1 ? head_dim / cols : 1, kv_heads, pages};
+  cuuint64_t strides[4] = {row_pitch * el, 128, head_pitch * el, page_pitch * el};
+  cuuint32_t box[5] = {(cuuint32_t)cols, box_rows, pieces, 1, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 5,
                   const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(FPB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);

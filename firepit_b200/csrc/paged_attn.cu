@@ -25,6 +25,7 @@ struct PagedArgs {
   long long q_pitch, q_head, gate_pitch, gate_head, table_pitch;  // elements
   int batch, q_heads, kv_heads, group, head_dim, max_pages, pages, page_size, q_bf16, q_vec;
   int box;     // tokens of a copy: the largest power of two that divides the page size, up to a step's
+  int whole;   // a copy takes all of a head vector's 128-byte pieces (else one: the last is not whole)
   int tiles;   // row tiles of a kv head's query heads
   int tok;     // tokens of a step
   int least;   // steps of a share, at least
@@ -508,15 +509,31 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
       uint8_t *to = mine + (j % kParts) * Sh::kPart + lane * a.box * 128;
       const CUtensorMap *map = j & 1 ? &v_map : &k_map;
       const int row = t % a.page_size;
+      if (a.whole) {
+        tma_load_5d(to, map, 0, row, 0, me.kvh, page, bar);
+      } else {
 #pragma unroll
-      for (int x = 0; x < Sh::kBoxes; ++x)
-        tma_load_4d(to + x * (kTok * 128), map, x * Sh::kCols, me.kvh, row, page, bar);
+        for (int x = 0; x < Sh::kBoxes; ++x)
+          tma_load_5d(to + x * (kTok * 128), map, x * Sh::kCols, row, 0, me.kvh, page, bar);
+      }
     }
     __syncwarp();
   };
+  // The queries, eight columns a lane and a row a warp, are asked for ahead of the
+  // first copies (behind them, which take the memory a few microseconds, they came
+  // 3 us later); the gates come to L2 meanwhile.
+  const int head0 = me.kvh * a.group + me.tile * NR, rows = min(NR, a.group - me.tile * NR);
+  constexpr int kMine = (NR + W - 1) / W;
+  float x[kMine][8];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int r = w + i * W, col = lane * 8;
+    load_q8(a, me.b, head0 + r, col, r < rows && col < D, x[i]);
+    if (a.gate && r < rows && col < D)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(a.gate + (size_t)me.b * a.gate_pitch + (size_t)(head0 + r) * a.gate_head + col));
+  }
   for (int j = 0; j < min(2 * count, kParts); ++j) fetch(j);
 
-  const int head0 = me.kvh * a.group + me.tile * NR, rows = min(NR, a.group - me.tile * NR);
   bool ok = true;
   auto wait = [&](int j) {
     if (ok) ok = mbar_wait(&full[w][j % kParts], (j / kParts) & 1, &abort_s);
@@ -567,17 +584,15 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
   if constexpr (Sh::kHalf) {
     const int g = lane >> 2, c = lane & 3, own = token_at<T>(g);
     __nv_bfloat16 *const qs = reinterpret_cast<__nv_bfloat16 *>(ring + Sh::kOver);  // [high, low][row][kQPitch]
-    constexpr int kPieces = DP / 32, kMT = DP / 16, kMine = (NR + W - 1) / W, kChains = NR == 8 ? 4 : 2;
+    constexpr int kPieces = DP / 32, kMT = DP / 16, kChains = NR == 8 ? 4 : 2;
     const bool low = !a.q_bf16;
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
       const int r = w + i * W, col = lane * 8;
-      float x[8];
-      load_q8(a, me.b, head0 + r, col, r < rows && col < D, x);
       if (col < DP && r < NR) {
         uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) hi[k] = split_bf16x2(x[2 * k], x[2 * k + 1], &lo[k]);
+        for (int k = 0; k < 4; ++k) hi[k] = split_bf16x2(x[i][2 * k], x[i][2 * k + 1], &lo[k]);
         *reinterpret_cast<uint4 *>(qs + r * Sh::kQPitch + col) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         *reinterpret_cast<uint4 *>(qs + (NR + r) * Sh::kQPitch + col) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
@@ -729,11 +744,20 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
     const int g = lane >> 2, c = lane & 3, own = token_at<T>(g);
     uint32_t *const qs = reinterpret_cast<uint32_t *>(ring + Sh::kOver);  // [high, low][row][kQPitch]
     constexpr int kBoxes = Sh::kBoxes, kMT = DP / 16;
-    for (int r = w; r < NR; r += W)
-      for (int col = lane; col < DP; col += 32) {
-        const float x = r < rows && col < D ? load_q(a, me.b, head0 + r, col) : 0.0f;
-        split_nearest(x, qs + r * Sh::kQPitch + col, qs + (NR + r) * Sh::kQPitch + col);
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int r = w + i * W, col = lane * 8;
+      if (col < DP && r < NR) {
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) split_nearest(x[i][k], &hi[k], &lo[k]);
+#pragma unroll
+        for (int k = 0; k < 8; k += 4) {
+          *reinterpret_cast<uint4 *>(qs + r * Sh::kQPitch + col + k) = make_uint4(hi[k], hi[k + 1], hi[k + 2], hi[k + 3]);
+          *reinterpret_cast<uint4 *>(qs + (NR + r) * Sh::kQPitch + col + k) = make_uint4(lo[k], lo[k + 1], lo[k + 2], lo[k + 3]);
+        }
       }
+    }
     __syncthreads();
     float acc[kMT][4], m = -INFINITY, l = 0.0f;  // the row g's maximum and sum
 #pragma unroll
@@ -905,7 +929,7 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
   const float2 *ml = a.part_ml + (size_t)slot0 * NR;
   const float *part = a.part + (size_t)slot0 * NR * D;
   // (a thread's fours of columns, and of eight shares each, are asked for together, and the gates with them)
-  constexpr int kItems = (NR * DP / 4 + Sh::kThreads - 1) / Sh::kThreads, kAtOnce = kItems >= 4 ? 4 : 8;
+  constexpr int kItems = (NR * DP / 4 + Sh::kThreads - 1) / Sh::kThreads, kAtOnce = kItems >= 4 ? 4 : kItems == 2 ? 10 : 12;
   float4 o[kItems], gate[kItems];
   float top[kItems], sum[kItems];
   int row[kItems], col[kItems];
@@ -1094,6 +1118,7 @@ extern "C" int fpb_paged_attn(const void *q, int q_dtype, size_t q_pitch, size_t
   a.q_vec = aligned_to(q, 16) && (q_pitch | q_head_pitch) * (a.q_bf16 ? 2 : 4) % 16 == 0;
   a.box = f32 ? 8 : 16;
   while (page_size % a.box) a.box /= 2;
+  a.whole = head_dim % (f32 ? 32 : 64) == 0 && a.box == (f32 ? 8 : 16);
   a.tiles = p.tiles;
   a.tok = f32 ? 8 : 16;
   a.least = p.least;
@@ -1109,10 +1134,10 @@ extern "C" int fpb_paged_attn(const void *q, int q_dtype, size_t q_pitch, size_t
   a.error = device_error_ptr();
   CUtensorMap k_map, v_map;
   if (int st = encode_pages(&k_map, k_pages, !f32, head_dim, kv_heads, page_size, pages, head_pitch, row_pitch,
-                            page_pitch, (uint32_t)a.box))
+                            page_pitch, (uint32_t)a.box, a.whole ? (head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256) / (f32 ? 32 : 64) : 1))
     return st;
   if (int st = encode_pages(&v_map, v_pages, !f32, head_dim, kv_heads, page_size, pages, head_pitch, row_pitch,
-                            page_pitch, (uint32_t)a.box))
+                            page_pitch, (uint32_t)a.box, a.whole ? (head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256) / (f32 ? 32 : 64) : 1))
     return st;
   cudaStream_t s = as_stream(stream);
   using bf = __nv_bfloat16;

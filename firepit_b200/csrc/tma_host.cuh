@@ -17,11 +17,13 @@ int encode_cache_u8(CUtensorMap *map, const void *base, uint64_t batch, uint64_t
                     uint64_t head_dim, uint32_t box_bytes, uint32_t box_rows);
 
 // Pages of a cache [pages, page_size, kv_heads, head_dim] bf16 or f32 (pitches in
-// elements), read in boxes of 128 bytes x 1 head x box_rows tokens with 128-byte
-// swizzle; out-of-range elements read as zero.  FPB status.
+// elements) as (column, row, piece, head, page), read in boxes of 128 bytes x
+// box_rows tokens x `pieces` 128-byte pieces of a head vector x 1 head with 128-byte
+// swizzle; out-of-range elements read as zero.  pieces 1: head_dim columns and one
+// piece; else head_dim is whole pieces.  FPB status.
 int encode_pages(CUtensorMap *map, const void *base, bool bf16, uint64_t head_dim, uint64_t kv_heads,
                  uint64_t page_size, uint64_t pages, uint64_t head_pitch, uint64_t row_pitch, uint64_t page_pitch,
-                 uint32_t box_rows);
+                 uint32_t box_rows, uint32_t pieces);
 
 // Output map for the GEMM epilogues' tiled stores: y [rows, cols] (bf16 or
 // f32, row pitch ld elements), boxes of box_cols x box_rows (box_cols 0: 128
