@@ -16,6 +16,10 @@ the prompt runs through the same decode step, one token per step.
 of drafted tokens a session through a model of full-attention layers in one
 step and keeps the path that the model accepts.
 
+``PagedDecoder`` serves requests of any length over a paged cache
+(firepit_b200/paged.py): they come and go while the others decode, each with its
+own sampling.
+
 Multi-GPU: ``replicas`` — every GPU holds the whole model and decodes its own
 sessions (no exchange).
 """
@@ -217,7 +221,6 @@ class Decoder:
     def __init__(self, model: HybridModel, batch: int, max_seq: int, history_len: int = 0, kv8: bool = False):
         import torch
 
-        from .speculative import Kv8Cache
         self.model, self.cfg = model, model.cfg
         c, dev, B = model.cfg, model.device, batch * self.nodes
         self.sessions, self.batch, self.max_seq, self.kv8 = batch, B, max_seq, kv8
@@ -245,9 +248,7 @@ class Decoder:
         self.vp = torch.zeros(B, c.kv_heads * c.head_dim, **f32)
         self.q_rot = torch.zeros(B, c.q_heads, c.head_dim, **f32)
         self.attn = torch.zeros(B, c.q_heads * c.head_dim, **bf)
-        ws = int(N.lib.fpb_tree_attn_workspace_bytes(batch, self.nodes, c.q_heads, c.kv_heads, c.head_dim, max_seq)
-                 if kv8 else N.lib.fpb_attn_decode_workspace_bytes(B, c.q_heads, c.head_dim, max_seq, 32))
-        self.attn_ws = torch.empty(ws, dtype=torch.uint8, device=dev)
+        self.attn_ws = torch.empty(self._attn_workspace(), dtype=torch.uint8, device=dev)
         self.logits_r = torch.zeros(B, c.route_rows, **f32)  # router logits, then the gate logit
         self.gate = torch.zeros(B, **f32)
         self.ids = torch.zeros(B, c.slots, **i32)
@@ -270,9 +271,7 @@ class Decoder:
         self.gdn = {}
         for i, L in enumerate(model.layers):
             if L["kind"] == "attention":
-                shape = (batch, max_seq, c.kv_heads, c.head_dim)
-                self.kv[i] = Kv8Cache.zeros(*shape, device=dev) if kv8 else (torch.zeros(shape, **f32),
-                                                                             torch.zeros(shape, **f32))
+                self.kv[i] = self._attn_cache()
             else:
                 self.gdn[i] = (torch.zeros(B, c.conv_dim, c.conv_kernel - 1, **f32),
                                torch.zeros(B, c.value_heads, c.key_head_dim, c.value_head_dim, **f32))
@@ -295,6 +294,25 @@ class Decoder:
         self._batched = {}
         self.graph = None
         self.route_log = None  # [layers, batch, slots] int32 when recording routes
+
+    def _attn_workspace(self) -> int:
+        """Bytes that the attention of one layer works in."""
+        c = self.cfg
+        if self.kv8:
+            return int(N.lib.fpb_tree_attn_workspace_bytes(self.sessions, self.nodes, c.q_heads, c.kv_heads, c.head_dim,
+                                                           self.max_seq))
+        return int(N.lib.fpb_attn_decode_workspace_bytes(self.batch, c.q_heads, c.head_dim, self.max_seq, 32))
+
+    def _attn_cache(self):
+        """The cache of one attention layer."""
+        import torch
+
+        from .speculative import Kv8Cache
+        c, dev = self.cfg, self.model.device
+        shape = (self.sessions, self.max_seq, c.kv_heads, c.head_dim)
+        if self.kv8:
+            return Kv8Cache.zeros(*shape, device=dev)
+        return torch.zeros(shape, device=dev), torch.zeros(shape, device=dev)
 
     def _gemv(self, key, members, x, sh, tensor_cores=False):
         """One batched NVFP4 GEMV launch of [(weight, y)] sharing input x: on
@@ -652,6 +670,223 @@ class SpeculativeDecoder(Decoder):
         if error:
             raise RuntimeError(f"generate: device error {error}")
         return [h[n:] for h, n in zip(history, start)]
+
+
+@dataclass
+class Request:
+    """A prompt (token ids), how many tokens to add to it, and how they are drawn
+    (``sample``'s filters; temperature 0: greedily)."""
+
+    prompt: list
+    new_tokens: int
+    temperature: float = 0.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+
+
+class PagedDecoder(Decoder):
+    """Serves requests on `sessions` rows whose attention layers share pools of
+    `pages` pages of `page_size` tokens (a pool a layer, one table for all), so
+    that a long session takes no more than its tokens' room and a row is free for
+    the next request as soon as one is done.
+
+    ``step()`` takes one token of every session under way: from its prompt, or the
+    one before it drawn (``noise``, from ``draw``).  It takes the pages, runs the
+    model and leaves each session's next token in ``tokens`` and, where that is a
+    drawn one, in ``emitted`` (-1 elsewhere).  Nothing of it looks from the host,
+    so ``capture()`` records it.  ``admit`` and ``release`` go between steps;
+    ``serve`` does it all.  Admission counts the pages that a request may come to,
+    so that no step finds the pool empty."""
+
+    def __init__(self, model: HybridModel, sessions: int, max_seq: int, pages: int, page_size: int = 16, dtype=None):
+        import torch
+
+        from .gemv import ShapeError
+        from .paged import PageMap, PageTables
+        if sessions < 1 or max_seq < 1 or pages < 1 or page_size < 1:
+            raise ShapeError(f"paged decoder: {sessions} sessions of {max_seq} tokens, {pages} pages of {page_size}")
+        c, dev = model.cfg, model.device
+        self.pages, self.page_size = pages, page_size
+        self.page_dtype = torch.bfloat16 if dtype is None else dtype
+        width = min(pages, -(-max_seq // page_size))
+        super().__init__(model, sessions, min(max_seq, width * page_size))
+        i32, f32 = dict(dtype=torch.int32, device=dev), dict(dtype=torch.float32, device=dev)
+        self.tables = PageTables.empty(sessions, pages, page_size, width, device=dev)
+        self.map = PageMap(*(torch.full((sessions,), -1, **i32) for _ in range(3)), torch.zeros(sessions + 1, **i32))
+        self.positions = self.tables.lengths
+        self.active = torch.zeros(sessions, **i32)
+        self.prompt = torch.zeros(sessions, self.max_seq, **i32)
+        self.prompt_len = torch.zeros(sessions, **i32)
+        self.temperature, self.min_p = torch.zeros(sessions, **f32), torch.zeros(sessions, **f32)
+        self.top_p, self.top_k = torch.ones(sessions, **f32), torch.zeros(sessions, **i32)
+        self.noise = torch.ones(sessions, c.vocab, **f32)
+        self.drawn = torch.zeros(sessions, **i32)
+        self.emitted = torch.full((sessions,), -1, **i32)
+        self.reserved = [0] * sessions
+
+    def _attn_workspace(self) -> int:
+        c = self.cfg
+        return int(N.lib.fpb_paged_attn_workspace_bytes(self.batch, c.q_heads, c.kv_heads, c.head_dim))
+
+    def _attn_cache(self):
+        from .paged import PagedCache
+        return PagedCache.zeros(self.pages, self.page_size, self.cfg.kv_heads, self.cfg.head_dim, self.page_dtype,
+                                self.model.device)
+
+    def _attend(self, i, L, sh: int) -> None:
+        c, B, D, kv, t = self.cfg, self.batch, self.cfg.head_dim, self.kv[i], self.tables
+        shape = (kv.code, self.pages, self.page_size, *kv.pitches)
+        N.call("fpb_paged_append", self.qg.data_ptr(), self.qg.shape[1], 2 * D, self.kp.data_ptr(), self.kp.shape[1],
+               self.vp.data_ptr(), self.vp.shape[1], N.FPB_F32, L["q_norm"].data_ptr(), L["k_norm"].data_ptr(),
+               self.map.slots.data_ptr(), self.map.positions.data_ptr(), B, c.q_heads, c.kv_heads, D, c.rotary_dim,
+               c.rope_theta, c.eps, self.q_rot.data_ptr(), N.FPB_F32, kv.k.data_ptr(), kv.v.data_ptr(), *shape, sh)
+        N.call("fpb_paged_attn", self.q_rot.data_ptr(), N.FPB_F32, c.q_heads * D, D, kv.k.data_ptr(), kv.v.data_ptr(),
+               *shape, t.table.data_ptr(), t.pitch, t.table.shape[1], t.lengths.data_ptr(),
+               self.qg.data_ptr() + 4 * D, self.qg.shape[1], 2 * D, B, c.q_heads, c.kv_heads, D, 1.0 / math.sqrt(D),
+               self.attn_ws.data_ptr(), self.attn_ws.numel(), self.attn.data_ptr(), N.FPB_BF16, sh)
+
+    def _sample(self, sh: int) -> None:
+        import torch
+        c = self.cfg
+        N.call("fpb_sample", self.logits.data_ptr(), N.FPB_F32, c.vocab, self.temperature.data_ptr(),
+               self.top_k.data_ptr(), self.top_p.data_ptr(), self.min_p.data_ptr(), self.noise.data_ptr(), c.vocab,
+               self.batch, c.vocab, self.drawn.data_ptr(), None, sh)
+        # the steps on the results, behind the kernels on their stream
+        now = torch.cuda.current_stream(self.model.device)
+        with torch.cuda.stream(now if now.cuda_stream == sh else
+                               torch.cuda.ExternalStream(sh, device=self.model.device)):
+            after = self.map.positions + 1
+            known = after < self.prompt_len
+            taken = self.map.slots >= 0
+            prompt = torch.gather(self.prompt, 1, after.clamp(0, self.max_seq - 1).long()[:, None])[:, 0]
+            self.emitted.copy_(torch.where(taken & ~known, self.drawn, -1))
+            self.tokens.copy_(torch.where(taken, torch.where(known, prompt, self.drawn), self.tokens))
+
+    def step(self, sh: int) -> None:
+        t, m = self.tables, self.map
+        N.call("fpb_page_extend", t.table.data_ptr(), t.pitch, self.batch, t.table.shape[1], t.lengths.data_ptr(),
+               self.active.data_ptr(), t.free.data_ptr(), t.free_count.data_ptr(), self.pages, self.page_size,
+               self.batch, 1, m.slots.data_ptr(), m.positions.data_ptr(), m.requests.data_ptr(), m.starts.data_ptr(), sh)
+        super().step(sh)
+
+    def draw(self, generator=None) -> None:
+        """New random numbers for the next step."""
+        self.noise.exponential_(generator=generator).clamp_(min=1e-20)
+
+    def reset(self) -> None:
+        """No session is under way, every page is free."""
+        from .paged import PageTables
+        t = self.tables
+        new = PageTables.empty(self.batch, self.pages, self.page_size, t.table.shape[1], device=self.model.device)
+        for old, x in ((t.table, new.table), (t.lengths, new.lengths), (t.free, new.free), (t.free_count, new.free_count)):
+            old.copy_(x)
+        for x in (self.tokens, self.active, self.prompt_len):
+            x.zero_()
+        for x in (self.map.slots, self.map.positions, self.map.requests, self.emitted):
+            x.fill_(-1)
+        for cs, rs in self.gdn.values():
+            cs.zero_()
+            rs.zero_()
+        self.reserved = [0] * self.sessions
+
+    def pages_for(self, request: Request) -> int:
+        """Pages that the request may come to (its last token is not run)."""
+        return -(-(len(request.prompt) + request.new_tokens - 1) // self.page_size)
+
+    def _check(self, request: Request) -> None:
+        from .gemv import ShapeError
+        n, k = len(request.prompt), request.new_tokens
+        if n < 1 or k < 1 or n + k - 1 > self.max_seq:
+            raise ShapeError(f"request: a prompt of {n} tokens and {k} new ones in sessions of up to {self.max_seq}")
+        if not all(0 <= t < self.cfg.vocab for t in request.prompt):
+            raise ShapeError(f"request: tokens outside the vocabulary ({self.cfg.vocab})")
+
+    def admit(self, session: int, request: Request) -> bool:
+        """Begins a request on a free row; False if the pool could run out of pages
+        for those under way with it."""
+        import torch
+
+        from .gemv import ShapeError
+        self._check(request)
+        if self.reserved[session]:
+            raise ShapeError(f"admit: session {session} is under way")
+        need = self.pages_for(request)
+        if sum(self.reserved) + need > self.pages:
+            return False
+        self.reserved[session] = need
+        n = len(request.prompt)
+        self.prompt[session, :n].copy_(torch.tensor(request.prompt, dtype=torch.int32))
+        self.prompt_len[session] = n
+        self.tokens[session] = request.prompt[0]
+        self.temperature[session], self.top_k[session] = request.temperature, request.top_k
+        self.top_p[session], self.min_p[session] = request.top_p, request.min_p
+        for cs, rs in self.gdn.values():
+            cs[session].zero_()
+            rs[session].zero_()
+        self.active[session] = 1
+        return True
+
+    def release(self, *sessions: int) -> None:
+        """Ends the sessions: their pages go back to the pool."""
+        import torch
+
+        from .paged import page_truncate
+        to = torch.full((self.sessions,), -1, dtype=torch.int32)
+        for s in sessions:
+            to[s] = 0
+            self.reserved[s] = 0
+        to = to.to(self.model.device)
+        page_truncate(self.tables, to)
+        self.active.masked_fill_(to == 0, 0)
+
+    def serve(self, requests, eos: int | None = None, generator=None) -> list[list[int]]:
+        """The new tokens of each request, in order: as many as it asks for, or up to
+        and with `eos`.  Requests begin in order as rows and pages are free; the steps
+        are a captured graph's replays.  A device error, which would make the tokens
+        doubtful, is raised (and left for ``device_error`` to read)."""
+        from .gemm import device_error
+        from .gemv import ShapeError
+        requests = list(requests)
+        for r in requests:
+            self._check(r)
+            if self.pages_for(r) > self.pages:
+                raise ShapeError(f"serve: {self.pages_for(r)} pages for one request, the pool has {self.pages}")
+        self.reset()
+        if self.graph is None:
+            import torch
+            self.step(torch.cuda.current_stream(self.model.device).cuda_stream)  # (with no session under way)
+            self.capture()
+            self.reset()
+        out: list[list[int]] = [[] for _ in requests]
+        live: dict[int, int] = {}
+        at = 0
+        while live or at < len(requests):
+            for s in range(self.sessions):
+                if s in live or at == len(requests):
+                    continue
+                if not self.admit(s, requests[at]):
+                    break
+                live[s] = at
+                at += 1
+            if any(requests[r].temperature > 0 for r in live.values()):
+                self.draw(generator)
+            self.graph.replay()
+            done = []
+            for s, t in enumerate(self.emitted.tolist()):
+                if s in live and t >= 0:
+                    r = live[s]
+                    out[r].append(t)
+                    if len(out[r]) == requests[r].new_tokens or t == eos:
+                        done.append(s)
+            if done:
+                self.release(*done)
+                for s in done:
+                    del live[s]
+            error = device_error(reset=False)
+            if error:
+                raise RuntimeError(f"serve: device error {error}")
+        return out
 
 
 def lookup_drafts(history: list[int], nodes: int, match: int = 2):
