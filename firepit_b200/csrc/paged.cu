@@ -15,7 +15,7 @@
 namespace fpb {
 namespace {
 
-constexpr int kPageThreads = 1024, kPageWarps = kPageThreads / 32, kPageCluster = 8, kPageMaxBatch = 16384;
+constexpr int kPageMaxThreads = 1024, kPageMaxBatch = 16384;
 
 struct PageArgs {
   int32_t *table, *lengths, *free, *free_count;
@@ -38,7 +38,7 @@ __device__ __forceinline__ int pages_of(int tokens, int page_size) {
 // Sum of the values before this thread's, and of all of them in *total; the
 // whole block calls this.
 __device__ __forceinline__ long long before(long long v, long long *total, long long *sums) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   long long x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -48,7 +48,7 @@ __device__ __forceinline__ long long before(long long v, long long *total, long 
   __syncthreads();  // the sums of the call before are read
   if (lane == 31) sums[warp] = x;
   __syncthreads();
-  long long s = lane < kPageWarps ? sums[lane] : 0;
+  long long s = lane < warps ? sums[lane] : 0;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const long long y = __shfl_up_sync(0xffffffffu, s, o);
@@ -72,16 +72,23 @@ __device__ __forceinline__ int last_at(const int *at, int n, int x) {
   return lo;
 }
 
-// One cluster: each CTA scans all requests for itself, then they share the rows
-// and the new pages.  A request is served whole (its rows fit, its table and the
-// pool have the pages) or not at all.
-__global__ void __launch_bounds__(kPageThreads) page_extend_kernel(const __grid_constant__ PageArgs a) {
+// What a launch does of a step: all of it (one block), the rows and pages (many
+// blocks), or the state that those have read (one block, behind them).
+enum PagePart { kPageAll, kPageRows, kPageState };
+
+// Each block scans all requests for itself, then the blocks share the rows and the
+// new pages.  A request is served whole (its rows fit, its table and the pool have
+// the pages) or not at all.  Bound by latency: two loads, two scans and the pages'
+// loads in a row (64 requests of a token each 3.5 us; 144000 rows of 96 requests,
+// 1.7 MB, in two launches 8 us, by a cluster of eight blocks 16).
+template <PagePart PART>
+__global__ void __launch_bounds__(kPageMaxThreads) page_extend_kernel(const __grid_constant__ PageArgs a) {
   pdl_enter();
   extern __shared__ int page_sm[];
   int *row0 = page_sm, *off = row0 + a.batch + 1, *len = off + a.batch + 1;  // len -1: not served
-  __shared__ long long sums[kPageWarps];
+  __shared__ long long sums[32];
   __shared__ int used_s;
-  const int tid = threadIdx.x, rank = (int)cluster_ctarank(), ctas = (int)cluster_nctarank();
+  const int tid = threadIdx.x, width = blockDim.x;
   if (tid == 0) used_s = 0;
   int free_n = *a.free_count;
   if (free_n < 0 || free_n > a.pages) {
@@ -90,7 +97,7 @@ __global__ void __launch_bounds__(kPageThreads) page_extend_kernel(const __grid_
   }
   const long long most = (long long)a.max_pages * a.page_size;
   long long rows_before = 0, pages_before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += kPageThreads) {
+  for (int b0 = 0; b0 < a.batch; b0 += width) {
     const int b = b0 + tid;
     const bool in = b < a.batch;
     const int n = in ? a.lengths[b] : 0, c = in ? a.change[b] : 0;
@@ -125,16 +132,17 @@ __global__ void __launch_bounds__(kPageThreads) page_extend_kernel(const __grid_
     row0[a.batch] = a.width ? a.rows : (int)min(rows_before, (long long)a.rows);
     off[a.batch] = (int)min(pages_before, (long long)free_n);
   }
-  cluster_sync();  // every CTA has read the state
+  __syncthreads();
   const int used = used_s;
-  if (rank == 0) {
-    for (int b = tid; b < a.batch; b += kPageThreads)
+  if (PART != kPageRows) {
+    for (int b = tid; b < a.batch; b += width)
       if (len[b] >= 0) a.lengths[b] = len[b] + a.change[b];
     if (a.starts)
-      for (int b = tid; b <= a.batch; b += kPageThreads) a.starts[b] = row0[b];
+      for (int b = tid; b <= a.batch; b += width) a.starts[b] = row0[b];
     if (tid == 0 && used > 0) *a.free_count = free_n - used;
+    if (PART == kPageState) return;
   }
-  const int threads = ctas * kPageThreads, me = rank * kPageThreads + tid;
+  const int threads = gridDim.x * width, me = blockIdx.x * width + tid;
   for (int i = me; i < used; i += threads) {
     const int b = last_at(off, a.batch, i);
     const int page = a.free[free_n - 1 - i];
@@ -176,17 +184,18 @@ __global__ void __launch_bounds__(kPageThreads) page_extend_kernel(const __grid_
   }
 }
 
-// Likewise: each CTA scans the requests, all share the pages.
-__global__ void __launch_bounds__(kPageThreads) page_truncate_kernel(const __grid_constant__ PageArgs a) {
+// Likewise.
+template <PagePart PART>
+__global__ void __launch_bounds__(kPageMaxThreads) page_truncate_kernel(const __grid_constant__ PageArgs a) {
   pdl_enter();
   extern __shared__ int page_sm[];
   int *off = page_sm, *kept = off + a.batch + 1;  // kept: pages that the request keeps
-  __shared__ long long sums[kPageWarps];
-  const int tid = threadIdx.x, rank = (int)cluster_ctarank(), ctas = (int)cluster_nctarank();
+  __shared__ long long sums[32];
+  const int tid = threadIdx.x, width = blockDim.x;
   const int free_n = *a.free_count;
   const long long most = (long long)a.max_pages * a.page_size;
   long long back = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += kPageThreads) {
+  for (int b0 = 0; b0 < a.batch; b0 += width) {
     const int b = b0 + tid;
     const bool in = b < a.batch;
     const int n = in ? a.lengths[b] : 0, to = in ? a.change[b] : -1;
@@ -203,17 +212,18 @@ __global__ void __launch_bounds__(kPageThreads) page_truncate_kernel(const __gri
     back += total;
   }
   if (tid == 0) off[a.batch] = (int)min(back, (long long)a.pages);
-  cluster_sync();  // every CTA has read the state
+  __syncthreads();
   if (free_n < 0 || back > a.pages - free_n) {  // more than the pool can have: nothing is taken back
     if (tid == 0) page_error(a, kErrLength);
     return;
   }
-  if (rank == 0) {
-    for (int b = tid; b < a.batch; b += kPageThreads)
+  if (PART != kPageRows) {
+    for (int b = tid; b < a.batch; b += width)
       if (kept[b] >= 0) a.lengths[b] = a.change[b];
     if (tid == 0 && back > 0) *a.free_count = free_n + (int)back;
+    if (PART == kPageState) return;
   }
-  for (int i = rank * kPageThreads + tid; i < (int)back; i += ctas * kPageThreads) {
+  for (int i = blockIdx.x * width + tid; i < (int)back; i += gridDim.x * width) {
     const int b = last_at(off, a.batch, i);
     int32_t *entry = a.table + b * a.pitch + kept[b] + i - off[b];
     const int page = *entry;
@@ -235,8 +245,9 @@ int check_tables(const char *name, const PageArgs &a, size_t table_pitch, size_t
   return FPB_OK;
 }
 
-// One cluster; one CTA where a step has few rows and pages.
-int launch_pages(void (*kernel)(PageArgs), const char *name, const PageArgs &a, size_t work, size_t smem,
+// One block where a step has few rows or pages; else many for those, and one behind
+// them for the state (from 8192 rows on: 6.4 us against 6.6).
+int launch_pages(void (*const (&kernel)[3])(PageArgs), const char *name, const PageArgs &a, size_t work, size_t smem,
                  cudaStream_t s) {
   {
     static std::mutex mu;
@@ -245,17 +256,25 @@ int launch_pages(void (*kernel)(PageArgs), const char *name, const PageArgs &a, 
     FPB_CUDA_TRY(cudaGetDevice(&dev));
     std::lock_guard<std::mutex> lock(mu);
     if (std::find(done.begin(), done.end(), dev) == done.end()) {
-      for (auto k : {page_extend_kernel, page_truncate_kernel})
+      for (auto k : {page_extend_kernel<kPageAll>, page_extend_kernel<kPageRows>, page_extend_kernel<kPageState>,
+                     page_truncate_kernel<kPageAll>, page_truncate_kernel<kPageRows>, page_truncate_kernel<kPageState>})
         FPB_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                           (int)(3 * (kPageMaxBatch + 1) * sizeof(int))));
       done.push_back(dev);
     }
   }
-  const unsigned ctas = work > 4 * kPageThreads ? kPageCluster : 1;
-  cudaError_t e = launch_pdl_cluster(kernel, ctas, kPageThreads, smem, s, ctas, a);
-  if (e != cudaSuccess) return cuda_fail(e, name);
-  FPB_LAUNCH_CHECK(name);
-  return FPB_OK;
+  auto launch = [&](PagePart part, unsigned blocks, unsigned threads) {
+    cudaError_t e = launch_pdl(kernel[part], blocks, threads, smem, s, a);
+    if (e != cudaSuccess) return cuda_fail(e, name);
+    FPB_LAUNCH_CHECK(name);
+    return (int)FPB_OK;
+  };
+  // (a wide block's barriers take longer, a narrow one goes through its work more often)
+  const unsigned scan = a.batch <= 256 ? 256 : kPageMaxThreads;
+  if (work <= 8192) return launch(kPageAll, 1, work <= 1024 ? scan : kPageMaxThreads);
+  const size_t blocks = std::min<size_t>((work + 4 * scan - 1) / (4 * scan), 2 * sm_count());
+  if (int st = launch(kPageRows, (unsigned)blocks, scan)) return st;
+  return launch(kPageState, 1, scan);
 }
 
 PageArgs page_args(int32_t *table, size_t table_pitch, size_t batch, size_t max_pages, int32_t *lengths,
@@ -297,8 +316,8 @@ extern "C" int fpb_page_extend(int32_t *table, size_t table_pitch, size_t batch,
   a.starts = starts;
   a.vec = aligned_to(slots, 16) && aligned_to(positions, 16) && aligned_to(requests, 16);
   a.error = device_error_ptr();
-  return launch_pages(page_extend_kernel, "page_extend_kernel", a, rows, 3 * (batch + 1) * sizeof(int),
-                      as_stream(stream));
+  return launch_pages({page_extend_kernel<kPageAll>, page_extend_kernel<kPageRows>, page_extend_kernel<kPageState>},
+                      "page_extend_kernel", a, rows, 3 * (batch + 1) * sizeof(int), as_stream(stream));
 }
 
 extern "C" int fpb_page_truncate(int32_t *table, size_t table_pitch, size_t batch, size_t max_pages, int32_t *lengths,
@@ -308,6 +327,7 @@ extern "C" int fpb_page_truncate(int32_t *table, size_t table_pitch, size_t batc
                          page_size);
   if (int st = check_tables("fpb_page_truncate", a, table_pitch, batch, max_pages, pages, page_size)) return st;
   a.error = device_error_ptr();
-  return launch_pages(page_truncate_kernel, "page_truncate_kernel", a, std::min(batch * max_pages, pages),
-                      2 * (batch + 1) * sizeof(int), as_stream(stream));
+  return launch_pages({page_truncate_kernel<kPageAll>, page_truncate_kernel<kPageRows>, page_truncate_kernel<kPageState>},
+                      "page_truncate_kernel", a, std::min(batch * max_pages, pages), 2 * (batch + 1) * sizeof(int),
+                      as_stream(stream));
 }

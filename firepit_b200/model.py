@@ -736,13 +736,12 @@ class PagedDecoder(Decoder):
 
     def _attend(self, i, L, sh: int) -> None:
         c, B, D, kv, t = self.cfg, self.batch, self.cfg.head_dim, self.kv[i], self.tables
-        shape = (kv.code, self.pages, self.page_size, *kv.pitches)
         N.call("fpb_paged_append", self.qg.data_ptr(), self.qg.shape[1], 2 * D, self.kp.data_ptr(), self.kp.shape[1],
                self.vp.data_ptr(), self.vp.shape[1], N.FPB_F32, L["q_norm"].data_ptr(), L["k_norm"].data_ptr(),
                self.map.slots.data_ptr(), self.map.positions.data_ptr(), B, c.q_heads, c.kv_heads, D, c.rotary_dim,
-               c.rope_theta, c.eps, self.q_rot.data_ptr(), N.FPB_F32, kv.k.data_ptr(), kv.v.data_ptr(), *shape, sh)
-        N.call("fpb_paged_attn", self.q_rot.data_ptr(), N.FPB_F32, c.q_heads * D, D, kv.k.data_ptr(), kv.v.data_ptr(),
-               *shape, t.table.data_ptr(), t.pitch, t.table.shape[1], t.lengths.data_ptr(),
+               c.rope_theta, c.eps, self.q_rot.data_ptr(), N.FPB_F32, *kv.address, *kv.layout, sh)
+        N.call("fpb_paged_attn", self.q_rot.data_ptr(), N.FPB_F32, c.q_heads * D, D, *kv.address, *kv.layout,
+               t.table.data_ptr(), t.pitch, t.table.shape[1], t.lengths.data_ptr(),
                self.qg.data_ptr() + 4 * D, self.qg.shape[1], 2 * D, B, c.q_heads, c.kv_heads, D, 1.0 / math.sqrt(D),
                self.attn_ws.data_ptr(), self.attn_ws.numel(), self.attn.data_ptr(), N.FPB_BF16, sh)
 
@@ -765,9 +764,8 @@ class PagedDecoder(Decoder):
 
     def step(self, sh: int) -> None:
         t, m = self.tables, self.map
-        N.call("fpb_page_extend", t.table.data_ptr(), t.pitch, self.batch, t.table.shape[1], t.lengths.data_ptr(),
-               self.active.data_ptr(), t.free.data_ptr(), t.free_count.data_ptr(), self.pages, self.page_size,
-               self.batch, 1, m.slots.data_ptr(), m.positions.data_ptr(), m.requests.data_ptr(), m.starts.data_ptr(), sh)
+        N.call("fpb_page_extend", *t.address, self.active.data_ptr(), *t.pool, self.batch, 1, m.slots.data_ptr(),
+               m.positions.data_ptr(), m.requests.data_ptr(), m.starts.data_ptr(), sh)
         super().step(sh)
 
     def draw(self, generator=None) -> None:

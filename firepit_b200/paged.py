@@ -18,10 +18,21 @@ from dataclasses import dataclass
 
 from . import _native as N
 from .gemv import ShapeError
-from .speculative import _code, _empty, _handle, _ints, _on_device, _ptr, _rows, _Torch
+from .speculative import _code, _empty, _ints, _Torch
+
+# (a decode step's calls take a few microseconds each: the entry points are looked
+# up once, and the checks read each property once)
+_extend, _truncate, _append = N.lib.fpb_page_extend, N.lib.fpb_page_truncate, N.lib.fpb_paged_append
+_attn, _attn_bytes, _sample = N.lib.fpb_paged_attn, N.lib.fpb_paged_attn_workspace_bytes, N.lib.fpb_sample
 
 
-@dataclass
+def _keep(self, **values) -> None:
+    """What the entry points take of an object, as they take it."""
+    for name, value in values.items():
+        object.__setattr__(self, name, value)
+
+
+@dataclass(frozen=True)
 class PagedCache:
     """k, v [pages, page_size, kv_heads, head_dim] f32 or bf16: any strides that
     are the same for both and multiples of 16 bytes, the last dimension
@@ -37,7 +48,7 @@ class PagedCache:
         if k.dim() != 4 or k.shape[3] % 16 or not 0 < k.shape[3] <= 256:
             raise ShapeError(f"pages: [pages, page_size, kv_heads, head_dim % 16 == 0 <= 256] expected, got "
                              f"{list(k.shape)}")
-        self.code = _code(k)
+        code = _code(k)
         if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device or v.stride() != k.stride():
             raise ShapeError("pages: k and v of one shape, type, device and stride expected")
         # (the pitch of a dimension of one is never used)
@@ -45,9 +56,11 @@ class PagedCache:
         st = k.stride()
         if st[3] != 1:
             raise ShapeError("pages: the last dimension must be contiguous")
-        self.pitches = (st[0] if n > 1 else p * h * d, st[1] if p > 1 else h * d, st[2] if h > 1 else d)
-        if any(s < d or s * k.element_size() % 16 for s in self.pitches):
+        pitches = (st[0] if n > 1 else p * h * d, st[1] if p > 1 else h * d, st[2] if h > 1 else d)
+        if any(s < d or s * k.element_size() % 16 for s in pitches):
             raise ShapeError(f"pages: strides {list(st)} have to be multiples of 16 bytes and hold a head vector")
+        _keep(self, code=code, device=k.get_device(), dtype=k.dtype, dims=(n, p, h, d),
+              address=(k.data_ptr(), v.data_ptr()), layout=(code, n, p, *pitches))
 
     @classmethod
     def zeros(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=None, device="cuda") -> "PagedCache":
@@ -64,7 +77,7 @@ class PagedCache:
         return 2 * self.k.numel() * self.k.element_size()
 
 
-@dataclass
+@dataclass(frozen=True)
 class PageTables:
     """Which pages of a pool are whose: table [batch, max_pages] (any row pitch),
     lengths [batch] (the tokens that each request holds), free [pages] (a stack of
@@ -88,6 +101,12 @@ class PageTables:
         _ints(self.free_count, "free_count", 1)
         if self.page_size < 1:
             raise ShapeError(f"tables: pages of {self.page_size} tokens")
+        for x in (self.lengths, self.free, self.free_count):
+            if x.device != t.device:
+                raise ShapeError(f"tables: tensors on {t.device} and {x.device}")
+        _keep(self, device=t.get_device(), batch=t.shape[0],
+              address=(t.data_ptr(), _pitch(t), t.shape[0], t.shape[1], self.lengths.data_ptr()),
+              pool=(self.free.data_ptr(), self.free_count.data_ptr(), self.free.shape[0], self.page_size))
 
     @classmethod
     def empty(cls, batch: int, pages: int, page_size: int, max_pages: int, device="cuda") -> "PageTables":
@@ -118,41 +137,79 @@ def _pitch(t) -> int:
     return t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1])
 
 
+def _heads(t, n: int, h: int, d: int):
+    """(row pitch, head pitch) of t [n, h, d], d contiguous."""
+    row, head, one = t.stride()
+    if one != 1 and d != 1:
+        raise ShapeError(f"a head vector must be contiguous, got strides {t.stride()}")
+    return row if n > 1 else h * d, head if h > 1 else d
+
+
+def _elsewhere(what: str, device: int, *tensors):
+    """The tensors' addresses are what the kernels get, so they lie on the current
+    CUDA device: the error that says which does not."""
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            return ShapeError(f"{what}: tensors on device {device} and on {t.device}")
+    return ShapeError(f"{what}: tensors on device {device}, which is not the current CUDA device")
+
+
+def _done(status: int, name: str) -> None:
+    if status:
+        N.check(status, name)
+
+
+def _at(t, device: int):
+    """The address of an optional tensor, which has to lie on the device (else -1)."""
+    return None if t is None else t.data_ptr() if t.get_device() == device else -1
+
+
 def page_extend(tables: PageTables, counts, rows: int, padded: bool = False, out: PageMap | None = None,
                 stream=None) -> PageMap:
     """Takes pages for counts [batch] new tokens of each request and says where
     they lie: rows in order of request (``padded``: rows / batch of them a request).
     A request that the pool, its table or the rows cannot hold whole keeps its
     length, and its rows are -1."""
-    b, width = tables.table.shape
+    b, device = tables.batch, tables.device
     _ints(counts, "counts", b)
     if rows < 1 or (padded and rows % b):
         raise ShapeError(f"page_extend: {rows} rows of {b} requests")
-    if out is not None:
-        for t, what, n in ((out.slots, "slots", rows), (out.positions, "positions", rows),
-                           (out.requests, "requests", rows), (out.starts, "starts", b + 1)):
+    if device < 0 or device != counts.get_device() or device != _Torch.current_device():
+        raise _elsewhere("page_extend", device, counts)
+    if out is None:
+        # one allocation: three rows of a multiple of four, and the starts
+        up = (rows + 3) // 4 * 4
+        flat = _empty(stream, counts, _Torch.i32, 3 * up + b + 1)
+        if up == rows:
+            out = PageMap(*flat.split_with_sizes((rows, rows, rows, b + 1)))
+        else:
+            parts = flat.split_with_sizes((rows, up - rows, rows, up - rows, rows, up - rows, b + 1))
+            out = PageMap(parts[0], parts[2], parts[4], parts[6])
+        first = flat.data_ptr()
+        at = first, first + 4 * up, first + 8 * up, first + 12 * up
+    else:
+        given = (out.slots, "slots", rows), (out.positions, "positions", rows), (out.requests, "requests", rows), (
+            out.starts, "starts", b + 1)
+        for t, what, n in given:
             if t is not None or what in ("slots", "positions"):
                 _ints(t, what, n)
-    _on_device("page_extend", tables.table, tables.lengths, tables.free, tables.free_count, counts,
-               *(() if out is None else (out.slots, out.positions, out.requests, out.starts)))
-    if out is None:
-        out = PageMap(*(_empty(stream, counts, _Torch.i32, n) for n in (rows, rows, rows, b + 1)))
-    N.call("fpb_page_extend", tables.table.data_ptr(), tables.pitch, b, width, tables.lengths.data_ptr(),
-           counts.data_ptr(), tables.free.data_ptr(), tables.free_count.data_ptr(), tables.free.shape[0],
-           tables.page_size, rows, int(padded), out.slots.data_ptr(), out.positions.data_ptr(), _ptr(out.requests),
-           _ptr(out.starts), _handle(stream, counts))
+        at = [_at(t, device) for t, _, _ in given]
+        if -1 in at:
+            raise _elsewhere("page_extend", device, out.slots, out.positions, out.requests, out.starts)
+    _done(_extend(*tables.address, counts.data_ptr(), *tables.pool, rows, padded, *at,
+                  _Torch.raw_stream(device) if stream is None else stream), "fpb_page_extend")
     return out
 
 
 def page_truncate(tables: PageTables, lengths, stream=None) -> None:
     """Cuts the requests to lengths [batch] (negative, or not below the present
     one: as it was; 0: the request is done) and gives their pages back."""
-    b, width = tables.table.shape
-    _ints(lengths, "lengths", b)
-    _on_device("page_truncate", tables.table, tables.lengths, tables.free, tables.free_count, lengths)
-    N.call("fpb_page_truncate", tables.table.data_ptr(), tables.pitch, b, width, tables.lengths.data_ptr(),
-           lengths.data_ptr(), tables.free.data_ptr(), tables.free_count.data_ptr(), tables.free.shape[0],
-           tables.page_size, _handle(stream, lengths))
+    device = tables.device
+    _ints(lengths, "lengths", tables.batch)
+    if device < 0 or device != lengths.get_device() or device != _Torch.current_device():
+        raise _elsewhere("page_truncate", device, lengths)
+    _done(_truncate(*tables.address, lengths.data_ptr(), *tables.pool,
+                    _Torch.raw_stream(device) if stream is None else stream), "fpb_page_truncate")
 
 
 def paged_append(cache: PagedCache, slots, positions, k, v, q=None, q_gamma=None, k_gamma=None, eps: float = 1e-6,
@@ -161,44 +218,51 @@ def paged_append(cache: PagedCache, slots, positions, k, v, q=None, q_gamma=None
     positions [rows] and writes it and v at slots [rows] (negative: no token; no two
     alike); q [rows, q_heads, head_dim] (any row and head pitch) is normed and rotated
     into q_out (allocated in q's dtype where None), which is returned."""
-    _, p, hk, d = cache.shape
-    if k.dim() != 3 or k.shape[1:] != (hk, d) or v.shape != k.shape or v.dtype != k.dtype:
-        raise ShapeError(f"paged_append: k, v [rows, {hk}, {d}] of one dtype expected, got {list(k.shape)} {k.dtype}, "
+    _, _, hk, d = cache.dims
+    device, shape, dtype = cache.device, k.shape, k.dtype
+    if len(shape) != 3 or shape[1] != hk or shape[2] != d or v.shape != shape or v.dtype is not dtype:
+        raise ShapeError(f"paged_append: k, v [rows, {hk}, {d}] of one dtype expected, got {list(shape)} {dtype}, "
                          f"{list(v.shape)} {v.dtype}")
-    n = k.shape[0]
+    n = shape[0]
+    code = _code(k)
     _ints(slots, "slots", n)
     _ints(positions, "positions", n)
-    for t, what in ((k, "k"), (v, "v")):
-        if hk > 1 and t.stride(1) != d:
-            raise ShapeError(f"paged_append: {what}'s heads must be contiguous")
+    k_pitch, k_head = _heads(k, n, hk, d)
+    v_pitch, v_head = _heads(v, n, hk, d)
+    if k_head != d or v_head != d:
+        raise ShapeError("paged_append: the heads of k and v must be contiguous")
     for g in (q_gamma, k_gamma):
-        if g is not None and (g.shape != (d,) or _code(g) != N.FPB_F32 or not g.is_contiguous()):
+        if g is not None and (g.dtype is not _Torch.f32 or g.shape != (d,) or not g.is_contiguous()):
             raise ShapeError(f"paged_append: gammas [{d}] f32 expected")
-    hq, q_pitch, q_head, out_code = 0, 0, 0, N.FPB_F32
+    hq = q_pitch = q_head = out_code = 0
     if q is not None:
-        if q.dim() != 3 or q.shape[0] != n or q.shape[2] != d or q.dtype != k.dtype:
+        if q.dim() != 3 or q.shape[0] != n or q.shape[2] != d or q.dtype is not dtype:
             raise ShapeError(f"paged_append: q [{n}, q_heads, {d}] of k's dtype expected, got {list(q.shape)} {q.dtype}")
-        hq, q_pitch = q.shape[1], _rows(q, "q", n, 1)
-        q_head = q.stride(1) if hq > 1 else d
-        if q_out is not None and (q_out.shape != (n, hq, d) or not q_out.is_contiguous()):
-            raise ShapeError(f"paged_append: q_out [{n}, {hq}, {d}] contiguous expected")
-        out_code = _code(q if q_out is None else q_out)
+        hq, out_code = q.shape[1], code
+        q_pitch, q_head = _heads(q, n, hq, d)
+        if q_out is not None:
+            out_code = _code(q_out)
+            if q_out.shape != (n, hq, d) or not q_out.is_contiguous():
+                raise ShapeError(f"paged_append: q_out [{n}, {hq}, {d}] contiguous expected")
     elif q_out is not None:
         raise ShapeError("paged_append: q_out without q")
-    k_code, k_pitch, v_pitch = _code(k), _rows(k, "k", n, 1), _rows(v, "v", n, 1)
-    _on_device("paged_append", cache.k, slots, positions, k, v, q, q_gamma, k_gamma, q_out)
+    at = [_at(t, device) for t in (q, q_gamma, k_gamma, q_out)]
+    if device < 0 or not (device == k.get_device() == v.get_device() == slots.get_device() == positions.get_device() ==
+                          _Torch.current_device()) or -1 in at:
+        raise _elsewhere("paged_append", device, k, v, slots, positions, q, q_gamma, k_gamma, q_out)
     if q is not None and q_out is None:
-        q_out = _empty(stream, q, q.dtype, n, hq, d)
+        q_out = _empty(stream, q, dtype, n, hq, d)
+        at[3] = q_out.data_ptr()
     if n:
-        N.call("fpb_paged_append", _ptr(q), q_pitch, q_head, k.data_ptr(), k_pitch, v.data_ptr(), v_pitch, k_code,
-               _ptr(q_gamma), _ptr(k_gamma), slots.data_ptr(), positions.data_ptr(), n, hq, hk, d, rotary_dim, theta,
-               eps, _ptr(q_out), out_code, cache.k.data_ptr(), cache.v.data_ptr(), cache.code, cache.shape[0], p,
-               *cache.pitches, _handle(stream, k))
+        _done(_append(at[0], q_pitch, q_head, k.data_ptr(), k_pitch, v.data_ptr(), v_pitch, code, at[1], at[2],
+                      slots.data_ptr(), positions.data_ptr(), n, hq, hk, d, rotary_dim, theta, eps, at[3], out_code,
+                      *cache.address, *cache.layout, _Torch.raw_stream(device) if stream is None else stream),
+              "fpb_paged_append")
     return q_out
 
 
 def paged_attention_workspace_bytes(cache: PagedCache, batch: int, q_heads: int) -> int:
-    return int(N.lib.fpb_paged_attn_workspace_bytes(batch, q_heads, cache.shape[2], cache.shape[3]))
+    return int(_attn_bytes(batch, q_heads, cache.shape[2], cache.shape[3]))
 
 
 def paged_attention(q, cache: PagedCache, table, lengths, gate=None, scale: float | None = None, out=None,
@@ -210,35 +274,48 @@ def paged_attention(q, cache: PagedCache, table, lengths, gate=None, scale: floa
     q [batch, q_heads, head_dim] f32 or bf16, any row and head pitch; scale default
     1 / sqrt(head_dim); ``workspace``: uint8 of ``paged_attention_workspace_bytes``
     (allocated where None), which calls on different streams must not share."""
-    pages, p, hk, d = cache.shape
-    if q.dim() != 3 or q.shape[2] != d or q.shape[1] % hk or not q.shape[1]:
-        raise ShapeError(f"paged_attention: q [batch, a multiple of {hk}, {d}] expected, got {list(q.shape)}")
-    b, hq = q.shape[0], q.shape[1]
-    if table.dim() != 2 or table.dtype is not _Torch.i32 or table.shape[0] != b or (
-            table.shape[1] > 1 and table.stride(1) != 1):
+    _, _, hk, d = cache.dims
+    device, shape = cache.device, q.shape
+    if len(shape) != 3 or shape[2] != d or shape[1] % hk or not shape[1]:
+        raise ShapeError(f"paged_attention: q [batch, a multiple of {hk}, {d}] expected, got {list(shape)}")
+    b, hq, _ = shape
+    width = table.shape
+    if len(width) != 2 or table.dtype is not _Torch.i32 or width[0] != b or (width[1] > 1 and table.stride(1) != 1):
         raise ShapeError(f"paged_attention: table int32 [{b}, max_pages] expected, got {table.dtype} "
                          f"{list(table.shape)}")
+    width = width[1]
     _ints(lengths, "lengths", b)
-    q_code, q_pitch, gate_pitch, gate_head = _code(q), _rows(q, "q", b, 1), 0, 0
+    q_code = _code(q)
+    q_pitch, q_head = _heads(q, b, hq, d)
+    gate_pitch = gate_head = 0
     if gate is not None:
-        if gate.shape != q.shape or gate.dtype is not _Torch.f32:
-            raise ShapeError(f"paged_attention: gate f32 {list(q.shape)} expected")
-        gate_pitch, gate_head = _rows(gate, "gate", b, 1), gate.stride(1) if hq > 1 else d
-    out_code = cache.code if out is None else _code(out)
-    if out is not None and (out.shape != q.shape or not out.is_contiguous()):
-        raise ShapeError("paged_attention: out of q's shape, contiguous, expected")
+        if gate.shape != shape or gate.dtype is not _Torch.f32:
+            raise ShapeError(f"paged_attention: gate f32 {list(shape)} expected")
+        gate_pitch, gate_head = _heads(gate, b, hq, d)
+    out_code = cache.code
+    if out is not None:
+        out_code = _code(out)
+        if out.shape != shape or not out.is_contiguous():
+            raise ShapeError("paged_attention: out of q's shape, contiguous, expected")
     if workspace is not None and (workspace.dtype is not _Torch.u8 or not workspace.is_contiguous()):
         raise ShapeError("paged_attention: workspace contiguous uint8 expected")
-    _on_device("paged_attention", cache.k, q, table, lengths, gate, out, workspace)
-    if out is None:
-        out = _empty(stream, q, cache.k.dtype, b, hq, d)
+    at = [_at(gate, device), _at(out, device), _at(workspace, device)]
+    if device < 0 or not (device == q.get_device() == table.get_device() == lengths.get_device() ==
+                          _Torch.current_device()) or -1 in at:
+        raise _elsewhere("paged_attention", device, q, table, lengths, gate, out, workspace)
     if workspace is None:
-        workspace = _empty(stream, q, _Torch.u8, N.lib.fpb_paged_attn_workspace_bytes(b, hq, hk, d))
-    N.call("fpb_paged_attn", q.data_ptr(), q_code, q_pitch, q.stride(1) if hq > 1 else d, cache.k.data_ptr(),
-           cache.v.data_ptr(), cache.code, pages, p, *cache.pitches, table.data_ptr(), _pitch(table), table.shape[1],
-           lengths.data_ptr(), _ptr(gate), gate_pitch, gate_head, b, hq, hk, d,
-           1.0 / math.sqrt(d) if scale is None else scale, workspace.data_ptr(), workspace.numel(), out.data_ptr(),
-           out_code, _handle(stream, q))
+        room = _attn_bytes(b, hq, hk, d)
+        workspace = _empty(stream, q, _Torch.u8, room)
+        at[2] = workspace.data_ptr()
+    else:
+        room = workspace.numel()
+    if out is None:
+        out = _empty(stream, q, cache.dtype, b, hq, d)
+        at[1] = out.data_ptr()
+    _done(_attn(q.data_ptr(), q_code, q_pitch, q_head, *cache.address, *cache.layout, table.data_ptr(),
+                table.stride(0) if b > 1 else max(1, width), width, lengths.data_ptr(), at[0], gate_pitch, gate_head, b,
+                hq, hk, d, 1.0 / math.sqrt(d) if scale is None else scale, at[2], room, at[1], out_code,
+                _Torch.raw_stream(device) if stream is None else stream), "fpb_paged_attn")
     return out
 
 
@@ -258,22 +335,26 @@ def sample(logits, temperature, noise, top_k=None, top_p=None, min_p=None, logpr
         _Torch.load()
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ShapeError(f"sample: logits [batch, vocab], rows contiguous, expected, got {list(logits.shape)}")
-    b, vocab = logits.shape
-    code = _code(logits)
-    if noise.dtype is not _Torch.f32 or noise.shape != (b, vocab) or (vocab > 1 and noise.stride(1) != 1):
+    b, vocab = shape = logits.shape
+    code, f32 = _code(logits), _Torch.f32
+    if noise.dtype is not f32 or noise.shape != shape or (vocab > 1 and noise.stride(1) != 1):
         raise ShapeError(f"sample: noise f32 [{b}, {vocab}] expected")
+    device = logits.get_device()
     for t, what in ((temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p")):
-        if (t is not None or what == "temperature") and (t.dtype is not _Torch.f32 or t.shape != (b,) or
+        if (t is not None or what == "temperature") and (t.dtype is not f32 or t.shape != (b,) or
                                                          not t.is_contiguous()):
             raise ShapeError(f"sample: {what} f32 [{b}] expected")
     if top_k is not None:
         _ints(top_k, "top_k", b)
     if out is not None:
         _ints(out, "out", b)
-    _on_device("sample", logits, temperature, noise, top_k, top_p, min_p, out)
+    at = [_at(t, device) for t in (temperature, top_k, top_p, min_p, noise, out)]
+    if device < 0 or device != _Torch.current_device() or -1 in at:
+        raise _elsewhere("sample", device, temperature, top_k, top_p, min_p, noise, out)
     tokens = _empty(stream, logits, _Torch.i32, b) if out is None else out
-    logs = _empty(stream, logits, _Torch.f32, b) if logprobs else None
-    N.call("fpb_sample", logits.data_ptr(), code, _pitch(logits), temperature.data_ptr(), _ptr(top_k), _ptr(top_p),
-           _ptr(min_p), noise.data_ptr(), _pitch(noise), b, vocab, tokens.data_ptr(), _ptr(logs),
-           _handle(stream, logits))
+    logs = _empty(stream, logits, f32, b) if logprobs else None
+    _done(_sample(logits.data_ptr(), code, logits.stride(0) if b > 1 else vocab, *at[:5],
+                  noise.stride(0) if b > 1 else vocab, b, vocab, tokens.data_ptr(),
+                  logs.data_ptr() if logprobs else None, _Torch.raw_stream(device) if stream is None else stream),
+          "fpb_sample")
     return (tokens, logs) if logprobs else tokens
