@@ -142,15 +142,17 @@ __global__ void __launch_bounds__(kPageMaxThreads) page_extend_kernel(const __gr
     if (tid == 0 && used > 0) *a.free_count = free_n - used;
     if (PART == kPageState) return;
   }
-  const int threads = gridDim.x * width, me = blockIdx.x * width + tid;
-  for (int i = me; i < used; i += threads) {
-    const int b = last_at(off, a.batch, i);
-    const int page = a.free[free_n - 1 - i];
+  // (whole numbers without a sign: a step past the last row may pass 2^31)
+  const uint32_t threads = gridDim.x * width, me = blockIdx.x * width + tid;
+  for (uint32_t i = me; i < (uint32_t)used; i += threads) {
+    const int b = last_at(off, a.batch, (int)i);
+    const int page = a.free[free_n - 1 - (int)i];
     if (page < 0 || page >= a.pages) page_error(a, kErrPage);
-    a.table[b * a.pitch + pages_of(len[b], a.page_size) + i - off[b]] = page;
+    a.table[b * a.pitch + pages_of(len[b], a.page_size) + (int)i - off[b]] = page;
   }
   // four rows a thread
-  for (int r0 = me * 4; r0 < a.rows; r0 += threads * 4) {
+  for (uint32_t u0 = me * 4; u0 < (uint32_t)a.rows; u0 += threads * 4) {
+    const int r0 = (int)u0;
     int slot[4], pos[4], req[4];
     int b = a.width ? r0 / a.width : last_at(row0, a.batch, r0);
 #pragma unroll
@@ -223,8 +225,8 @@ __global__ void __launch_bounds__(kPageMaxThreads) page_truncate_kernel(const __
     if (tid == 0 && back > 0) *a.free_count = free_n + (int)back;
     if (PART == kPageState) return;
   }
-  for (int i = blockIdx.x * width + tid; i < (int)back; i += gridDim.x * width) {
-    const int b = last_at(off, a.batch, i);
+  for (uint32_t u = blockIdx.x * width + tid; u < (uint32_t)back; u += gridDim.x * width) {
+    const int i = (int)u, b = last_at(off, a.batch, i);
     int32_t *entry = a.table + b * a.pitch + kept[b] + i - off[b];
     const int page = *entry;
     if (page < 0 || page >= a.pages) page_error(a, kErrPage);
@@ -308,6 +310,8 @@ extern "C" int fpb_page_extend(int32_t *table, size_t table_pitch, size_t batch,
   if (!slots || !positions) return fail(FPB_ERR_INVALID_ARGUMENT, "fpb_page_extend: null pointer");
   if (rows == 0 || rows > 0x7ffffff0 || (padded && rows % batch))
     return fail(FPB_ERR_SHAPE, "fpb_page_extend: %zu rows (padded: a multiple of the batch, %zu)", rows, batch);
+  if (counts < lengths + batch && lengths < counts + batch)  // (a block reads counts behind another's lengths)
+    return fail(FPB_ERR_INVALID_ARGUMENT, "fpb_page_extend: counts overlap the lengths");
   a.rows = (int)rows;
   a.width = padded ? (int)(rows / batch) : 0;
   a.slots = slots;

@@ -353,7 +353,7 @@ __device__ __forceinline__ bool paged_share(const PagedArgs &a, int *steps, Page
   // the session of this block, and the slots of split sessions before it
   int blocks0 = 0, slots0 = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
-    const int b = b0 + tid, n = b < a.batch ? (steps[b] + S - 1) / S : 0;
+    const int b = b0 + tid, n = b < a.batch ? (int)(((uint32_t)steps[b] + S - 1) / S) : 0;
     int blocks = n * heads, slots = n > 1 ? blocks : 0, x = blocks, y = slots;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {

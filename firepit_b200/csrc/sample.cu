@@ -511,7 +511,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       const double before = by_p ? before_in_list(w) : 0.0;
       if (by_k && by_p) whole = block_sum(w);
       const bool in = tid < most && (tid == 0 || !by_p || before < (double)p * whole) && w >= least;
-      const Best pick = block_best(in ? Best{w * inverse(e), token} : Best{0.0f, top.i});
+      // (a number that is none, of a noise of none or a weight of 0 over a noise of 0, wins no race)
+      const Best pick = block_best(in ? Best{fmaxf(w * inverse(e), 0.0f), token} : Best{0.0f, top.i});
       const double s = block_sum(in ? w : 0.0f);
       if (tid < most && token == pick.i) answer(token, x, s);
       __syncwarp();

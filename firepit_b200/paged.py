@@ -36,7 +36,8 @@ def _keep(self, **values) -> None:
 class PagedCache:
     """k, v [pages, page_size, kv_heads, head_dim] f32 or bf16: any strides that
     are the same for both and multiples of 16 bytes, the last dimension
-    contiguous (heads-first pages are a transposed view)."""
+    contiguous (heads-first pages are a transposed view).  Their addresses, shapes and
+    strides are read once, here: the tensors are written to, not given other storage."""
 
     k: object
     v: object
@@ -81,7 +82,8 @@ class PagedCache:
 class PageTables:
     """Which pages of a pool are whose: table [batch, max_pages] (any row pitch),
     lengths [batch] (the tokens that each request holds), free [pages] (a stack of
-    the pages that nobody holds) and free_count [1], all int32 on the device."""
+    the pages that nobody holds) and free_count [1], all int32 on the device.  As in
+    ``PagedCache``, their addresses and shapes are read once."""
 
     table: object
     lengths: object
@@ -166,8 +168,8 @@ def _at(t, device: int):
 
 def page_extend(tables: PageTables, counts, rows: int, padded: bool = False, out: PageMap | None = None,
                 stream=None) -> PageMap:
-    """Takes pages for counts [batch] new tokens of each request and says where
-    they lie: rows in order of request (``padded``: rows / batch of them a request).
+    """Takes pages for counts [batch] new tokens of each request (not the tables' own
+    lengths) and says where they lie: rows in order of request (``padded``: rows / batch of them a request).
     A request that the pool, its table or the rows cannot hold whole keeps its
     length, and its rows are -1."""
     b, device = tables.batch, tables.device
@@ -327,8 +329,8 @@ def sample(logits, temperature, noise, top_k=None, top_p=None, min_p=None, logpr
     shortest part of those whose weights exp((l - max) / temperature) reach p of their
     sum, min_p those of at least min_p of the largest weight; the token is argmax weight /
     noise over what is kept.  noise [batch, vocab] f32: exponential variates.
-    temperature (0 or below: greedy), top_p, min_p [batch] f32 and top_k [batch] int32,
-    on the device; None for a filter: none (top_k 0, top_p 1 and min_p 0 do nothing).
+    temperature (0 or below: greedy; None: 1), top_p, min_p [batch] f32 and top_k [batch]
+    int32, on the device; None for a filter: none (top_k 0, top_p 1 and min_p 0 do nothing).
     With ``logprobs``, (tokens, logprobs [batch] f32): the log of the token's weight
     among what is kept."""
     if _Torch.module is None:
@@ -341,8 +343,7 @@ def sample(logits, temperature, noise, top_k=None, top_p=None, min_p=None, logpr
         raise ShapeError(f"sample: noise f32 [{b}, {vocab}] expected")
     device = logits.get_device()
     for t, what in ((temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p")):
-        if (t is not None or what == "temperature") and (t.dtype is not f32 or t.shape != (b,) or
-                                                         not t.is_contiguous()):
+        if t is not None and (t.dtype is not f32 or t.shape != (b,) or not t.is_contiguous()):
             raise ShapeError(f"sample: {what} f32 [{b}] expected")
     if top_k is not None:
         _ints(top_k, "top_k", b)

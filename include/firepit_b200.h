@@ -860,8 +860,8 @@ int fpb_tree_verify(const void *logits, int logits_dtype, size_t logits_pitch, c
  * rows of requests that are not served stay in their place), or (padded) request b
  * has rows [b, b + 1) * rows / batch.  slots, positions, requests [rows]: the
  * token's slot, its position and its request, -1 in rows without one; starts [batch
- * + 1]: each request's first row.  requests and starts may be NULL.  batch at most
- * 16384. */
+ * + 1]: each request's first row.  requests and starts may be NULL.  counts must not
+ * overlap lengths.  batch at most 16384. */
 int fpb_page_extend(int32_t *table, size_t table_pitch, size_t batch, size_t max_pages, int32_t *lengths,
                     const int32_t *counts, int32_t *free_pages, int32_t *free_count, size_t pages, size_t page_size,
                     size_t rows, int padded, int32_t *slots, int32_t *positions, int32_t *requests, int32_t *starts,

@@ -6,10 +6,14 @@ Bars, derived from the arithmetic:
  - append: as in the 8-bit cache's tests: 3e-6 of the head's largest value for
    norms and rotation in f32, and half a step of the type that it is kept in
    (bf16 2^-8, f32 2^-24); v that fits its type is equal.
- - attention: f32 pages: products and sums in f32.  A score is off by at most
+ - attention: f32 pages, products and sums in f32: a score is off by at most
    ds = (d + 4) 2^-24 scale * sum |q_i k_i|, so a weight by 2 ds + 2^-21 (its
    power) of itself, the sums over n tokens by (n + 64) 2^-24, and the output by
-   (2 ds + 2^-20 + (n + 64) 2^-23) * sum p |v|.  bf16 pages: q and the weights are
+   (2 ds + 2^-20 + (n + 64) 2^-23) * sum p |v|.  Products of factors in two parts
+   of 11 bits stay within that: a product is off by 2^-20 (what the cut factor's two
+   parts leave), 2^-21 (the parts' own product, left out) and 2^-22, 1.75 * 2^-20 in
+   all, so the output by (3 * 2^-20 of the scores, twice, and 1.75 * 2^-20) * sum p
+   |v|, below 8 * 2^-20 where the bar's (64) 2^-23 alone is as much.  bf16 pages: q and the weights are
    split in two parts of 8 bits each (2^-16 with the sign), products exact in
    f32: 2^-16 more in ds and 2^-15 more of sum p |v|.  Then half a step of the
    output's type and 2^-21 for the gate.
@@ -79,7 +83,7 @@ def _maps(m, want):
 
 @pytest.mark.parametrize("batch,pages,p,width,rows,padded", [
     (1, 3, 1, 3, 4, False), (5, 40, 16, 9, 64, False), (7, 30, 3, 11, 35, True), (64, 900, 16, 20, 64, True),
-    (1030, 4000, 8, 6, 9001, False), (3, 2000, 24, 700, 30000, False), (300, 60, 4, 5, 800, False)])
+    (1030, 4000, 8, 6, 9001, False), (3, 2000, 24, 700, 30000, False), (300, 60, 4, 5, 800, False), (700, 9000, 1, 30, 9001, False)])
 def test_page_tables_follow_the_stack(F, torch, batch, pages, p, width, rows, padded):
     """Steps of extensions and truncations, among them more than the pool, the
     tables and the rows can hold."""
@@ -135,6 +139,17 @@ def test_page_tables_ranges_of_the_state(F, torch):
     tables.lengths.fill_(4)  # pages that nobody took cannot come back
     F.page_truncate(tables, _dev(torch, np.zeros(2, np.int32)))
     assert F.device_error(reset=True) == 507 and tables.lengths.cpu().tolist() == [4, 4]
+
+
+def test_page_tables_rows_up_to_2_31(F, torch):
+    """As many rows as there may be, all but five without a token, into vectors of
+    the caller's."""
+    tables, rows = F.PageTables.empty(1, 6, 2, 6), 0x7ffffff0
+    out = F.PageMap(*(torch.empty(rows, dtype=torch.int32, device="cuda") for _ in range(2)), None, None)
+    assert F.page_extend(tables, _dev(torch, np.array([5], np.int32)), rows, True, out) is out
+    for t, want in ((out.slots, [0, 1, 2, 3, 4]), (out.positions, [0, 1, 2, 3, 4])):
+        assert t[:5].tolist() == want and all(bool((x == -1).all()) for x in t[5:].split(1 << 28))
+    assert tables.lengths.tolist() == [5] and tables.free_count.tolist() == [3]
 
 
 def test_page_tables_in_a_graph(F, torch):
@@ -336,6 +351,65 @@ def test_paged_attention_many_sessions(F, torch, pages):
     _check_attention(out, q, gate, cache, table, n, 0.125, sessions=[0, 7, 100, 300] + rng.integers(0, 301, 30).tolist(),
                      heads=[0, 3, 7])
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("pages", ["f32", "bf16"])
+@pytest.mark.parametrize("b,hq,hk,d,most", [(70, 4, 1, 64, 900), (41, 12, 1, 256, 60), (20, 16, 8, 128, 700),
+                                            (32, 8, 4, 80, 300), (33, 8, 4, 80, 300), (1, 64, 64, 32, 2000)])
+def test_paged_attention_ways_to_cut(F, torch, pages, b, hq, hk, d, most):
+    """Few and many sessions, in one wave of blocks and in several, some without
+    tokens and one whose length cannot be."""
+    torch.manual_seed(b)
+    rng = np.random.default_rng(b + hk)
+    lengths = rng.integers(1, most, b)
+    lengths[rng.random(b) < 0.2] = 0
+    lengths[-1] = most
+    q, gate, cache, table, n = _attention_case(F, torch, rng, lengths, hq, hk, d, 16, "f32", pages)
+    out = F.paged_attention(q, cache, table, n, gate=gate)
+    _check_attention(out, q, gate, cache, table, n, d ** -0.5, heads=[0, hq - 1])
+    assert torch.equal(out, F.paged_attention(q, cache, table, n, gate=gate))
+    if b > 1:
+        n[0] = -7
+        out = F.paged_attention(q, cache, table, n, gate=gate)
+        assert F.device_error(reset=True) == 507
+        n[0] = 0
+        _check_attention(out, q, gate, cache, table, n, d ** -0.5, sessions=[0, b // 2, b - 1], heads=[hq // 2])
+
+
+def test_paged_attention_two_at_once(F, torch):
+    """Calls on two streams with a workspace each, and two graphs that share one and
+    are replayed in turn, the workspace written to in between."""
+    torch.manual_seed(21)
+    rng = np.random.default_rng(21)
+    cases = [_attention_case(F, torch, rng, lengths, 16, 2, 128, 16, "f32", "bf16")
+             for lengths in ([4000, 3, 700], [50, 9000, 0])]
+    want = [F.paged_attention(q, cache, table, n, gate=gate) for q, gate, cache, table, n in cases]
+    for w, (q, gate, cache, table, n) in zip(want, cases):
+        _check_attention(w, q, gate, cache, table, n, 128 ** -0.5, heads=[0, 15])
+    size = F.paged_attention_workspace_bytes(cases[0][2], 3, 16)
+    outs = [torch.empty_like(w) for w in want]
+    sides = [torch.cuda.Stream() for _ in cases]
+    spaces = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for side, ws, out, (q, gate, cache, table, n) in zip(sides, spaces, outs, cases):
+            F.paged_attention(q, cache, table, n, gate=gate, out=out, workspace=ws, stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    graphs = []
+    for out, (q, gate, cache, table, n) in zip(outs, cases):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=sides[0]):
+            F.paged_attention(q, cache, table, n, gate=gate, out=out, workspace=spaces[0])
+        graphs.append(g)
+    for fill in (0, 255, 17):
+        for g, out, w in zip(graphs, outs, want):
+            out.zero_()
+            g.replay()
+            assert torch.equal(out, w)
+            g.replay()
+            assert torch.equal(out, w)
+            spaces[0].fill_(fill)
 
 
 @pytest.mark.parametrize("pages", ["f32", "bf16"])
@@ -572,6 +646,34 @@ def test_sample_of_rows_that_are_not_finite(F, torch):
             assert tokens.cpu().tolist()[:3] == [-1, -1, 0] and tokens[8] == -1
 
 
+def test_sample_of_numbers_that_are_none(F, torch):
+    """Numbers of zero, where a weight of 0 over one is no number, and NaN: the token is
+    one of those that are kept, in every way to find it, and none that a NaN stands for
+    where there is another."""
+    vocab = 5000
+    g = torch.Generator(device="cuda").manual_seed(31)
+    ways = ((5, 1.0, 0.0), (40, 0.9, 0.0), (0, 0.7, 0.0), (2000, 1.0, 0.0), (0, 1.0, 0.0), (0, 0.999, 0.0), (0, 1.0, 1e-3))
+    t, k, p, m = (np.array(x) for x in zip(*((1.0, *w) for w in ways)))
+    f = t.astype(np.float32), k.astype(np.int32), p.astype(np.float32), m.astype(np.float32)
+    b = len(ways)
+    steep = -200.0 * torch.arange(vocab, device="cuda").float().expand(b, vocab).contiguous()
+    tokens, logprobs = _run_sample(F, torch, steep, torch.zeros(b, vocab, device="cuda"), *f)
+    assert tokens.tolist() == [0] * b and logprobs.abs().max() < 1e-6  # every other weight is 0
+    logits = torch.randn(b, vocab, generator=g, device="cuda") * 3
+    noise = torch.empty(b, vocab, device="cuda").exponential_(generator=g).clamp_(min=1e-20)
+    first = logits.argmax(1)
+    noise[torch.arange(b), first] = math.nan
+    tokens, logprobs = _run_sample(F, torch, logits, noise, *f)
+    less = noise.clone()
+    less[torch.arange(b), first] = 1e30  # (never drawn)
+    want, same = _run_sample(F, torch, logits, less, *f)
+    assert torch.equal(tokens, want) and torch.equal(logprobs, same)
+    tokens, _ = _run_sample(F, torch, logits, torch.full_like(noise, math.nan), *f)
+    for i in range(b):
+        order, _ = R.kept(_host(logits[i]), temperature=1.0, top_k=int(k[i]), top_p=float(p[i]), min_p=float(m[i]))
+        assert int(tokens[i]) in order
+
+
 def test_sample_draws_from_the_distribution(F, torch):
     """Frequencies of 40000 draws from one row, each within five standard
     deviations (a chance of 6e-7 each)."""
@@ -612,6 +714,7 @@ def test_sample_strides_streams_and_graphs(F, torch):
         g.replay()
         torch.cuda.synchronize()
         _check_sample(torch, out.cpu(), logprobs.cpu(), logits, noise, *again[2:])
+    assert torch.equal(F.sample(logits, None, noise), F.sample(logits, torch.ones_like(t), noise))
     plain = F.sample(logits, t, noise)
     ones = [np.float32([float(x) for x in t.cpu()]), np.zeros(b, np.int32), np.ones(b, np.float32), np.zeros(b, np.float32)]
     _, logs = F.sample(logits, t, noise, logprobs=True)

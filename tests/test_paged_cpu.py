@@ -28,6 +28,9 @@ def test_page_entry_points_check_arguments():
                dict(pitch=1 << 40)):
         assert extend(**kw) == shape, kw
 
+    for counts in (i, i + 4, i - 4):  # two requests' counts among their lengths
+        assert extend(counts=counts) == bad
+
     def cut(table=i, lengths=i, to=i, free=i, free_count=i, batch=2, pages=8):
         return N.lib.fpb_page_truncate(table, 4, batch, 4, lengths, to, free, free_count, pages, 16, None)
 
