@@ -68,6 +68,20 @@ __device__ __forceinline__ float unordered(uint32_t u) {
   return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
 }
 
+// [*lo, *hi], so ordered, without its ends that are no value of the type: -0 is none
+// (0 is its equal), and bf16 values lie 2^16 apart.  (Some value lies within.)
+template <typename T>
+__device__ __forceinline__ void to_values(uint32_t *lo, uint32_t *hi) {
+  constexpr uint32_t kNone = 0x7fffffffu;
+  uint32_t l = *lo, h = *hi - (*hi == kNone);
+  if (sizeof(T) == 2) {
+    l = l > kNone ? (l + 0xffffu) & 0xffff0000u : l | 0xffffu;
+    h = h > kNone ? h & 0xffff0000u : ((h + 1) & 0xffff0000u) - 1;
+  }
+  *lo = l + (l == kNone);
+  *hi = h;
+}
+
 __device__ __forceinline__ uint32_t peer_address(const void *p, unsigned rank) {
   const uint32_t local = (uint32_t)__cvta_generic_to_shared(p);
   uint32_t remote;
@@ -608,10 +622,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     bool all_of_it = false;
     uint32_t n_in = sh.n_in;
     while (true) {
+      to_values<T>(&lo, &hi);
+      if (lo == hi) break;
       const float low = unordered(lo), high = unordered(hi);
-      if (n_in <= (uint32_t)kList || lo == hi) {
+      if (n_in <= (uint32_t)kList) {
         n_in = gather(low, false, [&](float x, int) { return x <= high; });  // (meets: the histograms are read)
-        if (n_in <= (uint32_t)kList || lo == hi) break;
+        if (n_in <= (uint32_t)kList) break;
       } else {
         meet();
       }
@@ -640,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
     if (all_of_it) {
       set_cut(unordered(lo), 0x7fffffff);
-    } else if (n_in <= (uint32_t)kList) {
+    } else if (lo != hi) {
       if (rank == 0) {
         const unsigned long long mine = sorted(sh, (int)n_in, listed((int)n_in));
         const bool in = tid < (int)n_in;
@@ -658,35 +674,57 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       meet();
       set_cut(sh.cut, sh.cut_index);
     } else {
-      // equal logits: as many of them as are wanted, by index
+      // equal logits: as many of them as are wanted, by index.  A warp counts those of
+      // its own part of the slice, and the one that has the last goes through it again.
       const float equal = unordered(lo);
-      const double each = (double)pow2(-depth(equal));
-      int wanted = weigh ? (int)fmin(fmax(ceil((target - s_before) / each), 1.0), (double)n_in) : k - (int)n_before;
-      wanted = max(1, min(wanted, (int)n_in));
-      const int chunk = (len + kThreads - 1) / kThreads, i0 = min(len, tid * chunk), i1 = min(len, i0 + chunk);
+      const int quads = (len + 3) / 4, part = (quads + kWarps - 1) / kWarps, q1 = min(quads, (warp + 1) * part);
+      auto count4 = [&](int q) {  // a bit for each of the four that is one of them
+        if (q >= q1) return 0u;
+        const int i = 4 * q;
+        const float4 x = *reinterpret_cast<const float4 *>(xs + i);
+        return (uint32_t)((x.x == equal) & kept(equal, i)) | (uint32_t)((x.y == equal) & kept(equal, i + 1)) << 1 |
+               (uint32_t)((x.z == equal) & kept(equal, i + 2)) << 2 | (uint32_t)((x.w == equal) & kept(equal, i + 3)) << 3;
+      };
       int mine = 0;
-      for (int i = i0; i < i1; ++i) mine += xs[i] == equal && kept(equal, i);
-      int run = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, run, o);
-        if (lane >= o) run += y;
-      }
+#pragma unroll 4
+      for (int q = warp * part + lane; q < q1; q += 32) mine += __popc(count4(q));
+      mine = __reduce_add_sync(0xffffffffu, mine);
       __syncthreads();
-      if (lane == 31) sh.counts[warp] = run;
+      if (lane == 0) sh.counts[warp] = mine;
       __syncthreads();
-      int before = run - mine, all = 0;
+      int before = 0, all = 0;
       for (int i = 0; i < kWarps; ++i) {
         if (i < warp) before += sh.counts[i];
         all += sh.counts[i];
       }
-      tell((uint32_t)all, 0, 0, 0, 0);
-      for (int r = 0; r < (int)rank; ++r) before += heard(0, r);
-      if (before < wanted && before + mine >= wanted) {
-        int n = before, i = i0;
-        for (;; ++i)
-          if (xs[i] == equal && kept(equal, i) && ++n == wanted) break;
-        for (int r = 0; r < kCluster; ++r) peer_store(&sh.cut_index, r, (uint32_t)(v0 + i));
+      tell((uint32_t)all, 0, 0, 0, 0);  // (meets: the histograms are read)
+      int total = 0;
+      for (int r = 0; r < kCluster; ++r) {
+        if (r < (int)rank) before += heard(0, r);
+        total += heard(0, r);
+      }
+      const double each = (double)pow2(-depth(equal));
+      int wanted = weigh ? (int)fmin(fmax(ceil((target - s_before) / each), 1.0), (double)total) : k - (int)n_before;
+      wanted = max(1, min(wanted, total)) - before;  // the warp's
+      if (wanted >= 1 && wanted <= mine) {
+        for (int q = warp * part + lane;; q += 32) {
+          uint32_t bits = count4(q);
+          int run = __popc(bits);
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += y;
+          }
+          const int there = __shfl_sync(0xffffffffu, run, 31), skip = wanted - 1 - (run - __popc(bits));
+          if (there >= wanted) {
+            if (skip >= 0 && skip < __popc(bits)) {
+              for (int n = 0; n < skip; ++n) bits &= bits - 1;
+              for (int r = 0; r < kCluster; ++r) peer_store(&sh.cut_index, r, (uint32_t)(v0 + 4 * q + __ffs(bits) - 1));
+            }
+            break;
+          }
+          wanted -= there;
+        }
       }
       meet();
       set_cut(equal, sh.cut_index);
