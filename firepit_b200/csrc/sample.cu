@@ -8,6 +8,13 @@
 //   min-p   those with w >= min_p
 // The token is argmax w_i / e_i over what is kept: with exponential e it is
 // distributed as w.
+//
+// The bytes are a row's logits, and of its noise what is kept (0.6 MB each for 151936
+// f32, under 1 us at the memory's rate for eight rows); what takes the time is one
+// dependent step behind another, each of 1 to 4 us for passes over a slice, meetings of
+// the cluster's CTAs and a sort: 8 rows of 151936 f32 take 4 us greedily, 10 with top-k
+// (one list), 10 with every token in the race, 30 where top-p ends among tens of
+// thousands of tokens.  A row's slices stay in shared memory between the steps.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -18,13 +25,14 @@
 namespace fpb {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kCluster = 8;
-constexpr int kMaxSlice = 49152;  // f32 of shared memory a CTA: 192 KB
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kMaxSlice = 49152;  // logits of a CTA in shared memory, f32: 192 KB
+constexpr int kMaxVocab = 8 * kMaxSlice;
 constexpr int kBatch = 5;         // 16-byte loads a thread has under way (f32 logits: twice as many)
 constexpr int kBins = 256;        // bins of a histogram
 constexpr int kList = kThreads;   // tokens that one CTA orders
-constexpr int kLargest = kWarps * kCluster;  // warps of a cluster, each with its largest logit
-// What the k-th largest of the warps' 128 largest logits reaches is, with logits in
+constexpr int kLargest = 128;     // groups of a cluster's threads, each with its largest logit
+// What the k-th largest of the groups' 128 largest logits reaches is, with logits in
 // no order, -128 ln(1 - k / 128) tokens: for 120 of them 355, for 96 177.
 constexpr int kDirect = 120, kDirectSum = 96;
 constexpr int kLists = 16;  // at most: one, and for each of two filters one and 32 / 8 finer ones
@@ -121,13 +129,14 @@ __device__ __forceinline__ V warp_total(V v) {
   return v;
 }
 
+template <int C>
 struct Shared {
   unsigned long long list[kList];  // tokens to be ordered, (falling logit, index) as one number
   uint32_t hist[kBins];            // tokens, or their weights
   // what the CTAs tell one another; the halves alternate, so that one exchange's
   // reads may overlap the next one's stores
-  uint32_t got[2][5][kCluster];
-  float maxima[kLargest];
+  uint32_t got[2][5][C];
+  float maxima[kLargest], group[kLargest / C];  // the cluster's, the CTA's own
   double sums[kWarps];
   uint32_t counts[kWarps];
   Best best[kWarps];
@@ -143,7 +152,8 @@ struct Shared {
 
 // The block's n (<= kList) numbers x, one a thread, in order: the tid-th, or ~0 past
 // them.  All threads.  Bitonic, neighbours up to 16 apart through registers.
-__device__ __noinline__ unsigned long long sorted(Shared &sh, int n, unsigned long long x) {
+template <int C>
+__device__ __noinline__ unsigned long long sorted(Shared<C> &sh, int n, unsigned long long x) {
   const int tid = threadIdx.x;
   int size = 32;
   while (size < n) size *= 2;
@@ -172,14 +182,15 @@ __device__ __noinline__ unsigned long long sorted(Shared &sh, int n, unsigned lo
 // Over the cluster's histograms: the first bin at which the running count (from n0
 // on), or weight (from s0 on; bin i's numbers times `unit` and 2^-(i * step)),
 // reaches the target (-1: none), with what lies before it.  Every CTA finds the
-// same.  Two threads a bin, four CTAs' each.
-__device__ __noinline__ int find_border(Shared &sh, bool weigh, double target, uint32_t n0, double s0, double unit,
+// same.  Two threads a bin, half of the CTAs' each.
+template <int C>
+__device__ __noinline__ int find_border(Shared<C> &sh, bool weigh, double target, uint32_t n0, double s0, double unit,
                                         float step) {
-  static_assert(kThreads == 2 * kBins && kCluster == 8);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bin = tid >> 1, from = 4 * (tid & 1);
+  static_assert(kThreads == 2 * kBins);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bin = tid >> 1, from = C / 2 * (tid & 1);
   unsigned long long f = 0;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) f += peer_load(&sh.hist[bin], from + r);
+  for (int r = 0; r < C / 2; ++r) f += peer_load(&sh.hist[bin], from + r);
   f += __shfl_xor_sync(0xffffffffu, f, 1);
   uint32_t c = weigh ? 0 : (uint32_t)f;
   const bool one = (tid & 1) == 0;
@@ -219,9 +230,9 @@ __device__ __noinline__ int find_border(Shared &sh, bool weigh, double target, u
   return border < kBins ? border : -1;
 }
 
-// A cluster of kCluster CTAs a row: CTA `rank` keeps the vocabulary's slice [rank
+// A cluster of C CTAs a row: CTA `rank` keeps the vocabulary's slice [rank
 // * slice, +slice) in shared memory, so that the row is read once.
-//  1. Every warp's largest logit goes to every CTA: the row's largest, and with the
+//  1. The largest logit of each of 128 groups of threads goes to every CTA: the row's largest, and with the
 //     k-th largest of the 128 (all of them for top-p alone) a bound that at least k
 //     tokens reach.
 //  2. What reaches it (a few times k tokens) goes to the first CTA's list, which is
@@ -231,13 +242,14 @@ __device__ __noinline__ int find_border(Shared &sh, bool weigh, double target, u
 //     a histogram over the cluster, and in the border's bin by the list, or by finer
 //     histograms until the tokens there fit it, or are equal.  What is kept races
 //     where it lies.
-template <typename T>
+template <typename T, int C>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
   // every CTA of the cluster runs, before its shared memory is stored to
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   pdl_enter();
-  extern __shared__ __align__(16) float xs[];  // the slice's logits
-  __shared__ Shared sh;
+  extern __shared__ __align__(16) uint8_t xs_raw[];
+  T *const xs = reinterpret_cast<T *>(xs_raw);  // the slice's logits
+  __shared__ Shared<C> sh;
   const unsigned rank = cluster_ctarank();
   const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int v0 = (int)rank * a.slice, len = max(0, min(a.vocab - v0, a.slice)), padded = (len + 3) / 4 * 4;
@@ -258,6 +270,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   if (tid < kLists) sh.listed[tid] = 0;
   if (tid == 0) sh.bound = 0xffffffffu;
 
+  auto get4 = [&](int i) {  // four of them
+    if constexpr (sizeof(T) == 4) {
+      return *reinterpret_cast<const float4 *>(xs + i);
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2 *>(xs + i);
+      return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                         __uint_as_float(u.y & 0xffff0000u));
+    }
+  };
+
   // The slice to shared memory, and its largest logit: the first of the first four
   // that hold one.
   Best top{-INFINITY, 0x7fffffff};
@@ -266,7 +288,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     auto finite = [](float x) { return fabsf(x) <= 3.402823466e38f ? x : -INFINITY; };
     auto take = [&](float x0, float x1, float x2, float x3, int i) {
       const float4 y = make_float4(finite(x0), finite(x1), finite(x2), finite(x3));
-      *reinterpret_cast<float4 *>(xs + i) = y;
+      if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<float4 *>(xs + i) = y;
+      else
+        *reinterpret_cast<uint2 *>(xs + i) = make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
       const float most = fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w));
       if (most > top.v) top = Best{most, i};
     };
@@ -299,14 +324,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       take(x[0], x[1], x[2], x[3], i);
     }
     if (top.i != 0x7fffffff) {  // which of the four
-      const float4 y = *reinterpret_cast<const float4 *>(xs + top.i);
+      const float4 y = get4(top.i);
       top.i += v0 + (y.x == top.v ? 0 : y.y == top.v ? 1 : y.z == top.v ? 2 : 3);
     }
   }
-  auto block_best = [&](Best x) {  // (the warps' own are left in sh.best)
+  constexpr int kLanes = kThreads * C / kLargest;  // of a group
+  static_assert(kLanes <= 32);
+  auto block_best = [&](Best x, bool groups) {  // (the groups' own to sh.group)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
+    for (int o = 1; o < 32; o <<= 1) {
+      if (groups && o == kLanes && lane % kLanes == 0) sh.group[tid / kLanes] = x.v;
       x = better(x, Best{__shfl_xor_sync(0xffffffffu, x.v, o), __shfl_xor_sync(0xffffffffu, x.i, o)});
+    }
+    if (groups && kLanes == 32 && lane == 0) sh.group[warp] = x.v;
     if (lane == 0) sh.best[warp] = x;
     __syncthreads();
     x = sh.best[lane % kWarps];
@@ -328,9 +358,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   };
   int flip = 0;
   auto tell = [&](uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t w4) {
-    if (tid < 5 * kCluster) {
-      const int word = tid / kCluster;
-      peer_store(&sh.got[flip][word][rank], tid % kCluster,
+    if (tid < 5 * C) {
+      const int word = tid / C;
+      peer_store(&sh.got[flip][word][rank], tid % C,
                  word == 0 ? w0 : word == 1 ? w1 : word == 2 ? w2 : word == 3 ? w3 : w4);
     }
     meet();
@@ -347,23 +377,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   };
   auto over_ctas = [&](double s) {  // each lane with CTA lane % 8's: every lane gets the same
 #pragma unroll
-    for (int o = kCluster / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    for (int o = C / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     return s;
   };
-  auto heard_sum = [&]() { return over_ctas(heard_double(lane % kCluster)); };
+  auto heard_sum = [&]() { return over_ctas(heard_double(lane % C)); };
   auto heard_count = [&]() {
     uint32_t n = 0;
-    for (int r = 0; r < kCluster; ++r) n += heard(4, r);
+    for (int r = 0; r < C; ++r) n += heard(4, r);
     return n;
   };
   auto best_of_all = [&]() {
-    Best x{__uint_as_float(heard(0, lane % kCluster)), (int)heard(1, lane % kCluster)};
+    Best x{__uint_as_float(heard(0, lane % C)), (int)heard(1, lane % C)};
 #pragma unroll
-    for (int o = kCluster / 2; o > 0; o >>= 1)
+    for (int o = C / 2; o > 0; o >>= 1)
       x = better(x, Best{__shfl_xor_sync(0xffffffffu, x.v, o), __shfl_xor_sync(0xffffffffu, x.i, o)});
     return x;
   };
-  top = block_best(top);
+  top = block_best(top, true);
   // for top-p alone: the slice's weights over its largest logit
   double slice_sum = 0.0;
   if (by_p && !by_k && !greedy) {
@@ -371,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     float part = 0.0f;
 #pragma unroll 5
     for (int i = tid * 4; i < len; i += kThreads * 4) {
-      const float4 x = *reinterpret_cast<const float4 *>(xs + i);
+      const float4 x = get4(i);
       part += (pow2((x.x - over) * per) + pow2((x.y - over) * per)) + (pow2((x.z - over) * per) + pow2((x.w - over) * per));
     }
     slice_sum = block_sum(part);
@@ -380,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   static_assert(kLargest <= kThreads);
   if (tid < kLargest)
-    peer_store(&sh.maxima[rank * kWarps + tid / kCluster], tid % kCluster, __float_as_uint(sh.best[tid / kCluster].v));
+    peer_store(&sh.maxima[rank * (kLargest / C) + tid / C], tid % C, __float_as_uint(sh.group[tid / C]));
   tell_best(top, slice_sum, 0);
   top = best_of_all();
   if (greedy || top.i == 0x7fffffff) {
@@ -394,8 +424,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   auto depth = [&](float x) { return (largest - x) * per; };  // w = 2^-depth
   double whole;  // the weights' sum, for top-p alone
   {
-    const float theirs = fmaxf(__uint_as_float(heard(0, lane % kCluster)), kLowest);
-    whole = over_ctas(heard_double(lane % kCluster) * (double)pow2(-depth(theirs)));
+    const float theirs = fmaxf(__uint_as_float(heard(0, lane % C)), kLowest);
+    whole = over_ctas(heard_double(lane % C) * (double)pow2(-depth(theirs)));
   }
   // What is kept so far: logits above `cut`, and those equal to it up to the slice's
   // token `cut_index`.
@@ -409,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   auto kept = [&](float x, int i) { return x > cut || (x == cut && i <= cut_index); };
   // four of the slice's logits; -inf where they are not kept
   auto load4 = [&](int i) {
-    float4 y = *reinterpret_cast<const float4 *>(xs + i);
+    float4 y = get4(i);
     if (cut > -INFINITY) {
       const float from = i <= cut_index ? cut : above_cut;
       y.x = y.x >= from ? y.x : -INFINITY;
@@ -470,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   // CTA's threads).
   auto listed = [&](int n) {
     int r = 0, at = tid;
-    while (r < kCluster - 1 && at >= (int)heard(4, r)) at -= (int)heard(4, r++);
+    while (r < C - 1 && at >= (int)heard(4, r)) at -= (int)heard(4, r++);
     return tid < n ? peer_load(&sh.list[at], r) : ~0ull;
   };
   // The running sum of the weights w of the ordered list, without the thread's own.
@@ -491,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 
   if (by_k ? k <= kDirect : by_p) {
     const int wanted = by_k ? k : kDirectSum;
-    {  // The smallest of the warps' largest that fewer than `wanted` of them are above:
+    {  // The smallest of the groups' largest that fewer than `wanted` of them are above:
        // four threads each, a quarter of the others.
       static_assert(kThreads == 4 * kLargest);
       const float mine = sh.maxima[tid / 4];
@@ -526,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       if (by_k && by_p) whole = block_sum(w);
       const bool in = tid < most && (tid == 0 || !by_p || before < (double)p * whole) && w >= least;
       // (a number that is none, of a noise of none or a weight of 0 over a noise of 0, wins no race)
-      const Best pick = block_best(in ? Best{fmaxf(w * inverse(e), 0.0f), token} : Best{0.0f, top.i});
+      const Best pick = block_best(in ? Best{fmaxf(w * inverse(e), 0.0f), token} : Best{0.0f, top.i}, false);
       const double s = block_sum(in ? w : 0.0f);
       if (tid < most && token == pick.i) answer(token, x, s);
       __syncwarp();
@@ -666,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         if (weigh && in && run >= target) atomicMin(&sh.border, tid);
         __syncthreads();
         if (tid == max(0, sh.border))
-          for (int r = 0; r < kCluster; ++r) {
+          for (int r = 0; r < C; ++r) {
             peer_store(&sh.cut, r, __float_as_uint(x));
             peer_store(&sh.cut_index, r, (uint32_t)mine);
           }
@@ -681,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       auto count4 = [&](int q) {  // a bit for each of the four that is one of them
         if (q >= q1) return 0u;
         const int i = 4 * q;
-        const float4 x = *reinterpret_cast<const float4 *>(xs + i);
+        const float4 x = get4(i);
         return (uint32_t)((x.x == equal) & kept(equal, i)) | (uint32_t)((x.y == equal) & kept(equal, i + 1)) << 1 |
                (uint32_t)((x.z == equal) & kept(equal, i + 2)) << 2 | (uint32_t)((x.w == equal) & kept(equal, i + 3)) << 3;
       };
@@ -699,7 +729,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       }
       tell((uint32_t)all, 0, 0, 0, 0);  // (meets: the histograms are read)
       int total = 0;
-      for (int r = 0; r < kCluster; ++r) {
+      for (int r = 0; r < C; ++r) {
         if (r < (int)rank) before += heard(0, r);
         total += heard(0, r);
       }
@@ -719,7 +749,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           if (there >= wanted) {
             if (skip >= 0 && skip < __popc(bits)) {
               for (int n = 0; n < skip; ++n) bits &= bits - 1;
-              for (int r = 0; r < kCluster; ++r) peer_store(&sh.cut_index, r, (uint32_t)(v0 + 4 * q + __ffs(bits) - 1));
+              for (int r = 0; r < C; ++r) peer_store(&sh.cut_index, r, (uint32_t)(v0 + 4 * q + __ffs(bits) - 1));
             }
             break;
           }
@@ -821,13 +851,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const double all = heard_sum();
   if (rank == 0 && tid == 0) {
     float x = 0.0f;
-    for (int r = 0; r < kCluster; ++r)
+    for (int r = 0; r < C; ++r)
       if ((int)heard(1, r) == pick.i) x = __uint_as_float(heard(4, r));
     answer(pick.i, x, all);
   }
 }
 
-template <typename T>
+template <typename T, int C>
 int run_sample(const SampleArgs &a, size_t batch, cudaStream_t s) {
   {
     static std::mutex mu;
@@ -836,13 +866,13 @@ int run_sample(const SampleArgs &a, size_t batch, cudaStream_t s) {
     FPB_CUDA_TRY(cudaGetDevice(&dev));
     std::lock_guard<std::mutex> lock(mu);
     if (std::find(done.begin(), done.end(), dev) == done.end()) {
-      FPB_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        (int)(kMaxSlice * sizeof(float))));
+      FPB_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)(kMaxSlice * sizeof(T))));
       done.push_back(dev);
     }
   }
-  cudaError_t e = launch_pdl_cluster(sample_kernel<T>, dim3(kCluster, (unsigned)batch), kThreads,
-                                     (size_t)a.slice * sizeof(float), s, kCluster, a);
+  cudaError_t e = launch_pdl_cluster(sample_kernel<T, C>, dim3(C, (unsigned)batch), kThreads,
+                                     (size_t)a.slice * sizeof(T), s, C, a);
   if (e != cudaSuccess) return cuda_fail(e, "sample_kernel");
   FPB_LAUNCH_CHECK("sample_kernel");
   return FPB_OK;
@@ -860,9 +890,9 @@ extern "C" int fpb_sample(const void *logits, int logits_dtype, size_t logits_pi
   if (!logits || !noise || !tokens) return fail(FPB_ERR_INVALID_ARGUMENT, "fpb_sample: null pointer");
   if (logits_dtype != FPB_F32 && logits_dtype != FPB_BF16)
     return fail(FPB_ERR_INVALID_ARGUMENT, "fpb_sample: dtype");
-  if (batch == 0 || batch > 65535 || vocab == 0 || vocab > (size_t)kMaxSlice * kCluster || logits_pitch < vocab || noise_pitch < vocab ||
+  if (batch == 0 || batch > 65535 || vocab == 0 || vocab > (size_t)kMaxVocab || logits_pitch < vocab || noise_pitch < vocab ||
       (logits_pitch | noise_pitch) >> 38)
-    return fail(FPB_ERR_SHAPE, "fpb_sample: batch %zu, vocab %zu (at most %d), pitches", batch, vocab, kMaxSlice * kCluster);
+    return fail(FPB_ERR_SHAPE, "fpb_sample: batch %zu, vocab %zu (at most %d), pitches", batch, vocab, kMaxVocab);
   if (reinterpret_cast<uintptr_t>(logits) % (logits_dtype == FPB_F32 ? 4 : 2) ||
       reinterpret_cast<uintptr_t>(noise) % 4)
     return fail(FPB_ERR_INVALID_ARGUMENT, "fpb_sample: alignment");
@@ -878,10 +908,26 @@ extern "C" int fpb_sample(const void *logits, int logits_dtype, size_t logits_pi
   a.vocab = (int)vocab;
   a.tokens = tokens;
   a.logprobs = logprobs;
-  a.slice = (int)((vocab + kCluster - 1) / kCluster + 7) / 8 * 8;
+  // Two CTAs an SM: about 32 rows are there at once in clusters of eight, and most of a
+  // row's time goes by in its exchanges, so that many rows take fewer CTAs each, as long
+  // as two slices fit an SM (us for C = 8 / 4 / 2, each row with filters of its own:
+  // 250 x 151936 bf16 113 / 95 / -, 100 of them 59 / 59, 40 of them 35 / 45; 250 x 32000
+  // bf16 76 / 51 / 41, 100 of them 39 / 30 / 29, 56 of them 26 / 24 / 26, 24 of them 20 /
+  // 21 / 25; 150 x 100000 f32 70 / 63 / -, 72 of them 43 / 42).
+  const size_t el = logits_dtype == FPB_F32 ? 4 : 2, sms = sm_count();
+  auto slice = [&](size_t c) { return ((vocab + c - 1) / c + 7) / 8 * 8; };
+  const int C = batch * 8 > 5 * sms && slice(2) <= 16384 ? 2
+                : batch * 16 > 5 * sms && slice(4) <= 16384 ? 4
+                : batch * 8 > 5 * sms && slice(4) * el <= 100 * 1024 ? 4
+                    : 8;
+  a.slice = (int)slice(C);
   auto lies = [](const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && bytes % 16 == 0; };
-  a.vec = lies(logits, logits_pitch * (logits_dtype == FPB_F32 ? 4 : 2));
+  a.vec = lies(logits, logits_pitch * el);
   a.noise_vec = lies(noise, noise_pitch * 4);
-  return logits_dtype == FPB_F32 ? run_sample<float>(a, batch, as_stream(stream))
-                                 : run_sample<__nv_bfloat16>(a, batch, as_stream(stream));
+  cudaStream_t st = as_stream(stream);
+  auto run = [&](auto t) {
+    using T = decltype(t);
+    return C == 2 ? run_sample<T, 2>(a, batch, st) : C == 4 ? run_sample<T, 4>(a, batch, st) : run_sample<T, 8>(a, batch, st);
+  };
+  return logits_dtype == FPB_F32 ? run(0.0f) : run(__nv_bfloat16());
 }

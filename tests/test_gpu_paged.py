@@ -576,7 +576,8 @@ def _run_sample(F, torch, logits, noise, *filters, **kw):
 
 @pytest.mark.parametrize("b,vocab,dtype", [(1, 1, "f32"), (3, 2, "bf16"), (40, 33, "f32"), (64, 1000, "bf16"),
                                            (48, 4099, "f32"), (24, 32000, "bf16"), (40, 50257, "f32"),
-                                           (12, 151936, "f32"), (30, 151936, "bf16"), (3, 393216, "bf16")])
+                                           (12, 151936, "f32"), (30, 151936, "bf16"), (3, 393216, "bf16"),
+                                           (94, 151936, "bf16"), (47, 50257, "f32"), (93, 32000, "bf16"), (100, 4099, "f32")])
 def test_sample_matches_the_definition(F, torch, b, vocab, dtype):
     args = _sample_inputs(torch, b, vocab, dtype, b * 3 + vocab)
     tokens, logprobs = _run_sample(F, torch, *args)
