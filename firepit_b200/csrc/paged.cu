@@ -79,8 +79,8 @@ enum PagePart { kPageAll, kPageRows, kPageState };
 // Each block scans all requests for itself, then the blocks share the rows and the
 // new pages.  A request is served whole (its rows fit, its table and the pool have
 // the pages) or not at all.  Bound by latency: two loads, two scans and the pages'
-// loads in a row (64 requests of a token each 3.5 us; 144000 rows of 96 requests,
-// 1.7 MB, in two launches 8 us, by a cluster of eight blocks 16).
+// loads in a row (with page_truncate behind it, 64 requests of a token each 7.1 us,
+// 144000 rows of 96 requests, 1.7 MB, 14.3).
 template <PagePart PART>
 __global__ void __launch_bounds__(kPageMaxThreads) page_extend_kernel(const __grid_constant__ PageArgs a) {
   pdl_enter();
@@ -248,7 +248,8 @@ int check_tables(const char *name, const PageArgs &a, size_t table_pitch, size_t
 }
 
 // One block where a step has few rows or pages; else many for those, and one behind
-// them for the state (from 8192 rows on: 6.4 us against 6.6).
+// them for the state (extend and truncate, one block and many: 4096 rows 9.5 and 11.5
+// us, 8192 12.4 and 11.4, 144000 120 and 14).
 int launch_pages(void (*const (&kernel)[3])(PageArgs), const char *name, const PageArgs &a, size_t work, size_t smem,
                  cudaStream_t s) {
   {
@@ -273,7 +274,7 @@ int launch_pages(void (*const (&kernel)[3])(PageArgs), const char *name, const P
   };
   // (a wide block's barriers take longer, a narrow one goes through its work more often)
   const unsigned scan = a.batch <= 256 ? 256 : kPageMaxThreads;
-  if (work <= 8192) return launch(kPageAll, 1, work <= 1024 ? scan : kPageMaxThreads);
+  if (work <= 6144) return launch(kPageAll, 1, work <= 1024 ? scan : kPageMaxThreads);
   const size_t blocks = std::min<size_t>((work + 4 * scan - 1) / (4 * scan), 2 * sm_count());
   if (int st = launch(kPageRows, (unsigned)blocks, scan)) return st;
   return launch(kPageState, 1, scan);
