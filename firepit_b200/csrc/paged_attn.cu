@@ -2,6 +2,22 @@
 //
 // Session b's query heads see the tokens t < lengths[b].  With s_t = scale q . k_t:
 //   out = sum_t softmax(s)_t v_t, times sigmoid(gate) where a gate is given.
+// One pass over the tokens: a warp holds its rows' running maximum m, sum of weights l
+// and numerators, all f32, and two such parts meet as l1 2^(m1 - m) + l2 2^(m2 - m).
+//
+// Bound by the pages' bytes, each read once: 200 ragged sessions (1.65 GB) 255 us, 6.5
+// TB/s; 3 x 100003 tokens x 4 heads of 128, bf16, 106 us, 5.3; 16 x 8192 x 2 heads of
+// 256 47.7 us, 5.0; 8 x 2304 of f32 25.5 us.  9 to 10 us of a call do not depend on the
+// bytes: the launch, the cut into shares, the first copies' way and the shares' meeting
+// (1 x 777 tokens 10.2 us).
+// A warp takes steps of 16 tokens (f32: 8) through a ring of TMA copies that it alone
+// waits for, so that the block meets only at the end.  The products go by mma.sync: a
+// kv head has up to 16 rows of queries, which would leave most of a tcgen05 tile's 128
+// empty, and the copies are what takes the time.
+// Products keep f32's precision but for 2^-16 of a factor (bf16 pages: queries and
+// weights are two bf16 parts, exact in their products) or 2^-20 of a product (f32 pages:
+// every factor is two parts of 11 bits, and the parts' small product is left out);
+// sums are f32.
 #include <algorithm>
 #include <atomic>
 #include <chrono>
@@ -213,7 +229,8 @@ struct PagedShare {
 // finds its own: false where there is none.  `steps` [batch] in shared memory.
 // One wave: the smallest S whose shares the GPU has room for at once, among 32
 // between total / slots, which is below it, and total / (slots - items), whose
-// shares fit: each item rounds up by less than one.
+// shares fit: each item rounds up by less than one.  Several: total / (waves * slots).
+
 // Lane 0 lo, lane 31 hi, the others between them, in even ratios but for rounding.
 __device__ __forceinline__ int between(int lo, int hi) {
   const int lane = threadIdx.x & 31;
@@ -739,6 +756,9 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
         for (int e = 0; e < 4; ++e)
           mine_f[(8 * i + 2 * c + (e & 1)) * Sh::kEndPitch + 16 * k + g + 8 * (e >> 1)] = acc[k][i][e];
   } else {
+    // A product of parts is three of the tensor cores' (two parts each, without the small
+    // ones'), and takes the time that the copies do (8 x 18432 tokens of 256: with f32
+    // fma 111 us, so 102, 5.9 TB/s).
     // S = Q K^T with the rows as M (eight of sixteen), eight tokens as N; O^T = V^T P^T
     // with the dimensions as M, the rows as N: S's result is P^T's operand as it lies.
     const int g = lane >> 2, c = lane & 3, own = token_at<T>(g);
@@ -906,7 +926,7 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
   // so by its flag and then looks at the others', so that the last one does find
   // them (another that does as well writes the same).  What a flag says is the
   // call's own number, whatever lay there before; they are cleared for the next use.
-  // (A kernel behind this one for it: 1 x 777 tokens 10.9 us, so 8.)
+  // (A kernel behind this one for it: 16 x 1000 tokens 17.9 us, so 16.0.)
   __shared__ int last_s;
   const int slot0 = me.slot - me.part;
   __syncthreads();
@@ -1030,8 +1050,16 @@ Plan plan_for(size_t batch, size_t q_heads, size_t kv_heads, size_t head_dim, bo
   p.rows = group <= 8 || f32 ? 8 : 16;
   p.tiles = (int)((group + p.rows - 1) / p.rows);
   const size_t items = batch * kv_heads * p.tiles;
-  // one wave where half of the blocks at most can be short ones
-  p.waves = 2 * items <= (size_t)sm_count() ? 0 : kPagedWaves;
+  // One wave, where every item has a block then.  Sessions of different lengths leave
+  // some of those short; with heads of more than 128 that costs more than the blocks'
+  // coming and going where more than half of the blocks can be (us for one wave and two:
+  // 16 x 2000 tokens x 8 kv heads of 128, bf16, 27 and 35, 16 x 9000 92 and 117, 10 x
+  // 9000 77 and 73; 50 x 2000 x 2 heads of 256 44 and 44, 66 x 9000 142 and 127).
+  p.waves = (head_dim <= 128 ? items < (size_t)sm_count() : 2 * items <= (size_t)sm_count()) ? 0 : kPagedWaves;
+  // (64 steps at least where blocks follow one another: of 24 20 x 5000 tokens x 8 heads
+  // 89 us, so 76, 20 x 600 18 and 24; in one wave the SMs are empty otherwise: 1 x 777
+  // tokens with 32 15.5 us, with 8 10.2.  Shares of two waves: of four 200 ragged sessions
+  // take 276 us, so 255, of one as long.)
   p.least = p.waves ? 64 : 8;
   p.slots = sm_count() * blocks_of(head_dim > 128 ? 256 : 128, !p.waves);
   // an item that is cut has more than S steps, so at most twice its steps / S shares

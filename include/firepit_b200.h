@@ -887,7 +887,10 @@ int fpb_paged_append(const void *q, size_t q_pitch, size_t q_head_pitch, const v
  * softmax(scale q . k) v, times sigmoid(gate) where gate [batch rows of gate_pitch,
  * heads of gate_head_pitch] f32 is given.  A session of length 0 gets zeros.  Rows
  * behind its last token never reach an output, whatever they hold; a token whose
- * page is outside the pool counts as not there.  batch at most 4096. */
+ * page is outside the pool counts as not there.  Sums are f32; over bf16 pages q and
+ * the weights are taken to 16 bits, over f32 pages products to 2^-20 of themselves.
+ * The workspace needs no clearing; calls that may run at the same time must not share
+ * one.  batch at most 4096. */
 size_t fpb_paged_attn_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads, size_t head_dim);
 int fpb_paged_attn(const void *q, int q_dtype, size_t q_pitch, size_t q_head_pitch, const void *k_pages,
                    const void *v_pages, int page_dtype, size_t pages, size_t page_size, size_t page_pitch,
