@@ -1,4 +1,6 @@
-"""Builds the firepit_b200 CUDA library in-tree: firepit_b200/libfirepit_b200.so.
+"""Builds the firepit_b200 CUDA library in-tree: firepit_b200/libfirepit_b200.so,
+and firepit_b200/_calls.so, which makes the paged cache's calls on torch's tensors
+(csrc/calls.cpp).
 
 Every translation unit is compiled for sm_100a only
 (``-gencode arch=compute_100a,code=sm_100a``), objects go to
@@ -9,16 +11,19 @@ Rebuilds only what changed (sources or any header).
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libfirepit_b200.so"
+CALLS = PKG / "_calls.so"
 INCLUDE = PKG.parent / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -76,7 +81,29 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
+    _build_calls(force)
     return LIB
+
+
+def _build_calls(force: bool) -> None:
+    """The module links torch and the library above (found beside it)."""
+    spec = importlib.util.find_spec("torch")
+    src = CSRC / "calls.cpp"
+    newest = max(p.stat().st_mtime for p in (src, INCLUDE / "firepit_b200.h"))
+    if spec is None or not (force or not CALLS.exists() or newest > CALLS.stat().st_mtime):
+        return
+    torch = Path(spec.origin).parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    tmp = CALLS.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           *(f"-I{p}" for p in (INCLUDE, torch / "include", torch / "include/torch/csrc/api/include",
+                                sysconfig.get_paths()["include"], cuda / "include")),
+           str(src), "-o", str(tmp), f"-L{PKG}", f"-l:{LIB.name}", f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch",
+           "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src.name}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, CALLS)
 
 
 if __name__ == "__main__":

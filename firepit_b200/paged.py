@@ -20,8 +20,9 @@ from . import _native as N
 from .gemv import ShapeError
 from .speculative import _code, _empty, _ints, _Torch
 
-# (a decode step's calls take a few microseconds each: the entry points are looked
-# up once, and the checks read each property once)
+# (a decode step's calls take a few microseconds each: on the current stream a call
+# that is right goes by _calls; what that leaves alone is checked and made here, with
+# the entry points looked up once and each property read once)
 _extend, _truncate, _append = N.lib.fpb_page_extend, N.lib.fpb_page_truncate, N.lib.fpb_paged_append
 _attn, _attn_bytes, _sample = N.lib.fpb_paged_attn, N.lib.fpb_paged_attn_workspace_bytes, N.lib.fpb_sample
 
@@ -172,6 +173,14 @@ def page_extend(tables: PageTables, counts, rows: int, padded: bool = False, out
     lengths) and says where they lie: rows in order of request (``padded``: rows / batch of them a request).
     A request that the pool, its table or the rows cannot hold whole keeps its
     length, and its rows are -1."""
+    if stream is None and _Torch.calls is not None and (out is None or out.slots is not None):
+        m = (None, None, None, None) if out is None else (out.slots, out.positions, out.requests, out.starts)
+        got = _Torch.calls.page_extend(tables.table, tables.lengths, tables.free, tables.free_count, tables.page_size,
+                                       counts, rows, padded, *m)
+        if got is not NotImplemented:
+            if type(got) is int:
+                N.check(got, "fpb_page_extend")
+            return PageMap(*got) if out is None else out
     b, device = tables.batch, tables.device
     _ints(counts, "counts", b)
     if rows < 1 or (padded and rows % b):
@@ -206,6 +215,13 @@ def page_extend(tables: PageTables, counts, rows: int, padded: bool = False, out
 def page_truncate(tables: PageTables, lengths, stream=None) -> None:
     """Cuts the requests to lengths [batch] (negative, or not below the present
     one: as it was; 0: the request is done) and gives their pages back."""
+    if stream is None and _Torch.calls is not None:
+        got = _Torch.calls.page_truncate(tables.table, tables.lengths, tables.free, tables.free_count, tables.page_size,
+                                         lengths)
+        if got is not NotImplemented:
+            if got is not None:
+                N.check(got, "fpb_page_truncate")
+            return
     device = tables.device
     _ints(lengths, "lengths", tables.batch)
     if device < 0 or device != lengths.get_device() or device != _Torch.current_device():
@@ -220,6 +236,13 @@ def paged_append(cache: PagedCache, slots, positions, k, v, q=None, q_gamma=None
     positions [rows] and writes it and v at slots [rows] (negative: no token; no two
     alike); q [rows, q_heads, head_dim] (any row and head pitch) is normed and rotated
     into q_out (allocated in q's dtype where None), which is returned."""
+    if stream is None and _Torch.calls is not None:
+        got = _Torch.calls.paged_append(cache.k, cache.v, slots, positions, k, v, q, q_gamma, k_gamma, eps, rotary_dim,
+                                        theta, q_out)
+        if got is not NotImplemented:
+            if type(got) is int:
+                N.check(got, "fpb_paged_append")
+            return got
     _, _, hk, d = cache.dims
     device, shape, dtype = cache.device, k.shape, k.dtype
     if len(shape) != 3 or shape[1] != hk or shape[2] != d or v.shape != shape or v.dtype is not dtype:
@@ -276,6 +299,12 @@ def paged_attention(q, cache: PagedCache, table, lengths, gate=None, scale: floa
     q [batch, q_heads, head_dim] f32 or bf16, any row and head pitch; scale default
     1 / sqrt(head_dim); ``workspace``: uint8 of ``paged_attention_workspace_bytes``
     (allocated where None), which calls on different streams must not share."""
+    if stream is None and _Torch.calls is not None:
+        got = _Torch.calls.paged_attention(q, cache.k, cache.v, table, lengths, gate, scale, out, workspace)
+        if got is not NotImplemented:
+            if type(got) is int:
+                N.check(got, "fpb_paged_attn")
+            return got
     _, _, hk, d = cache.dims
     device, shape = cache.device, q.shape
     if len(shape) != 3 or shape[2] != d or shape[1] % hk or not shape[1]:
@@ -335,6 +364,12 @@ def sample(logits, temperature, noise, top_k=None, top_p=None, min_p=None, logpr
     among what is kept."""
     if _Torch.module is None:
         _Torch.load()
+    if stream is None and _Torch.calls is not None:
+        got = _Torch.calls.sample(logits, temperature, noise, top_k, top_p, min_p, logprobs, out)
+        if got is not NotImplemented:
+            if type(got) is int:
+                N.check(got, "fpb_sample")
+            return got
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ShapeError(f"sample: logits [batch, vocab], rows contiguous, expected, got {list(logits.shape)}")
     b, vocab = shape = logits.shape

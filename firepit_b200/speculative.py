@@ -29,11 +29,16 @@ class _Torch:
     """torch and what the calls need of it, looked up once (a decode step's
     calls take a few microseconds each)."""
 
-    module = None
+    module = calls = None
 
     @classmethod
     def load(cls):
         import torch
+        try:
+            from . import _calls as calls
+        except ImportError:  # (not built: the same calls through ctypes, a few microseconds longer)
+            calls = None
+        cls.calls = calls
         cls.f32, cls.bf16, cls.i32, cls.u8 = torch.float32, torch.bfloat16, torch.int32, torch.uint8
         cls.codes = {torch.float32: N.FPB_F32, torch.bfloat16: N.FPB_BF16}
         cls.raw_stream = staticmethod(torch._C._cuda_getCurrentRawStream) if hasattr(

@@ -720,3 +720,118 @@ def test_sample_strides_streams_and_graphs(F, torch):
     ones = [np.float32([float(x) for x in t.cpu()]), np.zeros(b, np.int32), np.ones(b, np.float32), np.zeros(b, np.float32)]
     _, logs = F.sample(logits, t, noise, logprobs=True)
     _check_sample(torch, plain.cpu(), logs.cpu(), logits, noise, *ones)
+
+
+# ---- the wrappers ---------------------------------------------------------------------------------------------------
+def _a_step(F, torch, seed):
+    """Every operator once, with everything that it can be given; what they wrote."""
+    torch.manual_seed(seed)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cache = F.PagedCache.zeros(40, 16, 2, 64)
+    tables = F.PageTables.empty(3, 40, 16, 12)
+    counts = torch.tensor([20, 0, 33], **i32)
+    m = F.page_extend(tables, counts, 53)
+    padded = F.page_extend(tables, torch.tensor([1, 2, 0], **i32), 6, True)
+    mine = F.PageMap(torch.zeros(3, **i32), torch.zeros(3, **i32), None, torch.zeros(4, **i32))
+    assert F.page_extend(tables, torch.ones(3, **i32), 3, out=mine) is mine
+    F.page_truncate(tables, torch.tensor([21, -1, 33], **i32))
+    x = torch.randn(53, 8, 64, device="cuda")
+    gamma = torch.rand(64, device="cuda") + 0.5
+    q = F.paged_append(cache, m.slots, m.positions, x[:, 4:6], x[:, 6:], q=x[:, :4], q_gamma=gamma, k_gamma=gamma, eps=1e-5,
+                       rotary_dim=32, theta=1e6)
+    q16 = torch.empty(53, 4, 64, dtype=torch.bfloat16, device="cuda")
+    assert F.paged_append(cache, m.slots, m.positions, x[:, 4:6], x[:, 6:], q=x[:, :4], q_out=q16) is q16
+    assert F.paged_append(cache, m.slots, m.positions, x[:, 4:6], x[:, 6:]) is None
+    rows = torch.tensor([19, 0, 52], device="cuda")
+    gate = torch.randn(3, 4, 2, 64, device="cuda")[:, :, 1]
+    att = F.paged_attention(q[rows], cache, tables.table, tables.lengths, gate=gate)
+    out = torch.empty(3, 4, 64, device="cuda")
+    ws = torch.empty(F.paged_attention_workspace_bytes(cache, 3, 4), dtype=torch.uint8, device="cuda")
+    assert F.paged_attention(q16[rows], cache, tables.table, tables.lengths, scale=0.1, out=out, workspace=ws) is out
+    logits = torch.randn(3, 1000, device="cuda")
+    noise = torch.empty_like(logits).exponential_()
+    t = torch.ones(3, device="cuda")
+    k, p = torch.tensor([5, 0, 0], **i32), torch.tensor([1.0, 0.9, 1.0], device="cuda")
+    tokens, logs = F.sample(logits, t, noise, top_k=k, top_p=p, min_p=p * 0.01, logprobs=True)
+    plain = F.sample(logits.bfloat16(), t, noise)
+    given = torch.zeros(3, **i32)
+    assert F.sample(logits, None, noise, out=given) is given
+    return [m.slots, m.positions, m.requests, m.starts, padded.slots, padded.positions, padded.requests, padded.starts,
+            mine.slots, mine.positions, mine.starts, tables.table, tables.lengths, tables.free, tables.free_count, q, q16,
+            cache.k, cache.v, att, out, tokens, logs, plain, given]
+
+
+def test_calls_by_both_ways(F, torch, monkeypatch):
+    """The module of calls is there, and what it makes is what the long way makes."""
+    from firepit_b200.speculative import _Torch
+    first = _a_step(F, torch, 3)
+    assert _Torch.calls is not None
+    seen = []
+    for name in ("page_extend", "page_truncate", "paged_append", "paged_attention", "sample"):
+        call = getattr(_Torch.calls, name)
+        monkeypatch.setattr(_Torch.calls, name, lambda *a, call=call, name=name: seen.append((name, call(*a))) or seen[-1][1])
+    for x, y in zip(first, _a_step(F, torch, 3)):
+        assert torch.equal(x, y)
+    assert len(seen) == 12 and not any(got is NotImplemented or type(got) is int for _, got in seen)
+    monkeypatch.setattr(_Torch, "calls", None)
+    for x, y in zip(first, _a_step(F, torch, 3)):
+        assert x.dtype == y.dtype and x.stride() == y.stride() and torch.equal(x, y)
+
+
+def test_calls_that_are_refused(F, torch):
+    """On the device, each by one fault: an error and no launch."""
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cache = F.PagedCache.zeros(6, 16, 2, 64)
+    tables = F.PageTables.empty(3, 6, 16, 4)
+    n3, rows, f3 = torch.zeros(3, **i32), torch.zeros(5, **i32), torch.ones(3, device="cuda")
+    kv, q, q3 = (torch.zeros(*s, device="cuda") for s in ((5, 2, 64), (5, 4, 64), (3, 4, 64)))
+    logits, noise = torch.zeros(3, 10, device="cuda"), torch.ones(3, 10, device="cuda")
+    host = lambda x: x.cpu()  # noqa: E731
+    calls = [
+        lambda: F.page_extend(tables, n3[:2], 5), lambda: F.page_extend(tables, n3.long(), 5),
+        lambda: F.page_extend(tables, n3, 0), lambda: F.page_extend(tables, n3, 5, padded=True),
+        lambda: F.page_extend(tables, host(n3), 5), lambda: F.page_extend(tables, tables.lengths, 5),
+        lambda: F.page_extend(tables, n3, 5, out=F.PageMap(rows, rows[:4], None, None)),
+        lambda: F.page_extend(tables, n3, 5, out=F.PageMap(rows, host(rows), None, None)),
+        lambda: F.page_truncate(tables, n3.float()), lambda: F.page_truncate(tables, host(n3)),
+        lambda: F.page_truncate(tables, torch.zeros(6, **i32)[::2]),
+        lambda: F.paged_append(cache, rows, rows, kv[:, :1], kv[:, :1]),
+        lambda: F.paged_append(cache, rows, rows, kv, kv.bfloat16()),
+        lambda: F.paged_append(cache, rows.long(), rows, kv, kv), lambda: F.paged_append(cache, rows, rows[:4], kv, kv),
+        lambda: F.paged_append(cache, rows, host(rows), kv, kv), lambda: F.paged_append(cache, rows, rows, kv, host(kv)),
+        lambda: F.paged_append(cache, rows, rows, kv, kv, q=q.bfloat16()),
+        lambda: F.paged_append(cache, rows, rows, kv, kv, q_out=q),
+        lambda: F.paged_append(cache, rows, rows, kv, kv, q=q, q_gamma=torch.zeros(32, device="cuda")),
+        lambda: F.paged_append(cache, rows, rows, kv, kv, q=q, q_gamma=torch.zeros(64)),
+        lambda: F.paged_append(cache, rows, rows, kv, kv, q=q, q_out=q[:, :2]),
+        lambda: F.paged_append(cache, rows, rows, kv, kv, q=q, rotary_dim=65),
+        lambda: F.paged_append(cache, rows, rows, kv, kv, q=q, rotary_dim=32, theta=math.nan),
+        lambda: F.paged_append(cache, rows, rows, kv.half(), kv.half()),
+        lambda: F.paged_append(cache, rows, rows, torch.zeros(5, 2, 128, device="cuda")[..., ::2], kv),
+        lambda: F.paged_append(cache, rows, rows, torch.zeros(5, 2, 80, device="cuda")[..., :64], kv),
+        lambda: F.paged_attention(q3[:, :3], cache, tables.table, n3), lambda: F.paged_attention(q3[..., :32], cache, tables.table, n3),
+        lambda: F.paged_attention(q3.half(), cache, tables.table, n3), lambda: F.paged_attention(q3, cache, tables.table[:2], n3),
+        lambda: F.paged_attention(q3, cache, tables.table.long(), n3), lambda: F.paged_attention(q3, cache, tables.table, n3[:2]),
+        lambda: F.paged_attention(q3, cache, host(tables.table), n3),
+        lambda: F.paged_attention(q3, cache, tables.table[:, :0], n3),
+        lambda: F.paged_attention(q3, cache, tables.table, n3, gate=q3.bfloat16()),
+        lambda: F.paged_attention(q3, cache, tables.table, n3, gate=host(q3)),
+        lambda: F.paged_attention(q3, cache, tables.table, n3, out=q3.half()),
+        lambda: F.paged_attention(q3, cache, tables.table, n3, workspace=q3),
+        lambda: F.paged_attention(q3, cache, tables.table, n3, workspace=torch.zeros(16, dtype=torch.uint8, device="cuda")),
+        lambda: F.paged_attention(q3, cache, tables.table, n3, scale=math.inf),
+        lambda: F.paged_attention(q3[:0], cache, tables.table[:0], n3[:0]),
+        lambda: F.sample(logits[0], f3, noise), lambda: F.sample(logits.half(), f3, noise), lambda: F.sample(logits, n3, noise),
+        lambda: F.sample(logits, f3, noise[:, :9]), lambda: F.sample(logits, f3, noise.bfloat16()),
+        lambda: F.sample(logits, f3, host(noise)), lambda: F.sample(logits, f3, noise, top_k=f3),
+        lambda: F.sample(logits, f3, noise, top_p=n3), lambda: F.sample(logits, f3, noise, min_p=f3[:2]),
+        lambda: F.sample(logits, f3, noise, out=n3.long()), lambda: F.sample(logits, host(f3), noise),
+        lambda: F.sample(logits[:0], f3[:0], noise[:0]), lambda: F.sample(logits[:1].expand(3, 10), f3, noise),
+        lambda: F.sample(logits.t(), torch.ones(10, device="cuda"), noise.t()),
+    ]
+    before = F.launch_count()
+    for at, call in enumerate(calls):
+        with pytest.raises((F.ShapeError, F.FpbError)):
+            call()
+            pytest.fail(f"call {at} was taken")
+    assert F.launch_count() == before
