@@ -132,6 +132,15 @@ Tensor empty(at::IntArrayRef shape, at::ScalarType type, const Device &dev) {
   return at::empty(shape, at::TensorOptions().dtype(type).device(at::Device(at::kCUDA, (c10::DeviceIndex)dev.index)));
 }
 
+// n elements of a vector from `at` on: a tensor of its own over the same memory (a view
+// through the dispatcher takes a microsecond).
+Tensor part(const Tensor &t, int64_t at, int64_t n) {
+  Tensor r = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()), t.key_set(), t.dtype());
+  r.unsafeGetTensorImpl()->set_storage_offset(at);
+  r.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return r;
+}
+
 PyObject *leave() {
   Py_INCREF(Py_NotImplemented);
   return Py_NotImplemented;
@@ -182,7 +191,7 @@ PyObject *page_extend(PyObject *, PyObject *const *a, Py_ssize_t count) {
     const int64_t up = (rows + 3) / 4 * 4;
     const Tensor flat = empty({3 * up + b + 1}, at::kInt, t.dev);
     for (int i = 0; i < 4; ++i) {
-      made[i] = flat.narrow(0, i * up, i < 3 ? rows : b + 1);
+      made[i] = part(flat, i * up, i < 3 ? rows : b + 1);
       out[i] = &made[i];
     }
   } else {
