@@ -146,13 +146,14 @@ PyObject *leave() {
   return Py_NotImplemented;
 }
 
+struct WithoutGil {
+  PyThreadState *state = PyEval_SaveThread();
+  ~WithoutGil() { PyEval_RestoreThread(state); }
+};
 template <typename Call>
 int without_gil(Call call) {
-  int status;
-  Py_BEGIN_ALLOW_THREADS;
-  status = call();
-  Py_END_ALLOW_THREADS;
-  return status;
+  WithoutGil released;
+  return call();
 }
 
 // table, lengths, free, free_count, page_size

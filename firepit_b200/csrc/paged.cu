@@ -72,9 +72,15 @@ __device__ __forceinline__ int last_at(const int *at, int n, int x) {
   return lo;
 }
 
-// What a launch does of a step: all of it (one block), the rows and pages (many
-// blocks), or the state that those have read (one block, behind them).
+// What a launch does of a step: all of it (a block, or a cluster), the rows and pages
+// (many blocks), or the state that those have read (one block, behind them).
 enum PagePart { kPageAll, kPageRows, kPageState };
+
+// Behind code that lanes may leave apart: the barrier counts whole warps.
+__device__ __forceinline__ void cluster_meet() {
+  __syncwarp();
+  cluster_sync();
+}
 
 // Each block scans all requests for itself, then the blocks share the rows and the
 // new pages.  A request is served whole (its rows fit, its table and the pool have
@@ -134,14 +140,14 @@ __global__ void __launch_bounds__(kPageMaxThreads) page_extend_kernel(const __gr
   }
   __syncthreads();
   const int used = used_s;
-  if (PART != kPageRows) {
+  auto state = [&]() {
     for (int b = tid; b < a.batch; b += width)
       if (len[b] >= 0) a.lengths[b] = len[b] + a.change[b];
     if (a.starts)
       for (int b = tid; b <= a.batch; b += width) a.starts[b] = row0[b];
     if (tid == 0 && used > 0) *a.free_count = free_n - used;
-    if (PART == kPageState) return;
-  }
+  };
+  if (PART == kPageState) return state();
   // (whole numbers without a sign: a step past the last row may pass 2^31)
   const uint32_t threads = gridDim.x * width, me = blockIdx.x * width + tid;
   for (uint32_t i = me; i < (uint32_t)used; i += threads) {
@@ -184,6 +190,10 @@ __global__ void __launch_bounds__(kPageMaxThreads) page_extend_kernel(const __gr
       }
     }
   }
+  if (PART == kPageAll) {
+    if (gridDim.x > 1) cluster_meet();  // every block has read the state
+    if (blockIdx.x == 0) state();
+  }
 }
 
 // Likewise.
@@ -219,12 +229,12 @@ __global__ void __launch_bounds__(kPageMaxThreads) page_truncate_kernel(const __
     if (tid == 0) page_error(a, kErrLength);
     return;
   }
-  if (PART != kPageRows) {
+  auto state = [&]() {
     for (int b = tid; b < a.batch; b += width)
       if (kept[b] >= 0) a.lengths[b] = a.change[b];
     if (tid == 0 && back > 0) *a.free_count = free_n + (int)back;
-    if (PART == kPageState) return;
-  }
+  };
+  if (PART == kPageState) return state();
   for (uint32_t u = blockIdx.x * width + tid; u < (uint32_t)back; u += gridDim.x * width) {
     const int i = (int)u, b = last_at(off, a.batch, i);
     int32_t *entry = a.table + b * a.pitch + kept[b] + i - off[b];
@@ -232,6 +242,10 @@ __global__ void __launch_bounds__(kPageMaxThreads) page_truncate_kernel(const __
     if (page < 0 || page >= a.pages) page_error(a, kErrPage);
     a.free[free_n + (int)back - 1 - i] = page;
     *entry = -1;
+  }
+  if (PART == kPageAll) {
+    if (gridDim.x > 1) cluster_meet();
+    if (blockIdx.x == 0) state();
   }
 }
 
@@ -249,9 +263,14 @@ int check_tables(const char *name, const PageArgs &a, size_t table_pitch, size_t
 
 // One block where a step has few rows or pages; else many for those, and one behind
 // them for the state (extend and truncate, one block and many: 4096 rows 9.5 and 11.5
-// us, 8192 12.4 and 11.4, 144000 120 and 14).
-int launch_pages(void (*const (&kernel)[3])(PageArgs), const char *name, const PageArgs &a, size_t work, size_t smem,
-                 cudaStream_t s) {
+// us, 8192 12.4 and 11.4, 144000 120 and 14).  Where it is not known how much of `work`
+// there is, as for the pages that a step gives back of all that the requests may hold, a
+// cluster takes it up to `cluster` (extend and truncate of 64 requests of 564 pages, by a
+// cluster and by many blocks: one page each 9.0 and 9.2 us, all 17.2 and 16.4; and the
+// host has a launch less, 2 us; rows, which are known, go better by many: 65536 15.7 and
+// 11.7).
+int launch_pages(void (*const (&kernel)[3])(PageArgs), const char *name, const PageArgs &a, size_t work,
+                 size_t cluster, size_t smem, cudaStream_t s) {
   {
     static std::mutex mu;
     static std::vector<int> done;
@@ -267,7 +286,8 @@ int launch_pages(void (*const (&kernel)[3])(PageArgs), const char *name, const P
     }
   }
   auto launch = [&](PagePart part, unsigned blocks, unsigned threads) {
-    cudaError_t e = launch_pdl(kernel[part], blocks, threads, smem, s, a);
+    cudaError_t e = part == kPageAll && blocks > 1 ? launch_pdl_cluster(kernel[part], blocks, threads, smem, s, blocks, a)
+                                                   : launch_pdl(kernel[part], blocks, threads, smem, s, a);
     if (e != cudaSuccess) return cuda_fail(e, name);
     FPB_LAUNCH_CHECK(name);
     return (int)FPB_OK;
@@ -275,6 +295,7 @@ int launch_pages(void (*const (&kernel)[3])(PageArgs), const char *name, const P
   // (a wide block's barriers take longer, a narrow one goes through its work more often)
   const unsigned scan = a.batch <= 256 ? 256 : kPageMaxThreads;
   if (work <= 6144) return launch(kPageAll, 1, work <= 1024 ? scan : kPageMaxThreads);
+  if (work <= cluster) return launch(kPageAll, 8, kPageMaxThreads);
   const size_t blocks = std::min<size_t>((work + 4 * scan - 1) / (4 * scan), 2 * sm_count());
   if (int st = launch(kPageRows, (unsigned)blocks, scan)) return st;
   return launch(kPageState, 1, scan);
@@ -322,7 +343,7 @@ extern "C" int fpb_page_extend(int32_t *table, size_t table_pitch, size_t batch,
   a.vec = aligned_to(slots, 16) && aligned_to(positions, 16) && aligned_to(requests, 16);
   a.error = device_error_ptr();
   return launch_pages({page_extend_kernel<kPageAll>, page_extend_kernel<kPageRows>, page_extend_kernel<kPageState>},
-                      "page_extend_kernel", a, rows, 3 * (batch + 1) * sizeof(int), as_stream(stream));
+                      "page_extend_kernel", a, rows, 0, 3 * (batch + 1) * sizeof(int), as_stream(stream));
 }
 
 extern "C" int fpb_page_truncate(int32_t *table, size_t table_pitch, size_t batch, size_t max_pages, int32_t *lengths,
@@ -333,6 +354,7 @@ extern "C" int fpb_page_truncate(int32_t *table, size_t table_pitch, size_t batc
   if (int st = check_tables("fpb_page_truncate", a, table_pitch, batch, max_pages, pages, page_size)) return st;
   a.error = device_error_ptr();
   return launch_pages({page_truncate_kernel<kPageAll>, page_truncate_kernel<kPageRows>, page_truncate_kernel<kPageState>},
-                      "page_truncate_kernel", a, std::min(batch * max_pages, pages), 2 * (batch + 1) * sizeof(int),
+                      "page_truncate_kernel", a, std::min(batch * max_pages, pages), 65536,
+                      2 * (batch + 1) * sizeof(int),
                       as_stream(stream));
 }

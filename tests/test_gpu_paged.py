@@ -83,7 +83,8 @@ def _maps(m, want):
 
 @pytest.mark.parametrize("batch,pages,p,width,rows,padded", [
     (1, 3, 1, 3, 4, False), (5, 40, 16, 9, 64, False), (7, 30, 3, 11, 35, True), (64, 900, 16, 20, 64, True),
-    (1030, 4000, 8, 6, 9001, False), (3, 2000, 24, 700, 30000, False), (300, 60, 4, 5, 800, False), (700, 9000, 1, 30, 9001, False)])
+    (1030, 4000, 8, 6, 9001, False), (3, 2000, 24, 700, 30000, False), (300, 60, 4, 5, 800, False), (700, 9000, 1, 30, 9001, False),
+    (40, 70000, 2, 2000, 4000, False)])
 def test_page_tables_follow_the_stack(F, torch, batch, pages, p, width, rows, padded):
     """Steps of extensions and truncations, among them more than the pool, the
     tables and the rows can hold."""
