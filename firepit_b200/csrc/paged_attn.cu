@@ -1124,7 +1124,11 @@ extern "C" int fpb_paged_attn(const void *q, int q_dtype, size_t q_pitch, size_t
   if (workspace_bytes < need)
     return fail(FPB_ERR_WORKSPACE, "fpb_paged_attn: workspace %zu < %zu bytes", workspace_bytes, need);
   const bool f32 = page_dtype == FPB_F32;
-  const Plan p = plan_for(batch, q_heads, kv_heads, head_dim, f32);
+  Plan p = plan_for(batch, q_heads, kv_heads, head_dim, f32);
+  {  // no more blocks than the tables' tokens can have shares
+    const size_t tok = f32 ? 8 : 16, steps = (max_pages * page_size + tok - 1) / tok;
+    p.blocks = std::min(p.blocks, batch * kv_heads * p.tiles * ((steps + p.least - 1) / p.least));
+  }
   if (p.blocks > 0x7fffffff) return fail(FPB_ERR_SHAPE, "fpb_paged_attn: %zu blocks", p.blocks);
   PagedArgs a{};
   a.q = q;

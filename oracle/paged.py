@@ -1,4 +1,4 @@
-"""numpy restatement in 64 bits of serving over a paged cache: the checker of
+"""numpy restatement in 64 bits of serving over a paged cache: the oracle of
 firepit_b200's page tables, paged attention and sampling.
 
 TEST INFRASTRUCTURE ONLY: the product never imports it.
