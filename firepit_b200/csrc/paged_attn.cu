@@ -227,9 +227,15 @@ struct PagedShare {
 // The sessions' steps are cut into shares of S, each session's evenly, and the
 // shares numbered in order of session, kv head, part and row tile.  Every block
 // finds its own: false where there is none.  `steps` [batch] in shared memory.
-// One wave: the smallest S whose shares the GPU has room for at once, among 32
-// between total / slots, which is below it, and total / (slots - items), whose
-// shares fit: each item rounds up by less than one.  Several: total / (waves * slots).
+// Where the GPU has room for an item a block: the smallest S whose shares it has room
+// for at once, total / slots or else among 32 between that, which is below it, and total
+// / (slots - items), whose shares fit (each item rounds up by less than one).  Shares
+// that may come one after another: total / (waves * slots); but where that is less than
+// a share's least, a few blocks more than there is room for would take as long as all of
+// them, so one wave then, too, with heads of up to 128 (us for two waves and one: f32
+// pages, 20 x 2000 tokens x 8 heads of 128 85 and 67, 55 x 600 73 and 53; longer ones want
+// the finer shares, 37 x 9000 492 and 579, and so do 110 x 2000 x 2 heads of 256, 51 and
+// 58).
 
 // Lane 0 lo, lane 31 hi, the others between them, in even ratios but for rounding.
 __device__ __forceinline__ int between(int lo, int hi) {
@@ -259,11 +265,12 @@ __device__ __noinline__ FewPlan few_plan(const PagedArgs &a, int n) {
   if (work == 0) return p;
   // ceil(work / n); 64-bit quotients take a few hundred cycles
   auto over = [&](uint32_t n) { return work >> 31 ? (int)min((work + n - 1) / n, 0x7fffffffull) : (int)(((uint32_t)work + n - 1) / n); };
-  int S;
-  if (a.waves) {
-    S = max(a.least, over((uint32_t)a.waves * a.slots));
-  } else {
-    const int items = __popc(alive) * heads, lo = over(a.slots), hi = over(a.slots - items);
+  const uint32_t items = __popc(alive) * heads;
+  int S = over((uint32_t)max(1, a.waves) * a.slots);
+  const bool one = items < (uint32_t)a.slots && (!a.waves || (a.head_dim <= 128 && S < a.least));
+  S = max(a.least, one ? over(a.slots) : S);
+  if (one && __reduce_add_sync(0xffffffffu, ((uint32_t)p.steps + S - 1) / S) * heads > (uint32_t)a.slots) {
+    const int lo = over(a.slots), hi = over(a.slots - items);
     const uint32_t trial = max(a.least, between(lo, hi));
     uint32_t blocks = 0;
 #pragma unroll 4
@@ -348,25 +355,37 @@ __device__ __forceinline__ bool paged_share(const PagedArgs &a, int *steps, Page
   const int heads = a.kv_heads * a.tiles;
   const unsigned long long work = sum * heads;
   if (work == 0) return false;
-  int S;
-  if (a.waves) {
-    const unsigned long long all = (unsigned long long)a.waves * a.slots;
-    S = (int)min((work + all - 1) / all, 0x7fffffffull);
-  } else {
-    const int items = alive * heads;
-    const int lo = (int)((work + a.slots - 1) / a.slots), hi = (int)((work + a.slots - items - 1) / (a.slots - items));
-    const int trial = max(a.least, between(lo, hi));
-    int n = 0;
-    for (int b = w; b < a.batch; b += W) n += (steps[b] + trial - 1) / trial;
-    blocks_s[w][lane] = n;
+  const uint32_t items = alive * heads;
+  auto over = [&](uint32_t n) { return (int)min((work + n - 1) / n, 0x7fffffffull); };
+  int S = over((uint32_t)max(1, a.waves) * a.slots);
+  const bool one = items < (uint32_t)a.slots && (!a.waves || (a.head_dim <= 128 && S < a.least));
+  S = max(a.least, one ? over(a.slots) : S);
+  bool fit = true;
+  if (one) {  // whether the blocks of that many steps each do
+    uint32_t n = 0;
+    for (int b = tid; b < a.batch; b += kThreads) n += ((uint32_t)steps[b] + S - 1) / S;
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) blocks_s[w][0] = (int)n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) n += blocks_s[i][0];
+    fit = n * heads <= (uint32_t)a.slots;
+    __syncthreads();
+  }
+  if (!fit) {
+    const int lo = over(a.slots), hi = over(a.slots - items);
+    const uint32_t trial = max(a.least, between(lo, hi));
+    uint32_t n = 0;
+    for (int b = w; b < a.batch; b += W) n += ((uint32_t)steps[b] + trial - 1) / trial;
+    blocks_s[w][lane] = (int)n;
     __syncthreads();
     n = 0;
 #pragma unroll
     for (int i = 0; i < W; ++i) n += blocks_s[i][lane];
-    const uint32_t fits = __ballot_sync(0xffffffffu, n * heads <= a.slots);
-    S = __shfl_sync(0xffffffffu, trial, __ffs(fits) - 1);
+    const uint32_t fits = __ballot_sync(0xffffffffu, n * heads <= (uint32_t)a.slots);
+    S = __shfl_sync(0xffffffffu, (int)trial, __ffs(fits) - 1);
   }
-  S = max(S, a.least);
   // the session of this block, and the slots of split sessions before it
   int blocks0 = 0, slots0 = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kThreads) {

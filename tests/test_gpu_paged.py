@@ -356,7 +356,8 @@ def test_paged_attention_many_sessions(F, torch, pages):
 
 @pytest.mark.parametrize("pages", ["f32", "bf16"])
 @pytest.mark.parametrize("b,hq,hk,d,most", [(70, 4, 1, 64, 900), (41, 12, 1, 256, 60), (20, 16, 8, 128, 700),
-                                            (32, 8, 4, 80, 300), (33, 8, 4, 80, 300), (1, 64, 64, 32, 2000)])
+                                            (32, 8, 4, 80, 300), (33, 8, 4, 80, 300), (1, 64, 64, 32, 2000), (30, 16, 8, 64, 4000),
+                                            (40, 8, 8, 64, 2500)])
 def test_paged_attention_ways_to_cut(F, torch, pages, b, hq, hk, d, most):
     """Few and many sessions, in one wave of blocks and in several, some without
     tokens and one whose length cannot be."""
