@@ -35,10 +35,11 @@ namespace {
 using namespace sm100;
 
 struct PagedArgs {
-  const void *q;
+  const void *q, *k, *v;
   const float *gate;
   const int32_t *table, *lengths;
   long long q_pitch, q_head, gate_pitch, gate_head, table_pitch;  // elements
+  long long page_pitch, row_pitch, head_pitch;                    // of k and v
   int batch, q_heads, kv_heads, group, head_dim, max_pages, pages, page_size, q_bf16, q_vec;
   int box;     // tokens of a copy: the largest power of two that divides the page size, up to a step's
   int whole;   // a copy takes all of a head vector's 128-byte pieces (else one: the last is not whole)
@@ -50,18 +51,21 @@ struct PagedArgs {
   float scale_log2;  // scale * log2(e): scores and maxima are held in powers of two
   void *out;
   int out_bf16;
-  float *part;      // [slot][row][head_dim] numerators
-  float2 *part_ml;  // [slot][row] maximum, sum
+  float *part;      // [slot][row][head_dim] the share's own outputs
+  float2 *part_ml;  // [slot][row] maximum, sum of weights
   unsigned long long *flags, token;  // [slot]: `token`, this call's own, where the share's results are there
   int *error;
 };
 
 constexpr int kPagedMaxBatch = 4096, kPagedWaves = 2;
 constexpr int kErrPagedWait = 503;
-// The maximum may lag by kLag (powers of two) before the sums are rescaled, and
-// weights are held as 2^(y - m - kBack): 2^20 of them times a value of the type's
-// largest then stay within f32, and weights down to 2^-98 of the largest count.
-constexpr float kLag = 8.0f, kBack = 28.0f;
+// The maximum may lag by kLag (powers of two) before the sums are rescaled: weights
+// are 2^(y - m), up to 2^8, so that values down to the smallest normal number give
+// normal numerators, and weights down to 2^-126 count.
+constexpr float kLag = 8.0f;
+// Outputs of a share below this (or not finite) are found again by plain_share(): of f32
+// values below 2^-112 the tensor cores' low parts are short of bits.
+constexpr float kSmall = 7.888609e-31f;  // 2^-100
 
 __device__ __forceinline__ float pow2(float x) {
   float y;
@@ -160,17 +164,16 @@ __device__ __forceinline__ void load_q8(const PagedArgs &a, int b, int h, int d,
   }
 }
 
-// N columns of head h from d on: the numerators x over the sum l, times the gate's
-// sigmoid where there is one.  No token: zeros.
+// N columns of head h from d on: the outputs x, times the gate's sigmoid where there is
+// one.  No weights (their sum l is 0): zeros.
 template <int N>
 __device__ __forceinline__ void store_out(const PagedArgs &a, int b, int h, int d, const float (&x)[N], float l,
                                           const float (&gate)[N]) {
   const size_t at = ((size_t)b * a.q_heads + h) * a.head_dim + d;
-  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
   float o[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) {
-    o[k] = l != 0.0f ? x[k] * inv : 0.0f;
+    o[k] = l != 0.0f ? x[k] : 0.0f;
     if (a.gate && l != 0.0f) o[k] /= 1.0f + expf(-gate[k]);
   }
 #pragma unroll
@@ -442,6 +445,94 @@ __device__ __forceinline__ bool paged_share(const PagedArgs &a, int *steps, Page
   fence_proxy_async_smem();  // the words in `steps` lie where the first copies go
   __syncthreads();
   return true;
+}
+
+// Whether a share's output is one that the tensor cores' products may have wrong.
+__device__ __forceinline__ bool unusual(float x) {
+  return !(fabsf(x) <= 3.402823466e38f) || (fabsf(x) < kSmall && x != 0.0f);
+}
+
+// The block's share again where some of its outputs are unusual(): the whole block calls
+// this, and finds numerators, maxima and sums in place of those in sm, m_s and l_s.
+// Scores in 64 bits, weights and values in f32, the warps' tokens one by one (a warp takes
+// every W-th) straight from the pages.  Two passes over them, of which the first finds a
+// row's maximum and the power of two at or above its sum, so that weights add up to 1 at
+// most: whatever the values are, their numerators stay within f32.
+template <typename T, int W, int NR, int PITCH>
+__device__ __noinline__ void plain_share(const PagedArgs &a, PagedShare me, int rows, int head0, float *sm,
+                                         float (*m_s)[NR], float (*l_s)[NR]) {
+  constexpr int kTok = sizeof(T) == 2 ? 16 : 8;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = lane * 8, D = a.head_dim;
+  // (without a sign: a step past the last token may pass 2^31)
+  const uint32_t first = (uint32_t)me.first * kTok + w, end = min((uint32_t)me.length, (uint32_t)(me.first + me.count) * kTok);
+  const int32_t *table = a.table + me.b * a.table_pitch;
+  // eight elements of token t, from the lane's column on; false where its page is none
+  auto load8 = [&](const void *base, uint32_t t, float (&x)[8]) {
+    const int row = (int)(t % (uint32_t)a.page_size), page = table[t / (uint32_t)a.page_size];
+    if (page < 0 || page >= a.pages) return false;
+    const T *p = static_cast<const T *>(base) + page * a.page_pitch + row * a.row_pitch + me.kvh * a.head_pitch + col;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = col < D ? static_cast<float>(p[k]) : 0.0f;
+    return true;
+  };
+  auto score = [&](const float (&q)[8], const float (&k)[8]) {
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s = fma((double)q[i], (double)k[i], s);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return (float)(s * (double)a.scale_log2);
+  };
+  for (int r = 0; r < rows; ++r) {
+    float q[8], x[8], m = -INFINITY, l = 0.0f;
+    load_q8(a, me.b, head0 + r, col, col < D, q);
+    for (uint32_t t = first; t < end; t += W) {
+      if (!load8(a.k, t, x)) continue;
+      const float y = score(q, x);
+      if (y == -INFINITY) continue;
+      if (y > m) {
+        l = m == -INFINITY ? 0.0f : l * pow2(m - y);
+        m = y;
+      }
+      l += pow2(y - m);
+    }
+    if (lane == 0) {
+      m_s[w][r] = m;
+      l_s[w][r] = l;
+    }
+  }
+  __syncthreads();
+  float my_l = 0.0f, my_base = -INFINITY;  // of row `lane`
+  for (int r = 0; r < rows; ++r) {
+    float q[8], x[8], acc[8], top = -INFINITY, sum = 0.0f, l = 0.0f;
+    for (int i = 0; i < W; ++i) top = fmaxf(top, m_s[i][r]);
+    for (int i = 0; i < W; ++i) sum = fmaf(l_s[i][r], m_s[i][r] == -INFINITY ? 0.0f : pow2(m_s[i][r] - top), sum);
+    const float base = sum == 0.0f ? 0.0f : top + ceilf(log2f(sum));
+    load_q8(a, me.b, head0 + r, col, col < D, q);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
+    for (uint32_t t = first; t < end; t += W) {
+      if (!load8(a.k, t, x)) continue;
+      const float y = score(q, x), p = pow2(y - base);
+      load8(a.v, t, x);
+      l += p;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) acc[k] = fmaf(p, x[k], acc[k]);
+    }
+    if (col < D) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sm[(w * NR + r) * PITCH + col + k] = acc[k];
+    }
+    if (lane == r) {
+      my_l = l;
+      if (sum != 0.0f) my_base = base;
+    }
+  }
+  __syncthreads();
+  if (lane < rows) {
+    m_s[w][lane] = my_base;
+    l_s[w][lane] = my_l;
+  }
 }
 
 template <typename T, int DP, int NR, bool ONCE>
@@ -724,8 +815,7 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
       uint32_t ph[kNT][2], pl[kNT][2];
 #pragma unroll
       for (int i = 0; i < kNT; ++i) {
-        const float base[2] = {m[i][0] == -INFINITY ? 0.0f : -kBack - m[i][0],
-                               m[i][1] == -INFINITY ? 0.0f : -kBack - m[i][1]};
+        const float base[2] = {m[i][0] == -INFINITY ? 0.0f : -m[i][0], m[i][1] == -INFINITY ? 0.0f : -m[i][1]};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float p0 = pow2(y[i][0][h] + base[0]), p1 = pow2(y[i][1][h] + base[1]);
@@ -859,7 +949,7 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
           acc[k][3] *= f1;
         }
       }
-      const float base = m == -INFINITY ? 0.0f : -kBack - m;
+      const float base = m == -INFINITY ? 0.0f : -m;
       const float p0 = pow2(y[0] + base), p1 = pow2(y[1] + base);
       l += p0 + p1;
       uint32_t ph[2], pl[2];
@@ -913,34 +1003,45 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
         mine_f[(2 * c + (e & 1)) * Sh::kEndPitch + 32 * (k >> 1) + 4 * g + 2 * (k & 1) + (e >> 1)] = acc[k][e];
   }
   __syncthreads();
-  // the warps' results meet: maxima, then sums over one maximum in warp order
-  for (int r = w; r < rows; r += W) {
-    float top = -INFINITY, f[W], sum = 0.0f;
+  // The warps' results meet: maxima, then sums over one maximum in warp order; weights
+  // over their sum, so that no sum passes the values it is of.
+  for (bool plain = false;; plain = true) {
+    bool again = false;
+    for (int r = w; r < rows; r += W) {
+      float top = -INFINITY, f[W], sum = 0.0f;
 #pragma unroll
-    for (int x = 0; x < W; ++x) top = fmaxf(top, m_s[x][r]);
-#pragma unroll
-    for (int x = 0; x < W; ++x) {
-      f[x] = m_s[x][r] == -INFINITY ? 0.0f : pow2(m_s[x][r] - top);
-      sum = fmaf(l_s[x][r], f[x], sum);
-    }
-    const size_t to = (size_t)me.slot * NR + r;
-    for (int d = lane * 2; d < D; d += 64) {
-      float2 o = make_float2(0.0f, 0.0f);
+      for (int x = 0; x < W; ++x) top = fmaxf(top, m_s[x][r]);
 #pragma unroll
       for (int x = 0; x < W; ++x) {
-        const float2 v = *reinterpret_cast<const float2 *>(sm + ((size_t)x * NR + r) * Sh::kEndPitch + d);
-        o.x = fmaf(v.x, f[x], o.x);
-        o.y = fmaf(v.y, f[x], o.y);
+        f[x] = m_s[x][r] == -INFINITY ? 0.0f : pow2(m_s[x][r] - top);
+        sum = fmaf(l_s[x][r], f[x], sum);
       }
-      if (me.parts > 1) {
-        *reinterpret_cast<float2 *>(a.part + to * D + d) = o;
-      } else {
-        const float *g = a.gate ? a.gate + (size_t)me.b * a.gate_pitch + (size_t)(head0 + r) * a.gate_head + d : nullptr;
-        const float x[2] = {o.x, o.y}, gate[2] = {g ? g[0] : 0.0f, g ? g[1] : 0.0f};
-        store_out<2>(a, me.b, head0 + r, d, x, sum, gate);
+      const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+      for (int x = 0; x < W; ++x) f[x] *= inv;
+      const size_t to = (size_t)me.slot * NR + r;
+      for (int d = lane * 2; d < D; d += 64) {
+        float2 o = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int x = 0; x < W; ++x) {
+          const float2 v = *reinterpret_cast<const float2 *>(sm + ((size_t)x * NR + r) * Sh::kEndPitch + d);
+          o.x = fmaf(v.x, f[x], o.x);
+          o.y = fmaf(v.y, f[x], o.y);
+        }
+        again |= unusual(o.x) | unusual(o.y);
+        if (me.parts > 1) {
+          *reinterpret_cast<float2 *>(a.part + to * D + d) = o;
+        } else {
+          const float *g = a.gate ? a.gate + (size_t)me.b * a.gate_pitch + (size_t)(head0 + r) * a.gate_head + d : nullptr;
+          const float x[2] = {o.x, o.y}, gate[2] = {g ? g[0] : 0.0f, g ? g[1] : 0.0f};
+          store_out<2>(a, me.b, head0 + r, d, x, sum, gate);
+        }
       }
+      if (me.parts > 1 && lane == 0) a.part_ml[to] = make_float2(top, sum);
     }
-    if (me.parts > 1 && lane == 0) a.part_ml[to] = make_float2(top, sum);
+    if (!__syncthreads_or(again) || plain) break;
+    plain_share<T, W, NR, Sh::kEndPitch>(a, me, rows, head0, sm, m_s, l_s);
+    __syncthreads();
   }
   if (me.parts == 1) return;
   // The shares of an item meet in the block that finds all of them there: each says
@@ -969,8 +1070,8 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
   if (!last_s) return;
   const float2 *ml = a.part_ml + (size_t)slot0 * NR;
   const float *part = a.part + (size_t)slot0 * NR * D;
-  // (a thread's fours of columns, and of eight shares each, are asked for together, and the gates with them)
-  constexpr int kItems = (NR * DP / 4 + Sh::kThreads - 1) / Sh::kThreads, kAtOnce = kItems >= 4 ? 4 : kItems == 2 ? 10 : 12;
+  // (a thread's fours of columns, of a few shares at once, are asked for together, and the gates with them)
+  constexpr int kItems = (NR * DP / 4 + Sh::kThreads - 1) / Sh::kThreads, kAtOnce = kItems >= 8 ? 2 : kItems >= 4 ? 4 : kItems == 2 ? 10 : 12;
   float4 o[kItems], gate[kItems];
   float top[kItems], sum[kItems];
   int row[kItems], col[kItems];
@@ -1005,17 +1106,23 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
       float high = top[j];
 #pragma unroll
       for (int k = 0; k < kAtOnce; ++k) high = fmaxf(high, y[j][k].x);
-      const float old = top[j] == -INFINITY ? 0.0f : pow2(top[j] - high);
+      float old = top[j] == -INFINITY ? 0.0f : sum[j] * pow2(top[j] - high);
       top[j] = high;
+      sum[j] = old;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        y[j][k].y *= y[j][k].x == -INFINITY ? 0.0f : pow2(y[j][k].x - high);
+        sum[j] += y[j][k].y;
+      }
+      const float inv = sum[j] != 0.0f ? 1.0f / sum[j] : 0.0f;
+      old *= inv;
       o[j].x *= old;
       o[j].y *= old;
       o[j].z *= old;
       o[j].w *= old;
-      sum[j] *= old;
 #pragma unroll
       for (int k = 0; k < kAtOnce; ++k) {
-        const float f = y[j][k].x == -INFINITY ? 0.0f : pow2(y[j][k].x - high);
-        sum[j] = fmaf(y[j][k].y, f, sum[j]);
+        const float f = y[j][k].y * inv;
         o[j].x = fmaf(v[j][k].x, f, o[j].x);
         o[j].y = fmaf(v[j][k].y, f, o[j].y);
         o[j].z = fmaf(v[j][k].z, f, o[j].z);
@@ -1151,6 +1258,11 @@ extern "C" int fpb_paged_attn(const void *q, int q_dtype, size_t q_pitch, size_t
   if (p.blocks > 0x7fffffff) return fail(FPB_ERR_SHAPE, "fpb_paged_attn: %zu blocks", p.blocks);
   PagedArgs a{};
   a.q = q;
+  a.k = k_pages;
+  a.v = v_pages;
+  a.page_pitch = (long long)page_pitch;
+  a.row_pitch = (long long)row_pitch;
+  a.head_pitch = (long long)head_pitch;
   a.gate = gate;
   a.table = table;
   a.lengths = lengths;

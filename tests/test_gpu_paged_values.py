@@ -1,0 +1,90 @@
+"""Attention over the paged cache where numbers leave the usual range: values from the
+smallest normal number to the largest, against the formula in 64 bits.
+
+The bars are test_gpu_paged.py's, and n * 2^-148 for sums and products below the normal
+range (each is off by 2^-149 at most).
+"""
+import math
+
+import numpy as np
+import pytest
+
+from test_gpu_paged import F, _attention_case, _dev, _host, _no_device_error, torch  # noqa: F401  (fixtures)
+
+pytestmark = pytest.mark.gpu
+
+KINDS = ("plain", "columns", "small", "large")
+
+
+def _special(torch, kind, rng, i, n, q, k, v, scale):
+    """What is out of the ordinary in session i; k, v [n, heads, d] and q [heads, d] are
+    f32 copies on the host, in place."""
+    d = q.shape[1]
+    if kind == "columns":
+        v *= 2.0 ** np.linspace(-120, 120, d).round().astype(np.float32)
+    elif kind == "small":
+        v *= np.float32(2.0 ** -118)
+    elif kind == "large":
+        v *= np.float32(2.0 ** 122)
+
+
+def _want(q, k, v, scale):
+    """(output, sum of p |v| over finite values, largest sum of |q k| scale of a finite score)."""
+    with np.errstate(invalid="ignore", over="ignore"):
+        s = (k @ q) * scale
+        p = np.exp(s - s.max())
+        p /= p.sum()
+        out = np.array([(p * col)[(p != 0) | ~np.isfinite(col) | np.isnan(p)].sum() for col in v.T])
+        fine = np.isfinite(s)
+        most = float((np.abs(k[fine]) @ np.abs(q)).max() * scale) if fine.any() else 0.0
+        return out, np.nan_to_num(p) @ np.where(np.isfinite(v), np.abs(v), 0.0), most
+
+
+@pytest.mark.parametrize("pages", ["f32", "bf16"])
+@pytest.mark.parametrize("n,hq,hk,d,p,times,dtype", [
+    (40, 8, 2, 64, 16, 1, "f32"), (1, 4, 2, 64, 8, 1, "f32"), (3001, 4, 2, 128, 16, 1, "f32"),
+    (1500, 32, 2, 128, 32, 1, "f32"), (700, 4, 1, 256, 16, 1, "bf16"), (333, 16, 1, 256, 64, 1, "f32"),
+    (90, 6, 2, 80, 24, 1, "f32"), (450, 8, 8, 64, 7, 5, "f32"), (130, 20, 2, 192, 16, 9, "bf16")])
+def test_paged_attention_values_out_of_the_ordinary(F, torch, n, hq, hk, d, p, times, dtype, pages):
+    """Sessions of each kind beside one another, whole and in shares, in one wave of
+    blocks and (many sessions) in several."""
+    torch.manual_seed(n + d)
+    rng = np.random.default_rng(n + d)
+    b = len(KINDS) * times
+    lengths = [max(1, n - 3 * (i % 4)) for i in range(b)]
+    q, gate, cache, table, lens = _attention_case(F, torch, rng, lengths, hq, hk, d, p, dtype, pages)
+    scale = d ** -0.5
+    host, tab = [], table.cpu().long()
+    for i, m in enumerate(lengths):
+        ids = tab[i, :-(-m // p)].cuda()
+        qi = q[i].float().cpu().numpy()
+        ki, vi = (t[ids].float().cpu().numpy().reshape(-1, hk, d)[:m] for t in (cache.k, cache.v))
+        _special(torch, KINDS[i % len(KINDS)], rng, i, m, qi, ki, vi, scale)
+        rows = torch.arange(m, device="cuda")
+        for t, x in ((cache.k, ki), (cache.v, vi)):
+            t.view(-1, hk, d)[ids[rows // p] * p + rows % p] = _dev(torch, x).to(t.dtype)
+        q[i] = _dev(torch, qi).to(q.dtype)
+        host.append((_host(q[i]), *(_host(t[ids]).reshape(-1, hk, d)[:m] for t in (cache.k, cache.v))))
+    out = torch.full(q.shape, 7.0, device="cuda")
+    assert F.paged_attention(q, cache, table, lens, gate=gate, out=out) is out
+    again = F.paged_attention(q, cache, table, lens, gate=gate)
+    assert torch.equal(torch.nan_to_num(again), torch.nan_to_num(out.to(again.dtype)))
+    got, g = _host(out), 1.0 / (1.0 + np.exp(-_host(gate)))
+    two = 2.0 ** -16 if pages == "bf16" else 0.0
+    for i, (qi, ki, vi) in enumerate(host):
+        kind = KINDS[i % len(KINDS)]
+        for h in range(hq):
+            want, pv, most = _want(qi[h], ki[:, h // (hq // hk)], vi[:, h // (hq // hk)], scale)
+            where = (kind, i, h)
+            with np.errstate(invalid="ignore"):
+                ds = most * ((d + 4) * 2.0 ** -24 + two)
+                bar = (2 * ds + 2.0 ** -20 + (lengths[i] + 64) * 2.0 ** -23 + 2 * two) * pv + lengths[i] * 2.0 ** -148
+                want, bar = want * g[i, h], bar * g[i, h] + 2.0 ** -148
+                bar = bar + np.abs(want) * (2.0 ** -24 + 2.0 ** -21)
+                fine = np.isfinite(want)
+                assert (np.isnan(got[i, h]) == np.isnan(want)).all(), where
+                inf = np.isinf(want)
+                assert (got[i, h][inf] == want[inf]).all(), where
+                off = np.abs(got[i, h] - want)[fine] / bar[fine]
+                assert (off <= 1).all(), (*where, float(np.nanmax(off)))
+        assert np.isfinite(got[i]).all() and (kind != "small" or (got[i] != 0).all())
