@@ -185,6 +185,23 @@ __device__ __forceinline__ void store_out(const PagedArgs &a, int b, int h, int 
   }
 }
 
+// What a block does: steps [first, first + count) of a session's kv head and row tile.
+struct PagedShare {
+  int b, kvh, tile, length, first, count, part, parts, slot;
+};
+
+// Two columns of a share's row r: its output where the session is whole, else for the join.
+__device__ __forceinline__ void keep_out(const PagedArgs &a, const PagedShare &me, int rows, int r, int h, int d, float2 o,
+                                         float sum) {
+  if (me.parts > 1) {
+    *reinterpret_cast<float2 *>(a.part + ((size_t)me.slot * rows + r) * a.head_dim + d) = o;
+    return;
+  }
+  const float *g = a.gate ? a.gate + (size_t)me.b * a.gate_pitch + (size_t)h * a.gate_head + d : nullptr;
+  const float x[2] = {o.x, o.y}, gate[2] = {g ? g[0] : 0.0f, g ? g[1] : 0.0f};
+  store_out<2>(a, me.b, h, d, x, sum, gate);
+}
+
 // Operand row i of eight is token token_at(i) of its eight: a quarter of a warp
 // then reads 16 bytes from all of the banks.  For f32 the values' rows are read by
 // pairs of them too.
@@ -220,11 +237,6 @@ struct PagedShape {
   static constexpr size_t kQueries = (size_t)2 * NR * kQPitch * sizeof(T);
   static constexpr size_t smem = 1023 + kOver + kQueries;
   static_assert(kPlan <= kOver && kBlocks * (smem + 4 * 1024) <= 228 * 1024);
-};
-
-// What a block does: steps [first, first + count) of a session's kv head and row tile.
-struct PagedShare {
-  int b, kvh, tile, length, first, count, part, parts, slot;
 };
 
 // The sessions' steps are cut into shares of S, each session's evenly, and the
@@ -452,28 +464,33 @@ __device__ __forceinline__ bool unusual(float x) {
   return !(fabsf(x) <= 3.402823466e38f) || (fabsf(x) < kSmall && x != 0.0f);
 }
 
-// The block's share again where some of its outputs are unusual(): the whole block calls
-// this, and finds numerators, maxima and sums in place of those in sm, m_s and l_s.
-// Scores in 64 bits, weights and values in f32, the warps' tokens one by one (a warp takes
-// every W-th) straight from the pages.  Two passes over them, of which the first finds a
-// row's maximum and the power of two at or above its sum, so that weights add up to 1 at
-// most: whatever the values are, their numerators stay within f32.
+// The block's share again, where some of its outputs are unusual(): the whole block calls
+// this, with the warps' numerators, maxima and sums in sm, m_s and l_s.  Outputs that a NaN
+// among the inputs makes NaN are to be that, so NaN is looked for first.  Other outputs mean
+// that the share is done again: scores in 64 bits, weights and values in f32, straight from
+// the pages, a token at a time (a warp takes every W-th).  Two passes, of which the first
+// finds a row's maximum and the power of two at or above its sum, so that weights add up to
+// 1 at most: whatever the values are, their numerators stay within f32.  An infinite value
+// counts whole however small its weight is: only a score of -inf has one of 0.
+// (16 x 8192 tokens x 2 heads of 256, with one NaN or one a page: 249 and 279 us for 47;
+// twenty times that where everything is done again.)
 template <typename T, int W, int NR, int PITCH>
 __device__ __noinline__ void plain_share(const PagedArgs &a, PagedShare me, int rows, int head0, float *sm,
                                          float (*m_s)[NR], float (*l_s)[NR]) {
   constexpr int kTok = sizeof(T) == 2 ? 16 : 8;
+  __shared__ uint32_t nan_columns[32], nan_rows;  // outputs that are to be NaN: eight columns a word, or whole rows
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = lane * 8, D = a.head_dim;
   // (without a sign: a step past the last token may pass 2^31)
   const uint32_t first = (uint32_t)me.first * kTok + w, end = min((uint32_t)me.length, (uint32_t)(me.first + me.count) * kTok);
   const int32_t *table = a.table + me.b * a.table_pitch;
-  // eight elements of token t, from the lane's column on; false where its page is none
-  auto load8 = [&](const void *base, uint32_t t, float (&x)[8]) {
+  // where the lane's columns of token t lie, in elements; -1: its page is none
+  auto place = [&](uint32_t t) {
     const int row = (int)(t % (uint32_t)a.page_size), page = table[t / (uint32_t)a.page_size];
-    if (page < 0 || page >= a.pages) return false;
-    const T *p = static_cast<const T *>(base) + page * a.page_pitch + row * a.row_pitch + me.kvh * a.head_pitch + col;
+    return page >= 0 && page < a.pages ? page * a.page_pitch + row * a.row_pitch + me.kvh * a.head_pitch + col : -1ll;
+  };
+  auto load8 = [&](const void *base, long long at, float (&x)[8]) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = col < D ? static_cast<float>(p[k]) : 0.0f;
-    return true;
+    for (int k = 0; k < 8; ++k) x[k] = col < D ? static_cast<float>(static_cast<const T *>(base)[at + k]) : 0.0f;
   };
   auto score = [&](const float (&q)[8], const float (&k)[8]) {
     double s = 0.0;
@@ -483,15 +500,77 @@ __device__ __noinline__ void plain_share(const PagedArgs &a, PagedShare me, int 
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     return (float)(s * (double)a.scale_log2);
   };
+  // row r's maximum over the warps, and sum over that
+  auto sum_of = [&](int r, float *top) {
+    float sum = 0.0f;
+    *top = -INFINITY;
+    for (int x = 0; x < W; ++x) *top = fmaxf(*top, m_s[x][r]);
+    for (int x = 0; x < W; ++x) sum += l_s[x][r] * (m_s[x][r] == -INFINITY ? 0.0f : pow2(m_s[x][r] - *top));
+    return sum;
+  };
+  // f(r, d, o, sum) for two columns of each row, as the warps' results have them; the top and sum of each row
+  auto meet = [&](auto f, auto end_of_row) {
+    for (int r = w; r < rows; r += W) {
+      float top;
+      const float sum = sum_of(r, &top), inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+      for (int d = lane * 2; d < D; d += 64) {
+        float2 o = make_float2(0.0f, 0.0f);
+        for (int x = 0; x < W; ++x) {
+          const float g = m_s[x][r] == -INFINITY ? 0.0f : pow2(m_s[x][r] - top) * inv;
+          const float2 v = *reinterpret_cast<const float2 *>(sm + (x * NR + r) * PITCH + d);
+          o.x = fmaf(v.x, g, o.x);
+          o.y = fmaf(v.y, g, o.y);
+        }
+        f(r, d, o, sum);
+      }
+      end_of_row(r, top, sum);
+    }
+  };
+  if (w == 0) nan_columns[lane] = 0;
+  if (threadIdx.x == 0) nan_rows = 0;
+  __syncthreads();
+  uint32_t bits = 0, keys = 0;
+#pragma unroll 4
+  for (uint32_t t = first; t < end; t += W) {
+    const long long at = place(t);
+    if (at < 0) continue;
+    float k8[8], v8[8];
+    load8(a.k, at, k8);
+    load8(a.v, at, v8);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      keys |= isnan(k8[k]);
+      bits |= (uint32_t)isnan(v8[k]) << k;
+    }
+  }
+  if (__any_sync(0xffffffffu, keys)) bits = 0xff;  // a score of NaN is the whole row
+  if (bits) atomicOr(nan_columns + lane, bits);
+  for (int r = w; r < rows; r += W) {
+    float q[8];
+    load_q8(a, me.b, head0 + r, col, col < D, q);
+    bool none = false;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) none |= isnan(q[k]);
+    if (__any_sync(0xffffffffu, none) && lane == 0) atomicOr(&nan_rows, 1u << r);
+  }
+  __syncthreads();
+  bool again = false;
+  auto doubtful = [&](float x, int r, int d) {
+    return unusual(x) && !(isnan(x) && ((nan_columns[d >> 3] >> (d & 7) | nan_rows >> r) & 1));
+  };
+  meet([&](int r, int d, float2 o, float) { again |= doubtful(o.x, r, d) | doubtful(o.y, r, d + 1); }, [](int, float, float) {});
+  if (!__syncthreads_or(again)) return;
   for (int r = 0; r < rows; ++r) {
     float q[8], x[8], m = -INFINITY, l = 0.0f;
     load_q8(a, me.b, head0 + r, col, col < D, q);
     for (uint32_t t = first; t < end; t += W) {
-      if (!load8(a.k, t, x)) continue;
+      const long long at = place(t);
+      if (at < 0) continue;
+      load8(a.k, at, x);
       const float y = score(q, x);
       if (y == -INFINITY) continue;
       if (y > m) {
-        l = m == -INFINITY ? 0.0f : l * pow2(m - y);
+        l = m == -INFINITY ? l : l * pow2(m - y);
         m = y;
       }
       l += pow2(y - m);
@@ -504,20 +583,20 @@ __device__ __noinline__ void plain_share(const PagedArgs &a, PagedShare me, int 
   __syncthreads();
   float my_l = 0.0f, my_base = -INFINITY;  // of row `lane`
   for (int r = 0; r < rows; ++r) {
-    float q[8], x[8], acc[8], top = -INFINITY, sum = 0.0f, l = 0.0f;
-    for (int i = 0; i < W; ++i) top = fmaxf(top, m_s[i][r]);
-    for (int i = 0; i < W; ++i) sum = fmaf(l_s[i][r], m_s[i][r] == -INFINITY ? 0.0f : pow2(m_s[i][r] - top), sum);
-    const float base = sum == 0.0f ? 0.0f : top + ceilf(log2f(sum));
+    float q[8], x[8], acc[8], l = 0.0f, top;
+    const float sum = sum_of(r, &top), base = sum == 0.0f ? 0.0f : top + ceilf(log2f(sum));
     load_q8(a, me.b, head0 + r, col, col < D, q);
 #pragma unroll
     for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
     for (uint32_t t = first; t < end; t += W) {
-      if (!load8(a.k, t, x)) continue;
+      const long long at = place(t);
+      if (at < 0) continue;
+      load8(a.k, at, x);
       const float y = score(q, x), p = pow2(y - base);
-      load8(a.v, t, x);
+      load8(a.v, at, x);
       l += p;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) acc[k] = fmaf(p, x[k], acc[k]);
+      for (int k = 0; k < 8; ++k) acc[k] = isinf(x[k]) && y > -INFINITY ? acc[k] + x[k] : fmaf(p, x[k], acc[k]);
     }
     if (col < D) {
 #pragma unroll
@@ -533,6 +612,41 @@ __device__ __noinline__ void plain_share(const PagedArgs &a, PagedShare me, int 
     m_s[w][lane] = my_base;
     l_s[w][lane] = my_l;
   }
+  __syncthreads();
+  meet([&](int r, int d, float2 o, float sum) { keep_out(a, me, NR, r, head0 + r, d, o, sum); },
+       [&](int r, float top, float sum) {
+         if (me.parts > 1 && lane == 0) a.part_ml[(size_t)me.slot * NR + r] = make_float2(top, sum);
+       });
+}
+
+// The join of an item's shares for the thread's columns again, where infinite outputs of
+// shares whose weights are nothing beside another's made NaN: as in plain_share(),
+// infinities count whole.
+template <int NR>
+__device__ __noinline__ void plain_join(const PagedArgs &a, PagedShare me, int rows, int head0) {
+  const int D = a.head_dim, slot0 = me.slot - me.part;
+  for (int i = threadIdx.x; i < rows * D / 4; i += blockDim.x) {
+    const int row = i / (D / 4), col = (i - row * (D / 4)) * 4;
+    const float2 *ml = a.part_ml + (size_t)slot0 * NR + row;
+    const float *part = a.part + ((size_t)slot0 * NR + row) * D + col;
+    float top = -INFINITY, sum = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, gate[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int x = 0; x < me.parts; ++x) top = fmaxf(top, __ldcg(ml + (size_t)x * NR).x);
+    auto weight = [&](float2 y) { return y.y * (y.x == -INFINITY ? 0.0f : pow2(y.x - top)); };
+    for (int x = 0; x < me.parts; ++x) sum += weight(__ldcg(ml + (size_t)x * NR));
+    for (int x = 0; x < me.parts; ++x) {
+      const float2 y = __ldcg(ml + (size_t)x * NR);
+      const float4 v = __ldcg(reinterpret_cast<const float4 *>(part + (size_t)x * NR * D));
+      const float u[4] = {v.x, v.y, v.z, v.w}, f = weight(y) / sum;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] = isinf(u[k]) && y.y > 0.0f ? o[k] + u[k] : fmaf(u[k], f, o[k]);
+    }
+    if (a.gate) {
+      const float *g = a.gate + (size_t)me.b * a.gate_pitch + (size_t)(head0 + row) * a.gate_head + col;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) gate[k] = g[k];
+    }
+    store_out<4>(a, me.b, head0 + row, col, o, sum, gate);
+  }
 }
 
 template <typename T, int DP, int NR, bool ONCE>
@@ -546,6 +660,7 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
   float *const sm = reinterpret_cast<float *>(ring);          // at the end: the warps' results
   __shared__ uint64_t full[W][kParts];
   __shared__ int abort_s;
+  __shared__ PagedShare me_s;
   __shared__ float m_s[W][NR], l_s[W][NR];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, D = a.head_dim;
   if (lane == 0) {
@@ -649,7 +764,8 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
   // The queries, eight columns a lane and a row a warp, are asked for ahead of the
   // first copies (behind them, which take the memory a few microseconds, they came
   // 3 us later); the gates come to L2 meanwhile.
-  const int head0 = me.kvh * a.group + me.tile * NR, rows = min(NR, a.group - me.tile * NR);
+  int head0 = me.kvh * a.group + me.tile * NR, rows = min(NR, a.group - me.tile * NR);
+  if (tid == 0) me_s = me;
   constexpr int kMine = (NR + W - 1) / W;
   float x[kMine][8];
 #pragma unroll
@@ -1003,46 +1119,39 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
         mine_f[(2 * c + (e & 1)) * Sh::kEndPitch + 32 * (k >> 1) + 4 * g + 2 * (k & 1) + (e >> 1)] = acc[k][e];
   }
   __syncthreads();
+  // (what only the end needs of it takes no registers meanwhile: 3 x 100003 tokens 112 us, so 103)
+  me = me_s;
+  head0 = me.kvh * a.group + me.tile * NR;
+  rows = min(NR, a.group - me.tile * NR);
   // The warps' results meet: maxima, then sums over one maximum in warp order; weights
   // over their sum, so that no sum passes the values it is of.
-  for (bool plain = false;; plain = true) {
-    bool again = false;
-    for (int r = w; r < rows; r += W) {
-      float top = -INFINITY, f[W], sum = 0.0f;
+  bool again = false;
+  for (int r = w; r < rows; r += W) {
+    float top = -INFINITY, f[W], sum = 0.0f;
 #pragma unroll
-      for (int x = 0; x < W; ++x) top = fmaxf(top, m_s[x][r]);
+    for (int x = 0; x < W; ++x) top = fmaxf(top, m_s[x][r]);
+#pragma unroll
+    for (int x = 0; x < W; ++x) {
+      f[x] = m_s[x][r] == -INFINITY ? 0.0f : pow2(m_s[x][r] - top);
+      sum = fmaf(l_s[x][r], f[x], sum);
+    }
+    const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+    for (int x = 0; x < W; ++x) f[x] *= inv;
+    for (int d = lane * 2; d < D; d += 64) {
+      float2 o = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int x = 0; x < W; ++x) {
-        f[x] = m_s[x][r] == -INFINITY ? 0.0f : pow2(m_s[x][r] - top);
-        sum = fmaf(l_s[x][r], f[x], sum);
+        const float2 v = *reinterpret_cast<const float2 *>(sm + ((size_t)x * NR + r) * Sh::kEndPitch + d);
+        o.x = fmaf(v.x, f[x], o.x);
+        o.y = fmaf(v.y, f[x], o.y);
       }
-      const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-#pragma unroll
-      for (int x = 0; x < W; ++x) f[x] *= inv;
-      const size_t to = (size_t)me.slot * NR + r;
-      for (int d = lane * 2; d < D; d += 64) {
-        float2 o = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int x = 0; x < W; ++x) {
-          const float2 v = *reinterpret_cast<const float2 *>(sm + ((size_t)x * NR + r) * Sh::kEndPitch + d);
-          o.x = fmaf(v.x, f[x], o.x);
-          o.y = fmaf(v.y, f[x], o.y);
-        }
-        again |= unusual(o.x) | unusual(o.y);
-        if (me.parts > 1) {
-          *reinterpret_cast<float2 *>(a.part + to * D + d) = o;
-        } else {
-          const float *g = a.gate ? a.gate + (size_t)me.b * a.gate_pitch + (size_t)(head0 + r) * a.gate_head + d : nullptr;
-          const float x[2] = {o.x, o.y}, gate[2] = {g ? g[0] : 0.0f, g ? g[1] : 0.0f};
-          store_out<2>(a, me.b, head0 + r, d, x, sum, gate);
-        }
-      }
-      if (me.parts > 1 && lane == 0) a.part_ml[to] = make_float2(top, sum);
+      again |= unusual(o.x) | unusual(o.y);
+      keep_out(a, me, NR, r, head0 + r, d, o, sum);
     }
-    if (!__syncthreads_or(again) || plain) break;
-    plain_share<T, W, NR, Sh::kEndPitch>(a, me, rows, head0, sm, m_s, l_s);
-    __syncthreads();
+    if (me.parts > 1 && lane == 0) a.part_ml[(size_t)me.slot * NR + r] = make_float2(top, sum);
   }
+  if (__syncthreads_or(again)) plain_share<T, W, NR, Sh::kEndPitch>(a, me, rows, head0, sm, m_s, l_s);
   if (me.parts == 1) return;
   // The shares of an item meet in the block that finds all of them there: each says
   // so by its flag and then looks at the others', so that the last one does find
@@ -1130,12 +1239,15 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
       }
     }
   }
+  bool odd = false;
 #pragma unroll
   for (int j = 0; j < kItems; ++j) {
     if (row[j] >= rows) continue;
+    odd |= isnan(o[j].x + o[j].y + o[j].z + o[j].w);
     const float x[4] = {o[j].x, o[j].y, o[j].z, o[j].w}, g[4] = {gate[j].x, gate[j].y, gate[j].z, gate[j].w};
     store_out<4>(a, me.b, head0 + row[j], col[j], x, sum[j], g);
   }
+  if (odd) plain_join<NR>(a, me, rows, head0);
   for (int i = tid; i < me.parts; i += Sh::kThreads) a.flags[slot0 + i] = 0;
 }
 

@@ -889,6 +889,8 @@ int fpb_paged_append(const void *q, size_t q_pitch, size_t q_head_pitch, const v
  * behind its last token never reach an output, whatever they hold; a token whose
  * page is outside the pool counts as not there.  Sums are f32; over bf16 pages q and
  * the weights are taken to 16 bits, over f32 pages products to 2^-20 of themselves.
+ * Infinities are as the formula has them: a score of -inf is a weight of 0 (nothing
+ * else: zeros), one of +inf NaN, an infinite value its column.
  * The workspace needs no clearing; calls that may run at the same time must not share
  * one.  batch at most 4096. */
 size_t fpb_paged_attn_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads, size_t head_dim);

@@ -1,8 +1,13 @@
-"""Attention over the paged cache where numbers leave the usual range: values from the
-smallest normal number to the largest, against the formula in 64 bits.
+"""Attention over the paged cache where numbers leave the usual range: infinite keys,
+values and queries, values from the smallest normal number to the largest, against the
+formula in 64 bits.
 
-The bars are test_gpu_paged.py's, and n * 2^-148 for sums and products below the normal
-range (each is off by 2^-149 at most).
+NaN stays where it is seen.  What the formula gives for infinities: a score of -inf a
+weight of 0 (with no other, zeros, as without tokens), one of +inf NaN in the whole
+head, an infinite value its column (NaN where both signs meet), however small its
+token's weight.  Finite numbers have test_gpu_paged.py's bars, taken over the finite
+terms, and n * 2^-148 for sums and products below the normal range (each is off by
+2^-149 at most).
 """
 import math
 
@@ -13,14 +18,41 @@ from test_gpu_paged import F, _attention_case, _dev, _host, _no_device_error, to
 
 pytestmark = pytest.mark.gpu
 
-KINDS = ("plain", "columns", "small", "large")
+KINDS = ("key -inf", "key +inf", "value", "query", "hopeless", "nan", "masked", "plain", "columns", "small", "large")
 
 
 def _special(torch, kind, rng, i, n, q, k, v, scale):
     """What is out of the ordinary in session i; k, v [n, heads, d] and q [heads, d] are
     f32 copies on the host, in place."""
     d = q.shape[1]
-    if kind == "columns":
+    if kind == "key -inf":
+        q[:, 3], q[:, d - 1] = np.abs(q[:, 3]) + 0.125, -np.abs(q[:, d - 1]) - 0.37
+        for t in {0, n // 2, n - 1}:
+            if n > 1 and t != 1:
+                k[t, :, 3] = -math.inf
+        if n > 6:
+            k[5, :, d - 1] = math.inf
+    elif kind == "key +inf":
+        q[:, 2] = np.abs(q[:, 2]) + 0.125
+        k[n // 3, 0, 2] = math.inf
+    elif kind == "value":
+        v[n // 2, 0, 5], v[0, 0, 7], v[n - 1, 0, 7] = math.inf, -math.inf, -math.inf
+        v[n // 2, 0, 9] = math.inf
+        v[(n // 2 + 1) % n, 0, 9] = -math.inf if n > 1 else math.inf
+    elif kind == "query":
+        q[1, 4] = math.inf
+        k[n // 2, :, 4] = np.abs(k[n // 2, :, 4]) + 0.1
+    elif kind == "hopeless":
+        q[:, 6] = 8.0
+        k[:, :, 6] = 0.0
+        k[n // 2, :, 6] = -200.0 / (8.0 * scale) if n > 1 else 0.0
+        v[n // 2, :, 1] = -math.inf
+    elif kind == "nan":
+        v[0, 0, 5], v[n // 2, 0, 6], q[1, 2] = math.nan, math.inf, math.nan
+    elif kind == "masked":
+        q[:, 1] = np.abs(q[:, 1]) + 0.125
+        k[:, :, 1] = -math.inf
+    elif kind == "columns":
         v *= 2.0 ** np.linspace(-120, 120, d).round().astype(np.float32)
     elif kind == "small":
         v *= np.float32(2.0 ** -118)
@@ -73,6 +105,9 @@ def test_paged_attention_values_out_of_the_ordinary(F, torch, n, hq, hk, d, p, t
     two = 2.0 ** -16 if pages == "bf16" else 0.0
     for i, (qi, ki, vi) in enumerate(host):
         kind = KINDS[i % len(KINDS)]
+        if kind == "masked":
+            assert not got[i].any()
+            continue
         for h in range(hq):
             want, pv, most = _want(qi[h], ki[:, h // (hq // hk)], vi[:, h // (hq // hk)], scale)
             where = (kind, i, h)
@@ -87,4 +122,8 @@ def test_paged_attention_values_out_of_the_ordinary(F, torch, n, hq, hk, d, p, t
                 assert (got[i, h][inf] == want[inf]).all(), where
                 off = np.abs(got[i, h] - want)[fine] / bar[fine]
                 assert (off <= 1).all(), (*where, float(np.nanmax(off)))
-        assert np.isfinite(got[i]).all() and (kind != "small" or (got[i] != 0).all())
+        if kind == "key +inf":
+            assert np.isnan(got[i, :hq // hk]).all()
+        elif kind in ("key -inf", "plain", "columns", "small", "large"):
+            if kind != "key -inf" or lengths[i] > 3:
+                assert np.isfinite(got[i]).all() and (kind != "small" or (got[i] != 0).all())
