@@ -28,6 +28,7 @@ namespace {
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxSlice = 49152;  // logits of a CTA in shared memory, f32: 192 KB
 constexpr int kMaxVocab = 8 * kMaxSlice;
+constexpr size_t kPairSlice = 100 * 1024;  // bytes of a slice of which two fit an SM
 constexpr int kBatch = 5;         // 16-byte loads a thread has under way (f32 logits: twice as many)
 constexpr int kBins = 256;        // bins of a histogram
 constexpr int kList = kThreads;   // tokens that one CTA orders
@@ -867,7 +868,7 @@ int run_sample(const SampleArgs &a, size_t batch, cudaStream_t s) {
     std::lock_guard<std::mutex> lock(mu);
     if (std::find(done.begin(), done.end(), dev) == done.end()) {
       FPB_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        (int)(kMaxSlice * sizeof(T))));
+                                        (int)std::max(kMaxSlice * sizeof(T), kPairSlice)));
       done.push_back(dev);
     }
   }
@@ -918,7 +919,7 @@ extern "C" int fpb_sample(const void *logits, int logits_dtype, size_t logits_pi
   auto slice = [&](size_t c) { return ((vocab + c - 1) / c + 7) / 8 * 8; };
   const int C = batch * 8 > 5 * sms && slice(2) <= 16384 ? 2
                 : batch * 16 > 5 * sms && slice(4) <= 16384 ? 4
-                : batch * 8 > 5 * sms && slice(4) * el <= 100 * 1024 ? 4
+                : batch * 8 > 5 * sms && slice(4) * el <= kPairSlice ? 4
                     : 8;
   a.slice = (int)slice(C);
   auto lies = [](const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && bytes % 16 == 0; };

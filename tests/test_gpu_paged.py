@@ -586,6 +586,18 @@ def test_sample_matches_the_definition(F, torch, b, vocab, dtype):
     _check_sample(torch, tokens.cpu(), logprobs.cpu(), *args)
 
 
+@pytest.mark.parametrize("b,vocab,dtype", [
+    (93, 196608, "bf16"), (93, 196609, "bf16"), (93, 202048, "bf16"), (100, 204800, "bf16"), (93, 204801, "bf16"),
+    (92, 204800, "bf16"), (93, 102400, "f32"), (93, 102401, "f32"), (93, 393216, "bf16"), (93, 393216, "f32"),
+    (93, 32768, "f32"), (93, 32769, "bf16"), (47, 65536, "bf16"), (47, 65537, "f32")])
+def test_sample_at_the_limits_of_its_ways(F, torch, b, vocab, dtype):
+    """Rows and vocabularies on both sides of where a row takes two, four and eight CTAs."""
+    args = _sample_inputs(torch, b, vocab, dtype, b + vocab)
+    tokens, logprobs = _run_sample(F, torch, *args)
+    rows = [0, 1, b // 2, b - 1]
+    _check_sample(torch, tokens[rows].cpu(), logprobs[rows].cpu(), *(x[rows] for x in args))
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_sample_equal_logits_go_by_index(F, torch, dtype):
     """Ties at the border of each filter: rows of one value, of a few values, and
