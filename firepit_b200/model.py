@@ -788,6 +788,13 @@ class PagedDecoder(Decoder):
             rs.zero_()
         self.reserved = [0] * self.sessions
 
+    def prefill(self, prompt) -> None:
+        """Prompts are requests': a step takes a token of each that is under way."""
+        raise NotImplementedError("PagedDecoder takes requests: admit() and step(), or serve()")
+
+    def generate(self, steps: int) -> None:
+        raise NotImplementedError("PagedDecoder takes requests: admit() and step(), or serve()")
+
     def pages_for(self, request: Request) -> int:
         """Pages that the request may come to (its last token is not run)."""
         return -(-(len(request.prompt) + request.new_tokens - 1) // self.page_size)

@@ -213,3 +213,20 @@ def test_paged_decoder_refuses_what_does_not_fit(torch, model):
     for bad in ((0, 16, 5, 4), (2, 0, 5, 4), (2, 16, 0, 4), (2, 16, 5, 0)):
         with pytest.raises(F.ShapeError):
             PagedDecoder(model, *bad)
+
+
+def test_paged_decoder_takes_no_batch(torch, model):
+    """The other decoders' prefill and generate would run steps beside the requests:
+    they say what to call instead, and leave the sessions as they were."""
+    from firepit_b200.model import PagedDecoder, Request
+    dec = PagedDecoder(model, 2, 16, 8, 4)
+    dec.step(torch.cuda.current_stream().cuda_stream)
+    dec.capture()
+    dec.reset()
+    assert dec.admit(0, Request([3, 1, 4], 4))
+    before = [t.clone() for t in (dec.tokens, dec.tables.lengths, dec.active, dec.prompt)]
+    for call in (lambda: dec.prefill(torch.ones(2, 3, dtype=torch.int32, device="cuda")), lambda: dec.generate(3)):
+        with pytest.raises(NotImplementedError, match="serve"):
+            call()
+    for t, w in zip((dec.tokens, dec.tables.lengths, dec.active, dec.prompt), before):
+        assert torch.equal(t, w)
