@@ -697,7 +697,8 @@ class PagedDecoder(Decoder):
     drawn one, in ``emitted`` (-1 elsewhere).  Nothing of it looks from the host,
     so ``capture()`` records it.  ``admit`` and ``release`` go between steps;
     ``serve`` does it all.  Admission counts the pages that a request may come to,
-    so that no step finds the pool empty."""
+    and a session that has its tokens takes no further one, released or not, so that
+    no step finds the pool empty."""
 
     def __init__(self, model: HybridModel, sessions: int, max_seq: int, pages: int, page_size: int = 16, dtype=None):
         import torch
@@ -718,6 +719,7 @@ class PagedDecoder(Decoder):
         self.active = torch.zeros(sessions, **i32)
         self.prompt = torch.zeros(sessions, self.max_seq, **i32)
         self.prompt_len = torch.zeros(sessions, **i32)
+        self.last = torch.zeros(sessions, **i32)  # tokens that the request runs: its last one is not
         self.temperature, self.min_p = torch.zeros(sessions, **f32), torch.zeros(sessions, **f32)
         self.top_p, self.top_k = torch.ones(sessions, **f32), torch.zeros(sessions, **i32)
         self.noise = torch.ones(sessions, c.vocab, **f32)
@@ -761,6 +763,7 @@ class PagedDecoder(Decoder):
             prompt = torch.gather(self.prompt, 1, after.clamp(0, self.max_seq - 1).long()[:, None])[:, 0]
             self.emitted.copy_(torch.where(taken & ~known, self.drawn, -1))
             self.tokens.copy_(torch.where(taken, torch.where(known, prompt, self.drawn), self.tokens))
+            self.active.mul_(after < self.last)  # (a row without a token this step: 0 < last)
 
     def step(self, sh: int) -> None:
         t, m = self.tables, self.map
@@ -779,7 +782,7 @@ class PagedDecoder(Decoder):
         new = PageTables.empty(self.batch, self.pages, self.page_size, t.table.shape[1], device=self.model.device)
         for old, x in ((t.table, new.table), (t.lengths, new.lengths), (t.free, new.free), (t.free_count, new.free_count)):
             old.copy_(x)
-        for x in (self.tokens, self.active, self.prompt_len):
+        for x in (self.tokens, self.active, self.prompt_len, self.last):
             x.zero_()
         for x in (self.map.slots, self.map.positions, self.map.requests, self.emitted):
             x.fill_(-1)
@@ -823,6 +826,7 @@ class PagedDecoder(Decoder):
         n = len(request.prompt)
         self.prompt[session, :n].copy_(torch.tensor(request.prompt, dtype=torch.int32))
         self.prompt_len[session] = n
+        self.last[session] = n + request.new_tokens - 1
         self.tokens[session] = request.prompt[0]
         self.temperature[session], self.top_k[session] = request.temperature, request.top_k
         self.top_p[session], self.min_p[session] = request.top_p, request.min_p

@@ -230,3 +230,28 @@ def test_paged_decoder_takes_no_batch(torch, model):
             call()
     for t, w in zip((dec.tokens, dec.tables.lengths, dec.active, dec.prompt), before):
         assert torch.equal(t, w)
+
+
+def test_paged_decoder_sessions_end_by_themselves(torch, model):
+    """A session that has its tokens takes no further page, released or not: what was
+    counted for the others stays theirs."""
+    from firepit_b200.model import PagedDecoder, Request
+    a, b = Request([1, 2, 3], 2), Request([9, 8, 7, 6, 5], 16)  # four tokens run, and twenty: one page and five
+    runs = []
+    for late in (False, True):
+        dec = PagedDecoder(model, 2, 32, 6, 4, torch.float32)
+        assert dec.admit(0, a) and dec.admit(1, b)
+        out = [[], []]
+        for step in range(22):
+            dec.step(torch.cuda.current_stream().cuda_stream)
+            for o, t in zip(out, dec.emitted.tolist()):
+                o.append(t)
+            assert dec.tables.lengths.tolist()[0] <= 4 and dec.tables.lengths.tolist()[1] == min(step + 1, 20)
+            if step == 3 and not late:
+                dec.release(0)
+        runs.append(out)
+        assert [t >= 0 for t in out[0]] == [2 <= step < 4 for step in range(22)]
+        assert [t >= 0 for t in out[1]] == [4 <= step < 20 for step in range(22)]
+        dec.release(0, 1)
+        assert int(dec.tables.free_count) == 6 and dec.admit(0, b) and dec.reserved == [5, 0]
+    assert runs[0] == runs[1]
