@@ -26,6 +26,7 @@ sessions (no exchange).
 from __future__ import annotations
 
 import math
+import operator
 from dataclasses import dataclass
 
 from . import _native as N
@@ -809,6 +810,20 @@ class PagedDecoder(Decoder):
             raise ShapeError(f"request: a prompt of {n} tokens and {k} new ones in sessions of up to {self.max_seq}")
         if not all(0 <= t < self.cfg.vocab for t in request.prompt):
             raise ShapeError(f"request: tokens outside the vocabulary ({self.cfg.vocab})")
+        self._filters(request)
+
+    @staticmethod
+    def _filters(request: Request):
+        """(temperature, top_k, top_p, min_p) as the device holds them."""
+        from .gemv import ShapeError
+        try:
+            real = [float(x) for x in (request.temperature, request.top_p, request.min_p)]
+            top_k = operator.index(request.top_k)
+        except (TypeError, ValueError) as e:
+            raise ShapeError(f"request: filters {e}") from None
+        if any(math.isnan(x) for x in real) or not -2 ** 31 <= top_k < 2 ** 31:
+            raise ShapeError(f"request: temperature, top_p, min_p {real}, top_k {top_k}")
+        return real[0], top_k, real[1], real[2]
 
     def admit(self, session: int, request: Request) -> bool:
         """Begins a request on a free row; False if the pool could run out of pages
@@ -828,8 +843,8 @@ class PagedDecoder(Decoder):
         self.prompt_len[session] = n
         self.last[session] = n + request.new_tokens - 1
         self.tokens[session] = request.prompt[0]
-        self.temperature[session], self.top_k[session] = request.temperature, request.top_k
-        self.top_p[session], self.min_p[session] = request.top_p, request.min_p
+        for x, value in zip((self.temperature, self.top_k, self.top_p, self.min_p), self._filters(request)):
+            x[session] = value
         for cs, rs in self.gdn.values():
             cs[session].zero_()
             rs[session].zero_()

@@ -255,3 +255,17 @@ def test_paged_decoder_sessions_end_by_themselves(torch, model):
         dec.release(0, 1)
         assert int(dec.tables.free_count) == 6 and dec.admit(0, b) and dec.reserved == [5, 0]
     assert runs[0] == runs[1]
+
+
+def test_paged_decoder_a_refused_request_leaves_the_row_free(torch, model):
+    import firepit_b200 as F
+    from firepit_b200.model import PagedDecoder, Request
+    dec = PagedDecoder(model, 2, 16, 8, 4)
+    for bad in (dict(temperature=None), dict(top_k=2 ** 40), dict(top_k=0.5), dict(top_p="x"), dict(min_p=float("nan")),
+                dict(temperature=float("nan"))):
+        with pytest.raises(F.ShapeError):
+            dec.admit(0, Request([1, 2], 3, **bad))
+        with pytest.raises(F.ShapeError):
+            dec.serve([Request([1, 2], 3), Request([1, 2], 3, **bad)])
+        assert dec.reserved == [0, 0] and not dec.active.any()
+    assert dec.admit(0, Request([1, 2], 3, temperature=1, top_k=2 ** 31 - 1, top_p=0, min_p=2))
