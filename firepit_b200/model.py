@@ -817,7 +817,7 @@ class PagedDecoder(Decoder):
         """(temperature, top_k, top_p, min_p) as the device holds them."""
         from .gemv import ShapeError
         try:
-            real = [float(x) for x in (request.temperature, request.top_p, request.min_p)]
+            real = [min(max(float(x), -1e30), 1e30) for x in (request.temperature, request.top_p, request.min_p)]
             top_k = operator.index(request.top_k)
         except (TypeError, ValueError) as e:
             raise ShapeError(f"request: filters {e}") from None
@@ -837,7 +837,6 @@ class PagedDecoder(Decoder):
         need = self.pages_for(request)
         if sum(self.reserved) + need > self.pages:
             return False
-        self.reserved[session] = need
         n = len(request.prompt)
         self.prompt[session, :n].copy_(torch.tensor(request.prompt, dtype=torch.int32))
         self.prompt_len[session] = n
@@ -849,6 +848,7 @@ class PagedDecoder(Decoder):
             cs[session].zero_()
             rs[session].zero_()
         self.active[session] = 1
+        self.reserved[session] = need
         return True
 
     def release(self, *sessions: int) -> None:

@@ -269,3 +269,4 @@ def test_paged_decoder_a_refused_request_leaves_the_row_free(torch, model):
             dec.serve([Request([1, 2], 3), Request([1, 2], 3, **bad)])
         assert dec.reserved == [0, 0] and not dec.active.any()
     assert dec.admit(0, Request([1, 2], 3, temperature=1, top_k=2 ** 31 - 1, top_p=0, min_p=2))
+    assert dec.admit(1, Request([1, 2], 3, temperature=1e300, top_p=-1e300, min_p=float("inf")))  # (no f32 numbers)
