@@ -352,6 +352,9 @@ extern "C" int fpb_page_truncate(int32_t *table, size_t table_pitch, size_t batc
   PageArgs a = page_args(table, table_pitch, batch, max_pages, lengths, new_lengths, free_pages, free_count, pages,
                          page_size);
   if (int st = check_tables("fpb_page_truncate", a, table_pitch, batch, max_pages, pages, page_size)) return st;
+  // (read again where lengths are written; the lengths themselves change nothing)
+  if (new_lengths != lengths && new_lengths < lengths + batch && lengths < new_lengths + batch)
+    return fail(FPB_ERR_INVALID_ARGUMENT, "fpb_page_truncate: new_lengths overlap the lengths");
   a.error = device_error_ptr();
   return launch_pages({page_truncate_kernel<kPageAll>, page_truncate_kernel<kPageRows>, page_truncate_kernel<kPageState>},
                       "page_truncate_kernel", a, std::min(batch * max_pages, pages), 65536,

@@ -868,7 +868,8 @@ int fpb_page_extend(int32_t *table, size_t table_pitch, size_t batch, size_t max
                     void *stream);
 /* Cuts requests to new_lengths[b] tokens (negative, or not below the present
  * length: as it was; 0: done) and gives the pages back, so that what fpb_page_extend
- * took and this gives back leaves the stack as it was.  Entries given back become -1. */
+ * took and this gives back leaves the stack as it was.  Entries given back become -1.
+ * new_lengths may be the lengths, but not overlap them otherwise. */
 int fpb_page_truncate(int32_t *table, size_t table_pitch, size_t batch, size_t max_pages, int32_t *lengths,
                       const int32_t *new_lengths, int32_t *free_pages, int32_t *free_count, size_t pages,
                       size_t page_size, void *stream);

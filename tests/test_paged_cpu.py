@@ -39,6 +39,14 @@ def test_page_entry_points_check_arguments():
     assert cut(batch=0) == shape and cut(pages=0) == shape
 
 
+def test_page_truncate_takes_no_lengths_among_the_lengths():
+    """New lengths that are read again behind the writes of others' lengths."""
+    def cut(lengths, to):
+        return N.lib.fpb_page_truncate(i, 4, 2, 4, lengths, to, i, i, 8, 16, None)
+
+    assert cut(i, i + 4) == bad and cut(i + 4, i) == bad
+
+
 def test_paged_append_checks_arguments():
     def append(q=f, q_pitch=64, q_head=32, k=f, k_pitch=64, v=f, v_pitch=64, dtype=0, qg=f, kg=f, slots=i, pos=i, rows=2,
                hq=2, hk=2, d=32, rot=32, theta=1e4, eps=1e-6, q_out=f, q_out_dtype=0, kp=f, vp=f, page_dtype=1, pages=4,
