@@ -17,6 +17,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -86,24 +87,31 @@ def build(verbose: bool = False, force: bool = False) -> Path:
 
 
 def _build_calls(force: bool) -> None:
-    """The module links torch and the library above (found beside it)."""
+    """The module links torch and the library above (found beside it).  It saves a call
+    some microseconds and nothing else needs it, so what keeps it from being built is
+    noted and an older one removed (the calls go by ctypes)."""
     spec = importlib.util.find_spec("torch")
-    src = CSRC / "calls.cpp"
-    newest = max(p.stat().st_mtime for p in (src, INCLUDE / "firepit_b200.h"))
-    if spec is None or not (force or not CALLS.exists() or newest > CALLS.stat().st_mtime):
+    if spec is None or spec.origin is None:
         return
-    torch = Path(spec.origin).parent
-    cuda = Path(nvcc()).resolve().parent.parent
+    src, torch = CSRC / "calls.cpp", Path(spec.origin).parent
     tmp = CALLS.with_suffix(".so.tmp")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           *(f"-I{p}" for p in (INCLUDE, torch / "include", torch / "include/torch/csrc/api/include",
-                                sysconfig.get_paths()["include"], cuda / "include")),
-           str(src), "-o", str(tmp), f"-L{PKG}", f"-l:{LIB.name}", f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch",
-           "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"g++ failed for {src.name}:\n{r.stdout}\n{r.stderr}")
-    os.replace(tmp, CALLS)
+    try:
+        newest = max(p.stat().st_mtime for p in (src, INCLUDE / "firepit_b200.h"))
+        if not force and CALLS.exists() and newest <= CALLS.stat().st_mtime:
+            return
+        cuda = Path(nvcc()).resolve().parent.parent
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+               *(f"-I{p}" for p in (INCLUDE, torch / "include", torch / "include/torch/csrc/api/include",
+                                    sysconfig.get_paths()["include"], cuda / "include")),
+               str(src), "-o", str(tmp), f"-L{PKG}", f"-l:{LIB.name}", f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch",
+               "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"g++ failed for {src.name}:\n{r.stdout}\n{r.stderr}")
+        os.replace(tmp, CALLS)
+    except (OSError, RuntimeError) as e:
+        CALLS.unlink(missing_ok=True)
+        warnings.warn(f"{CALLS.name} was not built, the paged cache's calls go by ctypes: {e}", stacklevel=2)
 
 
 if __name__ == "__main__":
