@@ -13,6 +13,7 @@ from __future__ import annotations
 import concurrent.futures as cf
 import importlib.util
 import os
+import runpy
 import shutil
 import subprocess
 import sys
@@ -87,20 +88,23 @@ def build(verbose: bool = False, force: bool = False) -> Path:
 
 
 def _build_calls(force: bool) -> None:
-    """The module links torch and the library above (found beside it).  It saves a call
-    some microseconds and nothing else needs it, so what keeps it from being built is
-    noted and an older one removed (the calls go by ctypes)."""
+    """The module links torch and the library above (found beside it), for the torch
+    and the Python that are here: it is made again for others.  It saves a call some
+    microseconds and nothing else needs it, so what keeps it from being built is noted
+    and an older one removed (the calls go by ctypes)."""
     spec = importlib.util.find_spec("torch")
     if spec is None or spec.origin is None:
         return
-    src, torch = CSRC / "calls.cpp", Path(spec.origin).parent
+    src, torch, stamp = CSRC / "calls.cpp", Path(spec.origin).parent, BUILD / "calls.for"
     tmp = CALLS.with_suffix(".so.tmp")
     try:
+        made_for = f"{runpy.run_path(str(torch / 'version.py'))['__version__']} {sys.implementation.cache_tag}"
         newest = max(p.stat().st_mtime for p in (src, INCLUDE / "firepit_b200.h"))
-        if not force and CALLS.exists() and newest <= CALLS.stat().st_mtime:
+        if not force and CALLS.exists() and newest <= CALLS.stat().st_mtime and stamp.exists() and (
+                stamp.read_text() == made_for):
             return
         cuda = Path(nvcc()).resolve().parent.parent
-        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f'-DFPB_CALLS_FOR="{made_for}"',
                *(f"-I{p}" for p in (INCLUDE, torch / "include", torch / "include/torch/csrc/api/include",
                                     sysconfig.get_paths()["include"], cuda / "include")),
                str(src), "-o", str(tmp), f"-L{PKG}", f"-l:{LIB.name}", f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch",
@@ -109,7 +113,8 @@ def _build_calls(force: bool) -> None:
         if r.returncode != 0:
             raise RuntimeError(f"g++ failed for {src.name}:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, CALLS)
-    except (OSError, RuntimeError) as e:
+        stamp.write_text(made_for)
+    except (OSError, RuntimeError, KeyError) as e:
         CALLS.unlink(missing_ok=True)
         warnings.warn(f"{CALLS.name} was not built, the paged cache's calls go by ctypes: {e}", stacklevel=2)
 

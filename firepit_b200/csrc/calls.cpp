@@ -375,4 +375,18 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nul
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__calls() { return PyModule_Create(&module); }
+// Torch's tensors are read by the layout that this was compiled for: "<torch's version>
+// <Python's cache tag>", or the import fails.
+PyMODINIT_FUNC PyInit__calls() {
+  PyObject *torch = PyImport_ImportModule("torch"), *sys = PyImport_ImportModule("sys");
+  PyObject *version = torch ? PyObject_GetAttrString(torch, "__version__") : nullptr;
+  PyObject *python = sys ? PyObject_GetAttrString(sys, "implementation") : nullptr;
+  PyObject *tag = python ? PyObject_GetAttrString(python, "cache_tag") : nullptr;
+  PyObject *here = version && tag ? PyUnicode_FromFormat("%S %S", version, tag) : nullptr, *made = nullptr;
+  if (here && PyUnicode_CompareWithASCIIString(here, FPB_CALLS_FOR) == 0)
+    made = PyModule_Create(&module);
+  else if (here)
+    PyErr_Format(PyExc_ImportError, "_calls is built for \"%s\", this is \"%U\"", FPB_CALLS_FOR, here);
+  for (PyObject *o : {torch, sys, version, python, tag, here}) Py_XDECREF(o);
+  return made;
+}

@@ -17,6 +17,7 @@ one); the outputs it allocates belong to it.
 from __future__ import annotations
 
 import math
+import warnings
 from dataclasses import dataclass
 
 from . import _native as N
@@ -36,8 +37,10 @@ class _Torch:
         import torch
         try:
             from . import _calls as calls
-        except ImportError:  # (not built: the same calls through ctypes, a few microseconds longer)
+        except ImportError as e:  # (not built: the same calls through ctypes, a few microseconds longer)
             calls = None
+            if (N.LIB_PATH.parent / "_calls.so").exists():
+                warnings.warn(f"_calls.so is not used, the paged cache's calls go by ctypes: {e}", stacklevel=2)
         cls.calls = calls
         cls.f32, cls.bf16, cls.i32, cls.u8 = torch.float32, torch.bfloat16, torch.int32, torch.uint8
         cls.codes = {torch.float32: N.FPB_F32, torch.bfloat16: N.FPB_BF16}
