@@ -180,7 +180,8 @@ PyObject *page_extend(PyObject *, PyObject *const *a, Py_ssize_t count) {
   Tables t(a);
   const Tensor *counts, *out[4];
   int64_t rows;
-  if (!t.of(a) || !ints(a[5], t.dev, t.table.batch, &counts) || !whole(a[6], &rows) || rows < 1 || !PyBool_Check(a[7]))
+  if (!t.of(a) || !ints(a[5], t.dev, t.table.batch, &counts) || !whole(a[6], &rows) || rows < 1 ||
+      rows > FPB_PAGE_MAX_ROWS || !PyBool_Check(a[7]))
     return leave();
   const bool padded = a[7] == Py_True, fresh = a[8] == Py_None;
   const int64_t b = t.table.batch;

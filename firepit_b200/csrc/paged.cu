@@ -330,7 +330,7 @@ extern "C" int fpb_page_extend(int32_t *table, size_t table_pitch, size_t batch,
                          page_size);
   if (int st = check_tables("fpb_page_extend", a, table_pitch, batch, max_pages, pages, page_size)) return st;
   if (!slots || !positions) return fail(FPB_ERR_INVALID_ARGUMENT, "fpb_page_extend: null pointer");
-  if (rows == 0 || rows > 0x7ffffff0 || (padded && rows % batch))
+  if (rows == 0 || rows > FPB_PAGE_MAX_ROWS || (padded && rows % batch))
     return fail(FPB_ERR_SHAPE, "fpb_page_extend: %zu rows (padded: a multiple of the batch, %zu)", rows, batch);
   if (counts < lengths + batch && lengths < counts + batch)  // (a block reads counts behind another's lengths)
     return fail(FPB_ERR_INVALID_ARGUMENT, "fpb_page_extend: counts overlap the lengths");

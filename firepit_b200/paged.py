@@ -27,6 +27,9 @@ _extend, _truncate, _append = N.lib.fpb_page_extend, N.lib.fpb_page_truncate, N.
 _attn, _attn_bytes, _sample = N.lib.fpb_paged_attn, N.lib.fpb_paged_attn_workspace_bytes, N.lib.fpb_sample
 
 
+PAGE_MAX_ROWS = 0x7ffffff0  # of a page map
+
+
 def _keep(self, **values) -> None:
     """What the entry points take of an object, as they take it."""
     for name, value in values.items():
@@ -183,7 +186,7 @@ def page_extend(tables: PageTables, counts, rows: int, padded: bool = False, out
             return PageMap(*got) if out is None else out
     b, device = tables.batch, tables.device
     _ints(counts, "counts", b)
-    if rows < 1 or (padded and rows % b):
+    if not 1 <= rows <= PAGE_MAX_ROWS or (padded and rows % b):
         raise ShapeError(f"page_extend: {rows} rows of {b} requests")
     if device < 0 or device != counts.get_device() or device != _Torch.current_device():
         raise _elsewhere("page_extend", device, counts)

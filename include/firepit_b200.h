@@ -861,7 +861,8 @@ int fpb_tree_verify(const void *logits, int logits_dtype, size_t logits_pitch, c
  * has rows [b, b + 1) * rows / batch.  slots, positions, requests [rows]: the
  * token's slot, its position and its request, -1 in rows without one; starts [batch
  * + 1]: each request's first row.  requests and starts may be NULL.  counts must not
- * overlap lengths.  batch at most 16384. */
+ * overlap lengths.  batch at most 16384, rows FPB_PAGE_MAX_ROWS. */
+#define FPB_PAGE_MAX_ROWS 0x7ffffff0
 int fpb_page_extend(int32_t *table, size_t table_pitch, size_t batch, size_t max_pages, int32_t *lengths,
                     const int32_t *counts, int32_t *free_pages, int32_t *free_count, size_t pages, size_t page_size,
                     size_t rows, int padded, int32_t *slots, int32_t *positions, int32_t *requests, int32_t *starts,

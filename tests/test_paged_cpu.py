@@ -39,6 +39,14 @@ def test_page_entry_points_check_arguments():
     assert cut(batch=0) == shape and cut(pages=0) == shape
 
 
+def test_page_maps_of_too_many_rows_are_refused_before_memory_is_asked_for():
+    torch = pytest.importorskip("torch")
+    tables = F.PageTables.empty(3, 6, 16, 4, device="cpu")
+    for rows in (0x7ffffff1, 1 << 40, 1 << 62):
+        with pytest.raises(F.ShapeError, match="rows"):
+            F.page_extend(tables, torch.zeros(3, dtype=torch.int32), rows)
+
+
 def test_page_truncate_takes_no_lengths_among_the_lengths():
     """New lengths that are read again behind the writes of others' lengths."""
     def cut(lengths, to):
