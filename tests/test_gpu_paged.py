@@ -105,6 +105,29 @@ def test_page_tables_follow_the_stack(F, torch, batch, pages, p, width, rows, pa
         _same(tables, pool)
 
 
+@pytest.mark.parametrize("batch,pages,p,width,rows", [
+    (16384, 40000, 4, 4, 20000), (16384, 16384, 1, 1, 16384), (64, 65536, 2, 1100, 6144), (64, 65537, 2, 1100, 6145),
+    (9, 65536, 1, 7300, 20000), (9, 70000, 1, 7281, 20000)])
+def test_page_tables_at_the_limits_of_their_ways(F, torch, batch, pages, p, width, rows):
+    """The most requests, and pages and rows on both sides of where one block, a cluster
+    and many blocks take a step."""
+    rng = np.random.default_rng(batch + pages)
+    tables, pool = F.PageTables.empty(batch, pages, p, width), R.Pool(batch, pages, p, width)
+    for step in range(6):
+        counts = rng.integers(0, 2 * rows // batch + 2, batch)
+        m = F.page_extend(tables, _dev(torch, counts.astype(np.int32)), rows)
+        _maps(m, pool.extend(counts, rows))
+        _same(tables, pool)
+        if step % 3 == 2:  # everything goes back at once
+            cut = np.zeros(batch, np.int64)
+        else:
+            cut = np.where(rng.random(batch) < 0.7, -1, rng.integers(0, width * p + 1, batch))
+        F.page_truncate(tables, _dev(torch, cut.astype(np.int32)))
+        pool.truncate(cut)
+        _same(tables, pool)
+    assert len(pool.free) == pages
+
+
 def test_page_tables_what_a_step_took_goes_back(F, torch):
     tables = F.PageTables.empty(6, 50, 4, 8)
     F.page_extend(tables, _dev(torch, np.array([3, 9, 0, 4, 5, 1], np.int32)), 22)
@@ -352,6 +375,21 @@ def test_paged_attention_many_sessions(F, torch, pages):
     _check_attention(out, q, gate, cache, table, n, 0.125, sessions=[0, 7, 100, 300] + rng.integers(0, 301, 30).tolist(),
                      heads=[0, 3, 7])
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("pages", ["f32", "bf16"])
+def test_paged_attention_of_the_most_sessions(F, torch, pages):
+    torch.manual_seed(41)
+    rng = np.random.default_rng(41)
+    lengths = rng.integers(0, 40, 4096)
+    lengths[4095], lengths[17] = 3000, 0
+    q, gate, cache, table, n = _attention_case(F, torch, rng, lengths, 4, 2, 64, 16, "f32", pages)
+    out = F.paged_attention(q, cache, table, n, gate=gate)
+    _check_attention(out, q, gate, cache, table, n, 0.125, sessions=[0, 17, 4095, *rng.integers(0, 4096, 40).tolist()])
+    assert torch.isfinite(out).all() and not out[n == 0].any()
+    with pytest.raises(F.FpbError):
+        more = torch.zeros(4097, 4, 64, device="cuda")
+        F.paged_attention(more, cache, table[:1].expand(4097, -1).contiguous(), torch.zeros(4097, dtype=torch.int32, device="cuda"))
 
 
 @pytest.mark.parametrize("pages", ["f32", "bf16"])
