@@ -14,10 +14,14 @@
 // waits for, so that the block meets only at the end.  The products go by mma.sync: a
 // kv head has up to 16 rows of queries, which would leave most of a tcgen05 tile's 128
 // empty, and the copies are what takes the time.
-// Products keep f32's precision but for 2^-16 of a factor (bf16 pages: queries and
-// weights are two bf16 parts, exact in their products) or 2^-20 of a product (f32 pages:
-// every factor is two parts of 11 bits, and the parts' small product is left out);
-// sums are f32.
+// Products keep f32's precision: over bf16 pages f32 queries, and the weights beside
+// them, are three bf16 parts, exact in their products (with two, 2^-16 of a factor, 16 x
+// 8192 tokens were 5.3e-6 off in relative 2-norm, so 1.1e-6, where f32 arithmetic is 1.7e-6.
+// Two and three: 16 x 8192 tokens 47.2 and 47.6 us, 1 x 777 10.2 and 10.6; where 16 rows
+// make the products the bound 53 and 60, 40 x 4000 x 4 heads of 128 85 and 101).  Beside bf16
+// queries, which are exact, weights are two (2^-16 of themselves).  Over f32 pages products
+// are good to 2^-20: every factor is two parts of 11 bits, and the parts' small product is
+// left out.  Sums are f32.
 #include <algorithm>
 #include <atomic>
 #include <chrono>
@@ -127,11 +131,15 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   return y;
 }
 
-// (lo, hi) as bf16 pairs, and what the rounding left of them.
-__device__ __forceinline__ uint32_t split_bf16x2(float lo, float hi, uint32_t *rest) {
-  const uint32_t x = pack_bf16x2(lo, hi);
-  *rest = pack_bf16x2(lo - __uint_as_float(x << 16), hi - __uint_as_float(x & 0xffff0000u));
-  return x;
+// (lo, hi) as bf16 pairs, and what the rounding left of them in further ones.
+template <int N>
+__device__ __forceinline__ void split_bf16x2(float lo, float hi, uint32_t (&parts)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    parts[i] = pack_bf16x2(lo, hi);
+    lo -= __uint_as_float(parts[i] << 16);
+    hi -= __uint_as_float(parts[i] & 0xffff0000u);
+  }
 }
 
 __device__ __forceinline__ float load_q(const PagedArgs &a, int b, int h, int d) {
@@ -218,7 +226,8 @@ __device__ __forceinline__ int token_at(int i) {
 constexpr int warps_of(int DP, bool f32, bool once) { return !once ? 4 : DP == 256 && !f32 ? 8 : 12; }
 constexpr int blocks_of(int DP, bool once) { return once ? 1 : DP == 256 ? 2 : 3; }
 
-template <typename T, int DP, int NR, bool ONCE>
+// QF: f32 queries (over f32 pages always: what there is of bf16 ones is converted).
+template <typename T, int DP, int NR, bool ONCE, bool QF>
 struct PagedShape {
   static constexpr bool kHalf = sizeof(T) == 2;
   static constexpr int W = warps_of(DP, !kHalf, ONCE), kThreads = 32 * W, kBlocks = blocks_of(DP, ONCE);
@@ -234,9 +243,10 @@ struct PagedShape {
   static constexpr size_t kEnd = (size_t)W * NR * kEndPitch * 4;  // the warps' results, over the ring
   static constexpr size_t kPlan = (size_t)kPagedMaxBatch * 4;     // the sessions' steps, over the ring
   static constexpr size_t kOver = kRing > kEnd ? kRing : kEnd;
-  static constexpr size_t kQueries = (size_t)2 * NR * kQPitch * sizeof(T);
+  static constexpr int kQParts = !kHalf ? 2 : QF ? 3 : 1, kPParts = QF ? 3 : 2;  // of the queries, of the weights over bf16 pages
+  static constexpr size_t kQueries = (size_t)kQParts * NR * kQPitch * sizeof(T);
   static constexpr size_t smem = 1023 + kOver + kQueries;
-  static_assert(kPlan <= kOver && kBlocks * (smem + 4 * 1024) <= 228 * 1024);
+  static_assert(kPlan <= kOver && kBlocks * (smem + 3 * 1024) <= 228 * 1024);
 };
 
 // The sessions' steps are cut into shares of S, each session's evenly, and the
@@ -649,11 +659,11 @@ __device__ __noinline__ void plain_join(const PagedArgs &a, PagedShare me, int r
   }
 }
 
-template <typename T, int DP, int NR, bool ONCE>
-__global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (PagedShape<T, DP, NR, ONCE>::kBlocks))
+template <typename T, int DP, int NR, bool ONCE, bool QF>
+__global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE, QF>::kThreads), (PagedShape<T, DP, NR, ONCE, QF>::kBlocks))
     paged_attn_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ CUtensorMap k_map,
                       const __grid_constant__ CUtensorMap v_map) {
-  using Sh = PagedShape<T, DP, NR, ONCE>;
+  using Sh = PagedShape<T, DP, NR, ONCE, QF>;
   constexpr int W = Sh::W, kTok = Sh::kTok, kParts = Sh::kParts, kNT = NR / 8;
   extern __shared__ uint8_t raw_sm[];
   uint8_t *const ring = raw_sm + (-smem_u32(raw_sm) & 1023);  // the swizzle goes by the address
@@ -826,34 +836,39 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
 
   if constexpr (Sh::kHalf) {
     const int g = lane >> 2, c = lane & 3, own = token_at<T>(g);
-    __nv_bfloat16 *const qs = reinterpret_cast<__nv_bfloat16 *>(ring + Sh::kOver);  // [high, low][row][kQPitch]
-    constexpr int kPieces = DP / 32, kMT = DP / 16, kChains = NR == 8 ? 4 : 2;
-    const bool low = !a.q_bf16;
+    __nv_bfloat16 *const qs = reinterpret_cast<__nv_bfloat16 *>(ring + Sh::kOver);  // [part][row][kQPitch]
+    // (of three parts the last is read where it is used, beside the registers of the others; a
+    // sum of the first parts is kept apart from what the others add, which it would cut)
+    constexpr int kPieces = DP / 32, kMT = DP / 16, kChains = !QF ? 2 : NR == 8 ? 4 : 3, kQP = Sh::kQParts, kPP = Sh::kPParts;
+    constexpr int kHeld = Sh::kQShared ? 0 : kQP < 2 ? kQP : 2;
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
       const int r = w + i * W, col = lane * 8;
       if (col < DP && r < NR) {
-        uint32_t hi[4], lo[4];
+        uint32_t u[4][kQP];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) hi[k] = split_bf16x2(x[i][2 * k], x[i][2 * k + 1], &lo[k]);
-        *reinterpret_cast<uint4 *>(qs + r * Sh::kQPitch + col) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4 *>(qs + (NR + r) * Sh::kQPitch + col) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        for (int k = 0; k < 4; ++k) split_bf16x2(x[i][2 * k], x[i][2 * k + 1], u[k]);
+#pragma unroll
+        for (int part = 0; part < kQP; ++part)
+          *reinterpret_cast<uint4 *>(qs + (part * NR + r) * Sh::kQPitch + col) =
+              make_uint4(u[0][part], u[1][part], u[2][part], u[3][part]);
       }
     }
     __syncthreads();
     // Q operands of piece p: row g (+ 8 i)'s dimensions 32 p + 8 c + [0, 8)
-    auto query = [&](int part, int i, int p) {
+    auto stored = [&](int part, int i, int p) {
       return *reinterpret_cast<const uint4 *>(qs + (part * NR + g + 8 * i) * Sh::kQPitch + 32 * p + 8 * c);
     };
-    uint4 qr[Sh::kQShared ? 1 : 2 * kNT * kPieces];
-    if constexpr (!Sh::kQShared) {
+    uint4 qr[kHeld ? kHeld * kNT * kPieces : 1];
 #pragma unroll
-      for (int part = 0; part < 2; ++part)
+    for (int part = 0; part < kHeld; ++part)
 #pragma unroll
-        for (int i = 0; i < kNT; ++i)
+      for (int i = 0; i < kNT; ++i)
 #pragma unroll
-          for (int p = 0; p < kPieces; ++p) qr[(part * kNT + i) * kPieces + p] = query(part, i, p);
-    }
+        for (int p = 0; p < kPieces; ++p) qr[(part * kNT + i) * kPieces + p] = stored(part, i, p);
+    auto query = [&](int part, int i, int p) {
+      return part < kHeld ? qr[part < kHeld ? (part * kNT + i) * kPieces + p : 0] : stored(part, i, p);
+    };
     float acc[kMT][kNT][4], m[kNT][2], l[kNT][2];
 #pragma unroll
     for (int i = 0; i < kNT; ++i) {
@@ -883,13 +898,11 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
         const uint4 u = *reinterpret_cast<const uint4 *>(row), v = *reinterpret_cast<const uint4 *>(row + 8 * 128);
 #pragma unroll
         for (int i = 0; i < kNT; ++i) {
-          const uint4 q = Sh::kQShared ? query(0, i, p) : qr[Sh::kQShared ? 0 : i * kPieces + p];
-          mma_bf16(s[i][0], u.x, v.x, u.y, v.y, q.x, q.y);
-          mma_bf16(s[i][1], u.z, v.z, u.w, v.w, q.z, q.w);
-          if (low) {
-            const uint4 r = Sh::kQShared ? query(1, i, p) : qr[Sh::kQShared ? 0 : (kNT + i) * kPieces + p];
-            mma_bf16(s[i][kChains - 2], u.x, v.x, u.y, v.y, r.x, r.y);
-            mma_bf16(s[i][kChains - 1], u.z, v.z, u.w, v.w, r.z, r.w);
+#pragma unroll
+          for (int part = 0; part < kQP; ++part) {
+            const uint4 q = query(part, i, p);
+            mma_bf16(s[i][part ? (kChains == 4 ? 2 : kChains - 1) : 0], u.x, v.x, u.y, v.y, q.x, q.y);
+            mma_bf16(s[i][part ? kChains - 1 : 1], u.z, v.z, u.w, v.w, q.z, q.w);
           }
         }
       }
@@ -904,6 +917,7 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float x = s[i][0][2 * h + e] + s[i][1][2 * h + e];
+            if (kChains == 3) x += s[i][kChains - 1][2 * h + e];
             if (kChains == 4) x += s[i][kChains - 2][2 * h + e] + s[i][kChains - 1][2 * h + e];
             y[i][e][h] = x * a.scale_log2;
             if (open && !token_there(t0 + own + 8 * h)) y[i][e][h] = -INFINITY;
@@ -928,7 +942,7 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
             }
           }
       }
-      uint32_t ph[kNT][2], pl[kNT][2];
+      uint32_t pp[kPP][kNT][2];
 #pragma unroll
       for (int i = 0; i < kNT; ++i) {
         const float base[2] = {m[i][0] == -INFINITY ? 0.0f : -m[i][0], m[i][1] == -INFINITY ? 0.0f : -m[i][1]};
@@ -937,10 +951,10 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
           const float p0 = pow2(y[i][0][h] + base[0]), p1 = pow2(y[i][1][h] + base[1]);
           l[i][0] += p0;
           l[i][1] += p1;
-          uint32_t rest;
-          const uint32_t x = split_bf16x2(p0, p1, &rest);
-          ph[i][h] = transposed(x);
-          pl[i][h] = transposed(rest);
+          uint32_t u[kPP];
+          split_bf16x2(p0, p1, u);
+#pragma unroll
+          for (int part = 0; part < kPP; ++part) pp[part][i][h] = transposed(u[part]);
         }
       }
       uint8_t *vst = mine + (2 * at + 1) % kParts * Sh::kPart;
@@ -953,10 +967,10 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE>::kThreads), (Page
         uint32_t x[4];
         load_transposed(x, v0 + (k >> 2) * (kTok * 128) + ((2 * (k & 3) + half) ^ vrow) * 16);
 #pragma unroll
-        for (int i = 0; i < kNT; ++i) {
-          mma_bf16(acc[k][i], x[0], x[1], x[2], x[3], ph[i][0], ph[i][1]);
-          mma_bf16(acc[k][i], x[0], x[1], x[2], x[3], pl[i][0], pl[i][1]);
-        }
+        for (int i = 0; i < kNT; ++i)
+#pragma unroll
+          for (int part = 0; part < kPP; ++part)
+            mma_bf16(acc[k][i], x[0], x[1], x[2], x[3], pp[part][i][0], pp[part][i][1]);
       }
       done(2 * at + 1);
     }
@@ -1257,9 +1271,9 @@ struct Plan {
   size_t blocks, parts;
 };
 
-template <typename T, int DP, int NR, bool ONCE>
+template <typename T, int DP, int NR, bool ONCE, bool QF>
 int run_shape(const PagedArgs &a, const Plan &p, const CUtensorMap &k_map, const CUtensorMap &v_map, cudaStream_t s) {
-  using Sh = PagedShape<T, DP, NR, ONCE>;
+  using Sh = PagedShape<T, DP, NR, ONCE, QF>;
   {
     static std::mutex mu;
     static std::vector<int> done;
@@ -1267,12 +1281,12 @@ int run_shape(const PagedArgs &a, const Plan &p, const CUtensorMap &k_map, const
     FPB_CUDA_TRY(cudaGetDevice(&dev));
     std::lock_guard<std::mutex> lock(mu);
     if (std::find(done.begin(), done.end(), dev) == done.end()) {
-      FPB_CUDA_TRY(cudaFuncSetAttribute(paged_attn_kernel<T, DP, NR, ONCE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      FPB_CUDA_TRY(cudaFuncSetAttribute(paged_attn_kernel<T, DP, NR, ONCE, QF>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         (int)Sh::smem));
       done.push_back(dev);
     }
   }
-  cudaError_t e = launch_pdl(paged_attn_kernel<T, DP, NR, ONCE>, (unsigned)p.blocks, Sh::kThreads, Sh::smem, s, a, k_map,
+  cudaError_t e = launch_pdl(paged_attn_kernel<T, DP, NR, ONCE, QF>, (unsigned)p.blocks, Sh::kThreads, Sh::smem, s, a, k_map,
                              v_map);
   if (e != cudaSuccess) return cuda_fail(e, "paged_attn_kernel");
   FPB_LAUNCH_CHECK("paged_attn_kernel");
@@ -1281,7 +1295,12 @@ int run_shape(const PagedArgs &a, const Plan &p, const CUtensorMap &k_map, const
 
 template <typename T, int DP, int NR>
 int run_paged(const PagedArgs &a, const Plan &p, const CUtensorMap &k_map, const CUtensorMap &v_map, cudaStream_t s) {
-  return p.waves ? run_shape<T, DP, NR, false>(a, p, k_map, v_map, s) : run_shape<T, DP, NR, true>(a, p, k_map, v_map, s);
+  if constexpr (sizeof(T) == 2)
+    if (a.q_bf16)
+      return p.waves ? run_shape<T, DP, NR, false, false>(a, p, k_map, v_map, s)
+                     : run_shape<T, DP, NR, true, false>(a, p, k_map, v_map, s);
+  return p.waves ? run_shape<T, DP, NR, false, true>(a, p, k_map, v_map, s)
+                 : run_shape<T, DP, NR, true, true>(a, p, k_map, v_map, s);
 }
 
 Plan plan_for(size_t batch, size_t q_heads, size_t kv_heads, size_t head_dim, bool f32) {

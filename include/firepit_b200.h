@@ -889,8 +889,9 @@ int fpb_paged_append(const void *q, size_t q_pitch, size_t q_head_pitch, const v
  * softmax(scale q . k) v, times sigmoid(gate) where gate [batch rows of gate_pitch,
  * heads of gate_head_pitch] f32 is given.  A session of length 0 gets zeros.  Rows
  * behind its last token never reach an output, whatever they hold; a token whose
- * page is outside the pool counts as not there.  Sums are f32; over bf16 pages q and
- * the weights are taken to 16 bits, over f32 pages products to 2^-20 of themselves.
+ * page is outside the pool counts as not there.  Sums are f32, and so are products
+ * but for 2^-20 of themselves over f32 pages, and 2^-16 of the weights for bf16 q over
+ * bf16 pages.
  * Infinities are as the formula has them: a score of -inf is a weight of 0 (nothing
  * else: zeros), one of +inf NaN, an infinite value its column.
  * The workspace needs no clearing; calls that may run at the same time must not share

@@ -127,3 +127,40 @@ def test_paged_attention_values_out_of_the_ordinary(F, torch, n, hq, hk, d, p, t
         elif kind in ("key -inf", "plain", "columns", "small", "large"):
             if kind != "key -inf" or lengths[i] > 3:
                 assert np.isfinite(got[i]).all() and (kind != "small" or (got[i] != 0).all())
+
+
+@pytest.mark.parametrize("hq,hk", [(8, 8), (64, 8), (64, 4)])
+def test_paged_attention_f32_queries_keep_their_bits(F, torch, hq, hk):
+    """f32 queries over bf16 pages: bits of the queries and of the weights that only a
+    third part of 8 holds.
+
+    First two tokens whose scores 2^20 + 2^11 differ by 1 through elements 1 + 2^-9 +
+    2^-20: f32 scores in powers of two are off by 2^-4 at most each, so the first
+    token's weight 1 / (1 + e^-1) lies within [0.71, 0.75]; without that bit it is a half.
+    Then weights p = e^-x of one element against 1, values 1 and -c with c the bf16 number
+    nearest to p: (p - c) / (1 + p) is off by p (2^-23 of the power's argument, 2^-22 of the
+    power) and 2^-22 of the sums, below 2^-20; two parts leave up to 2^-18 of p."""
+    d, heads = 256, hq // hk
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    n = torch.full((1,), 2, dtype=torch.int32, device="cuda")
+    cache = F.PagedCache.zeros(1, 16, hk, d)
+    q = torch.full((1, hq, d), 1 + 2.0 ** -9, device="cuda")
+    q[..., :d // 2] += 2.0 ** -20
+    cache.k[0, 0, :, :d // 2], cache.k[0, 1, :, d // 2:] = 8192.0, 8192.0
+    cache.v[0, 0] = 1.0
+    out = F.paged_attention(q, cache, table, n, scale=1.0, out=torch.empty_like(q))
+    assert 0.71 <= float(out.min()) and float(out.max()) <= 0.75
+    rng = np.random.default_rng(hq + hk)
+    x = np.float32(rng.uniform(0.01, 1.3, hq))
+    q.zero_()
+    q[0, :, 0] = -_dev(torch, x)
+    cache.k.zero_()
+    cache.k[0, 0, :, 0] = 1.0
+    p = np.exp(-x.astype(np.float64))
+    c = _host(_dev(torch, p.astype(np.float32)).bfloat16())
+    cache.v.zero_()
+    cache.v[0, 0, :, :heads] = 1.0
+    cache.v[0, 1, :, :heads] = -_dev(torch, c.astype(np.float32)).bfloat16().view(hk, heads)
+    out = _host(F.paged_attention(q, cache, table, n, scale=1.0, out=torch.empty_like(q)))[0]
+    got = out[np.arange(hq), np.arange(hq) % heads]
+    assert np.abs(got - (p - c) / (1 + p)).max() <= 2.0 ** -20
