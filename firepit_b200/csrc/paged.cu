@@ -85,8 +85,8 @@ __device__ __forceinline__ void cluster_meet() {
 // Each block scans all requests for itself, then the blocks share the rows and the
 // new pages.  A request is served whole (its rows fit, its table and the pool have
 // the pages) or not at all.  Bound by latency: two loads, two scans and the pages'
-// loads in a row (with page_truncate behind it, 64 requests of a token each 7.1 us,
-// 144000 rows of 96 requests, 1.7 MB, 14.3).
+// loads in a row (with page_truncate behind it, 64 requests of a token each 9.7 us,
+// 144000 rows of 96 requests, 1.7 MB, 14.5).
 template <PagePart PART>
 __global__ void __launch_bounds__(kPageMaxThreads) page_extend_kernel(const __grid_constant__ PageArgs a) {
   pdl_enter();
@@ -265,10 +265,10 @@ int check_tables(const char *name, const PageArgs &a, size_t table_pitch, size_t
 // them for the state (extend and truncate, one block and many: 4096 rows 9.5 and 11.5
 // us, 8192 12.4 and 11.4, 144000 120 and 14).  Where it is not known how much of `work`
 // there is, as for the pages that a step gives back of all that the requests may hold, a
-// cluster takes it up to `cluster` (extend and truncate of 64 requests of 564 pages, by a
-// cluster and by many blocks: one page each 9.0 and 9.2 us, all 17.2 and 16.4; and the
-// host has a launch less, 2 us; rows, which are known, go better by many: 65536 15.7 and
-// 11.7).
+// cluster takes it up to `cluster` (a truncation of 64 requests of 564 pages, by a cluster
+// and by many blocks: one page each 5.4 and 6.1 us, all of them 9.5 and 8.7; of 1024 pages
+// 5.4 and 6.1, 12.3 and 8.2: a step gives few back, and the host has a launch less, 2 us;
+// rows, which are known, go better by many: 65536 15.7 and 11.7).
 int launch_pages(void (*const (&kernel)[3])(PageArgs), const char *name, const PageArgs &a, size_t work,
                  size_t cluster, size_t smem, cudaStream_t s) {
   {

@@ -5,11 +5,11 @@
 // One pass over the tokens: a warp holds its rows' running maximum m, sum of weights l
 // and numerators, all f32, and two such parts meet as l1 2^(m1 - m) + l2 2^(m2 - m).
 //
-// Bound by the pages' bytes, each read once: 200 ragged sessions (1.65 GB) 255 us, 6.5
-// TB/s; 3 x 100003 tokens x 4 heads of 128, bf16, 106 us, 5.3; 16 x 8192 x 2 heads of
-// 256 47.7 us, 5.0; 8 x 2304 of f32 25.5 us.  9 to 10 us of a call do not depend on the
+// Bound by the pages' bytes, each read once: 200 ragged sessions (1.65 GB) 253 us, 6.5
+// TB/s; 3 x 100003 tokens x 4 heads of 128, bf16, 103 us, 5.5; 16 x 8192 x 2 heads of
+// 256 47.6 us, 5.0; 8 x 2304 of f32 25.0 us.  About 10 us of a call do not depend on the
 // bytes: the launch, the cut into shares, the first copies' way and the shares' meeting
-// (1 x 777 tokens 10.2 us).
+// (1 x 777 tokens 10.6 us).
 // A warp takes steps of 16 tokens (f32: 8) through a ring of TMA copies that it alone
 // waits for, so that the block meets only at the end.  The products go by mma.sync: a
 // kv head has up to 16 rows of queries, which would leave most of a tcgen05 tile's 128
@@ -997,7 +997,7 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE, QF>::kThreads), (
   } else {
     // A product of parts is three of the tensor cores' (two parts each, without the small
     // ones'), and takes the time that the copies do (8 x 18432 tokens of 256: with f32
-    // fma 111 us, so 102, 5.9 TB/s).
+    // fma 111 us, so 102, 5.9 TB/s).  Of the scores' operand rows 8 to 15 are zeros.
     // S = Q K^T with the rows as M (eight of sixteen), eight tokens as N; O^T = V^T P^T
     // with the dimensions as M, the rows as N: S's result is P^T's operand as it lies.
     const int g = lane >> 2, c = lane & 3, own = token_at<T>(g);

@@ -690,7 +690,7 @@ class PagedDecoder(Decoder):
     """Serves requests on `sessions` rows whose attention layers share pools of
     `pages` pages of `page_size` tokens (a pool a layer, one table for all), so
     that a long session takes no more than its tokens' room and a row is free for
-    the next request as soon as one is done.
+    the next request as soon as one is done.  The pools are bf16, or of `dtype`.
 
     ``step()`` takes one token of every session under way: from its prompt, or the
     one before it drawn (``noise``, from ``draw``).  It takes the pages, runs the

@@ -217,7 +217,8 @@ def page_extend(tables: PageTables, counts, rows: int, padded: bool = False, out
 
 def page_truncate(tables: PageTables, lengths, stream=None) -> None:
     """Cuts the requests to lengths [batch] (negative, or not below the present
-    one: as it was; 0: the request is done) and gives their pages back."""
+    one: as it was; 0: the request is done; not otherwise among the tables' own) and
+    gives their pages back."""
     if stream is None and _Torch.calls is not None:
         got = _Torch.calls.page_truncate(tables.table, tables.lengths, tables.free, tables.free_count, tables.page_size,
                                          lengths)
@@ -299,6 +300,7 @@ def paged_attention(q, cache: PagedCache, table, lengths, gate=None, scale: floa
     f32 or bf16): each session's attention over its first lengths [batch] tokens,
     those of its row of table [batch, max_pages] (int32, any row pitch), times
     sigmoid(gate) where a gate (f32, q's shape) is given; zeros for a length of 0.
+    Infinities and NaN are as the formula has them.
     q [batch, q_heads, head_dim] f32 or bf16, any row and head pitch; scale default
     1 / sqrt(head_dim); ``workspace``: uint8 of ``paged_attention_workspace_bytes``
     (allocated where None), which calls on different streams must not share."""
