@@ -67,9 +67,10 @@ constexpr int kErrPagedWait = 503;
 // are 2^(y - m), up to 2^8, so that values down to the smallest normal number give
 // normal numerators, and weights down to 2^-126 count.
 constexpr float kLag = 8.0f;
-// Outputs of a share below this (or not finite) are found again by plain_share(): of f32
-// values below 2^-112 the tensor cores' low parts are short of bits.
-constexpr float kSmall = 7.888609e-31f;  // 2^-100
+// Outputs of a share over f32 pages below this (or not finite ones over any) are found again
+// by plain_share(): the tensor cores hold the low parts of numbers below 2^-116 to 2^-136.
+// (bf16 parts are whole down to 2^-133 of a sum.)
+constexpr float kSmall = 1.9259299e-34f;  // 2^-112
 
 __device__ __forceinline__ float pow2(float x) {
   float y;
@@ -470,8 +471,9 @@ __device__ __forceinline__ bool paged_share(const PagedArgs &a, int *steps, Page
 }
 
 // Whether a share's output is one that the tensor cores' products may have wrong.
+template <typename T>
 __device__ __forceinline__ bool unusual(float x) {
-  return !(fabsf(x) <= 3.402823466e38f) || (fabsf(x) < kSmall && x != 0.0f);
+  return !(fabsf(x) <= 3.402823466e38f) || (sizeof(T) == 4 && fabsf(x) < kSmall && x != 0.0f);
 }
 
 // The block's share again, where some of its outputs are unusual(): the whole block calls
@@ -566,7 +568,7 @@ __device__ __noinline__ void plain_share(const PagedArgs &a, PagedShare me, int 
   __syncthreads();
   bool again = false;
   auto doubtful = [&](float x, int r, int d) {
-    return unusual(x) && !(isnan(x) && ((nan_columns[d >> 3] >> (d & 7) | nan_rows >> r) & 1));
+    return unusual<T>(x) && !(isnan(x) && ((nan_columns[d >> 3] >> (d & 7) | nan_rows >> r) & 1));
   };
   meet([&](int r, int d, float2 o, float) { again |= doubtful(o.x, r, d) | doubtful(o.y, r, d + 1); }, [](int, float, float) {});
   if (!__syncthreads_or(again)) return;
@@ -1160,7 +1162,7 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE, QF>::kThreads), (
         o.x = fmaf(v.x, f[x], o.x);
         o.y = fmaf(v.y, f[x], o.y);
       }
-      again |= unusual(o.x) | unusual(o.y);
+      again |= unusual<T>(o.x) | unusual<T>(o.y);
       keep_out(a, me, NR, r, head0 + r, d, o, sum);
     }
     if (me.parts > 1 && lane == 0) a.part_ml[(size_t)me.slot * NR + r] = make_float2(top, sum);

@@ -18,7 +18,7 @@ from test_gpu_paged import F, _attention_case, _dev, _host, _no_device_error, to
 
 pytestmark = pytest.mark.gpu
 
-KINDS = ("key -inf", "key +inf", "value", "query", "hopeless", "nan", "masked", "plain", "columns", "small", "large")
+KINDS = ("key -inf", "key +inf", "value", "query", "hopeless", "nan", "masked", "plain", "columns", "small", "large", "sparse")
 
 
 def _special(torch, kind, rng, i, n, q, k, v, scale):
@@ -56,6 +56,11 @@ def _special(torch, kind, rng, i, n, q, k, v, scale):
         v *= 2.0 ** np.linspace(-120, 120, d).round().astype(np.float32)
     elif kind == "small":
         v *= np.float32(2.0 ** -118)
+    elif kind == "sparse":  # columns of a few tokens each, most of them of next to no weight
+        at = np.arange(n)
+        q[:, 6] = 2.0
+        k[:, :, 6] = -(37.5 / scale * (at % d) / d)[:, None]
+        v *= (at[:, None] % d == np.arange(d))[:, None, :]
     elif kind == "large":
         v *= np.float32(2.0 ** 122)
 
