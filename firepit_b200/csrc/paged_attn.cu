@@ -486,10 +486,12 @@ __device__ __forceinline__ bool unusual(float x) {
 // counts whole however small its weight is: only a score of -inf has one of 0.
 // (16 x 8192 tokens x 2 heads of 256, with one NaN or one a page: 249 and 279 us for 47;
 // twenty times that where everything is done again.)
-template <typename T, int W, int NR, int PITCH>
+// Queries are taken from the block's own parts of them: where the output goes over them,
+// the first one has been stored.
+template <typename T, int DP, int NR, typename Sh>
 __device__ __noinline__ void plain_share(const PagedArgs &a, PagedShare me, int rows, int head0, float *sm,
                                          float (*m_s)[NR], float (*l_s)[NR]) {
-  constexpr int kTok = sizeof(T) == 2 ? 16 : 8;
+  constexpr int kTok = Sh::kTok, W = Sh::W, PITCH = Sh::kEndPitch;
   __shared__ uint32_t nan_columns[32], nan_rows;  // outputs that are to be NaN: eight columns a word, or whole rows
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = lane * 8, D = a.head_dim;
   // (without a sign: a step past the last token may pass 2^31)
@@ -503,6 +505,18 @@ __device__ __noinline__ void plain_share(const PagedArgs &a, PagedShare me, int 
   auto load8 = [&](const void *base, long long at, float (&x)[8]) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = col < D ? static_cast<float>(static_cast<const T *>(base)[at + k]) : 0.0f;
+  };
+  // the lane's columns of row r's query: its parts are exact, but for an infinite one's rest
+  auto query8 = [&](int r, float (&x)[8]) {
+    const uint8_t *const qs = reinterpret_cast<const uint8_t *>(sm) + Sh::kOver;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      x[k] = 0.0f;
+      for (int part = Sh::kQParts - 1; part >= 0 && col < DP; --part) {
+        const float y = static_cast<float>(reinterpret_cast<const T *>(qs)[(part * NR + r) * Sh::kQPitch + col + k]);
+        x[k] = part == 0 && isinf(y) ? y : x[k] + y;
+      }
+    }
   };
   auto score = [&](const float (&q)[8], const float (&k)[8]) {
     double s = 0.0;
@@ -559,7 +573,7 @@ __device__ __noinline__ void plain_share(const PagedArgs &a, PagedShare me, int 
   if (bits) atomicOr(nan_columns + lane, bits);
   for (int r = w; r < rows; r += W) {
     float q[8];
-    load_q8(a, me.b, head0 + r, col, col < D, q);
+    query8(r, q);
     bool none = false;
 #pragma unroll
     for (int k = 0; k < 8; ++k) none |= isnan(q[k]);
@@ -574,7 +588,7 @@ __device__ __noinline__ void plain_share(const PagedArgs &a, PagedShare me, int 
   if (!__syncthreads_or(again)) return;
   for (int r = 0; r < rows; ++r) {
     float q[8], x[8], m = -INFINITY, l = 0.0f;
-    load_q8(a, me.b, head0 + r, col, col < D, q);
+    query8(r, q);
     for (uint32_t t = first; t < end; t += W) {
       const long long at = place(t);
       if (at < 0) continue;
@@ -597,7 +611,7 @@ __device__ __noinline__ void plain_share(const PagedArgs &a, PagedShare me, int 
   for (int r = 0; r < rows; ++r) {
     float q[8], x[8], acc[8], l = 0.0f, top;
     const float sum = sum_of(r, &top), base = sum == 0.0f ? 0.0f : top + ceilf(log2f(sum));
-    load_q8(a, me.b, head0 + r, col, col < D, q);
+    query8(r, q);
 #pragma unroll
     for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
     for (uint32_t t = first; t < end; t += W) {
@@ -1167,7 +1181,7 @@ __global__ void __launch_bounds__((PagedShape<T, DP, NR, ONCE, QF>::kThreads), (
     }
     if (me.parts > 1 && lane == 0) a.part_ml[(size_t)me.slot * NR + r] = make_float2(top, sum);
   }
-  if (__syncthreads_or(again)) plain_share<T, W, NR, Sh::kEndPitch>(a, me, rows, head0, sm, m_s, l_s);
+  if (__syncthreads_or(again)) plain_share<T, DP, NR, Sh>(a, me, rows, head0, sm, m_s, l_s);
   if (me.parts == 1) return;
   // The shares of an item meet in the block that finds all of them there: each says
   // so by its flag and then looks at the others', so that the last one does find

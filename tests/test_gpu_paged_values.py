@@ -104,6 +104,10 @@ def test_paged_attention_values_out_of_the_ordinary(F, torch, n, hq, hk, d, p, t
         host.append((_host(q[i]), *(_host(t[ids]).reshape(-1, hk, d)[:m] for t in (cache.k, cache.v))))
     out = torch.full(q.shape, 7.0, device="cuda")
     assert F.paged_attention(q, cache, table, lens, gate=gate, out=out) is out
+    if dtype == "f32":  # in the queries' place
+        mine = q.clone()
+        assert F.paged_attention(mine, cache, table, lens, gate=gate, out=mine) is mine
+        assert torch.equal(torch.nan_to_num(mine), torch.nan_to_num(out))
     again = F.paged_attention(q, cache, table, lens, gate=gate)
     assert torch.equal(torch.nan_to_num(again), torch.nan_to_num(out.to(again.dtype)))
     got, g = _host(out), 1.0 / (1.0 + np.exp(-_host(gate)))
