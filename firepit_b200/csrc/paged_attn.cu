@@ -1396,6 +1396,23 @@ extern "C" int fpb_paged_attn(const void *q, int q_dtype, size_t q_pitch, size_t
   const size_t need = fpb_paged_attn_workspace_bytes(batch, q_heads, kv_heads, head_dim);
   if (workspace_bytes < need)
     return fail(FPB_ERR_WORKSPACE, "fpb_paged_attn: workspace %zu < %zu bytes", workspace_bytes, need);
+  {
+    // The head vectors x [batch rows of pitch, q_heads of head] against the output, which is one piece
+    const char *o = static_cast<const char *>(out), *end = o + batch * q_heads * head_dim * (out_dtype == FPB_F32 ? 4 : 2);
+    auto meets = [&](const void *x, size_t pitch, size_t head, size_t el) {
+      const char *v = static_cast<const char *>(x);
+      if (!x || v >= end || v + ((batch - 1) * pitch + (q_heads - 1) * head + head_dim) * el <= o) return false;
+      for (size_t b = 0; b < batch; ++b)
+        for (size_t h = 0; h < q_heads; ++h)
+          if (const char *u = v + (b * pitch + h * head) * el; u < end && u + head_dim * el > o) return true;
+      return false;
+    };
+    const bool in_place = q == out && q_dtype == out_dtype && (q_heads == 1 || q_head_pitch == head_dim) &&
+                          (batch == 1 || q_pitch == q_heads * head_dim);
+    if ((!in_place && meets(q, q_pitch, q_head_pitch, q_dtype == FPB_F32 ? 4 : 2)) ||
+        meets(gate, gate_pitch, gate_head_pitch, 4))
+      return fail(FPB_ERR_INVALID_ARGUMENT, "fpb_paged_attn: out overlaps the gate, or q otherwise than in its place");
+  }
   const bool f32 = page_dtype == FPB_F32;
   Plan p = plan_for(batch, q_heads, kv_heads, head_dim, f32);
   {  // no more blocks than the tables' tokens can have shares

@@ -894,7 +894,8 @@ int fpb_paged_append(const void *q, size_t q_pitch, size_t q_head_pitch, const v
  * bf16 pages.
  * Infinities are as the formula has them: a score of -inf is a weight of 0 (nothing
  * else: zeros), one of +inf NaN, an infinite value its column.
- * out may be q itself (of its type and layout).  The workspace needs no clearing; calls that may run at the same time must not share
+ * out may be q itself (of its type and layout); it must not overlap q otherwise, nor the
+ * gate.  The workspace needs no clearing; calls that may run at the same time must not share
  * one.  batch at most 4096. */
 size_t fpb_paged_attn_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads, size_t head_dim);
 int fpb_paged_attn(const void *q, int q_dtype, size_t q_pitch, size_t q_head_pitch, const void *k_pages,

@@ -173,3 +173,22 @@ def test_paged_attention_f32_queries_keep_their_bits(F, torch, hq, hk):
     out = _host(F.paged_attention(q, cache, table, n, scale=1.0, out=torch.empty_like(q)))[0]
     got = out[np.arange(hq), np.arange(hq) % heads]
     assert np.abs(got - (p - c) / (1 + p)).max() <= 2.0 ** -20
+
+
+def test_paged_attention_outputs_beside_the_inputs(F, torch):
+    """Next to the queries and the gate, and between their rows."""
+    torch.manual_seed(7)
+    rng = np.random.default_rng(7)
+    q, gate, cache, table, n = _attention_case(F, torch, rng, [40, 70], 4, 2, 64, 16, "f32", "f32")
+    want = F.paged_attention(q, cache, table, n, gate=gate)
+    both = torch.zeros(4, 4, 64, device="cuda")
+    both[:2] = q
+    assert torch.equal(F.paged_attention(both[:2], cache, table, n, gate=gate, out=both[2:]), want)
+    wide = torch.zeros(2, 4096, device="cuda")
+    mine, g, out = wide[:, :256].unflatten(1, (4, 64)), wide[:, 256:512].unflatten(1, (4, 64)), wide[0, 512:1024].view(2, 4, 64)
+    mine.copy_(q)
+    g.copy_(gate)
+    assert torch.equal(F.paged_attention(mine, cache, table, n, gate=g, out=out), want)
+    for bad in (wide[0, 128:640], wide[0, 256:768], wide.view(-1)[3840:4352]):
+        with pytest.raises(F.FpbError):
+            F.paged_attention(mine, cache, table, n, gate=g, out=bad.view(2, 4, 64))

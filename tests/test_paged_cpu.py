@@ -94,6 +94,22 @@ def test_paged_attention_checks_arguments():
     assert attn(ws_bytes=0) == N.FPB_ERR_WORKSPACE
 
 
+def test_paged_attention_checks_where_its_output_lies():
+    """Over the gate, which blocks read behind one another's outputs, or over other rows'
+    queries: refused."""
+    buf = (C.c_float * 4096)()
+    p = C.addressof(buf) // 16 * 16 + 16
+
+    def attn(q, out, out_dtype=0, q_pitch=64, q_head=32, gate=None, gate_pitch=64, gate_head=32):
+        return N.lib.fpb_paged_attn(q, 0, q_pitch, q_head, f, f, 1, 4, 16, 1024, 64, 32, i, 4, 4, i, gate, gate_pitch,
+                                    gate_head, 2, 2, 2, 32, 0.1, f, 1 << 30, out, out_dtype, None)
+
+    for kw in (dict(q=p, out=p, out_dtype=1), dict(q=p, out=p + 16), dict(q=p + 16, out=p), dict(q=p, out=p, q_pitch=128),
+               dict(q=p, out=p, q_head=64, q_pitch=128), dict(q=p + 4096, out=p, gate=p),
+               dict(q=p + 4096, out=p, gate=p + 508), dict(q=p + 4096, out=p + 256, gate=p, gate_pitch=128, gate_head=64)):
+        assert attn(**kw) == bad, kw
+
+
 def test_sample_checks_arguments():
     def sample(logits=f, dtype=0, pitch=100, t=f, noise=f, noise_pitch=100, batch=2, vocab=100, tokens=i):
         return N.lib.fpb_sample(logits, dtype, pitch, t, None, None, None, noise, noise_pitch, batch, vocab, tokens, None,
