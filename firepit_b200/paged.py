@@ -297,7 +297,7 @@ def paged_attention_workspace_bytes(cache: PagedCache, batch: int, q_heads: int)
 def paged_attention(q, cache: PagedCache, table, lengths, gate=None, scale: float | None = None, out=None,
                     workspace=None, stream=None):
     """out [batch, q_heads, head_dim] (allocated in the pages' type where None;
-    f32 or bf16): each session's attention over its first lengths [batch] tokens,
+    f32 or bf16; q itself or apart from q and the gate): each session's attention over its first lengths [batch] tokens,
     those of its row of table [batch, max_pages] (int32, any row pitch), times
     sigmoid(gate) where a gate (f32, q's shape) is given; zeros for a length of 0.
     Infinities and NaN are as the formula has them.
